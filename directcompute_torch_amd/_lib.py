@@ -2,7 +2,8 @@
 
 The argtypes/restype blocks mirror the reference's binding of engine.dll
 (nn_engine.py:42-121) symbol for symbol, plus the additions declared in
-include/dcengine.h (GetLastErrorString, AdamBatch, ClipGradNorm, profiling).
+include/dcengine.h (GetLastErrorString, AdamBatch, ClipGradNorm, profiling,
+rotary positions, attention, MuonBatch).
 
 Loading never falls back to anything: if the library is missing or no HIP
 device is usable, :func:`load` raises.
@@ -129,6 +130,16 @@ def bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.AdamBatchCounted.argtypes = ([P(c_void_p)] * 4 + [P(c_uint), c_uint, c_void_p, c_uint, c_float]
                                      + [ctypes.c_double] * 3 + [c_float] * 3)
     lib.AdamBatchCounted.restype = None
+    lib.RotaryApply.argtypes = [c_void_p] * 3 + [c_uint] * 6
+    lib.RotaryApply.restype = c_void_p
+    lib.AttentionForward.argtypes = [c_void_p] * 4 + [c_uint] * 7 + [c_float, P(c_void_p)]
+    lib.AttentionForward.restype = c_void_p
+    lib.AttentionBackward.argtypes = ([c_void_p] * 7 + [c_uint] * 7 + [c_float] + [c_uint] * 3
+                                      + [P(c_void_p)] * 3)
+    lib.AttentionBackward.restype = None
+    lib.MuonBatch.argtypes = ([P(c_void_p)] * 3 + [P(c_uint)] * 2 + [P(c_float), c_uint, c_float, c_uint]
+                              + [c_float] * 2 + [c_uint])
+    lib.MuonBatch.restype = ctypes.c_bool
     lib.SetProfiling.argtypes = [ctypes.c_int]
     lib.SetProfiling.restype = None
     lib.GetProfile.argtypes = [ctypes.c_char_p, P(ctypes.c_uint64), P(ctypes.c_double), P(ctypes.c_double), P(ctypes.c_double)]

@@ -1287,6 +1287,162 @@ float ClipGradNormNoAlloc(void** grads, uint32_t* sizes, uint32_t numGrads, floa
   return clip_grad_norm_noalloc(g_device, grads, sizes, numGrads, maxNorm, g_capturing);
 }
 
+// ------------------------------------------------------------- transformers
+void* RotaryApply(void* x, void* table, void* positions, uint32_t batch, uint32_t seq,
+                  uint32_t heads, uint32_t headDim, uint32_t rotaryDim, uint32_t flags) {
+  if (!ensure_init()) return nullptr;
+  Buffer* X = as_buffer(x, "RotaryApply(x)");
+  Buffer* W = X ? as_buffer(table, "RotaryApply(table)") : nullptr;
+  Buffer* P = positions && W ? as_buffer(positions, "RotaryApply(positions)") : nullptr;
+  if (!X || !W || (positions && !P)) return nullptr;
+  const uint64_t tokens = uint64_t(batch) * seq, n = tokens * heads * headDim;
+  if (!batch || !seq || !heads || !headDim || tokens >= 0x80000000ull ||
+      uint64_t(heads) * headDim >= kOob || X->count < n) {
+    set_error("RotaryApply: x holds %u values, not %u x %u x %u x %u", X->count, batch, seq, heads,
+              headDim);
+    return nullptr;
+  }
+  if (rotaryDim < 2 || rotaryDim % 2 || rotaryDim > headDim || W->count < rotaryDim) {
+    set_error("RotaryApply: %u turned values (an even number up to the head's %u, one table row or more)",
+              rotaryDim, headDim);
+    return nullptr;
+  }
+  if (P && P->count < tokens) {
+    set_error("RotaryApply: %u positions for %llu tokens", P->count, (unsigned long long)tokens);
+    return nullptr;
+  }
+  void* y = create_buffer(nullptr, uint32_t(n));
+  if (!y) return nullptr;
+  if (!rotary(X->ptr, W->ptr, P ? P->ptr : nullptr, static_cast<Buffer*>(y)->ptr, uint32_t(tokens),
+              seq, heads, headDim, rotaryDim, W->count / rotaryDim, flags & 1, flags & 2)) {
+    release_buffer(y);
+    return nullptr;
+  }
+  return y;
+}
+
+// The checked arguments of an attention call; false with the error set.
+static bool attn_args(const char* what, void* q, void* k, void* v, void* lengths, uint32_t batch,
+                      uint32_t seq, uint32_t keys, uint32_t heads, uint32_t kvHeads,
+                      uint32_t headDim, uint32_t flags, float scale, AttnArgs* a) {
+  Buffer* Q = as_buffer(q, what);
+  Buffer* K = Q ? as_buffer(k, what) : nullptr;
+  Buffer* V = K ? as_buffer(v, what) : nullptr;
+  Buffer* L = lengths && V ? as_buffer(lengths, what) : nullptr;
+  if (!Q || !K || !V || (lengths && !L)) return false;
+  if (!batch || !seq || !keys || !heads || !kvHeads || heads % kvHeads || !headDim || headDim > 256) {
+    set_error("%s: %u heads over %u key heads of %u values, %u x %u queries, %u keys (no zeros, key "
+              "heads divide heads, at most 256 values)", what, heads, kvHeads, headDim, batch, seq, keys);
+    return false;
+  }
+  const uint64_t vec = uint64_t(heads) * headDim, rows = uint64_t(batch) * seq * heads;
+  // 32-bit offsets inside a key tile, row and workgroup counts below 2^31
+  if (vec * 64 >= kOob || rows >= 0x80000000ull || uint64_t(batch) * keys * kvHeads >= 0x80000000ull) {
+    set_error("%s: %u x %u tokens of %u heads of %u values, %u keys: too many for one call", what,
+              batch, seq, heads, headDim, keys);
+    return false;
+  }
+  const uint64_t nq = rows * headDim, nk = uint64_t(batch) * keys * kvHeads * headDim;
+  if (Q->count < nq || K->count < nk || V->count < nk || (L && L->count < batch)) {
+    set_error("%s: q, k, v%s hold %u, %u, %u values for %u x %u x %u x %u and %u x %u x %u x %u", what,
+              L ? " (or lengths)" : "", Q->count, K->count, V->count, batch, seq, heads, headDim,
+              batch, keys, kvHeads, headDim);
+    return false;
+  }
+  *a = AttnArgs{Q->ptr, K->ptr, V->ptr, L ? L->ptr : nullptr, nullptr, nullptr, batch, seq, keys,
+                heads, kvHeads, headDim, scale, (flags & 1) != 0};
+  return true;
+}
+
+void* AttentionForward(void* q, void* k, void* v, void* lengths, uint32_t batch, uint32_t seq,
+                       uint32_t keys, uint32_t heads, uint32_t kvHeads, uint32_t headDim,
+                       uint32_t flags, float scale, void** pStats) {
+  if (pStats) *pStats = nullptr;
+  if (!ensure_init()) return nullptr;
+  AttnArgs a;
+  if (!attn_args("AttentionForward", q, k, v, lengths, batch, seq, keys, heads, kvHeads, headDim,
+                 flags, scale, &a))
+    return nullptr;
+  const uint32_t rows = batch * seq * heads;
+  void* o = create_buffer(nullptr, rows * headDim);
+  void* st = o && pStats ? create_buffer(nullptr, 2 * rows) : nullptr;
+  if (o && (st || !pStats)) {
+    a.o = static_cast<Buffer*>(o)->ptr;
+    a.stats = st ? static_cast<Buffer*>(st)->ptr : nullptr;
+    if (attention_forward(a)) {
+      if (pStats) *pStats = st;
+      return o;
+    }
+  }
+  if (o) release_buffer(o);
+  if (st) release_buffer(st);
+  return nullptr;
+}
+
+void AttentionBackward(void* gradOut, void* out, void* q, void* k, void* v, void* lengths,
+                       void* stats, uint32_t batch, uint32_t seq, uint32_t keys, uint32_t heads,
+                       uint32_t kvHeads, uint32_t headDim, uint32_t flags, float scale,
+                       uint32_t qReq, uint32_t kReq, uint32_t vReq, void** pDQ, void** pDK,
+                       void** pDV) {
+  if (pDQ) *pDQ = nullptr;
+  if (pDK) *pDK = nullptr;
+  if (pDV) *pDV = nullptr;
+  if (!ensure_init()) return;
+  AttnArgs a;
+  if (!attn_args("AttentionBackward", q, k, v, lengths, batch, seq, keys, heads, kvHeads, headDim,
+                 flags, scale, &a))
+    return;
+  Buffer* DY = as_buffer(gradOut, "AttentionBackward(gradOut)");
+  Buffer* O = DY ? as_buffer(out, "AttentionBackward(out)") : nullptr;
+  Buffer* ST = O ? as_buffer(stats, "AttentionBackward(stats)") : nullptr;
+  if (!ST) return;
+  const uint32_t rows = batch * seq * heads, nq = rows * headDim, nk = batch * keys * kvHeads * headDim;
+  if (DY->count < nq || O->count < nq || ST->count < 2 * rows) {
+    set_error("AttentionBackward: gradOut, out, stats hold %u, %u, %u values for %u rows of %u",
+              DY->count, O->count, ST->count, rows, headDim);
+    return;
+  }
+  a.o = O->ptr;
+  a.stats = ST->ptr;
+  void** want[3] = {qReq ? pDQ : nullptr, kReq ? pDK : nullptr, vReq ? pDV : nullptr};
+  void* got[3] = {nullptr, nullptr, nullptr};
+  float* ptr[3] = {nullptr, nullptr, nullptr};
+  bool ok = true, any = false;
+  for (int i = 0; i < 3 && ok; ++i)
+    if (want[i]) {
+      any = true;
+      got[i] = create_buffer(nullptr, i ? nk : nq);
+      ok = got[i] != nullptr;
+      if (ok) ptr[i] = static_cast<Buffer*>(got[i])->ptr;
+    }
+  if (ok && any) ok = attention_backward(a, DY->ptr, ptr[0], ptr[1], ptr[2]);
+  for (int i = 0; i < 3; ++i) {
+    if (!got[i]) continue;
+    if (ok)
+      *want[i] = got[i];
+    else
+      release_buffer(got[i]);
+  }
+}
+
+bool MuonBatch(void** params, void** grads, void** momenta, uint32_t* rows, uint32_t* cols,
+               float* stepSizes, uint32_t numParams, float momentum, uint32_t nesterov,
+               float weightDecay, float clip, uint32_t steps) {
+  if (!ensure_init()) return false;
+  if (!params || !grads || !momenta || !rows || !cols || !stepSizes) {
+    set_error("MuonBatch: NULL table");
+    return false;
+  }
+  if (steps < 1 || steps > 20) {
+    set_error("MuonBatch: %u steps (1 to 20)", steps);
+    return false;
+  }
+  drop_tags(params, numParams);
+  drop_tags(momenta, numParams);
+  return muon_multi(params, grads, momenta, rows, cols, stepSizes, numParams, momentum,
+                    nesterov != 0, weightDecay, clip, steps);
+}
+
 // ----------------------------------------------------------------- profiling
 void SetProfiling(int enabled) {
   if (!enabled) resolve_profile();

@@ -494,6 +494,33 @@ bool conv_backward(const float* dy, const float* y, const float* x, const float*
 bool gemm(const float* a, const float* b, float* c, uint32_t M, uint32_t K,
           uint32_t N, uint32_t flags);
 
+// Rotary positions (dce_rotary.hip): y = x with the first `rot` values of every
+// head turned in pairs; table [rows][rot / 2][cos, sin], pos one table row per
+// token (null: token % S).
+bool rotary(const float* x, const float* table, const float* pos, float* y, uint32_t tokens,
+            uint32_t S, uint32_t H, uint32_t D, uint32_t rot, uint32_t rows, bool interleaved,
+            bool inverse);
+
+// Attention (dce_attention.hip).  q, o: [B][S][H][D], k, v: [B][T][G][D], H a
+// multiple of G; len: B key counts as floats, or null (T); stats: 2 B H S
+// floats that the forward leaves for the backward (null: not kept).
+struct AttnArgs {
+  const float *q, *k, *v, *len;
+  float *o, *stats;
+  uint32_t B, S, T, H, G, D;
+  float scale;
+  bool causal;
+};
+bool attention_forward(const AttnArgs& x);
+// x.o, x.stats: the forward's.  dq, dk, dv: null when not wanted.
+bool attention_backward(const AttnArgs& x, const float* dy, float* dq, float* dk, float* dv);
+
+// Orthogonalised momentum update (dce_muon.hip) of n matrices of rows[i] x
+// cols[i] values; entries with a null param or grad are skipped.
+bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* rows,
+                const uint32_t* cols, const float* stepSizes, uint32_t n, float mu, bool nesterov,
+                float decay, float clip, uint32_t steps);
+
 // Profiling hooks (dce_engine.hip): kernel-family timing with HIP events on
 // the engine stream.  `family` is a short static string.
 struct ProfScope {

@@ -1,0 +1,557 @@
+// The orthogonalised momentum update of many matrices at once.
+//
+//   m <- mu m + g,  d = g + mu m (or m),  X = d / (|d| + eps),
+//   five times:  A = X X^T,  B = b A + c A^2,  X <- a X + B X,
+//   w <- w - decay w - step X.
+//
+// The quintic a s + b s^3 + c s^5 takes every singular value s of X towards 1
+// (K. Jordan, "Muon: an optimizer for hidden layers in neural networks", 2024,
+// whose coefficients these are): X tends to the orthogonal factor of d.  A
+// matrix with more rows than columns is worked on transposed, so that A is the
+// smaller Gram matrix.
+//
+// Every matrix of a call runs in the same launches: a workgroup finds its
+// matrix and tile in a table that travels as a kernel argument.  A and A^2 are
+// symmetric: only tiles on or above the diagonal are multiplied, and stored
+// twice.  A Gram product with long dot products and few tiles is split over
+// them and summed by a pass of its own.
+//
+// Products: a value is kept as two fp16 parts, x 2^e = h + l, each rounded to
+// nearest, and h h + (h l + l h) stands for the product: 22 to 24 bits at a
+// third of the fp16 MFMA rate, which is 16 times the fp32 one.  Ranges are
+// known, so the exponents are fixed: |X| <= 1.21 (|d| bounds its singular
+// values by 1, and the quintic's largest value on [0, 1.21] is 1.21), |A| <=
+// 1.47, |B| <= 2.81.  X is normalised, so its typical value is at least 2^-16
+// and l's smallest step, 2^-39, is below the fp32 rounding of such a value.  X
+// itself stays in fp32, for the term a X.  The two small products have an
+// accumulator of their own: an MFMA cuts what it adds off at the scale of the
+// largest addend, always downwards.
+#include "dce_internal.h"
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+namespace dce {
+
+namespace {
+
+constexpr int kT = 256;
+constexpr int kBlk = 128;     // tile of a product
+constexpr int kStep = 32;     // its depth per LDS stage
+constexpr int kMaxM = 40;     // matrices of a launch
+constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
+constexpr int kExpX = 15, kExpA = 14;  // parts hold X 2^15, A 2^14, B 2^14
+
+using h8 = _Float16 __attribute__((ext_vector_type(8)));
+using f16v = float __attribute__((ext_vector_type(16)));
+
+// One matrix, r x c as the caller has it; m <= n after the transposition.
+struct Mat {
+  float *w, *g, *mom;
+  uint32_t m, n, mp, np;  // padded to whole tiles (zeros)
+  uint32_t tall, splits;
+  float step;
+  uint32_t x, xp, xt[2], a, b, part;  // places in the workspace, in units of 64 floats
+};
+struct Mats {
+  Mat t[kMaxM];
+  uint32_t start[kMaxM + 1];  // first workgroup of each
+  uint32_t count;
+};
+__device__ __forceinline__ int find_mat(const Mats& t, uint32_t blk) {
+  int lo = 0, hi = int(t.count) - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.start[mid] <= blk) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+__device__ __forceinline__ float* at(float* ws, uint32_t place) { return ws + size_t(place) * 64; }
+
+// Parts in memory: 8 consecutive values of a row are 8 h, then 8 l (32 bytes).
+__device__ __forceinline__ void split8(const float* x, float by, h8& h, h8& l) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = x[e] * by;
+    h[e] = _Float16(v);
+    l[e] = _Float16(v - float(h[e]));
+  }
+}
+__device__ __forceinline__ void put8(float* row, uint32_t k, const float* x, float by) {
+  h8 h, l;
+  split8(x, by, h, l);
+  h8* p = reinterpret_cast<h8*>(row + k);
+  p[0] = h;
+  p[1] = l;
+}
+
+// ---------------------------------------------------------------------------
+// d = g + mu m, m <- mu m + g, and the sums of d^2 (in double, one per
+// workgroup of 4096 values); d goes to X's place, as the caller's matrix lies.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kChunk = 4096;
+__global__ void __launch_bounds__(kT)
+    k_muon_momentum(const Mats t, float* ws, double* sums, float mu, float clip, int nesterov) {
+  __shared__ double sh[4];
+  const int i = find_mat(t, blockIdx.x);
+  const Mat& M = t.t[i];
+  const uint32_t n = M.m * M.n, c0 = (blockIdx.x - t.start[i]) * kChunk;
+  float* d = at(ws, M.xt[1]);  // free until the first step
+  double sum = 0;
+#pragma unroll 4
+  for (uint32_t k = c0 + threadIdx.x; k < min(n, c0 + kChunk); k += kT) {
+    float g = M.g[k];
+    if (g > clip) g = clip;
+    if (g < -clip) g = -clip;
+    const float m = mu * M.mom[k] + g;
+    M.mom[k] = m;
+    const float v = nesterov ? mu * m + g : m;
+    d[k] = v;
+    sum += double(v) * v;
+  }
+  sum = block_sum256(sum, sh);
+  if (threadIdx.x == 0) sums[blockIdx.x] = sum;
+}
+
+// 1 / (|d| + eps) of each matrix.
+__global__ void __launch_bounds__(kT) k_muon_norm(const Mats t, const double* sums, float* inv) {
+  __shared__ double sh[4];
+  const uint32_t i = blockIdx.x;
+  double s = 0;
+  for (uint32_t k = t.start[i] + threadIdx.x; k < t.start[i + 1]; k += kT) s += sums[k];
+  s = block_sum256(s, sh);
+  if (threadIdx.x == 0) inv[i] = float(1.0 / (sqrt(s) + 1e-7));
+}
+
+// A 64 x 64 tile through LDS: X in fp32 and as parts, along rows and columns.
+constexpr int kSq = 64, kPitch = 68;
+__device__ __forceinline__ void put_tile(const float (&S)[kSq * kPitch], float* rows, uint32_t rowPitch,
+                                         float* cols, uint32_t colPitch, uint32_t i0, uint32_t j0) {
+#pragma unroll
+  for (int u = 0; u < kSq * kSq / 8 / kT; ++u) {
+    const uint32_t slot = threadIdx.x + kT * u;
+    float v[8];
+    {
+      const uint32_t r = slot / 8, k = slot % 8 * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = S[r * kPitch + k + e];
+      put8(rows + size_t(i0 + r) * rowPitch, j0 + k, v, ldexpf(1.f, kExpX));
+    }
+    {
+      const uint32_t r = slot % 64, k = slot / 64 * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = S[(k + e) * kPitch + r];
+      put8(cols + size_t(j0 + r) * colPitch, i0 + k, v, ldexpf(1.f, kExpX));
+    }
+  }
+}
+__global__ void __launch_bounds__(kT) k_muon_scale(const Mats t, float* ws, const float* inv) {
+  __shared__ float S[kSq * kPitch];
+  const int i = find_mat(t, blockIdx.x);
+  const Mat& M = t.t[i];
+  const uint32_t tn = M.np / kSq, id = blockIdx.x - t.start[i], i0 = id / tn * kSq, j0 = id % tn * kSq;
+  const float by = inv[i];
+  const float* d = at(ws, M.xt[1]);
+  float* x = at(ws, M.x);
+#pragma unroll 4
+  for (int u = 0; u < kSq * kSq / kT; ++u) {
+    const uint32_t s = threadIdx.x + kT * u;
+    // consecutive threads along the caller's rows
+    const uint32_t r = M.tall ? s % kSq : s / kSq, c = M.tall ? s / kSq : s % kSq, mi = i0 + r, nj = j0 + c;
+    const bool ok = mi < M.m && nj < M.n;
+    S[r * kPitch + c] = ok ? d[M.tall ? size_t(nj) * M.m + mi : size_t(mi) * M.n + nj] * by : 0.f;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int u = 0; u < kSq * kSq / kT; ++u) {
+    const uint32_t s = threadIdx.x + kT * u, r = s / kSq, c = s % kSq;
+    x[size_t(i0 + r) * M.np + j0 + c] = S[r * kPitch + c];
+  }
+  put_tile(S, at(ws, M.xp), M.np, at(ws, M.xt[0]), M.mp, i0, j0);
+}
+
+// w <- w - decay w - step X
+__global__ void __launch_bounds__(kT) k_muon_update(const Mats t, float* ws, float decay) {
+  __shared__ float S[kSq * kPitch];
+  const int i = find_mat(t, blockIdx.x);
+  const Mat& M = t.t[i];
+  const uint32_t tn = M.np / kSq, id = blockIdx.x - t.start[i], i0 = id / tn * kSq, j0 = id % tn * kSq;
+  const float* x = at(ws, M.x);
+#pragma unroll 4
+  for (int u = 0; u < kSq * kSq / kT; ++u) {
+    const uint32_t s = threadIdx.x + kT * u, r = s / kSq, c = s % kSq;
+    S[r * kPitch + c] = x[size_t(i0 + r) * M.np + j0 + c];
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int u = 0; u < kSq * kSq / kT; ++u) {
+    const uint32_t s = threadIdx.x + kT * u;
+    const uint32_t r = M.tall ? s % kSq : s / kSq, c = M.tall ? s / kSq : s % kSq, mi = i0 + r, nj = j0 + c;
+    if (mi < M.m && nj < M.n) {
+      float* w = M.w + (M.tall ? size_t(nj) * M.m + mi : size_t(mi) * M.n + nj);
+      *w = *w - decay * *w - M.step * S[r * kPitch + c];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Products C = P Q^T of parts, both along their rows, in 128 x 128 tiles: four
+// waves of 64 x 64 (2 x 2 blocks of 32 x 32), the depth in steps of 32 through
+// two LDS stages, the next one's direct loads in flight while one is multiplied.
+// A stage row is 128 bytes (4 blocks of 8 h, 8 l); its 16-byte slots are XORed
+// by row % 8, so that eight rows' equal slots lie in different banks.
+// ---------------------------------------------------------------------------
+enum Op { GRAM, POLY, APPLY, LAST };
+constexpr int kStage = kBlk * kStep * 4;  // bytes of one operand's stage
+constexpr int kCp = 132;                  // pitch of the result tile in LDS
+constexpr int kLds = 4 * kStage > kBlk * kCp * 4 ? 4 * kStage : kBlk * kCp * 4;
+
+__device__ __forceinline__ void stage_load(const BRes& b, uint32_t pitchBytes, uint32_t k, char* S) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+  for (int i = 0; i < kStage / 16 / kT; ++i) {
+    const uint32_t slot = threadIdx.x + kT * i, row = slot >> 3, c = (slot & 7) ^ (row & 7);
+    b.ld16_lds(row * pitchBytes + k * 4 + c * 16, S + (wave * 64 + i * kT) * 16);
+  }
+}
+__device__ __forceinline__ h8 stage_frag(const char* S, int row, int c) {
+  return *reinterpret_cast<const h8*>(S + row * 128 + ((c ^ (row & 7)) * 16));
+}
+// Tile (i, j), i <= j, of the upper triangle in row order.
+__device__ __forceinline__ void triangle(uint32_t id, uint32_t n, uint32_t& i, uint32_t& j) {
+  i = 0;
+  while (id >= n - i) {
+    id -= n - i;
+    ++i;
+  }
+  j = i + id;
+}
+
+template <Op OP>
+__global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2)))
+    k_muon_product(const Mats t, float* ws, uint32_t cur) {
+  __shared__ __attribute__((aligned(16))) char S[kLds];
+  const uint32_t blk = xcd_block_id();
+  const int mi = find_mat(t, blk);
+  const Mat& M = t.t[mi];
+  uint32_t id = blk - t.start[mi], ti, tj, sp = 0;
+  const uint32_t tm = M.mp / kBlk;
+  uint32_t depth = OP == GRAM ? M.np : M.mp, k0 = 0;
+  if constexpr (OP == GRAM) {
+    const uint32_t tiles = tm * (tm + 1) / 2;
+    sp = id / tiles;
+    id -= sp * tiles;
+    const uint32_t steps = depth / kStep;
+    k0 = uint32_t(uint64_t(steps) * sp / M.splits) * kStep;
+    depth = uint32_t(uint64_t(steps) * (sp + 1) / M.splits) * kStep;
+  }
+  if constexpr (OP == GRAM || OP == POLY) {
+    triangle(id, tm, ti, tj);
+  } else {
+    ti = id % tm;
+    tj = id / tm;
+  }
+  const float* P = at(ws, OP == GRAM ? M.xp : OP == POLY ? M.a : M.b);
+  const float* Q = at(ws, OP == GRAM ? M.xp : OP == POLY ? M.a : M.xt[cur]);
+  const uint32_t pitch = OP == GRAM ? M.np : M.mp;
+  BRes bp, bq;
+  bp.init(P + size_t(ti) * kBlk * pitch, kBlk * pitch);
+  bq.init(Q + size_t(tj) * kBlk * pitch, kBlk * pitch);
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  const int col = lane & 31, half = lane >> 5;
+  f16v big[2][2], small[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) big[i][j][e] = small[i][j][e] = 0.f;
+
+  stage_load(bp, pitch * 4, k0, S);
+  stage_load(bq, pitch * 4, k0, S + kStage);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  int s = 0;
+  for (uint32_t k = k0; k < depth; k += kStep, s ^= 1) {
+    const char* Sp = S + s * 2 * kStage;
+    const char* Sq = Sp + kStage;
+    // Fragments first: a direct load in flight would make the compiler wait
+    // for it before any LDS read.
+    h8 p[2][2][2], q[2][2][2];  // [16-deep step][block][h, l]
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          p[kk][i][e] = stage_frag(Sp, wm + 32 * i + col, 2 * (2 * kk + half) + e);
+          q[kk][i][e] = stage_frag(Sq, wn + 32 * i + col, 2 * (2 * kk + half) + e);
+        }
+    if (k + kStep < depth) {
+      char* N = S + (s ^ 1) * 2 * kStage;
+      stage_load(bp, pitch * 4, k + kStep, N);
+      stage_load(bq, pitch * 4, k + kStep, N + kStage);
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          big[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][0], big[i][j], 0, 0, 0);
+          small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][1], small[i][j], 0, 0, 0);
+          small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][1], q[kk][j][0], small[i][j], 0, 0, 0);
+        }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+  // The tile in LDS, in its own scale.
+  float* C = reinterpret_cast<float*>(S);
+  const float unit = OP == GRAM ? ldexpf(1.f, -2 * kExpX) : OP == POLY ? ldexpf(1.f, -2 * kExpA)
+                                                                       : ldexpf(1.f, -kExpX - kExpA);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        C[(wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3)) * kCp + wn + 32 * j + col] =
+            (big[i][j][e] + small[i][j][e]) * unit;
+  __syncthreads();
+  const uint32_t i0 = ti * kBlk, j0 = tj * kBlk;
+  if constexpr (OP == GRAM) {
+    if (M.splits > 1) {  // summed by k_muon_sum
+      float* out = at(ws, M.part) + (size_t(sp) * (tm * (tm + 1) / 2) + id) * (kBlk * kBlk);
+#pragma unroll 4
+      for (int u = 0; u < kBlk * kBlk / 4 / kT; ++u) {
+        const uint32_t slot = threadIdx.x + kT * u;
+        *reinterpret_cast<f4*>(out + slot * 4) = *reinterpret_cast<const f4*>(C + (slot >> 5) * kCp + (slot & 31) * 4);
+      }
+      return;
+    }
+  }
+  float* out = at(ws, OP == GRAM ? M.a : OP == POLY ? M.b : M.xp);
+#pragma unroll 1
+  for (int u = 0; u < kBlk * kBlk / 8 / kT; ++u) {
+    const uint32_t slot = threadIdx.x + kT * u, r = slot >> 4, k = (slot & 15) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = C[r * kCp + k + e];
+    if constexpr (OP == POLY) {  // B = b A + c A^2
+      const h8* a = reinterpret_cast<const h8*>(at(ws, M.a) + size_t(i0 + r) * M.mp + j0 + k);
+      const h8 ah = a[0], al = a[1];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v[e] = kB * ((float(ah[e]) + float(al[e])) * ldexpf(1.f, -kExpA)) + kC * v[e];
+    }
+    if constexpr (OP == APPLY || OP == LAST) {  // X <- a X + B X
+      float* x = at(ws, M.x) + size_t(i0 + r) * M.np + j0 + k;
+      f4 x0 = reinterpret_cast<const f4*>(x)[0], x1 = reinterpret_cast<const f4*>(x)[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = x0[e] = kA * x0[e] + v[e];
+        v[4 + e] = x1[e] = kA * x1[e] + v[4 + e];
+      }
+      reinterpret_cast<f4*>(x)[0] = x0;
+      reinterpret_cast<f4*>(x)[1] = x1;
+    }
+    if constexpr (OP != LAST)
+      put8(out + size_t(i0 + r) * (OP == APPLY ? M.np : M.mp), j0 + k, v, ldexpf(1.f, OP == APPLY ? kExpX : kExpA));
+    if constexpr (OP == POLY || OP == APPLY) {  // for the transposed copy
+#pragma unroll
+      for (int e = 0; e < 8; ++e) C[r * kCp + k + e] = v[e];
+    }
+  }
+  if constexpr (OP == LAST) return;
+  if ((OP == GRAM || OP == POLY) && ti == tj) return;
+  __syncthreads();
+  float* tr = OP == APPLY ? at(ws, M.xt[cur ^ 1]) : out;
+#pragma unroll 1
+  for (int u = 0; u < kBlk * kBlk / 8 / kT; ++u) {
+    const uint32_t slot = threadIdx.x + kT * u, r = slot & 127, k = (slot >> 7) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = C[(k + e) * kCp + r];
+    put8(tr + size_t(j0 + r) * M.mp, i0 + k, v, ldexpf(1.f, OP == APPLY ? kExpX : kExpA));
+  }
+}
+
+// A from the partial tiles of a split Gram product: a workgroup per 32 x 128
+// piece of a tile, eight values a thread at a time.
+__global__ void __launch_bounds__(kT) k_muon_sum(const Mats t, float* ws) {
+  __shared__ float C[32 * kCp];
+  const int mi = find_mat(t, blockIdx.x);
+  const Mat& M = t.t[mi];
+  const uint32_t id = blockIdx.x - t.start[mi], piece = id & 3, tile = id >> 2, tm = M.mp / kBlk;
+  const uint32_t tiles = tm * (tm + 1) / 2;
+  uint32_t ti, tj;
+  triangle(tile, tm, ti, tj);
+  const float* part = at(ws, M.part) + size_t(tile) * (kBlk * kBlk) + piece * 32 * kBlk;
+  float* a = at(ws, M.a);
+  const uint32_t i0 = ti * kBlk + piece * 32, j0 = tj * kBlk;
+#pragma unroll
+  for (int u = 0; u < 32 * kBlk / 8 / kT; ++u) {
+    const uint32_t slot = threadIdx.x + kT * u, r = slot >> 4, k = (slot & 15) * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (uint32_t s = 0; s < M.splits; ++s) {
+      const f4* p = reinterpret_cast<const f4*>(part + size_t(s) * tiles * (kBlk * kBlk) + slot * 8);
+      const f4 p0 = p[0], p1 = p[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] += p0[e];
+        v[4 + e] += p1[e];
+      }
+    }
+    put8(a + size_t(i0 + r) * M.mp, j0 + k, v, ldexpf(1.f, kExpA));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) C[r * kCp + k + e] = v[e];
+  }
+  if (ti == tj) return;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 32 * kBlk / 8 / kT; ++u) {
+    const uint32_t slot = threadIdx.x + kT * u, r = slot & 127, k = (slot >> 7) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = C[(k + e) * kCp + r];
+    put8(a + size_t(j0 + r) * M.mp, i0 + k, v, ldexpf(1.f, kExpA));
+  }
+}
+
+inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b); }
+inline uint32_t pad(uint32_t v) { return (v + kBlk - 1) / kBlk * kBlk; }
+
+// start[] for `f(matrix)` workgroups each; returns their number.
+template <class F>
+uint32_t blocks(Mats& t, F&& f) {
+  uint32_t n = 0;
+  for (uint32_t i = 0; i < t.count; ++i) {
+    t.start[i] = n;
+    n += f(t.t[i]);
+  }
+  t.start[t.count] = n;
+  return n;
+}
+
+struct Places {
+  size_t next = 0;  // in units of 64 floats
+  uint32_t take(size_t floats) {
+    const size_t p = next;
+    next += (floats + 63) / 64;
+    return uint32_t(p);
+  }
+};
+
+bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32_t steps) {
+  // A Gram product is split so that no workgroup has more than 1 / (2 CUs) of
+  // the launch's steps, and none fewer than 8.
+  auto tri = [](const Mat& m) { return m.mp / kBlk * (m.mp / kBlk + 1) / 2; };
+  double all = 0;
+  for (uint32_t i = 0; i < t.count; ++i) all += double(tri(t.t[i])) * (t.t[i].np / kStep);
+  const double most = std::max(8.0, std::ceil(all / (2.0 * num_cus())));
+  Places at;
+  size_t chunks = 0;
+  bool split = false;
+  for (uint32_t i = 0; i < t.count; ++i) {
+    Mat& m = t.t[i];
+    m.splits = std::max<uint32_t>(1, uint32_t(std::ceil((m.np / kStep) / most)));
+    split |= m.splits > 1;
+    const size_t xn = size_t(m.mp) * m.np, an = size_t(m.mp) * m.mp;
+    m.x = at.take(xn);
+    m.xp = at.take(xn);
+    m.xt[0] = at.take(xn);
+    m.xt[1] = at.take(xn);
+    m.a = at.take(an);
+    m.b = at.take(an);
+    m.part = m.splits > 1 ? at.take(size_t(m.splits) * tri(m) * kBlk * kBlk) : 0;
+    chunks += cdiv(size_t(m.m) * m.n, kChunk);
+  }
+  const size_t sums = at.take(2 * chunks), inv = at.take(kMaxM);
+  float* ws = workspace(at.next * 64);
+  if (!ws) return false;
+  double* dsum = reinterpret_cast<double*>(ws + sums * 64);
+  float* dinv = ws + inv * 64;
+
+  uint32_t n = blocks(t, [](const Mat& m) { return cdiv(size_t(m.m) * m.n, kChunk); });
+  hipLaunchKernelGGL(k_muon_momentum, dim3(n), dim3(kT), 0, stream(), t, ws, dsum, mu, clip, int(nesterov));
+  hipLaunchKernelGGL(k_muon_norm, dim3(t.count), dim3(kT), 0, stream(), t, dsum, dinv);
+  auto squares = [](const Mat& m) { return m.mp / kSq * (m.np / kSq); };
+  n = blocks(t, squares);
+  hipLaunchKernelGGL(k_muon_scale, dim3(n), dim3(kT), 0, stream(), t, ws, dinv);
+  for (uint32_t s = 0; s < steps; ++s) {
+    n = blocks(t, [&](const Mat& m) { return tri(m) * m.splits; });
+    hipLaunchKernelGGL(k_muon_product<GRAM>, dim3(n), dim3(kT), 0, stream(), t, ws, s & 1);
+    if (split) {
+      n = blocks(t, [&](const Mat& m) { return m.splits > 1 ? tri(m) * 4 : 0; });
+      hipLaunchKernelGGL(k_muon_sum, dim3(n), dim3(kT), 0, stream(), t, ws);
+    }
+    n = blocks(t, tri);
+    hipLaunchKernelGGL(k_muon_product<POLY>, dim3(n), dim3(kT), 0, stream(), t, ws, s & 1);
+    n = blocks(t, [](const Mat& m) { return m.mp / kBlk * (m.np / kBlk); });
+    if (s + 1 < steps)
+      hipLaunchKernelGGL(k_muon_product<APPLY>, dim3(n), dim3(kT), 0, stream(), t, ws, s & 1);
+    else
+      hipLaunchKernelGGL(k_muon_product<LAST>, dim3(n), dim3(kT), 0, stream(), t, ws, s & 1);
+  }
+  n = blocks(t, squares);
+  hipLaunchKernelGGL(k_muon_update, dim3(n), dim3(kT), 0, stream(), t, ws, decay);
+  return check_launch("MuonBatch");
+}
+
+}  // namespace
+
+bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* rows, const uint32_t* cols,
+                const float* stepSizes, uint32_t n, float mu, bool nesterov, float decay, float clip,
+                uint32_t steps) {
+  std::vector<Mat> all;
+  double bytes = 0, flops = 0;
+  for (uint32_t i = 0; i < n; ++i) {
+    if (!params[i] || !grads[i]) continue;
+    Buffer* W = as_buffer(params[i], "MuonBatch(param)");
+    Buffer* G = as_buffer(grads[i], "MuonBatch(grad)");
+    Buffer* V = as_buffer(momenta[i], "MuonBatch(momentum)");
+    if (!W || !G || !V) return false;
+    const uint64_t size = uint64_t(rows[i]) * cols[i];
+    if (!size || size >= 0x80000000ull || W->count < size || G->count < size || V->count < size) {
+      set_error("MuonBatch: matrix %u of %u x %u does not fit its buffers", i, rows[i], cols[i]);
+      return false;
+    }
+    Mat m{};
+    m.w = W->ptr;
+    m.g = G->ptr;
+    m.mom = V->ptr;
+    m.tall = rows[i] > cols[i];
+    m.m = std::min(rows[i], cols[i]);
+    m.n = std::max(rows[i], cols[i]);
+    m.mp = pad(m.m);
+    m.np = pad(m.n);
+    m.step = stepSizes[i];
+    // a tile's operand rows are reached with 32-bit offsets
+    if (uint64_t(m.np) * kBlk >= kOob) {
+      set_error("MuonBatch: matrix %u has %u columns: too many", i, m.n);
+      return false;
+    }
+    all.push_back(m);
+    bytes += 20.0 * size;
+    flops += steps * (3.0 * m.m * m.m * m.n + double(m.m) * m.m * m.m);
+  }
+  if (all.empty()) return true;
+  ProfScope prof("muon", flops, bytes);
+  // Groups of up to kMaxM matrices, and of up to 2^28 values unless one is larger.
+  for (size_t i = 0; i < all.size();) {
+    Mats t{};
+    size_t values = 0;
+    while (i < all.size() && t.count < uint32_t(kMaxM) &&
+           (!t.count || values + size_t(all[i].mp) * all[i].np <= (size_t(1) << 28))) {
+      values += size_t(all[i].mp) * all[i].np;
+      t.t[t.count++] = all[i++];
+    }
+    if (!run_group(t, mu, nesterov, decay, clip, steps)) return false;
+  }
+  return true;
+}
+
+}  // namespace dce

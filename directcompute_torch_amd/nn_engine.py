@@ -11,9 +11,9 @@ Importing this module initialises the HIP device (as the reference
 initialises D3D11 at import, nn_engine.py:121) and raises if that fails --
 there is no CPU fallback.
 
-Not provided (outside the backward path): custom HLSL shaders, the
-GELU / LayerNorm / attention family (their kernels do not exist in the
-reference tree), ONNX export/import, Muon, and the Python-side profilers.
+Not provided (outside the backward path): custom HLSL shaders, GELU and
+LayerNorm (their kernels do not exist in the reference tree), ONNX
+export/import, and the Python-side profilers.
 """
 from __future__ import annotations
 
@@ -833,6 +833,111 @@ class BatchNorm2dFunc(Function):
         self.batch_mean_handle = self.batch_var_handle = None
 
 
+class Reshape(Function):
+    """The same buffer under another shape (a new reference, as Flatten)."""
+
+    def forward(self, x, shape):
+        shape = tuple(int(d) for d in shape)
+        if _shape_size(shape) != x.size or any(d < 1 for d in shape):
+            raise ValueError(f"reshape: {tuple(x.shape)} does not hold the values of {shape}")
+        self.inputs = (x,)
+        lib.AddRefBuffer(x.gpu_buf)
+        res = Tensor.from_gpu(x.gpu_buf, shape, requires_grad=x.requires_grad, track=False)
+        res._ctx = self
+        return res
+
+    def backward(self, grad_output):
+        x = self.inputs[0]
+        if x.requires_grad:
+            lib.AddRefBuffer(grad_output.gpu_buf)
+            x._accumulate_grad(Tensor.from_gpu(grad_output.gpu_buf, x.shape, track=False))
+
+
+class RotaryFunc(Function):
+    """RotaryApply; the gradient is the rotation by the opposite angles."""
+
+    def forward(self, x, table, positions=None, interleaved=False):
+        if len(x.shape) != 4:
+            raise ValueError(f"rotary: x is (batch, seq, heads, head_dim), not {tuple(x.shape)}")
+        if len(table.shape) != 3 or table.shape[2] != 2:
+            raise ValueError(f"rotary: the table is (positions, pairs, 2), not {tuple(table.shape)}")
+        if positions is not None and tuple(positions.shape) != tuple(x.shape[:2]):
+            raise ValueError(f"rotary: positions of {tuple(positions.shape)} for tokens of {tuple(x.shape[:2])}")
+        if positions is None and x.shape[1] > table.shape[0]:
+            raise ValueError(f"rotary: {x.shape[1]} tokens, {table.shape[0]} positions in the table")
+        self.inputs = (x,)
+        self.table, self.positions, self.flags = table, positions, 1 if interleaved else 0
+        res = Tensor.from_gpu(self._apply(x, self.flags), x.shape, requires_grad=x.requires_grad)
+        res._ctx = self
+        return res
+
+    def _apply(self, x, flags):
+        pos = self.positions.gpu_buf if self.positions is not None else None
+        return _check(lib.RotaryApply(x.gpu_buf, self.table.gpu_buf, pos, *x.shape, 2 * self.table.shape[1],
+                                      flags), "RotaryApply")
+
+    def backward(self, grad_output):
+        x = self.inputs[0]
+        if x.requires_grad:
+            g = Tensor.from_gpu(self._apply(grad_output, self.flags | 2), x.shape, track=True)
+            x._accumulate_grad(g)
+
+
+class AttentionFunc(Function):
+    """AttentionForward / AttentionBackward, which computes the probabilities
+    again from two statistics per row (`stats_handle`, owned by this node)."""
+
+    def __del__(self):
+        h = getattr(self, "stats_handle", None)
+        if h:
+            try:
+                lib.ReleaseBuffer(h)
+            except Exception:
+                pass
+            self.stats_handle = None
+
+    def forward(self, q, k, v, causal=False, scale=None, lengths=None):
+        if len(q.shape) != 4 or len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape):
+            raise ValueError("attention: q is (batch, seq, heads, head_dim), k and v alike (batch, keys, kv_heads, "
+                             f"head_dim); got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+        B, S, H, D = q.shape
+        T, G = k.shape[1], k.shape[2]
+        if k.shape[0] != B or k.shape[3] != D or H % G:
+            raise ValueError(f"attention: q {tuple(q.shape)} does not go with k {tuple(k.shape)}: same batch and "
+                             "head_dim, heads a multiple of the key heads")
+        if lengths is not None and lengths.size != B:
+            raise ValueError(f"attention: {lengths.size} lengths for {B} sequences")
+        self.inputs = (q, k, v)
+        self.lengths = lengths
+        self.dims = (B, S, T, H, G, D, 1 if causal else 0, float(scale) if scale is not None else D ** -0.5)
+        req = q.requires_grad or k.requires_grad or v.requires_grad
+        st = ctypes.c_void_p()
+        h = lib.AttentionForward(q.gpu_buf, k.gpu_buf, v.gpu_buf, self._lengths(), *self.dims,
+                                 ctypes.byref(st) if req else None)
+        _check(h, "AttentionForward")
+        self.stats_handle = st.value
+        res = Tensor.from_gpu(h, q.shape, requires_grad=req)
+        # kept by handle: a reference to `res` itself would be a cycle
+        self.out_handle = h
+        res._ctx = self
+        return res
+
+    def _lengths(self):
+        return self.lengths.gpu_buf if self.lengths is not None else None
+
+    def backward(self, grad_output):
+        q, k, v = self.inputs
+        got = [ctypes.c_void_p() for _ in range(3)]
+        want = [1 if t.requires_grad else 0 for t in (q, k, v)]
+        lib.AttentionBackward(grad_output.gpu_buf, self.out_handle, q.gpu_buf, k.gpu_buf, v.gpu_buf, self._lengths(),
+                              self.stats_handle, *self.dims, *want, *[ctypes.byref(p) for p in got])
+        if any(w and not p.value for w, p in zip(want, got)):
+            raise RuntimeError(f"AttentionBackward failed: {last_error()}")
+        for t, p in zip((q, k, v), got):
+            if p.value:
+                t._accumulate_grad(Tensor.from_gpu(p.value, t.shape, track=True))
+
+
 def _absent(name):
     def f(*args, **kwargs):
         raise NotImplementedError(f"{name}: its kernels do not exist in the reference tree "
@@ -842,7 +947,6 @@ def _absent(name):
 
 gelu = _absent("gelu")
 layernorm = _absent("layernorm")
-attention = _absent("attention")
 
 
 def matmul(A, B, transA=False, transB=False): return MatMul().forward(A, B, transA, transB)
@@ -862,6 +966,48 @@ def dice_loss(pred, target): return DiceLossFunc().forward(pred, target)
 def add(A, B): return AddFunc().forward(A, B)
 def depthwise_conv2d(x, f, b, stride=1, padding=0): return DepthwiseConv2DFunc().forward(x, f, b, stride, padding)
 def global_avg_pool2d(x): return GlobalAvgPool2DFunc().forward(x)
+
+
+def reshape(x, shape): return Reshape().forward(x, shape)
+
+
+def rotary(x, table, positions=None, interleaved=False):
+    """x (batch, seq, heads, head_dim) with the first 2 * table.shape[1] values
+    of every head turned by its position's row of `table` (rotary_table).
+    positions: a (batch, seq) tensor of whole numbers; None: 0 .. seq - 1.  A
+    position outside the table turns into zeros.  The pairs are values (2i,
+    2i + 1) when interleaved, else (i, i + pairs)."""
+    return RotaryFunc().forward(x, table, positions, interleaved)
+
+
+def attention(q, k, v, causal=False, scale=None, lengths=None):
+    """softmax(scale * q k^T + mask) v per head.  q: (batch, seq, heads,
+    head_dim); k, v: (batch, keys, kv_heads, head_dim), kv_heads dividing heads
+    (query head h reads key head h * kv_heads // heads), head_dim up to 256.
+    causal: query i sees keys up to i + keys - seq.  lengths: a tensor of batch
+    values, the keys of each sequence that count; None: all.  scale: 1 /
+    sqrt(head_dim) by default.  A query that sees no key gets zeros."""
+    return AttentionFunc().forward(q, k, v, causal, scale, lengths)
+
+
+def rotary_table(positions, rotary_dim, base=10000.0, factor=1.0, original=None, ramp=(1.0, 32.0)):
+    """(positions, rotary_dim / 2, 2) tensor of cos and sin of position * f_i,
+    f_i = base ** (-2 i / rotary_dim), evaluated in float64.  factor > 1
+    stretches it for contexts longer than the model was trained on: without
+    `original` every f_i is divided by it; with the trained context `original`,
+    a pair that makes at least ramp[1] turns in it keeps its f_i, one of at most
+    ramp[0] turns is divided, and those between go over linearly in their turns
+    (B. Peng, J. Quesnelle, H. Fan, E. Shippole, "YaRN", 2023)."""
+    if positions < 1 or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_table: {positions} positions of {rotary_dim} values (an even number)")
+    f = float(base) ** (-np.arange(0, rotary_dim, 2, dtype=np.float64) / rotary_dim)
+    if factor != 1.0:
+        keep = 0.0
+        if original is not None:
+            keep = np.clip((original * f / (2 * np.pi) - ramp[0]) / (ramp[1] - ramp[0]), 0.0, 1.0)
+        f = keep * f + (1.0 - keep) * f / factor
+    angles = np.arange(positions, dtype=np.float64)[:, None] * f
+    return Tensor(np.stack([np.cos(angles), np.sin(angles)], -1), track=False)
 
 
 def batchnorm2d(x, gamma, beta, rm, rv, eps=1e-5, momentum=0.1, training=True):
@@ -953,6 +1099,17 @@ class BatchNorm2d:
     def __call__(self, x):
         return batchnorm2d(x, self.gamma, self.beta, self.running_mean, self.running_var, self.eps,
                            self.momentum, self.training)
+
+
+class Rotary:
+    """Rotary positions with their table: no parameters."""
+
+    def __init__(self, max_positions, rotary_dim, base=10000.0, interleaved=False, factor=1.0, original=None):
+        self.interleaved = interleaved
+        self.table = rotary_table(max_positions, rotary_dim, base, factor, original)
+
+    def __call__(self, x, positions=None):
+        return rotary(x, self.table, positions, self.interleaved)
 
 
 def _param_attrs(obj):
@@ -1085,6 +1242,58 @@ class AdamW(_Optimizer):
 class Adam(AdamW):
     def __init__(self, params, lr=0.001, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0):
         super().__init__(params, lr, betas, eps, weight_decay=weight_decay)
+
+
+class Muon(_Optimizer):
+    """Momentum whose update is orthogonalised (MuonBatch): every parameter of
+    two or more dimensions as the matrix (shape[0], the rest), w -= lr *
+    weight_decay * w + lr * rms * sqrt(max(rows, cols)) * X, so that a
+    full-rank update has a root mean square of about lr * rms whatever the
+    shape (0.2 is AdamW's typical one: its learning rates carry over).
+    Parameters of one dimension are updated by AdamW with the same lr, `betas`
+    and `eps`, and no decay.  All matrices share their launches."""
+
+    def __init__(self, params, lr=0.001, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, rms=0.2,
+                 betas=(0.9, 0.999), eps=1e-8):
+        super().__init__([p for p in params if len(p.shape) >= 2], lr)
+        if not 1 <= steps <= 20:
+            raise ValueError(f"Muon: {steps} steps (1 to 20)")
+        self.matrices, self.params = self.params, list(params)
+        self.momentum, self.nesterov, self.weight_decay = momentum, nesterov, weight_decay
+        self.steps, self.rms = steps, rms
+        self.m = [Tensor(np.zeros(p.shape, np.float32), track=False) for p in self.matrices]
+        self.vectors = AdamW([p for p in params if len(p.shape) < 2], lr, betas, eps, weight_decay=0.0)
+        n = len(self.matrices)
+        self._ma = (ctypes.c_void_p * n)()
+        self._rows, self._cols = (ctypes.c_uint * n)(), (ctypes.c_uint * n)()
+        self._sizes = (ctypes.c_float * n)()
+
+    @property
+    def t(self):
+        """Steps taken (the vectors' AdamW counts them)."""
+        return self.vectors.t
+
+    @t.setter
+    def t(self, value):
+        self.vectors.t = value
+
+    def step(self, clip=1.0):
+        self.vectors.lr = self.lr
+        self.vectors.step(clip)
+        n = 0
+        for p, m in zip(self.matrices, self.m):
+            if p.grad is None:
+                continue
+            rows = p.shape[0]
+            cols = p.size // rows
+            self._pa[n], self._ga[n], self._ma[n] = p.gpu_buf, p.grad.gpu_buf, m.gpu_buf
+            self._rows[n], self._cols[n] = rows, cols
+            self._sizes[n] = self.lr * self.rms * max(rows, cols) ** 0.5
+            n += 1
+        if n and not lib.MuonBatch(self._pa, self._ga, self._ma, self._rows, self._cols, self._sizes, n,
+                                   self.momentum, 1 if self.nesterov else 0, self.lr * self.weight_decay, clip,
+                                   self.steps):
+            raise RuntimeError(f"MuonBatch failed: {last_error()}")
 
 
 # --------------------------------------------------------------------------
@@ -1389,7 +1598,7 @@ class KernelProfiler:
                 "maxpool_fwd", "maxpool_bwd", "bn_stats", "bn_stats_side", "bn_fwd", "bn_bwd_reduce",
                 "bn_bwd_reduce_side", "bn_bwd_dx",
                 "dw_bwd_input", "dw_bwd_filter", "gap_bwd", "upsample", "upsample_bwd", "bias_grad",
-                "dice_loss_grad", "sgd", "sgd_clipped", "adam", "grad_norm", "clip_scale",
+                "dice_loss_grad", "sgd", "sgd_clipped", "adam", "muon", "rotary", "attention", "attention_bwd", "grad_norm", "clip_scale",
                 "relu", "relu_grad", "relu6", "relu6_grad", "leaky_relu", "leaky_relu_grad",
                 "sigmoid", "sigmoid_grad", "add", "scale_add", "grad_accum")
 

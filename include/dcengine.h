@@ -223,6 +223,52 @@ void AdamBatchCounted(void** params, void** grads, void** m, void** v, uint32_t*
  * returns the norm (NaN while a capture is open). */
 float ClipGradNormNoAlloc(void** grads, uint32_t* sizes, uint32_t numGrads, float maxNorm);
 
+/* ---- transformer blocks.  Tokens are [batch][seq][heads][headDim], dense;
+ * every call returns NULL / false (and sets the error) for a size that its
+ * buffers do not hold.
+ *
+ * RotaryApply: y = x with the first rotaryDim (even) values of every head
+ * turned in pairs by their position's angles.  table: rows of rotaryDim / 2
+ * (cos, sin) pairs, one row per position.  positions: batch * seq floats
+ * holding whole numbers, or NULL (0 .. seq - 1 in every sequence); one outside
+ * the table reads a row of zeros, as any read outside a buffer.  flags bit0:
+ * the pairs are values (2i, 2i + 1), else (i, i + rotaryDim / 2); bit1: turn
+ * the other way (the gradient).  Values from rotaryDim on are copied. */
+void* RotaryApply(void* x, void* table, void* positions, uint32_t batch, uint32_t seq,
+                  uint32_t heads, uint32_t headDim, uint32_t rotaryDim, uint32_t flags);
+
+/* AttentionForward: softmax(scale * q k^T + mask) v.  q and the result are
+ * [batch][seq][heads][headDim], k and v [batch][keys][kvHeads][headDim], query
+ * head h reading key head h / (heads / kvHeads); headDim up to 256.  lengths:
+ * batch floats, the keys of each sequence that are read (clamped to 0 .. keys;
+ * memory past them may hold anything), or NULL: all.  flags bit0: causal, query
+ * i sees the keys up to i + keys - seq.  A query that sees no key gets zeros,
+ * and gradients of zero.  A value that is not finite in a key or vector that
+ * some query may see can reach the neighbouring queries of its tile too, as 0 *
+ * NaN does in the formula.  pStats, when not NULL, receives 2 * batch * heads *
+ * seq floats for AttentionBackward (the maximum and 1 / sum of each row). */
+void* AttentionForward(void* q, void* k, void* v, void* lengths, uint32_t batch, uint32_t seq,
+                       uint32_t keys, uint32_t heads, uint32_t kvHeads, uint32_t headDim,
+                       uint32_t flags, float scale, void** pStats);
+/* The gradients of q, k, v, each only when requested (NULL otherwise), from
+ * the forward's operands, its result and its stats, none of which are
+ * released.  Gradients of key heads that several heads share are summed in a
+ * fixed order; those of keys past a sequence's length are zeros. */
+void AttentionBackward(void* gradOut, void* out, void* q, void* k, void* v, void* lengths,
+                       void* stats, uint32_t batch, uint32_t seq, uint32_t keys, uint32_t heads,
+                       uint32_t kvHeads, uint32_t headDim, uint32_t flags, float scale,
+                       uint32_t qReq, uint32_t kReq, uint32_t vReq, void** pDQ, void** pDK,
+                       void** pDV);
+
+/* Orthogonalised momentum update of matrices of rows[i] x cols[i] values, all
+ * in the same launches: g clamped to +-clip, m = momentum * m + g, d = g +
+ * momentum * m (nesterov) or m, X = d / (|d| + 1e-7), `steps` (1 to 20) times
+ * X <- 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X, and w -= weightDecay *
+ * w + stepSizes[i] * X.  NULL params / grads are skipped. */
+bool MuonBatch(void** params, void** grads, void** momenta, uint32_t* rows, uint32_t* cols,
+               float* stepSizes, uint32_t numParams, float momentum, uint32_t nesterov,
+               float weightDecay, float clip, uint32_t steps);
+
 /* Kernel-family timing with HIP events on the engine stream (for bench.py).
  * SetProfiling(1) starts recording every launch of the named families;
  * GetProfile returns launches, summed milliseconds, summed algorithmic
