@@ -213,6 +213,7 @@ def prepare(case, seed):
         if own:
             from directcompute_torch_amd import nn_engine as nn
             s["opt"] = nn.Muon(s["w"], lr=LR, momentum=MU, weight_decay=DECAY, steps=STEPS, rms=RMS)
+            nn.sync_gpu()  # its zeros are on their way, on another stream than torch's
             for have, m in zip(s["opt"].m, d["m"]):
                 _view(have).copy_(m)
         else:
