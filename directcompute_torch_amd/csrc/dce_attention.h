@@ -1,0 +1,79 @@
+// What the attention kernels on fp32 MFMAs (dce_attention.hip) and those on
+// fp16 parts (dce_attention_parts.hip) share: the problem's description and the
+// mask.
+#pragma once
+#include "dce_internal.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace dce {
+
+// Tokens come as [batch][token][head][dim].  `rep` query heads share one key
+// head, so the problem of one (sequence, key head) pair is N = rep * S query
+// rows against up to T keys: row n is query n / rep of head n % rep.
+struct Attn {
+  const float *q, *k, *v, *len;  // len: keys of each sequence, or null
+  float* o;
+  float *m, *il;                 // row statistics [problem][N]; null: not kept
+  float *pm, *pl, *po;           // partials of the key splits
+  const float* dy;               // backward
+  float *delta, *dq, *dk, *dv;
+  const uint32_t* only;          // problems to run (non-zero); null: all
+  uint32_t B, S, T, G, D, rep, N;
+  uint32_t tiles, splits, perSplit;  // key tiles of a split
+  FastDiv dRep, dG;
+  float c, scale;
+  int causal;
+};
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ uint32_t keys_of(const Attn& a, uint32_t b) {
+  if (!a.len) return a.T;
+  const float n = a.len[b];
+  return n >= 1.f ? (n < float(a.T) ? uint32_t(n) : a.T) : 0u;  // NaN: none
+}
+// Keys that row n sees (row n of the problem, `len` keys in the sequence).
+__device__ __forceinline__ uint32_t limit_of(const Attn& a, uint32_t n, uint32_t len) {
+  if (!a.causal) return len;
+  const int64_t e = int64_t(fdiv(n, a.dRep)) + int64_t(a.T) - int64_t(a.S) + 1;
+  return e <= 0 ? 0u : uint32_t(min(e, int64_t(len)));
+}
+// Keys that `rows` rows from n on see, for a wave that holds them.
+__device__ __forceinline__ uint32_t wave_limit(const Attn& a, uint32_t n, uint32_t rows, uint32_t len) {
+  return __builtin_amdgcn_readfirstlane(n < a.N ? limit_of(a, min(n + rows, a.N) - 1, len) : 0u);
+}
+// First row that sees key k0.
+__device__ __forceinline__ uint32_t first_row(const Attn& a, uint32_t k0) {
+  const int64_t i = int64_t(k0) - (int64_t(a.T) - int64_t(a.S));
+  return a.causal && i > 0 ? uint32_t(i) * a.rep : 0u;
+}
+// First value of row n's vector in a [batch][seq][heads][dim] tensor.
+__device__ __forceinline__ size_t q_at(const Attn& a, uint32_t b, uint32_t g, uint32_t n) {
+  const uint32_t i = fdiv(n, a.dRep), h = g * a.rep + (n - i * a.rep);
+  return ((size_t(b) * a.S + i) * (size_t(a.G) * a.rep) + h) * a.D;
+}
+__device__ __forceinline__ size_t k_at(const Attn& a, uint32_t b, uint32_t g, uint32_t j) {
+  return ((size_t(b) * a.T + j) * a.G + g) * a.D;
+}
+
+inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b); }
+
+// Pairs of a query and a key that the mask of full lengths leaves.
+inline double pairs_of(const AttnArgs& x) {
+  if (!x.causal) return double(x.S) * x.T;
+  const double rows = std::min(x.S, x.T), last = x.T;
+  return rows * last - rows * (rows - 1) / 2;
+}
+
+// Joins the key splits of a forward into o (and the statistics).
+bool attn_join(const Attn& a);
+// The forward / backward on fp32 MFMAs with a's operands (a.only, a.delta as set).
+bool attn_fwd_fp32(Attn a);
+bool attn_bwd_fp32(Attn a);
+// On fp16 parts, where they are faster; `took` tells.
+bool attn_fwd_parts(const AttnArgs& x, Attn a, bool* took);
+bool attn_bwd_parts(const AttnArgs& x, Attn a, bool* took);
+
+}  // namespace dce

@@ -1,11 +1,8 @@
 // Attention: O = softmax(scale * Q K^T + mask) V and its gradients, without a
 // matrix of scores in memory.
 //
-// Tokens come as [batch][token][head][dim].  `rep` query heads share one key
-// head, so the problem of one (sequence, key head) pair is N = rep * seq query
-// rows against up to `keys` keys: row n is query n / rep of head n % rep.
-// Query i sees the keys below min(length, i + keys - seq + 1) when causal, else
-// below length.
+// Query i sees the keys below min(length, i + T - S + 1) when causal, else below
+// length.
 //
 // Forward, per row, over tiles of keys with a running maximum m and sum l:
 //   s_j = c q.k_j (c = scale * log2 e),  p_j = 2^(s_j - m),  l = sum p_j,
@@ -23,10 +20,7 @@
 // fragments are read as 16 bytes (dims 16 j + 4 g + e feed step e of lane group
 // g), and the transposed operands as up to 16 bytes too (row m of block e is
 // dim 16 EG q + EG m + e).
-#include "dce_internal.h"
-
-#include <algorithm>
-#include <cmath>
+#include "dce_attention.h"
 
 namespace dce {
 
@@ -38,42 +32,6 @@ constexpr int kKeys = 32; // keys (rows in the dK / dV kernel) of an LDS tile
 __device__ __forceinline__ f4 mfma4(float a, float b, const f4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
-
-struct Attn {
-  const float *q, *k, *v, *len;  // len: keys of each sequence, or null
-  float* o;
-  float *m, *il;                 // row statistics [problem][N]; null: not kept
-  float *pm, *pl, *po;           // partials of the key splits
-  const float* dy;               // backward
-  float *delta, *dq, *dk, *dv;
-  uint32_t B, S, T, G, D, rep, N;
-  uint32_t tiles, splits, perSplit;  // key tiles of a split
-  FastDiv dRep, dG;
-  float c, scale;
-  int causal;
-};
-
-__device__ __forceinline__ uint32_t keys_of(const Attn& a, uint32_t b) {
-  if (!a.len) return a.T;
-  const float n = a.len[b];
-  return n >= 1.f ? (n < float(a.T) ? uint32_t(n) : a.T) : 0u;  // NaN: none
-}
-// Keys that row n sees (row n of the problem, `len` keys in the sequence).
-__device__ __forceinline__ uint32_t limit_of(const Attn& a, uint32_t n, uint32_t len) {
-  if (!a.causal) return len;
-  const int64_t e = int64_t(fdiv(n, a.dRep)) + int64_t(a.T) - int64_t(a.S) + 1;
-  return e <= 0 ? 0u : uint32_t(min(e, int64_t(len)));
-}
-// First value of row n's vector in a [batch][seq][heads][dim] tensor.
-__device__ __forceinline__ size_t q_at(const Attn& a, uint32_t b, uint32_t g, uint32_t n) {
-  const uint32_t i = fdiv(n, a.dRep), h = g * a.rep + (n - i * a.rep);
-  return ((size_t(b) * a.S + i) * (size_t(a.G) * a.rep) + h) * a.D;
-}
-__device__ __forceinline__ size_t k_at(const Attn& a, uint32_t b, uint32_t g, uint32_t j) {
-  return ((size_t(b) * a.T + j) * a.G + g) * a.D;
-}
-
 // A 16-lane fragment of vectors: lane group g takes dims 16 j + 4 g .. + 3.
 template <int DP, bool VEC>
 __device__ __forceinline__ void load_frag(const float* p, bool ok, uint32_t D, int g, f4 (&r)[DP / 16]) {
@@ -184,10 +142,12 @@ __global__ void __launch_bounds__(kT) k_attn_fwd(const Attn a) {
   const uint32_t id = xcd_block_id();
   const uint32_t per = a.tiles * a.splits, pr = id / per, rest = id - pr * per;
   const uint32_t sp = rest / a.tiles, tile = a.tiles - 1 - (rest - sp * a.tiles);  // long rows first
+  if (a.only && !a.only[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const uint32_t n0 = tile * 64 * QT, len = keys_of(a, b);
   const uint32_t least = limit_of(a, n0, len), most = limit_of(a, min(n0 + 64 * QT, a.N) - 1, len);
+  const uint32_t mine = wave_limit(a, n0 + wave * 16 * QT, 16 * QT, len);
 
   f4 q[QT][DP / 16];
   uint32_t lim[QT];
@@ -221,6 +181,7 @@ __global__ void __launch_bounds__(kT) k_attn_fwd(const Attn a) {
     TL::store(Vs, rv);
     __syncthreads();
     if (j + kKeys < j1) fetch(j + kKeys);
+    if (j >= mine) continue;
     // S^T: keys 16 kt + 4 g + r of query `col`
     f4 s[QT][2];
 #pragma unroll
@@ -342,10 +303,12 @@ __global__ void __launch_bounds__(kT) k_attn_dq(const Attn a) {
   __shared__ __attribute__((aligned(16))) float Ks[kKeys * DP], Vs[kKeys * DP];
   const uint32_t id = xcd_block_id();
   const uint32_t pr = id / a.tiles, tile = a.tiles - 1 - (id - pr * a.tiles);
+  if (a.only && !a.only[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const uint32_t n0 = tile * 64 * QT, len = keys_of(a, b);
   const uint32_t least = limit_of(a, n0, len), most = limit_of(a, min(n0 + 64 * QT, a.N) - 1, len);
+  const uint32_t mine = wave_limit(a, n0 + wave * 16 * QT, 16 * QT, len);
 
   f4 q[QT][DP / 16], dy[QT][DP / 16], dq[QT][DP / 16];
   uint32_t lim[QT];
@@ -386,6 +349,7 @@ __global__ void __launch_bounds__(kT) k_attn_dq(const Attn a) {
     TL::store(Vs, rv);
     __syncthreads();
     if (j + kKeys < most) fetch(j + kKeys);
+    if (j >= mine) continue;
     f4 s[QT][2], dp[QT][2];
 #pragma unroll
     for (int t = 0; t < QT; ++t)
@@ -449,20 +413,17 @@ __global__ void __launch_bounds__(kT) k_attn_dkv(const Attn a) {
   __shared__ uint32_t Lim[kKeys];
   const uint32_t id = xcd_block_id();
   const uint32_t pr = id / a.tiles, tile = id - pr * a.tiles;
+  if (a.only && !a.only[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const uint32_t k0 = tile * 64, len = keys_of(a, b), key = k0 + wave * 16 + col;
+  const uint32_t kw = __builtin_amdgcn_readfirstlane(k0 + wave * 16);
   f4 kf[DP / 16], vf[DP / 16], dk[DP / 16], dv[DP / 16];
   load_frag<DP, VEC>(a.k + (key < len ? k_at(a, b, gh, key) : 0), key < len, a.D, g, kf);
   load_frag<DP, VEC>(a.v + (key < len ? k_at(a, b, gh, key) : 0), key < len, a.D, g, vf);
 #pragma unroll
   for (int i = 0; i < DP / 16; ++i) dk[i] = dv[i] = f4{0.f, 0.f, 0.f, 0.f};
-  // Rows from the first that sees key k0 on.
-  uint32_t first = 0;
-  if (a.causal && int64_t(k0) > int64_t(a.T) - int64_t(a.S))
-    first = uint32_t(int64_t(k0) - (int64_t(a.T) - int64_t(a.S))) * a.rep;
-  if (k0 >= len) first = a.N;
-  first = min(first, a.N);
+  const uint32_t first = k0 < len ? min(first_row(a, k0), a.N) : a.N;
   f4 rq[TL::LOADS], ry[TL::LOADS];
   float st = 0.f;
   uint32_t lm = 0;
@@ -503,6 +464,7 @@ __global__ void __launch_bounds__(kT) k_attn_dkv(const Attn a) {
     if (threadIdx.x < kKeys) Lim[threadIdx.x] = lm;
     __syncthreads();
     if (n0 + kKeys < a.N) fetch(n0 + kKeys);
+    if (wave_limit(a, n0, kKeys, len) <= kw) continue;
     // S: rows 16 t + 4 g + r of key `col`
     f4 s[2], dp[2];
 #pragma unroll
@@ -553,8 +515,6 @@ __global__ void __launch_bounds__(kT) k_attn_dkv(const Attn a) {
   }
 }
 
-inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b); }
-
 Attn params(const AttnArgs& x) {
   Attn a{};
   a.q = x.q;
@@ -581,24 +541,15 @@ Attn params(const AttnArgs& x) {
   return a;
 }
 
-bool quads(const AttnArgs& x) { return x.D % 4 == 0; }
-
 // The head dims a kernel is built for: the least that holds D.
 template <class F>
-bool by_dim(uint32_t D, bool vec, F&& f) {
+bool by_dim(uint32_t D, bool vec, F f) {
 #define DCE_D(n) \
   if (D <= n) return vec ? f.template run<n, true>() : f.template run<n, false>();
   DCE_D(32) DCE_D(64) DCE_D(96) DCE_D(128) DCE_D(256)
 #undef DCE_D
   set_error("attention: a head has at most 256 values (got %u)", D);
   return false;
-}
-
-// Pairs of a query and a key that the mask of full lengths leaves.
-double pairs_of(const AttnArgs& x) {
-  if (!x.causal) return double(x.S) * x.T;
-  const double rows = std::min(x.S, x.T), last = x.T;
-  return rows * last - rows * (rows - 1) / 2;
 }
 
 struct FwdRun {
@@ -611,7 +562,7 @@ struct FwdRun {
     a.tiles = cdiv(a.N, wide ? 128 : 64);
     const uint32_t kt = cdiv(a.T, kKeys);
     a.splits = 1;
-    if (uint64_t(a.tiles) * prob < 2 * cus) {
+    if (!a.only && uint64_t(a.tiles) * prob < 2 * cus) {
       a.splits = std::min(cdiv(kt, 4), cdiv(4 * cus, a.tiles * prob));
       if (a.splits < 1) a.splits = 1;
     }
@@ -632,12 +583,7 @@ struct FwdRun {
     else
       hipLaunchKernelGGL((k_attn_fwd<DP, 1, VEC>), grid, dim3(kT), 0, stream(), a);
     if (!check_launch("AttentionForward")) return false;
-    if (a.splits > 1) {
-      const size_t values = rows * a.D;
-      hipLaunchKernelGGL(k_attn_join, dim3(cdiv(values, kT)), dim3(kT), 0, stream(), a, values);
-      return check_launch("AttentionForward (join)");
-    }
-    return true;
+    return a.splits == 1 || attn_join(a);
   }
 };
 
@@ -659,23 +605,35 @@ struct BwdRun {
 
 }  // namespace
 
+bool attn_join(const Attn& a) {
+  const size_t values = size_t(a.B) * a.G * a.N * a.D;
+  hipLaunchKernelGGL(k_attn_join, dim3(cdiv(values, kT)), dim3(kT), 0, stream(), a, values);
+  return check_launch("AttentionForward (join)");
+}
+bool attn_fwd_fp32(Attn a) { return by_dim(a.D, a.D % 4 == 0, FwdRun{a}); }
+bool attn_bwd_fp32(Attn a) { return by_dim(a.D, a.D % 4 == 0, BwdRun{a}); }
+
 bool attention_forward(const AttnArgs& x) {
   ProfScope prof("attention", 4.0 * x.D * x.B * x.H * pairs_of(x),
                  4.0 * x.D * (2.0 * x.B * x.S * x.H + 2.0 * x.B * x.T * x.G));
-  FwdRun r{params(x)};
-  return by_dim(x.D, quads(x), r);
+  const Attn a = params(x);
+  bool took = false;
+  return attn_fwd_parts(x, a, &took) && (took || attn_fwd_fp32(a));
 }
 
 bool attention_backward(const AttnArgs& x, const float* dy, float* dq, float* dk, float* dv) {
   ProfScope prof("attention_bwd", 10.0 * x.D * x.B * x.H * pairs_of(x),
                  4.0 * x.D * (4.0 * x.B * x.S * x.H + 4.0 * x.B * x.T * x.G));
-  BwdRun r{params(x)};
-  r.a.dy = dy;
-  r.a.dq = dq;
-  r.a.dk = dk;
-  r.a.dv = dv;
-  r.a.delta = workspace(size_t(x.B) * x.H * x.S);
-  return r.a.delta && by_dim(x.D, quads(x), r);
+  Attn a = params(x);
+  a.dy = dy;
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  bool took = false;
+  if (!attn_bwd_parts(x, a, &took)) return false;
+  if (took) return true;
+  a.delta = workspace(size_t(x.B) * x.H * x.S);
+  return a.delta && attn_bwd_fp32(a);
 }
 
 }  // namespace dce

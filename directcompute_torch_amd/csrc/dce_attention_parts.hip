@@ -1,0 +1,784 @@
+// Attention on fp16 parts: the products of large calls at a third of the fp16
+// MFMA rate, which is 16 times the fp32 one, with fp32's accuracy.
+//
+// A value x is kept as x 2^e = h + l, two fp16 values rounded to nearest, and
+// h h + (h l + l h) stands for a product: the parts carry 22 to 24 bits, and a
+// dot product rounds its sum once per 16 terms instead of at every one.  The
+// exponent e is one for each tile of 32 vectors, chosen so that the tile's
+// largest value lies in [2^14, 2^15): l's half step is then 2^-25, so a vector
+// whose own largest value is within 2^14 of the tile's keeps at least 24 bits of
+// it.  A (sequence, key head) with a tile that has smaller vectors than that
+// (zeros aside), values outside of 2^+-30 (gradients: 2^+-60) or any that is not finite is left
+// to the fp32 kernels: the pass that splits marks it, both sets of kernels are
+// launched, and the workgroups of the one that is not meant return at once.
+//
+// Everything that the scores do not need is a factor of a whole tile, so the
+// exponents cost next to nothing: c 2^-(eq + ek) is the factor that turns a
+// score into base 2 anyway, and where a sum goes over tiles of different
+// exponents (over V's in the forward, dO's and Q's for dV and dK) its terms are
+// brought to the smallest exponent so far, which the exponential's offset takes.
+//
+// P is relative to its row's maximum here, within [0, 1], and kept as 2^14 P; the
+// backward's 1 / l goes into dO (dO' = dO / l) when that is split, so that
+// dV = P^T dO' and dS = scale P (dO' V^T - delta'), delta' = rowsum(dO' * O).
+// delta' is of the size of the largest vector that a row sees, whatever tile it
+// is compared in: with E the least exponent of V's tiles up to the row's last
+// key, |dO' V^T - delta'| is at most 2 D 2^(30 - ey - E), which bounds dS's parts.
+#include "dce_attention.h"
+
+namespace dce {
+
+namespace {
+
+constexpr int kT = 256;
+constexpr int kRows = 32;         // vectors of a tile
+constexpr int kRange = 30;        // exponents of values that parts are made of
+constexpr int kRangeGrad = 60;    // and of gradients
+constexpr float kWide = 16384.f;  // largest ratio of the vectors' sizes in a tile
+
+using h4 = _Float16 __attribute__((ext_vector_type(4)));
+using h8 = _Float16 __attribute__((ext_vector_type(8)));
+using f16v = float __attribute__((ext_vector_type(16)));
+using s4v = short __attribute__((ext_vector_type(4)));
+using u4v = uint32_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f16v mma(const h8& a, const h8& b, const f16v& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void zero(f16v& v) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] = 0.f;
+}
+// 2^e, for e < 128; no less than 2^-126.
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + max(e, -126)) << 23); }
+
+// The parts of one operand: [problem][vector][h | l], DP halves each, zero past
+// D and past the last vector up to whole tiles; one exponent per tile.
+struct Part {
+  char* p;
+  int* e;
+  uint32_t pad;  // vectors of a problem, a multiple of 128
+};
+struct Parts {
+  Part q, k, v, y;
+  float* dl;      // delta' 2^e of dO's tile, [problem][q.pad]
+  int* least;     // least exponent of V's tiles up to each, [problem][v.pad / kRows]
+  uint32_t* bad;  // problems left to the fp32 kernels
+};
+
+// ---------------------------------------------------------------------------
+// The pass that splits: a workgroup per tile.
+// ---------------------------------------------------------------------------
+enum Which { QUERY, KEY, VALUE, GRAD };
+template <int DP, bool VEC, int W>
+__device__ __forceinline__ void split_tile(const Attn& a, const Part& P, const Parts& ps, uint32_t pr, uint32_t tile) {
+  constexpr int CH = DP / 8, SLOTS = (kRows * CH + kT - 1) / kT;
+  constexpr bool ROWS = W == QUERY || W == GRAD;
+  __shared__ uint32_t top[kRows];
+  __shared__ float dots[kRows];
+  __shared__ int all[3];
+  const uint32_t b = fdiv(pr, a.dG), g = pr - b * a.G;
+  const uint32_t n0 = tile * kRows, have = ROWS ? a.N : keys_of(a, b);
+  if (threadIdx.x < kRows) {
+    top[threadIdx.x] = 0;
+    dots[threadIdx.x] = 0.f;
+  }
+  __syncthreads();
+  float v[SLOTS][8];
+  float part[SLOTS];
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) {
+    const uint32_t slot = threadIdx.x + kT * i, row = slot / CH, d = slot % CH * 8, n = n0 + row;
+    part[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+    if (row >= kRows || n >= have) continue;
+    const size_t at = (ROWS ? q_at(a, b, g, n) : k_at(a, b, g, n)) + d;
+    const float* src = (W == QUERY ? a.q : W == KEY ? a.k : W == VALUE ? a.v : a.dy) + at;
+    const float by = W == GRAD ? a.il[size_t(pr) * a.N + n] : 1.f;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+        if (d + 4 * hf < a.D) {
+          const f4 x = *reinterpret_cast<const f4*>(src + 4 * hf);
+          f4 o = {0.f, 0.f, 0.f, 0.f};
+          if (W == GRAD) o = *reinterpret_cast<const f4*>(a.o + at + 4 * hf);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[i][4 * hf + e] = x[e] * by;
+            if (W == GRAD) part[i] += v[i][4 * hf + e] * o[e];
+          }
+        }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (d + e < a.D) {
+          v[i][e] = src[e] * by;
+          if (W == GRAD) part[i] += v[i][e] * a.o[at + e];
+        }
+    }
+    float m = 0.f;
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      m = fmaxf(m, fabsf(v[i][e]));
+      fine &= fabsf(v[i][e]) < INFINITY;  // false for NaN too
+    }
+    // The largest value of a vector, as bits (which order as the values do).
+    atomicMax(&top[row], fine ? __float_as_uint(m) : 0x7f800000u);
+  }
+  if constexpr (W == GRAD) {
+    // rowsum(dO' * O), the partial sums of a row in a fixed order
+    __shared__ float sums[kRows * CH];
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i)
+      if (threadIdx.x + kT * i < kRows * CH) sums[threadIdx.x + kT * i] = part[i];
+    __syncthreads();
+    if (threadIdx.x < kRows) {
+      float s = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) s += sums[threadIdx.x * CH + c];
+      dots[threadIdx.x] = s;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const uint32_t mine = threadIdx.x < kRows ? top[threadIdx.x] : 0u;
+    const float most = wave_reduce(__uint_as_float(mine), OpMaxR());
+    const float least = -wave_reduce(mine ? -__uint_as_float(mine) : -INFINITY, OpMaxR());
+    if (threadIdx.x == 0) {
+      constexpr int range = W == GRAD ? kRangeGrad : kRange;
+      int e = 14 + range;  // zeros: no smaller than another tile's
+      if (most > 0.f) {
+        const bool bad = !(most < pow2(range)) || most < pow2(-range) || most > kWide * least;
+        if (bad)
+          ps.bad[pr] = 1u;
+        else
+          e = 14 + 127 - int(__float_as_uint(most) >> 23);
+      }
+      all[0] = e;
+      P.e[size_t(pr) * (P.pad / kRows) + tile] = e;
+    }
+  }
+  __syncthreads();
+  const float by = pow2(all[0]);
+  char* out = P.p + (size_t(pr) * P.pad + n0) * (DP * 4);
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) {
+    const uint32_t slot = threadIdx.x + kT * i, row = slot / CH, c = slot % CH;
+    if (row >= kRows) continue;
+    h8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = v[i][e] * by;
+      h[e] = _Float16(x);
+      l[e] = _Float16(x - float(h[e]));
+    }
+    *reinterpret_cast<h8*>(out + row * (DP * 4) + c * 16) = h;
+    *reinterpret_cast<h8*>(out + row * (DP * 4) + DP * 2 + c * 16) = l;
+  }
+  if (W == GRAD && threadIdx.x < kRows) ps.dl[size_t(pr) * P.pad + n0 + threadIdx.x] = dots[threadIdx.x] * by;
+}
+// E: the running minimum of the exponents of V's tiles; a workgroup per problem,
+// a run of tiles per thread.
+__global__ void __launch_bounds__(kT) k_attn_least(const Parts ps) {
+  __shared__ int runs[kT];
+  const int n = int(ps.v.pad / kRows), per = (n + kT - 1) / kT;
+  const int* e = ps.v.e + size_t(blockIdx.x) * n;
+  int* out = ps.least + size_t(blockIdx.x) * n;
+  const int t0 = int(threadIdx.x) * per, t1 = min(n, t0 + per);
+  int m = 1000;
+  for (int t = t0; t < t1; ++t) m = min(m, e[t]);
+  runs[threadIdx.x] = m;
+  __syncthreads();
+  m = 1000;
+  for (int i = 0; i < int(threadIdx.x); ++i) m = min(m, runs[i]);
+  for (int t = t0; t < t1; ++t) {
+    m = min(m, e[t]);
+    out[t] = m;
+  }
+}
+// Tiles of q (and dO), then of k and v, of each problem.
+template <int DP, bool VEC, bool BWD>
+__global__ void __launch_bounds__(kT) k_attn_split(const Attn a, const Parts ps) {
+  const uint32_t tq = ps.q.pad / kRows, tk = ps.k.pad / kRows, per = (BWD ? 2 : 1) * tq + 2 * tk;
+  const uint32_t pr = blockIdx.x / per;
+  uint32_t t = blockIdx.x - pr * per;
+  if (t < tq) return split_tile<DP, VEC, QUERY>(a, ps.q, ps, pr, t);
+  t -= tq;
+  if (t < tk) return split_tile<DP, VEC, KEY>(a, ps.k, ps, pr, t);
+  t -= tk;
+  if (t < tk) return split_tile<DP, VEC, VALUE>(a, ps.v, ps, pr, t);
+  if constexpr (BWD) split_tile<DP, VEC, GRAD>(a, ps.y, ps, pr, t - tk);
+}
+
+// ---------------------------------------------------------------------------
+// An LDS tile of 32 vectors' parts: the h plane, then the l plane, the 16-byte
+// chunks of a row XORed by the row, so that eight rows' equal chunks lie in
+// different banks, and neighbouring rows in different halves of them (a
+// transposed read takes 64 bytes of each of eight rows).
+// ---------------------------------------------------------------------------
+template <int DP>
+struct PTile {
+  static constexpr int CH = DP / 8, PLANE = kRows * DP * 2, BYTES = 2 * PLANE, LOADS = BYTES / 16 / kT;
+  static_assert(BYTES % (16 * kT) == 0, "whole slots");
+  __device__ static __forceinline__ int swz(int row) {
+    return CH % 8 == 0 ? ((row & 1) << 2) | ((row >> 1) & 3) : (row >> 1) & 3;
+  }
+  __device__ static __forceinline__ void load(const char* p, u4v (&r)[LOADS]) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) r[i] = reinterpret_cast<const u4v*>(p)[threadIdx.x + kT * i];
+  }
+  __device__ static __forceinline__ void store(char* S, const u4v (&r)[LOADS]) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int m = threadIdx.x + kT * i, row = m / (2 * CH), pl = m / CH & 1, c = m % CH;
+      *reinterpret_cast<u4v*>(S + pl * PLANE + (row * CH + (c ^ swz(row))) * 16) = r[i];
+    }
+  }
+  // Row `row`, dims 8 c .. + 7.
+  __device__ static __forceinline__ h8 rows(const char* S, int pl, int row, int c) {
+    return *reinterpret_cast<const h8*>(S + pl * PLANE + (row * CH + (c ^ swz(row))) * 16);
+  }
+  // Dim 32 t + lane % 32, rows 16 k + 4 (lane / 32) + 0 .. 3 and the same + 8: the
+  // rows that a lane's accumulator values 8 k .. 8 k + 7 belong to.
+  __device__ static __forceinline__ h8 cols(const char* S, int pl, int k, int t, int lane) {
+    const int j = lane & 15, d = 32 * t + (lane & 16) + 4 * (j & 3);
+    h4 v[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = 16 * k + 8 * e + 4 * (lane >> 5) + (j >> 2);
+      const s4v w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s4v*)(S + pl * PLANE + (row * CH + ((d >> 3) ^ swz(row))) * 16 + (d & 7) * 2));
+      v[e] = __builtin_bit_cast(h4, w);
+    }
+    return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+// A lane's vector as B operands: dims 16 i + 8 (lane / 32) + 0 .. 7.
+template <int DP>
+__device__ __forceinline__ void load_vec(const char* p, int half, h8 (&h)[DP / 16], h8 (&l)[DP / 16]) {
+#pragma unroll
+  for (int i = 0; i < DP / 16; ++i) {
+    h[i] = *reinterpret_cast<const h8*>(p + i * 32 + half * 16);
+    l[i] = *reinterpret_cast<const h8*>(p + DP * 2 + i * 32 + half * 16);
+  }
+}
+// Accumulator values 8 k .. 8 k + 7 as parts.  x is made opaque: where it is a
+// product, the compiler would round h from the unrounded product in one place
+// and from the float in another, which differ by a step once in some 2^12 values.
+__device__ __forceinline__ void split_acc(const f16v& s, int k, h8& h, h8& l) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float x = s[8 * k + e];
+    asm("" : "+v"(x));
+    h[e] = _Float16(x);
+    l[e] = _Float16(x - float(h[e]));
+  }
+}
+// The tile's vectors times a lane's: out[e] is row 8 (e / 4) + 4 (lane / 32) + e % 4.
+template <int DP>
+__device__ __forceinline__ f16v scores(const char* S, const h8 (&h)[DP / 16], const h8 (&l)[DP / 16], int col, int half) {
+  f16v big, small;
+  zero(big);
+  zero(small);
+#pragma unroll
+  for (int i = 0; i < DP / 16; ++i) {
+    const h8 th = PTile<DP>::rows(S, 0, col, 2 * i + half), tl = PTile<DP>::rows(S, 1, col, 2 * i + half);
+    big = mma(th, h[i], big);
+    small = mma(th, l[i], small);
+    small = mma(tl, h[i], small);
+  }
+  return big + small;
+}
+// acc += (tile transposed) (parts of s).
+template <int DP>
+__device__ __forceinline__ void add_cols(const char* S, const f16v& s, f16v (&acc)[DP / 32], int lane) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    h8 h, l;
+    split_acc(s, k, h, l);
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) {
+      const h8 th = PTile<DP>::cols(S, 0, k, t, lane), tl = PTile<DP>::cols(S, 1, k, t, lane);
+      acc[t] = mma(th, h, acc[t]);
+      acc[t] = mma(th, l, acc[t]);
+      acc[t] = mma(tl, h, acc[t]);
+    }
+  }
+}
+// A lane's vector from its accumulators: dims 32 t + 8 q + 4 half + 0 .. 3.
+template <int DP, bool VEC>
+__device__ __forceinline__ void write_vec(float* p, uint32_t D, int half, const f16v (&acc)[DP / 32], float by, float by2) {
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t d = 32 * t + 8 * q + 4 * half;
+      f4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[t][4 * q + e] * by * by2;
+      if constexpr (VEC) {
+        if (d < D) *reinterpret_cast<f4*>(p + d) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < D) p[d + e] = v[e];
+      }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Forward: 128 query rows per workgroup, 32 per wave, in registers.
+// ---------------------------------------------------------------------------
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Parts ps) {
+  using TL = PTile<DP>;
+  __shared__ __attribute__((aligned(16))) char Ks[TL::BYTES], Vs[TL::BYTES];
+  const uint32_t id = xcd_block_id();
+  const uint32_t per = a.tiles * a.splits, pr = id / per, rest = id - pr * per;
+  const uint32_t sp = rest / a.tiles, tile = a.tiles - 1 - (rest - sp * a.tiles);  // long rows first
+  if (ps.bad[pr]) return;
+  const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  const uint32_t n0 = tile * 128, n = n0 + wave * 32 + col, len = keys_of(a, b);
+  const uint32_t least = limit_of(a, n0, len), most = limit_of(a, min(n0 + 128, a.N) - 1, len);
+  const uint32_t lim = n < a.N ? limit_of(a, n, len) : 0u, mine = wave_limit(a, n0 + wave * 32, kRows, len);
+  h8 qh[DP / 16], ql[DP / 16];
+  load_vec<DP>(ps.q.p + (size_t(pr) * ps.q.pad + n) * (DP * 4), half, qh, ql);
+  const float cq = a.c * pow2(-ps.q.e[size_t(pr) * (ps.q.pad / kRows) + n0 / kRows + wave]);
+  const int* ek = ps.k.e + size_t(pr) * (ps.k.pad / kRows);
+  const int* ev = ps.v.e + size_t(pr) * (ps.v.pad / kRows);
+  const char* kp = ps.k.p + size_t(pr) * ps.k.pad * (DP * 4);
+  const char* vp = ps.v.p + size_t(pr) * ps.v.pad * (DP * 4);
+  f16v o[DP / 32];
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) zero(o[t]);
+  float m = -INFINITY, l = 0.f;
+  int R = 1000;  // o counts in units of 2^-(14 + R)
+  const uint32_t j0 = sp * a.perSplit * kRows, j1 = min(most, (sp + 1) * a.perSplit * kRows);
+  u4v rk[TL::LOADS], rv[TL::LOADS];
+  auto fetch = [&](uint32_t j) {
+    TL::load(kp + size_t(j) * (DP * 4), rk);
+    TL::load(vp + size_t(j) * (DP * 4), rv);
+  };
+  if (j0 < j1) fetch(j0);
+  for (uint32_t j = j0; j < j1; j += kRows) {
+    __syncthreads();
+    TL::store(Ks, rk);
+    TL::store(Vs, rv);
+    __syncthreads();
+    if (j + kRows < j1) fetch(j + kRows);
+    if (j >= mine) continue;
+    const float cs = cq * pow2(-ek[j / kRows]);
+    const int e = ev[j / kRows];
+    f16v s = scores<DP>(Ks, qh, ql, col, half);
+    float top = -INFINITY;
+    if (j + kRows > least) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t key = j + 8 * (i >> 2) + 4 * half + (i & 3);
+        s[i] = key < lim ? s[i] * cs : -INFINITY;
+        top = fmaxf(top, s[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] *= cs;
+        top = fmaxf(top, s[i]);
+      }
+    }
+    top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+    const float base = top == -INFINITY ? 0.f : top;  // nothing seen yet: every p is 0
+    float down = 1.f;
+    bool move = __any(top > m);
+    if (move) {
+      down = exp2_(m - base);
+      l *= down;
+      m = top;
+    }
+    if (e < R) {
+      down *= R == 1000 ? 1.f : pow2(e - R);
+      R = e;
+      move = true;
+    }
+    if (move) {
+#pragma unroll
+      for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] *= down;
+    }
+    // p 2^(14 + R - e), which the exponential's offset brings in
+    const int lg = 14 + max(R - e, -60);
+    const float off = base - float(lg);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = exp2_(s[i] - off);
+      sum += s[i];
+    }
+    l += sum * pow2(-lg);
+    add_cols<DP>(Vs, s, o, lane);
+  }
+  l += __shfl_xor(l, 32);
+  if (n >= a.N) return;
+  const float unit = R == 1000 ? 0.f : pow2(-14);
+  const float unit2 = R == 1000 ? 0.f : pow2(-R);
+  if (a.splits > 1) {
+    const size_t row = (size_t(sp) * a.B * a.G + pr) * a.N + n;
+    if (half == 0) {
+      a.pm[row] = m;
+      a.pl[row] = l;
+    }
+    write_vec<DP, VEC>(a.po + row * a.D, a.D, half, o, unit, unit2);
+    return;
+  }
+  const float il = lim ? 1.f / l : 0.f;  // a row that sees nothing: zeros
+  if (a.m && half == 0) {
+    a.m[size_t(pr) * a.N + n] = lim ? m : 0.f;
+    a.il[size_t(pr) * a.N + n] = il;
+  }
+  write_vec<DP, VEC>(a.o + q_at(a, b, gh, n), a.D, half, o, unit * il, unit2);
+}
+
+// dS's parts: p (at most 2^14) times dP - delta (at most 2^(31 + log2 DP)) times
+// 2^-kDown lies below 2^15.
+template <int DP>
+constexpr int down_bits() {
+  return 30 + (DP <= 32 ? 5 : DP <= 64 ? 6 : 7);
+}
+
+// ---------------------------------------------------------------------------
+// dQ: 128 query rows per workgroup, Q and dO' in registers.
+// ---------------------------------------------------------------------------
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(kT, DP <= 64 ? 2 : 1) k_attn_dq_parts(const Attn a, const Parts ps) {
+  using TL = PTile<DP>;
+  __shared__ __attribute__((aligned(16))) char Ks[TL::BYTES], Vs[TL::BYTES];
+  const uint32_t id = xcd_block_id();
+  const uint32_t pr = id / a.tiles, tile = a.tiles - 1 - (id - pr * a.tiles);
+  if (ps.bad[pr]) return;
+  const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  const uint32_t n0 = tile * 128, n = n0 + wave * 32 + col, len = keys_of(a, b);
+  const uint32_t least = limit_of(a, n0, len), most = limit_of(a, min(n0 + 128, a.N) - 1, len);
+  const uint32_t lim = n < a.N ? limit_of(a, n, len) : 0u, mine = wave_limit(a, n0 + wave * 32, kRows, len);
+  const size_t row = size_t(pr) * ps.q.pad + n;
+  h8 qh[DP / 16], ql[DP / 16], yh[DP / 16], yl[DP / 16];
+  load_vec<DP>(ps.q.p + row * (DP * 4), half, qh, ql);
+  load_vec<DP>(ps.y.p + row * (DP * 4), half, yh, yl);
+  const size_t et = size_t(pr) * (ps.q.pad / kRows) + n0 / kRows + wave;
+  const float cq = a.c * pow2(-ps.q.e[et]), m = n < a.N ? a.m[size_t(pr) * a.N + n] : 0.f;
+  const float delta = ps.dl[row];
+  const int ey = ps.y.e[et];
+  const int* ek = ps.k.e + size_t(pr) * (ps.k.pad / kRows);
+  const int* ev = ps.v.e + size_t(pr) * (ps.v.pad / kRows);
+  const char* kp = ps.k.p + size_t(pr) * ps.k.pad * (DP * 4);
+  const char* vp = ps.v.p + size_t(pr) * ps.v.pad * (DP * 4);
+  f16v dq[DP / 32];
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) zero(dq[t]);
+  const int E = mine ? ps.least[size_t(pr) * (ps.v.pad / kRows) + (mine - 1) / kRows] : 0;
+  int R = 1000;  // dq counts in units of 2^-(R + E + ey - down_bits + 14)
+  u4v rk[TL::LOADS], rv[TL::LOADS];
+  auto fetch = [&](uint32_t j) {
+    TL::load(kp + size_t(j) * (DP * 4), rk);
+    TL::load(vp + size_t(j) * (DP * 4), rv);
+  };
+  if (most) fetch(0);
+  for (uint32_t j = 0; j < most; j += kRows) {
+    __syncthreads();
+    TL::store(Ks, rk);
+    TL::store(Vs, rv);
+    __syncthreads();
+    if (j + kRows < most) fetch(j + kRows);
+    if (j >= mine) continue;
+    const int xk = ek[j / kRows], xv = ev[j / kRows];
+    const float cs = cq * pow2(-xk);
+    f16v s = scores<DP>(Ks, qh, ql, col, half);
+    f16v dp = scores<DP>(Vs, yh, yl, col, half);
+    if (xk < R) {
+      if (R != 1000) {
+        const float down = pow2(xk - R);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dq[t][i] *= down;
+      }
+      R = xk;
+    }
+    const float dl = delta * pow2(xv), by = pow2(R - xk + E - xv - down_bits<DP>() + 14);
+    const bool masked = j + kRows > least;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float v = exp2_(s[i] * cs - m) * ((dp[i] - dl) * by);
+      const uint32_t key = j + 8 * (i >> 2) + 4 * half + (i & 3);
+      s[i] = masked && key >= lim ? 0.f : v;
+    }
+    add_cols<DP>(Ks, s, dq, lane);
+  }
+  if (n >= a.N) return;
+  // 2^(down_bits - 14 - R - E - ey), in two factors that stay in range
+  const float u = R == 1000 ? 0.f : pow2(down_bits<DP>() - 14 - R - E) * a.scale;
+  write_vec<DP, VEC>(a.dq + q_at(a, b, gh, n), a.D, half, dq, u, pow2(-ey));
+}
+
+// ---------------------------------------------------------------------------
+// dK, dV: 128 keys per workgroup, 32 per wave, K and V in registers; tiles of
+// query rows of every head that shares them through LDS.
+// ---------------------------------------------------------------------------
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(kT, DP <= 64 ? 2 : 1) k_attn_dkv_parts(const Attn a, const Parts ps) {
+  using TL = PTile<DP>;
+  __shared__ __attribute__((aligned(16))) char Qs[TL::BYTES], Ys[TL::BYTES];
+  __shared__ __attribute__((aligned(16))) float Ms[kRows], Ds[kRows];
+  __shared__ uint32_t Ls[kRows];
+  const uint32_t id = xcd_block_id();
+  const uint32_t pr = id / a.tiles, tile = id - pr * a.tiles;
+  if (ps.bad[pr]) return;
+  const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  const uint32_t k0 = tile * 128, kw = k0 + wave * 32, key = kw + col, len = keys_of(a, b);
+  const uint32_t kws = __builtin_amdgcn_readfirstlane(kw);
+  const size_t row = size_t(pr) * ps.k.pad + key;
+  h8 kh[DP / 16], kl[DP / 16], vh[DP / 16], vl[DP / 16];
+  load_vec<DP>(ps.k.p + row * (DP * 4), half, kh, kl);
+  load_vec<DP>(ps.v.p + row * (DP * 4), half, vh, vl);
+  const size_t kt = size_t(pr) * (ps.k.pad / kRows) + kw / kRows;
+  const int xk = ps.k.e[kt], xv = ps.v.e[kt];
+  const float ck = a.c * pow2(-xk), vs = pow2(xv);
+  const int* eq = ps.q.e + size_t(pr) * (ps.q.pad / kRows);
+  const int* ey = ps.y.e + size_t(pr) * (ps.q.pad / kRows);
+  const int* least = ps.least + size_t(pr) * (ps.v.pad / kRows);
+  const char* qp = ps.q.p + size_t(pr) * ps.q.pad * (DP * 4);
+  const char* yp = ps.y.p + size_t(pr) * ps.q.pad * (DP * 4);
+  f16v dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) {
+    zero(dk[t]);
+    zero(dv[t]);
+  }
+  int Rv = 1000, Rk = 1000;  // dv counts in units of 2^-(14 + Rv), dk of 2^-(Rk - down_bits + 14)
+  const uint32_t first = k0 < len ? min(first_row(a, k0), a.N) & ~uint32_t(kRows - 1) : a.N;
+  u4v rq[TL::LOADS], ry[TL::LOADS];
+  float rm = 0.f, rd = 0.f;
+  uint32_t rl = 0;
+  auto fetch = [&](uint32_t n) {
+    TL::load(qp + size_t(n) * (DP * 4), rq);
+    TL::load(yp + size_t(n) * (DP * 4), ry);
+    if (threadIdx.x < kRows) {
+      const uint32_t i = n + threadIdx.x;
+      rm = i < a.N ? a.m[size_t(pr) * a.N + i] : 0.f;
+      rl = i < a.N ? limit_of(a, i, len) : 0u;
+      rd = ps.dl[size_t(pr) * ps.q.pad + i];
+    }
+  };
+  if (first < a.N) fetch(first);
+  for (uint32_t n0 = first; n0 < a.N; n0 += kRows) {
+    __syncthreads();
+    TL::store(Qs, rq);
+    TL::store(Ys, ry);
+    if (threadIdx.x < kRows) {
+      Ms[threadIdx.x] = rm;
+      Ds[threadIdx.x] = rd;
+      Ls[threadIdx.x] = rl;
+    }
+    __syncthreads();
+    if (n0 + kRows < a.N) fetch(n0 + kRows);
+    const uint32_t seen = wave_limit(a, n0, kRows, len);
+    if (seen <= kws) continue;
+    const int xq = eq[n0 / kRows], xy = ey[n0 / kRows], E = least[(seen - 1) / kRows], x = xq + xy + E;
+    const float cs = ck * pow2(-xq);
+    f16v s = scores<DP>(Qs, kh, kl, col, half);
+    f16v dp = scores<DP>(Ys, vh, vl, col, half);
+    if (xy < Rv) {
+      if (Rv != 1000) {
+        const float down = pow2(xy - Rv);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dv[t][i] *= down;
+      }
+      Rv = xy;
+    }
+    if (x < Rk) {
+      if (Rk != 1000) {
+        const float down = pow2(x - Rk);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dk[t][i] *= down;
+      }
+      Rk = x;
+    }
+    const int lg = 14 + max(Rv - xy, -60);
+    const float flg = float(lg), by = pow2(Rk - x + E - xv - down_bits<DP>() + 14 - lg);
+    const bool masked = limit_of(a, n0, len) < kw + kRows;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f4 m = *reinterpret_cast<const f4*>(Ms + 8 * q + 4 * half);
+      const f4 d = *reinterpret_cast<const f4*>(Ds + 8 * q + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * q + e;
+        float p = exp2_(s[i] * cs - (m[e] - flg));
+        if (masked && key >= Ls[8 * q + 4 * half + e]) p = 0.f;
+        s[i] = p;
+        dp[i] = p * ((dp[i] - d[e] * vs) * by);
+      }
+    }
+    add_cols<DP>(Ys, s, dv, lane);
+    add_cols<DP>(Qs, dp, dk, lane);
+  }
+  if (key >= a.T) return;
+  const bool none = key >= len;  // keys past the length get zeros
+  if (none) {
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) {
+      zero(dk[t]);
+      zero(dv[t]);
+    }
+  }
+  if (a.dv)
+    write_vec<DP, VEC>(a.dv + k_at(a, b, gh, key), a.D, half, dv, pow2(-14), Rv == 1000 ? 0.f : pow2(-Rv));
+  if (a.dk)
+    write_vec<DP, VEC>(a.dk + k_at(a, b, gh, key), a.D, half, dk,
+                       Rk == 1000 ? 0.f : pow2(down_bits<DP>() - 14 - Rk / 2) * a.scale, pow2(Rk / 2 - Rk));
+}
+
+__global__ void k_attn_no_bad(uint32_t* bad, uint32_t n) {
+  const uint32_t i = blockIdx.x * kT + threadIdx.x;
+  if (i < n) bad[i] = 0u;
+}
+
+struct Places {
+  size_t next = 0;
+  size_t take(size_t floats) {
+    const size_t p = next;
+    next += (floats + 63) & ~size_t(63);
+    return p;
+  }
+};
+
+// The parts' places and the pass that fills them.
+struct Prep {
+  Attn a;
+  Parts ps;
+  bool bwd;
+  size_t extra;   // floats behind the parts
+  float* more;    // they
+  template <int DP, bool VEC>
+  bool run() {
+    const uint32_t prob = a.B * a.G;
+    const uint32_t nq = (a.N + 127) & ~127u, nk = (a.T + 127) & ~127u;
+    Places at;
+    const size_t bad = at.take(prob);
+    const size_t q = at.take(size_t(prob) * nq * DP), qe = at.take(size_t(prob) * (nq / kRows));
+    const size_t k = at.take(size_t(prob) * nk * DP), ke = at.take(size_t(prob) * (nk / kRows));
+    const size_t v = at.take(size_t(prob) * nk * DP), ve = at.take(size_t(prob) * (nk / kRows));
+    const size_t y = bwd ? at.take(size_t(prob) * nq * DP) : 0, ye = bwd ? at.take(size_t(prob) * (nq / kRows)) : 0;
+    const size_t dl = bwd ? at.take(size_t(prob) * nq) : 0, least = bwd ? at.take(size_t(prob) * (nk / kRows)) : 0;
+    const size_t ex = at.take(extra);
+    float* ws = workspace(at.next);
+    if (!ws) return false;
+    auto part = [&](size_t p, size_t e, uint32_t pad) {
+      return Part{reinterpret_cast<char*>(ws + p), reinterpret_cast<int*>(ws + e), pad};
+    };
+    ps.q = part(q, qe, nq);
+    ps.k = part(k, ke, nk);
+    ps.v = part(v, ve, nk);
+    ps.y = part(y, ye, nq);
+    ps.dl = ws + dl;
+    ps.least = reinterpret_cast<int*>(ws + least);
+    ps.bad = reinterpret_cast<uint32_t*>(ws + bad);
+    more = ws + ex;
+    hipLaunchKernelGGL(k_attn_no_bad, dim3(cdiv(prob, kT)), dim3(kT), 0, stream(), ps.bad, prob);
+    const uint32_t per = (bwd ? 2 : 1) * (nq / kRows) + 2 * (nk / kRows);
+    if (bwd)
+      hipLaunchKernelGGL((k_attn_split<DP, VEC, true>), dim3(per * prob), dim3(kT), 0, stream(), a, ps);
+    else
+      hipLaunchKernelGGL((k_attn_split<DP, VEC, false>), dim3(per * prob), dim3(kT), 0, stream(), a, ps);
+    if (bwd) hipLaunchKernelGGL(k_attn_least, dim3(prob), dim3(kT), 0, stream(), ps);
+    return check_launch("attention (parts)");
+  }
+};
+struct Forward {
+  Attn a;
+  Parts ps;
+  template <int DP, bool VEC>
+  bool run() {
+    hipLaunchKernelGGL((k_attn_fwd_parts<DP, VEC>), dim3(a.tiles * a.splits * a.B * a.G), dim3(kT), 0, stream(), a, ps);
+    return check_launch("AttentionForward (parts)");
+  }
+};
+struct Backward {
+  Attn a;
+  Parts ps;
+  template <int DP, bool VEC>
+  bool run() {
+    const uint32_t prob = a.B * a.G;
+    if (a.dq) {
+      a.tiles = cdiv(a.N, 128);
+      hipLaunchKernelGGL((k_attn_dq_parts<DP, VEC>), dim3(a.tiles * prob), dim3(kT), 0, stream(), a, ps);
+    }
+    if (a.dk || a.dv) {
+      a.tiles = cdiv(a.T, 128);
+      hipLaunchKernelGGL((k_attn_dkv_parts<DP, VEC>), dim3(a.tiles * prob), dim3(kT), 0, stream(), a, ps);
+    }
+    return check_launch("AttentionBackward (parts)");
+  }
+};
+
+template <class F>
+bool by_dim(uint32_t D, F& f) {
+  const bool vec = D % 4 == 0;
+#define DCE_D(n) \
+  if (D <= n) return vec ? f.template run<n, true>() : f.template run<n, false>();
+  DCE_D(32) DCE_D(64) DCE_D(96) DCE_D(128)
+#undef DCE_D
+  return false;
+}
+
+bool worth(const AttnArgs& x) {
+  return x.D <= 128 && x.S >= 32 && 4.0 * x.D * x.B * x.H * pairs_of(x) >= 1e9 &&
+         uint64_t(x.B) * x.G * (uint64_t(x.H / x.G) * x.S + x.T) < 0x20000000ull;
+}
+
+}  // namespace
+
+bool attn_fwd_parts(const AttnArgs& x, Attn a, bool* took) {
+  if (!worth(x)) return true;
+  *took = true;
+  const uint32_t prob = a.B * a.G, cus = uint32_t(num_cus()), kt = cdiv(a.T, kRows);
+  a.tiles = cdiv(a.N, 128);
+  a.splits = 1;
+  if (uint64_t(a.tiles) * prob < cus) a.splits = std::max(1u, std::min(cdiv(kt, 8), cdiv(2 * cus, a.tiles * prob)));
+  a.perSplit = cdiv(kt, a.splits);
+  a.splits = cdiv(kt, a.perSplit);
+  const size_t rows = size_t(prob) * a.N, stat = (rows * a.splits + 63) & ~size_t(63);
+  Prep p{a, {}, false, a.splits > 1 ? 2 * stat + rows * a.splits * a.D : 0, nullptr};
+  if (!by_dim(a.D, p)) return false;
+  a.pm = p.more;
+  a.pl = p.more + stat;
+  a.po = p.more + 2 * stat;
+  Forward f{a, p.ps};
+  if (!by_dim(a.D, f)) return false;
+  if (a.splits > 1 && !attn_join(a)) return false;
+  a.only = p.ps.bad;
+  return attn_fwd_fp32(a);
+}
+
+bool attn_bwd_parts(const AttnArgs& x, Attn a, bool* took) {
+  if (!worth(x)) return true;
+  *took = true;
+  Prep p{a, {}, true, size_t(a.B) * a.G * a.N, nullptr};
+  if (!by_dim(a.D, p)) return false;
+  Backward f{a, p.ps};
+  if (!by_dim(a.D, f)) return false;
+  a.only = p.ps.bad;
+  a.delta = p.more;
+  return attn_bwd_fp32(a);
+}
+
+}  // namespace dce

@@ -560,3 +560,79 @@ def test_reshape(eng):
         with pytest.raises(ValueError):
             eng.reshape(t, bad)
     eng.end_batch()
+
+
+# ------------------------------------------------- large calls, on fp16 parts
+LARGE = [  # from 1e9 operations on
+    (1, 1024, 1024, 8, 8, 64, True, None),
+    (2, 700, 700, 12, 4, 40, False, [700, 333]),
+    (1, 1100, 1300, 4, 2, 128, True, None),
+    (3, 515, 777, 6, 3, 96, True, [777, 0, 261]),
+    (1, 1500, 1500, 8, 1, 30, True, None),
+    (1, 33, 9000, 8, 8, 128, True, [8999]),
+    (2, 1300, 400, 8, 2, 100, False, None),
+    (1, 2000, 1024, 4, 4, 80, True, None),          # 976 rows see nothing
+]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: "x".join(map(str, c[:6])) + ("c" if c[6] else "") + ("l" if c[7] else ""))
+def test_attention_large(eng, case):
+    test_attention(eng, case)
+
+
+@pytest.mark.parametrize("change", ["rows", "tiles", "tiny", "huge", "grads"])
+def test_attention_large_of_uneven_sizes(eng, change):
+    """Vectors of very different sizes: between the tiles of a call (the parts
+    of each tile have an exponent of their own) and within one (those problems
+    run on fp32)."""
+    case = (2, 1024, 1024, 4, 4, 64, True, None)
+    q, k, v, dy = attention_inputs(case, 60)
+    r = rng(61)
+    if change == "tiles":            # values and gradients grow and shrink along the sequence
+        v *= np.exp2(np.round(10 * np.sin(np.arange(1024) / 90)))[None, :, None, None].astype(np.float32)
+        dy *= np.exp2(np.round(10 * np.cos(np.arange(1024) / 70)))[None, :, None, None].astype(np.float32)
+    elif change == "rows":           # one head of a sequence has vectors 2^20 apart side by side
+        v[1, :, 2] *= np.exp2(r.choice([-20, 0], 1024))[:, None].astype(np.float32)
+    elif change == "tiny":
+        v *= np.float32(2.0 ** -40)
+    elif change == "huge":
+        v *= np.float32(2.0 ** 40)
+    else:                            # gradients as a mean over many tokens gives them, some of them zero
+        dy *= np.float32(2.0 ** -45)
+        dy[:, ::3] = 0
+    ts = [dev(eng, a, True) for a in (q, k, v)]
+    out = eng.attention(*ts, causal=True)
+    out.backward(dev(eng, dy))
+    ref = [torch.tensor(a, dtype=torch.float64, requires_grad=True) for a in (q, k, v)]
+    o, s_max = attend64(*ref, True, 64 ** -0.5, None)
+    o.backward(torch.tensor(dy, dtype=torch.float64))
+    tol = attention_tol(case, s_max)
+    # tol is relative to a result's largest value where all terms are of one
+    # size; here each value gets the sum of its terms' sizes instead
+    qa, ka, va, ya = (torch.tensor(a, dtype=torch.float64).permute(0, 2, 1, 3) for a in (q, k, v, dy))
+    p = torch.softmax((qa @ ka.transpose(2, 3) / 8).masked_fill(~torch.ones(1024, 1024, dtype=torch.bool).tril(), -math.inf), -1)
+    big = lambda t: t.abs().amax(-1, keepdim=True)  # noqa: E731
+    dp = ya.abs() @ va.abs().transpose(2, 3)
+    ds = p * (dp + (p * dp).sum(-1, keepdim=True)) / 8
+    size = [p @ big(va), ds @ big(ka), ds.transpose(2, 3) @ big(qa), p.transpose(2, 3) @ big(ya)]
+    for i, (got, want, z) in enumerate(zip([out.sync()] + [t.grad.sync() for t in ts],
+                                           [o.detach()] + [t.grad for t in ref], size)):
+        z = z.permute(0, 2, 1, 3).numpy()
+        e = np.abs(got - want.numpy()).max(-1, keepdims=True)
+        print(change, "%.2g of the terms' size, tol %.2g" % ((e[z > 0] / z[z > 0]).max(), (4 if i else 1) * tol), flush=True)
+        assert (e <= (4 if i else 1) * tol * z).all()
+    eng.end_batch()
+
+
+def test_attention_large_not_finite(eng):
+    case = (2, 1024, 1024, 4, 4, 64, True, None)
+    q, k, v, _ = attention_inputs(case, 62)
+    clean = eng.attention(dev(eng, q), dev(eng, k), dev(eng, v), causal=True).sync().copy()
+    v[1, 500, 3] = np.inf
+    q[0, 9, 1] = np.nan
+    out = eng.attention(dev(eng, q), dev(eng, k), dev(eng, v), causal=True).sync()
+    assert np.array_equal(out[0, :, [0, 2, 3]], clean[0, :, [0, 2, 3]]) and np.array_equal(out[1, :, :3], clean[1, :, :3])
+    assert np.isnan(out[0, 9, 1]).all() and np.array_equal(np.isnan(out[0, :, 1]).any(-1).nonzero()[0], [9])
+    # dim by dim: an infinite value is in every later sum
+    assert not np.isfinite(out[1, 500:, 3]).any() and np.isfinite(out[1, :480, 3]).all()
+    eng.end_batch()
