@@ -12,6 +12,11 @@ namespace dce {
 // Tokens come as [batch][token][head][dim].  `rep` query heads share one key
 // head, so the problem of one (sequence, key head) pair is N = rep * S query
 // rows against up to T keys: row n is query n / rep of head n % rep.
+//
+// Workgroups go through the problems first and their tiles next, the tiles with
+// most work ahead: the last ones to start are the shortest, and as consecutive
+// workgroups go to the 8 XCDs in turn, each XCD's L2 sees an eighth of the
+// problems, or one of them where they are few.
 struct Attn {
   const float *q, *k, *v, *len;  // len: keys of each sequence, or null
   float* o;

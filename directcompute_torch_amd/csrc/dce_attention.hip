@@ -49,9 +49,13 @@ __device__ __forceinline__ void load_frag(const float* p, bool ok, uint32_t D, i
   }
 }
 
+template <int CH>
+__device__ __forceinline__ int swz(int row) {
+  return CH % 16 == 0 ? row & 15 : (row >> 1) & 7;
+}
 // An LDS tile of R vectors padded to DP dims, row pitch DP, the 16-byte chunks
-// of a row XORed by row % 8 so that eight rows' equal chunks lie in different
-// banks.  Loaded through registers; rows and dims past the ends read zeros
+// of a row XORed by the row so that a read of one chunk of 16 rows covers the 64
+// banks once.  Loaded through registers; rows and dims past the ends read zeros
 // (never what memory holds there, which may be NaN).
 template <int DP, int R, bool VEC>
 struct Tile {
@@ -73,12 +77,12 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const uint32_t slot = threadIdx.x + kT * i, row = slot / CH, c = slot % CH;
-      *reinterpret_cast<f4*>(S + (row * CH + (c ^ (row & 7))) * 4) = r[i];
+      *reinterpret_cast<f4*>(S + (row * CH + (c ^ swz<CH>(row))) * 4) = r[i];
     }
   }
   // Dims 4 c .. + 3 of a row.
   __device__ static __forceinline__ f4 chunk(const float* S, int row, int c) {
-    return *reinterpret_cast<const f4*>(S + (row * CH + (c ^ (row & 7))) * 4);
+    return *reinterpret_cast<const f4*>(S + (row * CH + (c ^ swz<CH>(row))) * 4);
   }
 };
 // Blocks of a transposed operand read at once: 16 EG dims, lane m's are EG m .. + EG - 1.
@@ -89,7 +93,7 @@ struct Cols {
   __device__ static __forceinline__ V read(const float* S, int row, int q, int m) {
     constexpr int CH = DP / 4;
     const int d = 16 * EG * q + EG * m;
-    return *reinterpret_cast<const V*>(S + (row * CH + ((d >> 2) ^ (row & 7))) * 4 + (d & 3));
+    return *reinterpret_cast<const V*>(S + (row * CH + ((d >> 2) ^ swz<CH>(row))) * 4 + (d & 3));
   }
   // acc blocks of one vector (a lane's column): dims 16 EG q + EG (4 g + r) + e.
   template <bool VEC>
@@ -139,9 +143,8 @@ __global__ void __launch_bounds__(kT) k_attn_fwd(const Attn a) {
   using TL = Tile<DP, kKeys, VEC>;
   using CL = Cols<DP>;
   __shared__ __attribute__((aligned(16))) float Ks[kKeys * DP], Vs[kKeys * DP];
-  const uint32_t id = xcd_block_id();
-  const uint32_t per = a.tiles * a.splits, pr = id / per, rest = id - pr * per;
-  const uint32_t sp = rest / a.tiles, tile = a.tiles - 1 - (rest - sp * a.tiles);  // long rows first
+  const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
+  const uint32_t back = rest / a.splits, sp = rest - back * a.splits, tile = a.tiles - 1 - back;
   if (a.only && !a.only[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
@@ -301,8 +304,8 @@ __global__ void __launch_bounds__(kT) k_attn_dq(const Attn a) {
   using TL = Tile<DP, kKeys, VEC>;
   using CL = Cols<DP>;
   __shared__ __attribute__((aligned(16))) float Ks[kKeys * DP], Vs[kKeys * DP];
-  const uint32_t id = xcd_block_id();
-  const uint32_t pr = id / a.tiles, tile = a.tiles - 1 - (id - pr * a.tiles);
+  const uint32_t prob = a.B * a.G, back = blockIdx.x / prob, pr = blockIdx.x - back * prob;
+  const uint32_t tile = a.tiles - 1 - back;
   if (a.only && !a.only[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
@@ -411,8 +414,7 @@ __global__ void __launch_bounds__(kT) k_attn_dkv(const Attn a) {
   using CL = Cols<DP>;
   __shared__ __attribute__((aligned(16))) float Qs[kKeys * DP], Ys[kKeys * DP], St[3 * kKeys];
   __shared__ uint32_t Lim[kKeys];
-  const uint32_t id = xcd_block_id();
-  const uint32_t pr = id / a.tiles, tile = id - pr * a.tiles;
+  const uint32_t prob = a.B * a.G, tile = blockIdx.x / prob, pr = blockIdx.x - tile * prob;
   if (a.only && !a.only[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;

@@ -18,7 +18,9 @@
 // exponents (over V's in the forward, dO's and Q's for dV and dK) its terms are
 // brought to the smallest exponent so far, which the exponential's offset takes.
 //
-// P is relative to its row's maximum here, within [0, 1], and kept as 2^14 P; the
+// P is relative to its row's maximum, within [0, 1], and kept as 2^14 P.  The
+// forward only follows its running maximum, and scales the sums so far, where a
+// score passes it by more than 2^8: its P is at most 2^8, kept as 2^7 P.  The
 // backward's 1 / l goes into dO (dO' = dO / l) when that is split, so that
 // dV = P^T dO' and dS = scale P (dO' V^T - delta'), delta' = rowsum(dO' * O).
 // delta' is of the size of the largest vector that a row sees, whatever tile it
@@ -34,8 +36,11 @@ constexpr int kT = 256;
 constexpr int kRows = 32;         // vectors of a tile
 constexpr int kRange = 30;        // exponents of values that parts are made of
 constexpr int kRangeGrad = 60;    // and of gradients
+constexpr float kSlack = 8.f;     // of the forward's running maximum, in powers of 2
+constexpr int kExpP = 7;          // the forward's P parts hold p 2^7, p up to 2^kSlack
 constexpr float kWide = 16384.f;  // largest ratio of the vectors' sizes in a tile
 
+using h2 = _Float16 __attribute__((ext_vector_type(2)));
 using h4 = _Float16 __attribute__((ext_vector_type(4)));
 using h8 = _Float16 __attribute__((ext_vector_type(8)));
 using f16v = float __attribute__((ext_vector_type(16)));
@@ -214,16 +219,16 @@ __global__ void __launch_bounds__(kT) k_attn_split(const Attn a, const Parts ps)
 
 // ---------------------------------------------------------------------------
 // An LDS tile of 32 vectors' parts: the h plane, then the l plane, the 16-byte
-// chunks of a row XORed by the row, so that eight rows' equal chunks lie in
-// different banks, and neighbouring rows in different halves of them (a
-// transposed read takes 64 bytes of each of eight rows).
+// chunks of a row XORed by the row: a read of one chunk of 16 rows covers the 64
+// banks once, and so does a transposed read, 64 bytes of each of four rows.
 // ---------------------------------------------------------------------------
 template <int DP>
 struct PTile {
   static constexpr int CH = DP / 8, PLANE = kRows * DP * 2, BYTES = 2 * PLANE, LOADS = BYTES / 16 / kT;
   static_assert(BYTES % (16 * kT) == 0, "whole slots");
   __device__ static __forceinline__ int swz(int row) {
-    return CH % 8 == 0 ? ((row & 1) << 2) | ((row >> 1) & 3) : (row >> 1) & 3;
+    const int low = (row >> 2) & 3;
+    return CH % 16 == 0 ? ((row & 3) << 2) | low : CH % 8 == 0 ? ((row & 2) << 1) | low : low;
   }
   __device__ static __forceinline__ void load(const char* p, u4v (&r)[LOADS]) {
 #pragma unroll
@@ -270,11 +275,16 @@ __device__ __forceinline__ void load_vec(const char* p, int half, h8 (&h)[DP / 1
 // and from the float in another, which differ by a step once in some 2^12 values.
 __device__ __forceinline__ void split_acc(const f16v& s, int k, h8& h, h8& l) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float x = s[8 * k + e];
+  for (int e = 0; e < 8; e += 2) {
+    f2 x = {s[8 * k + e], s[8 * k + e + 1]};
     asm("" : "+v"(x));
-    h[e] = _Float16(x);
-    l[e] = _Float16(x - float(h[e]));
+    const h2 hh = __builtin_convertvector(x, h2);
+    const f2 r = {__builtin_fmaf(float(hh[0]), -1.f, x[0]), __builtin_fmaf(float(hh[1]), -1.f, x[1])};
+    const h2 ll = __builtin_convertvector(r, h2);
+    h[e] = hh[0];
+    h[e + 1] = hh[1];
+    l[e] = ll[0];
+    l[e + 1] = ll[1];
   }
 }
 // The tile's vectors times a lane's: out[e] is row 8 (e / 4) + 4 (lane / 32) + e % 4.
@@ -336,9 +346,8 @@ template <int DP, bool VEC>
 __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Parts ps) {
   using TL = PTile<DP>;
   __shared__ __attribute__((aligned(16))) char Ks[TL::BYTES], Vs[TL::BYTES];
-  const uint32_t id = xcd_block_id();
-  const uint32_t per = a.tiles * a.splits, pr = id / per, rest = id - pr * per;
-  const uint32_t sp = rest / a.tiles, tile = a.tiles - 1 - (rest - sp * a.tiles);  // long rows first
+  const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
+  const uint32_t back = rest / a.splits, sp = rest - back * a.splits, tile = a.tiles - 1 - back;
   if (ps.bad[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
@@ -355,8 +364,8 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
   f16v o[DP / 32];
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) zero(o[t]);
-  float m = -INFINITY, l = 0.f;
-  int R = 1000;  // o counts in units of 2^-(14 + R)
+  float m = -INFINITY, l = 0.f, most_s = -INFINITY;
+  int R = 1000;  // o counts in units of 2^-(kExpP + R)
   const uint32_t j0 = sp * a.perSplit * kRows, j1 = min(most, (sp + 1) * a.perSplit * kRows);
   u4v rk[TL::LOADS], rv[TL::LOADS];
   auto fetch = [&](uint32_t j) {
@@ -389,15 +398,17 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
         top = fmaxf(top, s[i]);
       }
     }
-    top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
-    const float base = top == -INFINITY ? 0.f : top;  // nothing seen yet: every p is 0
+    top = fmaxf(top, __shfl_xor(top, 32));
+    most_s = fmaxf(most_s, top);
     float down = 1.f;
-    bool move = __any(top > m);
+    bool move = __any(top > m + kSlack);
     if (move) {
-      down = exp2_(m - base);
+      top = fmaxf(m, top);
+      down = m == -INFINITY ? 0.f : exp2_(m - top);
       l *= down;
       m = top;
     }
+    const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet: every p is 0
     if (e < R) {
       down *= R == 1000 ? 1.f : pow2(e - R);
       R = e;
@@ -409,8 +420,8 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] *= down;
     }
-    // p 2^(14 + R - e), which the exponential's offset brings in
-    const int lg = 14 + max(R - e, -60);
+    // p 2^(kExpP + R - e), which the exponential's offset brings in
+    const int lg = kExpP + max(R - e, -60);
     const float off = base - float(lg);
     float sum = 0.f;
 #pragma unroll
@@ -423,7 +434,11 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
   }
   l += __shfl_xor(l, 32);
   if (n >= a.N) return;
-  const float unit = R == 1000 ? 0.f : pow2(-14);
+  // From here on relative to the largest score itself, as the backward has it.
+  const float up = m == -INFINITY ? 1.f : exp2_(m - most_s);
+  l *= up;
+  m = most_s;
+  const float unit = R == 1000 ? 0.f : pow2(-kExpP) * up;
   const float unit2 = R == 1000 ? 0.f : pow2(-R);
   if (a.splits > 1) {
     const size_t row = (size_t(sp) * a.B * a.G + pr) * a.N + n;
@@ -456,8 +471,8 @@ template <int DP, bool VEC>
 __global__ void __launch_bounds__(kT, DP <= 64 ? 2 : 1) k_attn_dq_parts(const Attn a, const Parts ps) {
   using TL = PTile<DP>;
   __shared__ __attribute__((aligned(16))) char Ks[TL::BYTES], Vs[TL::BYTES];
-  const uint32_t id = xcd_block_id();
-  const uint32_t pr = id / a.tiles, tile = a.tiles - 1 - (id - pr * a.tiles);
+  const uint32_t prob = a.B * a.G, back = blockIdx.x / prob, pr = blockIdx.x - back * prob;
+  const uint32_t tile = a.tiles - 1 - back;
   if (ps.bad[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
@@ -534,8 +549,7 @@ __global__ void __launch_bounds__(kT, DP <= 64 ? 2 : 1) k_attn_dkv_parts(const A
   __shared__ __attribute__((aligned(16))) char Qs[TL::BYTES], Ys[TL::BYTES];
   __shared__ __attribute__((aligned(16))) float Ms[kRows], Ds[kRows];
   __shared__ uint32_t Ls[kRows];
-  const uint32_t id = xcd_block_id();
-  const uint32_t pr = id / a.tiles, tile = id - pr * a.tiles;
+  const uint32_t prob = a.B * a.G, tile = blockIdx.x / prob, pr = blockIdx.x - tile * prob;
   if (ps.bad[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;

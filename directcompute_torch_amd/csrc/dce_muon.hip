@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kT) k_muon_update(const Mats t, float* ws, flo
 // waves of 64 x 64 (2 x 2 blocks of 32 x 32), the depth in steps of 32 through
 // two LDS stages, the next one's direct loads in flight while one is multiplied.
 // A stage row is 128 bytes (4 blocks of 8 h, 8 l); its 16-byte slots are XORed
-// by row % 8, so that eight rows' equal slots lie in different banks.
+// by row / 2 % 8, so that a read of one slot of 16 rows covers the 64 banks once.
 // ---------------------------------------------------------------------------
 enum Op { GRAM, POLY, APPLY, LAST };
 constexpr int kStage = kBlk * kStep * 4;  // bytes of one operand's stage
@@ -211,12 +211,12 @@ __device__ __forceinline__ void stage_load(const BRes& b, uint32_t pitchBytes, u
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
   for (int i = 0; i < kStage / 16 / kT; ++i) {
-    const uint32_t slot = threadIdx.x + kT * i, row = slot >> 3, c = (slot & 7) ^ (row & 7);
+    const uint32_t slot = threadIdx.x + kT * i, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
     b.ld16_lds(row * pitchBytes + k * 4 + c * 16, S + (wave * 64 + i * kT) * 16);
   }
 }
 __device__ __forceinline__ h8 stage_frag(const char* S, int row, int c) {
-  return *reinterpret_cast<const h8*>(S + row * 128 + ((c ^ (row & 7)) * 16));
+  return *reinterpret_cast<const h8*>(S + row * 128 + ((c ^ ((row >> 1) & 7)) * 16));
 }
 // Tile (i, j), i <= j, of the upper triangle in row order.
 __device__ __forceinline__ void triangle(uint32_t id, uint32_t n, uint32_t& i, uint32_t& j) {
