@@ -222,23 +222,25 @@ __global__ void __launch_bounds__(kT) k_attn_split(const Attn a, const Parts ps)
 // chunks of a row XORed by the row: a read of one chunk of 16 rows covers the 64
 // banks once, and so does a transposed read, 64 bytes of each of four rows.
 // ---------------------------------------------------------------------------
-template <int DP>
+template <int DP, int NT = kT>
 struct PTile {
-  static constexpr int CH = DP / 8, PLANE = kRows * DP * 2, BYTES = 2 * PLANE, LOADS = BYTES / 16 / kT;
-  static_assert(BYTES % (16 * kT) == 0, "whole slots");
+  static constexpr int CH = DP / 8, PLANE = kRows * DP * 2, BYTES = 2 * PLANE, SLOTS = BYTES / 16;
+  static constexpr int LOADS = (SLOTS + NT - 1) / NT;
+  static constexpr bool WHOLE = SLOTS % NT == 0;  // else the last load is for some threads only
   __device__ static __forceinline__ int swz(int row) {
     const int low = (row >> 2) & 3;
     return CH % 16 == 0 ? ((row & 3) << 2) | low : CH % 8 == 0 ? ((row & 2) << 1) | low : low;
   }
   __device__ static __forceinline__ void load(const char* p, u4v (&r)[LOADS]) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) r[i] = reinterpret_cast<const u4v*>(p)[threadIdx.x + kT * i];
+    for (int i = 0; i < LOADS; ++i)
+      if (WHOLE || threadIdx.x + NT * i < SLOTS) r[i] = reinterpret_cast<const u4v*>(p)[threadIdx.x + NT * i];
   }
   __device__ static __forceinline__ void store(char* S, const u4v (&r)[LOADS]) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int m = threadIdx.x + kT * i, row = m / (2 * CH), pl = m / CH & 1, c = m % CH;
-      *reinterpret_cast<u4v*>(S + pl * PLANE + (row * CH + (c ^ swz(row))) * 16) = r[i];
+      const int m = threadIdx.x + NT * i, row = m / (2 * CH), pl = m / CH & 1, c = m % CH;
+      if (WHOLE || m < SLOTS) *reinterpret_cast<u4v*>(S + pl * PLANE + (row * CH + (c ^ swz(row))) * 16) = r[i];
     }
   }
   // Row `row`, dims 8 c .. + 7.
@@ -465,73 +467,123 @@ constexpr int down_bits() {
 }
 
 // ---------------------------------------------------------------------------
-// dQ: 128 query rows per workgroup, Q and dO' in registers.
+// The backward kernels: eight waves, in pairs of one 32-vector block each.  The
+// first of a pair computes P = exp(S - m) and leaves it in LDS; the second, a
+// tile behind it, dP and dS.  Each holds only its own operand and sums, half of
+// what one wave would need (over 256 registers at 128 dims, one wave per SIMD:
+// 1400 and 784 us for dK, dV and dQ of 2 x 4096 tokens, 16 heads of 128), and a
+// SIMD, which has one of each, multiplies for one while the other is at its
+// exponentials.  Three LDS stages, one barrier per tile.
+// ---------------------------------------------------------------------------
+constexpr int kPair = 512;  // threads
+constexpr int kStages = 3;
+
+__device__ __forceinline__ void put_p(float* P, int lane, const f16v& s) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<f4*>(P + (q * 64 + lane) * 4) = f4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+}
+__device__ __forceinline__ f4 get_p(const float* P, int lane, int q) {
+  return *reinterpret_cast<const f4*>(P + (q * 64 + lane) * 4);
+}
+template <int N>
+__device__ __forceinline__ void scale_acc(f16v (&acc)[N], float by) {
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] *= by;
+}
+
+// ---------------------------------------------------------------------------
+// dQ: 128 query rows per workgroup; Q in the first waves' registers, dO' and the
+// sums in the second ones'.
 // ---------------------------------------------------------------------------
 template <int DP, bool VEC>
-__global__ void __launch_bounds__(kT, DP <= 64 ? 2 : 1) k_attn_dq_parts(const Attn a, const Parts ps) {
-  using TL = PTile<DP>;
-  __shared__ __attribute__((aligned(16))) char Ks[TL::BYTES], Vs[TL::BYTES];
+__global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const Parts ps) {
+  using TL = PTile<DP, kPair>;
+  __shared__ __attribute__((aligned(16))) char Ks[kStages][TL::BYTES], Vs[kStages][TL::BYTES];
+  __shared__ __attribute__((aligned(16))) float Ps[2][4][1024];
   const uint32_t prob = a.B * a.G, back = blockIdx.x / prob, pr = blockIdx.x - back * prob;
   const uint32_t tile = a.tiles - 1 - back;
   if (ps.bad[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
-  const uint32_t n0 = tile * 128, n = n0 + wave * 32 + col, len = keys_of(a, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blk = wave & 3, col = lane & 31, half = lane >> 5;
+  const bool first = __builtin_amdgcn_readfirstlane(wave) < 4;
+  const uint32_t n0 = tile * 128, n = n0 + blk * 32 + col, len = keys_of(a, b);
   const uint32_t least = limit_of(a, n0, len), most = limit_of(a, min(n0 + 128, a.N) - 1, len);
-  const uint32_t lim = n < a.N ? limit_of(a, n, len) : 0u, mine = wave_limit(a, n0 + wave * 32, kRows, len);
+  const uint32_t lim = n < a.N ? limit_of(a, n, len) : 0u, mine = wave_limit(a, n0 + blk * 32, kRows, len);
   const size_t row = size_t(pr) * ps.q.pad + n;
-  h8 qh[DP / 16], ql[DP / 16], yh[DP / 16], yl[DP / 16];
-  load_vec<DP>(ps.q.p + row * (DP * 4), half, qh, ql);
-  load_vec<DP>(ps.y.p + row * (DP * 4), half, yh, yl);
-  const size_t et = size_t(pr) * (ps.q.pad / kRows) + n0 / kRows + wave;
-  const float cq = a.c * pow2(-ps.q.e[et]), m = n < a.N ? a.m[size_t(pr) * a.N + n] : 0.f;
-  const float delta = ps.dl[row];
-  const int ey = ps.y.e[et];
+  const size_t et = size_t(pr) * (ps.q.pad / kRows) + n0 / kRows + blk;
   const int* ek = ps.k.e + size_t(pr) * (ps.k.pad / kRows);
   const int* ev = ps.v.e + size_t(pr) * (ps.v.pad / kRows);
   const char* kp = ps.k.p + size_t(pr) * ps.k.pad * (DP * 4);
   const char* vp = ps.v.p + size_t(pr) * ps.v.pad * (DP * 4);
+  const uint32_t tiles = (most + kRows - 1) / kRows;
+  u4v rk[TL::LOADS], rv[TL::LOADS];
+  auto fetch = [&](uint32_t t) {
+    TL::load(kp + size_t(t) * kRows * (DP * 4), rk);
+    TL::load(vp + size_t(t) * kRows * (DP * 4), rv);
+  };
+  auto stage = [&](uint32_t t) {  // tile t from the registers, which then take t + 1
+    if (t >= tiles) return;
+    TL::store(Ks[t % kStages], rk);
+    TL::store(Vs[t % kStages], rv);
+    if (t + 1 < tiles) fetch(t + 1);
+  };
+  if (tiles) fetch(0);
+  stage(0);
+  __syncthreads();
+  h8 xh[DP / 16], xl[DP / 16];
+  if (first) {
+    load_vec<DP>(ps.q.p + row * (DP * 4), half, xh, xl);
+    const float cq = a.c * pow2(-ps.q.e[et]), m = n < a.N ? a.m[size_t(pr) * a.N + n] : 0.f;
+    for (uint32_t t = 0; t <= tiles; ++t) {
+      stage(t + 1);
+      const uint32_t j = t * kRows;
+      if (j < mine) {
+        const float cs = cq * pow2(-ek[t]);
+        f16v s = scores<DP>(Ks[t % kStages], xh, xl, col, half);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = exp2_(s[i] * cs - m);
+        if (j + kRows > least) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (j + 8 * (i >> 2) + 4 * half + (i & 3) >= lim) s[i] = 0.f;
+        }
+        put_p(Ps[t & 1][blk], lane, s);
+      }
+      __syncthreads();
+    }
+    return;
+  }
+  load_vec<DP>(ps.y.p + row * (DP * 4), half, xh, xl);
+  const float delta = ps.dl[row];
+  const int ey = ps.y.e[et];
   f16v dq[DP / 32];
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) zero(dq[t]);
   const int E = mine ? ps.least[size_t(pr) * (ps.v.pad / kRows) + (mine - 1) / kRows] : 0;
   int R = 1000;  // dq counts in units of 2^-(R + E + ey - down_bits + 14)
-  u4v rk[TL::LOADS], rv[TL::LOADS];
-  auto fetch = [&](uint32_t j) {
-    TL::load(kp + size_t(j) * (DP * 4), rk);
-    TL::load(vp + size_t(j) * (DP * 4), rv);
-  };
-  if (most) fetch(0);
-  for (uint32_t j = 0; j < most; j += kRows) {
-    __syncthreads();
-    TL::store(Ks, rk);
-    TL::store(Vs, rv);
-    __syncthreads();
-    if (j + kRows < most) fetch(j + kRows);
-    if (j >= mine) continue;
-    const int xk = ek[j / kRows], xv = ev[j / kRows];
-    const float cs = cq * pow2(-xk);
-    f16v s = scores<DP>(Ks, qh, ql, col, half);
-    f16v dp = scores<DP>(Vs, yh, yl, col, half);
-    if (xk < R) {
-      if (R != 1000) {
-        const float down = pow2(xk - R);
-#pragma unroll
-        for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) dq[t][i] *= down;
+  for (uint32_t t = 0; t <= tiles; ++t) {
+    stage(t + 1);
+    const uint32_t u = t - 1;  // the tile before the first waves'
+    if (t && u * kRows < mine) {
+      const int xk = ek[u], xv = ev[u];
+      f16v dp = scores<DP>(Vs[u % kStages], xh, xl, col, half);
+      if (xk < R) {
+        if (R != 1000) scale_acc(dq, pow2(xk - R));
+        R = xk;
       }
-      R = xk;
-    }
-    const float dl = delta * pow2(xv), by = pow2(R - xk + E - xv - down_bits<DP>() + 14);
-    const bool masked = j + kRows > least;
+      const float dl = delta * pow2(xv), by = pow2(R - xk + E - xv - down_bits<DP>() + 14);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float v = exp2_(s[i] * cs - m) * ((dp[i] - dl) * by);
-      const uint32_t key = j + 8 * (i >> 2) + 4 * half + (i & 3);
-      s[i] = masked && key >= lim ? 0.f : v;
+      for (int q = 0; q < 4; ++q) {
+        const f4 p = get_p(Ps[u & 1][blk], lane, q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * q + e] = p[e] * ((dp[4 * q + e] - dl) * by);
+      }
+      add_cols<DP>(Ks[u % kStages], dp, dq, lane);
     }
-    add_cols<DP>(Ks, s, dq, lane);
+    __syncthreads();
   }
   if (n >= a.N) return;
   // 2^(down_bits - 14 - R - E - ey), in two factors that stay in range
@@ -540,125 +592,139 @@ __global__ void __launch_bounds__(kT, DP <= 64 ? 2 : 1) k_attn_dq_parts(const At
 }
 
 // ---------------------------------------------------------------------------
-// dK, dV: 128 keys per workgroup, 32 per wave, K and V in registers; tiles of
-// query rows of every head that shares them through LDS.
+// dK, dV: 128 keys per workgroup; K and dV's sums in the first waves' registers,
+// V and dK's in the second ones'; tiles of query rows of every head that shares
+// the keys through LDS.
 // ---------------------------------------------------------------------------
 template <int DP, bool VEC>
-__global__ void __launch_bounds__(kT, DP <= 64 ? 2 : 1) k_attn_dkv_parts(const Attn a, const Parts ps) {
-  using TL = PTile<DP>;
-  __shared__ __attribute__((aligned(16))) char Qs[TL::BYTES], Ys[TL::BYTES];
-  __shared__ __attribute__((aligned(16))) float Ms[kRows], Ds[kRows];
-  __shared__ uint32_t Ls[kRows];
+__global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const Parts ps) {
+  using TL = PTile<DP, kPair>;
+  __shared__ __attribute__((aligned(16))) char Qs[kStages][TL::BYTES], Ys[kStages][TL::BYTES];
+  __shared__ __attribute__((aligned(16))) float Ps[2][4][1024];
+  __shared__ __attribute__((aligned(16))) float Ms[kStages][kRows], Ds[kStages][kRows];
+  __shared__ uint32_t Ls[kStages][kRows];
   const uint32_t prob = a.B * a.G, tile = blockIdx.x / prob, pr = blockIdx.x - tile * prob;
   if (ps.bad[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
-  const uint32_t k0 = tile * 128, kw = k0 + wave * 32, key = kw + col, len = keys_of(a, b);
-  const uint32_t kws = __builtin_amdgcn_readfirstlane(kw);
-  const size_t row = size_t(pr) * ps.k.pad + key;
-  h8 kh[DP / 16], kl[DP / 16], vh[DP / 16], vl[DP / 16];
-  load_vec<DP>(ps.k.p + row * (DP * 4), half, kh, kl);
-  load_vec<DP>(ps.v.p + row * (DP * 4), half, vh, vl);
-  const size_t kt = size_t(pr) * (ps.k.pad / kRows) + kw / kRows;
-  const int xk = ps.k.e[kt], xv = ps.v.e[kt];
-  const float ck = a.c * pow2(-xk), vs = pow2(xv);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blk = wave & 3, col = lane & 31, half = lane >> 5;
+  const bool first = __builtin_amdgcn_readfirstlane(wave) < 4;
+  const uint32_t k0 = tile * 128, kw = __builtin_amdgcn_readfirstlane(k0 + blk * 32), key = kw + col;
+  const uint32_t len = keys_of(a, b);
+  const size_t row = size_t(pr) * ps.k.pad + key, kt = size_t(pr) * (ps.k.pad / kRows) + kw / kRows;
   const int* eq = ps.q.e + size_t(pr) * (ps.q.pad / kRows);
   const int* ey = ps.y.e + size_t(pr) * (ps.q.pad / kRows);
-  const int* least = ps.least + size_t(pr) * (ps.v.pad / kRows);
   const char* qp = ps.q.p + size_t(pr) * ps.q.pad * (DP * 4);
   const char* yp = ps.y.p + size_t(pr) * ps.q.pad * (DP * 4);
-  f16v dk[DP / 32], dv[DP / 32];
-#pragma unroll
-  for (int t = 0; t < DP / 32; ++t) {
-    zero(dk[t]);
-    zero(dv[t]);
-  }
-  int Rv = 1000, Rk = 1000;  // dv counts in units of 2^-(14 + Rv), dk of 2^-(Rk - down_bits + 14)
-  const uint32_t first = k0 < len ? min(first_row(a, k0), a.N) & ~uint32_t(kRows - 1) : a.N;
+  const uint32_t t0 = (k0 < len ? min(first_row(a, k0), a.N) : a.N) / kRows;
+  const uint32_t t1 = k0 < len ? (a.N + kRows - 1) / kRows : t0;
   u4v rq[TL::LOADS], ry[TL::LOADS];
   float rm = 0.f, rd = 0.f;
   uint32_t rl = 0;
-  auto fetch = [&](uint32_t n) {
-    TL::load(qp + size_t(n) * (DP * 4), rq);
-    TL::load(yp + size_t(n) * (DP * 4), ry);
+  auto fetch = [&](uint32_t t) {
+    TL::load(qp + size_t(t) * kRows * (DP * 4), rq);
+    TL::load(yp + size_t(t) * kRows * (DP * 4), ry);
     if (threadIdx.x < kRows) {
-      const uint32_t i = n + threadIdx.x;
+      const uint32_t i = t * kRows + threadIdx.x;
       rm = i < a.N ? a.m[size_t(pr) * a.N + i] : 0.f;
       rl = i < a.N ? limit_of(a, i, len) : 0u;
       rd = ps.dl[size_t(pr) * ps.q.pad + i];
     }
   };
-  if (first < a.N) fetch(first);
-  for (uint32_t n0 = first; n0 < a.N; n0 += kRows) {
-    __syncthreads();
-    TL::store(Qs, rq);
-    TL::store(Ys, ry);
+  auto stage = [&](uint32_t t) {  // tile t from the registers, which then take t + 1
+    if (t >= t1) return;
+    const uint32_t s = t % kStages;
+    TL::store(Qs[s], rq);
+    TL::store(Ys[s], ry);
     if (threadIdx.x < kRows) {
-      Ms[threadIdx.x] = rm;
-      Ds[threadIdx.x] = rd;
-      Ls[threadIdx.x] = rl;
+      Ms[s][threadIdx.x] = rm;
+      Ds[s][threadIdx.x] = rd;
+      Ls[s][threadIdx.x] = rl;
+    }
+    if (t + 1 < t1) fetch(t + 1);
+  };
+  if (t0 < t1) fetch(t0);
+  stage(t0);
+  __syncthreads();
+  h8 xh[DP / 16], xl[DP / 16];
+  f16v acc[DP / 32];
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) zero(acc[t]);
+  int Rv = 1000;  // dv counts in units of 2^-(14 + Rv)
+  if (first) {
+    load_vec<DP>(ps.k.p + row * (DP * 4), half, xh, xl);
+    const float ck = a.c * pow2(-ps.k.e[kt]);
+    for (uint32_t t = t0; t <= t1; ++t) {
+      stage(t + 1);
+      if (t < t1 && wave_limit(a, t * kRows, kRows, len) > kw) {
+        const uint32_t st = t % kStages;
+        const int xy = ey[t];
+        const float cs = ck * pow2(-eq[t]);
+        f16v s = scores<DP>(Qs[st], xh, xl, col, half);
+        if (xy < Rv) {
+          if (Rv != 1000) scale_acc(acc, pow2(xy - Rv));
+          Rv = xy;
+        }
+        const float lg = float(14 + max(Rv - xy, -60));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f4 m = *reinterpret_cast<const f4*>(Ms[st] + 8 * q + 4 * half);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * q + e] = exp2_(s[4 * q + e] * cs - (m[e] - lg));
+        }
+        if (limit_of(a, t * kRows, len) < kw + kRows) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (key >= Ls[st][8 * (i >> 2) + 4 * half + (i & 3)]) s[i] = 0.f;
+        }
+        put_p(Ps[t & 1][blk], lane, s);
+        add_cols<DP>(Ys[st], s, acc, lane);
+      }
+      __syncthreads();
+    }
+    if (key >= a.T || !a.dv) return;
+    if (key >= len)  // keys past the length get zeros
+#pragma unroll
+      for (int t = 0; t < DP / 32; ++t) zero(acc[t]);
+    write_vec<DP, VEC>(a.dv + k_at(a, b, gh, key), a.D, half, acc, pow2(-14), Rv == 1000 ? 0.f : pow2(-Rv));
+    return;
+  }
+  load_vec<DP>(ps.v.p + row * (DP * 4), half, xh, xl);
+  const int xv = ps.v.e[kt];
+  const float vs = pow2(xv);
+  const int* least = ps.least + size_t(pr) * (ps.v.pad / kRows);
+  int Rk = 1000;  // dk counts in units of 2^-(Rk - down_bits + 14)
+  for (uint32_t t = t0; t <= t1; ++t) {
+    stage(t + 1);
+    const uint32_t u = t - 1;  // the tile before the first waves'
+    const uint32_t seen = t > t0 ? wave_limit(a, u * kRows, kRows, len) : 0u;
+    if (seen > kw) {
+      const uint32_t st = u % kStages;
+      const int xy = ey[u], E = least[(seen - 1) / kRows], x = eq[u] + xy + E;
+      f16v dp = scores<DP>(Ys[st], xh, xl, col, half);
+      Rv = min(Rv, xy);
+      if (x < Rk) {
+        if (Rk != 1000) scale_acc(acc, pow2(x - Rk));
+        Rk = x;
+      }
+      const int lg = 14 + max(Rv - xy, -60);
+      const float by = pow2(Rk - x + E - xv - down_bits<DP>() + 14 - lg);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f4 p = get_p(Ps[u & 1][blk], lane, q);
+        const f4 d = *reinterpret_cast<const f4*>(Ds[st] + 8 * q + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * q + e] = p[e] * ((dp[4 * q + e] - d[e] * vs) * by);
+      }
+      add_cols<DP>(Qs[st], dp, acc, lane);
     }
     __syncthreads();
-    if (n0 + kRows < a.N) fetch(n0 + kRows);
-    const uint32_t seen = wave_limit(a, n0, kRows, len);
-    if (seen <= kws) continue;
-    const int xq = eq[n0 / kRows], xy = ey[n0 / kRows], E = least[(seen - 1) / kRows], x = xq + xy + E;
-    const float cs = ck * pow2(-xq);
-    f16v s = scores<DP>(Qs, kh, kl, col, half);
-    f16v dp = scores<DP>(Ys, vh, vl, col, half);
-    if (xy < Rv) {
-      if (Rv != 1000) {
-        const float down = pow2(xy - Rv);
-#pragma unroll
-        for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) dv[t][i] *= down;
-      }
-      Rv = xy;
-    }
-    if (x < Rk) {
-      if (Rk != 1000) {
-        const float down = pow2(x - Rk);
-#pragma unroll
-        for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) dk[t][i] *= down;
-      }
-      Rk = x;
-    }
-    const int lg = 14 + max(Rv - xy, -60);
-    const float flg = float(lg), by = pow2(Rk - x + E - xv - down_bits<DP>() + 14 - lg);
-    const bool masked = limit_of(a, n0, len) < kw + kRows;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f4 m = *reinterpret_cast<const f4*>(Ms + 8 * q + 4 * half);
-      const f4 d = *reinterpret_cast<const f4*>(Ds + 8 * q + 4 * half);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 4 * q + e;
-        float p = exp2_(s[i] * cs - (m[e] - flg));
-        if (masked && key >= Ls[8 * q + 4 * half + e]) p = 0.f;
-        s[i] = p;
-        dp[i] = p * ((dp[i] - d[e] * vs) * by);
-      }
-    }
-    add_cols<DP>(Ys, s, dv, lane);
-    add_cols<DP>(Qs, dp, dk, lane);
   }
-  if (key >= a.T) return;
-  const bool none = key >= len;  // keys past the length get zeros
-  if (none) {
+  if (key >= a.T || !a.dk) return;
+  if (key >= len)
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t) {
-      zero(dk[t]);
-      zero(dv[t]);
-    }
-  }
-  if (a.dv)
-    write_vec<DP, VEC>(a.dv + k_at(a, b, gh, key), a.D, half, dv, pow2(-14), Rv == 1000 ? 0.f : pow2(-Rv));
-  if (a.dk)
-    write_vec<DP, VEC>(a.dk + k_at(a, b, gh, key), a.D, half, dk,
-                       Rk == 1000 ? 0.f : pow2(down_bits<DP>() - 14 - Rk / 2) * a.scale, pow2(Rk / 2 - Rk));
+    for (int t = 0; t < DP / 32; ++t) zero(acc[t]);
+  write_vec<DP, VEC>(a.dk + k_at(a, b, gh, key), a.D, half, acc,
+                     Rk == 1000 ? 0.f : pow2(down_bits<DP>() - 14 - Rk / 2) * a.scale, pow2(Rk / 2 - Rk));
 }
 
 __global__ void k_attn_no_bad(uint32_t* bad, uint32_t n) {
@@ -734,11 +800,11 @@ struct Backward {
     const uint32_t prob = a.B * a.G;
     if (a.dq) {
       a.tiles = cdiv(a.N, 128);
-      hipLaunchKernelGGL((k_attn_dq_parts<DP, VEC>), dim3(a.tiles * prob), dim3(kT), 0, stream(), a, ps);
+      hipLaunchKernelGGL((k_attn_dq_parts<DP, VEC>), dim3(a.tiles * prob), dim3(kPair), 0, stream(), a, ps);
     }
     if (a.dk || a.dv) {
       a.tiles = cdiv(a.T, 128);
-      hipLaunchKernelGGL((k_attn_dkv_parts<DP, VEC>), dim3(a.tiles * prob), dim3(kT), 0, stream(), a, ps);
+      hipLaunchKernelGGL((k_attn_dkv_parts<DP, VEC>), dim3(a.tiles * prob), dim3(kPair), 0, stream(), a, ps);
     }
     return check_launch("AttentionBackward (parts)");
   }
