@@ -28,6 +28,8 @@
 // key, |dO' V^T - delta'| is at most 2 D 2^(30 - ey - E), which bounds dS's parts.
 #include "dce_attention.h"
 
+#include <type_traits>
+
 namespace dce {
 
 namespace {
@@ -486,6 +488,17 @@ __device__ __forceinline__ void put_p(float* P, int lane, const f16v& s) {
 __device__ __forceinline__ f4 get_p(const float* P, int lane, int q) {
   return *reinterpret_cast<const f4*>(P + (q * 64 + lane) * 4);
 }
+// f(t, stage) for t0 <= t <= t1, the stage (t - t0) % kStages a constant: the
+// places in LDS are then offsets in the instructions (worked out per tile, they
+// were a third of the vector instructions).
+template <class F>
+__device__ __forceinline__ void each_tile(uint32_t t0, uint32_t t1, F&& f) {
+  for (uint32_t t = t0; t <= t1; t += kStages) {
+    f(t, std::integral_constant<int, 0>{});
+    if (t + 1 <= t1) f(t + 1, std::integral_constant<int, 1>{});
+    if (t + 2 <= t1) f(t + 2, std::integral_constant<int, 2>{});
+  }
+}
 template <int N>
 __device__ __forceinline__ void scale_acc(f16v (&acc)[N], float by) {
 #pragma unroll
@@ -524,25 +537,25 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
     TL::load(kp + size_t(t) * kRows * (DP * 4), rk);
     TL::load(vp + size_t(t) * kRows * (DP * 4), rv);
   };
-  auto stage = [&](uint32_t t) {  // tile t from the registers, which then take t + 1
+  auto stage = [&](uint32_t t, auto place) {  // tile t from the registers, which then take t + 1
     if (t >= tiles) return;
-    TL::store(Ks[t % kStages], rk);
-    TL::store(Vs[t % kStages], rv);
+    TL::store(Ks[place], rk);
+    TL::store(Vs[place], rv);
     if (t + 1 < tiles) fetch(t + 1);
   };
   if (tiles) fetch(0);
-  stage(0);
+  stage(0, std::integral_constant<int, 0>{});
   __syncthreads();
   h8 xh[DP / 16], xl[DP / 16];
   if (first) {
     load_vec<DP>(ps.q.p + row * (DP * 4), half, xh, xl);
     const float cq = a.c * pow2(-ps.q.e[et]), m = n < a.N ? a.m[size_t(pr) * a.N + n] : 0.f;
-    for (uint32_t t = 0; t <= tiles; ++t) {
-      stage(t + 1);
+    each_tile(0, tiles, [&](uint32_t t, auto st) {
+      stage(t + 1, std::integral_constant<int, (st + 1) % kStages>{});
       const uint32_t j = t * kRows;
       if (j < mine) {
         const float cs = cq * pow2(-ek[t]);
-        f16v s = scores<DP>(Ks[t % kStages], xh, xl, col, half);
+        f16v s = scores<DP>(Ks[st], xh, xl, col, half);
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = exp2_(s[i] * cs - m);
         if (j + kRows > least) {
@@ -553,7 +566,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
         put_p(Ps[t & 1][blk], lane, s);
       }
       __syncthreads();
-    }
+    });
     return;
   }
   load_vec<DP>(ps.y.p + row * (DP * 4), half, xh, xl);
@@ -564,12 +577,13 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
   for (int t = 0; t < DP / 32; ++t) zero(dq[t]);
   const int E = mine ? ps.least[size_t(pr) * (ps.v.pad / kRows) + (mine - 1) / kRows] : 0;
   int R = 1000;  // dq counts in units of 2^-(R + E + ey - down_bits + 14)
-  for (uint32_t t = 0; t <= tiles; ++t) {
-    stage(t + 1);
+  each_tile(0, tiles, [&](uint32_t t, auto st) {
+    stage(t + 1, std::integral_constant<int, (st + 1) % kStages>{});
     const uint32_t u = t - 1;  // the tile before the first waves'
+    constexpr int su = (st + kStages - 1) % kStages;
     if (t && u * kRows < mine) {
       const int xk = ek[u], xv = ev[u];
-      f16v dp = scores<DP>(Vs[u % kStages], xh, xl, col, half);
+      f16v dp = scores<DP>(Vs[su], xh, xl, col, half);
       if (xk < R) {
         if (R != 1000) scale_acc(dq, pow2(xk - R));
         R = xk;
@@ -581,10 +595,10 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
 #pragma unroll
         for (int e = 0; e < 4; ++e) dp[4 * q + e] = p[e] * ((dp[4 * q + e] - dl) * by);
       }
-      add_cols<DP>(Ks[u % kStages], dp, dq, lane);
+      add_cols<DP>(Ks[su], dp, dq, lane);
     }
     __syncthreads();
-  }
+  });
   if (n >= a.N) return;
   // 2^(down_bits - 14 - R - E - ey), in two factors that stay in range
   const float u = R == 1000 ? 0.f : pow2(down_bits<DP>() - 14 - R - E) * a.scale;
@@ -630,9 +644,8 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
       rd = ps.dl[size_t(pr) * ps.q.pad + i];
     }
   };
-  auto stage = [&](uint32_t t) {  // tile t from the registers, which then take t + 1
+  auto stage = [&](uint32_t t, auto s) {  // tile t from the registers, which then take t + 1
     if (t >= t1) return;
-    const uint32_t s = t % kStages;
     TL::store(Qs[s], rq);
     TL::store(Ys[s], ry);
     if (threadIdx.x < kRows) {
@@ -643,7 +656,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
     if (t + 1 < t1) fetch(t + 1);
   };
   if (t0 < t1) fetch(t0);
-  stage(t0);
+  stage(t0, std::integral_constant<int, 0>{});
   __syncthreads();
   h8 xh[DP / 16], xl[DP / 16];
   f16v acc[DP / 32];
@@ -653,10 +666,9 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   if (first) {
     load_vec<DP>(ps.k.p + row * (DP * 4), half, xh, xl);
     const float ck = a.c * pow2(-ps.k.e[kt]);
-    for (uint32_t t = t0; t <= t1; ++t) {
-      stage(t + 1);
+    each_tile(t0, t1, [&](uint32_t t, auto st) {
+      stage(t + 1, std::integral_constant<int, (st + 1) % kStages>{});
       if (t < t1 && wave_limit(a, t * kRows, kRows, len) > kw) {
-        const uint32_t st = t % kStages;
         const int xy = ey[t];
         const float cs = ck * pow2(-eq[t]);
         f16v s = scores<DP>(Qs[st], xh, xl, col, half);
@@ -680,7 +692,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
         add_cols<DP>(Ys[st], s, acc, lane);
       }
       __syncthreads();
-    }
+    });
     if (key >= a.T || !a.dv) return;
     if (key >= len)  // keys past the length get zeros
 #pragma unroll
@@ -693,12 +705,12 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   const float vs = pow2(xv);
   const int* least = ps.least + size_t(pr) * (ps.v.pad / kRows);
   int Rk = 1000;  // dk counts in units of 2^-(Rk - down_bits + 14)
-  for (uint32_t t = t0; t <= t1; ++t) {
-    stage(t + 1);
+  each_tile(t0, t1, [&](uint32_t t, auto sn) {
+    stage(t + 1, std::integral_constant<int, (sn + 1) % kStages>{});
     const uint32_t u = t - 1;  // the tile before the first waves'
     const uint32_t seen = t > t0 ? wave_limit(a, u * kRows, kRows, len) : 0u;
     if (seen > kw) {
-      const uint32_t st = u % kStages;
+      constexpr int st = (sn + kStages - 1) % kStages;
       const int xy = ey[u], E = least[(seen - 1) / kRows], x = eq[u] + xy + E;
       f16v dp = scores<DP>(Ys[st], xh, xl, col, half);
       Rv = min(Rv, xy);
@@ -718,7 +730,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
       add_cols<DP>(Qs[st], dp, acc, lane);
     }
     __syncthreads();
-  }
+  });
   if (key >= a.T || !a.dk) return;
   if (key >= len)
 #pragma unroll
