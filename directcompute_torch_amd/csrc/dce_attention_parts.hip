@@ -617,7 +617,8 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   __shared__ __attribute__((aligned(16))) float Ps[2][4][1024];
   __shared__ __attribute__((aligned(16))) float Ms[kStages][kRows], Ds[kStages][kRows];
   __shared__ uint32_t Ls[kStages][kRows];
-  const uint32_t prob = a.B * a.G, tile = blockIdx.x / prob, pr = blockIdx.x - tile * prob;
+  const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
+  const uint32_t tile = rest / a.splits, sp = rest - tile * a.splits;
   if (ps.bad[pr]) return;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blk = wave & 3, col = lane & 31, half = lane >> 5;
@@ -629,8 +630,11 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   const int* ey = ps.y.e + size_t(pr) * (ps.q.pad / kRows);
   const char* qp = ps.q.p + size_t(pr) * ps.q.pad * (DP * 4);
   const char* yp = ps.y.p + size_t(pr) * ps.q.pad * (DP * 4);
-  const uint32_t t0 = (k0 < len ? min(first_row(a, k0), a.N) : a.N) / kRows;
-  const uint32_t t1 = k0 < len ? (a.N + kRows - 1) / kRows : t0;
+  // Row tiles from the first that sees key k0 on; the share of this split of them.
+  const uint32_t from = (k0 < len ? min(first_row(a, k0), a.N) : a.N) / kRows;
+  const uint32_t to = k0 < len ? (a.N + kRows - 1) / kRows : from;
+  const uint32_t t0 = from + (to - from) * sp / a.splits, t1 = from + (to - from) * (sp + 1) / a.splits;
+  const size_t part = size_t(sp) * a.B * a.T * a.G * a.D;
   u4v rq[TL::LOADS], ry[TL::LOADS];
   float rm = 0.f, rd = 0.f;
   uint32_t rl = 0;
@@ -697,7 +701,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
     if (key >= len)  // keys past the length get zeros
 #pragma unroll
       for (int t = 0; t < DP / 32; ++t) zero(acc[t]);
-    write_vec<DP, VEC>(a.dv + k_at(a, b, gh, key), a.D, half, acc, pow2(-14), Rv == 1000 ? 0.f : pow2(-Rv));
+    write_vec<DP, VEC>(a.dv + part + k_at(a, b, gh, key), a.D, half, acc, pow2(-14), Rv == 1000 ? 0.f : pow2(-Rv));
     return;
   }
   load_vec<DP>(ps.v.p + row * (DP * 4), half, xh, xl);
@@ -735,10 +739,23 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   if (key >= len)
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) zero(acc[t]);
-  write_vec<DP, VEC>(a.dk + k_at(a, b, gh, key), a.D, half, acc,
+  write_vec<DP, VEC>(a.dk + part + k_at(a, b, gh, key), a.D, half, acc,
                      Rk == 1000 ? 0.f : pow2(down_bits<DP>() - 14 - Rk / 2) * a.scale, pow2(Rk / 2 - Rk));
 }
 
+// dK, dV from the row splits' shares (`values` of each, in a row), added in order.
+__global__ void __launch_bounds__(kT)
+    k_attn_sum(const float* pk, const float* pv, float* dk, float* dv, size_t values, uint32_t splits) {
+  const size_t i = size_t(blockIdx.x) * kT + threadIdx.x;
+  if (i >= values) return;
+  float x = 0.f, y = 0.f;
+  for (uint32_t s = 0; s < splits; ++s) {
+    if (dk) x += pk[s * values + i];
+    if (dv) y += pv[s * values + i];
+  }
+  if (dk) dk[i] = x;
+  if (dv) dv[i] = y;
+}
 __global__ void k_attn_no_bad(uint32_t* bad, uint32_t n) {
   const uint32_t i = blockIdx.x * kT + threadIdx.x;
   if (i < n) bad[i] = 0u;
@@ -804,9 +821,16 @@ struct Forward {
     return check_launch("AttentionForward (parts)");
   }
 };
+// Splits of the rows in the dK / dV kernel: where its 128-key blocks fill less
+// than the CUs, and no less than eight row tiles each.
+uint32_t row_splits(const Attn& a) {
+  const uint32_t wgs = cdiv(a.T, 128) * a.B * a.G, cus = uint32_t(num_cus());
+  return wgs >= cus ? 1u : std::max(1u, std::min(cdiv(cus, wgs), cdiv(a.N, 8 * kRows)));
+}
 struct Backward {
   Attn a;
   Parts ps;
+  float* more;
   template <int DP, bool VEC>
   bool run() {
     const uint32_t prob = a.B * a.G;
@@ -815,8 +839,18 @@ struct Backward {
       hipLaunchKernelGGL((k_attn_dq_parts<DP, VEC>), dim3(a.tiles * prob), dim3(kPair), 0, stream(), a, ps);
     }
     if (a.dk || a.dv) {
-      a.tiles = cdiv(a.T, 128);
-      hipLaunchKernelGGL((k_attn_dkv_parts<DP, VEC>), dim3(a.tiles * prob), dim3(kPair), 0, stream(), a, ps);
+      const size_t values = size_t(a.B) * a.T * a.G * a.D;
+      Attn d = a;
+      d.tiles = cdiv(a.T, 128);
+      d.splits = row_splits(a);
+      if (d.splits > 1) {
+        if (a.dk) d.dk = more;
+        if (a.dv) d.dv = more + d.splits * values;
+      }
+      hipLaunchKernelGGL((k_attn_dkv_parts<DP, VEC>), dim3(d.tiles * d.splits * prob), dim3(kPair), 0, stream(), d, ps);
+      if (d.splits > 1)
+        hipLaunchKernelGGL(k_attn_sum, dim3(cdiv(values, kT)), dim3(kT), 0, stream(), d.dk, d.dv, a.dk, a.dv, values,
+                           d.splits);
     }
     return check_launch("AttentionBackward (parts)");
   }
@@ -864,9 +898,11 @@ bool attn_fwd_parts(const AttnArgs& x, Attn a, bool* took) {
 bool attn_bwd_parts(const AttnArgs& x, Attn a, bool* took) {
   if (!worth(x)) return true;
   *took = true;
-  Prep p{a, {}, true, size_t(a.B) * a.G * a.N, nullptr};
+  const size_t rows = (size_t(a.B) * a.G * a.N + 63) & ~size_t(63);
+  const uint32_t sp = row_splits(a);
+  Prep p{a, {}, true, rows + (sp > 1 ? 2 * sp * size_t(a.B) * a.T * a.G * a.D : 0), nullptr};
   if (!by_dim(a.D, p)) return false;
-  Backward f{a, p.ps};
+  Backward f{a, p.ps, p.more + rows};
   if (!by_dim(a.D, f)) return false;
   a.only = p.ps.bad;
   a.delta = p.more;
