@@ -37,8 +37,8 @@ namespace dce {
 namespace {
 
 constexpr int kT = 256;
-constexpr int kBlk = 128;     // tile of a product
-constexpr int kStep = 32;     // its depth per LDS stage
+constexpr int kStep = 32;     // depth of an LDS stage of the 128 x 128 tiles
+constexpr int kDepth = 128;   // and of the 64 x 64 tiles' only one
 constexpr int kMaxM = 40;     // matrices of a launch
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr int kExpX = 15, kExpA = 14;  // parts hold X 2^15, A 2^14, B 2^14
@@ -99,16 +99,41 @@ __global__ void __launch_bounds__(kT)
   const uint32_t n = M.m * M.n, c0 = (blockIdx.x - t.start[i]) * kChunk;
   float* d = at(ws, M.xt[1]);  // free until the first step
   double sum = 0;
-#pragma unroll 4
-  for (uint32_t k = c0 + threadIdx.x; k < min(n, c0 + kChunk); k += kT) {
-    float g = M.g[k];
+  auto one = [&](float g, float& m) {
     if (g > clip) g = clip;
     if (g < -clip) g = -clip;
-    const float m = mu * M.mom[k] + g;
-    M.mom[k] = m;
+    m = mu * m + g;
     const float v = nesterov ? mu * m + g : m;
-    d[k] = v;
     sum += double(v) * v;
+    return v;
+  };
+  if (c0 + kChunk <= n) {
+    f4 G[4], V[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t k = c0 + (j * kT + threadIdx.x) * 4;
+      G[j] = *reinterpret_cast<const f4*>(M.g + k);
+      V[j] = *reinterpret_cast<const f4*>(M.mom + k);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t k = c0 + (j * kT + threadIdx.x) * 4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float m = V[j][e];
+        G[j][e] = one(G[j][e], m);
+        V[j][e] = m;
+      }
+      *reinterpret_cast<f4*>(M.mom + k) = V[j];
+      *reinterpret_cast<f4*>(d + k) = G[j];
+    }
+  } else {
+#pragma unroll 4
+    for (uint32_t k = c0 + threadIdx.x; k < n; k += kT) {
+      float m = M.mom[k];
+      d[k] = one(M.g[k], m);
+      M.mom[k] = m;
+    }
   }
   sum = block_sum256(sum, sh);
   if (threadIdx.x == 0) sums[blockIdx.x] = sum;
@@ -154,70 +179,65 @@ __global__ void __launch_bounds__(kT) k_muon_scale(const Mats t, float* ws, cons
   const float by = inv[i];
   const float* d = at(ws, M.xt[1]);
   float* x = at(ws, M.x);
-#pragma unroll 4
+  float v[kSq * kSq / kT];
+#pragma unroll
   for (int u = 0; u < kSq * kSq / kT; ++u) {
     const uint32_t s = threadIdx.x + kT * u;
     // consecutive threads along the caller's rows
     const uint32_t r = M.tall ? s % kSq : s / kSq, c = M.tall ? s / kSq : s % kSq, mi = i0 + r, nj = j0 + c;
     const bool ok = mi < M.m && nj < M.n;
-    S[r * kPitch + c] = ok ? d[M.tall ? size_t(nj) * M.m + mi : size_t(mi) * M.n + nj] * by : 0.f;
+    v[u] = ok ? d[M.tall ? size_t(nj) * M.m + mi : size_t(mi) * M.n + nj] * by : 0.f;
+  }
+#pragma unroll
+  for (int u = 0; u < kSq * kSq / kT; ++u) {
+    const uint32_t s = threadIdx.x + kT * u;
+    S[(M.tall ? s % kSq : s / kSq) * kPitch + (M.tall ? s / kSq : s % kSq)] = v[u];
   }
   __syncthreads();
-#pragma unroll 4
-  for (int u = 0; u < kSq * kSq / kT; ++u) {
-    const uint32_t s = threadIdx.x + kT * u, r = s / kSq, c = s % kSq;
-    x[size_t(i0 + r) * M.np + j0 + c] = S[r * kPitch + c];
+#pragma unroll
+  for (int u = 0; u < kSq * kSq / 4 / kT; ++u) {
+    const uint32_t s = threadIdx.x + kT * u, r = s / (kSq / 4), c = s % (kSq / 4) * 4;
+    *reinterpret_cast<f4*>(x + size_t(i0 + r) * M.np + j0 + c) = *reinterpret_cast<const f4*>(S + r * kPitch + c);
   }
   put_tile(S, at(ws, M.xp), M.np, at(ws, M.xt[0]), M.mp, i0, j0);
 }
 
-// w <- w - decay w - step X
-__global__ void __launch_bounds__(kT) k_muon_update(const Mats t, float* ws, float decay) {
-  __shared__ float S[kSq * kPitch];
-  const int i = find_mat(t, blockIdx.x);
-  const Mat& M = t.t[i];
-  const uint32_t tn = M.np / kSq, id = blockIdx.x - t.start[i], i0 = id / tn * kSq, j0 = id % tn * kSq;
-  const float* x = at(ws, M.x);
-#pragma unroll 4
-  for (int u = 0; u < kSq * kSq / kT; ++u) {
-    const uint32_t s = threadIdx.x + kT * u, r = s / kSq, c = s % kSq;
-    S[r * kPitch + c] = x[size_t(i0 + r) * M.np + j0 + c];
-  }
-  __syncthreads();
-#pragma unroll 4
-  for (int u = 0; u < kSq * kSq / kT; ++u) {
-    const uint32_t s = threadIdx.x + kT * u;
-    const uint32_t r = M.tall ? s % kSq : s / kSq, c = M.tall ? s / kSq : s % kSq, mi = i0 + r, nj = j0 + c;
-    if (mi < M.m && nj < M.n) {
-      float* w = M.w + (M.tall ? size_t(nj) * M.m + mi : size_t(mi) * M.n + nj);
-      *w = *w - decay * *w - M.step * S[r * kPitch + c];
-    }
-  }
-}
-
 // ---------------------------------------------------------------------------
-// Products C = P Q^T of parts, both along their rows, in 128 x 128 tiles: four
-// waves of 64 x 64 (2 x 2 blocks of 32 x 32), the depth in steps of 32 through
-// two LDS stages, the next one's direct loads in flight while one is multiplied.
-// A stage row is 128 bytes (4 blocks of 8 h, 8 l); its 16-byte slots are XORed
-// by row / 2 % 8, so that a read of one slot of 16 rows covers the 64 banks once.
+// Products C = P Q^T of parts, both along their rows, in BLK x BLK tiles of four
+// waves.
+//   128: 64 x 64 per wave (2 x 2 blocks of 32 x 32), the depth in steps of 32
+//        through two LDS stages, the next one's direct loads in flight while one
+//        is multiplied; two workgroups per CU.  For launches that fill the chip.
+//   64:  32 x 32 per wave, depths of 128 loaded at once.  A step of the other
+//        kernel takes a load's latency where a CU has one workgroup (about 1 us);
+//        here one latency covers four times the depth, over four times the
+//        workgroups.
+// A stage's rows are 16-byte slots, h and l of 8 values in turn, XORed by the row
+// so that a read of one slot of 16 rows covers the 64 banks once.
 // ---------------------------------------------------------------------------
 enum Op { GRAM, POLY, APPLY, LAST };
-constexpr int kStage = kBlk * kStep * 4;  // bytes of one operand's stage
-constexpr int kCp = 132;                  // pitch of the result tile in LDS
-constexpr int kLds = 4 * kStage > kBlk * kCp * 4 ? 4 * kStage : kBlk * kCp * 4;
-
-__device__ __forceinline__ void stage_load(const BRes& b, uint32_t pitchBytes, uint32_t k, char* S) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+template <int BLK>
+struct Lds {
+  static constexpr int DEPTH = BLK == 128 ? kStep : kDepth, SLOTS = DEPTH / 4;  // slots of a row
+  static constexpr int STAGE = BLK * DEPTH * 4;   // bytes of one operand's stage
+  static constexpr int CP = BLK + 4;              // pitch of the result tile
+  static constexpr int IN = (BLK == 128 ? 4 : 2) * STAGE, OUT = BLK * CP * 4;
+  static constexpr int BYTES = IN > OUT ? IN : OUT;
+  __device__ static __forceinline__ int swz(int row) { return SLOTS == 8 ? (row >> 1) & 7 : row & 15; }
+  // A slot from `end` on is zeros.
+  __device__ static __forceinline__ void load(const BRes& b, uint32_t pitchBytes, uint32_t k, uint32_t end, char* S) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-  for (int i = 0; i < kStage / 16 / kT; ++i) {
-    const uint32_t slot = threadIdx.x + kT * i, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
-    b.ld16_lds(row * pitchBytes + k * 4 + c * 16, S + (wave * 64 + i * kT) * 16);
+    for (int i = 0; i < STAGE / 16 / kT; ++i) {
+      const uint32_t slot = threadIdx.x + kT * i, row = slot / SLOTS, c = (slot % SLOTS) ^ swz(row);
+      const uint32_t off = row * pitchBytes + k * 4 + c * 16;
+      b.ld16_lds(SLOTS == 8 || k + c * 4 < end ? off : kOob * 4u, S + (wave * 64 + i * kT) * 16);
+    }
   }
-}
-__device__ __forceinline__ h8 stage_frag(const char* S, int row, int c) {
-  return *reinterpret_cast<const h8*>(S + row * 128 + ((c ^ ((row >> 1) & 7)) * 16));
-}
+  __device__ static __forceinline__ h8 frag(const char* S, int row, int c) {
+    return *reinterpret_cast<const h8*>(S + (row * SLOTS + (c ^ swz(row))) * 16);
+  }
+};
 // Tile (i, j), i <= j, of the upper triangle in row order.
 __device__ __forceinline__ void triangle(uint32_t id, uint32_t n, uint32_t& i, uint32_t& j) {
   i = 0;
@@ -228,23 +248,24 @@ __device__ __forceinline__ void triangle(uint32_t id, uint32_t n, uint32_t& i, u
   j = i + id;
 }
 
-template <Op OP>
+template <Op OP, int BLK>
 __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2)))
-    k_muon_product(const Mats t, float* ws, uint32_t cur) {
-  __shared__ __attribute__((aligned(16))) char S[kLds];
+    k_muon_product(const Mats t, float* ws, uint32_t cur, float decay) {
+  using L = Lds<BLK>;
+  constexpr int F = BLK / 64;  // blocks of a wave, each way
+  __shared__ __attribute__((aligned(16))) char S[L::BYTES];
   const uint32_t blk = xcd_block_id();
   const int mi = find_mat(t, blk);
   const Mat& M = t.t[mi];
   uint32_t id = blk - t.start[mi], ti, tj, sp = 0;
-  const uint32_t tm = M.mp / kBlk;
-  uint32_t depth = OP == GRAM ? M.np : M.mp, k0 = 0;
+  const uint32_t tm = M.mp / BLK;
+  uint32_t end = OP == GRAM ? M.np : M.mp, k0 = 0;
   if constexpr (OP == GRAM) {
-    const uint32_t tiles = tm * (tm + 1) / 2;
+    const uint32_t tiles = tm * (tm + 1) / 2, steps = (end + L::DEPTH - 1) / L::DEPTH;
     sp = id / tiles;
     id -= sp * tiles;
-    const uint32_t steps = depth / kStep;
-    k0 = uint32_t(uint64_t(steps) * sp / M.splits) * kStep;
-    depth = uint32_t(uint64_t(steps) * (sp + 1) / M.splits) * kStep;
+    k0 = uint32_t(uint64_t(steps) * sp / M.splits) * L::DEPTH;
+    end = min(end, uint32_t(uint64_t(steps) * (sp + 1) / M.splits) * L::DEPTH);
   }
   if constexpr (OP == GRAM || OP == POLY) {
     triangle(id, tm, ti, tj);
@@ -256,90 +277,115 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2)))
   const float* Q = at(ws, OP == GRAM ? M.xp : OP == POLY ? M.a : M.xt[cur]);
   const uint32_t pitch = OP == GRAM ? M.np : M.mp;
   BRes bp, bq;
-  bp.init(P + size_t(ti) * kBlk * pitch, kBlk * pitch);
-  bq.init(Q + size_t(tj) * kBlk * pitch, kBlk * pitch);
+  bp.init(P + size_t(ti) * BLK * pitch, BLK * pitch);
+  bq.init(Q + size_t(tj) * BLK * pitch, BLK * pitch);
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave >> 1) * 32 * F, wn = (wave & 1) * 32 * F;
   const int col = lane & 31, half = lane >> 5;
-  f16v big[2][2], small[2][2];
+  f16v big[F][F], small[F][F];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < F; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < F; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) big[i][j][e] = small[i][j][e] = 0.f;
+  auto mul = [&](const h8 (&p)[F][2], const h8 (&q)[F][2]) {
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+      for (int j = 0; j < F; ++j) {
+        big[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i][0], q[j][0], big[i][j], 0, 0, 0);
+        small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i][0], q[j][1], small[i][j], 0, 0, 0);
+        small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i][1], q[j][0], small[i][j], 0, 0, 0);
+      }
+  };
+  auto frags = [&](const char* St, int w, int kk, h8 (&f)[F][2]) {
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) f[i][e] = L::frag(St, w + 32 * i + col, 2 * (2 * kk + half) + e);
+  };
 
-  stage_load(bp, pitch * 4, k0, S);
-  stage_load(bq, pitch * 4, k0, S + kStage);
+  L::load(bp, pitch * 4, k0, end, S);
+  L::load(bq, pitch * 4, k0, end, S + L::STAGE);
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  int s = 0;
-  for (uint32_t k = k0; k < depth; k += kStep, s ^= 1) {
-    const char* Sp = S + s * 2 * kStage;
-    const char* Sq = Sp + kStage;
-    // Fragments first: a direct load in flight would make the compiler wait
-    // for it before any LDS read.
-    h8 p[2][2][2], q[2][2][2];  // [16-deep step][block][h, l]
+  if constexpr (BLK == 128) {
+    int s = 0;
+    for (uint32_t k = k0; k < end; k += kStep, s ^= 1) {
+      const char* Sp = S + s * 2 * L::STAGE;
+      // Fragments first: a direct load in flight would make the compiler wait
+      // for it before any LDS read.
+      h8 p[2][F][2], q[2][F][2];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+      for (int kk = 0; kk < 2; ++kk) {
+        frags(Sp, wm, kk, p[kk]);
+        frags(Sp + L::STAGE, wn, kk, q[kk]);
+      }
+      if (k + kStep < end) {
+        char* N = S + (s ^ 1) * 2 * L::STAGE;
+        L::load(bp, pitch * 4, k + kStep, end, N);
+        L::load(bq, pitch * 4, k + kStep, end, N + L::STAGE);
+      }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          p[kk][i][e] = stage_frag(Sp, wm + 32 * i + col, 2 * (2 * kk + half) + e);
-          q[kk][i][e] = stage_frag(Sq, wn + 32 * i + col, 2 * (2 * kk + half) + e);
-        }
-    if (k + kStep < depth) {
-      char* N = S + (s ^ 1) * 2 * kStage;
-      stage_load(bp, pitch * 4, k + kStep, N);
-      stage_load(bq, pitch * 4, k + kStep, N + kStage);
+      for (int kk = 0; kk < 2; ++kk) mul(p[kk], q[kk]);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
     }
+  } else {
+    for (uint32_t k = k0;;) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          big[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][0], big[i][j], 0, 0, 0);
-          small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][1], small[i][j], 0, 0, 0);
-          small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][1], q[kk][j][0], small[i][j], 0, 0, 0);
-        }
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
+      for (int kk = 0; kk < kDepth / 16; ++kk) {
+        if (kk == 4 && end - k <= 64) break;  // the depth is a multiple of 64
+        h8 p[F][2], q[F][2];
+        frags(S, wm, kk, p);
+        frags(S + L::STAGE, wn, kk, q);
+        mul(p, q);
+      }
+      __syncthreads();
+      k += kDepth;
+      if (k >= end) break;
+      L::load(bp, pitch * 4, k, end, S);
+      L::load(bq, pitch * 4, k, end, S + L::STAGE);
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    }
   }
   // The tile in LDS, in its own scale.
   float* C = reinterpret_cast<float*>(S);
+  constexpr int CP = L::CP;
   const float unit = OP == GRAM ? ldexpf(1.f, -2 * kExpX) : OP == POLY ? ldexpf(1.f, -2 * kExpA)
                                                                        : ldexpf(1.f, -kExpX - kExpA);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < F; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < F; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        C[(wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3)) * kCp + wn + 32 * j + col] =
+        C[(wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3)) * CP + wn + 32 * j + col] =
             (big[i][j][e] + small[i][j][e]) * unit;
   __syncthreads();
-  const uint32_t i0 = ti * kBlk, j0 = tj * kBlk;
+  const uint32_t i0 = ti * BLK, j0 = tj * BLK;
   if constexpr (OP == GRAM) {
     if (M.splits > 1) {  // summed by k_muon_sum
-      float* out = at(ws, M.part) + (size_t(sp) * (tm * (tm + 1) / 2) + id) * (kBlk * kBlk);
+      float* out = at(ws, M.part) + (size_t(sp) * (tm * (tm + 1) / 2) + id) * (BLK * BLK);
 #pragma unroll 4
-      for (int u = 0; u < kBlk * kBlk / 4 / kT; ++u) {
-        const uint32_t slot = threadIdx.x + kT * u;
-        *reinterpret_cast<f4*>(out + slot * 4) = *reinterpret_cast<const f4*>(C + (slot >> 5) * kCp + (slot & 31) * 4);
+      for (int u = 0; u < BLK * BLK / 4 / kT; ++u) {
+        const uint32_t slot = threadIdx.x + kT * u, r = slot / (BLK / 4), c = slot % (BLK / 4) * 4;
+        *reinterpret_cast<f4*>(out + slot * 4) = *reinterpret_cast<const f4*>(C + r * CP + c);
       }
       return;
     }
   }
+  constexpr int UNROLL = BLK == 128 ? 1 : 2;
   float* out = at(ws, OP == GRAM ? M.a : OP == POLY ? M.b : M.xp);
-#pragma unroll 1
-  for (int u = 0; u < kBlk * kBlk / 8 / kT; ++u) {
-    const uint32_t slot = threadIdx.x + kT * u, r = slot >> 4, k = (slot & 15) * 8;
+#pragma unroll UNROLL
+  for (int u = 0; u < BLK * BLK / 8 / kT; ++u) {
+    const uint32_t slot = threadIdx.x + kT * u, r = slot / (BLK / 8), k = slot % (BLK / 8) * 8;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = C[r * kCp + k + e];
+    for (int e = 0; e < 8; ++e) v[e] = C[r * CP + k + e];
     if constexpr (OP == POLY) {  // B = b A + c A^2
       const h8* a = reinterpret_cast<const h8*>(at(ws, M.a) + size_t(i0 + r) * M.mp + j0 + k);
       const h8 ah = a[0], al = a[1];
@@ -355,49 +401,72 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2)))
         v[e] = x0[e] = kA * x0[e] + v[e];
         v[4 + e] = x1[e] = kA * x1[e] + v[4 + e];
       }
-      reinterpret_cast<f4*>(x)[0] = x0;
-      reinterpret_cast<f4*>(x)[1] = x1;
+      if constexpr (OP == APPLY) {
+        reinterpret_cast<f4*>(x)[0] = x0;
+        reinterpret_cast<f4*>(x)[1] = x1;
+      }
     }
     if constexpr (OP != LAST)
       put8(out + size_t(i0 + r) * (OP == APPLY ? M.np : M.mp), j0 + k, v, ldexpf(1.f, OP == APPLY ? kExpX : kExpA));
-    if constexpr (OP == POLY || OP == APPLY) {  // for the transposed copy
+    if constexpr (OP != GRAM) {  // for the pass over columns
 #pragma unroll
-      for (int e = 0; e < 8; ++e) C[r * kCp + k + e] = v[e];
+      for (int e = 0; e < 8; ++e) C[r * CP + k + e] = v[e];
     }
   }
-  if constexpr (OP == LAST) return;
   if ((OP == GRAM || OP == POLY) && ti == tj) return;
   __syncthreads();
-  float* tr = OP == APPLY ? at(ws, M.xt[cur ^ 1]) : out;
+  if constexpr (OP == LAST) {  // w <- w - decay w - step X, along the caller's rows
+    constexpr int W = 8;
 #pragma unroll 1
-  for (int u = 0; u < kBlk * kBlk / 8 / kT; ++u) {
-    const uint32_t slot = threadIdx.x + kT * u, r = slot & 127, k = (slot >> 7) * 8;
+    for (int u = 0; u < BLK * BLK / kT; u += W) {
+      float w[W];
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const uint32_t s = threadIdx.x + kT * (u + e), r = M.tall ? s % BLK : s / BLK, c = M.tall ? s / BLK : s % BLK;
+        const size_t i = M.tall ? size_t(j0 + c) * M.m + i0 + r : size_t(i0 + r) * M.n + j0 + c;
+        w[e] = i0 + r < M.m && j0 + c < M.n ? M.w[i] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const uint32_t s = threadIdx.x + kT * (u + e), r = M.tall ? s % BLK : s / BLK, c = M.tall ? s / BLK : s % BLK;
+        const size_t i = M.tall ? size_t(j0 + c) * M.m + i0 + r : size_t(i0 + r) * M.n + j0 + c;
+        if (i0 + r < M.m && j0 + c < M.n) M.w[i] = w[e] - decay * w[e] - M.step * C[r * CP + c];
+      }
+    }
+    return;
+  }
+  float* tr = OP == APPLY ? at(ws, M.xt[cur ^ 1]) : out;
+#pragma unroll UNROLL
+  for (int u = 0; u < BLK * BLK / 8 / kT; ++u) {
+    const uint32_t slot = threadIdx.x + kT * u, r = slot % BLK, k = slot / BLK * 8;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = C[(k + e) * kCp + r];
+    for (int e = 0; e < 8; ++e) v[e] = C[(k + e) * CP + r];
     put8(tr + size_t(j0 + r) * M.mp, i0 + k, v, ldexpf(1.f, OP == APPLY ? kExpX : kExpA));
   }
 }
 
-// A from the partial tiles of a split Gram product: a workgroup per 32 x 128
-// piece of a tile, eight values a thread at a time.
+// A from the partial tiles of a split Gram product: a workgroup per 16 rows of a
+// tile.
+template <int BLK>
 __global__ void __launch_bounds__(kT) k_muon_sum(const Mats t, float* ws) {
-  __shared__ float C[32 * kCp];
+  constexpr int RW = 16, CP = BLK + 4, PIECES = BLK / RW;
+  __shared__ float C[RW * CP];
   const int mi = find_mat(t, blockIdx.x);
   const Mat& M = t.t[mi];
-  const uint32_t id = blockIdx.x - t.start[mi], piece = id & 3, tile = id >> 2, tm = M.mp / kBlk;
+  const uint32_t id = blockIdx.x - t.start[mi], piece = id % PIECES, tile = id / PIECES, tm = M.mp / BLK;
   const uint32_t tiles = tm * (tm + 1) / 2;
   uint32_t ti, tj;
   triangle(tile, tm, ti, tj);
-  const float* part = at(ws, M.part) + size_t(tile) * (kBlk * kBlk) + piece * 32 * kBlk;
+  const float* part = at(ws, M.part) + size_t(tile) * (BLK * BLK) + piece * RW * BLK;
   float* a = at(ws, M.a);
-  const uint32_t i0 = ti * kBlk + piece * 32, j0 = tj * kBlk;
-#pragma unroll
-  for (int u = 0; u < 32 * kBlk / 8 / kT; ++u) {
-    const uint32_t slot = threadIdx.x + kT * u, r = slot >> 4, k = (slot & 15) * 8;
+  const uint32_t i0 = ti * BLK + piece * RW, j0 = tj * BLK;
+  const uint32_t r = threadIdx.x / (BLK / 8), k = threadIdx.x % (BLK / 8) * 8;
+  if (r < RW) {
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (uint32_t s = 0; s < M.splits; ++s) {
-      const f4* p = reinterpret_cast<const f4*>(part + size_t(s) * tiles * (kBlk * kBlk) + slot * 8);
+      const f4* p = reinterpret_cast<const f4*>(part + size_t(s) * tiles * (BLK * BLK) + threadIdx.x * 8);
       const f4 p0 = p[0], p1 = p[1];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -407,22 +476,21 @@ __global__ void __launch_bounds__(kT) k_muon_sum(const Mats t, float* ws) {
     }
     put8(a + size_t(i0 + r) * M.mp, j0 + k, v, ldexpf(1.f, kExpA));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) C[r * kCp + k + e] = v[e];
+    for (int e = 0; e < 8; ++e) C[r * CP + k + e] = v[e];
   }
   if (ti == tj) return;
   __syncthreads();
-#pragma unroll
-  for (int u = 0; u < 32 * kBlk / 8 / kT; ++u) {
-    const uint32_t slot = threadIdx.x + kT * u, r = slot & 127, k = (slot >> 7) * 8;
+  const uint32_t c = threadIdx.x % BLK, q = threadIdx.x / BLK * 8;
+  if (q < RW) {
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = C[(k + e) * kCp + r];
-    put8(a + size_t(j0 + r) * M.mp, i0 + k, v, ldexpf(1.f, kExpA));
+    for (int e = 0; e < 8; ++e) v[e] = C[(q + e) * CP + c];
+    put8(a + size_t(j0 + c) * M.mp, i0 + q, v, ldexpf(1.f, kExpA));
   }
 }
 
 inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b); }
-inline uint32_t pad(uint32_t v) { return (v + kBlk - 1) / kBlk * kBlk; }
+inline uint32_t pad(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
 
 // start[] for `f(matrix)` workgroups each; returns their number.
 template <class F>
@@ -445,19 +513,25 @@ struct Places {
   }
 };
 
+template <int BLK>
 bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32_t steps) {
-  // A Gram product is split so that no workgroup has more than 1 / (2 CUs) of
-  // the launch's steps, and none fewer than 8.
-  auto tri = [](const Mat& m) { return m.mp / kBlk * (m.mp / kBlk + 1) / 2; };
+  constexpr uint32_t depth = Lds<BLK>::DEPTH;
+  // A Gram product is split so that no workgroup has more than its share of the
+  // launch's depth, and none less than 256.
+  auto tri = [](const Mat& m) { return m.mp / BLK * (m.mp / BLK + 1) / 2; };
   double all = 0;
-  for (uint32_t i = 0; i < t.count; ++i) all += double(tri(t.t[i])) * (t.t[i].np / kStep);
-  const double most = std::max(8.0, std::ceil(all / (2.0 * num_cus())));
+  for (uint32_t i = 0; i < t.count; ++i) {
+    t.t[i].mp = pad(t.t[i].m, BLK);
+    t.t[i].np = pad(t.t[i].n, BLK);
+    all += double(tri(t.t[i])) * t.t[i].np;
+  }
+  const double most = std::max(256.0, all / (2.0 * num_cus()));
   Places at;
   size_t chunks = 0;
   bool split = false;
   for (uint32_t i = 0; i < t.count; ++i) {
     Mat& m = t.t[i];
-    m.splits = std::max<uint32_t>(1, uint32_t(std::ceil((m.np / kStep) / most)));
+    m.splits = std::min<uint32_t>(cdiv(m.np, depth), std::max<uint32_t>(1, uint32_t(std::ceil(m.np / most))));
     split |= m.splits > 1;
     const size_t xn = size_t(m.mp) * m.np, an = size_t(m.mp) * m.mp;
     m.x = at.take(xn);
@@ -466,7 +540,7 @@ bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32
     m.xt[1] = at.take(xn);
     m.a = at.take(an);
     m.b = at.take(an);
-    m.part = m.splits > 1 ? at.take(size_t(m.splits) * tri(m) * kBlk * kBlk) : 0;
+    m.part = m.splits > 1 ? at.take(size_t(m.splits) * tri(m) * BLK * BLK) : 0;
     chunks += cdiv(size_t(m.m) * m.n, kChunk);
   }
   const size_t sums = at.take(2 * chunks), inv = at.take(kMaxM);
@@ -478,26 +552,23 @@ bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32
   uint32_t n = blocks(t, [](const Mat& m) { return cdiv(size_t(m.m) * m.n, kChunk); });
   hipLaunchKernelGGL(k_muon_momentum, dim3(n), dim3(kT), 0, stream(), t, ws, dsum, mu, clip, int(nesterov));
   hipLaunchKernelGGL(k_muon_norm, dim3(t.count), dim3(kT), 0, stream(), t, dsum, dinv);
-  auto squares = [](const Mat& m) { return m.mp / kSq * (m.np / kSq); };
-  n = blocks(t, squares);
+  n = blocks(t, [](const Mat& m) { return m.mp / kSq * (m.np / kSq); });
   hipLaunchKernelGGL(k_muon_scale, dim3(n), dim3(kT), 0, stream(), t, ws, dinv);
   for (uint32_t s = 0; s < steps; ++s) {
     n = blocks(t, [&](const Mat& m) { return tri(m) * m.splits; });
-    hipLaunchKernelGGL(k_muon_product<GRAM>, dim3(n), dim3(kT), 0, stream(), t, ws, s & 1);
+    hipLaunchKernelGGL((k_muon_product<GRAM, BLK>), dim3(n), dim3(kT), 0, stream(), t, ws, s & 1, decay);
     if (split) {
-      n = blocks(t, [&](const Mat& m) { return m.splits > 1 ? tri(m) * 4 : 0; });
-      hipLaunchKernelGGL(k_muon_sum, dim3(n), dim3(kT), 0, stream(), t, ws);
+      n = blocks(t, [&](const Mat& m) { return m.splits > 1 ? tri(m) * (BLK / 16) : 0; });
+      hipLaunchKernelGGL(k_muon_sum<BLK>, dim3(n), dim3(kT), 0, stream(), t, ws);
     }
     n = blocks(t, tri);
-    hipLaunchKernelGGL(k_muon_product<POLY>, dim3(n), dim3(kT), 0, stream(), t, ws, s & 1);
-    n = blocks(t, [](const Mat& m) { return m.mp / kBlk * (m.np / kBlk); });
+    hipLaunchKernelGGL((k_muon_product<POLY, BLK>), dim3(n), dim3(kT), 0, stream(), t, ws, s & 1, decay);
+    n = blocks(t, [](const Mat& m) { return m.mp / BLK * (m.np / BLK); });
     if (s + 1 < steps)
-      hipLaunchKernelGGL(k_muon_product<APPLY>, dim3(n), dim3(kT), 0, stream(), t, ws, s & 1);
+      hipLaunchKernelGGL((k_muon_product<APPLY, BLK>), dim3(n), dim3(kT), 0, stream(), t, ws, s & 1, decay);
     else
-      hipLaunchKernelGGL(k_muon_product<LAST>, dim3(n), dim3(kT), 0, stream(), t, ws, s & 1);
+      hipLaunchKernelGGL((k_muon_product<LAST, BLK>), dim3(n), dim3(kT), 0, stream(), t, ws, s & 1, decay);
   }
-  n = blocks(t, squares);
-  hipLaunchKernelGGL(k_muon_update, dim3(n), dim3(kT), 0, stream(), t, ws, decay);
   return check_launch("MuonBatch");
 }
 
@@ -526,11 +597,9 @@ bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* row
     m.tall = rows[i] > cols[i];
     m.m = std::min(rows[i], cols[i]);
     m.n = std::max(rows[i], cols[i]);
-    m.mp = pad(m.m);
-    m.np = pad(m.n);
     m.step = stepSizes[i];
     // a tile's operand rows are reached with 32-bit offsets
-    if (uint64_t(m.np) * kBlk >= kOob) {
+    if (uint64_t(m.n) * 128 + (1u << 14) >= kOob) {
       set_error("MuonBatch: matrix %u has %u columns: too many", i, m.n);
       return false;
     }
@@ -544,12 +613,15 @@ bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* row
   for (size_t i = 0; i < all.size();) {
     Mats t{};
     size_t values = 0;
+    uint64_t tiles = 0;
     while (i < all.size() && t.count < uint32_t(kMaxM) &&
-           (!t.count || values + size_t(all[i].mp) * all[i].np <= (size_t(1) << 28))) {
-      values += size_t(all[i].mp) * all[i].np;
+           (!t.count || values + size_t(all[i].m) * all[i].n <= (size_t(1) << 28))) {
+      values += size_t(all[i].m) * all[i].n;
+      tiles += uint64_t(cdiv(all[i].m, 128)) * cdiv(all[i].n, 128);
       t.t[t.count++] = all[i++];
     }
-    if (!run_group(t, mu, nesterov, decay, clip, steps)) return false;
+    const bool big = tiles > uint64_t(num_cus());
+    if (!(big ? run_group<128> : run_group<64>)(t, mu, nesterov, decay, clip, steps)) return false;
   }
   return true;
 }
