@@ -269,31 +269,31 @@ __global__ void __launch_bounds__(kT) k_attn_fwd(const Attn a) {
   }
 }
 
-// Joins the key splits: one thread per value of O.
-__global__ void __launch_bounds__(kT) k_attn_join(const Attn a, size_t values) {
-  const size_t v = size_t(blockIdx.x) * kT + threadIdx.x;
-  if (v >= values) return;
-  const size_t row = v / a.D;
-  const uint32_t d = uint32_t(v - row * a.D);
-  const size_t rows = size_t(a.B) * a.G * a.N;
-  const uint32_t pr = uint32_t(row / a.N), n = uint32_t(row - size_t(pr) * a.N);
-  const uint32_t b = fdiv(pr, a.dG), g = pr - b * a.G;
-  float m = -INFINITY;
-  for (uint32_t s = 0; s < a.splits; ++s) m = fmaxf(m, a.pm[s * rows + row]);
+// Joins the key splits: a workgroup per row, a thread per value (or several).
+__global__ void __launch_bounds__(kT) k_attn_join(const Attn a) {
+  const uint32_t row = blockIdx.x, rows = a.B * a.G * a.N;
+  const uint32_t pr = row / a.N, n = row - pr * a.N, b = fdiv(pr, a.dG), g = pr - b * a.G;
   const bool none = limit_of(a, n, keys_of(a, b)) == 0;
+  float m = -INFINITY;
+#pragma unroll 8
+  for (uint32_t s = 0; s < a.splits; ++s) m = fmaxf(m, a.pm[size_t(s) * rows + row]);
   const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o = 0.f;
-  for (uint32_t s = 0; s < a.splits; ++s) {
-    const float w = exp2_(a.pm[s * rows + row] - base);
-    l += w * a.pl[s * rows + row];
-    o += w * a.po[(s * rows + row) * a.D + d];
+  for (uint32_t d = threadIdx.x; d < a.D; d += blockDim.x) {
+    float l = 0.f, o = 0.f;
+#pragma unroll 8
+    for (uint32_t s = 0; s < a.splits; ++s) {
+      const size_t i = size_t(s) * rows + row;
+      const float w = exp2_(a.pm[i] - base);
+      l += w * a.pl[i];
+      o += w * a.po[i * a.D + d];
+    }
+    const float il = none ? 0.f : 1.f / l;
+    if (a.m && d == 0) {
+      a.m[row] = none ? 0.f : m;
+      a.il[row] = il;
+    }
+    a.o[q_at(a, b, g, n) + d] = none ? 0.f : o * il;
   }
-  const float il = none ? 0.f : 1.f / l;
-  if (a.m && d == 0) {
-    a.m[row] = none ? 0.f : m;
-    a.il[row] = il;
-  }
-  a.o[q_at(a, b, g, n) + d] = none ? 0.f : o * il;
 }
 
 // ---------------------------------------------------------------------------
@@ -564,7 +564,7 @@ struct FwdRun {
     a.tiles = cdiv(a.N, wide ? 128 : 64);
     const uint32_t kt = cdiv(a.T, kKeys);
     a.splits = 1;
-    if (!a.only && uint64_t(a.tiles) * prob < 2 * cus) {
+    if (!a.only && uint64_t(a.tiles) * prob < cus) {
       a.splits = std::min(cdiv(kt, 4), cdiv(4 * cus, a.tiles * prob));
       if (a.splits < 1) a.splits = 1;
     }
@@ -595,8 +595,12 @@ struct BwdRun {
   bool run() {
     constexpr int QT = DP <= 64 ? 2 : 1;
     const uint32_t prob = a.B * a.G;
-    a.tiles = cdiv(a.N, 64 * QT);
-    hipLaunchKernelGGL((k_attn_dq<DP, QT, VEC>), dim3(a.tiles * prob), dim3(kT), 0, stream(), a);
+    const bool wide = QT == 2 && uint64_t(cdiv(a.N, 128)) * prob >= 2 * uint32_t(num_cus());
+    a.tiles = cdiv(a.N, wide ? 128 : 64);
+    if (wide)
+      hipLaunchKernelGGL((k_attn_dq<DP, QT, VEC>), dim3(a.tiles * prob), dim3(kT), 0, stream(), a);
+    else
+      hipLaunchKernelGGL((k_attn_dq<DP, 1, VEC>), dim3(a.tiles * prob), dim3(kT), 0, stream(), a);
     if (!check_launch("AttentionBackward (dQ)")) return false;
     if (!a.dk && !a.dv) return true;
     a.tiles = cdiv(a.T, 64);
@@ -608,8 +612,7 @@ struct BwdRun {
 }  // namespace
 
 bool attn_join(const Attn& a) {
-  const size_t values = size_t(a.B) * a.G * a.N * a.D;
-  hipLaunchKernelGGL(k_attn_join, dim3(cdiv(values, kT)), dim3(kT), 0, stream(), a, values);
+  hipLaunchKernelGGL(k_attn_join, dim3(a.B * a.G * a.N), dim3(std::min(kT, int(a.D + 63) / 64 * 64)), 0, stream(), a);
   return check_launch("AttentionForward (join)");
 }
 bool attn_fwd_fp32(Attn a) { return by_dim(a.D, a.D % 4 == 0, FwdRun{a}); }
