@@ -28,6 +28,7 @@ namespace {
 
 constexpr int kT = 256;   // threads: four waves
 constexpr int kKeys = 32; // keys (rows in the dK / dV kernel) of an LDS tile
+constexpr int kFew = 64;  // and in the kernel for few rows
 
 __device__ __forceinline__ f4 mfma4(float a, float b, const f4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
@@ -266,6 +267,139 @@ __global__ void __launch_bounds__(kT) k_attn_fwd(const Attn a) {
       a.il[size_t(pr) * a.N + n] = il;
     }
     CL::template write<VEC>(a.o + q_at(a, b, gh, n), a.D, g, o[t], il);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Forward of up to 16 rows (a new token or a few, all heads of a key head): bound
+// by reading K and V once.  Tiles of 64 keys, 16 to each wave, which keeps sums of
+// its own; the four waves' are joined at the end.  In the general kernel one wave
+// would multiply for all four: 8 sequences of up to 8191 keys, 8 key heads of 128,
+// took 114 us there and take 87 here, at the rate of a large copy.  Operands straight from memory, without LDS, took 155 us: the K
+// fragment's 64 bytes of each of 16 rows keep the address unit busy.
+// ---------------------------------------------------------------------------
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(kT, 2) k_attn_few(const Attn a) {
+  using CL = Cols<DP>;
+  using TL = Tile<DP, kFew, VEC>;
+  constexpr int EG = CL::EG, NG = CL::NG, NI = DP / 16;
+  __shared__ __attribute__((aligned(16))) float Tiles[2][kFew * DP];
+  float* Ks = Tiles[0];
+  float* Vs = Tiles[1];
+  float (*Os)[16][DP + 4] = reinterpret_cast<float (*)[16][DP + 4]>(Ks);  // after the last tile
+  static_assert(4 * 16 * (DP + 4) <= 2 * kFew * DP, "the sums fit the tiles");
+  __shared__ float Ms[4][16], Ss[4][16];
+  const uint32_t prob = a.B * a.G, sp = blockIdx.x / prob, pr = blockIdx.x - sp * prob;
+  const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t n = col, len = keys_of(a, b), lim = n < a.N ? limit_of(a, n, len) : 0u;
+  const uint32_t least = limit_of(a, 0, len), most = limit_of(a, a.N - 1, len);
+  f4 q[NI];
+  load_frag<DP, VEC>(a.q + (n < a.N ? q_at(a, b, gh, n) : 0), n < a.N, a.D, g, q);
+  f4 o[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  const uint32_t stride = a.G * a.D, j0 = sp * a.perSplit * kFew, j1 = min(most, (sp + 1) * a.perSplit * kFew);
+  f4 rk[TL::LOADS], rv[TL::LOADS];
+  auto fetch = [&](uint32_t j) {
+    const uint32_t n = min(len - j, uint32_t(kFew));
+    TL::load(rows_view(a.k + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rk);
+    TL::load(rows_view(a.v + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rv);
+  };
+  if (j0 < j1) fetch(j0);
+  for (uint32_t j = j0; j < j1; j += kFew) {
+    __syncthreads();
+    TL::store(Ks, rk);
+    TL::store(Vs, rv);
+    __syncthreads();
+    if (j + kFew < j1) fetch(j + kFew);
+    const uint32_t jw = j + wave * 16;
+    if (jw >= most) continue;
+    f4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const f4 kf = TL::chunk(Ks, wave * 16 + col, 4 * i + g);
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        s0 = mfma4(kf[e], q[i][e], s0);
+        s1 = mfma4(kf[e + 1], q[i][e + 1], s1);
+      }
+    }
+    f4 s;
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[r] = (s0[r] + s1[r]) * a.c;
+      if (jw + 16 > least && jw + 4 * g + r >= lim) s[r] = -INFINITY;
+      top = fmaxf(top, s[r]);
+    }
+    top = fmaxf(m, max_g(top));
+    const float base = top == -INFINITY ? 0.f : top;
+    if (__any(top > m)) {
+      const float down = exp2_(m - base);
+      l *= down;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[i][r] *= down;
+      m = top;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[r] = exp2_(s[r] - base);
+      l += s[r];
+#pragma unroll
+      for (int p = 0; p < NG; ++p) {
+        const typename CL::V vf = CL::read(Vs, wave * 16 + 4 * g + r, p, col);
+#pragma unroll
+        for (int e = 0; e < EG; ++e) o[p * EG + e] = mfma4(vf[e], s[r], o[p * EG + e]);
+      }
+    }
+  }
+  __syncthreads();
+  l = sum_g(l);
+  if (g == 0) {
+    Ms[wave][col] = m;
+    Ss[wave][col] = l;
+  }
+#pragma unroll
+  for (int p = 0; p < NG; ++p)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < EG; ++e) Os[wave][col][16 * EG * p + EG * (4 * g + r) + e] = o[p * EG + e][r];
+  __syncthreads();
+  const bool one = a.splits == 1;
+  for (uint32_t i = threadIdx.x; i < a.N * DP; i += kT) {
+    const uint32_t row = i / DP, d = i % DP;
+    float top = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, Ms[w][row]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float by = exp2_(Ms[w][row] - base);
+      sum += by * Ss[w][row];
+      v += by * Os[w][row][d];
+    }
+    const size_t at = size_t(pr) * a.N + row, part = size_t(sp) * prob * a.N + at;
+    const bool none = limit_of(a, row, len) == 0;
+    const float il = none ? 0.f : 1.f / sum;
+    if (d == 0 && !one) {
+      a.pm[part] = top;
+      a.pl[part] = sum;
+    }
+    if (d == 0 && one && a.m) {
+      a.m[at] = none ? 0.f : top;
+      a.il[at] = il;
+    }
+    if (d >= a.D) continue;
+    if (one)
+      a.o[q_at(a, b, gh, row) + d] = none ? 0.f : v * il;
+    else
+      a.po[part * a.D + d] = v;
   }
 }
 
@@ -560,11 +694,14 @@ struct FwdRun {
   bool run() {
     constexpr int QT = DP <= 128 ? 2 : 1;
     const uint32_t cus = uint32_t(num_cus()), prob = a.B * a.G;
+    const bool few = a.N <= 16 && !a.only;
     const bool wide = QT == 2 && uint64_t(cdiv(a.N, 128)) * prob >= 2 * cus;
     a.tiles = cdiv(a.N, wide ? 128 : 64);
-    const uint32_t kt = cdiv(a.T, kKeys);
+    const uint32_t kt = cdiv(a.T, few ? kFew : kKeys);
     a.splits = 1;
-    if (!a.only && uint64_t(a.tiles) * prob < cus) {
+    if (few)
+      a.splits = std::max(1u, std::min(cdiv(kt, 4), 4 * cus / prob));
+    else if (!a.only && uint64_t(a.tiles) * prob < cus) {
       a.splits = std::min(cdiv(kt, 4), cdiv(4 * cus, a.tiles * prob));
       if (a.splits < 1) a.splits = 1;
     }
@@ -580,7 +717,9 @@ struct FwdRun {
       a.po = ws + 2 * stat;
     }
     const dim3 grid(a.tiles * a.splits * prob);
-    if (wide)
+    if (few)
+      hipLaunchKernelGGL((k_attn_few<DP, VEC>), grid, dim3(kT), 0, stream(), a);
+    else if (wide)
       hipLaunchKernelGGL((k_attn_fwd<DP, QT, VEC>), grid, dim3(kT), 0, stream(), a);
     else
       hipLaunchKernelGGL((k_attn_fwd<DP, 1, VEC>), grid, dim3(kT), 0, stream(), a);
