@@ -24,9 +24,8 @@ struct Attn {
   float *pm, *pl, *po;           // partials of the key splits
   const float* dy;               // backward
   float *delta, *dq, *dk, *dv;
-  const uint32_t* only;          // problems to run (non-zero); null: all
   uint32_t B, S, T, G, D, rep, N;
-  uint32_t tiles, splits, perSplit;  // key tiles of a split
+  uint32_t tiles, splits, perSplit;  // splits: of the keys (perSplit tiles each), or of the rows in dK, dV
   FastDiv dRep, dG;
   float c, scale;
   int causal;
@@ -54,6 +53,13 @@ __device__ __forceinline__ uint32_t first_row(const Attn& a, uint32_t k0) {
   const int64_t i = int64_t(k0) - (int64_t(a.T) - int64_t(a.S));
   return a.causal && i > 0 ? uint32_t(i) * a.rep : 0u;
 }
+// Rows [first, end) of split sp of those that see key k0 on, in whole 32-row tiles.
+__device__ __forceinline__ void split_rows(const Attn& a, uint32_t k0, uint32_t len, uint32_t sp, uint32_t& first,
+                                           uint32_t& end) {
+  const uint32_t from = k0 < len ? min(first_row(a, k0), a.N) / 32 : 0u, to = k0 < len ? (a.N + 31) / 32 : 0u;
+  first = (from + (to - from) * sp / a.splits) * 32;
+  end = min((from + (to - from) * (sp + 1) / a.splits) * 32, a.N);
+}
 // First value of row n's vector in a [batch][seq][heads][dim] tensor.
 __device__ __forceinline__ size_t q_at(const Attn& a, uint32_t b, uint32_t g, uint32_t n) {
   const uint32_t i = fdiv(n, a.dRep), h = g * a.rep + (n - i * a.rep);
@@ -72,11 +78,17 @@ inline double pairs_of(const AttnArgs& x) {
   return rows * last - rows * (rows - 1) / 2;
 }
 
+// Splits of the rows in a dK / dV kernel of `keys` keys per workgroup: where those
+// fill less than the CUs, and no less than eight row tiles each.
+inline uint32_t row_splits(const Attn& a, uint32_t keys) {
+  const uint32_t wgs = cdiv(a.T, keys) * a.B * a.G, cus = uint32_t(num_cus());
+  return wgs >= cus ? 1u : std::max(1u, std::min(cdiv(cus, wgs), cdiv(a.N, 8 * 32)));
+}
+
 // Joins the key splits of a forward into o (and the statistics).
 bool attn_join(const Attn& a);
-// The forward / backward on fp32 MFMAs with a's operands (a.only, a.delta as set).
-bool attn_fwd_fp32(Attn a);
-bool attn_bwd_fp32(Attn a);
+// Adds the row splits' dk, dv (`from`) into `to`'s.
+bool attn_sum(const Attn& from, const Attn& to);
 // On fp16 parts, where they are faster; `took` tells.
 bool attn_fwd_parts(const AttnArgs& x, Attn a, bool* took);
 bool attn_bwd_parts(const AttnArgs& x, Attn a, bool* took);

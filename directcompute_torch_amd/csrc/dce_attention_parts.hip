@@ -7,10 +7,9 @@
 // exponent e is one for each tile of 32 vectors, chosen so that the tile's
 // largest value lies in [2^14, 2^15): l's half step is then 2^-25, so a vector
 // whose own largest value is within 2^14 of the tile's keeps at least 24 bits of
-// it.  A (sequence, key head) with a tile that has smaller vectors than that
-// (zeros aside), values outside of 2^+-30 (gradients: 2^+-60) or any that is not finite is left
-// to the fp32 kernels: the pass that splits marks it, both sets of kernels are
-// launched, and the workgroups of the one that is not meant return at once.
+// it.  A tile that has smaller vectors than that (zeros aside), values outside of
+// 2^+-30 (gradients: 2^+-60) or any that is not finite is marked by the pass that
+// splits, and the workgroups of its (sequence, key head) run the fp32 code.
 //
 // Everything that the scores do not need is a factor of a whole tile, so the
 // exponents cost next to nothing: c 2^-(eq + ek) is the factor that turns a
@@ -26,7 +25,7 @@
 // delta' is of the size of the largest vector that a row sees, whatever tile it
 // is compared in: with E the least exponent of V's tiles up to the row's last
 // key, |dO' V^T - delta'| is at most 2 D 2^(30 - ey - E), which bounds dS's parts.
-#include "dce_attention.h"
+#include "dce_attention_fp32.h"
 
 #include <type_traits>
 
@@ -63,15 +62,31 @@ __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + max(
 // D and past the last vector up to whole tiles; one exponent per tile.
 struct Part {
   char* p;
-  int* e;
+  int* e;        // kBad: not made
   uint32_t pad;  // vectors of a problem, a multiple of 128
 };
 struct Parts {
   Part q, k, v, y;
-  float* dl;      // delta' 2^e of dO's tile, [problem][q.pad]
-  int* least;     // least exponent of V's tiles up to each, [problem][v.pad / kRows]
-  uint32_t* bad;  // problems left to the fp32 kernels
+  float* dl;  // delta' 2^e of dO's tile, [problem][q.pad]
 };
+constexpr int kBad = 1 << 20;
+// Has problem pr a tile that parts do not suit?  For all threads of the workgroup.
+template <bool BWD>
+__device__ __forceinline__ bool unsuited(const Parts& ps, uint32_t pr) {
+  const uint32_t nq = ps.q.pad / kRows, nk = ps.k.pad / kRows;
+  bool bad = false;
+  for (uint32_t t = threadIdx.x; t < max(nq, nk); t += blockDim.x) {
+    if (t < nq) bad |= ps.q.e[size_t(pr) * nq + t] == kBad || (BWD && ps.y.e[size_t(pr) * nq + t] == kBad);
+    if (t < nk) bad |= ps.k.e[size_t(pr) * nk + t] == kBad || ps.v.e[size_t(pr) * nk + t] == kBad;
+  }
+  return __syncthreads_or(bad);
+}
+// The least exponent of V's tiles [from, to), in every lane.
+__device__ __forceinline__ int least_of(const int* ev, uint32_t from, uint32_t to, int lane) {
+  float m = 1000.f;
+  for (uint32_t t = from + lane; t < to; t += 64) m = fminf(m, float(ev[t]));
+  return -int(wave_reduce(-m, OpMaxR()));
+}
 
 // ---------------------------------------------------------------------------
 // The pass that splits: a workgroup per tile.
@@ -83,7 +98,7 @@ __device__ __forceinline__ void split_tile(const Attn& a, const Part& P, const P
   constexpr bool ROWS = W == QUERY || W == GRAD;
   __shared__ uint32_t top[kRows];
   __shared__ float dots[kRows];
-  __shared__ int all[3];
+  __shared__ int all[1];
   const uint32_t b = fdiv(pr, a.dG), g = pr - b * a.G;
   const uint32_t n0 = tile * kRows, have = ROWS ? a.N : keys_of(a, b);
   if (threadIdx.x < kRows) {
@@ -113,7 +128,7 @@ __device__ __forceinline__ void split_tile(const Attn& a, const Part& P, const P
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             v[i][4 * hf + e] = x[e] * by;
-            if (W == GRAD) part[i] += v[i][4 * hf + e] * o[e];
+            if (W == GRAD) part[i] += x[e] * o[e];
           }
         }
     } else {
@@ -121,7 +136,7 @@ __device__ __forceinline__ void split_tile(const Attn& a, const Part& P, const P
       for (int e = 0; e < 8; ++e)
         if (d + e < a.D) {
           v[i][e] = src[e] * by;
-          if (W == GRAD) part[i] += v[i][e] * a.o[at + e];
+          if (W == GRAD) part[i] += src[e] * a.o[at + e];
         }
     }
     float m = 0.f;
@@ -135,7 +150,7 @@ __device__ __forceinline__ void split_tile(const Attn& a, const Part& P, const P
     atomicMax(&top[row], fine ? __float_as_uint(m) : 0x7f800000u);
   }
   if constexpr (W == GRAD) {
-    // rowsum(dO' * O), the partial sums of a row in a fixed order
+    // rowsum(dO * O), the partial sums of a row in a fixed order
     __shared__ float sums[kRows * CH];
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i)
@@ -158,12 +173,9 @@ __device__ __forceinline__ void split_tile(const Attn& a, const Part& P, const P
       int e = 14 + range;  // zeros: no smaller than another tile's
       if (most > 0.f) {
         const bool bad = !(most < pow2(range)) || most < pow2(-range) || most > kWide * least;
-        if (bad)
-          ps.bad[pr] = 1u;
-        else
-          e = 14 + 127 - int(__float_as_uint(most) >> 23);
+        e = bad ? kBad : 14 + 127 - int(__float_as_uint(most) >> 23);
       }
-      all[0] = e;
+      all[0] = e == kBad ? 0 : e;
       P.e[size_t(pr) * (P.pad / kRows) + tile] = e;
     }
   }
@@ -184,25 +196,11 @@ __device__ __forceinline__ void split_tile(const Attn& a, const Part& P, const P
     *reinterpret_cast<h8*>(out + row * (DP * 4) + c * 16) = h;
     *reinterpret_cast<h8*>(out + row * (DP * 4) + DP * 2 + c * 16) = l;
   }
-  if (W == GRAD && threadIdx.x < kRows) ps.dl[size_t(pr) * P.pad + n0 + threadIdx.x] = dots[threadIdx.x] * by;
-}
-// E: the running minimum of the exponents of V's tiles; a workgroup per problem,
-// a run of tiles per thread.
-__global__ void __launch_bounds__(kT) k_attn_least(const Parts ps) {
-  __shared__ int runs[kT];
-  const int n = int(ps.v.pad / kRows), per = (n + kT - 1) / kT;
-  const int* e = ps.v.e + size_t(blockIdx.x) * n;
-  int* out = ps.least + size_t(blockIdx.x) * n;
-  const int t0 = int(threadIdx.x) * per, t1 = min(n, t0 + per);
-  int m = 1000;
-  for (int t = t0; t < t1; ++t) m = min(m, e[t]);
-  runs[threadIdx.x] = m;
-  __syncthreads();
-  m = 1000;
-  for (int i = 0; i < int(threadIdx.x); ++i) m = min(m, runs[i]);
-  for (int t = t0; t < t1; ++t) {
-    m = min(m, e[t]);
-    out[t] = m;
+  if (W == GRAD && threadIdx.x < kRows) {
+    const uint32_t n = n0 + threadIdx.x;
+    const size_t row = size_t(pr) * a.N + n;
+    if (n < a.N) a.delta[row] = dots[threadIdx.x];
+    ps.dl[size_t(pr) * P.pad + n] = n < a.N ? dots[threadIdx.x] * a.il[row] * by : 0.f;
   }
 }
 // Tiles of q (and dO), then of k and v, of each problem.
@@ -352,7 +350,11 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
   __shared__ __attribute__((aligned(16))) char Ks[TL::BYTES], Vs[TL::BYTES];
   const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
   const uint32_t back = rest / a.splits, sp = rest - back * a.splits, tile = a.tiles - 1 - back;
-  if (ps.bad[pr]) return;
+  if (unsuited<false>(ps, pr)) {
+    for (uint32_t n = tile * 128; n < min(tile * 128 + 128, a.N); n += 64)
+      fwd_fp32<DP, 1, VEC>(a, pr, n, sp, reinterpret_cast<float*>(Ks), reinterpret_cast<float*>(Vs));
+    return;
+  }
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
   const uint32_t n0 = tile * 128, n = n0 + wave * 32 + col, len = keys_of(a, b);
@@ -518,7 +520,8 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
   __shared__ __attribute__((aligned(16))) float Ps[2][4][1024];
   const uint32_t prob = a.B * a.G, back = blockIdx.x / prob, pr = blockIdx.x - back * prob;
   const uint32_t tile = a.tiles - 1 - back;
-  if (ps.bad[pr]) return;
+  if (unsuited<true>(ps, pr))
+    return dq_fp32<DP, 1, VEC, kPair>(a, pr, tile * 128, reinterpret_cast<float*>(Ks[0]), reinterpret_cast<float*>(Vs[0]));
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blk = wave & 3, col = lane & 31, half = lane >> 5;
   const bool first = __builtin_amdgcn_readfirstlane(wave) < 4;
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
   f16v dq[DP / 32];
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) zero(dq[t]);
-  const int E = mine ? ps.least[size_t(pr) * (ps.v.pad / kRows) + (mine - 1) / kRows] : 0;
+  const int E = least_of(ev, 0, (mine + kRows - 1) / kRows, lane);
   int R = 1000;  // dq counts in units of 2^-(R + E + ey - down_bits + 14)
   each_tile(0, tiles, [&](uint32_t t, auto st) {
     stage(t + 1, std::integral_constant<int, (st + 1) % kStages>{});
@@ -619,7 +622,9 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   __shared__ uint32_t Ls[kStages][kRows];
   const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
   const uint32_t tile = rest / a.splits, sp = rest - tile * a.splits;
-  if (ps.bad[pr]) return;
+  if (unsuited<true>(ps, pr))
+    return dkv_fp32<DP, VEC, kPair>(a, pr, tile * 128, sp, reinterpret_cast<float*>(Qs[0]),
+                                    reinterpret_cast<float*>(Ys[0]), Ps[0][0], Ls[0]);
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blk = wave & 3, col = lane & 31, half = lane >> 5;
   const bool first = __builtin_amdgcn_readfirstlane(wave) < 4;
@@ -630,10 +635,9 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   const int* ey = ps.y.e + size_t(pr) * (ps.q.pad / kRows);
   const char* qp = ps.q.p + size_t(pr) * ps.q.pad * (DP * 4);
   const char* yp = ps.y.p + size_t(pr) * ps.q.pad * (DP * 4);
-  // Row tiles from the first that sees key k0 on; the share of this split of them.
-  const uint32_t from = (k0 < len ? min(first_row(a, k0), a.N) : a.N) / kRows;
-  const uint32_t to = k0 < len ? (a.N + kRows - 1) / kRows : from;
-  const uint32_t t0 = from + (to - from) * sp / a.splits, t1 = from + (to - from) * (sp + 1) / a.splits;
+  uint32_t first_n, end_n;
+  split_rows(a, k0, len, sp, first_n, end_n);
+  const uint32_t t0 = first_n / kRows, t1 = max(t0, (end_n + kRows - 1) / kRows);
   const size_t part = size_t(sp) * a.B * a.T * a.G * a.D;
   u4v rq[TL::LOADS], ry[TL::LOADS];
   float rm = 0.f, rd = 0.f;
@@ -707,7 +711,10 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   load_vec<DP>(ps.v.p + row * (DP * 4), half, xh, xl);
   const int xv = ps.v.e[kt];
   const float vs = pow2(xv);
-  const int* least = ps.least + size_t(pr) * (ps.v.pad / kRows);
+  // E, over V's tiles below `seen_tiles`, grows with the rows.
+  const int* ev = ps.v.e + size_t(pr) * (ps.v.pad / kRows);
+  uint32_t seen_tiles = t0 < t1 ? (wave_limit(a, t0 * kRows, kRows, len) + kRows - 1) / kRows : 0u;
+  int E = least_of(ev, 0, seen_tiles, lane);
   int Rk = 1000;  // dk counts in units of 2^-(Rk - down_bits + 14)
   each_tile(t0, t1, [&](uint32_t t, auto sn) {
     stage(t + 1, std::integral_constant<int, (sn + 1) % kStages>{});
@@ -715,7 +722,8 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
     const uint32_t seen = t > t0 ? wave_limit(a, u * kRows, kRows, len) : 0u;
     if (seen > kw) {
       constexpr int st = (sn + kStages - 1) % kStages;
-      const int xy = ey[u], E = least[(seen - 1) / kRows], x = eq[u] + xy + E;
+      for (; seen_tiles * kRows < seen; ++seen_tiles) E = min(E, ev[seen_tiles]);
+      const int xy = ey[u], x = eq[u] + xy + E;
       f16v dp = scores<DP>(Ys[st], xh, xl, col, half);
       Rv = min(Rv, xy);
       if (x < Rk) {
@@ -743,24 +751,6 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
                      Rk == 1000 ? 0.f : pow2(down_bits<DP>() - 14 - Rk / 2) * a.scale, pow2(Rk / 2 - Rk));
 }
 
-// dK, dV from the row splits' shares (`values` of each, in a row), added in order.
-__global__ void __launch_bounds__(kT)
-    k_attn_sum(const float* pk, const float* pv, float* dk, float* dv, size_t values, uint32_t splits) {
-  const size_t i = size_t(blockIdx.x) * kT + threadIdx.x;
-  if (i >= values) return;
-  float x = 0.f, y = 0.f;
-  for (uint32_t s = 0; s < splits; ++s) {
-    if (dk) x += pk[s * values + i];
-    if (dv) y += pv[s * values + i];
-  }
-  if (dk) dk[i] = x;
-  if (dv) dv[i] = y;
-}
-__global__ void k_attn_no_bad(uint32_t* bad, uint32_t n) {
-  const uint32_t i = blockIdx.x * kT + threadIdx.x;
-  if (i < n) bad[i] = 0u;
-}
-
 struct Places {
   size_t next = 0;
   size_t take(size_t floats) {
@@ -782,12 +772,11 @@ struct Prep {
     const uint32_t prob = a.B * a.G;
     const uint32_t nq = (a.N + 127) & ~127u, nk = (a.T + 127) & ~127u;
     Places at;
-    const size_t bad = at.take(prob);
     const size_t q = at.take(size_t(prob) * nq * DP), qe = at.take(size_t(prob) * (nq / kRows));
     const size_t k = at.take(size_t(prob) * nk * DP), ke = at.take(size_t(prob) * (nk / kRows));
     const size_t v = at.take(size_t(prob) * nk * DP), ve = at.take(size_t(prob) * (nk / kRows));
     const size_t y = bwd ? at.take(size_t(prob) * nq * DP) : 0, ye = bwd ? at.take(size_t(prob) * (nq / kRows)) : 0;
-    const size_t dl = bwd ? at.take(size_t(prob) * nq) : 0, least = bwd ? at.take(size_t(prob) * (nk / kRows)) : 0;
+    const size_t dl = bwd ? at.take(size_t(prob) * nq) : 0;
     const size_t ex = at.take(extra);
     float* ws = workspace(at.next);
     if (!ws) return false;
@@ -799,16 +788,13 @@ struct Prep {
     ps.v = part(v, ve, nk);
     ps.y = part(y, ye, nq);
     ps.dl = ws + dl;
-    ps.least = reinterpret_cast<int*>(ws + least);
-    ps.bad = reinterpret_cast<uint32_t*>(ws + bad);
     more = ws + ex;
-    hipLaunchKernelGGL(k_attn_no_bad, dim3(cdiv(prob, kT)), dim3(kT), 0, stream(), ps.bad, prob);
+    if (bwd) a.delta = more;
     const uint32_t per = (bwd ? 2 : 1) * (nq / kRows) + 2 * (nk / kRows);
     if (bwd)
       hipLaunchKernelGGL((k_attn_split<DP, VEC, true>), dim3(per * prob), dim3(kT), 0, stream(), a, ps);
     else
       hipLaunchKernelGGL((k_attn_split<DP, VEC, false>), dim3(per * prob), dim3(kT), 0, stream(), a, ps);
-    if (bwd) hipLaunchKernelGGL(k_attn_least, dim3(prob), dim3(kT), 0, stream(), ps);
     return check_launch("attention (parts)");
   }
 };
@@ -821,12 +807,6 @@ struct Forward {
     return check_launch("AttentionForward (parts)");
   }
 };
-// Splits of the rows in the dK / dV kernel: where its 128-key blocks fill less
-// than the CUs, and no less than eight row tiles each.
-uint32_t row_splits(const Attn& a) {
-  const uint32_t wgs = cdiv(a.T, 128) * a.B * a.G, cus = uint32_t(num_cus());
-  return wgs >= cus ? 1u : std::max(1u, std::min(cdiv(cus, wgs), cdiv(a.N, 8 * kRows)));
-}
 struct Backward {
   Attn a;
   Parts ps;
@@ -842,15 +822,13 @@ struct Backward {
       const size_t values = size_t(a.B) * a.T * a.G * a.D;
       Attn d = a;
       d.tiles = cdiv(a.T, 128);
-      d.splits = row_splits(a);
+      d.splits = row_splits(a, 128);
       if (d.splits > 1) {
         if (a.dk) d.dk = more;
         if (a.dv) d.dv = more + d.splits * values;
       }
       hipLaunchKernelGGL((k_attn_dkv_parts<DP, VEC>), dim3(d.tiles * d.splits * prob), dim3(kPair), 0, stream(), d, ps);
-      if (d.splits > 1)
-        hipLaunchKernelGGL(k_attn_sum, dim3(cdiv(values, kT)), dim3(kT), 0, stream(), d.dk, d.dv, a.dk, a.dv, values,
-                           d.splits);
+      if (d.splits > 1 && !attn_sum(d, a)) return false;
     }
     return check_launch("AttentionBackward (parts)");
   }
@@ -866,15 +844,21 @@ bool by_dim(uint32_t D, F& f) {
   return false;
 }
 
-bool worth(const AttnArgs& x) {
-  return x.D <= 128 && x.S >= 32 && 4.0 * x.D * x.B * x.H * pairs_of(x) >= 1e9 &&
+// Parts cost a pass over the operands and its launch, and win the more the more
+// keys a row goes over: taken from `least` products of operations and keys on.
+// Forward, causal (us on fp32 / on parts): 4 x 512 tokens, 12 heads of 64, 35 / 44;
+// 1 x 1024, 8 heads of 64, 38 / 34; 2 x 1024, 54 / 44; 1 x 2048, 4 heads of 128, 99 / 54.
+// Backward: 32 x 64 tokens, 8 heads of 64, 20 / 37; 8 x 256 50 / 50; 16 x 197, 6
+// heads, 69 / 48; 4 x 512, 8 heads, 90 / 63; 1 x 2048, 4 heads of 128, 410 / 208.
+bool worth(const AttnArgs& x, double least) {
+  return x.D <= 128 && x.S >= 32 && 4.0 * x.D * x.B * x.H * pairs_of(x) * x.T >= least &&
          uint64_t(x.B) * x.G * (uint64_t(x.H / x.G) * x.S + x.T) < 0x20000000ull;
 }
 
 }  // namespace
 
 bool attn_fwd_parts(const AttnArgs& x, Attn a, bool* took) {
-  if (!worth(x)) return true;
+  if (!worth(x, 1e12)) return true;
   *took = true;
   const uint32_t prob = a.B * a.G, cus = uint32_t(num_cus()), kt = cdiv(a.T, kRows);
   a.tiles = cdiv(a.N, 128);
@@ -890,23 +874,19 @@ bool attn_fwd_parts(const AttnArgs& x, Attn a, bool* took) {
   a.po = p.more + 2 * stat;
   Forward f{a, p.ps};
   if (!by_dim(a.D, f)) return false;
-  if (a.splits > 1 && !attn_join(a)) return false;
-  a.only = p.ps.bad;
-  return attn_fwd_fp32(a);
+  return a.splits == 1 || attn_join(a);
 }
 
 bool attn_bwd_parts(const AttnArgs& x, Attn a, bool* took) {
-  if (!worth(x)) return true;
+  if (!worth(x, 1e11)) return true;
   *took = true;
   const size_t rows = (size_t(a.B) * a.G * a.N + 63) & ~size_t(63);
-  const uint32_t sp = row_splits(a);
+  const uint32_t sp = row_splits(a, 128);
   Prep p{a, {}, true, rows + (sp > 1 ? 2 * sp * size_t(a.B) * a.T * a.G * a.D : 0), nullptr};
   if (!by_dim(a.D, p)) return false;
-  Backward f{a, p.ps, p.more + rows};
-  if (!by_dim(a.D, f)) return false;
-  a.only = p.ps.bad;
   a.delta = p.more;
-  return attn_bwd_fp32(a);
+  Backward f{a, p.ps, p.more + rows};
+  return by_dim(a.D, f);
 }
 
 }  // namespace dce

@@ -563,7 +563,7 @@ def test_reshape(eng):
 
 
 # ------------------------------------------------- large calls, on fp16 parts
-LARGE = [  # from 1e9 operations on
+LARGE = [  # operations times keys from 1e12 on (the last one's backward alone)
     (1, 1024, 1024, 8, 8, 64, True, None),
     (2, 700, 700, 12, 4, 40, False, [700, 333]),
     (1, 1100, 1300, 4, 2, 128, True, None),
