@@ -610,17 +610,20 @@ bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* row
   if (all.empty()) return true;
   ProfScope prof("muon", flops, bytes);
   // Groups of up to kMaxM matrices, and of up to 2^28 values unless one is larger.
+  // Tiles by the operations of a step (us on 128 / on 64): 1024 x 1024 435 / 281,
+  // 1536 x 1536 (1.4e10) 649 / 571, four 768 x 768 with two 768 x 2000 (1.5e10)
+  // 631 / 578, 2048 x 2048 (3.4e10) 914 / 1032, 2048 x 4096 1336 / 1652.
   for (size_t i = 0; i < all.size();) {
     Mats t{};
     size_t values = 0;
-    uint64_t tiles = 0;
+    double work = 0;  // of a step
     while (i < all.size() && t.count < uint32_t(kMaxM) &&
            (!t.count || values + size_t(all[i].m) * all[i].n <= (size_t(1) << 28))) {
       values += size_t(all[i].m) * all[i].n;
-      tiles += uint64_t(cdiv(all[i].m, 128)) * cdiv(all[i].n, 128);
+      work += (3.0 * all[i].n + all[i].m) * all[i].m * all[i].m;
       t.t[t.count++] = all[i++];
     }
-    const bool big = tiles > uint64_t(num_cus());
+    const bool big = work >= 2.2e10;
     if (!(big ? run_group<128> : run_group<64>)(t, mu, nesterov, decay, clip, steps)) return false;
   }
   return true;
