@@ -25,7 +25,7 @@ struct Attn {
   const float* dy;               // backward
   float *delta, *dq, *dk, *dv;
   uint32_t B, S, T, G, D, rep, N;
-  uint32_t tiles, splits, perSplit;  // splits: of the keys (perSplit tiles each), or of the rows in dK, dV
+  uint32_t tiles, splits, perSplit;  // splits: of the keys (perSplit tiles each in the forward), or of the rows in dK, dV
   FastDiv dRep, dG;
   float c, scale;
   int causal;
@@ -60,6 +60,16 @@ __device__ __forceinline__ void split_rows(const Attn& a, uint32_t k0, uint32_t 
   first = (from + (to - from) * sp / a.splits) * 32;
   end = min((from + (to - from) * (sp + 1) / a.splits) * 32, a.N);
 }
+// Keys [first, end) of split sp of the `most` that a block of rows sees, in whole
+// 32-key tiles, and the place of that split's dq.
+__device__ __forceinline__ void split_keys(const Attn& a, uint32_t most, uint32_t sp, uint32_t& first, uint32_t& end) {
+  const uint32_t tiles = (most + 31) / 32;
+  first = tiles * sp / a.splits * 32;
+  end = min(tiles * (sp + 1) / a.splits * 32, most);
+}
+__device__ __forceinline__ size_t dq_part(const Attn& a, uint32_t sp) {
+  return size_t(sp) * a.B * a.G * a.N * a.D;
+}
 // First value of row n's vector in a [batch][seq][heads][dim] tensor.
 __device__ __forceinline__ size_t q_at(const Attn& a, uint32_t b, uint32_t g, uint32_t n) {
   const uint32_t i = fdiv(n, a.dRep), h = g * a.rep + (n - i * a.rep);
@@ -85,10 +95,23 @@ inline uint32_t row_splits(const Attn& a, uint32_t keys) {
   return wgs >= cus ? 1u : std::max(1u, std::min(cdiv(cus, wgs), cdiv(a.N, 8 * 32)));
 }
 
+// Splits of the keys in a dQ kernel of `rows` rows per workgroup, likewise.
+inline uint32_t key_splits(const Attn& a, uint32_t rows) {
+  const uint32_t wgs = cdiv(a.N, rows) * a.B * a.G, cus = uint32_t(num_cus());
+  return wgs >= cus ? 1u : std::max(1u, std::min(cdiv(cus, wgs), cdiv(a.T, 8 * 32)));
+}
+
+// Floats of the splits' shares of a backward, one kernel's after the other's.
+inline size_t split_floats(const Attn& a, uint32_t rows, uint32_t keys) {
+  const uint32_t sk = a.dq ? key_splits(a, rows) : 1, sr = a.dk || a.dv ? row_splits(a, keys) : 1;
+  const size_t q = sk > 1 ? size_t(sk) * a.B * a.G * a.N * a.D : 0, k = sr > 1 ? 2 * size_t(sr) * a.B * a.T * a.G * a.D : 0;
+  return std::max(q, k);
+}
+
 // Joins the key splits of a forward into o (and the statistics).
 bool attn_join(const Attn& a);
-// Adds the row splits' dk, dv (`from`) into `to`'s.
-bool attn_sum(const Attn& from, const Attn& to);
+// Adds the splits' shares of one or two results of n values each (null: none).
+bool attn_sum(const float* p0, float* out0, const float* p1, float* out1, size_t n, uint32_t splits);
 // On fp16 parts, where they are faster; `took` tells.
 bool attn_fwd_parts(const AttnArgs& x, Attn a, bool* took);
 bool attn_bwd_parts(const AttnArgs& x, Attn a, bool* took);

@@ -39,8 +39,9 @@ __global__ void __launch_bounds__(kT) k_attn_fwd(const Attn a) {
 template <int DP, int QT, bool VEC>
 __global__ void __launch_bounds__(kT) k_attn_dq(const Attn a) {
   __shared__ __attribute__((aligned(16))) float Ks[kKeys * DP], Vs[kKeys * DP];
-  const uint32_t prob = a.B * a.G, back = blockIdx.x / prob, pr = blockIdx.x - back * prob;
-  dq_fp32<DP, QT, VEC, kT>(a, pr, (a.tiles - 1 - back) * 64 * QT, Ks, Vs);
+  const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
+  const uint32_t back = rest / a.splits, sp = rest - back * a.splits;
+  dq_fp32<DP, QT, VEC, kT>(a, pr, (a.tiles - 1 - back) * 64 * QT, sp, Ks, Vs);
 }
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(kT) k_attn_dkv(const Attn a) {
@@ -51,9 +52,9 @@ __global__ void __launch_bounds__(kT) k_attn_dkv(const Attn a) {
   dkv_fp32<DP, VEC, kT>(a, pr, tile * 64, sp, Qs, Ys, St, Lim);
 }
 
-// dK, dV from the row splits' shares (`values` of each, in a row), added in order.
+// Gradients from the splits' shares (`values` of each, in a row), added in order.
 __global__ void __launch_bounds__(kT)
-    k_attn_sum(const float* pk, const float* pv, float* dk, float* dv, size_t values, uint32_t splits) {
+    k_attn_sum(const float* pk, float* dk, const float* pv, float* dv, size_t values, uint32_t splits) {
   const size_t i = size_t(blockIdx.x) * kT + threadIdx.x;
   if (i >= values) return;
   float x = 0.f, y = 0.f;
@@ -304,18 +305,23 @@ struct FwdRun {
 
 struct BwdRun {
   Attn a;
-  float* more;  // the row splits' shares
+  float* more;  // the splits' shares
   template <int DP, bool VEC>
   bool run() {
     constexpr int QT = DP <= 64 ? 2 : 1;
     const uint32_t prob = a.B * a.G;
     const bool wide = QT == 2 && uint64_t(cdiv(a.N, 128)) * prob >= 2 * uint32_t(num_cus());
-    a.tiles = cdiv(a.N, wide ? 128 : 64);
+    Attn q = a;
+    q.tiles = cdiv(a.N, wide ? 128 : 64);
+    q.splits = a.dq ? key_splits(a, 64) : 1;
+    if (q.splits > 1) q.dq = more;
+    const dim3 grid(q.tiles * q.splits * prob);
     if (wide)
-      hipLaunchKernelGGL((k_attn_dq<DP, QT, VEC>), dim3(a.tiles * prob), dim3(kT), 0, stream(), a);
+      hipLaunchKernelGGL((k_attn_dq<DP, QT, VEC>), grid, dim3(kT), 0, stream(), q);
     else
-      hipLaunchKernelGGL((k_attn_dq<DP, 1, VEC>), dim3(a.tiles * prob), dim3(kT), 0, stream(), a);
+      hipLaunchKernelGGL((k_attn_dq<DP, 1, VEC>), grid, dim3(kT), 0, stream(), q);
     if (!check_launch("AttentionBackward (dQ)")) return false;
+    if (q.splits > 1 && !attn_sum(q.dq, a.dq, nullptr, nullptr, size_t(prob) * a.N * a.D, q.splits)) return false;
     if (!a.dk && !a.dv) return true;
     const size_t values = size_t(a.B) * a.T * a.G * a.D;
     Attn d = a;
@@ -326,7 +332,8 @@ struct BwdRun {
       if (a.dv) d.dv = more + d.splits * values;
     }
     hipLaunchKernelGGL((k_attn_dkv<DP, VEC>), dim3(d.tiles * d.splits * prob), dim3(kT), 0, stream(), d);
-    return check_launch("AttentionBackward (dK, dV)") && (d.splits == 1 || attn_sum(d, a));
+    return check_launch("AttentionBackward (dK, dV)") &&
+           (d.splits == 1 || attn_sum(d.dk, a.dk, d.dv, a.dv, values, d.splits));
   }
 };
 
@@ -336,10 +343,8 @@ bool attn_join(const Attn& a) {
   hipLaunchKernelGGL(k_attn_join, dim3(a.B * a.G * a.N), dim3(std::min(kT, int(a.D + 63) / 64 * 64)), 0, stream(), a);
   return check_launch("AttentionForward (join)");
 }
-bool attn_sum(const Attn& from, const Attn& to) {
-  const size_t values = size_t(to.B) * to.T * to.G * to.D;
-  hipLaunchKernelGGL(k_attn_sum, dim3(cdiv(values, kT)), dim3(kT), 0, stream(), from.dk, from.dv, to.dk, to.dv, values,
-                     from.splits);
+bool attn_sum(const float* p0, float* out0, const float* p1, float* out1, size_t n, uint32_t splits) {
+  hipLaunchKernelGGL(k_attn_sum, dim3(cdiv(n, kT)), dim3(kT), 0, stream(), p0, out0, p1, out1, n, splits);
   return check_launch("AttentionBackward (sum)");
 }
 
@@ -363,8 +368,7 @@ bool attention_backward(const AttnArgs& x, const float* dy, float* dq, float* dk
   if (!attn_bwd_parts(x, a, &took)) return false;
   if (took) return true;
   const size_t rows = (size_t(x.B) * x.H * x.S + 63) & ~size_t(63);
-  const uint32_t sp = dk || dv ? row_splits(a, 64) : 1;
-  a.delta = workspace(rows + (sp > 1 ? 2 * sp * size_t(a.B) * a.T * a.G * a.D : 0));
+  a.delta = workspace(rows + split_floats(a, 64, 64));
   return a.delta && by_dim(a.D, a.D % 4 == 0, BwdRun{a, a.delta + rows});
 }
 

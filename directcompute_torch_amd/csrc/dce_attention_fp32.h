@@ -249,7 +249,7 @@ __device__ __forceinline__ void fwd_fp32(const Attn& a, uint32_t pr, uint32_t n0
 // the other kernel.
 // ---------------------------------------------------------------------------
 template <int DP, int QT, bool VEC, int NT>
-__device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0, float* Ks, float* Vs) {
+__device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0, uint32_t sp, float* Ks, float* Vs) {
   using TL = Tile<DP, kKeys, VEC, NT>;
   using CL = Cols<DP>;
   constexpr uint32_t ROWS = NT / 4 * QT;
@@ -284,6 +284,8 @@ __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0,
     load_frag<DP, VEC>(a.q + at, ok, a.D, g, q[t]);
   }
   if (!a.dq) return;
+  uint32_t j0, j1;
+  split_keys(a, most, sp, j0, j1);
   const uint32_t stride = a.G * a.D;
   f4 rk[TL::LOADS], rv[TL::LOADS];
   auto fetch = [&](uint32_t j) {
@@ -291,13 +293,13 @@ __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0,
     TL::load(rows_view(a.k + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rk);
     TL::load(rows_view(a.v + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rv);
   };
-  if (most) fetch(0);
-  for (uint32_t j = 0; j < most; j += kKeys) {
+  if (j0 < j1) fetch(j0);
+  for (uint32_t j = j0; j < j1; j += kKeys) {
     __syncthreads();
     TL::store(Ks, rk);
     TL::store(Vs, rv);
     __syncthreads();
-    if (j + kKeys < most) fetch(j + kKeys);
+    if (j + kKeys < j1) fetch(j + kKeys);
     if (j >= mine) continue;
     f4 s[QT][2], dp[QT][2];
 #pragma unroll
@@ -345,7 +347,7 @@ __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0,
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const uint32_t n = n0 + (wave * QT + t) * 16 + col;
-    if (n < a.N) CL::template write<VEC>(a.dq + q_at(a, b, gh, n), a.D, g, dq[t], 1.f);
+    if (n < a.N) CL::template write<VEC>(a.dq + dq_part(a, sp) + q_at(a, b, gh, n), a.D, g, dq[t], 1.f);
   }
 }
 

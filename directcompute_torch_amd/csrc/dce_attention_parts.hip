@@ -518,10 +518,11 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
   using TL = PTile<DP, kPair>;
   __shared__ __attribute__((aligned(16))) char Ks[kStages][TL::BYTES], Vs[kStages][TL::BYTES];
   __shared__ __attribute__((aligned(16))) float Ps[2][4][1024];
-  const uint32_t prob = a.B * a.G, back = blockIdx.x / prob, pr = blockIdx.x - back * prob;
-  const uint32_t tile = a.tiles - 1 - back;
+  const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
+  const uint32_t back = rest / a.splits, sp = rest - back * a.splits, tile = a.tiles - 1 - back;
   if (unsuited<true>(ps, pr))
-    return dq_fp32<DP, 1, VEC, kPair>(a, pr, tile * 128, reinterpret_cast<float*>(Ks[0]), reinterpret_cast<float*>(Vs[0]));
+    return dq_fp32<DP, 1, VEC, kPair>(a, pr, tile * 128, sp, reinterpret_cast<float*>(Ks[0]),
+                                      reinterpret_cast<float*>(Vs[0]));
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blk = wave & 3, col = lane & 31, half = lane >> 5;
   const bool first = __builtin_amdgcn_readfirstlane(wave) < 4;
@@ -534,29 +535,31 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
   const int* ev = ps.v.e + size_t(pr) * (ps.v.pad / kRows);
   const char* kp = ps.k.p + size_t(pr) * ps.k.pad * (DP * 4);
   const char* vp = ps.v.p + size_t(pr) * ps.v.pad * (DP * 4);
-  const uint32_t tiles = (most + kRows - 1) / kRows;
+  uint32_t j0, j1;
+  split_keys(a, most, sp, j0, j1);
+  const uint32_t t0 = j0 / kRows, t1 = max(t0, (j1 + kRows - 1) / kRows);
   u4v rk[TL::LOADS], rv[TL::LOADS];
   auto fetch = [&](uint32_t t) {
     TL::load(kp + size_t(t) * kRows * (DP * 4), rk);
     TL::load(vp + size_t(t) * kRows * (DP * 4), rv);
   };
   auto stage = [&](uint32_t t, auto place) {  // tile t from the registers, which then take t + 1
-    if (t >= tiles) return;
+    if (t >= t1) return;
     TL::store(Ks[place], rk);
     TL::store(Vs[place], rv);
-    if (t + 1 < tiles) fetch(t + 1);
+    if (t + 1 < t1) fetch(t + 1);
   };
-  if (tiles) fetch(0);
-  stage(0, std::integral_constant<int, 0>{});
+  if (t0 < t1) fetch(t0);
+  stage(t0, std::integral_constant<int, 0>{});
   __syncthreads();
   h8 xh[DP / 16], xl[DP / 16];
   if (first) {
     load_vec<DP>(ps.q.p + row * (DP * 4), half, xh, xl);
     const float cq = a.c * pow2(-ps.q.e[et]), m = n < a.N ? a.m[size_t(pr) * a.N + n] : 0.f;
-    each_tile(0, tiles, [&](uint32_t t, auto st) {
+    each_tile(t0, t1, [&](uint32_t t, auto st) {
       stage(t + 1, std::integral_constant<int, (st + 1) % kStages>{});
       const uint32_t j = t * kRows;
-      if (j < mine) {
+      if (t < t1 && j < mine) {
         const float cs = cq * pow2(-ek[t]);
         f16v s = scores<DP>(Ks[st], xh, xl, col, half);
 #pragma unroll
@@ -580,11 +583,11 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
   for (int t = 0; t < DP / 32; ++t) zero(dq[t]);
   const int E = least_of(ev, 0, (mine + kRows - 1) / kRows, lane);
   int R = 1000;  // dq counts in units of 2^-(R + E + ey - down_bits + 14)
-  each_tile(0, tiles, [&](uint32_t t, auto st) {
+  each_tile(t0, t1, [&](uint32_t t, auto st) {
     stage(t + 1, std::integral_constant<int, (st + 1) % kStages>{});
     const uint32_t u = t - 1;  // the tile before the first waves'
     constexpr int su = (st + kStages - 1) % kStages;
-    if (t && u * kRows < mine) {
+    if (t > t0 && u * kRows < mine) {
       const int xk = ek[u], xv = ev[u];
       f16v dp = scores<DP>(Vs[su], xh, xl, col, half);
       if (xk < R) {
@@ -605,7 +608,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
   if (n >= a.N) return;
   // 2^(down_bits - 14 - R - E - ey), in two factors that stay in range
   const float u = R == 1000 ? 0.f : pow2(down_bits<DP>() - 14 - R - E) * a.scale;
-  write_vec<DP, VEC>(a.dq + q_at(a, b, gh, n), a.D, half, dq, u, pow2(-ey));
+  write_vec<DP, VEC>(a.dq + dq_part(a, sp) + q_at(a, b, gh, n), a.D, half, dq, u, pow2(-ey));
 }
 
 // ---------------------------------------------------------------------------
@@ -810,13 +813,17 @@ struct Forward {
 struct Backward {
   Attn a;
   Parts ps;
-  float* more;
+  float* more;  // the splits' shares
   template <int DP, bool VEC>
   bool run() {
     const uint32_t prob = a.B * a.G;
     if (a.dq) {
-      a.tiles = cdiv(a.N, 128);
-      hipLaunchKernelGGL((k_attn_dq_parts<DP, VEC>), dim3(a.tiles * prob), dim3(kPair), 0, stream(), a, ps);
+      Attn q = a;
+      q.tiles = cdiv(a.N, 128);
+      q.splits = key_splits(a, 128);
+      if (q.splits > 1) q.dq = more;
+      hipLaunchKernelGGL((k_attn_dq_parts<DP, VEC>), dim3(q.tiles * q.splits * prob), dim3(kPair), 0, stream(), q, ps);
+      if (q.splits > 1 && !attn_sum(q.dq, a.dq, nullptr, nullptr, size_t(prob) * a.N * a.D, q.splits)) return false;
     }
     if (a.dk || a.dv) {
       const size_t values = size_t(a.B) * a.T * a.G * a.D;
@@ -828,7 +835,7 @@ struct Backward {
         if (a.dv) d.dv = more + d.splits * values;
       }
       hipLaunchKernelGGL((k_attn_dkv_parts<DP, VEC>), dim3(d.tiles * d.splits * prob), dim3(kPair), 0, stream(), d, ps);
-      if (d.splits > 1 && !attn_sum(d, a)) return false;
+      if (d.splits > 1 && !attn_sum(d.dk, a.dk, d.dv, a.dv, values, d.splits)) return false;
     }
     return check_launch("AttentionBackward (parts)");
   }
@@ -881,8 +888,7 @@ bool attn_bwd_parts(const AttnArgs& x, Attn a, bool* took) {
   if (!worth(x, 1e11)) return true;
   *took = true;
   const size_t rows = (size_t(a.B) * a.G * a.N + 63) & ~size_t(63);
-  const uint32_t sp = row_splits(a, 128);
-  Prep p{a, {}, true, rows + (sp > 1 ? 2 * sp * size_t(a.B) * a.T * a.G * a.D : 0), nullptr};
+  Prep p{a, {}, true, rows + split_floats(a, 128, 128), nullptr};
   if (!by_dim(a.D, p)) return false;
   a.delta = p.more;
   Backward f{a, p.ps, p.more + rows};

@@ -156,6 +156,8 @@ CASES = [  # B, S, T, H, G, D, causal, lengths
     (1, 20, 90, 2, 2, 200, False, [33]),
     (1, 300, 300, 1, 1, 96, True, None),
     (5, 16, 16, 12, 4, 16, True, [16, 15, 1, 0, 7]),
+    (1, 60, 700, 1, 1, 32, True, None),             # keys split over workgroups in dQ
+    (2, 700, 60, 2, 1, 64, False, [60, 0]),         # rows split in dK, dV
 ]
 
 
@@ -572,6 +574,8 @@ LARGE = [  # operations times keys from 1e12 on (the last one's backward alone)
     (1, 33, 9000, 8, 8, 128, True, [8999]),
     (2, 1300, 400, 8, 2, 100, False, None),
     (1, 2000, 1024, 4, 4, 80, True, None),          # 976 rows see nothing
+    (1, 1200, 1200, 1, 1, 64, True, None),          # one head: both split
+    (2, 400, 1500, 1, 1, 128, True, [1500, 700]),
 ]
 
 
