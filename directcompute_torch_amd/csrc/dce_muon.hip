@@ -516,8 +516,9 @@ struct Places {
 template <int BLK>
 bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32_t steps) {
   constexpr uint32_t depth = Lds<BLK>::DEPTH;
-  // A Gram product is split so that no workgroup has more than its share of the
-  // launch's depth, and none less than 256.
+  // A Gram product is split so that no workgroup has more than a quarter of a CU's
+  // share of the launch's depth, and none less than 256 (AlexNet's matrices: half a
+  // share 14.7 ms, a third 14.7, a quarter or a sixth 13.4, an eighth 13.8).
   auto tri = [](const Mat& m) { return m.mp / BLK * (m.mp / BLK + 1) / 2; };
   double all = 0;
   for (uint32_t i = 0; i < t.count; ++i) {
@@ -525,7 +526,7 @@ bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32
     t.t[i].np = pad(t.t[i].n, BLK);
     all += double(tri(t.t[i])) * t.t[i].np;
   }
-  const double most = std::max(256.0, all / (2.0 * num_cus()));
+  const double most = std::max(256.0, all / (4.0 * num_cus()));
   Places at;
   size_t chunks = 0;
   bool split = false;
