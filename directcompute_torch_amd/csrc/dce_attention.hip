@@ -71,10 +71,11 @@ __global__ void __launch_bounds__(kT)
 // by reading K and V once.  Tiles of 64 keys, 16 to each wave, which keeps sums of
 // its own; the four waves' are joined at the end.  In the general kernel one wave
 // would multiply for all four: 8 sequences of up to 8191 keys, 8 key heads of 128,
-// took 114 us there and take 87 here, at the rate of a large copy.  Operands straight from memory, without LDS, took 155 us: the K
-// fragment's 64 bytes of each of 16 rows keep the address unit busy.
+// took 114 us there and take 81 here (5.2 TB/s; 87 without streaming loads).
+// Operands straight from memory, without LDS, took 155 us: the K fragment's 64
+// bytes of each of 16 rows keep the address unit busy.
 // ---------------------------------------------------------------------------
-template <int DP, bool VEC>
+template <int DP, bool VEC, bool NT>
 __global__ void __launch_bounds__(kT, DP <= 128 ? 2 : 1) k_attn_few(const Attn a) {
   using CL = Cols<DP>;
   using TL = Tile<DP, kFew, VEC, kT>;
@@ -101,8 +102,8 @@ __global__ void __launch_bounds__(kT, DP <= 128 ? 2 : 1) k_attn_few(const Attn a
   f4 rk[TL::LOADS], rv[TL::LOADS];
   auto fetch = [&](uint32_t j) {
     const uint32_t n = min(len - j, uint32_t(kFew));
-    TL::load(rows_view(a.k + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rk);
-    TL::load(rows_view(a.v + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rv);
+    TL::template load<NT>(rows_view(a.k + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rk);
+    TL::template load<NT>(rows_view(a.v + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rv);
   };
   if (j0 < j1) fetch(j0);
   for (uint32_t j = j0; j < j1; j += kFew) {
@@ -292,8 +293,10 @@ struct FwdRun {
       a.po = ws + 2 * stat;
     }
     const dim3 grid(a.tiles * a.splits * prob);
-    if (few)
-      hipLaunchKernelGGL((k_attn_few<DP, VEC>), grid, dim3(kT), 0, stream(), a);
+    if (few && stream_nt(8.0 * a.B * a.T * a.G * a.D))
+      hipLaunchKernelGGL((k_attn_few<DP, VEC, true>), grid, dim3(kT), 0, stream(), a);
+    else if (few)
+      hipLaunchKernelGGL((k_attn_few<DP, VEC, false>), grid, dim3(kT), 0, stream(), a);
     else if (wide)
       hipLaunchKernelGGL((k_attn_fwd<DP, QT, VEC>), grid, dim3(kT), 0, stream(), a);
     else

@@ -40,12 +40,14 @@ template <int DP, int R, bool VEC, int NT>
 struct Tile {
   static constexpr int CH = DP / 4, SLOTS = R * CH, LOADS = (SLOTS + NT - 1) / NT;
   static constexpr bool WHOLE = SLOTS % NT == 0;  // else the last load is for some threads only
+  // NT: streaming, for what is read once and larger than the caches.
+  template <bool NTL = false>
   __device__ static __forceinline__ void load(const BRes& b, uint32_t stride, uint32_t D, f4 (&r)[LOADS]) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const uint32_t slot = threadIdx.x + NT * i, row = slot / CH, d = slot % CH * 4, off = row * stride + d;
       if constexpr (VEC) {
-        r[i] = b.ld4(d < D ? off : kOob);
+        r[i] = NTL ? b.ld4nt(d < D ? off : kOob) : b.ld4(d < D ? off : kOob);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[i][e] = b.ld1(d + e < D ? off + e : kOob);

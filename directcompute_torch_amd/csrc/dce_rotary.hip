@@ -4,9 +4,12 @@
 // (i, i + rot / 2).  Values from `rot` on are copied.  The inverse (the
 // gradient) turns the other way.
 //
-// Bound by memory: 8 bytes per value.  A thread keeps its pairs' c and s in
-// registers over up to kHeads heads of the token, whose loads are all issued
-// before the first store.
+// Bound by memory: 8 bytes per value.  A wave loads whole vectors of neighbouring
+// heads, 16 bytes per lane, contiguous; in the half layout the other value of a
+// pair is then another lane's, and comes through the LDS crossbar.  (Loading both
+// halves in each lane, whose runs of rot / 2 values start and end inside cache
+// lines, ran at 4.7 TB/s over 4 x 4096 tokens of 32 heads of 128, 96 of them
+// turned.)
 #include "dce_internal.h"
 
 #include <algorithm>
@@ -16,15 +19,17 @@ namespace dce {
 namespace {
 
 constexpr int kT = 256;
-constexpr uint32_t kHeads = 4;
+constexpr int kLoads = 4;  // vectors in flight per lane
 
 struct Rot {
   const float *x, *table, *pos;
   float* y;
-  uint32_t S, H, D, rot, rows, units, groups;  // units: threads of a head's vector
-  FastDiv dU, dGr, dS;
+  uint32_t S, H, D, rot, rows;
+  uint32_t units;      // lanes, or threads, of a head's vector
+  uint32_t per;        // vectors of a wave's load
+  FastDiv dU, dH, dS;
   float sign;
-  uint64_t total;
+  uint64_t total;      // vectors, or threads
 };
 
 // The table row of token t (row t % S without positions); ~0: outside the
@@ -38,76 +43,54 @@ __device__ __forceinline__ uint32_t table_row(const Rot& a, uint32_t t) {
   return p >= 0.f && p < float(a.rows) ? uint32_t(p) : ~0u;
 }
 
-// Eight values per thread and head: four pairs, or a copy of up to eight.
+// Vectors of D / 4 lanes each, `per` of them to a load of a wave.
 template <bool INTER, bool NT>
 __global__ void __launch_bounds__(kT) k_rotary4(const Rot a) {
-  const uint64_t idx = uint64_t(xcd_block_id()) * kT + threadIdx.x;
-  if (idx >= a.total) return;
-  const uint32_t id = uint32_t(idx), tg = fdiv(id, a.dU), u = id - tg * a.units;
-  const uint32_t t = fdiv(tg, a.dGr), h0 = (tg - t * a.groups) * kHeads;
-  const uint32_t n = min(kHeads, a.H - h0);
-  const float* x = a.x + (size_t(t) * a.H + h0) * a.D;
-  float* y = a.y + (size_t(t) * a.H + h0) * a.D;
-  const uint32_t turned = a.rot / 8;
-  f4 A[kHeads], B[kHeads];
-  if (u < turned) {
-    const uint32_t i = INTER ? 8 * u : 4 * u, j = INTER ? 8 * u + 4 : 4 * u + a.rot / 2;
-    const uint32_t row = table_row(a, t);
-    f4 w0 = {0.f, 0.f, 0.f, 0.f}, w1 = w0;
-    if (row != ~0u) {
-      const f4* w = reinterpret_cast<const f4*>(a.table + size_t(row) * a.rot + 8 * u);
-      w0 = w[0];
-      w1 = w[1];
-    }
-    const f4 c = {w0[0], w0[2], w1[0], w1[2]};
-    const f4 s = {w0[1] * a.sign, w0[3] * a.sign, w1[1] * a.sign, w1[3] * a.sign};
+  const uint32_t lane = threadIdx.x & 63, own = fdiv(lane, a.dU), d = (lane - own * a.units) * 4;
+  const bool live = own < a.per, turns = live && d < a.rot;
+  const uint32_t half = a.rot / 2;
+  // The pairs of this lane's values in a table row, and (half layout) the lane
+  // of their other values.
+  const uint32_t p = INTER ? d / 2 : d < half ? d : d - half;
+  const int other = int(d < half ? lane + half / 4 : lane - half / 4) * 4;
+  const float sign = INTER || d >= half ? a.sign : -a.sign;
+  const uint64_t first = (uint64_t(blockIdx.x) * 4 + (threadIdx.x >> 6)) * (kLoads * a.per) + own;
+  f4 x[kLoads], w0[kLoads], w1[kLoads];
 #pragma unroll
-    for (uint32_t h = 0; h < kHeads; ++h)
-      if (h < n) {
-        A[h] = ld4s<NT>(x + size_t(h) * a.D + i);
-        B[h] = ld4s<NT>(x + size_t(h) * a.D + j);
-      }
-#pragma unroll
-    for (uint32_t h = 0; h < kHeads; ++h)
-      if (h < n) {
-        f4 p = A[h], q = B[h];
-        if constexpr (INTER) {
-          const f4 a0 = {p[0], p[2], q[0], q[2]}, b0 = {p[1], p[3], q[1], q[3]};
-          f4 ya, yb;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            ya[e] = a0[e] * c[e] - b0[e] * s[e];
-            yb[e] = a0[e] * s[e] + b0[e] * c[e];
-          }
-          p = f4{ya[0], yb[0], ya[1], yb[1]};
-          q = f4{ya[2], yb[2], ya[3], yb[3]};
-        } else {
-          const f4 a0 = p, b0 = q;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            p[e] = a0[e] * c[e] - b0[e] * s[e];
-            q[e] = a0[e] * s[e] + b0[e] * c[e];
-          }
-        }
-        st4s<NT>(y + size_t(h) * a.D + i, p);
-        st4s<NT>(y + size_t(h) * a.D + j, q);
-      }
-    return;
+  for (int k = 0; k < kLoads; ++k) {
+    const uint64_t v = first + uint64_t(k) * a.per;
+    x[k] = w0[k] = w1[k] = f4{0.f, 0.f, 0.f, 0.f};
+    if (!live || v >= a.total) continue;
+    x[k] = ld4s<NT>(a.x + v * a.D + d);
+    if (!turns) continue;
+    const uint32_t row = table_row(a, fdiv(uint32_t(v), a.dH));
+    if (row == ~0u) continue;
+    const f4* w = reinterpret_cast<const f4*>(a.table + size_t(row) * a.rot + 2 * p);
+    w0[k] = w[0];
+    if (!INTER) w1[k] = w[1];
   }
-  const uint32_t i = a.rot + 8 * (u - turned);
-  const bool two = i + 4 < a.D;
 #pragma unroll
-  for (uint32_t h = 0; h < kHeads; ++h)
-    if (h < n) {
-      A[h] = ld4s<NT>(x + size_t(h) * a.D + i);
-      if (two) B[h] = ld4s<NT>(x + size_t(h) * a.D + i + 4);
-    }
+  for (int k = 0; k < kLoads; ++k) {
+    const uint64_t v = first + uint64_t(k) * a.per;
+    f4 y;
+    if constexpr (INTER) {
 #pragma unroll
-  for (uint32_t h = 0; h < kHeads; ++h)
-    if (h < n) {
-      st4s<NT>(y + size_t(h) * a.D + i, A[h]);
-      if (two) st4s<NT>(y + size_t(h) * a.D + i + 4, B[h]);
+      for (int e = 0; e < 4; e += 2) {
+        const float c = w0[k][e], s = w0[k][e + 1] * sign;
+        y[e] = x[k][e] * c - x[k][e + 1] * s;
+        y[e + 1] = x[k][e] * s + x[k][e + 1] * c;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float c = e < 2 ? w0[k][2 * e] : w1[k][2 * e - 4], s = e < 2 ? w0[k][2 * e + 1] : w1[k][2 * e - 3];
+        const float o = __builtin_bit_cast(
+            float, __builtin_amdgcn_ds_bpermute(other, __builtin_bit_cast(int, float(x[k][e]))));
+        y[e] = x[k][e] * c + o * (s * sign);
+      }
     }
+    if (live && v < a.total) st4s<NT>(a.y + v * a.D + d, turns ? y : x[k]);
+  }
 }
 
 // Any sizes: a pair, or one copied value, per thread.
@@ -116,7 +99,7 @@ __global__ void __launch_bounds__(kT) k_rotary1(const Rot a) {
   const uint64_t idx = uint64_t(xcd_block_id()) * kT + threadIdx.x;
   if (idx >= a.total) return;
   const uint32_t id = uint32_t(idx), th = fdiv(id, a.dU), u = id - th * a.units;
-  const uint32_t t = fdiv(th, a.dGr);
+  const uint32_t t = fdiv(th, a.dH);
   const float* x = a.x + size_t(th) * a.D;
   float* y = a.y + size_t(th) * a.D;
   const uint32_t turned = a.rot / 2;
@@ -157,17 +140,19 @@ bool rotary(const float* x, const float* table, const float* pos, float* y, uint
   a.sign = inverse ? -1.f : 1.f;
   const double bytes = 8.0 * tokens * H * D;
   ProfScope prof("rotary", 3.0 * tokens * H * rot, bytes);
-  const bool quads = rot % 8 == 0 && D % 4 == 0;
-  a.groups = quads ? cdiv(H, kHeads) : H;
-  a.units = quads ? rot / 8 + cdiv(D - rot, 8) : rot / 2 + (D - rot);
+  const uint64_t vectors = uint64_t(tokens) * H;
+  // Whole quads of pairs' values, and vectors that fit a wave.
+  const bool quads = rot % (interleaved ? 4 : 8) == 0 && D % 4 == 0 && D <= 256;
+  a.units = quads ? D / 4 : rot / 2 + (D - rot);
+  a.per = 64 / (D / 4 ? D / 4 : 1);
   a.dU = make_fastdiv(a.units);
-  a.dGr = make_fastdiv(a.groups);
-  a.total = uint64_t(tokens) * a.groups * a.units;
+  a.dH = make_fastdiv(H);
+  a.total = quads ? vectors : vectors * a.units;
   if (a.total >= 0x80000000ull) {
     set_error("RotaryApply: %u tokens of %u heads of %u values are too many for one call", tokens, H, D);
     return false;
   }
-  const dim3 grid(cdiv(a.total, kT)), block(kT);
+  const dim3 grid(quads ? cdiv(vectors, 4 * kLoads * a.per) : cdiv(a.total, kT)), block(kT);
   const bool nt = stream_nt(bytes);
 #define DCE_ROT(I, N) hipLaunchKernelGGL((k_rotary4<I, N>), grid, block, 0, stream(), a)
   if (!quads) {

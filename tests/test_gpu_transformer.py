@@ -75,6 +75,26 @@ def test_rotary(eng, shape, rot, scattered, interleaved):
     eng.end_batch()
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_streaming_accesses_change_nothing(eng, interleaved):
+    """The kernels' nontemporal forms, taken above a size, at small sizes."""
+    r = rng(3)
+    x = dev(eng, r.standard_normal((3, 40, 6, 96)))
+    q, k, v = (dev(eng, r.standard_normal(s)) for s in ((2, 1, 4, 64), (2, 500, 2, 64), (2, 500, 2, 64)))
+    t = eng.rotary_table(40, 72)
+
+    def both():
+        return eng.rotary(x, t, None, interleaved).sync().copy(), eng.attention(q, k, v).sync().copy()
+    want = both()
+    eng.lib.SetStreamingThreshold(0.0)
+    try:
+        got = both()
+    finally:
+        eng.lib.SetStreamingThreshold(-1.0)
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
+    eng.end_batch()
+
+
 def test_rotary_outside_the_table_reads_zeros(eng):
     r = rng(1)
     x = r.standard_normal((1, 6, 2, 16)).astype(np.float32)
