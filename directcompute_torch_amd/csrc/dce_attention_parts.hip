@@ -859,7 +859,7 @@ bool by_dim(uint32_t D, F& f) {
 // heads, 69 / 48; 4 x 512, 8 heads, 90 / 63; 1 x 2048, 4 heads of 128, 410 / 208.
 bool worth(const AttnArgs& x, double least) {
   return x.D <= 128 && x.S >= 32 && 4.0 * x.D * x.B * x.H * pairs_of(x) * x.T >= least &&
-         uint64_t(x.B) * x.G * (uint64_t(x.H / x.G) * x.S + x.T) < 0x20000000ull;
+         uint64_t(x.B) * x.G * (uint64_t(x.H / x.G) * x.S + x.T + 256) < 0x08000000ull;  // threads below 2^32
 }
 
 }  // namespace

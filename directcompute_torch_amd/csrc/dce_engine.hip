@@ -1336,8 +1336,10 @@ static bool attn_args(const char* what, void* q, void* k, void* v, void* lengths
     return false;
   }
   const uint64_t vec = uint64_t(heads) * headDim, rows = uint64_t(batch) * seq * heads;
-  // 32-bit offsets inside a key tile, row and workgroup counts below 2^31
-  if (vec * 64 >= kOob || rows >= 0x80000000ull || uint64_t(batch) * keys * kvHeads >= 0x80000000ull) {
+  // 32-bit offsets inside a key tile, row counts below 2^31, fewer than 2^32 threads in a launch
+  const uint64_t tiles = (uint64_t(heads / kvHeads) * seq + 63) / 64 + (uint64_t(keys) + 63) / 64;
+  if (vec * 64 >= kOob || rows >= 0x80000000ull || uint64_t(batch) * keys * kvHeads >= 0x80000000ull ||
+      uint64_t(batch) * kvHeads * tiles >= (1u << 22)) {
     set_error("%s: %u x %u tokens of %u heads of %u values, %u keys: too many for one call", what,
               batch, seq, heads, headDim, keys);
     return false;

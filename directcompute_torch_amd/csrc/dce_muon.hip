@@ -30,6 +30,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <set>
 #include <vector>
 
 namespace dce {
@@ -579,6 +580,7 @@ bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* row
                 const float* stepSizes, uint32_t n, float mu, bool nesterov, float decay, float clip,
                 uint32_t steps) {
   std::vector<Mat> all;
+  std::set<const void*> written;
   double bytes = 0, flops = 0;
   for (uint32_t i = 0; i < n; ++i) {
     if (!params[i] || !grads[i]) continue;
@@ -591,6 +593,10 @@ bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* row
       set_error("MuonBatch: matrix %u of %u x %u does not fit its buffers", i, rows[i], cols[i]);
       return false;
     }
+    if (!written.insert(W).second || !written.insert(V).second) {
+      set_error("MuonBatch: the parameter or momentum of matrix %u is another one's too", i);
+      return false;
+    }
     Mat m{};
     m.w = W->ptr;
     m.g = G->ptr;
@@ -601,7 +607,7 @@ bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* row
     m.step = stepSizes[i];
     // a tile's operand rows are reached with 32-bit offsets
     if (uint64_t(m.n) * 128 + (1u << 14) >= kOob) {
-      set_error("MuonBatch: matrix %u has %u columns: too many", i, m.n);
+      set_error("MuonBatch: matrix %u is %u long (4 million at most)", i, m.n);
       return false;
     }
     all.push_back(m);

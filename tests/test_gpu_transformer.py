@@ -325,7 +325,7 @@ def test_attention_refusals(eng):
     lib, st = eng.lib, ctypes.c_void_p()
     args = [q.gpu_buf, k.gpu_buf, k.gpu_buf, None]
     for dims in ((2, 3, 6, 4, 2, 8), (2, 4, 5, 4, 2, 8), (2, 3, 5, 4, 3, 8), (0, 3, 5, 4, 2, 8), (2, 3, 0, 4, 2, 8),
-                 (65535, 65535, 65535, 4, 2, 8)):
+                 (65535, 65535, 65535, 4, 2, 8), (1 << 22, 1, 1, 1, 1, 1)):
         assert not lib.AttentionForward(*args, *dims, 0, 1.0, ctypes.byref(st)) and not st.value
         assert eng.last_error()
     assert not lib.AttentionForward(q.gpu_buf, None, k.gpu_buf, None, 2, 3, 5, 4, 2, 8, 0, 1.0, None)
@@ -452,6 +452,14 @@ def test_muon_refusals(eng):
     assert not lib.MuonBatch(P(), P(), P(), one(u, 0), one(u, 4), one(f, 1.0), 1, 0.9, 1, 0.0, 1.0, 5)
     assert not lib.MuonBatch(P(), P(), P(), one(u, 4), one(u, 4), one(f, 1.0), 1, 0.9, 1, 0.0, 1.0, 21)
     assert not lib.MuonBatch(P(), P(), one(h, None), one(u, 4), one(u, 4), one(f, 1.0), 1, 0.9, 1, 0.0, 1.0, 5)
+    w.grad = dev(eng, np.ones((4, 4)))
+    with pytest.raises(RuntimeError, match="another one"):
+        eng.Muon([w, w]).step()
+    wide = eng.Tensor.empty((1, 4200000), requires_grad=True, track=False)
+    wide.grad = wide
+    with pytest.raises(RuntimeError, match="4 million"):
+        eng.Muon([wide]).step()
+    w.grad = None
     lib.ClearLastError()
     eng.Muon([w]).step()        # no gradients: nothing to do
     assert np.array_equal(w.sync(), np.zeros((4, 4), np.float32))
@@ -602,6 +610,24 @@ LARGE = [  # operations times keys from 1e12 on (the last one's backward alone)
 @pytest.mark.parametrize("case", LARGE, ids=lambda c: "x".join(map(str, c[:6])) + ("c" if c[6] else "") + ("l" if c[7] else ""))
 def test_attention_large(eng, case):
     test_attention(eng, case)
+
+
+def test_attention_large_scores(eng):
+    """Scores of hundreds on parts: the maximum moves by more than its slack."""
+    case = (1, 1024, 1024, 8, 8, 64, True, None)
+    q, k, v, dy = attention_inputs(case, 63)
+    k *= np.linspace(0.2, 4, 1024, dtype=np.float32)[None, :, None, None]  # later keys score higher
+    ts = [dev(eng, a, True) for a in (q, k, v)]
+    out = eng.attention(*ts, causal=True, scale=1.0)
+    out.backward(dev(eng, dy))
+    ref = [torch.tensor(a, dtype=torch.float64, requires_grad=True) for a in (q, k, v)]
+    o, s_max = attend64(*ref, True, 1.0, None)
+    o.backward(torch.tensor(dy, dtype=torch.float64))
+    tol = attention_tol(case, s_max)
+    assert s_max > 100 and rel_max(out.sync(), o.detach().numpy()) <= tol
+    for t, r in zip(ts, ref):
+        assert rel_max(t.grad.sync(), r.grad.numpy()) <= 4 * tol
+    eng.end_batch()
 
 
 @pytest.mark.parametrize("change", ["rows", "tiles", "tiny", "huge", "grads"])
