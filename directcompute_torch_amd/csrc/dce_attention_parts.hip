@@ -16,10 +16,17 @@
 // score into base 2 anyway, and where a sum goes over tiles of different
 // exponents (over V's in the forward, dO's and Q's for dV and dK) its terms are
 // brought to the smallest exponent so far, which the exponential's offset takes.
+// That costs a tile of smaller vectors bits of P, seen only where a row (or key)
+// gives the larger ones no weight: P = 1 has 32 bits in the forward before the
+// first is lost, some 33 in dS.  Problems whose V tiles differ by more than 2^8
+// (backward: V's and K's together by 2^12, or Q's and dO's by 2^20, which 1 / l
+// of causal rows makes T of; 24, 21 and 13 bits at the least) run on fp32 too.
 //
 // P is relative to its row's maximum, within [0, 1], and kept as 2^14 P.  The
 // forward only follows its running maximum, and scales the sums so far, where a
-// score passes it by more than 2^8: its P is at most 2^8, kept as 2^7 P.  The
+// score passes it by more than 2^8: its P is at most 2^8, kept as 2^7 P.  P's
+// parts end at 2^-39 (forward: 2^-32), which is an error of P relative to the
+// row's largest; a key to which every row gives less gets dK = dV = 0.  The
 // backward's 1 / l goes into dO (dO' = dO / l) when that is split, so that
 // dV = P^T dO' and dS = scale P (dO' V^T - delta'), delta' = rowsum(dO' * O).
 // delta' is of the size of the largest vector that a row sees, whatever tile it
@@ -40,6 +47,8 @@ constexpr int kRangeGrad = 60;    // and of gradients
 constexpr float kSlack = 8.f;     // of the forward's running maximum, in powers of 2
 constexpr int kExpP = 7;          // the forward's P parts hold p 2^7, p up to 2^kSlack
 constexpr float kWide = 16384.f;  // largest ratio of the vectors' sizes in a tile
+constexpr int kZeros = 15 + kRange, kZerosGrad = 15 + kRangeGrad;  // exponents of tiles of zeros, larger than any other
+constexpr float kSpread = 8.f, kSpreadKeys = 12.f, kSpreadRows = 20.f;  // of the tiles' exponents
 
 using h2 = _Float16 __attribute__((ext_vector_type(2)));
 using h4 = _Float16 __attribute__((ext_vector_type(4)));
@@ -70,16 +79,51 @@ struct Parts {
   float* dl;  // delta' 2^e of dO's tile, [problem][q.pad]
 };
 constexpr int kBad = 1 << 20;
-// Has problem pr a tile that parts do not suit?  For all threads of the workgroup.
+// Does problem pr have a tile that parts do not suit, or tiles of too different
+// sizes?  For all threads of the workgroup.
 template <bool BWD>
 __device__ __forceinline__ bool unsuited(const Parts& ps, uint32_t pr) {
+  __shared__ float ends[8][8];
   const uint32_t nq = ps.q.pad / kRows, nk = ps.k.pad / kRows;
-  bool bad = false;
-  for (uint32_t t = threadIdx.x; t < max(nq, nk); t += blockDim.x) {
-    if (t < nq) bad |= ps.q.e[size_t(pr) * nq + t] == kBad || (BWD && ps.y.e[size_t(pr) * nq + t] == kBad);
-    if (t < nk) bad |= ps.k.e[size_t(pr) * nk + t] == kBad || ps.v.e[size_t(pr) * nk + t] == kBad;
+  // largest and smallest exponents of v, k, q, dO
+  float hi[4], lo[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) hi[i] = -1000.f, lo[i] = 1000.f;
+  auto take = [&](int i, const int* e, uint32_t n, int zeros) {
+    for (uint32_t t = threadIdx.x; t < n; t += blockDim.x) {
+      const int x = e[size_t(pr) * n + t];
+      if (x == zeros) continue;
+      hi[i] = fmaxf(hi[i], float(x));
+      lo[i] = fminf(lo[i], float(x));
+    }
+  };
+  take(0, ps.v.e, nk, kZeros);
+  take(1, ps.k.e, nk, kZeros);
+  take(2, ps.q.e, nq, kZeros);
+  if (BWD) take(3, ps.y.e, nq, kZerosGrad);
+  const uint32_t wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < (BWD ? 4 : 3); ++i) {
+    hi[i] = wave_reduce(hi[i], OpMaxR());
+    lo[i] = -wave_reduce(-lo[i], OpMaxR());
+    if ((threadIdx.x & 63) == 0) {
+      ends[wave][i] = hi[i];
+      ends[wave][4 + i] = lo[i];
+    }
   }
-  return __syncthreads_or(bad);
+  __syncthreads();
+  float spread[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < (BWD ? 4 : 3); ++i) {
+    for (uint32_t w = 0; w < blockDim.x / 64; ++w) {
+      hi[i] = fmaxf(hi[i], ends[w][i]);
+      lo[i] = fminf(lo[i], ends[w][4 + i]);
+    }
+    if (hi[i] >= float(kBad)) return true;
+    spread[i] = fmaxf(hi[i] - lo[i], 0.f);  // 0: only zeros
+  }
+  if (!BWD) return spread[0] > kSpread;
+  return spread[0] + spread[1] > kSpreadKeys || spread[2] + spread[3] > kSpreadRows;
 }
 // The least exponent of V's tiles [from, to), in every lane.
 __device__ __forceinline__ int least_of(const int* ev, uint32_t from, uint32_t to, int lane) {
@@ -170,7 +214,7 @@ __device__ __forceinline__ void split_tile(const Attn& a, const Part& P, const P
     const float least = -wave_reduce(mine ? -__uint_as_float(mine) : -INFINITY, OpMaxR());
     if (threadIdx.x == 0) {
       constexpr int range = W == GRAD ? kRangeGrad : kRange;
-      int e = 14 + range;  // zeros: no smaller than another tile's
+      int e = W == GRAD ? kZerosGrad : kZeros;
       if (most > 0.f) {
         const bool bad = !(most < pow2(range)) || most < pow2(-range) || most > kWide * least;
         e = bad ? kBad : 14 + 127 - int(__float_as_uint(most) >> 23);
@@ -464,7 +508,7 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
 }
 
 // dS's parts: p (at most 2^14) times dP - delta (at most 2^(31 + log2 DP)) times
-// 2^-kDown lies below 2^15.
+// 2^-down_bits lies below 2^15.
 template <int DP>
 constexpr int down_bits() {
   return 30 + (DP <= 32 ? 5 : DP <= 64 ? 6 : 7);

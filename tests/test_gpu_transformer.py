@@ -686,3 +686,44 @@ def test_attention_large_not_finite(eng):
     # dim by dim: an infinite value is in every later sum
     assert not np.isfinite(out[1, 500:, 3]).any() and np.isfinite(out[1, :480, 3]).all()
     eng.end_batch()
+
+
+@pytest.mark.parametrize("apart", [2.0 ** 6, 2.0 ** 24])
+@pytest.mark.parametrize("change", ["values", "gradients"])
+def test_attention_large_ignored_vectors(eng, change, apart):
+    """Large values that no row gives any weight, and large gradients of rows
+    that give a key none, cost the others nothing.  Each result is off by
+    attention_tol of its own terms' sizes."""
+    case = (1, 1024, 1024, 8, 8, 64, False, None)
+    q, k, v, dy = attention_inputs(case, 64)
+    first = np.arange(1024) < 512
+    q[..., 0] = 8
+    if change == "values":           # scores of -60 for the first half
+        k[..., 0] = np.where(first, -60, 0)[None, :, None]
+        v[:, first] *= np.float32(apart)
+    else:                            # 40 for a row's own half, -40 for the other
+        q[:, ~first, :, 0] = -8
+        k[..., 0] = np.where(first, 40, -40)[None, :, None]
+        dy[:, first] *= np.float32(apart)
+    ts = [dev(eng, a, True) for a in (q, k, v)]
+    out = eng.attention(*ts)
+    out.backward(dev(eng, dy))
+    ref = [torch.tensor(a, dtype=torch.float64, requires_grad=True) for a in (q, k, v)]
+    o, s_max = attend64(*ref, False, 64 ** -0.5, None)
+    o.backward(torch.tensor(dy, dtype=torch.float64))
+    tol = attention_tol(case, s_max)
+    qa, ka, va, ya = (torch.tensor(a, dtype=torch.float64).permute(0, 2, 1, 3) for a in (q, k, v, dy))
+    p = torch.softmax(qa @ ka.transpose(2, 3) / 8, -1)
+    big = lambda t: t.abs().amax(-1, keepdim=True)  # noqa: E731
+    dp = ya.abs() @ va.abs().transpose(2, 3)
+    ds = p * (dp + (p * dp).sum(-1, keepdim=True)) / 8
+    size = [p @ big(va), ds @ big(ka), ds.transpose(2, 3) @ big(qa), p.transpose(2, 3) @ big(ya)]
+    # keys to which no row gives 2^-60 of its weight have results of no size
+    for i, (got, want, z) in enumerate(zip([out.sync()] + [t.grad.sync() for t in ts],
+                                           [o.detach()] + [t.grad for t in ref], size)):
+        z = z.permute(0, 2, 1, 3).numpy()
+        z = np.maximum(z, z.max() * 2.0 ** -60)
+        e = np.abs(got - want.numpy()).max(-1, keepdims=True)
+        print(change, "%.2g of the terms' size, tol %.2g" % ((e / z).max(), (4 if i else 1) * tol), flush=True)
+        assert (e <= (4 if i else 1) * tol * z).all()
+    eng.end_batch()
