@@ -580,7 +580,7 @@ bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* row
                 const float* stepSizes, uint32_t n, float mu, bool nesterov, float decay, float clip,
                 uint32_t steps) {
   std::vector<Mat> all;
-  std::set<const void*> written;
+  std::set<const void*> written, read;
   double bytes = 0, flops = 0;
   for (uint32_t i = 0; i < n; ++i) {
     if (!params[i] || !grads[i]) continue;
@@ -597,6 +597,7 @@ bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* row
       set_error("MuonBatch: the parameter or momentum of matrix %u is another one's too", i);
       return false;
     }
+    read.insert(G);
     Mat m{};
     m.w = W->ptr;
     m.g = G->ptr;
@@ -615,6 +616,11 @@ bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* row
     flops += steps * (3.0 * m.m * m.m * m.n + double(m.m) * m.m * m.m);
   }
   if (all.empty()) return true;
+  for (const void* g : read)
+    if (written.count(g)) {
+      set_error("MuonBatch: a gradient is a parameter or momentum too");
+      return false;
+    }
   ProfScope prof("muon", flops, bytes);
   // Groups of up to kMaxM matrices, and of up to 2^28 values unless one is larger.
   // Tiles by the operations of a step (us on 128 / on 64): 1024 x 1024 435 / 281,

@@ -1255,10 +1255,11 @@ class Muon(_Optimizer):
 
     def __init__(self, params, lr=0.001, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, rms=0.2,
                  betas=(0.9, 0.999), eps=1e-8):
+        params = list(params)
         super().__init__([p for p in params if len(p.shape) >= 2], lr)
         if not 1 <= steps <= 20:
             raise ValueError(f"Muon: {steps} steps (1 to 20)")
-        self.matrices, self.params = self.params, list(params)
+        self.matrices, self.params = self.params, params
         self.momentum, self.nesterov, self.weight_decay = momentum, nesterov, weight_decay
         self.steps, self.rms = steps, rms
         self.m = [Tensor(np.zeros(p.shape, np.float32), track=False) for p in self.matrices]

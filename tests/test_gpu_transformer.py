@@ -727,3 +727,23 @@ def test_attention_large_ignored_vectors(eng, change, apart):
         print(change, "%.2g of the terms' size, tol %.2g" % ((e / z).max(), (4 if i else 1) * tol), flush=True)
         assert (e <= (4 if i else 1) * tol * z).all()
     eng.end_batch()
+
+
+def test_muon_gradient_that_is_written(eng):
+    a, b = (dev(eng, np.ones((6, 5)), True) for _ in range(2))
+    opt = eng.Muon([a, b])
+    a.grad, b.grad = dev(eng, np.ones((6, 5))), opt.m[0]
+    with pytest.raises(RuntimeError, match="gradient is a parameter or momentum"):
+        opt.step()
+    assert np.array_equal(a.sync(), np.ones((6, 5), np.float32))
+    b.grad = a.grad                  # one gradient for two parameters is fine
+    opt.step()
+    assert np.array_equal(a.sync(), b.sync()) and np.isfinite(a.sync()).all()
+
+
+def test_muon_takes_any_iterable(eng):
+    w, bias = dev(eng, np.ones((4, 3)), True), dev(eng, np.ones(3), True)
+    opt = eng.Muon(p for p in (w, bias))
+    w.grad, bias.grad = dev(eng, np.ones((4, 3))), dev(eng, np.ones(3))
+    opt.step()
+    assert opt.params == [w, bias] and (w.sync() != 1).all() and (bias.sync() != 1).all()
