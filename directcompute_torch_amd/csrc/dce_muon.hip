@@ -52,8 +52,9 @@ struct Mat {
   float *w, *g, *mom;
   uint32_t m, n, mp, np;  // padded to whole tiles (zeros)
   uint32_t tall, splits;
+  uint32_t chunk, chunks, sums;  // values of a momentum workgroup, their number, their sums' place
   float step;
-  uint32_t x, xp, xt[2], a, b, part;  // places in the workspace, in units of 64 floats
+  uint32_t x, xp, xt0, xt1, a, b, part;  // places in the workspace, in units of 64 floats
 };
 struct Mats {
   Mat t[kMaxM];
@@ -89,16 +90,17 @@ __device__ __forceinline__ void put8(float* row, uint32_t k, const float* x, flo
 
 // ---------------------------------------------------------------------------
 // d = g + mu m, m <- mu m + g, and the sums of d^2 (in double, one per
-// workgroup of 4096 values); d goes to X's place, as the caller's matrix lies.
+// workgroup: 4096 values, more where that would be over 1024 of them); d goes to
+// X's place, as the caller's matrix lies.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kChunk = 4096;
+constexpr uint32_t kChunk = 4096, kMaxChunks = 1024;
 __global__ void __launch_bounds__(kT)
     k_muon_momentum(const Mats t, float* ws, double* sums, float mu, float clip, int nesterov) {
   __shared__ double sh[4];
   const int i = find_mat(t, blockIdx.x);
-  const Mat& M = t.t[i];
-  const uint32_t n = M.m * M.n, c0 = (blockIdx.x - t.start[i]) * kChunk;
-  float* d = at(ws, M.xt[1]);  // free until the first step
+  const Mat M = t.t[i];
+  const uint32_t id = blockIdx.x - t.start[i], n = M.m * M.n, end = min(n, (id + 1) * M.chunk);
+  float* d = at(ws, M.xt1);  // free until the first step
   double sum = 0;
   auto one = [&](float g, float& m) {
     if (g > clip) g = clip;
@@ -108,7 +110,8 @@ __global__ void __launch_bounds__(kT)
     sum += double(v) * v;
     return v;
   };
-  if (c0 + kChunk <= n) {
+  uint32_t c0 = id * M.chunk;
+  for (; c0 + kChunk <= end; c0 += kChunk) {
     f4 G[4], V[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -128,26 +131,26 @@ __global__ void __launch_bounds__(kT)
       *reinterpret_cast<f4*>(M.mom + k) = V[j];
       *reinterpret_cast<f4*>(d + k) = G[j];
     }
-  } else {
-#pragma unroll 4
-    for (uint32_t k = c0 + threadIdx.x; k < n; k += kT) {
-      float m = M.mom[k];
-      d[k] = one(M.g[k], m);
-      M.mom[k] = m;
+  }
+  if (c0 < end) {  // the loads ahead of everything that depends on them
+    constexpr int W = kChunk / kT;
+    float G[W], V[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const uint32_t k = min(c0 + j * kT + threadIdx.x, end - 1);
+      G[j] = M.g[k];
+      V[j] = M.mom[k];
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const uint32_t k = c0 + j * kT + threadIdx.x;
+      if (k >= end) break;
+      d[k] = one(G[j], V[j]);
+      M.mom[k] = V[j];
     }
   }
   sum = block_sum256(sum, sh);
-  if (threadIdx.x == 0) sums[blockIdx.x] = sum;
-}
-
-// 1 / (|d| + eps) of each matrix.
-__global__ void __launch_bounds__(kT) k_muon_norm(const Mats t, const double* sums, float* inv) {
-  __shared__ double sh[4];
-  const uint32_t i = blockIdx.x;
-  double s = 0;
-  for (uint32_t k = t.start[i] + threadIdx.x; k < t.start[i + 1]; k += kT) s += sums[k];
-  s = block_sum256(s, sh);
-  if (threadIdx.x == 0) inv[i] = float(1.0 / (sqrt(s) + 1e-7));
+  if (threadIdx.x == 0) sums[M.sums + id] = sum;
 }
 
 // A 64 x 64 tile through LDS: X in fp32 and as parts, along rows and columns.
@@ -172,22 +175,40 @@ __device__ __forceinline__ void put_tile(const float (&S)[kSq * kPitch], float* 
     }
   }
 }
-__global__ void __launch_bounds__(kT) k_muon_scale(const Mats t, float* ws, const float* inv) {
+__global__ void __launch_bounds__(kT) k_muon_scale(const Mats t, float* ws, const double* sums) {
   __shared__ float S[kSq * kPitch];
+  __shared__ double sh[4];
+  __shared__ float norm[1];
   const int i = find_mat(t, blockIdx.x);
-  const Mat& M = t.t[i];
+  const Mat M = t.t[i];
   const uint32_t tn = M.np / kSq, id = blockIdx.x - t.start[i], i0 = id / tn * kSq, j0 = id % tn * kSq;
-  const float by = inv[i];
-  const float* d = at(ws, M.xt[1]);
+  const float* d = at(ws, M.xt1);
   float* x = at(ws, M.x);
+  const uint32_t si = M.tall ? 1 : M.n, sj = M.tall ? M.m : 1;
   float v[kSq * kSq / kT];
+  // Loads of clamped places: behind a branch each would wait for the one before.
 #pragma unroll
   for (int u = 0; u < kSq * kSq / kT; ++u) {
     const uint32_t s = threadIdx.x + kT * u;
     // consecutive threads along the caller's rows
-    const uint32_t r = M.tall ? s % kSq : s / kSq, c = M.tall ? s / kSq : s % kSq, mi = i0 + r, nj = j0 + c;
-    const bool ok = mi < M.m && nj < M.n;
-    v[u] = ok ? d[M.tall ? size_t(nj) * M.m + mi : size_t(mi) * M.n + nj] * by : 0.f;
+    const uint32_t r = M.tall ? s % kSq : s / kSq, c = M.tall ? s / kSq : s % kSq;
+    v[u] = d[min(i0 + r, M.m - 1) * si + min(j0 + c, M.n - 1) * sj];
+  }
+  // 1 / (|d| + eps), which every workgroup works out again: a launch less
+  double sum = 0;
+#pragma unroll
+  for (uint32_t k = 0; k < kMaxChunks / kT; ++k) {
+    const double more = sums[M.sums + min(k * kT + threadIdx.x, M.chunks - 1)];
+    sum += k * kT + threadIdx.x < M.chunks ? more : 0.0;
+  }
+  sum = block_sum256(sum, sh);
+  if (threadIdx.x == 0) norm[0] = float(1.0 / (sqrt(sum) + 1e-7));
+  __syncthreads();
+  const float by = norm[0];
+#pragma unroll
+  for (int u = 0; u < kSq * kSq / kT; ++u) {
+    const uint32_t s = threadIdx.x + kT * u, r = M.tall ? s % kSq : s / kSq, c = M.tall ? s / kSq : s % kSq;
+    v[u] = i0 + r < M.m && j0 + c < M.n ? v[u] * by : 0.f;
   }
 #pragma unroll
   for (int u = 0; u < kSq * kSq / kT; ++u) {
@@ -200,7 +221,7 @@ __global__ void __launch_bounds__(kT) k_muon_scale(const Mats t, float* ws, cons
     const uint32_t s = threadIdx.x + kT * u, r = s / (kSq / 4), c = s % (kSq / 4) * 4;
     *reinterpret_cast<f4*>(x + size_t(i0 + r) * M.np + j0 + c) = *reinterpret_cast<const f4*>(S + r * kPitch + c);
   }
-  put_tile(S, at(ws, M.xp), M.np, at(ws, M.xt[0]), M.mp, i0, j0);
+  put_tile(S, at(ws, M.xp), M.np, at(ws, M.xt0), M.mp, i0, j0);
 }
 
 // ---------------------------------------------------------------------------
@@ -257,7 +278,7 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2)))
   __shared__ __attribute__((aligned(16))) char S[L::BYTES];
   const uint32_t blk = xcd_block_id();
   const int mi = find_mat(t, blk);
-  const Mat& M = t.t[mi];
+  const Mat M = t.t[mi];
   uint32_t id = blk - t.start[mi], ti, tj, sp = 0;
   const uint32_t tm = M.mp / BLK;
   uint32_t end = OP == GRAM ? M.np : M.mp, k0 = 0;
@@ -275,7 +296,7 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2)))
     tj = id / tm;
   }
   const float* P = at(ws, OP == GRAM ? M.xp : OP == POLY ? M.a : M.b);
-  const float* Q = at(ws, OP == GRAM ? M.xp : OP == POLY ? M.a : M.xt[cur]);
+  const float* Q = at(ws, OP == GRAM ? M.xp : OP == POLY ? M.a : cur ? M.xt1 : M.xt0);
   const uint32_t pitch = OP == GRAM ? M.np : M.mp;
   BRes bp, bq;
   bp.init(P + size_t(ti) * BLK * pitch, BLK * pitch);
@@ -418,25 +439,25 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2)))
   __syncthreads();
   if constexpr (OP == LAST) {  // w <- w - decay w - step X, along the caller's rows
     constexpr int W = 8;
+    const uint32_t si = M.tall ? 1 : M.n, sj = M.tall ? M.m : 1;
 #pragma unroll 1
     for (int u = 0; u < BLK * BLK / kT; u += W) {
       float w[W];
 #pragma unroll
-      for (int e = 0; e < W; ++e) {
+      for (int e = 0; e < W; ++e) {  // of clamped places, as in k_muon_scale
         const uint32_t s = threadIdx.x + kT * (u + e), r = M.tall ? s % BLK : s / BLK, c = M.tall ? s / BLK : s % BLK;
-        const size_t i = M.tall ? size_t(j0 + c) * M.m + i0 + r : size_t(i0 + r) * M.n + j0 + c;
-        w[e] = i0 + r < M.m && j0 + c < M.n ? M.w[i] : 0.f;
+        w[e] = M.w[min(i0 + r, M.m - 1) * si + min(j0 + c, M.n - 1) * sj];
       }
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         const uint32_t s = threadIdx.x + kT * (u + e), r = M.tall ? s % BLK : s / BLK, c = M.tall ? s / BLK : s % BLK;
-        const size_t i = M.tall ? size_t(j0 + c) * M.m + i0 + r : size_t(i0 + r) * M.n + j0 + c;
-        if (i0 + r < M.m && j0 + c < M.n) M.w[i] = w[e] - decay * w[e] - M.step * C[r * CP + c];
+        const float next = w[e] - decay * w[e] - M.step * C[r * CP + c];
+        if (i0 + r < M.m && j0 + c < M.n) M.w[(i0 + r) * si + (j0 + c) * sj] = next;
       }
     }
     return;
   }
-  float* tr = OP == APPLY ? at(ws, M.xt[cur ^ 1]) : out;
+  float* tr = OP == APPLY ? at(ws, cur ? M.xt0 : M.xt1) : out;
 #pragma unroll UNROLL
   for (int u = 0; u < BLK * BLK / 8 / kT; ++u) {
     const uint32_t slot = threadIdx.x + kT * u, r = slot % BLK, k = slot / BLK * 8;
@@ -454,7 +475,7 @@ __global__ void __launch_bounds__(kT) k_muon_sum(const Mats t, float* ws) {
   constexpr int RW = 16, CP = BLK + 4, PIECES = BLK / RW;
   __shared__ float C[RW * CP];
   const int mi = find_mat(t, blockIdx.x);
-  const Mat& M = t.t[mi];
+  const Mat M = t.t[mi];
   const uint32_t id = blockIdx.x - t.start[mi], piece = id % PIECES, tile = id / PIECES, tm = M.mp / BLK;
   const uint32_t tiles = tm * (tm + 1) / 2;
   uint32_t ti, tj;
@@ -529,7 +550,7 @@ bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32
   }
   const double most = std::max(256.0, all / (4.0 * num_cus()));
   Places at;
-  size_t chunks = 0;
+  uint32_t chunks = 0;
   bool split = false;
   for (uint32_t i = 0; i < t.count; ++i) {
     Mat& m = t.t[i];
@@ -538,24 +559,26 @@ bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32
     const size_t xn = size_t(m.mp) * m.np, an = size_t(m.mp) * m.mp;
     m.x = at.take(xn);
     m.xp = at.take(xn);
-    m.xt[0] = at.take(xn);
-    m.xt[1] = at.take(xn);
+    m.xt0 = at.take(xn);
+    m.xt1 = at.take(xn);
     m.a = at.take(an);
     m.b = at.take(an);
     m.part = m.splits > 1 ? at.take(size_t(m.splits) * tri(m) * BLK * BLK) : 0;
-    chunks += cdiv(size_t(m.m) * m.n, kChunk);
+    const size_t size = size_t(m.m) * m.n;
+    m.chunk = cdiv(cdiv(size, kMaxChunks), kChunk) * kChunk;
+    m.chunks = cdiv(size, m.chunk);
+    m.sums = chunks;
+    chunks += m.chunks;
   }
-  const size_t sums = at.take(2 * chunks), inv = at.take(kMaxM);
+  const size_t sums = at.take(size_t(2) * chunks);
   float* ws = workspace(at.next * 64);
   if (!ws) return false;
   double* dsum = reinterpret_cast<double*>(ws + sums * 64);
-  float* dinv = ws + inv * 64;
 
-  uint32_t n = blocks(t, [](const Mat& m) { return cdiv(size_t(m.m) * m.n, kChunk); });
+  uint32_t n = blocks(t, [](const Mat& m) { return m.chunks; });
   hipLaunchKernelGGL(k_muon_momentum, dim3(n), dim3(kT), 0, stream(), t, ws, dsum, mu, clip, int(nesterov));
-  hipLaunchKernelGGL(k_muon_norm, dim3(t.count), dim3(kT), 0, stream(), t, dsum, dinv);
   n = blocks(t, [](const Mat& m) { return m.mp / kSq * (m.np / kSq); });
-  hipLaunchKernelGGL(k_muon_scale, dim3(n), dim3(kT), 0, stream(), t, ws, dinv);
+  hipLaunchKernelGGL(k_muon_scale, dim3(n), dim3(kT), 0, stream(), t, ws, dsum);
   for (uint32_t s = 0; s < steps; ++s) {
     n = blocks(t, [&](const Mat& m) { return tri(m) * m.splits; });
     hipLaunchKernelGGL((k_muon_product<GRAM, BLK>), dim3(n), dim3(kT), 0, stream(), t, ws, s & 1, decay);
