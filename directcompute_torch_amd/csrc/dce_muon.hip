@@ -328,8 +328,34 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2)))
       for (int e = 0; e < 2; ++e) f[i][e] = L::frag(St, w + 32 * i + col, 2 * (2 * kk + half) + e);
   };
 
+  // What the epilogue reads, in flight with the operands where registers allow.
+  constexpr bool EARLY = BLK == 64;
+  constexpr int NU = BLK * BLK / 8 / kT, NW = EARLY && OP == LAST ? BLK * BLK / kT : 1;
+  const uint32_t i0 = ti * BLK, j0 = tj * BLK;
+  f4 x0[EARLY ? NU : 1], x1[EARLY ? NU : 1];
+  float w0[NW];
+  auto epilogue_loads = [&](int u, f4& a, f4& b) {
+    const uint32_t slot = threadIdx.x + kT * u, r = slot / (BLK / 8), k = slot % (BLK / 8) * 8;
+    const float* p = OP == POLY ? at(ws, M.a) + size_t(i0 + r) * M.mp : at(ws, M.x) + size_t(i0 + r) * M.np;
+    a = reinterpret_cast<const f4*>(p + j0 + k)[0];
+    b = reinterpret_cast<const f4*>(p + j0 + k)[1];
+  };
+  // Consecutive threads along the caller's rows; of clamped places, as in k_muon_scale.
+  const uint32_t si = M.tall ? 1 : M.n, sj = M.tall ? M.m : 1;
+  auto weight = [&](int u) {
+    const uint32_t s = threadIdx.x + kT * u, r = M.tall ? s % BLK : s / BLK, c = M.tall ? s / BLK : s % BLK;
+    return M.w[min(i0 + r, M.m - 1) * si + min(j0 + c, M.n - 1) * sj];
+  };
   L::load(bp, pitch * 4, k0, end, S);
   L::load(bq, pitch * 4, k0, end, S + L::STAGE);
+  if constexpr (EARLY && OP != GRAM) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) epilogue_loads(u, x0[u], x1[u]);
+  }
+  if constexpr (EARLY && OP == LAST) {
+#pragma unroll
+    for (int u = 0; u < NW; ++u) w0[u] = weight(u);
+  }
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   if constexpr (BLK == 128) {
@@ -388,7 +414,6 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2)))
         C[(wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3)) * CP + wn + 32 * j + col] =
             (big[i][j][e] + small[i][j][e]) * unit;
   __syncthreads();
-  const uint32_t i0 = ti * BLK, j0 = tj * BLK;
   if constexpr (OP == GRAM) {
     if (M.splits > 1) {  // summed by k_muon_sum
       float* out = at(ws, M.part) + (size_t(sp) * (tm * (tm + 1) / 2) + id) * (BLK * BLK);
@@ -403,29 +428,34 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2)))
   constexpr int UNROLL = BLK == 128 ? 1 : 2;
   float* out = at(ws, OP == GRAM ? M.a : OP == POLY ? M.b : M.xp);
 #pragma unroll UNROLL
-  for (int u = 0; u < BLK * BLK / 8 / kT; ++u) {
+  for (int u = 0; u < NU; ++u) {
     const uint32_t slot = threadIdx.x + kT * u, r = slot / (BLK / 8), k = slot % (BLK / 8) * 8;
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = C[r * CP + k + e];
+    f4 p = {0.f, 0.f, 0.f, 0.f}, q = p;
+    if constexpr (EARLY && OP != GRAM) {
+      p = x0[u];
+      q = x1[u];
+    } else if constexpr (OP != GRAM) {
+      epilogue_loads(u, p, q);
+    }
     if constexpr (OP == POLY) {  // B = b A + c A^2
-      const h8* a = reinterpret_cast<const h8*>(at(ws, M.a) + size_t(i0 + r) * M.mp + j0 + k);
-      const h8 ah = a[0], al = a[1];
+      const h8 ah = __builtin_bit_cast(h8, p), al = __builtin_bit_cast(h8, q);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         v[e] = kB * ((float(ah[e]) + float(al[e])) * ldexpf(1.f, -kExpA)) + kC * v[e];
     }
     if constexpr (OP == APPLY || OP == LAST) {  // X <- a X + B X
-      float* x = at(ws, M.x) + size_t(i0 + r) * M.np + j0 + k;
-      f4 x0 = reinterpret_cast<const f4*>(x)[0], x1 = reinterpret_cast<const f4*>(x)[1];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        v[e] = x0[e] = kA * x0[e] + v[e];
-        v[4 + e] = x1[e] = kA * x1[e] + v[4 + e];
+        v[e] = p[e] = kA * p[e] + v[e];
+        v[4 + e] = q[e] = kA * q[e] + v[4 + e];
       }
       if constexpr (OP == APPLY) {
-        reinterpret_cast<f4*>(x)[0] = x0;
-        reinterpret_cast<f4*>(x)[1] = x1;
+        float* x = at(ws, M.x) + size_t(i0 + r) * M.np + j0 + k;
+        reinterpret_cast<f4*>(x)[0] = p;
+        reinterpret_cast<f4*>(x)[1] = q;
       }
     }
     if constexpr (OP != LAST)
@@ -438,16 +468,12 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2)))
   if ((OP == GRAM || OP == POLY) && ti == tj) return;
   __syncthreads();
   if constexpr (OP == LAST) {  // w <- w - decay w - step X, along the caller's rows
-    constexpr int W = 8;
-    const uint32_t si = M.tall ? 1 : M.n, sj = M.tall ? M.m : 1;
+    constexpr int W = EARLY ? NW : 8;
 #pragma unroll 1
     for (int u = 0; u < BLK * BLK / kT; u += W) {
       float w[W];
 #pragma unroll
-      for (int e = 0; e < W; ++e) {  // of clamped places, as in k_muon_scale
-        const uint32_t s = threadIdx.x + kT * (u + e), r = M.tall ? s % BLK : s / BLK, c = M.tall ? s / BLK : s % BLK;
-        w[e] = M.w[min(i0 + r, M.m - 1) * si + min(j0 + c, M.n - 1) * sj];
-      }
+      for (int e = 0; e < W; ++e) w[e] = EARLY ? w0[e] : weight(u + e);
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         const uint32_t s = threadIdx.x + kT * (u + e), r = M.tall ? s % BLK : s / BLK, c = M.tall ? s / BLK : s % BLK;
