@@ -93,7 +93,6 @@ __global__ void __launch_bounds__(kT, DP <= 128 ? 2 : 1) k_attn_few(const Attn a
   const uint32_t n = col, len = keys_of(a, b), lim = n < a.N ? limit_of(a, n, len) : 0u;
   const uint32_t least = limit_of(a, 0, len), most = limit_of(a, a.N - 1, len);
   f4 q[NI];
-  load_frag<DP, VEC>(a.q + (n < a.N ? q_at(a, b, gh, n) : 0), n < a.N, a.D, g, q);
   f4 o[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
@@ -106,6 +105,7 @@ __global__ void __launch_bounds__(kT, DP <= 128 ? 2 : 1) k_attn_few(const Attn a
     TL::template load<NT>(rows_view(a.v + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rv);
   };
   if (j0 < j1) fetch(j0);
+  load_frag<DP, VEC>(a.q + q_at(a, b, gh, min(n, a.N - 1)), true, a.D, g, q);
   for (uint32_t j = j0; j < j1; j += kFew) {
     __syncthreads();
     TL::store(Ks, rk);

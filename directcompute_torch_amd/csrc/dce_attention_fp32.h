@@ -11,21 +11,25 @@ constexpr int kKeys = 32;  // keys (rows in the dK / dV kernel) of an LDS tile
 __device__ __forceinline__ f4 mfma4(float a, float b, const f4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
-// A 16-lane fragment of vectors: lane group g takes dims 16 j + 4 g .. + 3.
+// A 16-lane fragment of vectors: lane group g takes dims 16 j + 4 g .. + 3; zeros
+// from D on and where not ok.  p is a vector in any case: the loads are of clamped
+// places, for behind a branch each could wait for the one before.
 template <int DP, bool VEC>
 __device__ __forceinline__ void load_frag(const float* p, bool ok, uint32_t D, int g, f4 (&r)[DP / 16]) {
 #pragma unroll
   for (int j = 0; j < DP / 16; ++j) {
     const uint32_t d = 16 * j + 4 * g;
-    r[j] = f4{0.f, 0.f, 0.f, 0.f};
     if constexpr (VEC) {
-      if (ok && d < D) r[j] = *reinterpret_cast<const f4*>(p + d);
+      r[j] = *reinterpret_cast<const f4*>(p + min(d, D - 4));
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (ok && d + e < D) r[j][e] = p[d + e];
+      for (int e = 0; e < 4; ++e) r[j][e] = p[min(d + e, D - 1)];
     }
   }
+#pragma unroll
+  for (int j = 0; j < DP / 16; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[j][e] = ok && 16 * j + 4 * g + e < D ? r[j][e] : 0.f;
 }
 
 template <int CH>
@@ -135,7 +139,6 @@ __device__ __forceinline__ void fwd_fp32(const Attn& a, uint32_t pr, uint32_t n0
   for (int t = 0; t < QT; ++t) {
     const uint32_t n = n0 + (wave * QT + t) * 16 + col;
     lim[t] = n < a.N ? limit_of(a, n, len) : 0u;
-    load_frag<DP, VEC>(a.q + (n < a.N ? q_at(a, b, gh, n) : 0), n < a.N, a.D, g, q[t]);
   }
   f4 o[QT][DP / 16];
   float m[QT], l[QT];
@@ -155,6 +158,11 @@ __device__ __forceinline__ void fwd_fp32(const Attn& a, uint32_t pr, uint32_t n0
     TL::load(rows_view(a.v + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rv);
   };
   if (j0 < j1) fetch(j0);
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const uint32_t n = n0 + (wave * QT + t) * 16 + col;
+    load_frag<DP, VEC>(a.q + q_at(a, b, gh, min(n, a.N - 1)), true, a.D, g, q[t]);
+  }
   for (uint32_t j = j0; j < j1; j += kKeys) {
     __syncthreads();
     TL::store(Ks, rk);
@@ -261,31 +269,23 @@ __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0,
   const uint32_t least = limit_of(a, n0, len), most = limit_of(a, min(n0 + ROWS, a.N) - 1, len);
   const uint32_t mine = wave_limit(a, n0 + wave * 16 * QT, 16 * QT, len);
 
-  f4 q[QT][DP / 16], dy[QT][DP / 16], dq[QT][DP / 16];
+  f4 q[QT][DP / 16], dy[QT][DP / 16], o[QT][DP / 16], dq[QT][DP / 16];
   uint32_t lim[QT];
   float m[QT], il[QT], delta[QT];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const uint32_t n = n0 + (wave * QT + t) * 16 + col;
-    const bool ok = n < a.N;
-    const size_t at = ok ? q_at(a, b, gh, n) : 0, row = size_t(pr) * a.N + n;
-    lim[t] = ok ? limit_of(a, n, len) : 0u;
-    m[t] = ok ? a.m[row] : 0.f;
-    il[t] = ok ? a.il[row] : 0.f;
-    load_frag<DP, VEC>(a.dy + at, ok, a.D, g, dy[t]);
-    load_frag<DP, VEC>(a.o + at, ok, a.D, g, q[t]);
-    float d = 0.f;
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) d += dy[t][i][e] * q[t][i][e];
-      dq[t][i] = f4{0.f, 0.f, 0.f, 0.f};
-    }
-    delta[t] = sum_g(d);
-    if (ok && g == 0) a.delta[row] = delta[t];
-    load_frag<DP, VEC>(a.q + at, ok, a.D, g, q[t]);
+    // Rows past the last are computed as it (without a branch, behind which every
+    // load would wait for the one before) and not written.
+    const uint32_t nn = min(n, a.N - 1);
+    const size_t at = q_at(a, b, gh, nn), row = size_t(pr) * a.N + nn;
+    lim[t] = limit_of(a, nn, len);
+    m[t] = a.m[row];
+    il[t] = a.il[row];
+    load_frag<DP, VEC>(a.dy + at, true, a.D, g, dy[t]);
+    load_frag<DP, VEC>(a.o + at, true, a.D, g, o[t]);
+    load_frag<DP, VEC>(a.q + at, true, a.D, g, q[t]);
   }
-  if (!a.dq) return;
   uint32_t j0, j1;
   split_keys(a, most, sp, j0, j1);
   const uint32_t stride = a.G * a.D;
@@ -295,7 +295,21 @@ __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0,
     TL::load(rows_view(a.k + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rk);
     TL::load(rows_view(a.v + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rv);
   };
-  if (j0 < j1) fetch(j0);
+  if (a.dq && j0 < j1) fetch(j0);
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const uint32_t n = n0 + (wave * QT + t) * 16 + col;
+    float d = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d += dy[t][i][e] * o[t][i][e];
+      dq[t][i] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    delta[t] = sum_g(d);
+    if (n < a.N && g == 0) a.delta[size_t(pr) * a.N + n] = delta[t];
+  }
+  if (!a.dq) return;
   for (uint32_t j = j0; j < j1; j += kKeys) {
     __syncthreads();
     TL::store(Ks, rk);
@@ -354,8 +368,9 @@ __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0,
 }
 
 // ---------------------------------------------------------------------------
-// dK, dV of NT / 4 keys (16 per wave, K and V in registers): tiles of query rows of every head that shares them through LDS: the sum over the
-// heads is part of the loop, in a fixed order.
+// dK, dV of NT / 4 keys (16 per wave, K and V in registers): tiles of query rows
+// of every head that shares them through LDS: the sum over the heads is part of
+// the loop, in a fixed order.
 // ---------------------------------------------------------------------------
 template <int DP, bool VEC, int NT>
 __device__ __forceinline__ void dkv_fp32(const Attn& a, uint32_t pr, uint32_t k0, uint32_t sp, float* Qs, float* Ys,
@@ -376,7 +391,7 @@ __device__ __forceinline__ void dkv_fp32(const Attn& a, uint32_t pr, uint32_t k0
   const uint32_t sees = first_row(a, k0);
   const size_t part = size_t(sp) * a.B * a.T * a.G * a.D;
   f4 rq[TL::LOADS], ry[TL::LOADS];
-  float st = 0.f;
+  float st[3] = {0.f, 0.f, 0.f};
   uint32_t lm = 0;
   auto fetch = [&](uint32_t n0) {
     // Row by row: they are not evenly spaced when heads share keys.  Rows that see
@@ -400,10 +415,12 @@ __device__ __forceinline__ void dkv_fp32(const Attn& a, uint32_t pr, uint32_t k0
           }
       }
     }
-    if (threadIdx.x < 3 * kKeys) {
-      const uint32_t w = threadIdx.x / kKeys, n = n0 + threadIdx.x % kKeys;
-      const float* src = w == 0 ? a.m : w == 1 ? a.il : a.delta;
-      st = n < a.N ? src[size_t(pr) * a.N + n] : 0.f;
+    if (threadIdx.x < kKeys) {
+      const uint32_t n = n0 + threadIdx.x;
+      const size_t row = size_t(pr) * a.N + min(n, a.N - 1);
+      st[0] = a.m[row];  // of rows past the last, which see nothing: any
+      st[1] = a.il[row];
+      st[2] = a.delta[row];
       lm = n < a.N ? limit_of(a, n, len) : 0u;
     }
   };
@@ -412,8 +429,11 @@ __device__ __forceinline__ void dkv_fp32(const Attn& a, uint32_t pr, uint32_t k0
     __syncthreads();
     TL::store(Qs, rq);
     TL::store(Ys, ry);
-    if (threadIdx.x < 3 * kKeys) St[threadIdx.x] = st;
-    if (threadIdx.x < kKeys) Lim[threadIdx.x] = lm;
+    if (threadIdx.x < kKeys) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) St[i * kKeys + threadIdx.x] = st[i];
+      Lim[threadIdx.x] = lm;
+    }
     __syncthreads();
     if (n0 + kKeys < end) fetch(n0 + kKeys);
     if (wave_limit(a, n0, kKeys, len) <= kw) continue;

@@ -150,39 +150,39 @@ __device__ __forceinline__ void split_tile(const Attn& a, const Part& P, const P
     dots[threadIdx.x] = 0.f;
   }
   __syncthreads();
-  float v[SLOTS][8];
+  float v[SLOTS][8], o[SLOTS][8], by_row[SLOTS];
   float part[SLOTS];
+  // Loads of clamped places: behind a branch each would wait for the one before.
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) {
+    const uint32_t slot = threadIdx.x + kT * i, d = slot % CH * 8, n = min(n0 + slot / CH, max(have, 1u) - 1);
+    const size_t at = ROWS ? q_at(a, b, g, n) : k_at(a, b, g, n);
+    const float* src = (W == QUERY ? a.q : W == KEY ? a.k : W == VALUE ? a.v : a.dy) + at;
+    by_row[i] = W == GRAD ? a.il[size_t(pr) * a.N + n] : 1.f;
+#pragma unroll
+    for (int e = 0; e < 8; e += VEC ? 4 : 1) {
+      const uint32_t k = min(d + e, a.D - (VEC ? 4 : 1));
+      if constexpr (VEC) {
+        *reinterpret_cast<f4*>(v[i] + e) = *reinterpret_cast<const f4*>(src + k);
+        if (W == GRAD) *reinterpret_cast<f4*>(o[i] + e) = *reinterpret_cast<const f4*>(a.o + at + k);
+      } else {
+        v[i][e] = src[k];
+        if (W == GRAD) o[i][e] = a.o[at + k];
+      }
+    }
+  }
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
     const uint32_t slot = threadIdx.x + kT * i, row = slot / CH, d = slot % CH * 8, n = n0 + row;
     part[i] = 0.f;
+    const bool live = row < kRows && n < have;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-    if (row >= kRows || n >= have) continue;
-    const size_t at = (ROWS ? q_at(a, b, g, n) : k_at(a, b, g, n)) + d;
-    const float* src = (W == QUERY ? a.q : W == KEY ? a.k : W == VALUE ? a.v : a.dy) + at;
-    const float by = W == GRAD ? a.il[size_t(pr) * a.N + n] : 1.f;
-    if constexpr (VEC) {
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-        if (d + 4 * hf < a.D) {
-          const f4 x = *reinterpret_cast<const f4*>(src + 4 * hf);
-          f4 o = {0.f, 0.f, 0.f, 0.f};
-          if (W == GRAD) o = *reinterpret_cast<const f4*>(a.o + at + 4 * hf);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[i][4 * hf + e] = x[e] * by;
-            if (W == GRAD) part[i] += x[e] * o[e];
-          }
-        }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (d + e < a.D) {
-          v[i][e] = src[e] * by;
-          if (W == GRAD) part[i] += src[e] * a.o[at + e];
-        }
+    for (int e = 0; e < 8; ++e) {
+      const bool ok = live && d + e < a.D;
+      if (W == GRAD) part[i] += ok ? v[i][e] * o[i][e] : 0.f;
+      v[i][e] = ok ? v[i][e] * by_row[i] : 0.f;
     }
+    if (!live) continue;
     float m = 0.f;
     bool fine = true;
 #pragma unroll
