@@ -88,17 +88,37 @@ inline double pairs_of(const AttnArgs& x) {
   return rows * last - rows * (rows - 1) / 2;
 }
 
-// Splits of the rows in a dK / dV kernel of `keys` keys per workgroup: where those
-// fill less than the CUs, and no less than eight row tiles each.
-inline uint32_t row_splits(const Attn& a, uint32_t keys) {
-  const uint32_t wgs = cdiv(a.T, keys) * a.B * a.G, cus = uint32_t(num_cus());
-  return wgs >= cus ? 1u : std::max(1u, std::min(cdiv(cus, wgs), cdiv(a.N, 8 * 32)));
+// Splits of a backward kernel's long side, `tiles` tiles of `us` microseconds each
+// for each of `wgs` workgroups: the number of least time, where workgroups take
+// the CUs in rounds (causal ones, longest first, fill them) and have some 8 us of
+// their own, and each split's shares are written and read at 4 TB/s by a launch more.  10 x 1169 tokens, 3
+// heads of 128 on one, 280 and 100 workgroups for 256 CUs: training 525 us with 1
+// and 3 splits, 472 with 2 and 5; 1 x 6000 tokens, 2 heads of 96, 658 and 496.
+inline uint32_t best_splits(double wgs, uint32_t tiles, double us, double shareBytes, bool causal) {
+  const double cus = num_cus();
+  uint32_t best = 1;
+  double least = INFINITY;
+  for (uint32_t s = 1; s <= std::min(64u, cdiv(tiles, 8)); ++s) {
+    const double one = tiles * us / s + 8;
+    double t = causal ? std::max(one, 0.5 * wgs * (tiles * us + s * 8) / cus + one / 2) : std::ceil(wgs * s / cus) * one;
+    if (s > 1) t += 5 + s * shareBytes * 2 / 4e6;
+    if (t < 0.97 * least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
 }
-
-// Splits of the keys in a dQ kernel of `rows` rows per workgroup, likewise.
+// Of the rows in a dK / dV kernel of `keys` keys per workgroup (64: on fp32, 128:
+// on parts), and of the keys in a dQ kernel of `rows` rows: a tile's time is about
+// proportional to the dims.
+inline uint32_t row_splits(const Attn& a, uint32_t keys) {
+  return best_splits(double(cdiv(a.T, keys)) * a.B * a.G, cdiv(a.N, 32), a.D * (keys == 64 ? 0.031 : 0.024),
+                     8.0 * a.B * a.T * a.G * a.D, a.causal);
+}
 inline uint32_t key_splits(const Attn& a, uint32_t rows) {
-  const uint32_t wgs = cdiv(a.N, rows) * a.B * a.G, cus = uint32_t(num_cus());
-  return wgs >= cus ? 1u : std::max(1u, std::min(cdiv(cus, wgs), cdiv(a.T, 8 * 32)));
+  return best_splits(double(cdiv(a.N, rows)) * a.B * a.G, cdiv(a.T, 32), a.D * (rows == 64 ? 0.023 : 0.02),
+                     4.0 * a.B * a.G * a.N * a.D, a.causal);
 }
 
 // Floats of the splits' shares of a backward, one kernel's after the other's.

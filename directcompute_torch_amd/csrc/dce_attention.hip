@@ -52,17 +52,20 @@ __global__ void __launch_bounds__(kT) k_attn_dkv(const Attn a) {
   dkv_fp32<DP, VEC, kT>(a, pr, tile * 64, sp, Qs, Ys, St, Lim);
 }
 
-// Gradients from the splits' shares (`values` of each, in a row), added in order.
+// Gradients from the splits' shares (`values` of each, in a row), added in order;
+// V: f4 or float.
+template <typename V>
 __global__ void __launch_bounds__(kT)
-    k_attn_sum(const float* pk, float* dk, const float* pv, float* dv, size_t values, uint32_t splits) {
+    k_attn_sum(const V* pk, V* dk, const V* pv, V* dv, size_t values, uint32_t splits) {
   const size_t i = size_t(blockIdx.x) * kT + threadIdx.x;
   if (i >= values) return;
-  float x = 0.f, y = 0.f;
-  for (uint32_t s = 0; s < splits; ++s) {
-    if (dk) x += pk[s * values + i];
+  V x = pk[i], y = dv ? pv[i] : x;
+#pragma unroll 4
+  for (uint32_t s = 1; s < splits; ++s) {
+    x += pk[s * values + i];
     if (dv) y += pv[s * values + i];
   }
-  if (dk) dk[i] = x;
+  dk[i] = x;
   if (dv) dv[i] = y;
 }
 
@@ -92,8 +95,8 @@ __global__ void __launch_bounds__(kT, DP <= 128 ? 2 : 1) k_attn_few(const Attn a
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t n = col, len = keys_of(a, b), lim = n < a.N ? limit_of(a, n, len) : 0u;
   const uint32_t least = limit_of(a, 0, len), most = limit_of(a, a.N - 1, len);
-  f4 q[NI];
-  f4 o[NI];
+  f4 q[NI], o[NI];
+  load_frag<DP, VEC>(a.q + q_at(a, b, gh, min(n, a.N - 1)), true, a.D, g, q);
 #pragma unroll
   for (int i = 0; i < NI; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
@@ -105,7 +108,6 @@ __global__ void __launch_bounds__(kT, DP <= 128 ? 2 : 1) k_attn_few(const Attn a
     TL::template load<NT>(rows_view(a.v + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rv);
   };
   if (j0 < j1) fetch(j0);
-  load_frag<DP, VEC>(a.q + q_at(a, b, gh, min(n, a.N - 1)), true, a.D, g, q);
   for (uint32_t j = j0; j < j1; j += kFew) {
     __syncthreads();
     TL::store(Ks, rk);
@@ -200,30 +202,39 @@ __global__ void __launch_bounds__(kT, DP <= 128 ? 2 : 1) k_attn_few(const Attn a
   }
 }
 
-// Joins the key splits: a workgroup per row, a thread per value (or several).
-__global__ void __launch_bounds__(kT) k_attn_join(const Attn a) {
-  const uint32_t row = blockIdx.x, rows = a.B * a.G * a.N;
+// Joins the key splits: a row per `lanes` threads of a wave, 4 values each (or, of
+// dims that are no multiple of 4, one at a time).  ONE: a row per workgroup, for
+// few rows: its statistics are then scalar loads (256 rows of 128 in 16 splits 4.9
+// us, two rows to a wave 6.8).
+template <bool VEC, bool ONE>
+__global__ void __launch_bounds__(64) k_attn_join(const Attn a, uint32_t lanes) {
+  const uint32_t own = ONE ? 0 : threadIdx.x / lanes, lane = threadIdx.x - own * lanes, rows = a.B * a.G * a.N;
+  const uint32_t row = ONE ? blockIdx.x : blockIdx.x * (64 / lanes) + own;
+  if (!ONE && (own >= 64 / lanes || row >= rows)) return;
   const uint32_t pr = row / a.N, n = row - pr * a.N, b = fdiv(pr, a.dG), g = pr - b * a.G;
   const bool none = limit_of(a, n, keys_of(a, b)) == 0;
   float m = -INFINITY;
 #pragma unroll 8
   for (uint32_t s = 0; s < a.splits; ++s) m = fmaxf(m, a.pm[size_t(s) * rows + row]);
   const float base = m == -INFINITY ? 0.f : m;
-  for (uint32_t d = threadIdx.x; d < a.D; d += blockDim.x) {
-    float l = 0.f, o = 0.f;
+  constexpr uint32_t W = VEC ? 4 : 1;
+  using V = float __attribute__((ext_vector_type(W)));
+  for (uint32_t d = lane * W; d < a.D; d += (ONE ? 64 : lanes) * W) {
+    float l = 0.f;
+    V o = {};
 #pragma unroll 8
     for (uint32_t s = 0; s < a.splits; ++s) {
       const size_t i = size_t(s) * rows + row;
       const float w = exp2_(a.pm[i] - base);
       l += w * a.pl[i];
-      o += w * a.po[i * a.D + d];
+      o += w * *reinterpret_cast<const V*>(a.po + i * a.D + d);
     }
     const float il = none ? 0.f : 1.f / l;
     if (a.m && d == 0) {
       a.m[row] = none ? 0.f : m;
       a.il[row] = il;
     }
-    a.o[q_at(a, b, g, n) + d] = none ? 0.f : o * il;
+    *reinterpret_cast<V*>(a.o + q_at(a, b, g, n) + d) = none ? V{} : o * il;
   }
 }
 
@@ -343,12 +354,35 @@ struct BwdRun {
 }  // namespace
 
 bool attn_join(const Attn& a) {
-  hipLaunchKernelGGL(k_attn_join, dim3(a.B * a.G * a.N), dim3(std::min(kT, int(a.D + 63) / 64 * 64)), 0, stream(), a);
+  const bool vec = a.D % 4 == 0;
+  const uint32_t lanes = vec ? a.D / 4 : std::min(64u, a.D);
+  const uint32_t rows = a.B * a.G * a.N;
+  const bool one = rows <= 4 * uint32_t(num_cus());
+  const dim3 grid(one ? rows : cdiv(rows, 64 / lanes));
+  if (vec && one)
+    hipLaunchKernelGGL((k_attn_join<true, true>), grid, dim3(64), 0, stream(), a, lanes);
+  else if (vec)
+    hipLaunchKernelGGL((k_attn_join<true, false>), grid, dim3(64), 0, stream(), a, lanes);
+  else if (one)
+    hipLaunchKernelGGL((k_attn_join<false, true>), grid, dim3(64), 0, stream(), a, lanes);
+  else
+    hipLaunchKernelGGL((k_attn_join<false, false>), grid, dim3(64), 0, stream(), a, lanes);
   return check_launch("AttentionForward (join)");
 }
+
 bool attn_sum(const float* p0, float* out0, const float* p1, float* out1, size_t n, uint32_t splits) {
-  hipLaunchKernelGGL(k_attn_sum, dim3(cdiv(n, kT)), dim3(kT), 0, stream(), p0, out0, p1, out1, n, splits);
-  return check_launch("AttentionBackward (sum)");
+  if (!out0) {
+    p0 = p1;
+    out0 = out1;
+    out1 = nullptr;
+  }
+  if (n % 4 == 0)
+    hipLaunchKernelGGL(k_attn_sum<f4>, dim3(cdiv(n / 4, kT)), dim3(kT), 0, stream(), reinterpret_cast<const f4*>(p0),
+                       reinterpret_cast<f4*>(out0), reinterpret_cast<const f4*>(p1), reinterpret_cast<f4*>(out1),
+                       n / 4, splits);
+  else
+    hipLaunchKernelGGL(k_attn_sum<float>, dim3(cdiv(n, kT)), dim3(kT), 0, stream(), p0, out0, p1, out1, n, splits);
+  return check_launch("AttentionBackward (splits)");
 }
 
 bool attention_forward(const AttnArgs& x) {
