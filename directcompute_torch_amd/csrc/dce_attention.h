@@ -88,7 +88,7 @@ inline double pairs_of(const AttnArgs& x) {
   return rows * last - rows * (rows - 1) / 2;
 }
 
-// Splits of a backward kernel's long side, `tiles` tiles of `us` microseconds each
+// Splits of a kernel's long side, `tiles` tiles of `us` microseconds each
 // for each of `wgs` workgroups: the number of least time, where workgroups take
 // the CUs in rounds (causal ones, longest first, fill them) and have some 8 us of
 // their own, and each split's shares are written and read at 4 TB/s by a launch more.  10 x 1169 tokens, 3
@@ -96,9 +96,10 @@ inline double pairs_of(const AttnArgs& x) {
 // and 3 splits, 472 with 2 and 5; 1 x 6000 tokens, 2 heads of 96, 658 and 496.
 inline uint32_t best_splits(double wgs, uint32_t tiles, double us, double shareBytes, bool causal) {
   const double cus = num_cus();
+  const uint32_t most = uint32_t(std::min({256.0, (tiles + 7) / 8 + 0.0, std::max(1.0, 8 * cus / wgs)}));
   uint32_t best = 1;
   double least = INFINITY;
-  for (uint32_t s = 1; s <= std::min(64u, cdiv(tiles, 8)); ++s) {
+  for (uint32_t s = 1; s <= most; ++s) {
     const double one = tiles * us / s + 8;
     double t = causal ? std::max(one, 0.5 * wgs * (tiles * us + s * 8) / cus + one / 2) : std::ceil(wgs * s / cus) * one;
     if (s > 1) t += 5 + s * shareBytes * 2 / 4e6;

@@ -911,10 +911,15 @@ bool worth(const AttnArgs& x, double least) {
 bool attn_fwd_parts(const AttnArgs& x, Attn a, bool* took) {
   if (!worth(x, 1e12)) return true;
   *took = true;
-  const uint32_t prob = a.B * a.G, cus = uint32_t(num_cus()), kt = cdiv(a.T, kRows);
+  const uint32_t prob = a.B * a.G, kt = cdiv(a.T, kRows);
   a.tiles = cdiv(a.N, 128);
-  a.splits = 1;
-  if (uint64_t(a.tiles) * prob < cus) a.splits = std::max(1u, std::min(cdiv(kt, 8), cdiv(2 * cus, a.tiles * prob)));
+  // Two workgroups live on a CU: keys are split to fill both (1 x 3000 tokens, 4
+  // heads of 128: 108 us in 600 workgroups, 107 in 288, 86 in 480); from one per CU
+  // on by the time of the longest (1 x 8192, 4 heads of 64, causal: 309 us unsplit,
+  // 170 split).
+  const uint32_t wgs = a.tiles * prob, cus = uint32_t(num_cus());
+  a.splits = wgs < cus ? std::max(1u, std::min(cdiv(kt, 8), 2 * cus / wgs))
+                       : best_splits(wgs, kt, a.D * 0.015, 4.0 * prob * a.N * (a.D + 2), a.causal);
   a.perSplit = cdiv(kt, a.splits);
   a.splits = cdiv(kt, a.perSplit);
   const size_t rows = size_t(prob) * a.N, stat = (rows * a.splits + 63) & ~size_t(63);
