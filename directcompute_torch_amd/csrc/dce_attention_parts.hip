@@ -914,7 +914,7 @@ bool attn_fwd_parts(const AttnArgs& x, Attn a, bool* took) {
   const uint32_t prob = a.B * a.G, kt = cdiv(a.T, kRows);
   a.tiles = cdiv(a.N, 128);
   // Two workgroups live on a CU: keys are split to fill both (1 x 3000 tokens, 4
-  // heads of 128: 108 us in 600 workgroups, 107 in 288, 86 in 480); from one per CU
+  // heads of 128: 108 us in 576 workgroups, 107 in 192, 86 in 480); from one per CU
   // on by the time of the longest (1 x 8192, 4 heads of 64, causal: 309 us unsplit,
   // 170 split).
   const uint32_t wgs = a.tiles * prob, cus = uint32_t(num_cus());
