@@ -747,3 +747,33 @@ def test_muon_takes_any_iterable(eng):
     w.grad, bias.grad = dev(eng, np.ones((4, 3))), dev(eng, np.ones(3))
     opt.step()
     assert opt.params == [w, bias] and (w.sync() != 1).all() and (bias.sync() != 1).all()
+
+
+SPLIT = [  # splits joined and summed: by 4 values and by one, few rows and many
+    (1, 61, 701, 1, 1, 33, False, None),
+    (1, 701, 61, 1, 1, 33, True, None),
+    (1, 1100, 300, 1, 1, 33, False, [299]),
+    (1, 1100, 300, 1, 1, 40, True, None),
+    (1, 3, 2100, 4, 2, 7, True, None),
+    # and where the blocks alone would fill the chip
+    (1, 2048, 2048, 16, 4, 128, True, None),
+    (1, 1100, 1100, 32, 32, 128, False, [1077]),
+]
+
+
+@pytest.mark.parametrize("case", SPLIT, ids=lambda c: "x".join(map(str, c[:6])) + ("c" if c[6] else "") + ("l" if c[7] else ""))
+def test_attention_split(eng, case):
+    test_attention(eng, case)
+
+
+@pytest.mark.parametrize("shape", [(2050, 2050), (3000, 5000), (4097, 1), (1, 4095)])
+def test_muon_of_many_values(eng, shape):
+    """Sums of the norm over more than 4096 values each, and ragged ends: one step
+    of zero weights.  Its products are off by 4 * 2^-23 of |X_0| = 1, grown by
+    3.4445 at most, and the update is rounded."""
+    g = rng(70).standard_normal(shape).astype(np.float32)
+    w = dev(eng, np.zeros(shape), True)
+    w.grad = dev(eng, g)
+    eng.Muon([w], lr=1.0, momentum=0.0, nesterov=False, steps=1, rms=1.0).step(clip=1e30)
+    x = orthogonalised64(g.astype(np.float64), 1)
+    assert rel2(w.sync(), -x * math.sqrt(max(shape))) <= 3.4445 * 4 * 2.0 ** -23 / np.linalg.norm(x) + 4 * EPS
