@@ -6,32 +6,28 @@
 // dot product rounds its sum once per 16 terms instead of at every one.  The
 // exponent e is one for each tile of 32 vectors, chosen so that the tile's
 // largest value lies in [2^14, 2^15): l's half step is then 2^-25, so a vector
-// whose own largest value is within 2^14 of the tile's keeps at least 24 bits of
+// whose own largest value is within 2^12 of the tile's keeps at least 24 bits of
 // it.  A tile that has smaller vectors than that (zeros aside), values outside of
 // 2^+-30 (gradients: 2^+-60) or any that is not finite is marked by the pass that
 // splits, and the workgroups of its (sequence, key head) run the fp32 code.
 //
-// Everything that the scores do not need is a factor of a whole tile, so the
-// exponents cost next to nothing: c 2^-(eq + ek) is the factor that turns a
-// score into base 2 anyway, and where a sum goes over tiles of different
-// exponents (over V's in the forward, dO's and Q's for dV and dK) its terms are
-// brought to the smallest exponent so far, which the exponential's offset takes.
-// That costs a tile of smaller vectors bits of P, seen only where a row (or key)
-// gives the larger ones no weight: P = 1 has 32 bits in the forward before the
-// first is lost, some 33 in dS.  Problems whose V tiles differ by more than 2^8
-// (backward: V's and K's together by 2^12, or Q's and dO's by 2^20, which 1 / l
-// of causal rows makes T of; 24, 21 and 13 bits at the least) run on fp32 too.
+// A tile's exponent costs a score nothing: c 2^-(eq + ek) is the factor that turns
+// it into base 2 anyway.  P and dS are made into parts with an exponent of their
+// own for every column of the transposed product (the row of O or dQ, the key of
+// dK or dV) and the tile's exponent, so that a column's largest term so far lies
+// in [2^12, 2^15): l's half step, 2^-25, is then 2^-37 of it.  Where it was made from
+// a vector 2^-12 of its tile's largest that is 2^-25 of the term, fp32's half step.
+// A larger term scales the column's sum down, which few tiles past the first need.
+// (One exponent for all columns, from a bound on dS, left dK 8 bits where other
+// rows' gradients were 2^18 larger.)
 //
-// P is relative to its row's maximum, within [0, 1], and kept as 2^14 P.  The
-// forward only follows its running maximum, and scales the sums so far, where a
-// score passes it by more than 2^8: its P is at most 2^8, kept as 2^7 P.  P's
-// parts end at 2^-39 (forward: 2^-32), which is an error of P relative to the
-// row's largest; a key to which every row gives less gets dK = dV = 0.  The
-// backward's 1 / l goes into dO (dO' = dO / l) when that is split, so that
-// dV = P^T dO' and dS = scale P (dO' V^T - delta'), delta' = rowsum(dO' * O).
-// delta' is of the size of the largest vector that a row sees, whatever tile it
-// is compared in: with E the least exponent of V's tiles up to the row's last
-// key, |dO' V^T - delta'| is at most 2 D 2^(30 - ey - E), which bounds dS's parts.
+// The forward: P is relative to its row's maximum and kept as 2^7 P; it only
+// follows its running maximum, and scales the sums so far, where a score passes it
+// by more than 2^8.  Its terms are brought to the smallest exponent of V's tiles so
+// far, which costs a tile of smaller vectors bits of P; problems whose V tiles differ
+// by more than 2^8 run on fp32.  The backward's 1 / l goes into dO (dO' = dO / l)
+// when that is split, so that dV = P^T dO' and dS = scale P (dO' V^T - delta'),
+// delta' = rowsum(dO' * O).
 #include "dce_attention_fp32.h"
 
 #include <type_traits>
@@ -46,9 +42,14 @@ constexpr int kRange = 30;        // exponents of values that parts are made of
 constexpr int kRangeGrad = 60;    // and of gradients
 constexpr float kSlack = 8.f;     // of the forward's running maximum, in powers of 2
 constexpr int kExpP = 7;          // the forward's P parts hold p 2^7, p up to 2^kSlack
-constexpr float kWide = 16384.f;  // largest ratio of the vectors' sizes in a tile
+constexpr float kWide = 4096.f;  // largest ratio of the vectors' sizes in a tile
 constexpr int kZeros = 15 + kRange, kZerosGrad = 15 + kRangeGrad;  // exponents of tiles of zeros, larger than any other
-constexpr float kSpread = 8.f, kSpreadKeys = 12.f, kSpreadRows = 20.f;  // of the tiles' exponents
+constexpr float kSpread = 8.f;  // of the exponents of V's tiles in the forward
+// A column's parts of P or dS are made with its largest value in [2^kTop, 2^(kTop + 1));
+// a later tile's may go up to 2^kFull before the column's sum is scaled down.
+constexpr int kTop = 12, kFull = 15;
+constexpr int kMost = 100;   // the largest factor that makes them, 2^kMost
+constexpr int kNone = 1000;  // exponent of a sum that has no terms yet
 
 using h2 = _Float16 __attribute__((ext_vector_type(2)));
 using h4 = _Float16 __attribute__((ext_vector_type(4)));
@@ -79,57 +80,46 @@ struct Parts {
   float* dl;  // delta' 2^e of dO's tile, [problem][q.pad]
 };
 constexpr int kBad = 1 << 20;
-// Does problem pr have a tile that parts do not suit, or tiles of too different
-// sizes?  For all threads of the workgroup.
+// Does problem pr have a tile that parts do not suit, or (forward) tiles of V of too
+// different sizes?  For all threads of the workgroup.
 template <bool BWD>
 __device__ __forceinline__ bool unsuited(const Parts& ps, uint32_t pr) {
-  __shared__ float ends[8][8];
-  const uint32_t nq = ps.q.pad / kRows, nk = ps.k.pad / kRows;
-  // largest and smallest exponents of v, k, q, dO
-  float hi[4], lo[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) hi[i] = -1000.f, lo[i] = 1000.f;
-  auto take = [&](int i, const int* e, uint32_t n, int zeros) {
+  __shared__ float ends[8][2];
+  __shared__ int bads[8];
+  const uint32_t nq = ps.q.pad / kRows, nk = ps.k.pad / kRows, wave = threadIdx.x >> 6;
+  float hi = -1000.f, lo = 1000.f;  // of V's exponents
+  bool bad = false;
+  auto take = [&](const int* e, uint32_t n, bool v) {
     for (uint32_t t = threadIdx.x; t < n; t += blockDim.x) {
       const int x = e[size_t(pr) * n + t];
-      if (x == zeros) continue;
-      hi[i] = fmaxf(hi[i], float(x));
-      lo[i] = fminf(lo[i], float(x));
+      bad |= x == kBad;
+      if (BWD || !v || x == kZeros) continue;
+      hi = fmaxf(hi, float(x));
+      lo = fminf(lo, float(x));
     }
   };
-  take(0, ps.v.e, nk, kZeros);
-  take(1, ps.k.e, nk, kZeros);
-  take(2, ps.q.e, nq, kZeros);
-  if (BWD) take(3, ps.y.e, nq, kZerosGrad);
-  const uint32_t wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 0; i < (BWD ? 4 : 3); ++i) {
-    hi[i] = wave_reduce(hi[i], OpMaxR());
-    lo[i] = -wave_reduce(-lo[i], OpMaxR());
-    if ((threadIdx.x & 63) == 0) {
-      ends[wave][i] = hi[i];
-      ends[wave][4 + i] = lo[i];
-    }
+  take(ps.v.e, nk, true);
+  take(ps.k.e, nk, false);
+  take(ps.q.e, nq, false);
+  if (BWD) take(ps.y.e, nq, false);
+  if (!BWD) {
+    hi = wave_reduce(hi, OpMaxR());
+    lo = -wave_reduce(-lo, OpMaxR());
+  }
+  const bool any = __any(bad);
+  if ((threadIdx.x & 63) == 0) {
+    bads[wave] = any;
+    ends[wave][0] = hi;
+    ends[wave][1] = lo;
   }
   __syncthreads();
-  float spread[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < (BWD ? 4 : 3); ++i) {
-    for (uint32_t w = 0; w < blockDim.x / 64; ++w) {
-      hi[i] = fmaxf(hi[i], ends[w][i]);
-      lo[i] = fminf(lo[i], ends[w][4 + i]);
-    }
-    if (hi[i] >= float(kBad)) return true;
-    spread[i] = fmaxf(hi[i] - lo[i], 0.f);  // 0: only zeros
+  bad = false;
+  for (uint32_t w = 0; w < blockDim.x / 64; ++w) {
+    bad |= bads[w] != 0;
+    hi = fmaxf(hi, ends[w][0]);
+    lo = fminf(lo, ends[w][1]);
   }
-  if (!BWD) return spread[0] > kSpread;
-  return spread[0] + spread[1] > kSpreadKeys || spread[2] + spread[3] > kSpreadRows;
-}
-// The least exponent of V's tiles [from, to), in every lane.
-__device__ __forceinline__ int least_of(const int* ev, uint32_t from, uint32_t to, int lane) {
-  float m = 1000.f;
-  for (uint32_t t = from + lane; t < to; t += 64) m = fminf(m, float(ev[t]));
-  return -int(wave_reduce(-m, OpMaxR()));
+  return bad || (!BWD && hi - lo > kSpread);
 }
 
 // ---------------------------------------------------------------------------
@@ -510,13 +500,6 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
   write_vec<DP, VEC>(a.o + q_at(a, b, gh, n), a.D, half, o, unit * il, unit2);
 }
 
-// dS's parts: p (at most 2^14) times dP - delta (at most 2^(31 + log2 DP)) times
-// 2^-down_bits lies below 2^15.
-template <int DP>
-constexpr int down_bits() {
-  return 30 + (DP <= 32 ? 5 : DP <= 64 ? 6 : 7);
-}
-
 // ---------------------------------------------------------------------------
 // The backward kernels: eight waves, in pairs of one 32-vector block each.  The
 // first of a pair computes P = exp(S - m) and leaves it in LDS; the second, a
@@ -554,6 +537,26 @@ __device__ __forceinline__ void scale_acc(f16v (&acc)[N], float by) {
   for (int t = 0; t < N; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] *= by;
+}
+// f's terms are f 2^-unit; f becomes what a column's sum adds, which counts in units
+// of 2^-A (a lane and the one 32 further on hold a column).  A goes down, and the sum
+// with it, where a value would pass 2^kFull or its factor 2^kMost.
+template <int N>
+__device__ __forceinline__ void fit_column(f16v& f, int unit, int& A, f16v (&acc)[N]) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(f[i]));
+  top = fmaxf(top, __shfl_xor(top, 32));
+  const int e = int(__float_as_uint(top) >> 23) - 127, room = A - unit;
+  const bool full = top > 0.f && (e + room >= kFull || room > kMost);
+  if (__any(full)) {
+    const int next = full ? min(kTop - e, kMost) + unit : A;
+    scale_acc(acc, pow2(next - A));
+    A = next;
+  }
+  const float by = pow2(min(A - unit, kMost));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] *= by;
 }
 
 // ---------------------------------------------------------------------------
@@ -629,8 +632,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
   f16v dq[DP / 32];
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) zero(dq[t]);
-  const int E = least_of(ev, 0, (mine + kRows - 1) / kRows, lane);
-  int R = 1000;  // dq counts in units of 2^-(R + E + ey - down_bits + 14)
+  int A = kNone;  // dq counts in units of 2^-A, a row's own
   each_tile(t0, t1, [&](uint32_t t, auto st) {
     stage(t + 1, std::integral_constant<int, (st + 1) % kStages>{});
     const uint32_t u = t - 1;  // the tile before the first waves'
@@ -638,25 +640,22 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
     if (t > t0 && u * kRows < mine) {
       const int xk = ek[u], xv = ev[u];
       f16v dp = scores<DP>(Vs[su], xh, xl, col, half);
-      if (xk < R) {
-        if (R != 1000) scale_acc(dq, pow2(xk - R));
-        R = xk;
-      }
-      const float dl = delta * pow2(xv), by = pow2(R - xk + E - xv - down_bits<DP>() + 14);
+      const float dl = delta * pow2(xv);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const f4 p = get_p(Ps[u & 1][blk], lane, q);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dp[4 * q + e] = p[e] * ((dp[4 * q + e] - dl) * by);
+        for (int e = 0; e < 4; ++e) dp[4 * q + e] = p[e] * (dp[4 * q + e] - dl);
       }
+      fit_column(dp, xk + xv + ey, A, dq);
       add_cols<DP>(Ks[su], dp, dq, lane);
     }
     __syncthreads();
   });
   if (n >= a.N) return;
-  // 2^(down_bits - 14 - R - E - ey), in two factors that stay in range
-  const float u = R == 1000 ? 0.f : pow2(down_bits<DP>() - 14 - R - E) * a.scale;
-  write_vec<DP, VEC>(a.dq + dq_part(a, sp) + q_at(a, b, gh, n), a.D, half, dq, u, pow2(-ey));
+  // 2^-A in two factors that stay in range
+  write_vec<DP, VEC>(a.dq + dq_part(a, sp) + q_at(a, b, gh, n), a.D, half, dq, pow2(-(A / 2)) * a.scale,
+                     pow2(A / 2 - A));
 }
 
 // ---------------------------------------------------------------------------
@@ -671,6 +670,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   __shared__ __attribute__((aligned(16))) float Ps[2][4][1024];
   __shared__ __attribute__((aligned(16))) float Ms[kStages][kRows], Ds[kStages][kRows];
   __shared__ uint32_t Ls[kStages][kRows];
+  __shared__ int Up[2][4][64];  // the exponents of P's columns
   const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
   const uint32_t tile = rest / a.splits, sp = rest - tile * a.splits;
   if (unsuited<true>(ps, pr))
@@ -721,7 +721,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   f16v acc[DP / 32];
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) zero(acc[t]);
-  int Rv = 1000;  // dv counts in units of 2^-(14 + Rv)
+  int A = kNone;  // dv (second waves: dk) counts in units of 2^-A, a key's own
   if (first) {
     load_vec<DP>(ps.k.p + row * (DP * 4), half, xh, xl);
     const float ck = a.c * pow2(-ps.k.e[kt]);
@@ -731,23 +731,34 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
         const int xy = ey[t];
         const float cs = ck * pow2(-eq[t]);
         f16v s = scores<DP>(Qs[st], xh, xl, col, half);
-        if (xy < Rv) {
-          if (Rv != 1000) scale_acc(acc, pow2(xy - Rv));
-          Rv = xy;
-        }
-        const float lg = float(14 + max(Rv - xy, -60));
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f4 m = *reinterpret_cast<const f4*>(Ms[st] + 8 * q + 4 * half);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[4 * q + e] = exp2_(s[4 * q + e] * cs - (m[e] - lg));
+          for (int e = 0; e < 4; ++e) s[4 * q + e] = s[4 * q + e] * cs - m[e];
         }
         if (limit_of(a, t * kRows, len) < kw + kRows) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (key >= Ls[st][8 * (i >> 2) + 4 * half + (i & 3)]) s[i] = 0.f;
+            if (key >= Ls[st][8 * (i >> 2) + 4 * half + (i & 3)]) s[i] = -INFINITY;
         }
+        // As fit_column, on the logarithms
+        float top = -kNone;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float room = float(A - xy);
+        const bool full = top > -kNone / 2 && (top + room >= float(kFull) || room > float(kMost));
+        if (__any(full)) {
+          const int next = full ? min(kTop - int(floorf(top)), kMost) + xy : A;
+          scale_acc(acc, pow2(next - A));
+          A = next;
+        }
+        const int up = min(A - xy, kMost);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = exp2_(s[i] + float(up));
         put_p(Ps[t & 1][blk], lane, s);
+        Up[t & 1][blk][lane] = up;
         add_cols<DP>(Ys[st], s, acc, lane);
       }
       __syncthreads();
@@ -756,40 +767,26 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
     if (key >= len)  // keys past the length get zeros
 #pragma unroll
       for (int t = 0; t < DP / 32; ++t) zero(acc[t]);
-    write_vec<DP, VEC>(a.dv + part + k_at(a, b, gh, key), a.D, half, acc, pow2(-14), Rv == 1000 ? 0.f : pow2(-Rv));
+    write_vec<DP, VEC>(a.dv + part + k_at(a, b, gh, key), a.D, half, acc, pow2(-(A / 2)), pow2(A / 2 - A));
     return;
   }
   load_vec<DP>(ps.v.p + row * (DP * 4), half, xh, xl);
   const int xv = ps.v.e[kt];
   const float vs = pow2(xv);
-  // E, over V's tiles below `seen_tiles`, grows with the rows.
-  const int* ev = ps.v.e + size_t(pr) * (ps.v.pad / kRows);
-  uint32_t seen_tiles = t0 < t1 ? (wave_limit(a, t0 * kRows, kRows, len) + kRows - 1) / kRows : 0u;
-  int E = least_of(ev, 0, seen_tiles, lane);
-  int Rk = 1000;  // dk counts in units of 2^-(Rk - down_bits + 14)
   each_tile(t0, t1, [&](uint32_t t, auto sn) {
     stage(t + 1, std::integral_constant<int, (sn + 1) % kStages>{});
     const uint32_t u = t - 1;  // the tile before the first waves'
-    const uint32_t seen = t > t0 ? wave_limit(a, u * kRows, kRows, len) : 0u;
-    if (seen > kw) {
+    if (t > t0 && wave_limit(a, u * kRows, kRows, len) > kw) {
       constexpr int st = (sn + kStages - 1) % kStages;
-      for (; seen_tiles * kRows < seen; ++seen_tiles) E = min(E, ev[seen_tiles]);
-      const int xy = ey[u], x = eq[u] + xy + E;
       f16v dp = scores<DP>(Ys[st], xh, xl, col, half);
-      Rv = min(Rv, xy);
-      if (x < Rk) {
-        if (Rk != 1000) scale_acc(acc, pow2(x - Rk));
-        Rk = x;
-      }
-      const int lg = 14 + max(Rv - xy, -60);
-      const float by = pow2(Rk - x + E - xv - down_bits<DP>() + 14 - lg);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const f4 p = get_p(Ps[u & 1][blk], lane, q);
         const f4 d = *reinterpret_cast<const f4*>(Ds[st] + 8 * q + 4 * half);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dp[4 * q + e] = p[e] * ((dp[4 * q + e] - d[e] * vs) * by);
+        for (int e = 0; e < 4; ++e) dp[4 * q + e] = p[e] * (dp[4 * q + e] - d[e] * vs);
       }
+      fit_column(dp, eq[u] + ey[u] + xv + Up[u & 1][blk][lane], A, acc);
       add_cols<DP>(Qs[st], dp, acc, lane);
     }
     __syncthreads();
@@ -798,8 +795,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   if (key >= len)
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) zero(acc[t]);
-  write_vec<DP, VEC>(a.dk + part + k_at(a, b, gh, key), a.D, half, acc,
-                     Rk == 1000 ? 0.f : pow2(down_bits<DP>() - 14 - Rk / 2) * a.scale, pow2(Rk / 2 - Rk));
+  write_vec<DP, VEC>(a.dk + part + k_at(a, b, gh, key), a.D, half, acc, pow2(-(A / 2)) * a.scale, pow2(A / 2 - A));
 }
 
 struct Places {
