@@ -20,14 +20,8 @@
 // A larger term scales the column's sum down, which few tiles past the first need.
 // (One exponent for all columns, from a bound on dS, left dK 8 bits where other
 // rows' gradients were 2^18 larger.)
-//
-// The forward: P is relative to its row's maximum and kept as 2^7 P; it only
-// follows its running maximum, and scales the sums so far, where a score passes it
-// by more than 2^8.  Its terms are brought to the smallest exponent of V's tiles so
-// far, which costs a tile of smaller vectors bits of P; problems whose V tiles differ
-// by more than 2^8 run on fp32.  The backward's 1 / l goes into dO (dO' = dO / l)
-// when that is split, so that dV = P^T dO' and dS = scale P (dO' V^T - delta'),
-// delta' = rowsum(dO' * O).
+// The backward's 1 / l goes into dO (dO' = dO / l) when that is split, so that
+// dV = P^T dO' and dS = scale P (dO' V^T - delta'), delta' = rowsum(dO' * O).
 #include "dce_attention_fp32.h"
 
 #include <type_traits>
@@ -40,11 +34,8 @@ constexpr int kT = 256;
 constexpr int kRows = 32;         // vectors of a tile
 constexpr int kRange = 30;        // exponents of values that parts are made of
 constexpr int kRangeGrad = 60;    // and of gradients
-constexpr float kSlack = 8.f;     // of the forward's running maximum, in powers of 2
-constexpr int kExpP = 7;          // the forward's P parts hold p 2^7, p up to 2^kSlack
 constexpr float kWide = 4096.f;  // largest ratio of the vectors' sizes in a tile
 constexpr int kZeros = 15 + kRange, kZerosGrad = 15 + kRangeGrad;  // exponents of tiles of zeros, larger than any other
-constexpr float kSpread = 8.f;  // of the exponents of V's tiles in the forward
 // A column's parts of P or dS are made with its largest value in [2^kTop, 2^(kTop + 1));
 // a later tile's may go up to 2^kFull before the column's sum is scaled down.
 constexpr int kTop = 12, kFull = 15;
@@ -80,46 +71,37 @@ struct Parts {
   float* dl;  // delta' 2^e of dO's tile, [problem][q.pad]
 };
 constexpr int kBad = 1 << 20;
-// Does problem pr have a tile that parts do not suit, or (forward) tiles of V of too
-// different sizes?  For all threads of the workgroup.
+// Does problem pr have a tile that parts do not suit, or (forward) vectors whose
+// scores might pass 2^24, past which they are no place to add an exponent to?  For
+// all threads of the workgroup.
 template <bool BWD>
-__device__ __forceinline__ bool unsuited(const Parts& ps, uint32_t pr) {
-  __shared__ float ends[8][2];
-  __shared__ int bads[8];
-  const uint32_t nq = ps.q.pad / kRows, nk = ps.k.pad / kRows, wave = threadIdx.x >> 6;
-  float hi = -1000.f, lo = 1000.f;  // of V's exponents
-  bool bad = false;
-  auto take = [&](const int* e, uint32_t n, bool v) {
+__device__ __forceinline__ bool unsuited(const Attn& a, const Parts& ps, uint32_t pr) {
+  __shared__ float ends[8][3];
+  const uint32_t nq = ps.q.pad / kRows, nk = ps.k.pad / kRows;
+  // kBad passes all others; of q and k the least exponents, negated, too
+  float most = 0.f, q = -1000.f, k = q;
+  auto take = [&](const int* e, uint32_t n, float* least) {
     for (uint32_t t = threadIdx.x; t < n; t += blockDim.x) {
-      const int x = e[size_t(pr) * n + t];
-      bad |= x == kBad;
-      if (BWD || !v || x == kZeros) continue;
-      hi = fmaxf(hi, float(x));
-      lo = fminf(lo, float(x));
+      const float x = float(e[size_t(pr) * n + t]);
+      most = fmaxf(most, x);
+      if (least) *least = fmaxf(*least, -x);
     }
   };
-  take(ps.v.e, nk, true);
-  take(ps.k.e, nk, false);
-  take(ps.q.e, nq, false);
-  if (BWD) take(ps.y.e, nq, false);
-  if (!BWD) {
-    hi = wave_reduce(hi, OpMaxR());
-    lo = -wave_reduce(-lo, OpMaxR());
-  }
-  const bool any = __any(bad);
-  if ((threadIdx.x & 63) == 0) {
-    bads[wave] = any;
-    ends[wave][0] = hi;
-    ends[wave][1] = lo;
-  }
+  take(ps.q.e, nq, BWD ? nullptr : &q);
+  take(ps.k.e, nk, BWD ? nullptr : &k);
+  take(ps.v.e, nk, nullptr);
+  if (BWD) take(ps.y.e, nq, nullptr);
+  const float w[3] = {wave_reduce(most, OpMaxR()), BWD ? q : wave_reduce(q, OpMaxR()), BWD ? k : wave_reduce(k, OpMaxR())};
+  if ((threadIdx.x & 63) == 0)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) ends[threadIdx.x >> 6][i] = w[i];
   __syncthreads();
-  bad = false;
-  for (uint32_t w = 0; w < blockDim.x / 64; ++w) {
-    bad |= bads[w] != 0;
-    hi = fmaxf(hi, ends[w][0]);
-    lo = fminf(lo, ends[w][1]);
+  for (uint32_t i = 0; i < blockDim.x / 64; ++i) {
+    most = fmaxf(most, ends[i][0]);
+    q = fmaxf(q, ends[i][1]);
+    k = fmaxf(k, ends[i][2]);
   }
-  return bad || (!BWD && hi - lo > kSpread);
+  return most >= float(kBad) || (!BWD && !(fabsf(a.c) * float(a.D) < pow2(24 - 30 - int(q + k))));
 }
 
 // ---------------------------------------------------------------------------
@@ -355,6 +337,13 @@ __device__ __forceinline__ void add_cols(const char* S, const f16v& s, f16v (&ac
     }
   }
 }
+template <int N>
+__device__ __forceinline__ void scale_acc(f16v (&acc)[N], float by) {
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] *= by;
+}
 // A lane's vector from its accumulators: dims 32 t + 8 q + 4 half + 0 .. 3.
 template <int DP, bool VEC>
 __device__ __forceinline__ void write_vec(float* p, uint32_t D, int half, const f16v (&acc)[DP / 32], float by, float by2) {
@@ -387,7 +376,7 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
   __shared__ __attribute__((aligned(16))) char Ks[TL::BYTES], Vs[TL::BYTES];
   const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
   const uint32_t back = rest / a.splits, sp = rest - back * a.splits, tile = a.tiles - 1 - back;
-  if (unsuited<false>(ps, pr)) {
+  if (unsuited<false>(a, ps, pr)) {
     for (uint32_t n = tile * 128; n < min(tile * 128 + 128, a.N); n += 64)
       fwd_fp32<DP, 1, VEC>(a, pr, n, sp, reinterpret_cast<float*>(Ks), reinterpret_cast<float*>(Vs));
     return;
@@ -407,8 +396,9 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
   f16v o[DP / 32];
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) zero(o[t]);
-  float m = -INFINITY, l = 0.f, most_s = -INFINITY;
-  int R = 1000;  // o counts in units of 2^-(kExpP + R)
+  // o and l count in units of 2^C, a row's own: P's parts are 2^(s - C - e), which
+  // the exponential's offset brings in
+  float C = -3e38f, l = 0.f, most_s = -INFINITY;
   const uint32_t j0 = sp * a.perSplit * kRows, j1 = min(most, (sp + 1) * a.perSplit * kRows);
   u4v rk[TL::LOADS], rv[TL::LOADS];
   auto fetch = [&](uint32_t j) {
@@ -443,61 +433,43 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
     }
     top = fmaxf(top, __shfl_xor(top, 32));
     most_s = fmaxf(most_s, top);
-    float down = 1.f;
-    bool move = __any(top > m + kSlack);
-    if (move) {
-      top = fmaxf(m, top);
-      down = m == -INFINITY ? 0.f : exp2_(m - top);
+    float off = C + float(e);
+    const bool full = top - off >= float(kFull);
+    if (__any(full)) {
+      const float next = full ? floorf(top) - float(kTop + e) : C;
+      const float down = pow2(int(fmaxf(C - next, -126.f)));
       l *= down;
-      m = top;
+      scale_acc(o, down);
+      C = next;
+      off = C + float(e);
     }
-    const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet: every p is 0
-    if (e < R) {
-      down *= R == 1000 ? 1.f : pow2(e - R);
-      R = e;
-      move = true;
-    }
-    if (move) {
-#pragma unroll
-      for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[t][i] *= down;
-    }
-    // p 2^(kExpP + R - e), which the exponential's offset brings in
-    const int lg = kExpP + max(R - e, -60);
-    const float off = base - float(lg);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[i] = exp2_(s[i] - off);
       sum += s[i];
     }
-    l += sum * pow2(-lg);
+    l += sum * pow2(e);
     add_cols<DP>(Vs, s, o, lane);
   }
   l += __shfl_xor(l, 32);
   if (n >= a.N) return;
-  // From here on relative to the largest score itself, as the backward has it.
-  const float up = m == -INFINITY ? 1.f : exp2_(m - most_s);
-  l *= up;
-  m = most_s;
-  const float unit = R == 1000 ? 0.f : pow2(-kExpP) * up;
-  const float unit2 = R == 1000 ? 0.f : pow2(-R);
+  // The statistics are relative to the largest score.
+  const float up = most_s == -INFINITY ? 1.f : exp2_(C - most_s);
   if (a.splits > 1) {
     const size_t row = (size_t(sp) * a.B * a.G + pr) * a.N + n;
     if (half == 0) {
-      a.pm[row] = m;
-      a.pl[row] = l;
+      a.pm[row] = most_s;
+      a.pl[row] = l * up;
     }
-    write_vec<DP, VEC>(a.po + row * a.D, a.D, half, o, unit, unit2);
+    write_vec<DP, VEC>(a.po + row * a.D, a.D, half, o, up, 1.f);
     return;
   }
-  const float il = lim ? 1.f / l : 0.f;  // a row that sees nothing: zeros
   if (a.m && half == 0) {
-    a.m[size_t(pr) * a.N + n] = lim ? m : 0.f;
-    a.il[size_t(pr) * a.N + n] = il;
+    a.m[size_t(pr) * a.N + n] = lim ? most_s : 0.f;
+    a.il[size_t(pr) * a.N + n] = lim ? 1.f / (l * up) : 0.f;
   }
-  write_vec<DP, VEC>(a.o + q_at(a, b, gh, n), a.D, half, o, unit * il, unit2);
+  write_vec<DP, VEC>(a.o + q_at(a, b, gh, n), a.D, half, o, lim ? 1.f / l : 0.f, 1.f);  // a row that sees nothing: zeros
 }
 
 // ---------------------------------------------------------------------------
@@ -530,13 +502,6 @@ __device__ __forceinline__ void each_tile(uint32_t t0, uint32_t t1, F&& f) {
     if (t + 1 <= t1) f(t + 1, std::integral_constant<int, 1>{});
     if (t + 2 <= t1) f(t + 2, std::integral_constant<int, 2>{});
   }
-}
-template <int N>
-__device__ __forceinline__ void scale_acc(f16v (&acc)[N], float by) {
-#pragma unroll
-  for (int t = 0; t < N; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[t][i] *= by;
 }
 // f's terms are f 2^-unit; f becomes what a column's sum adds, which counts in units
 // of 2^-A (a lane and the one 32 further on hold a column).  A goes down, and the sum
@@ -571,7 +536,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
   __shared__ __attribute__((aligned(16))) float Ps[2][4][1024];
   const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
   const uint32_t back = rest / a.splits, sp = rest - back * a.splits, tile = a.tiles - 1 - back;
-  if (unsuited<true>(ps, pr))
+  if (unsuited<true>(a, ps, pr))
     return dq_fp32<DP, 1, VEC, kPair>(a, pr, tile * 128, sp, reinterpret_cast<float*>(Ks[0]),
                                       reinterpret_cast<float*>(Vs[0]));
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
@@ -673,7 +638,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
   __shared__ int Up[2][4][64];  // the exponents of P's columns
   const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
   const uint32_t tile = rest / a.splits, sp = rest - tile * a.splits;
-  if (unsuited<true>(ps, pr))
+  if (unsuited<true>(a, ps, pr))
     return dkv_fp32<DP, VEC, kPair>(a, pr, tile * 128, sp, reinterpret_cast<float*>(Qs[0]),
                                     reinterpret_cast<float*>(Ys[0]), Ps[0][0], Ls[0]);
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;

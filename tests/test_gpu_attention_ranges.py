@@ -127,3 +127,18 @@ def test_keys_of_almost_no_weight(eng):
     q[..., 0] = 8
     k[..., 0] = np.where(np.arange(N) % 32 < 16, -35, 0)[None, :, None]
     check(eng, q, k, v, dy, "keys of almost no weight")
+
+
+@pytest.mark.parametrize("apart", [0, 6, 20])
+def test_output_beside_a_key_that_takes_the_weight(eng, apart):
+    """One key takes most of every row's weight and has a small vector; keys of
+    e^-20 of the weight have vectors 2^apart larger than the others, which make
+    the output."""
+    q, k, v, dy = inputs(208)
+    ignored = np.arange(N) // 32 % 2 == 0    # every other tile, in whatever way the keys are split
+    q[..., 0] = 8
+    k[..., 0] = np.where(ignored, -20, 0)[None, :, None]
+    k[:, 630, :, 0] = 9
+    v[:, ignored] *= np.float32(2.0 ** apart)
+    v[:, 630] *= np.float32(2.0 ** -9)
+    check(eng, q, k, v, dy, f"a key that takes the weight, values 2^{apart} apart")
