@@ -116,21 +116,17 @@ __global__ void __launch_bounds__(kT, DP <= 128 ? 2 : 1) k_attn_few(const Attn a
     if (j + kFew < j1) fetch(j + kFew);
     const uint32_t jw = j + wave * 16;
     if (jw >= most) continue;
-    f4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+    f4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const f4 kf = TL::chunk(Ks, wave * 16 + col, 4 * i + g);
 #pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        s0 = mfma4(kf[e], q[i][e], s0);
-        s1 = mfma4(kf[e + 1], q[i][e + 1], s1);
-      }
+      for (int e = 0; e < 4; ++e) s = mfma4(kf[e], q[i][e], s);
     }
-    f4 s;
     float top = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      s[r] = (s0[r] + s1[r]) * a.c;
+      s[r] = scaled(s[r], a.c);
       if (jw + 16 > least && jw + 4 * g + r >= lim) s[r] = -INFINITY;
       top = fmaxf(top, s[r]);
     }

@@ -32,6 +32,15 @@ __device__ __forceinline__ void load_frag(const float* p, bool ok, uint32_t D, i
     for (int e = 0; e < 4; ++e) r[j][e] = ok && 16 * j + 4 * g + e < D ? r[j][e] : 0.f;
 }
 
+// A score times c, rounded before the row's maximum is taken off, here and in the
+// backward: fused with the subtraction it would miss the (rounded) maximum by the
+// product's rounding, which of large scores is a factor of P.  For the same reason
+// the kernels multiply the terms of a score in one order.
+__device__ __forceinline__ float scaled(float s, float c) {
+#pragma clang fp contract(off)
+  return s * c;
+}
+
 template <int CH>
 __device__ __forceinline__ int swz(int row) {
   return CH % 16 == 0 ? row & 15 : (row >> 1) & 7;
@@ -192,7 +201,7 @@ __device__ __forceinline__ void fwd_fp32(const Attn& a, uint32_t pr, uint32_t n0
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float x = s[t][kt][r] * a.c;
+          float x = scaled(s[t][kt][r], a.c);
           if (masked && j + 16 * kt + 4 * g + r >= lim[t]) x = -INFINITY;
           s[t][kt][r] = x;
           top = fmaxf(top, x);
@@ -342,7 +351,7 @@ __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0,
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float p = exp2_(s[t][kt][r] * a.c - m[t]) * il[t];
+          const float p = exp2_(scaled(s[t][kt][r], a.c) - m[t]) * il[t];
           const float ds = p * (dp[t][kt][r] - delta[t]) * a.scale;
           s[t][kt][r] = masked && j + 16 * kt + 4 * g + r >= lim[t] ? 0.f : ds;
         }
@@ -461,7 +470,7 @@ __device__ __forceinline__ void dkv_fp32(const Attn& a, uint32_t pr, uint32_t k0
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const bool sees = key < Lim[16 * t + 4 * g + r];
-        const float p = sees ? exp2_(s[t][r] * a.c - m[r]) * il[r] : 0.f;
+        const float p = sees ? exp2_(scaled(s[t][r], a.c) - m[r]) * il[r] : 0.f;
         s[t][r] = p;
         dp[t][r] = sees ? p * (dp[t][r] - delta[r]) * a.scale : 0.f;
       }

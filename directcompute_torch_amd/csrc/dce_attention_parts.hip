@@ -71,9 +71,9 @@ struct Parts {
   float* dl;  // delta' 2^e of dO's tile, [problem][q.pad]
 };
 constexpr int kBad = 1 << 20;
-// Does problem pr have a tile that parts do not suit, or (forward) vectors whose
-// scores might pass 2^24, past which they are no place to add an exponent to?  For
-// all threads of the workgroup.
+// Does problem pr have a tile that parts do not suit, or vectors whose scores might
+// pass 2^24, past which they are no place to add an exponent to?  For all threads of
+// the workgroup.
 template <bool BWD>
 __device__ __forceinline__ bool unsuited(const Attn& a, const Parts& ps, uint32_t pr) {
   __shared__ float ends[8][3];
@@ -87,11 +87,11 @@ __device__ __forceinline__ bool unsuited(const Attn& a, const Parts& ps, uint32_
       if (least) *least = fmaxf(*least, -x);
     }
   };
-  take(ps.q.e, nq, BWD ? nullptr : &q);
-  take(ps.k.e, nk, BWD ? nullptr : &k);
+  take(ps.q.e, nq, &q);
+  take(ps.k.e, nk, &k);
   take(ps.v.e, nk, nullptr);
   if (BWD) take(ps.y.e, nq, nullptr);
-  const float w[3] = {wave_reduce(most, OpMaxR()), BWD ? q : wave_reduce(q, OpMaxR()), BWD ? k : wave_reduce(k, OpMaxR())};
+  const float w[3] = {wave_reduce(most, OpMaxR()), wave_reduce(q, OpMaxR()), wave_reduce(k, OpMaxR())};
   if ((threadIdx.x & 63) == 0)
 #pragma unroll
     for (int i = 0; i < 3; ++i) ends[threadIdx.x >> 6][i] = w[i];
@@ -101,7 +101,7 @@ __device__ __forceinline__ bool unsuited(const Attn& a, const Parts& ps, uint32_
     q = fmaxf(q, ends[i][1]);
     k = fmaxf(k, ends[i][2]);
   }
-  return most >= float(kBad) || (!BWD && !(fabsf(a.c) * float(a.D) < pow2(24 - 30 - int(q + k))));
+  return most >= float(kBad) || !(fabsf(a.c) * float(a.D) < pow2(24 - 30 - int(q + k)));
 }
 
 // ---------------------------------------------------------------------------
@@ -307,7 +307,10 @@ __device__ __forceinline__ void split_acc(const f16v& s, int k, h8& h, h8& l) {
   }
 }
 // The tile's vectors times a lane's: out[e] is row 8 (e / 4) + 4 (lane / 32) + e % 4.
-template <int DP>
+// QUERIES: the tile is the one of queries (or dO), and the small products are added
+// in the order in which they are where it is the one of keys, so that all kernels
+// have the same score to the last bit.
+template <int DP, bool QUERIES = false>
 __device__ __forceinline__ f16v scores(const char* S, const h8 (&h)[DP / 16], const h8 (&l)[DP / 16], int col, int half) {
   f16v big, small;
   zero(big);
@@ -316,8 +319,8 @@ __device__ __forceinline__ f16v scores(const char* S, const h8 (&h)[DP / 16], co
   for (int i = 0; i < DP / 16; ++i) {
     const h8 th = PTile<DP>::rows(S, 0, col, 2 * i + half), tl = PTile<DP>::rows(S, 1, col, 2 * i + half);
     big = mma(th, h[i], big);
-    small = mma(th, l[i], small);
-    small = mma(tl, h[i], small);
+    small = QUERIES ? mma(tl, h[i], small) : mma(th, l[i], small);
+    small = QUERIES ? mma(th, l[i], small) : mma(tl, h[i], small);
   }
   return big + small;
 }
@@ -421,13 +424,13 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const uint32_t key = j + 8 * (i >> 2) + 4 * half + (i & 3);
-        s[i] = key < lim ? s[i] * cs : -INFINITY;
+        s[i] = key < lim ? scaled(s[i], cs) : -INFINITY;
         top = fmaxf(top, s[i]);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[i] *= cs;
+        s[i] = scaled(s[i], cs);
         top = fmaxf(top, s[i]);
       }
     }
@@ -579,7 +582,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
         const float cs = cq * pow2(-ek[t]);
         f16v s = scores<DP>(Ks[st], xh, xl, col, half);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = exp2_(s[i] * cs - m);
+        for (int i = 0; i < 16; ++i) s[i] = exp2_(scaled(s[i], cs) - m);
         if (j + kRows > least) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -695,12 +698,12 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
       if (t < t1 && wave_limit(a, t * kRows, kRows, len) > kw) {
         const int xy = ey[t];
         const float cs = ck * pow2(-eq[t]);
-        f16v s = scores<DP>(Qs[st], xh, xl, col, half);
+        f16v s = scores<DP, true>(Qs[st], xh, xl, col, half);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f4 m = *reinterpret_cast<const f4*>(Ms[st] + 8 * q + 4 * half);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[4 * q + e] = s[4 * q + e] * cs - m[e];
+          for (int e = 0; e < 4; ++e) s[4 * q + e] = scaled(s[4 * q + e], cs) - m[e];
         }
         if (limit_of(a, t * kRows, len) < kw + kRows) {
 #pragma unroll

@@ -142,3 +142,33 @@ def test_output_beside_a_key_that_takes_the_weight(eng, apart):
     v[:, ignored] *= np.float32(2.0 ** apart)
     v[:, 630] *= np.float32(2.0 ** -9)
     check(eng, q, k, v, dy, f"a key that takes the weight, values 2^{apart} apart")
+
+
+@pytest.mark.parametrize("keys", [8, N])
+@pytest.mark.parametrize("power", [7, 10, 14])
+def test_scores_far_from_zero(eng, power, keys):
+    """Every row's last key leads by 2^power or more, of scores a thousand times
+    as large, whose own rounding is a part of one or more: P is 1 there all the
+    same.  The output is that key's vector and its gradient the sum of the
+    rows', each off by fp32's roundings of a sum of N terms at most.  The other
+    dims add scores of spread sqrt(63) = 8, differences of less than 64 among
+    these few million: the other keys have e^-(2^7 - 64) of the weight or less."""
+    q, k, v, dy = (a[:, :keys] for a in inputs(209))
+    g = np.float32(2.0 ** (power / 2))
+    q[..., 0] = g
+    k[..., 0] = g * np.arange(1000, 1000 + keys, dtype=np.float32)[None, :, None]
+    dev = lambda a: eng.Tensor(np.array(a, np.float32), requires_grad=True, track=False)  # noqa: E731
+    ts = [dev(a) for a in (q, k, v)]
+    out = eng.attention(*ts, scale=1.0)
+    out.backward(eng.Tensor(dy, track=False))
+    tol = keys * 2.0 ** -24
+    want = dy.astype(np.float64).sum(1)
+    e = [np.abs(out.sync() - v[:, -1:]).max() / np.abs(v).max(),
+         (np.abs(ts[2].grad.sync()[:, -1] - want).max() / np.abs(dy).sum(1).max())]
+    print("scores far from zero", power, keys, ["%.2g" % x for x in e], "tol %.2g" % tol, flush=True)
+    assert max(e) <= max(tol, 2.0 ** -22)
+    assert np.abs(ts[2].grad.data[:, :-1]).max() <= math.exp(-64) * np.abs(dy).sum(1).max()
+    # dS = P (dP - delta): what is left of two sums of D terms that are equal
+    left = 4 * D * 2.0 ** -24 * np.abs(dy).max() * np.abs(v).max() * keys
+    assert np.abs(ts[0].grad.sync()).max() <= left * np.abs(k).max() and np.abs(ts[1].grad.sync()).max() <= left * np.abs(q).max()
+    eng.end_batch()
