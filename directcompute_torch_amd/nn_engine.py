@@ -1279,8 +1279,7 @@ class Muon(_Optimizer):
         self.vectors.t = value
 
     def step(self, clip=1.0):
-        self.vectors.lr = self.lr
-        self.vectors.step(clip)
+        """A call that MuonBatch refuses raises before anything is updated."""
         n = 0
         for p, m in zip(self.matrices, self.m):
             if p.grad is None:
@@ -1295,6 +1294,8 @@ class Muon(_Optimizer):
                                    self.momentum, 1 if self.nesterov else 0, self.lr * self.weight_decay, clip,
                                    self.steps):
             raise RuntimeError(f"MuonBatch failed: {last_error()}")
+        self.vectors.lr = self.lr
+        self.vectors.step(clip)
 
 
 # --------------------------------------------------------------------------
