@@ -565,8 +565,17 @@ struct Places {
   }
 };
 
+// The matrices of one set of launches.
+struct Group {
+  Mats t{};
+  bool big = false, split = false;  // on 128 x 128 tiles; with a Gram product that is split
+  size_t sums = 0, floats = 0;      // the sums' place in the workspace, its size
+};
+
+// Places in the workspace, and splits.
 template <int BLK>
-bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32_t steps) {
+void plan_group(Group& gr) {
+  Mats& t = gr.t;
   constexpr uint32_t depth = Lds<BLK>::DEPTH;
   // A Gram product is split so that no workgroup has more than a quarter of a CU's
   // share of the launch's depth, and none less than 256 (AlexNet's matrices: half a
@@ -581,11 +590,10 @@ bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32
   const double most = std::max(256.0, all / (4.0 * num_cus()));
   Places at;
   uint32_t chunks = 0;
-  bool split = false;
   for (uint32_t i = 0; i < t.count; ++i) {
     Mat& m = t.t[i];
     m.splits = std::min<uint32_t>(cdiv(m.np, depth), std::max<uint32_t>(1, uint32_t(std::ceil(m.np / most))));
-    split |= m.splits > 1;
+    gr.split |= m.splits > 1;
     const size_t xn = size_t(m.mp) * m.np, an = size_t(m.mp) * m.mp;
     m.x = at.take(xn);
     m.xp = at.take(xn);
@@ -600,11 +608,15 @@ bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32
     m.sums = chunks;
     chunks += m.chunks;
   }
-  const size_t sums = at.take(size_t(2) * chunks);
-  float* ws = workspace(at.next * 64);
-  if (!ws) return false;
-  double* dsum = reinterpret_cast<double*>(ws + sums * 64);
+  gr.sums = size_t(at.take(size_t(2) * chunks)) * 64;
+  gr.floats = at.next * 64;
+}
 
+template <int BLK>
+bool run_group(Group& gr, float* ws, float mu, bool nesterov, float decay, float clip, uint32_t steps) {
+  Mats& t = gr.t;
+  auto tri = [](const Mat& m) { return m.mp / BLK * (m.mp / BLK + 1) / 2; };
+  double* dsum = reinterpret_cast<double*>(ws + gr.sums);
   uint32_t n = blocks(t, [](const Mat& m) { return m.chunks; });
   hipLaunchKernelGGL(k_muon_momentum, dim3(n), dim3(kT), 0, stream(), t, ws, dsum, mu, clip, int(nesterov));
   n = blocks(t, [](const Mat& m) { return m.mp / kSq * (m.np / kSq); });
@@ -612,7 +624,7 @@ bool run_group(Mats& t, float mu, bool nesterov, float decay, float clip, uint32
   for (uint32_t s = 0; s < steps; ++s) {
     n = blocks(t, [&](const Mat& m) { return tri(m) * m.splits; });
     hipLaunchKernelGGL((k_muon_product<GRAM, BLK>), dim3(n), dim3(kT), 0, stream(), t, ws, s & 1, decay);
-    if (split) {
+    if (gr.split) {
       n = blocks(t, [&](const Mat& m) { return m.splits > 1 ? tri(m) * (BLK / 16) : 0; });
       hipLaunchKernelGGL(k_muon_sum<BLK>, dim3(n), dim3(kT), 0, stream(), t, ws);
     }
@@ -675,23 +687,35 @@ bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* row
       return false;
     }
   ProfScope prof("muon", flops, bytes);
-  // Groups of up to kMaxM matrices, and of up to 2^28 values unless one is larger.
+  // Groups of up to kMaxM matrices, and of up to 2^28 values (padded to whole tiles, a
+  // thin matrix being up to 128 times its size) unless one is larger.
   // Tiles by the operations of a step (us on 128 / on 64): 1024 x 1024 435 / 281,
   // 1536 x 1536 (1.4e10) 649 / 571, four 768 x 768 with two 768 x 2000 (1.5e10)
   // 631 / 578, 2048 x 2048 (3.4e10) 914 / 1032, 2048 x 4096 1336 / 1652.
+  std::vector<Group> groups;
+  size_t floats = 0;
+  auto padded = [](const Mat& m) { return size_t(pad(m.m, 128)) * pad(m.n, 128); };
   for (size_t i = 0; i < all.size();) {
-    Mats t{};
+    Group gr;
+    Mats& t = gr.t;
     size_t values = 0;
     double work = 0;  // of a step
     while (i < all.size() && t.count < uint32_t(kMaxM) &&
-           (!t.count || values + size_t(all[i].m) * all[i].n <= (size_t(1) << 28))) {
-      values += size_t(all[i].m) * all[i].n;
+           (!t.count || values + padded(all[i]) <= (size_t(1) << 28))) {
+      values += padded(all[i]);
       work += (3.0 * all[i].n + all[i].m) * all[i].m * all[i].m;
       t.t[t.count++] = all[i++];
     }
-    const bool big = work >= 2.2e10;
-    if (!(big ? run_group<128> : run_group<64>)(t, mu, nesterov, decay, clip, steps)) return false;
+    gr.big = work >= 2.2e10;
+    (gr.big ? plan_group<128> : plan_group<64>)(gr);
+    floats = std::max(floats, gr.floats);
+    groups.push_back(gr);
   }
+  // The largest group's, before any launch: a call that it does not fit changes nothing.
+  float* ws = workspace(floats);
+  if (!ws) return false;
+  for (Group& gr : groups)
+    if (!(gr.big ? run_group<128> : run_group<64>)(gr, ws, mu, nesterov, decay, clip, steps)) return false;
   return true;
 }
 
