@@ -53,3 +53,30 @@ def test_thin_matrices_share_a_bounded_workspace(eng):
         want = -gs[i % 2].astype(np.float64) / np.linalg.norm(gs[i % 2].astype(np.float64)) * s * math.sqrt(n)
         # each step is off by 4 * 2^-23 of X, which the others grow by 3.4445 at most
         assert rel2(w.sync()[0], want) <= 485 * 4 * 2.0 ** -23 / abs(s)
+
+
+@pytest.mark.parametrize("steps", [2, 5])
+def test_large_and_small_matrices_in_one_call(eng, steps):
+    """128 x 128 tiles over several steps: a tall and a wide ragged matrix whose
+    Gram products are split, beside small ones whose are not.  A step rounds its
+    products to 4 * 2^-23 of |X|, and the steps grow |X_0| = 1 by 3.4445 each at
+    most: steps * 4 * 2^-23 * 3.4445^steps over the result's length; and the update
+    is rounded."""
+    r = rng(3)
+    shapes = [(4100, 2050), (33, 70), (700, 2300), (5, 5), (130, 3, 3, 3)]
+    ws = [dev(eng, np.zeros(s), True) for s in shapes]
+    gs = [r.standard_normal(s).astype(np.float32) for s in shapes]
+    for w, g in zip(ws, gs):
+        w.grad = dev(eng, g)
+    eng.Muon(ws, lr=1.0, momentum=0.0, nesterov=False, steps=steps, rms=1.0).step(clip=1e30)
+    for w, g in zip(ws, gs):
+        x = g.astype(np.float64).reshape(g.shape[0], -1)
+        tall = x.shape[0] > x.shape[1]
+        x = (x.T if tall else x) / np.linalg.norm(x)
+        for _ in range(steps):
+            a = x @ x.T
+            x = 3.4445 * x + (-4.7750 * a + 2.0315 * (a @ a)) @ x
+        want = -(x.T if tall else x).reshape(g.shape) * math.sqrt(max(x.shape))
+        e, tol = rel2(w.sync(), want), steps * 4 * 2.0 ** -23 * 3.4445 ** steps / np.linalg.norm(x) + 4 * 2.0 ** -24
+        print(g.shape, steps, "%.2g of %.2g" % (e, tol), flush=True)
+        assert e <= tol, g.shape
