@@ -4,6 +4,7 @@ import math
 
 import numpy as np
 import pytest
+import torch   # ahead of the engine, which then shares its HIP runtime
 
 from tests.helpers import rel2, rng
 
@@ -31,7 +32,6 @@ def test_thin_matrices_share_a_bounded_workspace(eng):
     """Sixteen rows of a million values in one call, each 64 times its size where
     it is padded to whole tiles (1 GB with its parts), take turns.  A row's X is
     d / |d| times what the quintic makes of 1 in five steps."""
-    import torch
     n = 1 << 20
     r = rng(2)
     gs = [r.standard_normal(n).astype(np.float32) for _ in range(2)]
