@@ -29,19 +29,19 @@ namespace {
 constexpr int kT = 256;   // threads: four waves
 constexpr int kFew = 64;  // keys of a tile in the kernel for few rows
 
-template <int DP, int QT, bool VEC>
+template <int DP, bool VEC>
 __global__ void __launch_bounds__(kT) k_attn_fwd(const Attn a) {
   __shared__ __attribute__((aligned(16))) float Ks[kKeys * DP], Vs[kKeys * DP];
   const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
   const uint32_t back = rest / a.splits, sp = rest - back * a.splits;
-  fwd_fp32<DP, QT, VEC>(a, pr, (a.tiles - 1 - back) * 64 * QT, sp, Ks, Vs);
+  fwd_fp32<DP, VEC>(a, pr, (a.tiles - 1 - back) * 64, sp, Ks, Vs);
 }
-template <int DP, int QT, bool VEC>
+template <int DP, bool VEC>
 __global__ void __launch_bounds__(kT) k_attn_dq(const Attn a) {
   __shared__ __attribute__((aligned(16))) float Ks[kKeys * DP], Vs[kKeys * DP];
   const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
   const uint32_t back = rest / a.splits, sp = rest - back * a.splits;
-  dq_fp32<DP, QT, VEC, kT>(a, pr, (a.tiles - 1 - back) * 64 * QT, sp, Ks, Vs);
+  dq_fp32<DP, VEC, kT>(a, pr, (a.tiles - 1 - back) * 64, sp, Ks, Vs);
 }
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(kT) k_attn_dkv(const Attn a) {
@@ -275,11 +275,9 @@ struct FwdRun {
   Attn a;
   template <int DP, bool VEC>
   bool run() {
-    constexpr int QT = DP <= 128 ? 2 : 1;
     const uint32_t cus = uint32_t(num_cus()), prob = a.B * a.G;
     const bool few = a.N <= 16;
-    const bool wide = QT == 2 && uint64_t(cdiv(a.N, 128)) * prob >= 2 * cus;
-    a.tiles = cdiv(a.N, wide ? 128 : 64);
+    a.tiles = cdiv(a.N, 64);
     const uint32_t kt = cdiv(a.T, few ? kFew : kKeys);
     a.splits = 1;
     if (few)
@@ -304,10 +302,8 @@ struct FwdRun {
       hipLaunchKernelGGL((k_attn_few<DP, VEC, true>), grid, dim3(kT), 0, stream(), a);
     else if (few)
       hipLaunchKernelGGL((k_attn_few<DP, VEC, false>), grid, dim3(kT), 0, stream(), a);
-    else if (wide)
-      hipLaunchKernelGGL((k_attn_fwd<DP, QT, VEC>), grid, dim3(kT), 0, stream(), a);
     else
-      hipLaunchKernelGGL((k_attn_fwd<DP, 1, VEC>), grid, dim3(kT), 0, stream(), a);
+      hipLaunchKernelGGL((k_attn_fwd<DP, VEC>), grid, dim3(kT), 0, stream(), a);
     if (!check_launch("AttentionForward")) return false;
     return a.splits == 1 || attn_join(a);
   }
@@ -318,18 +314,13 @@ struct BwdRun {
   float* more;  // the splits' shares
   template <int DP, bool VEC>
   bool run() {
-    constexpr int QT = DP <= 64 ? 2 : 1;
     const uint32_t prob = a.B * a.G;
-    const bool wide = QT == 2 && uint64_t(cdiv(a.N, 128)) * prob >= 2 * uint32_t(num_cus());
     Attn q = a;
-    q.tiles = cdiv(a.N, wide ? 128 : 64);
+    q.tiles = cdiv(a.N, 64);
     q.splits = a.dq ? key_splits(a, 64) : 1;
     if (q.splits > 1) q.dq = more;
     const dim3 grid(q.tiles * q.splits * prob);
-    if (wide)
-      hipLaunchKernelGGL((k_attn_dq<DP, QT, VEC>), grid, dim3(kT), 0, stream(), q);
-    else
-      hipLaunchKernelGGL((k_attn_dq<DP, 1, VEC>), grid, dim3(kT), 0, stream(), q);
+    hipLaunchKernelGGL((k_attn_dq<DP, VEC>), grid, dim3(kT), 0, stream(), q);
     if (!check_launch("AttentionBackward (dQ)")) return false;
     if (q.splits > 1 && !attn_sum(q.dq, a.dq, nullptr, nullptr, size_t(prob) * a.N * a.D, q.splits)) return false;
     if (!a.dk && !a.dv) return true;

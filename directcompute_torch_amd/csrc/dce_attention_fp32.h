@@ -129,35 +129,27 @@ __device__ __forceinline__ BRes rows_view(const float* p, uint32_t n, uint32_t s
 }
 
 // ---------------------------------------------------------------------------
-// Forward of the 64 QT query rows from n0 on (16 QT per wave, in registers): key
-// tiles through LDS, the next tile's loads in flight while one is multiplied.
+// Forward of the 64 query rows from n0 on (16 per wave, in registers): key tiles
+// through LDS, the next tile's loads in flight while one is multiplied.  Twice the
+// rows, which would reuse each fragment, hold the registers of two waves: 64 x 64
+// tokens, 16 heads of 64, 27.7 us against 17.5; 64 x 24 rows over 4096 keys, 64
+// heads of 64 on 8, 1195 against 1000.
 // ---------------------------------------------------------------------------
-template <int DP, int QT, bool VEC>
+template <int DP, bool VEC>
 __device__ __forceinline__ void fwd_fp32(const Attn& a, uint32_t pr, uint32_t n0, uint32_t sp, float* Ks, float* Vs) {
   using TL = Tile<DP, kKeys, VEC, 256>;
   using CL = Cols<DP>;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const uint32_t len = keys_of(a, b);
-  const uint32_t least = limit_of(a, n0, len), most = limit_of(a, min(n0 + 64 * QT, a.N) - 1, len);
-  const uint32_t mine = wave_limit(a, n0 + wave * 16 * QT, 16 * QT, len);
+  const uint32_t least = limit_of(a, n0, len), most = limit_of(a, min(n0 + 64, a.N) - 1, len);
+  const uint32_t mine = wave_limit(a, n0 + wave * 16, 16, len);
+  const uint32_t n = n0 + wave * 16 + col, lim = n < a.N ? limit_of(a, n, len) : 0u;
 
-  f4 q[QT][DP / 16];
-  uint32_t lim[QT];
+  f4 q[DP / 16], o[DP / 16];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const uint32_t n = n0 + (wave * QT + t) * 16 + col;
-    lim[t] = n < a.N ? limit_of(a, n, len) : 0u;
-  }
-  f4 o[QT][DP / 16];
-  float m[QT], l[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    m[t] = -INFINITY;
-    l[t] = 0.f;
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i) o[t][i] = f4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int i = 0; i < DP / 16; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
   const uint32_t stride = a.G * a.D;
   const uint32_t j0 = sp * a.perSplit * kKeys, j1 = min(most, (sp + 1) * a.perSplit * kKeys);
   f4 rk[TL::LOADS], rv[TL::LOADS];
@@ -167,11 +159,7 @@ __device__ __forceinline__ void fwd_fp32(const Attn& a, uint32_t pr, uint32_t n0
     TL::load(rows_view(a.v + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rv);
   };
   if (j0 < j1) fetch(j0);
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const uint32_t n = n0 + (wave * QT + t) * 16 + col;
-    load_frag<DP, VEC>(a.q + q_at(a, b, gh, min(n, a.N - 1)), true, a.D, g, q[t]);
-  }
+  load_frag<DP, VEC>(a.q + q_at(a, b, gh, min(n, a.N - 1)), true, a.D, g, q);
   for (uint32_t j = j0; j < j1; j += kKeys) {
     __syncthreads();
     TL::store(Ks, rk);
@@ -180,51 +168,45 @@ __device__ __forceinline__ void fwd_fp32(const Attn& a, uint32_t pr, uint32_t n0
     if (j + kKeys < j1) fetch(j + kKeys);
     if (j >= mine) continue;
     // S^T: keys 16 kt + 4 g + r of query `col`
-    f4 s[QT][2];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) s[t][0] = s[t][1] = f4{0.f, 0.f, 0.f, 0.f};
+    f4 s[2];
+    s[0] = s[1] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         const f4 kf = TL::chunk(Ks, 16 * kt + col, 4 * i + g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int t = 0; t < QT; ++t) s[t][kt] = mfma4(kf[e], q[t][i][e], s[t][kt]);
+        for (int e = 0; e < 4; ++e) s[kt] = mfma4(kf[e], q[i][e], s[kt]);
       }
     const bool masked = j + kKeys > least;
+    float top = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      float top = -INFINITY;
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = scaled(s[t][kt][r], a.c);
-          if (masked && j + 16 * kt + 4 * g + r >= lim[t]) x = -INFINITY;
-          s[t][kt][r] = x;
-          top = fmaxf(top, x);
-        }
-      top = fmaxf(m[t], max_g(top));
-      const float base = top == -INFINITY ? 0.f : top;  // nothing seen yet: every p is 0
-      if (__any(top > m[t])) {
-        const float down = exp2_(m[t] - base);
-        l[t] *= down;
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[t][i][r] *= down;
-        m[t] = top;
+      for (int r = 0; r < 4; ++r) {
+        float x = scaled(s[kt][r], a.c);
+        if (masked && j + 16 * kt + 4 * g + r >= lim) x = -INFINITY;
+        s[kt][r] = x;
+        top = fmaxf(top, x);
       }
+    top = fmaxf(m, max_g(top));
+    const float base = top == -INFINITY ? 0.f : top;  // nothing seen yet: every p is 0
+    if (__any(top > m)) {
+      const float down = exp2_(m - base);
+      l *= down;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[t][kt][r] = exp2_(s[t][kt][r] - base);
-          l[t] += s[t][kt][r];
-        }
+        for (int r = 0; r < 4; ++r) o[i][r] *= down;
+      m = top;
     }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[kt][r] = exp2_(s[kt][r] - base);
+        l += s[kt][r];
+      }
     // O^T += V^T P^T
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -234,67 +216,52 @@ __device__ __forceinline__ void fwd_fp32(const Attn& a, uint32_t pr, uint32_t n0
         for (int p = 0; p < CL::NG; ++p) {
           const typename CL::V vf = CL::read(Vs, 16 * kt + 4 * g + r, p, col);
 #pragma unroll
-          for (int e = 0; e < CL::EG; ++e)
-#pragma unroll
-            for (int t = 0; t < QT; ++t)
-              o[t][p * CL::EG + e] = mfma4(vf[e], s[t][kt][r], o[t][p * CL::EG + e]);
+          for (int e = 0; e < CL::EG; ++e) o[p * CL::EG + e] = mfma4(vf[e], s[kt][r], o[p * CL::EG + e]);
         }
   }
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const uint32_t n = n0 + (wave * QT + t) * 16 + col;
-    const float sum = sum_g(l[t]);
-    if (n >= a.N) continue;
-    if (a.splits > 1) {
-      const size_t row = (size_t(sp) * a.B * a.G + pr) * a.N + n;
-      if (g == 0) {
-        a.pm[row] = m[t];
-        a.pl[row] = sum;
-      }
-      CL::template write<VEC>(a.po + row * a.D, a.D, g, o[t], 1.f);
-      continue;
+  const float sum = sum_g(l);
+  if (n >= a.N) return;
+  if (a.splits > 1) {
+    const size_t row = (size_t(sp) * a.B * a.G + pr) * a.N + n;
+    if (g == 0) {
+      a.pm[row] = m;
+      a.pl[row] = sum;
     }
-    const float il = lim[t] ? 1.f / sum : 0.f;  // a row that sees nothing: zeros
-    if (a.m && g == 0) {
-      a.m[size_t(pr) * a.N + n] = lim[t] ? m[t] : 0.f;
-      a.il[size_t(pr) * a.N + n] = il;
-    }
-    CL::template write<VEC>(a.o + q_at(a, b, gh, n), a.D, g, o[t], il);
+    CL::template write<VEC>(a.po + row * a.D, a.D, g, o, 1.f);
+    return;
   }
+  const float il = lim ? 1.f / sum : 0.f;  // a row that sees nothing: zeros
+  if (a.m && g == 0) {
+    a.m[size_t(pr) * a.N + n] = lim ? m : 0.f;
+    a.il[size_t(pr) * a.N + n] = il;
+  }
+  CL::template write<VEC>(a.o + q_at(a, b, gh, n), a.D, g, o, il);
 }
 
 // ---------------------------------------------------------------------------
-// dQ of NT / 4 QT rows: as the forward, dQ^T += K^T dS^T.  Also leaves delta for
-// the other kernel.
+// dQ of NT / 4 rows: as the forward, dQ^T += K^T dS^T.  Also leaves delta for the
+// other kernel.
 // ---------------------------------------------------------------------------
-template <int DP, int QT, bool VEC, int NT>
+template <int DP, bool VEC, int NT>
 __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0, uint32_t sp, float* Ks, float* Vs) {
   using TL = Tile<DP, kKeys, VEC, NT>;
   using CL = Cols<DP>;
-  constexpr uint32_t ROWS = NT / 4 * QT;
+  constexpr uint32_t ROWS = NT / 4;
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const uint32_t len = keys_of(a, b);
   const uint32_t least = limit_of(a, n0, len), most = limit_of(a, min(n0 + ROWS, a.N) - 1, len);
-  const uint32_t mine = wave_limit(a, n0 + wave * 16 * QT, 16 * QT, len);
+  const uint32_t mine = wave_limit(a, n0 + wave * 16, 16, len);
 
-  f4 q[QT][DP / 16], dy[QT][DP / 16], o[QT][DP / 16], dq[QT][DP / 16];
-  uint32_t lim[QT];
-  float m[QT], il[QT], delta[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const uint32_t n = n0 + (wave * QT + t) * 16 + col;
-    // Rows past the last are computed as it (without a branch, behind which every
-    // load would wait for the one before) and not written.
-    const uint32_t nn = min(n, a.N - 1);
-    const size_t at = q_at(a, b, gh, nn), row = size_t(pr) * a.N + nn;
-    lim[t] = limit_of(a, nn, len);
-    m[t] = a.m[row];
-    il[t] = a.il[row];
-    load_frag<DP, VEC>(a.dy + at, true, a.D, g, dy[t]);
-    load_frag<DP, VEC>(a.o + at, true, a.D, g, o[t]);
-    load_frag<DP, VEC>(a.q + at, true, a.D, g, q[t]);
-  }
+  f4 q[DP / 16], dy[DP / 16], o[DP / 16], dq[DP / 16];
+  // Rows past the last are computed as it (without a branch, behind which every
+  // load would wait for the one before) and not written.
+  const uint32_t n = n0 + wave * 16 + col, nn = min(n, a.N - 1), lim = limit_of(a, nn, len);
+  const size_t at = q_at(a, b, gh, nn), row = size_t(pr) * a.N + nn;
+  const float m = a.m[row], il = a.il[row];
+  load_frag<DP, VEC>(a.dy + at, true, a.D, g, dy);
+  load_frag<DP, VEC>(a.o + at, true, a.D, g, o);
+  load_frag<DP, VEC>(a.q + at, true, a.D, g, q);
   uint32_t j0, j1;
   split_keys(a, most, sp, j0, j1);
   const uint32_t stride = a.G * a.D;
@@ -305,19 +272,15 @@ __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0,
     TL::load(rows_view(a.v + k_at(a, b, gh, j), n, stride, a.D), stride, a.D, rv);
   };
   if (a.dq && j0 < j1) fetch(j0);
+  float d = 0.f;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const uint32_t n = n0 + (wave * QT + t) * 16 + col;
-    float d = 0.f;
+  for (int i = 0; i < DP / 16; ++i) {
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) d += dy[t][i][e] * o[t][i][e];
-      dq[t][i] = f4{0.f, 0.f, 0.f, 0.f};
-    }
-    delta[t] = sum_g(d);
-    if (n < a.N && g == 0) a.delta[size_t(pr) * a.N + n] = delta[t];
+    for (int e = 0; e < 4; ++e) d += dy[i][e] * o[i][e];
+    dq[i] = f4{0.f, 0.f, 0.f, 0.f};
   }
+  const float delta = sum_g(d);
+  if (n < a.N && g == 0) a.delta[size_t(pr) * a.N + n] = delta;
   if (!a.dq) return;
   for (uint32_t j = j0; j < j1; j += kKeys) {
     __syncthreads();
@@ -326,10 +289,8 @@ __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0,
     __syncthreads();
     if (j + kKeys < j1) fetch(j + kKeys);
     if (j >= mine) continue;
-    f4 s[QT][2], dp[QT][2];
-#pragma unroll
-    for (int t = 0; t < QT; ++t)
-      s[t][0] = s[t][1] = dp[t][0] = dp[t][1] = f4{0.f, 0.f, 0.f, 0.f};
+    f4 s[2], dp[2];
+    s[0] = s[1] = dp[0] = dp[1] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
@@ -337,24 +298,20 @@ __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0,
         const f4 kf = TL::chunk(Ks, 16 * kt + col, 4 * i + g);
         const f4 vf = TL::chunk(Vs, 16 * kt + col, 4 * i + g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int t = 0; t < QT; ++t) {
-            s[t][kt] = mfma4(kf[e], q[t][i][e], s[t][kt]);
-            dp[t][kt] = mfma4(vf[e], dy[t][i][e], dp[t][kt]);
-          }
+        for (int e = 0; e < 4; ++e) {
+          s[kt] = mfma4(kf[e], q[i][e], s[kt]);
+          dp[kt] = mfma4(vf[e], dy[i][e], dp[kt]);
+        }
       }
     const bool masked = j + kKeys > least;
 #pragma unroll
-    for (int t = 0; t < QT; ++t)
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float p = exp2_(scaled(s[t][kt][r], a.c) - m[t]) * il[t];
-          const float ds = p * (dp[t][kt][r] - delta[t]) * a.scale;
-          s[t][kt][r] = masked && j + 16 * kt + 4 * g + r >= lim[t] ? 0.f : ds;
-        }
+      for (int r = 0; r < 4; ++r) {
+        const float p = exp2_(scaled(s[kt][r], a.c) - m) * il;
+        const float ds = p * (dp[kt][r] - delta) * a.scale;
+        s[kt][r] = masked && j + 16 * kt + 4 * g + r >= lim ? 0.f : ds;
+      }
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -363,17 +320,10 @@ __device__ __forceinline__ void dq_fp32(const Attn& a, uint32_t pr, uint32_t n0,
         for (int p = 0; p < CL::NG; ++p) {
           const typename CL::V kf = CL::read(Ks, 16 * kt + 4 * g + r, p, col);
 #pragma unroll
-          for (int e = 0; e < CL::EG; ++e)
-#pragma unroll
-            for (int t = 0; t < QT; ++t)
-              dq[t][p * CL::EG + e] = mfma4(kf[e], s[t][kt][r], dq[t][p * CL::EG + e]);
+          for (int e = 0; e < CL::EG; ++e) dq[p * CL::EG + e] = mfma4(kf[e], s[kt][r], dq[p * CL::EG + e]);
         }
   }
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const uint32_t n = n0 + (wave * QT + t) * 16 + col;
-    if (n < a.N) CL::template write<VEC>(a.dq + dq_part(a, sp) + q_at(a, b, gh, n), a.D, g, dq[t], 1.f);
-  }
+  if (n < a.N) CL::template write<VEC>(a.dq + dq_part(a, sp) + q_at(a, b, gh, n), a.D, g, dq, 1.f);
 }
 
 // ---------------------------------------------------------------------------

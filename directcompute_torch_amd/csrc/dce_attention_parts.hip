@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Pa
   const uint32_t back = rest / a.splits, sp = rest - back * a.splits, tile = a.tiles - 1 - back;
   if (unsuited<false>(a, ps, pr)) {
     for (uint32_t n = tile * 128; n < min(tile * 128 + 128, a.N); n += 64)
-      fwd_fp32<DP, 1, VEC>(a, pr, n, sp, reinterpret_cast<float*>(Ks), reinterpret_cast<float*>(Vs));
+      fwd_fp32<DP, VEC>(a, pr, n, sp, reinterpret_cast<float*>(Ks), reinterpret_cast<float*>(Vs));
     return;
   }
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
   const uint32_t prob = a.B * a.G, rest = blockIdx.x / prob, pr = blockIdx.x - rest * prob;
   const uint32_t back = rest / a.splits, sp = rest - back * a.splits, tile = a.tiles - 1 - back;
   if (unsuited<true>(a, ps, pr))
-    return dq_fp32<DP, 1, VEC, kPair>(a, pr, tile * 128, sp, reinterpret_cast<float*>(Ks[0]),
+    return dq_fp32<DP, VEC, kPair>(a, pr, tile * 128, sp, reinterpret_cast<float*>(Ks[0]),
                                       reinterpret_cast<float*>(Vs[0]));
   const uint32_t b = fdiv(pr, a.dG), gh = pr - b * a.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blk = wave & 3, col = lane & 31, half = lane >> 5;
