@@ -179,7 +179,7 @@ class Tensor:
 
     `data` is the host array the tensor was built from, or the array that
     sync() last filled; device work never updates it by itself."""
-    __slots__ = ["data", "shape", "size", "requires_grad", "grad", "gpu_buf", "_ctx", "_cached_topo"]
+    __slots__ = ["data", "shape", "size", "requires_grad", "grad", "gpu_buf", "_ctx", "_cached_topo", "_lent"]
 
     def __init__(self, data, requires_grad=False, track=True):
         arr = data if isinstance(data, np.ndarray) else np.array(data, dtype=np.float32)
@@ -195,6 +195,7 @@ class Tensor:
         self.size = _shape_size(shape)
         self.requires_grad = requires_grad
         self.grad = None
+        self._lent = False
         self.gpu_buf = handle
         self._ctx = None
         if track:
@@ -284,11 +285,17 @@ class Tensor:
             if ctx and node.grad is not None:
                 ctx.backward(node.grad)
 
-    def _accumulate_grad(self, grad):
+    def _accumulate_grad(self, grad, lent=False):
         """First gradient is aliased; later ones are added in place with
-        grad_accum (nn_engine.py:605-610)."""
+        grad_accum (nn_engine.py:605-610), but to a buffer of their own where the
+        first is `lent`: the gradient of the node's output handed on, which the
+        caller or another input of that node (of add, say) may have yet to read."""
         if self.grad is None or self.grad.gpu_buf is None:
-            self.grad = grad
+            self.grad, self._lent = grad, lent
+        elif self._lent:
+            h = _new(self.size, "grad_accum")
+            _dispatch(b"add", (self.grad.gpu_buf, grad.gpu_buf), (h,), (self.size + 255) // 256, 1, 1, u1=self.size, u2=1)
+            self.grad, self._lent = Tensor.from_gpu(h, self.shape, track=True), False
         else:
             _dispatch(b"grad_accum", (grad.gpu_buf,), (self.grad.gpu_buf,),
                       (self.size + 255) // 256, 1, 1, u1=self.size)
@@ -476,7 +483,7 @@ class Flatten(Function):
     def backward(self, grad_output):
         lib.AddRefBuffer(grad_output.gpu_buf)
         self.inputs[0]._accumulate_grad(
-            Tensor.from_gpu(grad_output.gpu_buf, self.inputs[0].shape, track=False))
+            Tensor.from_gpu(grad_output.gpu_buf, self.inputs[0].shape, track=False), lent=True)
 
 
 def _bias_grad(g_tensor, rows, n):
@@ -498,7 +505,7 @@ class AddBias(Function):
     def backward(self, grad_output):
         A, B = self.inputs
         if A.requires_grad:
-            A._accumulate_grad(grad_output)
+            A._accumulate_grad(grad_output, lent=True)
         if B.requires_grad:
             B._accumulate_grad(Tensor.from_gpu(_bias_grad(grad_output, grad_output.shape[0], B.size),
                                                B.shape, track=True))
@@ -712,7 +719,7 @@ class AddFunc(Function):
         for t in (A, B):
             if t.requires_grad:
                 lib.AddRefBuffer(grad_output.gpu_buf)
-                t._accumulate_grad(Tensor.from_gpu(grad_output.gpu_buf, t.shape, track=False))
+                t._accumulate_grad(Tensor.from_gpu(grad_output.gpu_buf, t.shape, track=False), lent=True)
 
 
 class DepthwiseConv2DFunc(Function):
@@ -850,7 +857,7 @@ class Reshape(Function):
         x = self.inputs[0]
         if x.requires_grad:
             lib.AddRefBuffer(grad_output.gpu_buf)
-            x._accumulate_grad(Tensor.from_gpu(grad_output.gpu_buf, x.shape, track=False))
+            x._accumulate_grad(Tensor.from_gpu(grad_output.gpu_buf, x.shape, track=False), lent=True)
 
 
 class RotaryFunc(Function):
