@@ -20,6 +20,7 @@
 // A larger term scales the column's sum down, which few tiles past the first need.
 // (One exponent for all columns, from a bound on dS, left dK 8 bits where other
 // rows' gradients were 2^18 larger.)
+//
 // The backward's 1 / l goes into dO (dO' = dO / l) when that is split, so that
 // dV = P^T dO' and dS = scale P (dO' V^T - delta'), delta' = rowsum(dO' * O).
 #include "dce_attention_fp32.h"
@@ -34,7 +35,7 @@ constexpr int kT = 256;
 constexpr int kRows = 32;         // vectors of a tile
 constexpr int kRange = 30;        // exponents of values that parts are made of
 constexpr int kRangeGrad = 60;    // and of gradients
-constexpr float kWide = 4096.f;  // largest ratio of the vectors' sizes in a tile
+constexpr float kWide = 4096.f;   // largest ratio of the vectors' sizes in a tile
 constexpr int kZeros = 15 + kRange, kZerosGrad = 15 + kRangeGrad;  // exponents of tiles of zeros, larger than any other
 // A column's parts of P or dS are made with its largest value in [2^kTop, 2^(kTop + 1));
 // a later tile's may go up to 2^kFull before the column's sum is scaled down.
@@ -370,8 +371,8 @@ __device__ __forceinline__ void write_vec(float* p, uint32_t D, int half, const 
 
 // ---------------------------------------------------------------------------
 // Forward: 128 query rows per workgroup, 32 per wave, in registers.  2 x 4096
-// tokens, 16 heads of 128, causal: 450 us, 306 TFLOP/s of fp32 products; the MFMAs
-// are busy 44 % of a clock that power holds at 1.9 GHz.
+// tokens, 16 heads of 128, causal: 442-450 us, 306-311 TFLOP/s of fp32 products; the
+// MFMAs are busy 46 % of a clock that power holds at 1.95 GHz.
 // ---------------------------------------------------------------------------
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(kT, 2) k_attn_fwd_parts(const Attn a, const Parts ps) {
@@ -528,9 +529,9 @@ __device__ __forceinline__ void fit_column(f16v& f, int unit, int& A, f16v (&acc
 }
 
 // ---------------------------------------------------------------------------
-// dQ (2 x 4096 tokens, 16 heads of 128, causal: 690 us, 299 TFLOP/s in three
+// dQ (2 x 4096 tokens, 16 heads of 128, causal: 656-683 us, 302-314 TFLOP/s in three
 // products): 128 query rows per workgroup; Q in the first waves' registers, dO' and the
-// sums in the second ones'.
+// sums in the second ones'.  A row's exponent costs 2 % of a training pass.
 // ---------------------------------------------------------------------------
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const Parts ps) {
@@ -627,9 +628,9 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dq_parts(const Attn a, const 
 }
 
 // ---------------------------------------------------------------------------
-// dK, dV (likewise: 840 us, 327 TFLOP/s in four): 128 keys per workgroup; K and dV's sums in the first waves' registers,
-// V and dK's in the second ones'; tiles of query rows of every head that shares
-// the keys through LDS.
+// dK, dV (likewise: 817-838 us, 328-336 TFLOP/s in four): 128 keys per workgroup; K
+// and dV's sums in the first waves' registers, V and dK's in the second ones'; tiles
+// of query rows of every head that shares the keys through LDS.
 // ---------------------------------------------------------------------------
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const Parts ps) {

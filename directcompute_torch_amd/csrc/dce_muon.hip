@@ -23,7 +23,10 @@
 // values by 1, and the quintic's largest value on [0, 1.21] is 1.21), |A| <=
 // 1.47, |B| <= 2.81.  X is normalised, so its typical value is at least 2^-16
 // and l's smallest step, 2^-39, is below the fp32 rounding of such a value.  X
-// itself stays in fp32, for the term a X.  The two small products have an
+// itself stays in fp32, for the term a X.  Errors are fp32's relative to the whole
+// matrix, and to each row down to rows 2^-16 of the largest; one of 2^-20 is off by
+// 2e-5 of its own length, one of 2^-24 by 3e-4, in an update that is as much smaller
+// than the other rows'.  The two small products have an
 // accumulator of their own: an MFMA cuts what it adds off at the scale of the
 // largest addend, always downwards.
 #include "dce_internal.h"

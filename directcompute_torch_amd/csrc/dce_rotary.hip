@@ -141,7 +141,9 @@ bool rotary(const float* x, const float* table, const float* pos, float* y, uint
   const double bytes = 8.0 * tokens * H * D;
   ProfScope prof("rotary", 3.0 * tokens * H * rot, bytes);
   const uint64_t vectors = uint64_t(tokens) * H;
-  // Whole quads of pairs' values, and vectors that fit a wave.
+  // Whole quads of pairs' values, and vectors that fit a wave: 4 x 4096 tokens of 32
+  // heads of 128, 96 turned, 83 us (212 pair by pair), interleaved 90 (158); one token
+  // or 3 x 1001 the same.  Other widths run pair by pair: 60 of 80 turned 142 us, 2.4 TB/s.
   const bool quads = rot % (interleaved ? 4 : 8) == 0 && D % 4 == 0 && D <= 256;
   a.units = quads ? D / 4 : rot / 2 + (D - rot);
   a.per = 64 / (D / 4 ? D / 4 : 1);

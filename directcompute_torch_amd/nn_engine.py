@@ -5,7 +5,8 @@ functional ops, layers, Model, SGD / AdamW / Adam, Metrics, end_batch, pool
 helpers), driving ``libdcengine.so`` through ctypes instead of engine.dll.
 The buffer-handle protocol is the reference's: every op asks the library for
 new handles, ``Tensor.from_gpu`` wraps them, ``_accumulate_grad`` aliases the
-first gradient and adds later ones in place (nn_engine.py:575-610).
+first gradient and adds later ones in place (nn_engine.py:575-610), or to a
+buffer of their own where the first is also another's.
 
 Importing this module initialises the HIP device (as the reference
 initialises D3D11 at import, nn_engine.py:121) and raises if that fails --

@@ -265,7 +265,9 @@ void AttentionBackward(void* gradOut, void* out, void* q, void* k, void* v, void
  * momentum * m (nesterov) or m, X = d / (|d| + 1e-7), `steps` (1 to 20) times
  * X <- 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X, and w -= weightDecay *
  * w + stepSizes[i] * X.  NULL params / grads are skipped.  Up to 4 million rows
- * or columns; no buffer may be the parameter or momentum of two matrices. */
+ * or columns; no buffer may be the parameter or momentum of two matrices.  A call
+ * that is refused, or whose workspace (some 24 bytes per value of the largest group of
+ * matrices, both sides padded to 64 or 128) cannot be had, changes nothing. */
 bool MuonBatch(void** params, void** grads, void** momenta, uint32_t* rows, uint32_t* cols,
                float* stepSizes, uint32_t numParams, float momentum, uint32_t nesterov,
                float weightDecay, float clip, uint32_t steps);
