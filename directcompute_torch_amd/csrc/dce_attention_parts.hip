@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(kPair, 2) k_attn_dkv_parts(const Attn a, const
     TL::load(yp + size_t(t) * kRows * (DP * 4), ry);
     if (threadIdx.x < kRows) {
       const uint32_t i = t * kRows + threadIdx.x;
-      rm = i < a.N ? a.m[size_t(pr) * a.N + i] : 0.f;
+      rm = i < a.N ? a.m[size_t(pr) * a.N + i] : 3e38f;  // P = 0 of rows past the last
       rl = i < a.N ? limit_of(a, i, len) : 0u;
       rd = ps.dl[size_t(pr) * ps.q.pad + i];
     }

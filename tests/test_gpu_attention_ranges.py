@@ -172,3 +172,14 @@ def test_scores_far_from_zero(eng, power, keys):
     left = 4 * D * 2.0 ** -24 * np.abs(dy).max() * np.abs(v).max() * keys
     assert np.abs(ts[0].grad.sync()).max() <= left * np.abs(k).max() and np.abs(ts[1].grad.sync()).max() <= left * np.abs(q).max()
     eng.end_batch()
+
+
+@pytest.mark.parametrize("rows", [33, 129, 1001])
+def test_keys_of_almost_no_weight_under_ragged_rows(eng, rows):
+    """As above, where the last tile of rows is not full: what stands in for the
+    missing rows takes no bits from the rows beside it."""
+    q, k, v, dy = inputs(210)
+    q, dy = q[:, :rows], dy[:, :rows]
+    q[..., 0] = 8
+    k[..., 0] = np.where(np.arange(N) % 32 < 16, -35, 0)[None, :, None]
+    check(eng, q, k, v, dy, f"keys of almost no weight, {rows} rows")
