@@ -3,7 +3,8 @@
 The argtypes/restype blocks mirror the reference's binding of engine.dll
 (nn_engine.py:42-121) symbol for symbol, plus the additions declared in
 include/dcengine.h (GetLastErrorString, AdamBatch, ClipGradNorm, profiling,
-rotary positions, attention, MuonBatch).
+rotary positions, attention, MuonBatch, residual norms, the gated feed-forward
+block, the gated recurrence).
 
 Loading never falls back to anything: if the library is missing or no HIP
 device is usable, :func:`load` raises.
@@ -140,6 +141,22 @@ def bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.MuonBatch.argtypes = ([P(c_void_p)] * 3 + [P(c_uint)] * 2 + [P(c_float), c_uint, c_float, c_uint]
                               + [c_float] * 2 + [c_uint])
     lib.MuonBatch.restype = ctypes.c_bool
+    lib.RmsNorm.argtypes = [c_void_p] * 2 + [c_uint] * 2 + [c_float, P(c_void_p)]
+    lib.RmsNorm.restype = c_void_p
+    lib.RmsNormBackward.argtypes = [c_void_p] * 4 + [c_uint] * 2 + [P(c_void_p)] * 2
+    lib.RmsNormBackward.restype = None
+    lib.ResidualNorm.argtypes = [c_void_p] * 5 + [c_uint] * 3 + [c_float] * 2 + [P(c_void_p)] * 2
+    lib.ResidualNorm.restype = c_void_p
+    lib.ResidualNormBackward.argtypes = [c_void_p] * 8 + [c_uint] * 3 + [c_float] + [P(c_void_p)] * 5
+    lib.ResidualNormBackward.restype = None
+    lib.GatedMlpForward.argtypes = [c_void_p] * 4 + [c_uint] * 5 + [P(c_void_p)]
+    lib.GatedMlpForward.restype = c_void_p
+    lib.GatedMlpBackward.argtypes = [c_void_p] * 6 + [c_uint] * 5 + [P(c_void_p)] * 4
+    lib.GatedMlpBackward.restype = None
+    lib.GatedScanForward.argtypes = [c_void_p] * 4 + [c_uint] * 3 + [P(c_void_p)]
+    lib.GatedScanForward.restype = c_void_p
+    lib.GatedScanBackward.argtypes = [c_void_p] * 6 + [c_uint] * 3 + [P(c_void_p)] * 3
+    lib.GatedScanBackward.restype = None
     lib.SetProfiling.argtypes = [ctypes.c_int]
     lib.SetProfiling.restype = None
     lib.GetProfile.argtypes = [ctypes.c_char_p, P(ctypes.c_uint64), P(ctypes.c_double), P(ctypes.c_double), P(ctypes.c_double)]

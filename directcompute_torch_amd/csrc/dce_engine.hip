@@ -1445,6 +1445,282 @@ bool MuonBatch(void** params, void** grads, void** momenta, uint32_t* rows, uint
                     nesterov != 0, weightDecay, clip, steps);
 }
 
+// ------------------------------------------- norms, feed-forward, recurrence
+// Results of one call: created in turn, handed over together or not at all.
+struct Results {
+  struct Item {
+    void** to;
+    void* h;
+  };
+  std::vector<Item> all;
+  bool ok = true;
+  // A buffer of `count` floats for *to (which is cleared); null where to is.
+  float* add(void** to, uint64_t count) {
+    if (!to || !ok) return nullptr;
+    void* h = create_buffer(nullptr, uint32_t(count));
+    if (!h) {
+      ok = false;
+      return nullptr;
+    }
+    all.push_back({to, h});
+    return static_cast<Buffer*>(h)->ptr;
+  }
+  bool give(bool done) {
+    for (const Item& i : all) {
+      if (done && ok)
+        *i.to = i.h;
+      else
+        release_buffer(i.h);
+    }
+    return done && ok;
+  }
+};
+// The buffer behind an optional handle: false for one that is no buffer or holds
+// fewer than `count` floats.
+static bool operand(const char* what, const char* name, void* h, uint64_t count, const float** p, bool optional = false) {
+  *p = nullptr;
+  if (!h && optional) return true;
+  Buffer* b = as_buffer(h, what);
+  if (!b) return false;
+  if (b->count < count) {
+    set_error("%s: %s holds %u values, not %llu", what, name, b->count, (unsigned long long)count);
+    return false;
+  }
+  *p = b->ptr;
+  return true;
+}
+static bool norm_size(const char* what, uint32_t rows, uint32_t cols) {
+  if (rows && cols && cols <= kNormCols && rows < 0x80000000u && uint64_t(rows) * cols <= 0xFFFFFFFFull) return true;
+  set_error("%s: %u rows of %u values (no zeros, up to %u values a row and 2^32 - 1 in all)", what, rows, cols, kNormCols);
+  return false;
+}
+
+void* RmsNorm(void* x, void* gain, uint32_t rows, uint32_t cols, float eps, void** pStats) {
+  if (pStats) *pStats = nullptr;
+  if (!ensure_init() || !norm_size("RmsNorm", rows, cols)) return nullptr;
+  const uint64_t n = uint64_t(rows) * cols;
+  NormArgs a{};
+  if (!operand("RmsNorm", "x", x, n, &a.x) || !operand("RmsNorm", "gain", gain, cols, &a.pre)) return nullptr;
+  a.rows = rows;
+  a.cols = cols;
+  a.scale = 1.f;
+  a.eps = eps;
+  void* y = nullptr;
+  Results r;
+  a.n = r.add(&y, n);
+  a.r2 = r.add(pStats, rows);
+  return r.give(r.ok && norm_forward(a)) ? y : nullptr;
+}
+
+void RmsNormBackward(void* gradOut, void* x, void* gain, void* stats, uint32_t rows, uint32_t cols, void** pDX,
+                     void** pDGain) {
+  if (pDX) *pDX = nullptr;
+  if (pDGain) *pDGain = nullptr;
+  if (!ensure_init() || !norm_size("RmsNormBackward", rows, cols)) return;
+  const uint64_t n = uint64_t(rows) * cols;
+  const char* what = "RmsNormBackward";
+  NormArgs a{};
+  NormGrads g{};
+  const float *h, *st;
+  if (!operand(what, "gradOut", gradOut, n, &g.dn) || !operand(what, "x", x, n, &h) ||
+      !operand(what, "gain", gain, cols, &a.pre) || !operand(what, "stats", stats, rows, &st))
+    return;
+  a.h = const_cast<float*>(h);
+  a.r2 = const_cast<float*>(st);
+  a.rows = rows;
+  a.cols = cols;
+  a.scale = 1.f;
+  Results r;
+  g.dx = r.add(pDX, n);
+  g.dpre = r.add(pDGain, cols);
+  if (r.ok && r.all.empty()) return;
+  r.give(r.ok && norm_backward(a, g));
+}
+
+// What both directions of a residual norm check; r1, r2 are in one buffer.
+static bool residual_args(const char* what, void* block, void* gate, void* post, void* pre, uint32_t rows, uint32_t cols,
+                          uint32_t gateRows, float scale, NormArgs* a) {
+  if (!norm_size(what, rows, cols)) return false;
+  if (gate && (!gateRows || rows % gateRows)) {
+    set_error("%s: a gate of %u rows for %u (it has to divide them)", what, gateRows, rows);
+    return false;
+  }
+  a->rows = rows;
+  a->cols = cols;
+  a->gateRows = gateRows;
+  a->scale = scale;
+  return operand(what, "block", block, uint64_t(rows) * cols, &a->block) &&
+         operand(what, "gate", gate, uint64_t(gateRows) * cols, &a->gate, true) &&
+         operand(what, "post", post, cols, &a->post, true) && operand(what, "pre", pre, cols, &a->pre, true);
+}
+
+void* ResidualNorm(void* x, void* block, void* gate, void* post, void* pre, uint32_t rows, uint32_t cols,
+                   uint32_t gateRows, float scale, float eps, void** pNormed, void** pStats) {
+  if (pNormed) *pNormed = nullptr;
+  if (pStats) *pStats = nullptr;
+  if (!ensure_init()) return nullptr;
+  const char* what = "ResidualNorm";
+  NormArgs a{};
+  if (!residual_args(what, block, gate, post, pre, rows, cols, gateRows, scale, &a)) return nullptr;
+  const uint64_t n = uint64_t(rows) * cols;
+  if (!operand(what, "x", x, n, &a.x)) return nullptr;
+  if (!a.pre != !pNormed) {
+    set_error("%s: a second norm takes a gain and a place for its result", what);
+    return nullptr;
+  }
+  a.eps = eps;
+  void* h = nullptr;
+  Results r;
+  a.h = r.add(&h, n);
+  a.n = r.add(pNormed, n);
+  if ((a.post || a.pre) && pStats) {
+    a.r1 = r.add(pStats, 2 * uint64_t(rows));
+    a.r2 = a.r1 ? a.r1 + rows : nullptr;
+  }
+  return r.give(r.ok && norm_forward(a)) ? h : nullptr;
+}
+
+void ResidualNormBackward(void* gradH, void* gradNormed, void* h, void* block, void* gate, void* post, void* pre,
+                          void* stats, uint32_t rows, uint32_t cols, uint32_t gateRows, float scale, void** pDX,
+                          void** pDBlock, void** pDGate, void** pDPost, void** pDPre) {
+  for (void** p : {pDX, pDBlock, pDGate, pDPost, pDPre})
+    if (p) *p = nullptr;
+  if (!ensure_init()) return;
+  const char* what = "ResidualNormBackward";
+  NormArgs a{};
+  NormGrads g{};
+  if (!residual_args(what, block, gate, post, pre, rows, cols, gateRows, scale, &a)) return;
+  const uint64_t n = uint64_t(rows) * cols;
+  const float *hp, *st;
+  if (!operand(what, "gradH", gradH, n, &g.dh, true) || !operand(what, "gradNormed", gradNormed, n, &g.dn, true) ||
+      !operand(what, "h", h, n, &hp, !g.dn) ||
+      !operand(what, "stats", stats, 2 * uint64_t(rows), &st, !a.post && !g.dn))
+    return;
+  if ((!g.dh && !g.dn) || (g.dn && !a.pre) || (pDGate && !a.gate) || (pDPost && !a.post) || (pDPre && !g.dn)) {
+    set_error("%s: a gradient of the result, and gradients of what the call has", what);
+    return;
+  }
+  a.h = const_cast<float*>(hp);
+  a.r1 = const_cast<float*>(st);
+  a.r2 = st ? a.r1 + rows : nullptr;
+  Results r;
+  g.dx = r.add(pDX, n);
+  g.db = r.add(pDBlock, n);
+  g.dgate = r.add(pDGate, uint64_t(gateRows) * cols);
+  g.dpost = r.add(pDPost, cols);
+  g.dpre = r.add(pDPre, cols);
+  if (r.ok && r.all.empty()) return;
+  r.give(r.ok && norm_backward(a, g));
+}
+
+static bool mlp_args(const char* what, void* x, void* wGate, void* wUp, void* wDown, uint32_t rows, uint32_t cols,
+                     uint32_t hidden, uint32_t outCols, uint32_t act, MlpArgs* a) {
+  if (act > kSigmoid) {
+    set_error("%s: activation %u (0 silu, 1 gelu, 2 relu, 3 sigmoid)", what, act);
+    return false;
+  }
+  const uint64_t most = std::max({uint64_t(rows) * std::max({cols, hidden, outCols}), uint64_t(hidden) * std::max(cols, outCols)});
+  if (!rows || !cols || !hidden || !outCols || most >= kOob) {
+    set_error("%s: %u rows, %u -> %u -> %u (no zeros, fewer than 2^29 values in a matrix)", what, rows, cols, hidden, outCols);
+    return false;
+  }
+  a->rows = rows;
+  a->cols = cols;
+  a->hidden = hidden;
+  a->out = outCols;
+  a->act = MlpAct(act);
+  const uint64_t w = uint64_t(cols) * hidden;
+  return operand(what, "x", x, uint64_t(rows) * cols, &a->x) && operand(what, "the gate's weights", wGate, w, &a->wg) &&
+         operand(what, "the upward weights", wUp, w, &a->wu) &&
+         operand(what, "the downward weights", wDown, uint64_t(hidden) * outCols, &a->wd);
+}
+
+void* GatedMlpForward(void* x, void* wGate, void* wUp, void* wDown, uint32_t rows, uint32_t cols, uint32_t hidden,
+                      uint32_t outCols, uint32_t act, void** pSaved) {
+  if (pSaved) *pSaved = nullptr;
+  if (!ensure_init()) return nullptr;
+  MlpArgs a{};
+  if (!mlp_args("GatedMlpForward", x, wGate, wUp, wDown, rows, cols, hidden, outCols, act, &a)) return nullptr;
+  void* y = nullptr;
+  Results r;
+  a.y = r.add(&y, uint64_t(rows) * outCols);
+  a.saved = r.add(pSaved, 2 * uint64_t(rows) * hidden);
+  return r.give(r.ok && mlp_forward(a)) ? y : nullptr;
+}
+
+void GatedMlpBackward(void* gradOut, void* x, void* wGate, void* wUp, void* wDown, void* saved, uint32_t rows,
+                      uint32_t cols, uint32_t hidden, uint32_t outCols, uint32_t act, void** pDX, void** pDGate,
+                      void** pDUp, void** pDDown) {
+  for (void** p : {pDX, pDGate, pDUp, pDDown})
+    if (p) *p = nullptr;
+  if (!ensure_init()) return;
+  const char* what = "GatedMlpBackward";
+  MlpArgs a{};
+  const float *dy, *st;
+  if (!mlp_args(what, x, wGate, wUp, wDown, rows, cols, hidden, outCols, act, &a) ||
+      !operand(what, "gradOut", gradOut, uint64_t(rows) * outCols, &dy) ||
+      !operand(what, "saved", saved, 2 * uint64_t(rows) * hidden, &st))
+    return;
+  a.saved = const_cast<float*>(st);
+  const uint64_t w = uint64_t(cols) * hidden;
+  Results r;
+  float* dx = r.add(pDX, uint64_t(rows) * cols);
+  float* dg = r.add(pDGate, w);
+  float* du = r.add(pDUp, w);
+  float* dd = r.add(pDDown, uint64_t(hidden) * outCols);
+  if (r.ok && r.all.empty()) return;
+  r.give(r.ok && mlp_backward(a, dy, dx, dg, du, dd));
+}
+
+static bool scan_args(const char* what, void* x, void* gate, void* state, void* lengths, uint32_t batch, uint32_t seq,
+                      uint32_t chans, ScanArgs* a) {
+  const uint64_t n = uint64_t(batch) * seq * chans;
+  if (!batch || !seq || !chans || uint64_t(batch) * seq > 0xFFFFFFFFull || n > 0xFFFFFFFFull) {
+    set_error("%s: %u x %u tokens of %u channels (no zeros, up to 2^32 - 1 values)", what, batch, seq, chans);
+    return false;
+  }
+  a->B = batch;
+  a->S = seq;
+  a->C = chans;
+  return operand(what, "x", x, n, &a->x) && operand(what, "gate", gate, n, &a->z) &&
+         operand(what, "state", state, uint64_t(batch) * chans, &a->state, true) &&
+         operand(what, "lengths", lengths, batch, &a->len, true);
+}
+
+void* GatedScanForward(void* x, void* gate, void* state, void* lengths, uint32_t batch, uint32_t seq, uint32_t chans,
+                       void** pLast) {
+  if (pLast) *pLast = nullptr;
+  if (!ensure_init()) return nullptr;
+  ScanArgs a{};
+  if (!scan_args("GatedScanForward", x, gate, state, lengths, batch, seq, chans, &a)) return nullptr;
+  void* y = nullptr;
+  Results r;
+  a.y = r.add(&y, uint64_t(batch) * seq * chans);
+  a.last = r.add(pLast, uint64_t(batch) * chans);
+  return r.give(r.ok && scan_forward(a)) ? y : nullptr;
+}
+
+void GatedScanBackward(void* gradOut, void* out, void* x, void* gate, void* state, void* lengths, uint32_t batch,
+                       uint32_t seq, uint32_t chans, void** pDX, void** pDGate, void** pDState) {
+  for (void** p : {pDX, pDGate, pDState})
+    if (p) *p = nullptr;
+  if (!ensure_init()) return;
+  const char* what = "GatedScanBackward";
+  ScanArgs a{};
+  const uint64_t n = uint64_t(batch) * seq * chans;
+  const float* y;
+  if (!scan_args(what, x, gate, state, lengths, batch, seq, chans, &a) || !operand(what, "gradOut", gradOut, n, &a.dy) ||
+      !operand(what, "out", out, n, &y))
+    return;
+  a.y = const_cast<float*>(y);
+  Results r;
+  a.dx = r.add(pDX, n);
+  a.dz = r.add(pDGate, n);
+  a.dstate = r.add(pDState, uint64_t(batch) * chans);
+  if (r.ok && r.all.empty()) return;
+  r.give(r.ok && scan_backward(a));
+}
+
 // ----------------------------------------------------------------- profiling
 void SetProfiling(int enabled) {
   if (!enabled) resolve_profile();

@@ -521,6 +521,50 @@ bool muon_multi(void** params, void** grads, void** momenta, const uint32_t* row
                 const uint32_t* cols, const float* stepSizes, uint32_t n, float mu, bool nesterov,
                 float decay, float clip, uint32_t steps);
 
+// The norms around a residual stream (dce_norm.hip), rows x cols values:
+//   u = post ? block r1 post : block, h = scale x + gate u, n = h r2 pre.
+// block null: h is x.  gate: gateRows rows, each for rows / gateRows of them, or
+// null; n null: no second norm.  r1, r2: the rows' 1 / rms, null where not kept
+// (the backward reads them).
+constexpr uint32_t kNormCols = 16384;  // the widest row
+struct NormArgs {
+  const float *x, *block, *gate, *post, *pre;
+  float *h, *n, *r1, *r2;
+  uint32_t rows, cols, gateRows;
+  float scale, eps;
+};
+struct NormGrads {
+  const float *dh, *dn;                     // null: zeros
+  float *dx, *db, *dgate, *dpost, *dpre;    // null where not wanted
+};
+bool norm_forward(const NormArgs& a);
+bool norm_backward(const NormArgs& a, const NormGrads& g);
+
+// The gated feed-forward block (dce_mlp.hip): y = (act(x wg) * (x wu)) wd over
+// rows x cols values, `hidden` between.  saved: x wg and x wu, 2 rows x hidden
+// floats, that the forward leaves for the backward (null: not kept).
+enum MlpAct { kSilu, kGelu, kRelu, kSigmoid };
+struct MlpArgs {
+  const float *x, *wg, *wu, *wd;
+  float *y, *saved;
+  uint32_t rows, cols, hidden, out;
+  MlpAct act;
+};
+bool mlp_forward(const MlpArgs& a);
+bool mlp_backward(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd);
+
+// The gated linear recurrence (dce_scan.hip) over [B][S][C]: f = sigmoid(z),
+// y_t = f_t y_(t-1) + (1 - f_t) x_t from state [B][C] (null: zeros).  len: B token
+// counts as floats, or null (S).  last (may be null): the state after the last
+// token.  The backward reads y, too.
+struct ScanArgs {
+  const float *x, *z, *state, *len, *dy;
+  float *y, *last, *dx, *dz, *dstate;
+  uint32_t B, S, C;
+};
+bool scan_forward(const ScanArgs& a);
+bool scan_backward(const ScanArgs& a);
+
 // Profiling hooks (dce_engine.hip): kernel-family timing with HIP events on
 // the engine stream.  `family` is a short static string.
 struct ProfScope {

@@ -946,6 +946,194 @@ class AttentionFunc(Function):
                 t._accumulate_grad(Tensor.from_gpu(p.value, t.shape, track=True))
 
 
+def _backward_call(fn, what, args, targets):
+    """fn(*args, a pointer for each target that takes a gradient), whose results
+    are added to those targets."""
+    got = [ctypes.c_void_p() if t is not None and t.requires_grad else None for t in targets]
+    if all(p is None for p in got):
+        return
+    fn(*args, *[None if p is None else ctypes.byref(p) for p in got])
+    if any(p is not None and not p.value for p in got):
+        for p in got:
+            if p is not None and p.value:
+                lib.ReleaseBuffer(p)
+        raise RuntimeError(f"{what} failed: {last_error()}")
+    for t, p in zip(targets, got):
+        if p is not None:
+            t._accumulate_grad(Tensor.from_gpu(p.value, t.shape, track=True))
+
+
+class _Keeps(Function):
+    """A node that owns a buffer its backward reads (`kept`, or None)."""
+    kept = None
+
+    def __del__(self):
+        h, self.kept = self.kept, None
+        if h:
+            try:
+                lib.ReleaseBuffer(h)
+            except Exception:
+                pass
+
+
+def _gain_of(what, name, gain, width):
+    if gain is not None and tuple(gain.shape) != (width,):
+        raise ValueError(f"{what}: {name} is ({width},), not {tuple(gain.shape)}")
+
+
+class RmsNormFunc(_Keeps):
+    def forward(self, x, gain, eps):
+        width = x.shape[-1]
+        _gain_of("rms_norm", "gain", gain, width)
+        self.inputs = (x, gain)
+        self.dims = (x.size // width, width)
+        req = x.requires_grad or gain.requires_grad
+        st = ctypes.c_void_p()
+        h = lib.RmsNorm(x.gpu_buf, gain.gpu_buf, *self.dims, eps, ctypes.byref(st) if req else None)
+        _check(h, "RmsNorm")
+        self.kept = st.value
+        res = Tensor.from_gpu(h, x.shape, requires_grad=req)
+        res._ctx = self
+        return res
+
+    def backward(self, grad_output):
+        x, gain = self.inputs
+        _backward_call(lib.RmsNormBackward, "RmsNormBackward",
+                       (grad_output.gpu_buf, x.gpu_buf, gain.gpu_buf, self.kept, *self.dims), (x, gain))
+
+
+class ResidualNormFunc(_Keeps):
+    """The node of h.  Its backward is also that of the norm of h where that
+    norm's gradient (`normed_grad`) has been left here by NormedFunc."""
+    normed_grad = None
+
+    def forward(self, x, block, gate, post, pre, scale, eps):
+        shape = tuple(x.shape)
+        width = shape[-1]
+        rows = x.size // width
+        if tuple(block.shape) != shape:
+            raise ValueError(f"residual_norm: x {shape} and the block's result {tuple(block.shape)} differ")
+        _gain_of("residual_norm", "post", post, width)
+        _gain_of("residual_norm", "pre", pre, width)
+        gate_rows = 0
+        if gate is not None:
+            gate_rows = gate.size // width
+            if not gate.shape or gate.shape[-1] != width or rows % gate_rows:
+                raise ValueError(f"residual_norm: a gate of {tuple(gate.shape)} for {shape}: rows of {width} values, "
+                                 f"a number of them that divides {rows}")
+        # pre is here for its place in the traversal: its gradient may come from this node
+        self.inputs = (x, block, gate, post, pre)
+        self.dims = (rows, width, gate_rows, float(scale))
+        own = any(t is not None and t.requires_grad for t in (x, block, gate, post))
+        req = own or (pre is not None and pre.requires_grad)
+        st, n = ctypes.c_void_p(), ctypes.c_void_p()
+        h = lib.ResidualNorm(*[t.gpu_buf if t is not None else None for t in (x, block, gate, post, pre)], *self.dims,
+                             eps, ctypes.byref(n) if pre is not None else None, ctypes.byref(st) if req else None)
+        _check(h, "ResidualNorm")
+        self.kept = st.value
+        self.h = h    # by handle: a reference to the tensor would be a cycle
+        res = Tensor.from_gpu(h, shape, requires_grad=own)
+        res._ctx = self
+        if pre is None:
+            return res
+        normed = Tensor.from_gpu(n.value, shape, requires_grad=req)
+        normed._ctx = NormedFunc(res, pre)
+        normed._ctx.node = self
+        return res, normed
+
+    def call(self, dh, dn, targets):
+        x, block, gate, post, pre = self.inputs
+        ops = [t.gpu_buf if t is not None else None for t in (dh, dn)] + [self.h] + [
+            t.gpu_buf if t is not None else None for t in (block, gate, post, pre)]
+        _backward_call(lib.ResidualNormBackward, "ResidualNormBackward", (*ops, self.kept, *self.dims), targets)
+
+    def backward(self, grad_output):
+        dn, self.normed_grad = self.normed_grad, None
+        self.call(grad_output, dn, self.inputs[:4] + (self.inputs[4] if dn is not None else None,))
+
+
+class NormedFunc(Function):
+    """The norm of a ResidualNormFunc's h.  Where h has a gradient already (the
+    next block's), both go through h's node in one pass; else this one's is
+    the first that h gets."""
+
+    def backward(self, grad_output):
+        h, pre = self.inputs
+        node = self.node
+        if h.requires_grad and h.grad is not None and h.grad.gpu_buf is not None:
+            node.normed_grad = grad_output
+            return
+        rows, width = node.dims[:2]
+        got = [ctypes.c_void_p() if t.requires_grad else None for t in (h, pre)]
+        lib.ResidualNormBackward(None, grad_output.gpu_buf, node.h, node.inputs[1].gpu_buf, None, None, pre.gpu_buf,
+                                 node.kept, rows, width, 0, 1.0, *[p and ctypes.byref(p) for p in (got[0], None, None, None, got[1])])
+        if any(p is not None and not p.value for p in got):
+            raise RuntimeError(f"ResidualNormBackward failed: {last_error()}")
+        for t, p in zip((h, pre), got):
+            if p is not None:
+                t._accumulate_grad(Tensor.from_gpu(p.value, t.shape, track=True))
+
+
+_ACTS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+
+
+class GatedMlpFunc(_Keeps):
+    """GatedMlpForward / GatedMlpBackward; keeps x Wg and x Wu for the backward."""
+
+    def forward(self, x, w_gate, w_up, w_down, act):
+        if act not in _ACTS:
+            raise ValueError(f"gated_mlp: activation {act!r} (one of {', '.join(_ACTS)})")
+        width = x.shape[-1] if x.shape else 0
+        if (len(w_gate.shape) != 2 or tuple(w_gate.shape) != tuple(w_up.shape) or len(w_down.shape) != 2
+                or w_gate.shape[0] != width or w_down.shape[0] != w_gate.shape[1]):
+            raise ValueError("gated_mlp: x is (..., width), w_gate and w_up (width, hidden), w_down (hidden, out); got "
+                             f"{tuple(x.shape)}, {tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
+        self.inputs = (x, w_gate, w_up, w_down)
+        self.dims = (x.size // width, width, w_gate.shape[1], w_down.shape[1], _ACTS[act])
+        req = any(t.requires_grad for t in self.inputs)
+        st = ctypes.c_void_p()
+        h = lib.GatedMlpForward(*[t.gpu_buf for t in self.inputs], *self.dims, ctypes.byref(st) if req else None)
+        _check(h, "GatedMlpForward")
+        self.kept = st.value
+        res = Tensor.from_gpu(h, tuple(x.shape[:-1]) + (w_down.shape[1],), requires_grad=req)
+        res._ctx = self
+        return res
+
+    def backward(self, grad_output):
+        _backward_call(lib.GatedMlpBackward, "GatedMlpBackward",
+                       (grad_output.gpu_buf, *[t.gpu_buf for t in self.inputs], self.kept, *self.dims), self.inputs)
+
+
+class GatedScanFunc(Function):
+    """GatedScanForward / GatedScanBackward, which reads the result again."""
+
+    def forward(self, x, gate, state, lengths, return_state):
+        if len(x.shape) != 3 or tuple(gate.shape) != tuple(x.shape):
+            raise ValueError(f"gated_scan: x and gate are (batch, seq, channels), not {tuple(x.shape)} and {tuple(gate.shape)}")
+        B, S, C = x.shape
+        if state is not None and tuple(state.shape) != (B, C):
+            raise ValueError(f"gated_scan: the state is ({B}, {C}), not {tuple(state.shape)}")
+        if lengths is not None and lengths.size != B:
+            raise ValueError(f"gated_scan: {lengths.size} lengths for {B} sequences")
+        self.inputs = (x, gate, state)
+        self.lengths = lengths
+        self.dims = (B, S, C)
+        last = ctypes.c_void_p()
+        h = lib.GatedScanForward(*self._operands(), *self.dims, ctypes.byref(last) if return_state else None)
+        _check(h, "GatedScanForward")
+        res = Tensor.from_gpu(h, (B, S, C), requires_grad=any(t is not None and t.requires_grad for t in self.inputs))
+        self.out_handle = h    # by handle: a reference to `res` itself would be a cycle
+        res._ctx = self
+        return (res, Tensor.from_gpu(last.value, (B, C))) if return_state else res
+
+    def _operands(self):
+        return [t.gpu_buf if t is not None else None for t in (*self.inputs, self.lengths)]
+
+    def backward(self, grad_output):
+        _backward_call(lib.GatedScanBackward, "GatedScanBackward",
+                       (grad_output.gpu_buf, self.out_handle, *self._operands(), *self.dims), self.inputs)
+
+
 def _absent(name):
     def f(*args, **kwargs):
         raise NotImplementedError(f"{name}: its kernels do not exist in the reference tree "
@@ -996,6 +1184,39 @@ def attention(q, k, v, causal=False, scale=None, lengths=None):
     values, the keys of each sequence that count; None: all.  scale: 1 /
     sqrt(head_dim) by default.  A query that sees no key gets zeros."""
     return AttentionFunc().forward(q, k, v, causal, scale, lengths)
+
+
+def rms_norm(x, gain, eps=1e-6):
+    """x / sqrt(mean(x ** 2) + eps) * gain over the last axis (up to 16384
+    values); gain: that many values."""
+    return RmsNormFunc().forward(x, gain, eps)
+
+
+def residual_norm(x, block, gate=None, post=None, pre=None, scale=1.0, eps=1e-6):
+    """The step from one block of a residual stream to the next, in one pass:
+    h = scale * x + gate * u, where u is `block` (a block's result, of x's shape)
+    or, with a gain `post`, its rms_norm.  With a gain `pre` returns (h, rms_norm(h,
+    pre)), the second the next block's input; else h.  gate: rows of x's last
+    axis, each for an equal share of x's rows in turn: (width,) for all of them,
+    (batch, width) for x of (batch, seq, width), or x's shape."""
+    return ResidualNormFunc().forward(x, block, gate, post, pre, scale, eps)
+
+
+def gated_mlp(x, w_gate, w_up, w_down, act="silu"):
+    """(act(x @ w_gate) * (x @ w_up)) @ w_down for x of (..., width), w_gate and
+    w_up of (width, hidden), w_down of (hidden, out); act: silu, gelu (by erf),
+    relu or sigmoid."""
+    return GatedMlpFunc().forward(x, w_gate, w_up, w_down, act)
+
+
+def gated_scan(x, gate, state=None, lengths=None, return_state=False):
+    """y_t = f_t * y_(t-1) + (1 - f_t) * x_t with f = sigmoid(gate), for every
+    channel of x and gate, both (batch, seq, channels).  state: (batch, channels),
+    what comes before the first token; None: zeros.  lengths: a tensor of batch
+    values, the tokens of each sequence that count; y is zeros past them.
+    return_state: also the state after the last of them, for the next call's
+    `state`; it carries no gradient."""
+    return GatedScanFunc().forward(x, gate, state, lengths, return_state)
 
 
 def rotary_table(positions, rotary_dim, base=10000.0, factor=1.0, original=None, ramp=(1.0, 32.0)):
@@ -1120,6 +1341,33 @@ class Rotary:
         return rotary(x, self.table, positions, self.interleaved)
 
 
+class RMSNorm:
+    """rms_norm with its gain, of ones at first."""
+
+    def __init__(self, num_features, eps=1e-6):
+        self.eps = eps
+        self.gain = Tensor(np.ones(num_features, np.float32), requires_grad=True, track=False)
+
+    def __call__(self, x):
+        return rms_norm(x, self.gain, self.eps)
+
+
+class GatedMLP:
+    """gated_mlp with its weights, initialised as Linear's."""
+
+    def __init__(self, in_features, hidden, out_features=None, act="silu"):
+        out = in_features if out_features is None else out_features
+
+        def weights(a, b):
+            limit = np.sqrt(6 / (a + b))
+            return Tensor(np.random.uniform(-limit, limit, (a, b)), requires_grad=True, track=False)
+        self.act = act
+        self.w_gate, self.w_up, self.w_down = weights(in_features, hidden), weights(in_features, hidden), weights(hidden, out)
+
+    def __call__(self, x):
+        return gated_mlp(x, self.w_gate, self.w_up, self.w_down, self.act)
+
+
 def _param_attrs(obj):
     """Attributes holding a layer's trainable tensors, in the order
     Model.parameters lists them.  Normalisation layers are matched by class
@@ -1129,6 +1377,10 @@ def _param_attrs(obj):
         return ("filters", "bias")
     if isinstance(obj, Linear):
         return ("w", "b")
+    if isinstance(obj, RMSNorm):
+        return ("gain",)
+    if isinstance(obj, GatedMLP):
+        return ("w_gate", "w_up", "w_down")
     if type(obj).__name__ in ("BatchNorm2d", "LayerNorm"):
         return ("gamma", "beta")
     return ()

@@ -272,6 +272,58 @@ bool MuonBatch(void** params, void** grads, void** momenta, uint32_t* rows, uint
                float* stepSizes, uint32_t numParams, float momentum, uint32_t nesterov,
                float weightDecay, float clip, uint32_t steps);
 
+/* ---- the rest of a transformer or recurrent block.
+ *
+ * The norms around a residual stream, over rows of `cols` (up to 16384) values:
+ *   RmsNorm: x / sqrt(mean(x^2) + eps) * gain, gain of cols values.
+ *   ResidualNorm: u = block, or its RmsNorm with gain `post` when that is not
+ *   NULL; h = scale * x + gate * u (the result); *pNormed = the RmsNorm of h
+ *   with gain `pre` (both NULL: none).  gate: gateRows x cols values, each of
+ *   its rows for rows / gateRows rows in turn (1: all of them; rows: a value
+ *   each), or NULL: 1.
+ * pStats, when not NULL, receives the rows' factors for the backward (RmsNorm:
+ * rows floats; ResidualNorm: 2 * rows, NULL when it has neither norm). */
+void* RmsNorm(void* x, void* gain, uint32_t rows, uint32_t cols, float eps, void** pStats);
+void* ResidualNorm(void* x, void* block, void* gate, void* post, void* pre, uint32_t rows,
+                   uint32_t cols, uint32_t gateRows, float scale, float eps, void** pNormed,
+                   void** pStats);
+/* Their gradients, each only when its pointer is not NULL, from the forward's
+ * operands and stats.  ResidualNormBackward: gradH or gradNormed may be NULL
+ * (zeros), and without gradNormed there is no gradient of pre and h is not
+ * read.  Sums over rows are in a fixed order. */
+void RmsNormBackward(void* gradOut, void* x, void* gain, void* stats, uint32_t rows, uint32_t cols,
+                     void** pDX, void** pDGain);
+void ResidualNormBackward(void* gradH, void* gradNormed, void* h, void* block, void* gate,
+                          void* post, void* pre, void* stats, uint32_t rows, uint32_t cols,
+                          uint32_t gateRows, float scale, void** pDX, void** pDBlock, void** pDGate,
+                          void** pDPost, void** pDPre);
+
+/* Gated feed-forward block: y = (act(x Wg) * (x Wu)) Wd.  x is rows x cols, Wg
+ * and Wu cols x hidden, Wd hidden x outCols, y rows x outCols; fewer than 2^29
+ * values in each, and in rows x hidden.  act: 0 silu, 1 gelu (by erf), 2 relu, 3
+ * sigmoid.  pSaved, when not NULL, receives x Wg and x Wu (2 * rows * hidden
+ * floats) for the backward, which gives each gradient only when its pointer is
+ * not NULL. */
+void* GatedMlpForward(void* x, void* wGate, void* wUp, void* wDown, uint32_t rows, uint32_t cols,
+                      uint32_t hidden, uint32_t outCols, uint32_t act, void** pSaved);
+void GatedMlpBackward(void* gradOut, void* x, void* wGate, void* wUp, void* wDown, void* saved,
+                      uint32_t rows, uint32_t cols, uint32_t hidden, uint32_t outCols, uint32_t act,
+                      void** pDX, void** pDGate, void** pDUp, void** pDDown);
+
+/* Gated linear recurrence over [batch][seq][chans]: f = sigmoid(gate), y_t = f_t
+ * y_(t-1) + (1 - f_t) x_t for every channel, from `state` (batch x chans values, or
+ * NULL: zeros).  lengths: batch floats, the tokens of each sequence that count
+ * (clamped to 0 .. seq; memory past them may hold anything), or NULL: all; y is
+ * zeros past them.  pLast, when not NULL, receives the state after the last token
+ * that counts (batch x chans): the next call's `state`.  The backward reads the
+ * forward's result; gradients past the lengths are zeros, and none flows in
+ * through *pLast. */
+void* GatedScanForward(void* x, void* gate, void* state, void* lengths, uint32_t batch,
+                       uint32_t seq, uint32_t chans, void** pLast);
+void GatedScanBackward(void* gradOut, void* out, void* x, void* gate, void* state, void* lengths,
+                       uint32_t batch, uint32_t seq, uint32_t chans, void** pDX, void** pDGate,
+                       void** pDState);
+
 /* Kernel-family timing with HIP events on the engine stream (for bench.py).
  * SetProfiling(1) starts recording every launch of the named families;
  * GetProfile returns launches, summed milliseconds, summed algorithmic
