@@ -16,6 +16,12 @@
 // that is no multiple of 4 has its last quad end with the row, so that some of
 // its values are the quad's before it too: they are computed twice, to the same
 // bits, and left out of the sums.
+//
+// Bound by memory.  8192 x 2048, a gate for each channel: forward (16 bytes a value) 43
+// us, 6.3 TB/s; backward (24) 74 us, 5.4 TB/s, and 6 us for the sums over rows.  8191 x
+// 4096 with a gate for each value: 99 and 170 us, 6.8 and 6.3 TB/s.  Passes over more
+// than the last cache go past it (nontemporal), which is worth 20 to 25 % there.  The
+// next row's loads ahead of time, and gains held in registers, gained nothing.
 #include "dce_internal.h"
 
 #include <algorithm>
@@ -49,21 +55,23 @@ struct Span {
     at = min(c, cols - W);
     dup = int(min(c - at, uint32_t(W)));
   }
+  template <bool NT = false>
   __device__ __forceinline__ void load(const float* row, float* v) const {
     if constexpr (W == 4) {
-      const f4 q = ldu<f4>(row + at);
+      const f4u q = ldus<NT, f4u>(row + at);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = q[e];
     } else {
-      v[0] = row[at];
+      v[0] = ldus<NT, float>(row + at);
     }
   }
+  template <bool NT = false>
   __device__ __forceinline__ void store(float* row, const float* v) const {
     if (dup == W) return;
     if constexpr (W == 4) {
-      stu(row + at, f4{v[0], v[1], v[2], v[3]});
+      stus<NT>(row + at, f4u{v[0], v[1], v[2], v[3]});
     } else {
-      row[at] = v[0];
+      stus<NT>(row + at, v[0]);
     }
   }
 };
@@ -71,6 +79,12 @@ struct Span {
 // Sum over the TPR threads of a row, in every one of them.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* sh) {
+  if constexpr (TPR < 64) {
+    v = group8_reduce(v);
+    v += xl::dpp<xl::kRowMirror>(v);
+    if constexpr (TPR == 32) v += xl::swz(v);
+    return v;
+  }
   v = wave_reduce(v);
   if constexpr (TPR > 64) {
     __syncthreads();
@@ -86,7 +100,7 @@ __device__ __forceinline__ float row_sum(float v, float* sh) {
 template <int TPR>
 constexpr int threads_of = TPR < 256 ? 256 : TPR;
 
-template <int TPR, int NV, int W>
+template <int TPR, int NV, int W, bool NT>
 __global__ void __launch_bounds__(threads_of<TPR>) k_norm_fwd(const Norm a) {
   constexpr int T = threads_of<TPR>, RPB = T / TPR;
   __shared__ float sh[T / 64];
@@ -98,10 +112,10 @@ __global__ void __launch_bounds__(threads_of<TPR>) k_norm_fwd(const Norm a) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) s[j].init((j * TPR + lane) * W, a.cols);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) s[j].load(a.x + base, x[j]);
+  for (int j = 0; j < NV; ++j) s[j].template load<NT>(a.x + base, x[j]);
   if (a.block) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) s[j].load(a.block + base, b[j]);
+    for (int j = 0; j < NV; ++j) s[j].template load<NT>(a.block + base, b[j]);
     if (a.post) {
       float sum = 0.f;
 #pragma unroll
@@ -128,7 +142,7 @@ __global__ void __launch_bounds__(threads_of<TPR>) k_norm_fwd(const Norm a) {
 #pragma unroll
         for (int e = 0; e < W; ++e) x[j][e] = a.scale * x[j][e] + b[j][e];
       }
-      s[j].store(a.h + base, x[j]);
+      s[j].template store<NT>(a.h + base, x[j]);
     }
   }
   if (!a.n) return;
@@ -144,7 +158,7 @@ __global__ void __launch_bounds__(threads_of<TPR>) k_norm_fwd(const Norm a) {
     s[j].load(a.pre, t);
 #pragma unroll
     for (int e = 0; e < W; ++e) x[j][e] = x[j][e] * r * t[e];
-    s[j].store(a.n + base, x[j]);
+    s[j].template store<NT>(a.n + base, x[j]);
   }
 }
 
@@ -152,7 +166,7 @@ __global__ void __launch_bounds__(threads_of<TPR>) k_norm_fwd(const Norm a) {
 // one.  The sums over rows stay in registers until the last one; a workgroup
 // leaves one row of each in dpost and dpre, and one of dgate for each gate row it
 // has rows of.
-template <int TPR, int NV, int W>
+template <int TPR, int NV, int W, bool NT>
 __global__ void __launch_bounds__(threads_of<TPR>) k_norm_bwd(const Norm a) {
   constexpr int T = threads_of<TPR>, RPB = T / TPR;
   __shared__ float sh[T / 64];
@@ -171,6 +185,23 @@ __global__ void __launch_bounds__(threads_of<TPR>) k_norm_bwd(const Norm a) {
     for (int e = 0; e < W; ++e) dpost[j][e] = dpre[j][e] = 0.f;
   }
   const float inv = 1.f / float(a.cols);
+  auto fetch = [&](uint32_t row, float (&t)[NV][W], float (&h)[NV][W], float (&w)[NV][W], float (&b)[NV][W]) {
+    const size_t base = size_t(row) * a.cols;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (a.dh) {
+        s[j].template load<NT>(a.dh + base, t[j]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e) t[j][e] = 0.f;
+      }
+      if (a.dn) {
+        s[j].template load<NT>(a.h + base, h[j]);
+        s[j].template load<NT>(a.dn + base, w[j]);
+      }
+      if (a.post || a.dgate) s[j].template load<NT>(a.block + base, b[j]);
+    }
+  };
   // The threads' sums to one row of `to`.
   auto put = [&](float (&v)[NV][W], float* to) {
     if constexpr (RPB > 1) {
@@ -207,20 +238,7 @@ __global__ void __launch_bounds__(threads_of<TPR>) k_norm_bwd(const Norm a) {
       const size_t base = size_t(row) * a.cols;
       const float* gate = a.gate ? a.gate + (a.each ? base : size_t(g) * a.cols) : nullptr;
       float t[NV][W], h[NV][W], b[NV][W], w[NV][W], gain[W];
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (a.dh) {
-          s[j].load(a.dh + base, t[j]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < W; ++e) t[j][e] = 0.f;
-        }
-        if (a.dn) {
-          s[j].load(a.h + base, h[j]);
-          s[j].load(a.dn + base, w[j]);
-        }
-        if (a.post || a.dgate) s[j].load(a.block + base, b[j]);
-      }
+      fetch(row, t, h, w, b);
       if (a.dn) {
         const float r = a.r2[row];
         float sum = 0.f;
@@ -245,7 +263,7 @@ __global__ void __launch_bounds__(threads_of<TPR>) k_norm_bwd(const Norm a) {
         for (int j = 0; j < NV; ++j) {
 #pragma unroll
           for (int e = 0; e < W; ++e) w[j][e] = a.scale * t[j][e];
-          s[j].store(a.dx + base, w[j]);
+          s[j].template store<NT>(a.dx + base, w[j]);
         }
       }
       if (!a.db && !a.dgate && !a.dpost) continue;
@@ -284,7 +302,7 @@ __global__ void __launch_bounds__(threads_of<TPR>) k_norm_bwd(const Norm a) {
       }
       if (a.db && live) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) s[j].store(a.db + base, w[j]);
+        for (int j = 0; j < NV; ++j) s[j].template store<NT>(a.db + base, w[j]);
       }
     }
     if (a.dgate && !a.each) put(dgate, a.dgate + (size_t(g) * a.pieces + piece) * a.cols);
@@ -300,44 +318,57 @@ struct Cols {
   uint32_t count[3], groups[3];
   uint32_t cols, blocks;  // blocks: of 64 columns
 };
-__global__ void __launch_bounds__(256) k_norm_cols(const Cols a) {
-  __shared__ float sh[4][64];
+constexpr int kColWaves = 16;
+__global__ void __launch_bounds__(kColWaves * 64) k_norm_cols(const Cols a) {
+  __shared__ float sh[kColWaves][64];
   uint32_t id = blockIdx.x;
   int k = 0;
   while (id >= a.blocks * a.groups[k]) id -= a.blocks * a.groups[k++];
-  const uint32_t g = id / a.blocks, c = id % a.blocks * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-  const uint32_t n = a.count[k], lo = uint32_t(uint64_t(n) * w / 4), hi = uint32_t(uint64_t(n) * (w + 1) / 4);
+  const uint32_t g = id / a.blocks, lane = threadIdx.x & 63, c = id % a.blocks * 64 + lane, w = threadIdx.x >> 6;
+  const uint32_t n = a.count[k], lo = n * w / kColWaves, hi = n * (w + 1) / kColWaves;
   float v = 0.f;
   if (c < a.cols) {
     const float* p = a.part[k] + size_t(g) * n * a.cols + c;
-#pragma unroll 8
-    for (uint32_t i = lo; i < hi; ++i) v += p[size_t(i) * a.cols];
+    float part[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    uint32_t i = lo;
+    for (; i + 8 <= hi; i += 8)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) part[e] += p[size_t(i + e) * a.cols];
+    for (; i < hi; ++i) v += p[size_t(i) * a.cols];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v += part[e];
   }
-  sh[w][threadIdx.x & 63] = v;
+  sh[w][lane] = v;
   __syncthreads();
-  if (w == 0 && c < a.cols)
-    a.out[k][size_t(g) * a.cols + c] = (sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x]);
+  if (w || c >= a.cols) return;
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < kColWaves; ++i) v += sh[i][lane];
+  a.out[k][size_t(g) * a.cols + c] = v;
 }
 
 // f.run<TPR, NV, W>() for a width.
 template <class F>
 bool dispatch(uint32_t cols, const F& f) {
   if (cols < 4) return f.template run<64, 1, 1>();
+  if (cols <= 64) return f.template run<16, 1, 4>();
+  if (cols <= 128) return f.template run<32, 1, 4>();
   if (cols <= 256) return f.template run<64, 1, 4>();
   if (cols <= 512) return f.template run<64, 2, 4>();
   if (cols <= 1024) return f.template run<256, 1, 4>();
   if (cols <= 2048) return f.template run<256, 2, 4>();
-  if (cols <= 4096) return f.template run<256, 4, 4>();
-  if (cols <= 8192) return f.template run<1024, 2, 4>();
+  if (cols <= 4096) return f.template run<512, 2, 4>();
+  if (cols <= 8192) return f.template run<512, 4, 4>();
   return f.template run<1024, 4, 4>();
 }
 
 struct Fwd {
   const Norm& a;
+  bool nt;
   template <int TPR, int NV, int W>
   bool run() const {
     constexpr int T = threads_of<TPR>;
-    hipLaunchKernelGGL((k_norm_fwd<TPR, NV, W>), dim3(cdiv(a.rows, T / TPR)), dim3(T), 0, stream(), a);
+    hipLaunchKernelGGL((nt ? k_norm_fwd<TPR, NV, W, true> : k_norm_fwd<TPR, NV, W, false>), dim3(cdiv(a.rows, T / TPR)), dim3(T), 0, stream(), a);
     return check_launch("norm");
   }
 };
@@ -345,10 +376,13 @@ struct Fwd {
 struct Bwd {
   Norm& a;
   const NormGrads& g;
+  bool nt;
   template <int TPR, int NV, int W>
   bool run() const {
     constexpr int T = threads_of<TPR>, RPB = T / TPR;
-    const uint32_t gates = cdiv(a.rows, a.per), want = std::min(cdiv(a.rows, RPB), uint32_t(num_cus()) * 2048 / T);
+    // 1024 threads a CU: more leave more partial sums, fewer less in flight (8192 x 2048:
+    // 84 us with 512 or 1024, 94 with 1536, 88 with 2048; 4096 x 8192: 169, 173, 193, 185).
+    const uint32_t gates = cdiv(a.rows, a.per), want = std::min(cdiv(a.rows, RPB), uint32_t(num_cus()) * 1024 / T);
     uint32_t wgs;
     if (gates >= want) {
       a.pieces = 1;
@@ -376,7 +410,7 @@ struct Bwd {
     a.dgate = gatePart ? ws + pGate : g.dgate;
     a.dpost = g.dpost && wgs > 1 ? ws + pPost : g.dpost;
     a.dpre = g.dpre && wgs > 1 ? ws + pPre : g.dpre;
-    hipLaunchKernelGGL((k_norm_bwd<TPR, NV, W>), dim3(wgs), dim3(T), 0, stream(), a);
+    hipLaunchKernelGGL((nt ? k_norm_bwd<TPR, NV, W, true> : k_norm_bwd<TPR, NV, W, false>), dim3(wgs), dim3(T), 0, stream(), a);
     if (!check_launch("norm")) return false;
     uint32_t sums = 0, blocks = 0;
     auto add = [&](const float* part, float* out, uint32_t count, uint32_t groups) {
@@ -390,7 +424,7 @@ struct Bwd {
     if (g.dpost && wgs > 1) add(a.dpost, g.dpost, wgs, 1);
     if (g.dpre && wgs > 1) add(a.dpre, g.dpre, wgs, 1);
     if (!sums) return true;
-    hipLaunchKernelGGL(k_norm_cols, dim3(blocks), dim3(256), 0, stream(), c);
+    hipLaunchKernelGGL(k_norm_cols, dim3(blocks), dim3(kColWaves * 64), 0, stream(), c);
     return check_launch("norm");
   }
 };
@@ -419,9 +453,9 @@ Norm norm_of(const NormArgs& x) {
 
 bool norm_forward(const NormArgs& x) {
   const Norm a = norm_of(x);
-  const double n = double(x.rows) * x.cols;
-  ProfScope prof("norm", 10 * n, 4 * n * (x.block ? (x.n ? 4 : 3) : 2));
-  return dispatch(x.cols, Fwd{a});
+  const double n = double(x.rows) * x.cols, bytes = 4 * n * (x.block ? (x.n ? 4 : 3) : 2);
+  ProfScope prof("norm", 10 * n, bytes);
+  return dispatch(x.cols, Fwd{a, stream_nt(bytes)});
 }
 
 bool norm_backward(const NormArgs& x, const NormGrads& g) {
@@ -431,8 +465,9 @@ bool norm_backward(const NormArgs& x, const NormGrads& g) {
   a.dx = g.dx;
   a.db = g.db;
   const double n = double(x.rows) * x.cols;
-  ProfScope prof("norm", 20 * n, 4 * n * ((g.dh ? 1 : 0) + (g.dn ? 2 : 0) + (x.block ? 1 : 0) + (g.dx ? 1 : 0) + (g.db ? 1 : 0)));
-  return dispatch(x.cols, Bwd{a, g});
+  const double bytes = 4 * n * ((g.dh ? 1 : 0) + (g.dn ? 2 : 0) + (x.block ? 1 : 0) + (g.dx ? 1 : 0) + (g.db ? 1 : 0));
+  ProfScope prof("norm", 20 * n, bytes);
+  return dispatch(x.cols, Bwd{a, g, stream_nt(bytes)});
 }
 
 }  // namespace dce
