@@ -1,0 +1,49 @@
+// What the kernels of the gated feed-forward block (dce_mlp.hip, and those on fp16
+// parts, dce_mlp_parts.hip) share.
+#pragma once
+#include "dce_internal.h"
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+namespace dce {
+
+// act(g), and its derivative d.
+template <MlpAct ACT>
+__device__ __forceinline__ float act_grad(float g, float& d) {
+  if constexpr (ACT == kGelu) {  // erfc: 1 + erf would cancel for g << 0
+    const float p = 0.5f * erfcf(-g * 0.70710678f);
+    d = p + g * (0.39894228f * expf(-0.5f * g * g));
+    return g * p;
+  } else if constexpr (ACT == kRelu) {
+    d = g > 0.f ? 1.f : 0.f;
+    return g <= 0.f ? 0.f : g;  // NaN stays
+  } else {
+    float p, q;
+    sigmoid_pair(g, p, q);
+    d = ACT == kSilu ? p + g * p * q : p * q;
+    return ACT == kSilu ? g * p : p;
+  }
+}
+template <MlpAct ACT>
+__device__ __forceinline__ float act(float g) {
+  float d;
+  return act_grad<ACT>(g, d);
+}
+
+// f(std::integral_constant<MlpAct, act>)
+template <class F>
+void by_act(MlpAct act, F&& f) {
+  if (act == kSilu) f(std::integral_constant<MlpAct, kSilu>{});
+  if (act == kGelu) f(std::integral_constant<MlpAct, kGelu>{});
+  if (act == kRelu) f(std::integral_constant<MlpAct, kRelu>{});
+  if (act == kSigmoid) f(std::integral_constant<MlpAct, kSigmoid>{});
+}
+
+// On fp16 parts, for large calls.
+bool mlp_on_parts(const MlpArgs& a);
+bool mlp_forward_parts(const MlpArgs& a);
+bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd);
+
+}  // namespace dce

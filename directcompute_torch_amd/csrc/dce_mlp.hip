@@ -6,10 +6,7 @@
 //
 //   dm = dy Wd^T,  dg = dm u act'(g),  du = dm act(g),
 //   dWd = m^T dy,  dWg = x^T dg,  dWu = x^T du,  dx = dg Wg^T + du Wu^T.
-#include "dce_internal.h"
-
-#include <algorithm>
-#include <cmath>
+#include "dce_mlp.h"
 
 namespace dce {
 
@@ -17,34 +14,6 @@ namespace {
 
 constexpr int kT = 256;
 inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b); }
-
-// act(g) and its derivative d.
-__device__ __forceinline__ float sigmoid_(float g) {
-  const float e = expf(-fabsf(g)), big = 1.f / (1.f + e);
-  return g >= 0.f ? big : e * big + (g - g);  // NaN stays
-}
-template <MlpAct ACT>
-__device__ __forceinline__ float act(float g) {
-  if constexpr (ACT == kSilu) return g * sigmoid_(g);
-  if constexpr (ACT == kGelu) return g * (0.5f * erfcf(-g * 0.70710678f));
-  if constexpr (ACT == kRelu) return g <= 0.f ? 0.f : g;
-  return sigmoid_(g);
-}
-template <MlpAct ACT>
-__device__ __forceinline__ float act_grad(float g, float& d) {
-  if constexpr (ACT == kGelu) {
-    const float p = 0.5f * erfcf(-g * 0.70710678f);
-    d = p + g * (0.39894228f * expf(-0.5f * g * g));
-    return g * p;
-  } else if constexpr (ACT == kRelu) {
-    d = g > 0.f ? 1.f : 0.f;
-    return act<kRelu>(g);
-  } else {
-    const float p = sigmoid_(g), q = sigmoid_(-g);
-    d = ACT == kSilu ? p + g * p * q : p * q;
-    return ACT == kSilu ? g * p : p;
-  }
-}
 
 // m = act(g) u, n values.
 template <MlpAct ACT>
@@ -65,15 +34,6 @@ __global__ void __launch_bounds__(kT)
 }
 __global__ void __launch_bounds__(kT) k_mlp_add(const float* a, float* to, uint32_t n) {
   for (uint32_t i = blockIdx.x * kT + threadIdx.x; i < n; i += gridDim.x * kT) to[i] += a[i];
-}
-
-// f(std::integral_constant<MlpAct, act>)
-template <class F>
-void by_act(MlpAct act, F&& f) {
-  if (act == kSilu) f(std::integral_constant<MlpAct, kSilu>{});
-  if (act == kGelu) f(std::integral_constant<MlpAct, kGelu>{});
-  if (act == kRelu) f(std::integral_constant<MlpAct, kRelu>{});
-  if (act == kSigmoid) f(std::integral_constant<MlpAct, kSigmoid>{});
 }
 
 // A buffer that goes back to the pool with the scope: calls on the stream that
@@ -124,10 +84,10 @@ bool backward_plain(const MlpArgs& a, const float* dy, float* dx, float* dwg, fl
 
 }  // namespace
 
-bool mlp_forward(const MlpArgs& a) { return forward_plain(a); }
+bool mlp_forward(const MlpArgs& a) { return mlp_on_parts(a) ? mlp_forward_parts(a) : forward_plain(a); }
 
 bool mlp_backward(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
-  return backward_plain(a, dy, dx, dwg, dwu, dwd);
+  return mlp_on_parts(a) ? mlp_backward_parts(a, dy, dx, dwg, dwu, dwd) : backward_plain(a, dy, dx, dwg, dwu, dwd);
 }
 
 }  // namespace dce
