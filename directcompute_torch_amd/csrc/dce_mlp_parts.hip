@@ -2,18 +2,24 @@
 // third of the fp16 MFMA rate, which is 16 times the fp32 one, with fp32's accuracy.
 //
 // A value x is kept as x 2^e = h + l, two fp16 values rounded to nearest, and
-// h h + (h l + l h) stands for a product.  The exponent is one for each row of an
-// operand (a token's values, an output's weights), such that its largest value lies
-// in [2^14, 2^15): l's half step is then 2^-25, 2^-39 of that, so that values down to
-// 2^-15 of their row's largest keep 24 bits.  Rows only: the exponents are the product's
-// factors of its rows and columns, and cost its loop nothing.  So a matrix that is
-// summed over its rows in one product and over its columns in another is split twice.
+// h h + (h l + l h) stands for a product.  The exponent e of a product's operand is one
+// for each row (a token's values, an output's weights), such that its largest value
+// lies in [2^14, 2^15): l's half step is then 2^-25, 2^-39 of that, and values down to
+// 2^-15 of their row's largest keep 24 bits.  As factors of the product's rows and
+// columns the exponents cost its loop nothing.  A matrix that is summed over its rows
+// in one product and over its columns in another is split twice, with exponents each way.
 //
-// The steps, forward:  maxima -> parts of x, Wg, Wu, Wd -> g, u, m and m's maxima
-// (one product over Wg and Wu, whose columns lie in turn, 32 by 32, so that a wave has
-// g and u of one place) -> parts of m -> y.
-// Backward:  maxima -> parts of dy, Wd, x, W -> dm, and from it dg, du, m and their
-// maxima -> their parts -> dx, dWg, dWu, dWd.
+// For x, dy and the weights a pass finds the maxima and another makes the parts.  What a
+// product leaves for the next one (m forward; dg, du, m backward) is split by its
+// epilogue, which knows the largest value of its own tile's rows and columns only: the
+// parts get that exponent, kept in a byte per row and tile, and the next product's loop
+// takes them to the row's own, that of the largest of them, by a power of two.
+//
+// The steps, forward:  maxima -> parts of x, Wg, Wu, Wd -> g, u and m's parts (one
+// product over Wg and Wu, whose columns lie in turn, 32 by 32, so that a wave has g and
+// u of one place) -> y.
+// Backward:  maxima -> parts of dy, Wd, x, W -> dm, and from it parts of dg, du, m ->
+// dx, dWg, dWu, dWd.
 #include "dce_mlp.h"
 
 namespace dce {
@@ -29,21 +35,86 @@ using f16v = float __attribute__((ext_vector_type(16)));
 inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b); }
 inline uint32_t pad(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
 
-// The exponent for a row whose largest value has these bits (sign aside).
-__device__ __forceinline__ int exp_of(uint32_t bits) { return bits ? 14 + 127 - int(bits >> 23) : 0; }
+// The exponent for values of which the largest has this exponent field: it goes to
+// [2^14, 2^15), unless it is below 2^-112 (2^127 is the largest factor).
+__device__ __forceinline__ int exp_of(int field) { return min(141 - field, 127); }
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ int field_of(uint32_t bits) { return int(bits >> 23); }
 
-// Parts in memory: 8 consecutive values of a row are 8 h, then 8 l (32 bytes).
-__device__ __forceinline__ void put8(float* to, const float* x, int e) {
-  h8 h, l;
+// Parts in memory: 32 consecutive values of a row are 32 h, then 32 l (128 bytes).  x: 8
+// values of the row at `to`, from value c on, times `by`.
+__device__ __forceinline__ void split8(const float* x, float by, h8& h, h8& l) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float v = ldexpf(x[i], e);
+    const float v = x[i] * by;
     h[i] = _Float16(v);
     l[i] = _Float16(v - float(h[i]));
   }
-  h8* p = reinterpret_cast<h8*>(to);
+}
+__device__ __forceinline__ void put8(float* to, uint32_t c, const float (&x)[8], float by) {
+  h8 h, l;
+  split8(x, by, h, l);
+  h8* p = reinterpret_cast<h8*>(to + (c & ~31u)) + (c & 31u) / 8;
   p[0] = h;
-  p[1] = l;
+  p[4] = l;
+}
+// |v| for a maximum: fmaxf drops NaN, which then counts as infinity.
+__device__ __forceinline__ float size_of(float v) { return v == v ? fabsf(v) : INFINITY; }
+// One operand of a product: [rows][depth] as parts.
+struct Side {
+  float* p;
+  uint32_t* top;   // bits of the largest value of each row
+  uint8_t* field;  // exponent field of the largest value of each row's block, [block][rows]; null: that of its row
+  uint32_t rows, depth;
+};
+
+// A tile of 128 rows of COLS values in LDS, its octets of columns XORed by the octet of
+// rows, so that neither a row's octets nor a column's meet in a bank often.
+template <int COLS>
+__device__ __forceinline__ int tile_at(int r, int c) {
+  return r * COLS + ((((c >> 3) ^ (r >> 3)) & (COLS / 8 - 1)) << 3) + (c & 7);
+}
+// Parts of its rows, with the exponents that they have in this tile, at row r0 and value c0 of t.
+template <int COLS>
+__device__ __forceinline__ void put_rows(const float* S, const Side& t, uint32_t r0, uint32_t c0) {
+  constexpr int OCT = COLS / 8;
+  for (int u = threadIdx.x; u < 128 * OCT; u += kT) {
+    const int r = u / OCT, o = u % OCT;
+    const f4* p = reinterpret_cast<const f4*>(S + tile_at<COLS>(r, 8 * o));
+    const f4 a = p[0], b = p[1];
+    const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, size_of(v[e]));
+    m = group8_reduce(m, OpMaxR());
+    if constexpr (OCT == 16) m = fmaxf(m, xl::dpp<xl::kRowMirror>(m));
+    const uint32_t bits = __float_as_uint(m);
+    put8(t.p + size_t(r0 + r) * t.depth, c0 + 8 * o, v, pow2(exp_of(field_of(bits))));
+    if (o == 0) {
+      t.field[size_t(c0 / COLS) * t.rows + r0 + r] = uint8_t(field_of(bits));
+      if (bits) atomicMax(t.top + r0 + r, bits);
+    }
+  }
+}
+// Parts of a 128 x 128 tile's columns, likewise, at row c0 and value r0 of t.
+__device__ __forceinline__ void put_columns(const float* S, const Side& t, uint32_t r0, uint32_t c0) {
+  for (int u = threadIdx.x; u < 128 * 16; u += kT) {
+    const int c = u / 16, o = u % 16;
+    const float* p = S + tile_at<128>(8 * o, c);
+    float v[8], m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = p[e * 128];
+      m = fmaxf(m, size_of(v[e]));
+    }
+    m = group8_reduce(m, OpMaxR());
+    const uint32_t bits = __float_as_uint(fmaxf(m, xl::dpp<xl::kRowMirror>(m)));
+    put8(t.p + size_t(c0 + c) * t.depth, r0 + 8 * o, v, pow2(exp_of(field_of(bits))));
+    if (o == 0) {
+      t.field[size_t(r0 / 128) * t.rows + c0 + c] = uint8_t(field_of(bits));
+      if (bits) atomicMax(t.top + c0 + c, bits);
+    }
+  }
 }
 
 __global__ void __launch_bounds__(kT) k_mlp_clear(uint32_t* p, uint32_t n) {
@@ -51,18 +122,16 @@ __global__ void __launch_bounds__(kT) k_mlp_clear(uint32_t* p, uint32_t n) {
 }
 
 // ---------------------------------------------------------------------------
-// Maxima and parts of up to six matrices, [rows][pitch] of which rows x cols count.
+// Maxima and parts of up to five matrices, [rows][cols].
 // ---------------------------------------------------------------------------
 struct Job {
-  float* src;
-  uint32_t rows, cols, pitch;
-  uint32_t* rowMax;  // bits of the largest value of each row; null: not wanted
-  uint32_t* colMax;  // of each column; at place col, or with columns in turn at lane(col)
-  float *straight, *across;          // parts of the rows, of the columns; null: none
-  uint32_t sPitch, aPitch, sRows, aRows;  // in values; rows to write (zeros from the matrix's end on)
-  int turn;  // -1: no; 0, 1: its columns are those of Wg, Wu in turn
+  const float* src;
+  uint32_t rows, cols;
+  Side straight, across;  // of its rows, of its columns; p null: not wanted
+  uint32_t c0;            // straight: the place of its columns
+  int turn;               // across: 0, 1: its columns are those of Wg, Wu in turn; -1: no
 };
-constexpr int kJobs = 6;
+constexpr int kJobs = 5;
 struct Jobs {
   Job j[kJobs];
   uint32_t start[kJobs + 1];
@@ -76,64 +145,88 @@ __device__ __forceinline__ int find_job(const Jobs& t, uint32_t blk) {
 __device__ __forceinline__ uint32_t in_turn(uint32_t c, int turn) {
   return turn < 0 ? c : (c >> 5) * 64 + uint32_t(turn) * 32 + (c & 31);
 }
-// In a tile of 32 rows and 256 columns for each workgroup.
-constexpr uint32_t kMaxRows = 32;
+// 64 rows and 256 columns for each workgroup, 16 rows for each wave.  A width that is
+// no multiple of 4 has its last quad end with the row.
+constexpr uint32_t kMaxRows = 64;
 __global__ void __launch_bounds__(kT) k_mlp_max(const Jobs t) {
+  __shared__ uint32_t tops[4][kT];
   const int k = find_job(t, blockIdx.x);
   const Job J = t.j[k];
-  const uint32_t id = blockIdx.x - t.start[k], across = (J.cols + kT - 1) / kT;
-  const uint32_t r0 = id / across * kMaxRows, c = (id % across) * kT + threadIdx.x;
-  const bool in = c < J.cols;
-  const float* p = J.src + size_t(r0) * J.pitch + min(c, J.cols - 1);
-  uint32_t v[kMaxRows], top = 0;
+  const uint32_t id = blockIdx.x - t.start[k], wide = (J.cols + kT - 1) / kT, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint32_t r0 = id / wide * kMaxRows + w * 16, c0 = id % wide * kT, c = min(c0 + lane * 4, J.cols - 4);
+  f4u v[16];
 #pragma unroll
-  for (uint32_t i = 0; i < kMaxRows; ++i) v[i] = __float_as_uint(p[size_t(min(i, J.rows - 1 - r0)) * J.pitch]) & 0x7fffffffu;
+  for (uint32_t i = 0; i < 16; ++i) v[i] = ldus<false, f4u>(J.src + size_t(min(r0 + i, J.rows - 1)) * J.cols + c);
+  if (J.straight.p) {
 #pragma unroll
-  for (uint32_t i = 0; i < kMaxRows; ++i) top = max(top, v[i]);
-  if (J.colMax && in && top) atomicMax(J.colMax + in_turn(c, J.turn), top);
-  if (!J.rowMax) return;
+    for (uint32_t i = 0; i < 16; ++i) {
+      float m = 0.f;
 #pragma unroll
-  for (uint32_t i = 0; i < kMaxRows; ++i) {
-    // as floats, which order as their bits do; one that is not finite is infinity here
-    const float f = in ? (v[i] > 0x7f800000u ? INFINITY : __uint_as_float(v[i])) : 0.f;
-    const uint32_t m = __float_as_uint(wave_reduce(f, OpMaxR()));
-    if ((threadIdx.x & 63) == 0 && r0 + i < J.rows && m) atomicMax(J.rowMax + r0 + i, m);
+      for (int e = 0; e < 4; ++e) m = fmaxf(m, size_of(v[i][e]));
+      m = wave_reduce(m, OpMaxR());
+      if (lane == 0 && r0 + i < J.rows && m > 0.f) atomicMax(J.straight.top + r0 + i, __float_as_uint(m));
+    }
   }
+  if (!J.across.p) return;
+  float top[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (uint32_t i = 0; i < 16; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], size_of(v[i][e]));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) tops[w][lane * 4 + e] = __float_as_uint(top[e]);
+  __syncthreads();
+  // column threadIdx.x of the lanes' quads (two may be the same one)
+  const uint32_t m = max(max(tops[0][threadIdx.x], tops[1][threadIdx.x]), max(tops[2][threadIdx.x], tops[3][threadIdx.x]));
+  const uint32_t at = min(c0 + (threadIdx.x & ~3u), J.cols - 4) + (threadIdx.x & 3);
+  if (m) atomicMax(J.across.top + in_turn(at, J.turn), m);
 }
 
-// A 64 x 64 tile through LDS.  `straight` may be the matrix itself.
-constexpr int kSq = 64, kPitch = 68;
+// A 128 x 128 tile through LDS.
 __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
-  __shared__ float S[kSq * kPitch];
+  __shared__ __attribute__((aligned(16))) float S[128 * 128];
   const int k = find_job(t, blockIdx.x);
   const Job J = t.j[k];
-  const uint32_t across = max(J.straight ? J.sPitch / (J.turn < 0 ? 1 : 2) : 0u, J.across ? J.aRows / (J.turn < 0 ? 1 : 2) : 0u);
-  const uint32_t tc = (across + kSq - 1) / kSq;
-  const uint32_t id = blockIdx.x - t.start[k], i0 = id / tc * kSq, j0 = id % tc * kSq;
+  const uint32_t tc = (J.cols + 127) / 128, id = blockIdx.x - t.start[k], i0 = id / tc * 128, j0 = id % tc * 128;
+  {
+    // a quad of 16 rows for each thread; the last one ends with the row, as above
+    const uint32_t q = threadIdx.x & 31, c = j0 + q * 4, at = min(c, J.cols - 4), off = min(c - at, 4u);
+    f4u v[16];
 #pragma unroll
-  for (int u = 0; u < kSq * kSq / kT; ++u) {
-    const uint32_t s = threadIdx.x + kT * u, r = s / kSq, c = s % kSq;
-    const float v = J.src[size_t(min(i0 + r, J.rows - 1)) * J.pitch + min(j0 + c, J.cols - 1)];
-    S[r * kPitch + c] = i0 + r < J.rows && j0 + c < J.cols ? v : 0.f;
+    for (uint32_t i = 0; i < 16; ++i)
+      v[i] = ldus<false, f4u>(J.src + size_t(min(i0 + (threadIdx.x >> 5) + 8 * i, J.rows - 1)) * J.cols + at);
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      const uint32_t r = (threadIdx.x >> 5) + 8 * i;
+      f4 x = {v[i][0], v[i][1], v[i][2], v[i][3]};
+      if (off == 1) x = f4{x[1], x[2], x[3], 0.f};
+      if (off == 2) x = f4{x[2], x[3], 0.f, 0.f};
+      if (off == 3) x = f4{x[3], 0.f, 0.f, 0.f};
+      if (off == 4 || i0 + r >= J.rows) x = f4{0.f, 0.f, 0.f, 0.f};
+      *reinterpret_cast<f4*>(S + tile_at<128>(r, q * 4)) = x;
+    }
   }
   __syncthreads();
+  if (J.straight.p) {
+    for (int u = threadIdx.x; u < 128 * 16; u += kT) {
+      const int rl = u / 16, cl = u % 16 * 8;
+      const uint32_t r = i0 + rl;
+      float v[8];
 #pragma unroll
-  for (int u = 0; u < kSq * kSq / 8 / kT; ++u) {
-    const uint32_t slot = threadIdx.x + kT * u;
-    float v[8];
-    if (J.straight) {
-      const uint32_t r = slot / 8, c = slot % 8 * 8, to = in_turn(j0 + c, J.turn);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = S[r * kPitch + c + e];
-      if (i0 + r < J.sRows && to < J.sPitch)
-        put8(J.straight + size_t(i0 + r) * J.sPitch + to, v, i0 + r < J.rows ? exp_of(J.rowMax[i0 + r]) : 0);
+      for (int e = 0; e < 8; ++e) v[e] = S[tile_at<128>(rl, cl) + e];
+      if (r < J.straight.rows && j0 + cl < J.straight.depth)
+        put8(J.straight.p + size_t(r) * J.straight.depth, J.c0 + j0 + cl, v, pow2(exp_of(field_of(J.straight.top[r]))));
     }
-    if (J.across) {
-      const uint32_t c = slot % 64, r = slot / 64 * 8, to = in_turn(j0 + c, J.turn);
+  }
+  if (J.across.p) {
+    for (int u = threadIdx.x; u < 128 * 16; u += kT) {
+      const int cl = u / 16, rl = u % 16 * 8;
+      const uint32_t c = in_turn(j0 + cl, J.turn), r = i0 + rl;
+      float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = S[(r + e) * kPitch + c];
-      if (to < J.aRows && i0 + r < J.aPitch)
-        put8(J.across + size_t(to) * J.aPitch + i0 + r, v, j0 + c < J.cols ? exp_of(J.colMax[to]) : 0);
+      for (int e = 0; e < 8; ++e) v[e] = S[tile_at<128>(rl, cl) + 128 * e];
+      if (c < J.across.rows && r < J.across.depth)
+        put8(J.across.p + size_t(c) * J.across.depth, r, v, pow2(exp_of(field_of(J.across.top[c]))));
     }
   }
 }
@@ -142,24 +235,30 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
 // Products C = P Q^T of parts, both along their rows, in 128 x 128 tiles of four
 // waves, 64 x 64 each (2 x 2 blocks of 32 x 32).  The depth goes in steps of 32 through
 // two LDS stages, the next one's direct loads in flight while one is multiplied.  A
-// stage's rows are eight 16-byte slots, h and l of 8 values in turn, XORed by the row
+// stage's rows are eight 16-byte slots, four of h and four of l, XORed by the row
 // so that a read of one slot of 16 rows covers the 64 banks once.  The two small
 // products have an accumulator of their own: an MFMA cuts what it adds off at the
 // scale of the largest addend, always downwards.
 // ---------------------------------------------------------------------------
 enum Op { STORE, GATE, GRAD };
 struct Prod {
-  const float *p, *q;              // parts, padded to whole tiles
-  const uint32_t *pMax, *qMax;
-  uint32_t tm, tn, depth;          // tiles; values of a row
-  uint32_t rows, cols;             // of the result
-  float* out;                      // STORE; GATE: m; GRAD: dg, du in turn
-  float* out2;                     // STORE with columns in turn: the second matrix; GRAD: m
-  uint32_t pitch;                  // of out
-  int turn;                        // STORE: columns in turn
-  float *g, *u;                    // GATE: kept (null: not); GRAD: read
-  uint32_t hidden;                 // their pitch
-  uint32_t *rowMax, *colMax, *colMax2;  // GATE: m's rows; GRAD: rows and columns of dg, du; columns of m
+  Side p, q;
+  uint32_t right;          // STORE: the side whose parts have exponents of their blocks is q, not p
+  uint32_t tm, tn, depth;  // tiles; values of a row that are multiplied
+  uint32_t block;          // values of a block of the scaled side (a power of two)
+  uint32_t rows, cols;     // of the result
+  float* out;              // STORE
+  float *g, *u;            // GATE: kept (null: not); GRAD: read
+  uint32_t hidden;         // their pitch
+  uint32_t start;          // STORE: the first workgroup
+  Side m, mc, dr, dgc, duc;  // GATE: m; GRAD: m's columns (p null: not wanted), rows of dg and du, their columns
+};
+
+// Up to four products of one launch.
+template <int N>
+struct Prods {
+  Prod a[N];
+  uint32_t count;
 };
 
 constexpr int kStageBytes = kTile * kStep * 4;
@@ -175,24 +274,24 @@ __device__ __forceinline__ void load_stage(const BRes& b, uint32_t pitchBytes, u
 __device__ __forceinline__ h8 frag(const char* S, int row, int c) {
   return *reinterpret_cast<const h8*>(S + (row * 8 + (c ^ swz(row))) * 16);
 }
-__device__ __forceinline__ float max32(float v) {  // over the 32 lanes of a half
-  v = group8_reduce(v, OpMaxR());
-  v = fmaxf(v, xl::dpp<xl::kRowMirror>(v));
-  return fmaxf(v, xl::swz(v));
-}
-// |v| for a maximum: fmaxf drops NaN, which then counts as infinity.
-__device__ __forceinline__ float size_of(float v) { return v == v ? fabsf(v) : INFINITY; }
+// 2^-d, nothing for what is too small.
+__device__ __forceinline__ _Float16 down(int d) { return _Float16(ldexpf(1.f, -d)); }
 
-template <Op OP, MlpAct ACT>
-__global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_mlp_product(const Prod a) {
+template <Op OP, MlpAct ACT, int N>
+__global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_mlp_product(const Prods<N> all) {
+  constexpr bool SCALED = OP == STORE;
+  const uint32_t place = xcd_block_id();
+  int which = 0;
+  if constexpr (N > 1)
+    while (which + 1 < int(all.count) && all.a[which + 1].start <= place) ++which;
+  const Prod& a = all.a[which];
   __shared__ __attribute__((aligned(16))) char S[4 * kStageBytes];
   // bands of 8 rows of tiles: what an XCD runs at once reads few rows of either side
-  const uint32_t id = xcd_block_id(), band = id / (8 * a.tn), in = id - band * 8 * a.tn, high = min(8u, a.tm - band * 8);
+  const uint32_t id = place - a.start, band = id / (8 * a.tn), in = id - band * 8 * a.tn, high = min(8u, a.tm - band * 8);
   const uint32_t tj = in / high, ti = band * 8 + (in - tj * high);
-  const uint32_t pitch = a.depth * 4;
   BRes bp, bq;
-  bp.init(a.p + size_t(ti) * kTile * a.depth, kTile * a.depth);
-  bq.init(a.q + size_t(tj) * kTile * a.depth, kTile * a.depth);
+  bp.init(a.p.p + size_t(ti) * kTile * a.p.depth, kTile * a.p.depth);
+  bq.init(a.q.p + size_t(tj) * kTile * a.q.depth, kTile * a.q.depth);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
   const int col = lane & 31, half = lane >> 5;
   f16v big[2][2], small[2][2];
@@ -202,10 +301,26 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) big[i][j][e] = small[i][j][e] = 0.f;
-  load_stage(bp, pitch, 0, S);
-  load_stage(bq, pitch, 0, S + kStageBytes);
+  // The scaled side's rows of this lane: their own exponent field, and the blocks'.
+  const bool right = SCALED && a.right;
+  const Side& sc = right ? a.q : a.p;
+  const uint32_t srow = (right ? tj * kTile + wn : ti * kTile + wm) + col;
+  int own[2] = {};
+  uint8_t next[2] = {};
+  _Float16 by[2] = {};
+  if constexpr (SCALED) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      own[i] = exp_of(field_of(sc.top[srow + 32 * i]));
+      next[i] = sc.field[srow + 32 * i];
+    }
+  }
+  load_stage(bp, a.p.depth * 4, 0, S);
+  load_stage(bq, a.q.depth * 4, 0, S + kStageBytes);
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
+  auto loop = [&](auto side) {
+  constexpr int SIDE = decltype(side)::value;  // 0: p is scaled, 1: q, -1: neither
   int s = 0;
   for (uint32_t k = 0; k < a.depth; k += kStep, s ^= 1) {
     const char* St = S + s * 2 * kStageBytes;
@@ -218,16 +333,37 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          p[kk][i][e] = frag(St, wm + 32 * i + col, 2 * (2 * kk + half) + e);
-          q[kk][i][e] = frag(St + kStageBytes, wn + 32 * i + col, 2 * (2 * kk + half) + e);
+          p[kk][i][e] = frag(St, wm + 32 * i + col, 4 * e + 2 * kk + half);
+          q[kk][i][e] = frag(St + kStageBytes, wn + 32 * i + col, 4 * e + 2 * kk + half);
         }
+    if constexpr (SCALED) {
+      if ((k & (a.block - 1)) == 0) {
+        const uint32_t then = min(k + a.block, a.depth - 1) / a.block;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          by[i] = down(exp_of(next[i]) - own[i]);
+          next[i] = sc.field[size_t(then) * sc.rows + srow + 32 * i];
+        }
+      }
+    }
     if (k + kStep < a.depth) {
-      char* N = S + (s ^ 1) * 2 * kStageBytes;
-      load_stage(bp, pitch, k + kStep, N);
-      load_stage(bq, pitch, k + kStep, N + kStageBytes);
+      char* Sn = S + (s ^ 1) * 2 * kStageBytes;
+      load_stage(bp, a.p.depth * 4, k + kStep, Sn);
+      load_stage(bq, a.q.depth * 4, k + kStep, Sn + kStageBytes);
     }
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int kk = 0; kk < 2; ++kk) {
+      if constexpr (SCALED) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if constexpr (SIDE == 1)
+              q[kk][i][e] *= by[i];
+            else
+              p[kk][i][e] *= by[i];
+          }
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -236,84 +372,112 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
           small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][1], small[i][j], 0, 0, 0);
           small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][1], q[kk][j][0], small[i][j], 0, 0, 0);
         }
+    }
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
   }
+  };
+  if constexpr (!SCALED)
+    loop(std::integral_constant<int, -1>{});
+  else if (right)
+    loop(std::integral_constant<int, 1>{});
+  else
+    loop(std::integral_constant<int, 0>{});
   // Row 8 (e / 4) + 4 half + e % 4 of a block, column `col`.
-  const uint32_t r0 = ti * kTile + wm, c0 = tj * kTile + wn;
+  const uint32_t r0 = ti * kTile, c0 = tj * kTile;
+  float* T = reinterpret_cast<float*>(S);
   int eq[2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const uint32_t n = c0 + 32 * j + col;
-    eq[j] = exp_of(a.qMax[n]);
-  }
-  float top[2][3] = {};  // GRAD: of dg, du, m in the lane's columns
+  for (int j = 0; j < 2; ++j) eq[j] = exp_of(field_of(a.q.top[c0 + wn + 32 * j + col]));
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const uint32_t r = r0 + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3);
-      const int ep = exp_of(a.pMax[r]);
-      float v[2];
+      const int ep = exp_of(field_of(a.p.top[r0 + wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3)]));
 #pragma unroll
-      for (int j = 0; j < 2; ++j) v[j] = ldexpf(big[i][j][e] + small[i][j][e], -(ep + eq[j]));
-      if constexpr (OP == STORE) {
-        if (r >= a.rows) continue;
+      for (int j = 0; j < 2; ++j) big[i][j][e] = ldexpf(big[i][j][e] + small[i][j][e], -(ep + eq[j]));
+    }
+  if constexpr (OP == STORE) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t r = r0 + wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          uint32_t n = c0 + 32 * j + col;
-          float* to = a.out;
-          if (a.turn) {
-            to = j ? a.out2 : a.out;
-            n = (c0 >> 1) + col;
-          }
-          if (n < a.cols && to) to[size_t(r) * a.pitch + n] = v[j];
+          const uint32_t n = c0 + wn + 32 * j + col;
+          if (r < a.rows && n < a.cols) a.out[size_t(r) * a.cols + n] = big[i][j][e];
         }
       }
-      if constexpr (OP == GATE) {
-        const uint32_t f = (c0 >> 1) + col;
-        const float m = act<ACT>(v[0]) * v[1];
-        a.out[size_t(r) * a.pitch + f] = m;
+  }
+  if constexpr (OP == GATE) {
+    const uint32_t f = ((c0 + wn) >> 1) + col;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t r = r0 + wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3);
         if (a.g && r < a.rows && f < a.hidden) {
-          a.g[size_t(r) * a.hidden + f] = v[0];
-          a.u[size_t(r) * a.hidden + f] = v[1];
+          a.g[size_t(r) * a.hidden + f] = big[i][0][e];
+          a.u[size_t(r) * a.hidden + f] = big[i][1][e];
         }
-        const float most = max32(size_of(m));
-        if (col == 0 && most > 0.f) atomicMax(a.rowMax + r, __float_as_uint(most));
+        T[tile_at<64>(wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3), (wn >> 1) + col)] = act<ACT>(big[i][0][e]) * big[i][1][e];
       }
-      if constexpr (OP == GRAD) {
-        float most = 0.f;
+    __syncthreads();
+    put_rows<64>(T, a.m, r0, c0 / 2);
+  }
+  if constexpr (OP == GRAD) {
+    // g and u, zeros outside, where dm is zeros too (or its row has no value that counts).
+    f16v u[2][2];
+    const uint32_t at[2] = {c0 + wn + col < a.hidden ? (wm + 4 * half) * a.hidden + c0 + wn + col : kOob,
+                            c0 + wn + 32 + col < a.hidden ? (wm + 4 * half) * a.hidden + c0 + wn + 32 + col : kOob};
+    BRes bg, bu;
+    bg.init(a.g + size_t(r0) * a.hidden, min(a.rows - r0, 128u) * a.hidden);
+    bu.init(a.u + size_t(r0) * a.hidden, min(a.rows - r0, 128u) * a.hidden);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {  // small: g
+          const uint32_t off = at[j] + (32 * i + 8 * (e >> 2) + (e & 3)) * a.hidden;
+          small[i][j][e] = bg.ld1(off);
+          u[i][j][e] = bu.ld1(off);
+        }
+    // big: dm, then dg; small: g, then du; u, then m
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint32_t f = c0 + 32 * j + col;
-          const bool live = r < a.rows && f < a.hidden;
-          const size_t at = size_t(min(r, a.rows - 1)) * a.hidden + min(f, a.hidden - 1);
           float d;
-          const float g = a.g[at], u = a.u[at], y = act_grad<ACT>(g, d);
-          const float dg = live ? v[j] * u * d : 0.f, du = live ? v[j] * y : 0.f, m = live ? y * u : 0.f;
-          float* to = a.out + size_t(r) * a.pitch + in_turn(f, 0);
-          to[0] = dg;
-          to[32] = du;
-          a.out2[size_t(r) * (a.pitch / 2) + f] = m;
-          top[j][0] = fmaxf(top[j][0], size_of(dg));
-          top[j][1] = fmaxf(top[j][1], size_of(du));
-          top[j][2] = fmaxf(top[j][2], size_of(m));
-          most = fmaxf(most, fmaxf(size_of(dg), size_of(du)));
+          const float y = act_grad<ACT>(small[i][j][e], d), dm = big[i][j][e], v = u[i][j][e];
+          __builtin_amdgcn_sched_barrier(0);  // one at a time: no registers for more
+          big[i][j][e] = dm * v * d;
+          small[i][j][e] = dm * y;
+          u[i][j][e] = y * v;
         }
-        most = max32(most);
-        if (col == 0 && most > 0.f) atomicMax(a.rowMax + r, __float_as_uint(most));
-      }
-    }
-  if constexpr (OP == GRAD) {
+    auto tile = [&](const f16v (&v)[2][2]) {
+      __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint32_t f = c0 + 32 * j + col;
-      uint32_t* to[3] = {a.colMax + in_turn(f, 0), a.colMax + in_turn(f, 1), a.colMax2 + f};
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int w = 0; w < 3; ++w)
-        if (top[j][w] > 0.f) atomicMax(to[w], __float_as_uint(top[j][w]));
-    }
+        for (int e = 0; e < 16; ++e)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) T[tile_at<128>(wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3), wn + 32 * j + col)] = v[i][j][e];
+      __syncthreads();
+    };
+    tile(big);
+    if (a.dr.p) put_rows<128>(T, a.dr, r0, c0);
+    if (a.dgc.p) put_columns(T, a.dgc, r0, c0);
+    tile(small);
+    if (a.dr.p) put_rows<128>(T, a.dr, r0, a.dr.depth / 2 + c0);
+    if (a.duc.p) put_columns(T, a.duc, r0, c0);
+    if (!a.mc.p) return;
+    tile(u);
+    put_columns(T, a.mc, r0, c0);
   }
 }
 
@@ -327,248 +491,185 @@ struct Places {
   }
 };
 
-template <class F>
-uint32_t job_blocks(Jobs& t, F&& f) {
+// A side of whole tiles of rows, in the workspace; its maxima come after all parts.
+struct Plan {
+  Places at;
+  size_t tops = 0;  // floats of maxima
+  struct Made {
+    Side* s;
+    size_t p, top, field;
+  };
+  Made all[16];
+  int count = 0;
+  void side(Side& s, uint32_t rows, uint32_t depth, uint32_t block = 0) {
+    s.rows = rows;
+    s.depth = depth;
+    all[count++] = {&s, at.take(size_t(rows) * depth), tops, block ? at.take((size_t(rows) * (depth / block) + 3) / 4) : ~size_t(0)};
+    tops += rows;
+  }
+  // The workspace, with its maxima cleared.
+  bool lay() {
+    const size_t first = at.take(tops);
+    float* ws = workspace(at.next);
+    if (!ws) return false;
+    for (int i = 0; i < count; ++i) {
+      Side& s = *all[i].s;
+      s.p = ws + all[i].p;
+      s.top = reinterpret_cast<uint32_t*>(ws + first) + all[i].top;
+      s.field = all[i].field == ~size_t(0) ? nullptr : reinterpret_cast<uint8_t*>(ws + all[i].field);
+    }
+    hipLaunchKernelGGL(k_mlp_clear, dim3(std::min(cdiv(tops, kT), 256u)), dim3(kT), 0, stream(),
+                       reinterpret_cast<uint32_t*>(ws + first), uint32_t(tops));
+    return check_launch("gated_mlp");
+  }
+};
+
+void add(Jobs& t, const float* src, uint32_t rows, uint32_t cols, const Side& straight, const Side& across, uint32_t c0 = 0, int turn = -1) {
+  Job& j = t.j[t.count++];
+  j.src = src;
+  j.rows = rows;
+  j.cols = cols;
+  j.straight = straight;
+  j.across = across;
+  j.c0 = c0;
+  j.turn = turn;
+}
+bool run_jobs(Jobs& t) {
   uint32_t n = 0;
   for (uint32_t i = 0; i < t.count; ++i) {
     t.start[i] = n;
-    n += f(t.j[i]);
+    n += cdiv(t.j[i].rows, kMaxRows) * cdiv(t.j[i].cols, kT);
   }
-  t.start[t.count] = n;
-  return n;
-}
-bool run_max(Jobs& t) {
-  const uint32_t n = job_blocks(t, [](const Job& j) { return cdiv(j.rows, kMaxRows) * cdiv(j.cols, kT); });
   hipLaunchKernelGGL(k_mlp_max, dim3(n), dim3(kT), 0, stream(), t);
-  return check_launch("gated_mlp");
-}
-bool run_split(Jobs& t) {
-  const uint32_t n = job_blocks(t, [](const Job& j) {
-    const uint32_t by = j.turn < 0 ? 1 : 2, high = std::max(j.straight ? j.sRows : 0, j.across ? j.aPitch : 0);
-    const uint32_t wide = std::max(j.straight ? j.sPitch / by : 0, j.across ? j.aRows / by : 0);
-    return cdiv(high, kSq) * cdiv(wide, kSq);
-  });
+  if (!check_launch("gated_mlp")) return false;
+  n = 0;
+  for (uint32_t i = 0; i < t.count; ++i) {
+    t.start[i] = n;
+    n += cdiv(std::max(t.j[i].straight.p ? t.j[i].straight.rows : 0, t.j[i].across.p ? t.j[i].across.depth : 0), 128) * cdiv(t.j[i].cols, 128);
+  }
   hipLaunchKernelGGL(k_mlp_split, dim3(n), dim3(kT), 0, stream(), t);
   return check_launch("gated_mlp");
 }
-template <Op OP>
-bool run_product(const Prod& a, MlpAct act = kSilu) {
+template <Op OP, int N>
+bool run_products(Prods<N>& t, MlpAct act = kSilu) {
+  uint32_t n = 0;
+  for (uint32_t i = 0; i < t.count; ++i) {
+    Prod& a = t.a[i];
+    a.tm = a.p.rows / kTile;
+    a.tn = a.q.rows / kTile;
+    a.start = n;
+    n += a.tm * a.tn;
+  }
   by_act(act, [&](auto k) {
-    hipLaunchKernelGGL((k_mlp_product<OP, OP == STORE ? kSilu : decltype(k)::value>), dim3(a.tm * a.tn), dim3(kT), 0, stream(), a);
+    hipLaunchKernelGGL((k_mlp_product<OP, OP == STORE ? kSilu : decltype(k)::value, N>), dim3(n), dim3(kT), 0, stream(), t);
   });
   return check_launch("gated_mlp");
 }
-bool clear(uint32_t* p, size_t n) {
-  hipLaunchKernelGGL(k_mlp_clear, dim3(std::min(cdiv(n, kT), 256u)), dim3(kT), 0, stream(), p, uint32_t(n));
-  return check_launch("gated_mlp");
-}
-
-Job job(const float* src, uint32_t rows, uint32_t cols, uint32_t pitch, int turn = -1) {
-  Job j{};
-  j.src = const_cast<float*>(src);
-  j.rows = rows;
-  j.cols = cols;
-  j.pitch = pitch;
-  j.turn = turn;
-  return j;
+template <int N>
+void add(Prods<N>& t, const Side& p, const Side& q, bool right, uint32_t block, uint32_t rows, uint32_t cols, float* out) {
+  Prod& a = t.a[t.count++];
+  a.p = p;
+  a.q = q;
+  a.right = right;
+  a.depth = p.depth;
+  a.block = block;
+  a.rows = rows;
+  a.cols = cols;
+  a.out = out;
 }
 
 }  // namespace
 
 bool mlp_forward_parts(const MlpArgs& a) {
-  const uint32_t M = pad(a.rows, kTile), C = pad(a.cols, 64), F = pad(a.hidden, 64), O = pad(a.out, kTile);
-  Places at;
-  const size_t px = at.take(size_t(M) * C), pw = at.take(size_t(2) * F * C), pd = at.take(size_t(O) * F), pm = at.take(size_t(M) * F);
-  const size_t top = at.take(0), xMax = at.take(M), wMax = at.take(2 * size_t(F)), dMax = at.take(O), mMax = at.take(M), end = at.next;
-  float* ws = workspace(end);
-  if (!ws) return false;
-  auto bits = [&](size_t p) { return reinterpret_cast<uint32_t*>(ws + p); };
+  const uint32_t M = pad(a.rows, kTile), C = pad(a.cols, kTile), F = pad(a.hidden, kTile), O = pad(a.out, kTile);
+  Plan plan;
+  Side x, w, d, m;
+  plan.side(x, M, C);
+  plan.side(w, 2 * F, C);
+  plan.side(d, O, F);
+  plan.side(m, M, F, 64);
   ProfScope prof("mlp", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
-  if (!clear(bits(top), end - top)) return false;
+  if (!plan.lay()) return false;
   Jobs t{};
-  t.count = 4;
-  t.j[0] = job(a.x, a.rows, a.cols, a.cols);
-  t.j[0].rowMax = bits(xMax);
-  for (int w = 0; w < 2; ++w) {
-    t.j[1 + w] = job(w ? a.wu : a.wg, a.cols, a.hidden, a.hidden, w);
-    t.j[1 + w].colMax = bits(wMax);
-  }
-  t.j[3] = job(a.wd, a.hidden, a.out, a.out);
-  t.j[3].colMax = bits(dMax);
-  if (!run_max(t)) return false;
-  t.j[0].straight = ws + px;
-  t.j[0].sPitch = C;
-  t.j[0].sRows = M;
-  for (int w = 1; w < 3; ++w) {
-    t.j[w].across = ws + pw;
-    t.j[w].aPitch = C;
-    t.j[w].aRows = 2 * F;
-  }
-  t.j[3].across = ws + pd;
-  t.j[3].aPitch = F;
-  t.j[3].aRows = O;
-  if (!run_split(t)) return false;
-  Prod g{};
-  g.p = ws + px;
-  g.q = ws + pw;
-  g.pMax = bits(xMax);
-  g.qMax = bits(wMax);
-  g.tm = M / kTile;
-  g.tn = 2 * F / kTile;
+  add(t, a.x, a.rows, a.cols, x, {});
+  add(t, a.wg, a.cols, a.hidden, {}, w, 0, 0);
+  add(t, a.wu, a.cols, a.hidden, {}, w, 0, 1);
+  add(t, a.wd, a.hidden, a.out, {}, d);
+  if (!run_jobs(t)) return false;
+  Prods<1> t1{}, t2{};
+  t1.count = 1;
+  Prod& g = t1.a[0];
+  g.p = x;
+  g.q = w;
   g.depth = C;
   g.rows = a.rows;
-  g.out = ws + pm;
-  g.pitch = F;
+  g.m = m;
   g.hidden = a.hidden;
-  g.rowMax = bits(mMax);
   if (a.saved) {
     g.g = a.saved;
     g.u = a.saved + size_t(a.rows) * a.hidden;
   }
-  if (!run_product<GATE>(g, a.act)) return false;
-  t.count = 1;
-  t.j[0] = job(ws + pm, M, F, F);
-  t.j[0].rowMax = bits(mMax);
-  t.j[0].straight = ws + pm;
-  t.j[0].sPitch = F;
-  t.j[0].sRows = M;
-  if (!run_split(t)) return false;
-  Prod y{};
-  y.p = ws + pm;
-  y.q = ws + pd;
-  y.pMax = bits(mMax);
-  y.qMax = bits(dMax);
-  y.tm = M / kTile;
-  y.tn = O / kTile;
-  y.depth = F;
-  y.rows = a.rows;
-  y.cols = a.out;
-  y.out = a.y;
-  y.pitch = a.out;
-  return run_product<STORE>(y);
+  add(t2, m, d, false, 64, a.rows, a.out, a.y);
+  return run_products<GATE>(t1, a.act) && run_products<STORE>(t2);
 }
 
 bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
-  const bool weights = dwg || dwu;
-  // Each side of a product is padded to whole tiles, whichever it is.
   const uint32_t M = pad(a.rows, kTile), C = pad(a.cols, kTile), F = pad(a.hidden, kTile), O = pad(a.out, kTile);
-  Places at;
-  const size_t pyr = at.take(size_t(M) * O), pyc = dwd ? at.take(size_t(O) * M) : 0, pd = at.take(size_t(F) * O);
-  const size_t pxc = weights ? at.take(size_t(C) * M) : 0, pw = dx ? at.take(size_t(C) * 2 * F) : 0;
-  const size_t pg = at.take(size_t(M) * 2 * F), pgc = weights ? at.take(size_t(2) * F * M) : 0;
-  const size_t pm = at.take(size_t(M) * F), pmc = dwd ? at.take(size_t(F) * M) : 0;
-  const size_t top = at.take(0), yrMax = at.take(M), ycMax = at.take(O), dMax = at.take(F), xMax = at.take(C), wMax = at.take(C),
-               grMax = at.take(M), gcMax = at.take(2 * size_t(F)), mMax = at.take(F), end = at.next;
-  float* ws = workspace(end);
-  if (!ws) return false;
-  auto bits = [&](size_t p) { return reinterpret_cast<uint32_t*>(ws + p); };
+  Plan plan;
+  Side yr{}, yc{}, d{}, xc{}, w{}, dr{}, dgc{}, duc{}, mc{};
+  plan.side(yr, M, O);
+  plan.side(d, F, O);
+  if (dwd) {
+    plan.side(yc, O, M);
+    plan.side(mc, F, M, 128);
+  }
+  if (dwg || dwu) plan.side(xc, C, M);
+  if (dwg) plan.side(dgc, F, M, 128);
+  if (dwu) plan.side(duc, F, M, 128);
+  if (dx) {
+    plan.side(w, C, 2 * F);
+    plan.side(dr, M, 2 * F, 128);
+  }
   ProfScope prof("mlp", 12.0 * a.rows * a.cols * a.hidden, 8.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
-  if (!clear(bits(top), end - top)) return false;
+  if (!plan.lay()) return false;
   Jobs t{};
-  auto add = [&](const Job& j) -> Job& { return t.j[t.count++] = j; };
-  {
-    Job& j = add(job(dy, a.rows, a.out, a.out));
-    j.rowMax = bits(yrMax);
-    j.colMax = dwd ? bits(ycMax) : nullptr;
-    add(job(a.wd, a.hidden, a.out, a.out)).rowMax = bits(dMax);
-    if (weights) add(job(a.x, a.rows, a.cols, a.cols)).colMax = bits(xMax);
-    if (dx)
-      for (int w = 0; w < 2; ++w) add(job(w ? a.wu : a.wg, a.cols, a.hidden, a.hidden, w)).rowMax = bits(wMax);
+  add(t, dy, a.rows, a.out, yr, yc);
+  add(t, a.wd, a.hidden, a.out, d, {});
+  if (dwg || dwu) add(t, a.x, a.rows, a.cols, {}, xc);
+  if (dx) {
+    add(t, a.wg, a.cols, a.hidden, w, {}, 0);
+    add(t, a.wu, a.cols, a.hidden, w, {}, F);
   }
-  if (!run_max(t)) return false;
-  for (uint32_t i = 0; i < t.count; ++i) {
-    Job& j = t.j[i];
-    auto straight = [&](size_t p, uint32_t rows, uint32_t pitch) {
-      j.straight = ws + p;
-      j.sRows = rows;
-      j.sPitch = pitch;
-    };
-    auto across = [&](size_t p, uint32_t rows, uint32_t pitch) {
-      j.across = ws + p;
-      j.aRows = rows;
-      j.aPitch = pitch;
-    };
-    if (j.src == dy) {
-      straight(pyr, M, O);
-      if (dwd) across(pyc, O, M);
-    } else if (j.turn >= 0) {
-      straight(pw, C, 2 * F);
-    } else if (j.rowMax == bits(dMax)) {
-      straight(pd, F, O);
-    } else {
-      across(pxc, C, M);
-    }
-  }
-  if (!run_split(t)) return false;
-  Prod g{};
-  g.p = ws + pyr;
-  g.q = ws + pd;
-  g.pMax = bits(yrMax);
-  g.qMax = bits(dMax);
-  g.tm = M / kTile;
-  g.tn = F / kTile;
+  if (!run_jobs(t)) return false;
+  Prods<1> t1{};
+  t1.count = 1;
+  Prod& g = t1.a[0];
+  g.p = yr;
+  g.q = d;
   g.depth = O;
   g.rows = a.rows;
-  g.out = ws + pg;
-  g.out2 = ws + pm;
-  g.pitch = 2 * F;
   g.hidden = a.hidden;
   g.g = a.saved;
   g.u = a.saved + size_t(a.rows) * a.hidden;
-  g.rowMax = bits(grMax);
-  g.colMax = bits(gcMax);
-  g.colMax2 = bits(mMax);
-  if (!run_product<GRAD>(g, a.act)) return false;
-  t.count = 0;
-  if (dx || weights) {
-    Job& j = add(job(ws + pg, M, 2 * F, 2 * F));
-    j.rowMax = bits(grMax);
-    j.colMax = bits(gcMax);
-    if (dx) {
-      j.straight = ws + pg;
-      j.sRows = M;
-      j.sPitch = 2 * F;
-    }
-    if (weights) {
-      j.across = ws + pgc;
-      j.aRows = 2 * F;
-      j.aPitch = M;
-    }
-  }
-  if (dwd) {
-    Job& j = add(job(ws + pm, M, F, F));
-    j.colMax = bits(mMax);
-    j.across = ws + pmc;
-    j.aRows = F;
-    j.aPitch = M;
-  }
-  if (!run_split(t)) return false;
-  auto product = [&](size_t p, const uint32_t* pMax, uint32_t rows, uint32_t tm, size_t q, const uint32_t* qMax, uint32_t cols,
-                     uint32_t tn, uint32_t depth, float* out, float* out2, bool turn) {
-    Prod r{};
-    r.p = ws + p;
-    r.q = ws + q;
-    r.pMax = pMax;
-    r.qMax = qMax;
-    r.tm = tm;
-    r.tn = tn;
-    r.depth = depth;
-    r.rows = rows;
-    r.cols = cols;
-    r.out = out;
-    r.out2 = out2;
-    r.pitch = cols;
-    r.turn = turn;
-    return run_product<STORE>(r);
-  };
-  if (dwd && !product(pmc, bits(mMax), a.hidden, F / kTile, pyc, bits(ycMax), a.out, O / kTile, M, dwd, nullptr, false)) return false;
-  if (weights && !product(pxc, bits(xMax), a.cols, C / kTile, pgc, bits(gcMax), a.hidden, 2 * F / kTile, M, dwg, dwu, true)) return false;
-  return !dx || product(pg, bits(grMax), a.rows, M / kTile, pw, bits(wMax), a.cols, C / kTile, 2 * F, dx, nullptr, false);
+  g.dr = dr;
+  g.dgc = dgc;
+  g.duc = duc;
+  g.mc = mc;
+  if (!run_products<GRAD>(t1, a.act)) return false;
+  // All that follow in one launch, the deepest first: a last round of few workgroups instead of four.
+  Prods<4> t2{};
+  if (dx && 2 * F >= M) add(t2, dr, w, false, 128, a.rows, a.cols, dx);
+  if (dwd) add(t2, mc, yc, false, 128, a.hidden, a.out, dwd);
+  if (dwg) add(t2, xc, dgc, true, 128, a.cols, a.hidden, dwg);
+  if (dwu) add(t2, xc, duc, true, 128, a.cols, a.hidden, dwu);
+  if (dx && 2 * F < M) add(t2, dr, w, false, 128, a.rows, a.cols, dx);
+  return run_products<STORE>(t2);
 }
 
 bool mlp_on_parts(const MlpArgs& a) {
   // a tile's rows are reached with 32-bit offsets
-  return std::max({a.rows, a.cols, a.hidden, a.out}) <= (1u << 21) && double(a.rows) * a.cols * a.hidden >= 1e8;
+  return std::max({a.rows, a.cols, a.hidden, a.out}) <= (1u << 21) && std::min({a.rows, a.cols, a.hidden, a.out}) >= 32 &&
+         double(a.rows) * a.cols * a.hidden >= 1e8;
 }
 
 }  // namespace dce
