@@ -1620,8 +1620,8 @@ static bool mlp_args(const char* what, void* x, void* wGate, void* wUp, void* wD
     return false;
   }
   const uint64_t most = std::max({uint64_t(rows) * std::max({cols, hidden, outCols}), uint64_t(hidden) * std::max(cols, outCols)});
-  if (!rows || !cols || !hidden || !outCols || most >= kOob) {
-    set_error("%s: %u rows, %u -> %u -> %u (no zeros, fewer than 2^29 values in a matrix)", what, rows, cols, hidden, outCols);
+  if (!rows || !cols || !hidden || !outCols || most >= kOob || std::max({rows, cols, hidden, outCols}) > (1u << 24)) {
+    set_error("%s: %u rows, %u -> %u -> %u (1 to 2^24, fewer than 2^29 values in a matrix)", what, rows, cols, hidden, outCols);
     return false;
   }
   a->rows = rows;

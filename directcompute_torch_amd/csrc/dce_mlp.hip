@@ -12,82 +12,382 @@ namespace dce {
 
 namespace {
 
-constexpr int kT = 256;
+using f16v = float __attribute__((ext_vector_type(16)));
 inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b); }
 
-// m = act(g) u, n values.
-template <MlpAct ACT>
-__global__ void __launch_bounds__(kT) k_mlp_gate(const float* g, const float* u, float* m, uint32_t n) {
-  for (uint32_t i = blockIdx.x * kT + threadIdx.x; i < n; i += gridDim.x * kT) m[i] = act<ACT>(g[i]) * u[i];
-}
-// dg, du and m from dm; dg may be dm.
-template <MlpAct ACT>
-__global__ void __launch_bounds__(kT)
-    k_mlp_gate_grad(const float* dm, const float* g, const float* u, float* dg, float* du, float* m, uint32_t n) {
-  for (uint32_t i = blockIdx.x * kT + threadIdx.x; i < n; i += gridDim.x * kT) {
-    float d;
-    const float a = act_grad<ACT>(g[i], d), t = dm[i], v = u[i];
-    dg[i] = t * v * d;
-    du[i] = t * a;
-    m[i] = a * v;
-  }
-}
-__global__ void __launch_bounds__(kT) k_mlp_add(const float* a, float* to, uint32_t n) {
-  for (uint32_t i = blockIdx.x * kT + threadIdx.x; i < n; i += gridDim.x * kT) to[i] += a[i];
-}
-
-// A buffer that goes back to the pool with the scope: calls on the stream that
-// follow may take it over, in order.
-struct Temp {
-  void* h;
-  explicit Temp(size_t floats) : h(create_buffer(nullptr, uint32_t(floats))) {}
-  ~Temp() { release_buffer(h); }
-  Temp(const Temp&) = delete;
-  Temp& operator=(const Temp&) = delete;
-  float* ptr() const { return h ? static_cast<Buffer*>(h)->ptr : nullptr; }
+// ---------------------------------------------------------------------------
+// Products of small calls on fp32 MFMAs, C[r][c] = sum over k of A(r, k) B(c, k), in
+// tiles of 32 x 32 for each workgroup, whose waves share the depth and add up their sums
+// in LDS, in order.  No stage in between: an operand whose depth is contiguous comes by
+// 16 bytes a lane, 4 k of its row, the other one by a dword of each k, 32 neighbours
+// together.  The MFMA's two k of a step are then 4 apart, for both.  Rows and columns
+// outside are the last ones again; what comes of them is not stored.
+// ---------------------------------------------------------------------------
+enum Op { STORE, GATE, GRAD };
+struct Side {
+  const float* p;
+  uint32_t n, pitch;  // rows or columns of the result; from one row (contiguous: of the depth) to the next
+};
+struct Prod {
+  Side a, b, b2;   // b2: GATE: Wu; STORE: of the second part
+  const float* a2; // STORE: a second part of the depth, as long as the first (null: none)
+  uint32_t depth, start, across;  // first workgroup; tiles across the columns
+  uint32_t aDeep, bDeep;  // is the depth contiguous
+  float *out, *g, *u, *du, *m;
+};
+struct Prods {
+  Prod p[4];
+  uint32_t count;
 };
 
-inline dim3 grid_of(uint32_t n) { return dim3(std::min(cdiv(n, kT), uint32_t(num_cus()) * 32)); }
-
-bool forward_plain(const MlpArgs& a) {
-  const uint32_t n = a.rows * a.hidden;
-  const Temp m(n), gu(a.saved ? 1 : 2 * size_t(n));
-  float* g = a.saved ? a.saved : gu.ptr();
-  if (!m.h || !gu.h) return false;
-  if (!gemm(a.x, a.wg, g, a.rows, a.cols, a.hidden, 0) || !gemm(a.x, a.wu, g + n, a.rows, a.cols, a.hidden, 0)) return false;
-  by_act(a.act, [&](auto k) {
-    hipLaunchKernelGGL(k_mlp_gate<decltype(k)::value>, grid_of(n), dim3(kT), 0, stream(), g, g + n, m.ptr(), n);
-  });
-  return check_launch("GatedMlpForward") && gemm(m.ptr(), a.wd, a.y, a.rows, a.hidden, a.out, 0);
+// Octet o of the depth, k = 8 o + 4 half + i; WHOLE: all of it is there, else zeros past the
+// depth.  `off`: bytes of the lane's row (or column) and its half.
+template <bool DEEP, bool WHOLE>
+__device__ __forceinline__ void octet(const float* p, uint32_t pitch, uint32_t off, uint32_t o, uint32_t depth, int half, float (&v)[4]) {
+  if constexpr (WHOLE && DEEP) {
+    const f4u q = ldus<false, f4u>(reinterpret_cast<const char*>(p + 8 * o) + off);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = q[i];
+  } else if constexpr (WHOLE) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(p + size_t(8 * o + i) * pitch) + off);
+  } else {
+    const float* row = reinterpret_cast<const float*>(reinterpret_cast<const char*>(p) + off) - (DEEP ? 4 * half : size_t(4 * half) * pitch);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t k = 8 * o + 4 * half + i;
+      const float x = row[size_t(min(k, depth - 1)) * (DEEP ? 1 : pitch)];
+      v[i] = k < depth ? x : 0.f;
+    }
+  }
 }
 
-bool backward_plain(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
-  const uint32_t n = a.rows * a.hidden;
-  const Temp dg(n), du(n), m(n), part(dx ? size_t(a.rows) * a.cols : 1);
-  if (!dg.h || !du.h || !m.h || !part.h) return false;
-  if (!gemm(dy, a.wd, dg.ptr(), a.rows, a.out, a.hidden, 2)) return false;
-  by_act(a.act, [&](auto k) {
-    hipLaunchKernelGGL(k_mlp_gate_grad<decltype(k)::value>, grid_of(n), dim3(kT), 0, stream(), dg.ptr(), a.saved,
-                       a.saved + n, dg.ptr(), du.ptr(), m.ptr(), n);
+constexpr int kWaves = 8;
+template <Op OP, MlpAct ACT>
+__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4, 4))) k_mlp_small(const Prods all) {
+  constexpr int NW = kWaves;
+  constexpr bool DUAL = OP == GATE;
+  __shared__ float S[NW][32 * 32];
+  uint32_t id = blockIdx.x;
+  int which = 0;
+  while (which + 1 < int(all.count) && all.p[which + 1].start <= id) ++which;
+  const Prod& P = all.p[which];
+  id -= P.start;
+  const uint32_t r0 = id / P.across * 32, c0 = id % P.across * 32;
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  f16v acc[DUAL ? 2 : 1];
+#pragma unroll
+  for (int d = 0; d < (DUAL ? 2 : 1); ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+  const uint32_t ar = min(r0 + col, P.a.n - 1), bc = min(c0 + col, P.b.n - 1);
+  const uint32_t octets = P.depth / 8, lo = octets * w / NW, hi = octets * (w + 1) / NW;
+  const bool tail = P.depth % 8 && w == NW - 1;
+  auto run = [&](auto aDeep, auto bDeep, const float* a, const float* b, const float* b2) {
+    constexpr bool AD = decltype(aDeep)::value, BD = decltype(bDeep)::value;
+    const uint32_t ao = (AD ? ar * P.a.pitch + 4 * half : 4 * half * P.a.pitch + ar) * 4;
+    const uint32_t bo = (BD ? bc * P.b.pitch + 4 * half : 4 * half * P.b.pitch + bc) * 4;
+    constexpr int U = 4;  // octets in flight
+    float x[U][4], y[U][4], z[DUAL ? U : 1][4];
+    auto mul = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j][i], y[j][i], acc[0], 0, 0, 0);
+        if constexpr (DUAL) acc[DUAL ? 1 : 0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j][i], z[DUAL ? j : 0][i], acc[DUAL ? 1 : 0], 0, 0, 0);
+      }
+    };
+    uint32_t o = lo;
+    for (; o + U <= hi; o += U) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        octet<AD, true>(a, P.a.pitch, ao, o + j, P.depth, half, x[j]);
+        octet<BD, true>(b, P.b.pitch, bo, o + j, P.depth, half, y[j]);
+        if constexpr (DUAL) octet<BD, true>(b2, P.b.pitch, bo, o + j, P.depth, half, z[DUAL ? j : 0]);
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) mul(j);
+    }
+    for (; o < hi; ++o) {
+      octet<AD, true>(a, P.a.pitch, ao, o, P.depth, half, x[0]);
+      octet<BD, true>(b, P.b.pitch, bo, o, P.depth, half, y[0]);
+      if constexpr (DUAL) octet<BD, true>(b2, P.b.pitch, bo, o, P.depth, half, z[0]);
+      mul(0);
+    }
+    if (tail) {
+      octet<AD, false>(a, P.a.pitch, ao, octets, P.depth, half, x[0]);
+      octet<BD, false>(b, P.b.pitch, bo, octets, P.depth, half, y[0]);
+      if constexpr (DUAL) octet<BD, false>(b2, P.b.pitch, bo, octets, P.depth, half, z[0]);
+      mul(0);
+    }
+  };
+  auto pass = [&](const float* a, const float* b, const float* b2) {
+    if (!P.aDeep)
+      run(std::false_type{}, std::false_type{}, a, b, b2);
+    else if (P.bDeep)
+      run(std::true_type{}, std::true_type{}, a, b, b2);
+    else
+      run(std::true_type{}, std::false_type{}, a, b, b2);
+  };
+  pass(P.a.p, P.b.p, P.b2.p);
+  if (OP == STORE && P.a2) pass(P.a2, P.b2.p, nullptr);
+  // The waves' sums: thread t takes every NW * 64-th value of the tile.
+  constexpr int EACH = 1024 / (NW * 64);
+  float v[DUAL ? 2 : 1][EACH];
+#pragma unroll
+  for (int d = 0; d < (DUAL ? 2 : 1); ++d) {
+    if (d) __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) S[w][(8 * (e >> 2) + 4 * half + (e & 3)) * 32 + col] = acc[d][e];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      v[d][i] = 0.f;
+#pragma unroll
+      for (int n = 0; n < NW; ++n) v[d][i] += S[n][threadIdx.x + i * NW * 64];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const uint32_t t = threadIdx.x + i * NW * 64, r = r0 + t / 32, c = c0 + t % 32;
+    if (r >= P.a.n || c >= P.b.n) continue;
+    const size_t at = size_t(r) * P.b.n + c;
+    if constexpr (OP == STORE) P.out[at] = v[0][i];
+    if constexpr (OP == GATE) {
+      P.out[at] = act<ACT>(v[0][i]) * v[DUAL ? 1 : 0][i];
+      if (P.g) {
+        P.g[at] = v[0][i];
+        P.u[at] = v[DUAL ? 1 : 0][i];
+      }
+    }
+    if constexpr (OP == GRAD) {
+      float d;
+      const float y = act_grad<ACT>(P.g[at], d), u = P.u[at];
+      P.out[at] = v[0][i] * u * d;
+      P.du[at] = v[0][i] * y;
+      P.m[at] = y * u;
+    }
+  }
+}
+
+template <Op OP>
+bool run_small(Prods& t, MlpAct act = kSilu) {
+  uint32_t n = 0;
+  for (uint32_t i = 0; i < t.count; ++i) {
+    Prod& p = t.p[i];
+    p.start = n;
+    p.across = cdiv(p.b.n, 32);
+    n += cdiv(p.a.n, 32) * p.across;
+  }
+  by_act(act, [&](auto k) {
+    constexpr MlpAct A = OP == STORE ? kSilu : decltype(k)::value;
+    hipLaunchKernelGGL((k_mlp_small<OP, A>), dim3(n), dim3(kWaves * 64), 0, stream(), t);
   });
-  if (!check_launch("GatedMlpBackward")) return false;
-  if (dwd && !gemm(m.ptr(), dy, dwd, a.hidden, a.rows, a.out, 1)) return false;
-  if (dwg && !gemm(a.x, dg.ptr(), dwg, a.cols, a.rows, a.hidden, 1)) return false;
-  if (dwu && !gemm(a.x, du.ptr(), dwu, a.cols, a.rows, a.hidden, 1)) return false;
-  if (!dx) return true;
-  const uint32_t nx = a.rows * a.cols;
-  if (!gemm(dg.ptr(), a.wg, dx, a.rows, a.hidden, a.cols, 2) || !gemm(du.ptr(), a.wu, part.ptr(), a.rows, a.hidden, a.cols, 2))
-    return false;
-  hipLaunchKernelGGL(k_mlp_add, grid_of(nx), dim3(kT), 0, stream(), part.ptr(), dx, nx);
-  return check_launch("GatedMlpBackward");
+  return check_launch("gated_mlp");
+}
+Prod& add(Prods& t, const float* a, uint32_t rows, uint32_t aPitch, bool aDeep, const float* b, uint32_t cols, uint32_t bPitch, bool bDeep,
+          uint32_t depth, float* out) {
+  Prod& p = t.p[t.count++];
+  p.a = {a, rows, aPitch};
+  p.b = {b, cols, bPitch};
+  p.depth = depth;
+  p.aDeep = aDeep;
+  p.bDeep = bDeep;
+  p.out = out;
+  return p;
+}
+
+bool forward_small(const MlpArgs& a) {
+  const size_t n = size_t(a.rows) * a.hidden;
+  float* m = workspace(n);
+  if (!m) return false;
+  ProfScope prof("mlp", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
+  Prods t{};
+  Prod& p = add(t, a.x, a.rows, a.cols, true, a.wg, a.hidden, a.hidden, false, a.cols, m);
+  p.b2.p = a.wu;
+  p.g = a.saved;
+  p.u = a.saved ? a.saved + n : nullptr;
+  if (!run_small<GATE>(t, a.act)) return false;
+  Prods y{};
+  add(y, m, a.rows, a.hidden, true, a.wd, a.out, a.out, false, a.hidden, a.y);
+  return run_small<STORE>(y);
+}
+
+bool backward_small(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
+  const size_t n = size_t(a.rows) * a.hidden, at = (n + 63) & ~size_t(63);
+  float* dg = workspace(3 * at);
+  if (!dg) return false;
+  float *du = dg + at, *m = du + at;
+  ProfScope prof("mlp", 12.0 * a.rows * a.cols * a.hidden, 8.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
+  Prods t{};
+  Prod& p = add(t, dy, a.rows, a.out, true, a.wd, a.hidden, a.out, true, a.out, dg);
+  p.g = a.saved;
+  p.u = a.saved + n;
+  p.du = du;
+  p.m = m;
+  if (!run_small<GRAD>(t, a.act)) return false;
+  Prods r{};
+  if (dx) {
+    Prod& q = add(r, dg, a.rows, a.hidden, true, a.wg, a.cols, a.hidden, true, a.hidden, dx);
+    q.a2 = du;
+    q.b2.p = a.wu;
+  }
+  if (dwd) add(r, m, a.hidden, a.hidden, false, dy, a.out, a.out, false, a.rows, dwd);
+  if (dwg) add(r, a.x, a.cols, a.cols, false, dg, a.hidden, a.hidden, false, a.rows, dwg);
+  if (dwu) add(r, a.x, a.cols, a.cols, false, du, a.hidden, a.hidden, false, a.rows, dwu);
+  return run_small<STORE>(r);
+}
+
+// ---------------------------------------------------------------------------
+// Up to 16 rows (new tokens): the weights are read once, on vector units.  A lane has one
+// column (of each of Wg, Wu) and sums for all rows; a workgroup has 64 columns and 128 k,
+// 16 for each of its 8 waves, all of whose loads are in flight at once.  Sums of the
+// depth's shares are left in memory and added up, in order, by what reads them: those of g
+// and u by the second product's workgroups, each for the 128 of its share, those of y by
+// a pass of its own.
+// ---------------------------------------------------------------------------
+constexpr int kFew = 16, kFewWaves = 8, kFewDepth = 16 * kFewWaves;
+struct Few {
+  const float *x, *w, *w2;  // w2: Wu, or null
+  float* part;              // [shares][1 or 2][rows][cols]
+  uint32_t rows, depth, cols, blocks;
+  // second product: x from g's and u's sums of `shares` shares
+  const float* gu;
+  uint32_t shares;
+  float *g, *u;  // kept (or null)
+};
+template <int R, bool FIRST, MlpAct ACT>
+__global__ void __launch_bounds__(kFewWaves * 64) k_mlp_few(const Few a) {
+  constexpr int T = kFewWaves * 64, D = FIRST ? 2 : 1, KW = kFewDepth / kFewWaves;
+  __shared__ __attribute__((aligned(16))) float X[R][kFewDepth];
+  __shared__ float S[kFewWaves][D * R * 64];
+  const uint32_t share = blockIdx.x / a.blocks, block = blockIdx.x - share * a.blocks;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t k0 = share * kFewDepth, c = block * 64 + lane, col = min(c, a.cols - 1);
+  float y[D][KW];
+#pragma unroll
+  for (int i = 0; i < KW; ++i) {
+    const size_t at = size_t(min(k0 + w * KW + i, a.depth - 1)) * a.cols + col;
+    y[0][i] = a.w[at];
+    if constexpr (FIRST) y[D - 1][i] = a.w2[at];
+  }
+  // The rows' values, zeros past the depth (what the weights' clamped loads meet).
+#pragma unroll
+  for (int t = threadIdx.x; t < R * kFewDepth; t += T) {
+    const uint32_t r = t / kFewDepth, k = k0 + t % kFewDepth;
+    const bool in = r < a.rows && k < a.depth;
+    const size_t at = size_t(in ? r : 0) * a.depth + min(k, a.depth - 1);
+    float v = 0.f;
+    if constexpr (FIRST) {
+      v = a.x[at];
+    } else {
+      const size_t n = size_t(a.rows) * a.depth;
+      float g = 0.f, u = 0.f;
+#pragma unroll 8
+      for (uint32_t s = 0; s < a.shares; ++s) {
+        g += a.gu[2 * s * n + at];
+        u += a.gu[(2 * s + 1) * n + at];
+      }
+      v = act<ACT>(g) * u;
+      if (a.g && block == 0 && in) {
+        a.g[at] = g;
+        a.u[at] = u;
+      }
+    }
+    X[r][t % kFewDepth] = in ? v : 0.f;
+  }
+  __syncthreads();
+  float acc[D][R];
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[d][r] = 0.f;
+#pragma unroll
+  for (int i = 0; i < KW; i += 4)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const f4 x = *reinterpret_cast<const f4*>(&X[r][w * KW + i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int d = 0; d < D; ++d) acc[d][r] = fmaf(x[e], y[d][i + e], acc[d][r]);
+    }
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+#pragma unroll
+    for (int r = 0; r < R; ++r) S[w][(d * R + r) * 64 + lane] = acc[d][r];
+  __syncthreads();
+  for (int t = threadIdx.x; t < D * R * 64; t += T) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < kFewWaves; ++i) v += S[i][t];
+    const uint32_t d = t / (R * 64), r = t / 64 % R, n = block * 64 + t % 64;
+    if (r < a.rows && n < a.cols) a.part[((size_t(share) * D + d) * a.rows + r) * a.cols + n] = v;
+  }
+}
+__global__ void __launch_bounds__(256) k_mlp_few_sum(const float* part, float* y, uint32_t n, uint32_t shares) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float v = 0.f;
+#pragma unroll 8
+  for (uint32_t s = 0; s < shares; ++s) v += part[size_t(s) * n + i];
+  y[i] = v;
+}
+
+bool forward_few(const MlpArgs& a) {
+  const uint32_t s1 = cdiv(a.cols, kFewDepth), s2 = cdiv(a.hidden, kFewDepth);
+  const size_t gu = 2 * size_t(s1) * a.rows * a.hidden, ny = size_t(s2) * a.rows * a.out;
+  float* ws = workspace(((gu + 63) & ~size_t(63)) + (s2 > 1 ? ny : 0));
+  if (!ws) return false;
+  float* part = s2 > 1 ? ws + ((gu + 63) & ~size_t(63)) : a.y;
+  ProfScope prof("mlp", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
+  Few f{}, s{};
+  f.x = a.x;
+  f.w = a.wg;
+  f.w2 = a.wu;
+  f.part = ws;
+  f.rows = a.rows;
+  f.depth = a.cols;
+  f.cols = a.hidden;
+  f.blocks = cdiv(a.hidden, 64);
+  s.w = a.wd;
+  s.part = part;
+  s.rows = a.rows;
+  s.depth = a.hidden;
+  s.cols = a.out;
+  s.blocks = cdiv(a.out, 64);
+  s.gu = ws;
+  s.shares = s1;
+  s.g = a.saved;
+  s.u = a.saved ? a.saved + size_t(a.rows) * a.hidden : nullptr;
+  auto run = [&](auto rows) {
+    constexpr int R = decltype(rows)::value;
+    hipLaunchKernelGGL((k_mlp_few<R, true, kSilu>), dim3(f.blocks * s1), dim3(kFewWaves * 64), 0, stream(), f);
+    by_act(a.act, [&](auto k) {
+      hipLaunchKernelGGL((k_mlp_few<R, false, decltype(k)::value>), dim3(s.blocks * s2), dim3(kFewWaves * 64), 0, stream(), s);
+    });
+  };
+  if (a.rows == 1)
+    run(std::integral_constant<int, 1>{});
+  else if (a.rows <= 4)
+    run(std::integral_constant<int, 4>{});
+  else if (a.rows <= 8)
+    run(std::integral_constant<int, 8>{});
+  else
+    run(std::integral_constant<int, 16>{});
+  if (s2 > 1)
+    hipLaunchKernelGGL(k_mlp_few_sum, dim3(cdiv(a.rows * a.out, 256)), dim3(256), 0, stream(), part, a.y, a.rows * a.out, s2);
+  return check_launch("GatedMlpForward");
 }
 
 }  // namespace
 
-bool mlp_forward(const MlpArgs& a) { return mlp_on_parts(a) ? mlp_forward_parts(a) : forward_plain(a); }
+bool mlp_forward(const MlpArgs& a) {
+  if (a.rows <= uint32_t(kFew)) return forward_few(a);
+  return mlp_on_parts(a) ? mlp_forward_parts(a) : forward_small(a);
+}
 
 bool mlp_backward(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
-  return mlp_on_parts(a) ? mlp_backward_parts(a, dy, dx, dwg, dwu, dwd) : backward_plain(a, dy, dx, dwg, dwu, dwd);
+  return mlp_on_parts(a) ? mlp_backward_parts(a, dy, dx, dwg, dwu, dwd) : backward_small(a, dy, dx, dwg, dwu, dwd);
 }
 
 }  // namespace dce

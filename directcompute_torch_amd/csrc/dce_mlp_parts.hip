@@ -147,32 +147,40 @@ __device__ __forceinline__ uint32_t in_turn(uint32_t c, int turn) {
 }
 // 64 rows and 256 columns for each workgroup, 16 rows for each wave.  A width that is
 // no multiple of 4 has its last quad end with the row.
-constexpr uint32_t kMaxRows = 64;
+// Several such blocks of rows for each where there are many: an atomic on one place takes
+// some 0.4 us after the other (8192 x 128: 128 blocks 53 us).
+constexpr uint32_t kMaxRows = 64, kMaxBlocks = 32;
+__host__ __device__ inline uint32_t max_rows(uint32_t rows) {
+  const uint32_t blocks = (rows + kMaxRows - 1) / kMaxRows;
+  return (blocks + kMaxBlocks - 1) / kMaxBlocks * kMaxRows;
+}
 __global__ void __launch_bounds__(kT) k_mlp_max(const Jobs t) {
   __shared__ uint32_t tops[4][kT];
   const int k = find_job(t, blockIdx.x);
   const Job J = t.j[k];
   const uint32_t id = blockIdx.x - t.start[k], wide = (J.cols + kT - 1) / kT, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const uint32_t r0 = id / wide * kMaxRows + w * 16, c0 = id % wide * kT, c = min(c0 + lane * 4, J.cols - 4);
-  f4u v[16];
+  const uint32_t high = max_rows(J.rows), first = id / wide * high, c0 = id % wide * kT, c = min(c0 + lane * 4, J.cols - 4);
+  float top[4] = {0.f, 0.f, 0.f, 0.f};
+  for (uint32_t r0 = first + w * 16; r0 < min(first + high, J.rows); r0 += kMaxRows) {
+    f4u v[16];
 #pragma unroll
-  for (uint32_t i = 0; i < 16; ++i) v[i] = ldus<false, f4u>(J.src + size_t(min(r0 + i, J.rows - 1)) * J.cols + c);
-  if (J.straight.p) {
+    for (uint32_t i = 0; i < 16; ++i) v[i] = ldus<false, f4u>(J.src + size_t(min(r0 + i, J.rows - 1)) * J.cols + c);
+    if (J.straight.p) {
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) {
-      float m = 0.f;
+      for (uint32_t i = 0; i < 16; ++i) {
+        float m = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) m = fmaxf(m, size_of(v[i][e]));
-      m = wave_reduce(m, OpMaxR());
-      if (lane == 0 && r0 + i < J.rows && m > 0.f) atomicMax(J.straight.top + r0 + i, __float_as_uint(m));
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, size_of(v[i][e]));
+        m = wave_reduce(m, OpMaxR());
+        if (lane == 0 && r0 + i < J.rows && m > 0.f) atomicMax(J.straight.top + r0 + i, __float_as_uint(m));
+      }
     }
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], size_of(v[i][e]));
   }
   if (!J.across.p) return;
-  float top[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (uint32_t i = 0; i < 16; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], size_of(v[i][e]));
 #pragma unroll
   for (int e = 0; e < 4; ++e) tops[w][lane * 4 + e] = __float_as_uint(top[e]);
   __syncthreads();
@@ -248,6 +256,8 @@ struct Prod {
   uint32_t block;          // values of a block of the scaled side (a power of two)
   uint32_t rows, cols;     // of the result
   float* out;              // STORE
+  float* part;             // splits > 1: their shares of out, one after the other
+  uint32_t splits;         // of the depth
   float *g, *u;            // GATE: kept (null: not); GRAD: read
   uint32_t hidden;         // their pitch
   uint32_t start;          // STORE: the first workgroup
@@ -287,7 +297,15 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
   const Prod& a = all.a[which];
   __shared__ __attribute__((aligned(16))) char S[4 * kStageBytes];
   // bands of 8 rows of tiles: what an XCD runs at once reads few rows of either side
-  const uint32_t id = place - a.start, band = id / (8 * a.tn), in = id - band * 8 * a.tn, high = min(8u, a.tm - band * 8);
+  uint32_t id = place - a.start, sp = 0, k0 = 0, k1 = a.depth;
+  if constexpr (OP == STORE) {
+    const uint32_t blocks = a.depth / kTile;
+    sp = id / (a.tm * a.tn);
+    id -= sp * a.tm * a.tn;
+    k0 = blocks * sp / a.splits * kTile;
+    k1 = blocks * (sp + 1) / a.splits * kTile;
+  }
+  const uint32_t band = id / (8 * a.tn), in = id - band * 8 * a.tn, high = min(8u, a.tm - band * 8);
   const uint32_t tj = in / high, ti = band * 8 + (in - tj * high);
   BRes bp, bq;
   bp.init(a.p.p + size_t(ti) * kTile * a.p.depth, kTile * a.p.depth);
@@ -312,17 +330,17 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       own[i] = exp_of(field_of(sc.top[srow + 32 * i]));
-      next[i] = sc.field[srow + 32 * i];
+      next[i] = sc.field[size_t(k0 / a.block) * sc.rows + srow + 32 * i];
     }
   }
-  load_stage(bp, a.p.depth * 4, 0, S);
-  load_stage(bq, a.q.depth * 4, 0, S + kStageBytes);
+  load_stage(bp, a.p.depth * 4, k0, S);
+  load_stage(bq, a.q.depth * 4, k0, S + kStageBytes);
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   auto loop = [&](auto side) {
   constexpr int SIDE = decltype(side)::value;  // 0: p is scaled, 1: q, -1: neither
   int s = 0;
-  for (uint32_t k = 0; k < a.depth; k += kStep, s ^= 1) {
+  for (uint32_t k = k0; k < k1; k += kStep, s ^= 1) {
     const char* St = S + s * 2 * kStageBytes;
     // Fragments first: a direct load in flight would make the compiler wait for it
     // before any LDS read.
@@ -338,7 +356,7 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
         }
     if constexpr (SCALED) {
       if ((k & (a.block - 1)) == 0) {
-        const uint32_t then = min(k + a.block, a.depth - 1) / a.block;
+        const uint32_t then = min(k + a.block, k1 - 1) / a.block;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           by[i] = down(exp_of(next[i]) - own[i]);
@@ -346,7 +364,7 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
         }
       }
     }
-    if (k + kStep < a.depth) {
+    if (k + kStep < k1) {
       char* Sn = S + (s ^ 1) * 2 * kStageBytes;
       load_stage(bp, a.p.depth * 4, k + kStep, Sn);
       load_stage(bq, a.q.depth * 4, k + kStep, Sn + kStageBytes);
@@ -399,6 +417,7 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
       for (int j = 0; j < 2; ++j) big[i][j][e] = ldexpf(big[i][j][e] + small[i][j][e], -(ep + eq[j]));
     }
   if constexpr (OP == STORE) {
+    float* out = a.splits > 1 ? a.part + size_t(sp) * a.rows * a.cols : a.out;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -407,7 +426,7 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t n = c0 + wn + 32 * j + col;
-          if (r < a.rows && n < a.cols) a.out[size_t(r) * a.cols + n] = big[i][j][e];
+          if (r < a.rows && n < a.cols) out[size_t(r) * a.cols + n] = big[i][j][e];
         }
       }
   }
@@ -481,6 +500,30 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
   }
 }
 
+// Sums of the splits' shares, in order.
+struct Sum {
+  const float* part;
+  float* out;
+  uint32_t n, splits, start;
+};
+struct Sums {
+  Sum s[4];
+  uint32_t count, blocks;
+};
+__global__ void __launch_bounds__(kT) k_mlp_sum(const Sums t) {
+  int k = 0;
+  while (k + 1 < int(t.count) && t.s[k + 1].start <= blockIdx.x) ++k;
+  const Sum s = t.s[k];
+  const uint32_t i = ((blockIdx.x - s.start) * kT + threadIdx.x) * 4;
+  if (i >= s.n) return;
+  // the last quad ends with the matrix; fewer than 4 values there are none
+  const uint32_t at = min(i, s.n - 4);
+  f4u v = ldus<false, f4u>(s.part + at);
+#pragma unroll 4
+  for (uint32_t k = 1; k < s.splits; ++k) v += ldus<false, f4u>(s.part + size_t(k) * s.n + at);
+  stus<false>(s.out + at, v);
+}
+
 // Places in the workspace.
 struct Places {
   size_t next = 0;
@@ -507,11 +550,12 @@ struct Plan {
     all[count++] = {&s, at.take(size_t(rows) * depth), tops, block ? at.take((size_t(rows) * (depth / block) + 3) / 4) : ~size_t(0)};
     tops += rows;
   }
-  // The workspace, with its maxima cleared.
-  bool lay() {
-    const size_t first = at.take(tops);
+  // The workspace, with its maxima cleared; room for `more` floats at *extra.
+  bool lay(size_t more, float** extra) {
+    const size_t first = at.take(tops), tail = at.take(more);
     float* ws = workspace(at.next);
     if (!ws) return false;
+    *extra = ws + tail;
     for (int i = 0; i < count; ++i) {
       Side& s = *all[i].s;
       s.p = ws + all[i].p;
@@ -538,7 +582,7 @@ bool run_jobs(Jobs& t) {
   uint32_t n = 0;
   for (uint32_t i = 0; i < t.count; ++i) {
     t.start[i] = n;
-    n += cdiv(t.j[i].rows, kMaxRows) * cdiv(t.j[i].cols, kT);
+    n += cdiv(t.j[i].rows, max_rows(t.j[i].rows)) * cdiv(t.j[i].cols, kT);
   }
   hipLaunchKernelGGL(k_mlp_max, dim3(n), dim3(kT), 0, stream(), t);
   if (!check_launch("gated_mlp")) return false;
@@ -550,19 +594,46 @@ bool run_jobs(Jobs& t) {
   hipLaunchKernelGGL(k_mlp_split, dim3(n), dim3(kT), 0, stream(), t);
   return check_launch("gated_mlp");
 }
+// Splits of the depths: no workgroup has more than a slot's share of the launch (two a CU),
+// or `kLeast` where that is more (1024 x 1024 x 4096, training: 631 us without splits, 426
+// with 256, 424 with 512, 446 with 2048; 1024 x 512 x 2048: 254, 183, 189, 212).  Floats of
+// their shares.
+constexpr uint32_t kLeast = 512;
+template <int N>
+size_t split(Prods<N>& t) {
+  double all = 0;
+  for (uint32_t i = 0; i < t.count; ++i) all += double(t.a[i].p.rows / kTile) * (t.a[i].q.rows / kTile) * t.a[i].depth;
+  const double most = std::max<double>(kLeast, all / (2 * num_cus()));
+  size_t floats = 0;
+  for (uint32_t i = 0; i < t.count; ++i) {
+    Prod& a = t.a[i];
+    a.splits = std::min(uint32_t(std::ceil(a.depth / most)), a.depth / kTile);
+    if (a.splits > 1) floats += (size_t(a.splits) * a.rows * a.cols + 63) & ~size_t(63);
+  }
+  return floats;
+}
 template <Op OP, int N>
-bool run_products(Prods<N>& t, MlpAct act = kSilu) {
+bool run_products(Prods<N>& t, MlpAct act = kSilu, float* part = nullptr) {
   uint32_t n = 0;
+  Sums sums{};
   for (uint32_t i = 0; i < t.count; ++i) {
     Prod& a = t.a[i];
     a.tm = a.p.rows / kTile;
     a.tn = a.q.rows / kTile;
     a.start = n;
-    n += a.tm * a.tn;
+    a.splits = std::max(a.splits, 1u);
+    n += a.tm * a.tn * a.splits;
+    if (a.splits == 1) continue;
+    a.part = part;
+    const size_t values = size_t(a.rows) * a.cols;
+    part += (size_t(a.splits) * values + 63) & ~size_t(63);
+    sums.s[sums.count++] = {a.part, a.out, uint32_t(values), a.splits, sums.blocks};
+    sums.blocks += cdiv(values, 4 * kT);
   }
   by_act(act, [&](auto k) {
     hipLaunchKernelGGL((k_mlp_product<OP, OP == STORE ? kSilu : decltype(k)::value, N>), dim3(n), dim3(kT), 0, stream(), t);
   });
+  if (sums.count) hipLaunchKernelGGL(k_mlp_sum, dim3(sums.blocks), dim3(kT), 0, stream(), sums);
   return check_launch("gated_mlp");
 }
 template <int N>
@@ -589,14 +660,19 @@ bool mlp_forward_parts(const MlpArgs& a) {
   plan.side(d, O, F);
   plan.side(m, M, F, 64);
   ProfScope prof("mlp", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
-  if (!plan.lay()) return false;
+  // The second product's sides get their places with the others.
+  Prods<1> t1{}, t2{};
+  add(t2, m, d, false, 64, a.rows, a.out, a.y);
+  float* part;
+  if (!plan.lay(split(t2), &part)) return false;
+  t2.a[0].p = m;
+  t2.a[0].q = d;
   Jobs t{};
   add(t, a.x, a.rows, a.cols, x, {});
   add(t, a.wg, a.cols, a.hidden, {}, w, 0, 0);
   add(t, a.wu, a.cols, a.hidden, {}, w, 0, 1);
   add(t, a.wd, a.hidden, a.out, {}, d);
   if (!run_jobs(t)) return false;
-  Prods<1> t1{}, t2{};
   t1.count = 1;
   Prod& g = t1.a[0];
   g.p = x;
@@ -609,8 +685,7 @@ bool mlp_forward_parts(const MlpArgs& a) {
     g.g = a.saved;
     g.u = a.saved + size_t(a.rows) * a.hidden;
   }
-  add(t2, m, d, false, 64, a.rows, a.out, a.y);
-  return run_products<GATE>(t1, a.act) && run_products<STORE>(t2);
+  return run_products<GATE>(t1, a.act) && run_products<STORE>(t2, kSilu, part);
 }
 
 bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
@@ -631,7 +706,23 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
     plan.side(dr, M, 2 * F, 128);
   }
   ProfScope prof("mlp", 12.0 * a.rows * a.cols * a.hidden, 8.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
-  if (!plan.lay()) return false;
+  // All that follow dm's in one launch, the deepest first: a last round of few workgroups
+  // instead of four.  Twice: their sizes first, their places once they have them.
+  Prods<4> t2{};
+  auto rest = [&] {
+    const Prods<4> had = t2;
+    t2 = {};
+    if (dx && 2 * F >= M) add(t2, dr, w, false, 128, a.rows, a.cols, dx);
+    if (dwd) add(t2, mc, yc, false, 128, a.hidden, a.out, dwd);
+    if (dwg) add(t2, xc, dgc, true, 128, a.cols, a.hidden, dwg);
+    if (dwu) add(t2, xc, duc, true, 128, a.cols, a.hidden, dwu);
+    if (dx && 2 * F < M) add(t2, dr, w, false, 128, a.rows, a.cols, dx);
+    for (uint32_t i = 0; i < had.count; ++i) t2.a[i].splits = had.a[i].splits;
+  };
+  rest();
+  float* part;
+  if (!plan.lay(split(t2), &part)) return false;
+  rest();
   Jobs t{};
   add(t, dy, a.rows, a.out, yr, yc);
   add(t, a.wd, a.hidden, a.out, d, {});
@@ -656,20 +747,17 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
   g.duc = duc;
   g.mc = mc;
   if (!run_products<GRAD>(t1, a.act)) return false;
-  // All that follow in one launch, the deepest first: a last round of few workgroups instead of four.
-  Prods<4> t2{};
-  if (dx && 2 * F >= M) add(t2, dr, w, false, 128, a.rows, a.cols, dx);
-  if (dwd) add(t2, mc, yc, false, 128, a.hidden, a.out, dwd);
-  if (dwg) add(t2, xc, dgc, true, 128, a.cols, a.hidden, dwg);
-  if (dwu) add(t2, xc, duc, true, 128, a.cols, a.hidden, dwu);
-  if (dx && 2 * F < M) add(t2, dr, w, false, 128, a.rows, a.cols, dx);
-  return run_products<STORE>(t2);
+  return run_products<STORE>(t2, kSilu, part);
 }
 
+// The parts of the weights are made anew at each call, which few rows do not pay for.
+// Forward and training us on fp32 / on parts: 256 x 1024 x 2816 70 and 212 / 78 and 210, 512 x
+// 512 x 2048 52 and 160 / 60 and 185, 2048 x 256 x 1024 56 and 167 / 54 and 141, 8192 x 128 x
+// 512 74 and 205 / 62 and 182, 200 x 2048 x 8192 323 and 1029 / 235 and 894.
 bool mlp_on_parts(const MlpArgs& a) {
   // a tile's rows are reached with 32-bit offsets
-  return std::max({a.rows, a.cols, a.hidden, a.out}) <= (1u << 21) && std::min({a.rows, a.cols, a.hidden, a.out}) >= 32 &&
-         double(a.rows) * a.cols * a.hidden >= 1e8;
+  if (std::max({a.rows, a.cols, a.hidden, a.out}) > (1u << 21) || std::min({a.rows, a.cols, a.hidden, a.out}) < 32) return false;
+  return (double(a.rows) - 100) * std::sqrt(double(a.cols) * a.out) * a.hidden >= 4.5e8;
 }
 
 }  // namespace dce

@@ -299,8 +299,8 @@ void ResidualNormBackward(void* gradH, void* gradNormed, void* h, void* block, v
                           void** pDPost, void** pDPre);
 
 /* Gated feed-forward block: y = (act(x Wg) * (x Wu)) Wd.  x is rows x cols, Wg
- * and Wu cols x hidden, Wd hidden x outCols, y rows x outCols; fewer than 2^29
- * values in each, and in rows x hidden.  act: 0 silu, 1 gelu (by erf), 2 relu, 3
+ * and Wu cols x hidden, Wd hidden x outCols, y rows x outCols; sizes up to 2^24,
+ * fewer than 2^29 values in each matrix and in rows x hidden.  act: 0 silu, 1 gelu (by erf), 2 relu, 3
  * sigmoid.  pSaved, when not NULL, receives x Wg and x Wu (2 * rows * hidden
  * floats) for the backward, which gives each gradient only when its pointer is
  * not NULL. */
