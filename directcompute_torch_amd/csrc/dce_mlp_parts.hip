@@ -69,18 +69,20 @@ struct Side {
 };
 
 // A tile of 128 rows of COLS values in LDS, its octets of columns XORed by the octet of
-// rows, so that neither a row's octets nor a column's meet in a bank often.
+// rows, so that neither a row's octets nor a column's meet in a bank often.  Rows of 128
+// are in two arrays of 64 rows (a product's two stages), those of 64 in the first.
 template <int COLS>
-__device__ __forceinline__ int tile_at(int r, int c) {
-  return r * COLS + ((((c >> 3) ^ (r >> 3)) & (COLS / 8 - 1)) << 3) + (c & 7);
+__device__ __forceinline__ float* tile_at(float* S0, float* S1, int r, int c) {
+  float* S = COLS == 64 || r < 64 ? S0 : S1;
+  return S + (COLS == 64 ? r : r & 63) * COLS + ((((c >> 3) ^ (r >> 3)) & (COLS / 8 - 1)) << 3) + (c & 7);
 }
 // Parts of its rows, with the exponents that they have in this tile, at row r0 and value c0 of t.
 template <int COLS>
-__device__ __forceinline__ void put_rows(const float* S, const Side& t, uint32_t r0, uint32_t c0) {
+__device__ __forceinline__ void put_rows(float* S0, float* S1, const Side& t, uint32_t r0, uint32_t c0) {
   constexpr int OCT = COLS / 8;
   for (int u = threadIdx.x; u < 128 * OCT; u += kT) {
     const int r = u / OCT, o = u % OCT;
-    const f4* p = reinterpret_cast<const f4*>(S + tile_at<COLS>(r, 8 * o));
+    const f4* p = reinterpret_cast<const f4*>(tile_at<COLS>(S0, S1, r, 8 * o));
     const f4 a = p[0], b = p[1];
     const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     float m = 0.f;
@@ -97,10 +99,10 @@ __device__ __forceinline__ void put_rows(const float* S, const Side& t, uint32_t
   }
 }
 // Parts of a 128 x 128 tile's columns, likewise, at row c0 and value r0 of t.
-__device__ __forceinline__ void put_columns(const float* S, const Side& t, uint32_t r0, uint32_t c0) {
+__device__ __forceinline__ void put_columns(float* S0, float* S1, const Side& t, uint32_t r0, uint32_t c0) {
   for (int u = threadIdx.x; u < 128 * 16; u += kT) {
     const int c = u / 16, o = u % 16;
-    const float* p = S + tile_at<128>(8 * o, c);
+    const float* p = tile_at<128>(S0, S1, 8 * o, c);
     float v[8], m = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -147,11 +149,11 @@ __device__ __forceinline__ uint32_t in_turn(uint32_t c, int turn) {
 }
 // 64 rows and 256 columns for each workgroup, 16 rows for each wave.  A width that is
 // no multiple of 4 has its last quad end with the row.
-// Several such blocks of rows for each where there are many: an atomic on one place takes
-// some 0.4 us after the other (8192 x 128: 128 blocks 53 us).
-constexpr uint32_t kMaxRows = 64, kMaxBlocks = 32;
-__host__ __device__ inline uint32_t max_rows(uint32_t rows) {
-  const uint32_t blocks = (rows + kMaxRows - 1) / kMaxRows;
+// Several such blocks of rows for each where columns are wanted over many: an atomic on one
+// place takes some 0.4 us after the other (8192 x 128: 128 blocks 53 us).
+constexpr uint32_t kMaxRows = 64, kMaxBlocks = 64;
+__host__ __device__ inline uint32_t max_rows(const Job& j) {
+  const uint32_t blocks = j.across.p ? (j.rows + kMaxRows - 1) / kMaxRows : 1;
   return (blocks + kMaxBlocks - 1) / kMaxBlocks * kMaxRows;
 }
 __global__ void __launch_bounds__(kT) k_mlp_max(const Jobs t) {
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(kT) k_mlp_max(const Jobs t) {
   const int k = find_job(t, blockIdx.x);
   const Job J = t.j[k];
   const uint32_t id = blockIdx.x - t.start[k], wide = (J.cols + kT - 1) / kT, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const uint32_t high = max_rows(J.rows), first = id / wide * high, c0 = id % wide * kT, c = min(c0 + lane * 4, J.cols - 4);
+  const uint32_t high = max_rows(J), first = id / wide * high, c0 = id % wide * kT, c = min(c0 + lane * 4, J.cols - 4);
   float top[4] = {0.f, 0.f, 0.f, 0.f};
   for (uint32_t r0 = first + w * 16; r0 < min(first + high, J.rows); r0 += kMaxRows) {
     f4u v[16];
@@ -192,7 +194,8 @@ __global__ void __launch_bounds__(kT) k_mlp_max(const Jobs t) {
 
 // A 128 x 128 tile through LDS.
 __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
-  __shared__ __attribute__((aligned(16))) float S[128 * 128];
+  __shared__ __attribute__((aligned(16))) float S0[64 * 128];
+  __shared__ __attribute__((aligned(16))) float S1[64 * 128];
   const int k = find_job(t, blockIdx.x);
   const Job J = t.j[k];
   const uint32_t tc = (J.cols + 127) / 128, id = blockIdx.x - t.start[k], i0 = id / tc * 128, j0 = id % tc * 128;
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
       if (off == 2) x = f4{x[2], x[3], 0.f, 0.f};
       if (off == 3) x = f4{x[3], 0.f, 0.f, 0.f};
       if (off == 4 || i0 + r >= J.rows) x = f4{0.f, 0.f, 0.f, 0.f};
-      *reinterpret_cast<f4*>(S + tile_at<128>(r, q * 4)) = x;
+      *reinterpret_cast<f4*>(tile_at<128>(S0, S1, r, q * 4)) = x;
     }
   }
   __syncthreads();
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
       const uint32_t r = i0 + rl;
       float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = S[tile_at<128>(rl, cl) + e];
+      for (int e = 0; e < 8; ++e) v[e] = tile_at<128>(S0, S1, rl, cl)[e];
       if (r < J.straight.rows && j0 + cl < J.straight.depth)
         put8(J.straight.p + size_t(r) * J.straight.depth, J.c0 + j0 + cl, v, pow2(exp_of(field_of(J.straight.top[r]))));
     }
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
       const uint32_t c = in_turn(j0 + cl, J.turn), r = i0 + rl;
       float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = S[tile_at<128>(rl, cl) + 128 * e];
+      for (int e = 0; e < 8; ++e) v[e] = tile_at<128>(S0, S1, rl, cl)[128 * e];
       if (c < J.across.rows && r < J.across.depth)
         put8(J.across.p + size_t(c) * J.across.depth, r, v, pow2(exp_of(field_of(J.across.top[c]))));
     }
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
 // ---------------------------------------------------------------------------
 // Products C = P Q^T of parts, both along their rows, in 128 x 128 tiles of four
 // waves, 64 x 64 each (2 x 2 blocks of 32 x 32).  The depth goes in steps of 32 through
-// two LDS stages, the next one's direct loads in flight while one is multiplied.  A
+// two LDS stages, the next one's direct loads in flight while one is read and multiplied.  A
 // stage's rows are eight 16-byte slots, four of h and four of l, XORed by the row
 // so that a read of one slot of 16 rows covers the 64 banks once.  The two small
 // products have an accumulator of their own: an MFMA cuts what it adds off at the
@@ -295,7 +298,10 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
   if constexpr (N > 1)
     while (which + 1 < int(all.count) && all.a[which + 1].start <= place) ++which;
   const Prod& a = all.a[which];
-  __shared__ __attribute__((aligned(16))) char S[4 * kStageBytes];
+  // An array for each stage: the compiler then knows that a direct load into one is
+  // nothing that a read of the other has to wait for.
+  __shared__ __attribute__((aligned(16))) char S0[2 * kStageBytes];
+  __shared__ __attribute__((aligned(16))) char S1[2 * kStageBytes];
   // bands of 8 rows of tiles: what an XCD runs at once reads few rows of either side
   uint32_t id = place - a.start, sp = 0, k0 = 0, k1 = a.depth;
   if constexpr (OP == STORE) {
@@ -333,68 +339,67 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
       next[i] = sc.field[size_t(k0 / a.block) * sc.rows + srow + 32 * i];
     }
   }
-  load_stage(bp, a.p.depth * 4, k0, S);
-  load_stage(bq, a.q.depth * 4, k0, S + kStageBytes);
+  load_stage(bp, a.p.depth * 4, k0, S0);
+  load_stage(bq, a.q.depth * 4, k0, S0 + kStageBytes);
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   auto loop = [&](auto side) {
-  constexpr int SIDE = decltype(side)::value;  // 0: p is scaled, 1: q, -1: neither
-  int s = 0;
-  for (uint32_t k = k0; k < k1; k += kStep, s ^= 1) {
-    const char* St = S + s * 2 * kStageBytes;
-    // Fragments first: a direct load in flight would make the compiler wait for it
-    // before any LDS read.
-    h8 p[2][2][2], q[2][2][2];
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          p[kk][i][e] = frag(St, wm + 32 * i + col, 4 * e + 2 * kk + half);
-          q[kk][i][e] = frag(St + kStageBytes, wn + 32 * i + col, 4 * e + 2 * kk + half);
-        }
-    if constexpr (SCALED) {
-      if ((k & (a.block - 1)) == 0) {
-        const uint32_t then = min(k + a.block, k1 - 1) / a.block;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          by[i] = down(exp_of(next[i]) - own[i]);
-          next[i] = sc.field[size_t(then) * sc.rows + srow + 32 * i];
-        }
+    constexpr int SIDE = decltype(side)::value;  // 0: p is scaled, 1: q, -1: neither
+    auto step = [&](uint32_t k, const char* St, char* Sn) {
+      if (k + kStep < k1) {
+        load_stage(bp, a.p.depth * 4, k + kStep, Sn);
+        load_stage(bq, a.q.depth * 4, k + kStep, Sn + kStageBytes);
       }
-    }
-    if (k + kStep < k1) {
-      char* Sn = S + (s ^ 1) * 2 * kStageBytes;
-      load_stage(bp, a.p.depth * 4, k + kStep, Sn);
-      load_stage(bq, a.q.depth * 4, k + kStep, Sn + kStageBytes);
-    }
+      h8 p[2][2][2], q[2][2][2];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      if constexpr (SCALED) {
+      for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            if constexpr (SIDE == 1)
-              q[kk][i][e] *= by[i];
-            else
-              p[kk][i][e] *= by[i];
+            p[kk][i][e] = frag(St, wm + 32 * i + col, 4 * e + 2 * kk + half);
+            q[kk][i][e] = frag(St + kStageBytes, wn + 32 * i + col, 4 * e + 2 * kk + half);
           }
+      if constexpr (SCALED) {
+        if ((k & (a.block - 1)) == 0) {
+          const uint32_t then = min(k + a.block, k1 - 1) / a.block;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            by[i] = down(exp_of(next[i]) - own[i]);
+            next[i] = sc.field[size_t(then) * sc.rows + srow + 32 * i];
+          }
+        }
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int kk = 0; kk < 2; ++kk) {
+        if constexpr (SCALED) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          big[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][0], big[i][j], 0, 0, 0);
-          small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][1], small[i][j], 0, 0, 0);
-          small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][1], q[kk][j][0], small[i][j], 0, 0, 0);
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if constexpr (SIDE == 1)
+                q[kk][i][e] *= by[i];
+              else
+                p[kk][i][e] *= by[i];
+            }
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            big[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][0], big[i][j], 0, 0, 0);
+            small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][1], small[i][j], 0, 0, 0);
+            small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][1], q[kk][j][0], small[i][j], 0, 0, 0);
+          }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    };
+    for (uint32_t k = k0; k < k1; k += 2 * kStep) {  // the depth is a multiple of 128
+      step(k, S0, S1);
+      step(k + kStep, S1, S0);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-  }
   };
   if constexpr (!SCALED)
     loop(std::integral_constant<int, -1>{});
@@ -404,7 +409,7 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
     loop(std::integral_constant<int, 0>{});
   // Row 8 (e / 4) + 4 half + e % 4 of a block, column `col`.
   const uint32_t r0 = ti * kTile, c0 = tj * kTile;
-  float* T = reinterpret_cast<float*>(S);
+  float *T0 = reinterpret_cast<float*>(S0), *T1 = reinterpret_cast<float*>(S1);
   int eq[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) eq[j] = exp_of(field_of(a.q.top[c0 + wn + 32 * j + col]));
@@ -441,10 +446,10 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
           a.g[size_t(r) * a.hidden + f] = big[i][0][e];
           a.u[size_t(r) * a.hidden + f] = big[i][1][e];
         }
-        T[tile_at<64>(wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3), (wn >> 1) + col)] = act<ACT>(big[i][0][e]) * big[i][1][e];
+        *tile_at<64>(T0, T1, wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3), (wn >> 1) + col) = act<ACT>(big[i][0][e]) * big[i][1][e];
       }
     __syncthreads();
-    put_rows<64>(T, a.m, r0, c0 / 2);
+    put_rows<64>(T0, T1, a.m, r0, c0 / 2);
   }
   if constexpr (OP == GRAD) {
     // g and u, zeros outside, where dm is zeros too (or its row has no value that counts).
@@ -473,10 +478,12 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
         for (int j = 0; j < 2; ++j) {
           float d;
           const float y = act_grad<ACT>(small[i][j][e], d), dm = big[i][j][e], v = u[i][j][e];
-          __builtin_amdgcn_sched_barrier(0);  // one at a time: no registers for more
-          big[i][j][e] = dm * v * d;
-          small[i][j][e] = dm * y;
-          u[i][j][e] = y * v;
+          float dg = dm * v * d, du = dm * y, m = y * v;
+          // Here and now: put off to where they are stored, they keep more alive than there are registers.
+          asm volatile("" : "+v"(dg), "+v"(du), "+v"(m));
+          big[i][j][e] = dg;
+          small[i][j][e] = du;
+          u[i][j][e] = m;
         }
     auto tile = [&](const f16v (&v)[2][2]) {
       __syncthreads();
@@ -485,18 +492,18 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
 #pragma unroll
         for (int e = 0; e < 16; ++e)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) T[tile_at<128>(wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3), wn + 32 * j + col)] = v[i][j][e];
+          for (int j = 0; j < 2; ++j) *tile_at<128>(T0, T1, wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3), wn + 32 * j + col) = v[i][j][e];
       __syncthreads();
     };
     tile(big);
-    if (a.dr.p) put_rows<128>(T, a.dr, r0, c0);
-    if (a.dgc.p) put_columns(T, a.dgc, r0, c0);
+    if (a.dr.p) put_rows<128>(T0, T1, a.dr, r0, c0);
+    if (a.dgc.p) put_columns(T0, T1, a.dgc, r0, c0);
     tile(small);
-    if (a.dr.p) put_rows<128>(T, a.dr, r0, a.dr.depth / 2 + c0);
-    if (a.duc.p) put_columns(T, a.duc, r0, c0);
+    if (a.dr.p) put_rows<128>(T0, T1, a.dr, r0, a.dr.depth / 2 + c0);
+    if (a.duc.p) put_columns(T0, T1, a.duc, r0, c0);
     if (!a.mc.p) return;
     tile(u);
-    put_columns(T, a.mc, r0, c0);
+    put_columns(T0, T1, a.mc, r0, c0);
   }
 }
 
@@ -582,7 +589,7 @@ bool run_jobs(Jobs& t) {
   uint32_t n = 0;
   for (uint32_t i = 0; i < t.count; ++i) {
     t.start[i] = n;
-    n += cdiv(t.j[i].rows, max_rows(t.j[i].rows)) * cdiv(t.j[i].cols, kT);
+    n += cdiv(t.j[i].rows, max_rows(t.j[i])) * cdiv(t.j[i].cols, kT);
   }
   hipLaunchKernelGGL(k_mlp_max, dim3(n), dim3(kT), 0, stream(), t);
   if (!check_launch("gated_mlp")) return false;
