@@ -223,6 +223,9 @@ struct BRes {
   __device__ __forceinline__ float ld1(uint32_t off) const {
     return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off * 4u, 0, 0));
   }
+  __device__ __forceinline__ float ld1nt(uint32_t off) const {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off * 4u, 0, 2));
+  }
   __device__ __forceinline__ f2 ld2(uint32_t off) const {
     return __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(r, off * 4u, 0, 0));
   }
