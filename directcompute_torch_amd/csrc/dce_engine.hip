@@ -1675,9 +1675,9 @@ void GatedMlpBackward(void* gradOut, void* x, void* wGate, void* wUp, void* wDow
 static bool scan_args(const char* what, void* x, void* gate, void* state, void* lengths, uint32_t batch, uint32_t seq,
                       uint32_t chans, ScanArgs* a) {
   const uint64_t n = uint64_t(batch) * seq * chans;
-  if (!batch || !seq || !chans || uint64_t(batch) * seq > 0xFFFFFFFFull || uint64_t(batch) * chans >= 0x80000000ull ||
+  if (!batch || !seq || !chans || seq >= 0x7F000000u || uint64_t(batch) * chans >= 0x80000000ull || uint64_t(batch) * seq > 0xFFFFFFFFull ||
       n > 0xFFFFFFFFull) {
-    set_error("%s: %u x %u tokens of %u channels (no zeros, fewer than 2^31 states and 2^32 values)", what, batch, seq, chans);
+    set_error("%s: %u x %u tokens of %u channels (no zeros, some 2^31 tokens or states and 2^32 values at most)", what, batch, seq, chans);
     return false;
   }
   a->B = batch;

@@ -38,6 +38,7 @@ struct Norm {
   const float *dh, *dn;
   float *dx, *db, *dgate, *dpost, *dpre;  // dgate .. dpre: partial sums of the workgroups
   uint32_t rows, cols;
+  uint32_t first;   // of this launch's rows (forward)
   uint32_t per;     // rows of a gate row
   uint32_t each;    // every row has a gate row of its own (per then counts all rows)
   uint32_t pieces;  // workgroups of a gate row's rows (backward)
@@ -104,7 +105,7 @@ template <int TPR, int NV, int W, bool NT>
 __global__ void __launch_bounds__(threads_of<TPR>) k_norm_fwd(const Norm a) {
   constexpr int T = threads_of<TPR>, RPB = T / TPR;
   __shared__ float sh[T / 64];
-  const uint32_t lane = threadIdx.x % TPR, row = blockIdx.x * RPB + threadIdx.x / TPR;
+  const uint32_t lane = threadIdx.x % TPR, row = a.first + blockIdx.x * RPB + threadIdx.x / TPR;
   if (RPB > 1 && row >= a.rows) return;
   const size_t base = size_t(row) * a.cols;
   Span<W> s[NV];
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(kColWaves * 64) k_norm_cols(const Cols a) {
 // f.run<TPR, NV, W>() for a width.
 template <class F>
 bool dispatch(uint32_t cols, const F& f) {
-  if (cols < 4) return f.template run<64, 1, 1>();
+  if (cols < 4) return f.template run<16, 1, 1>();
   if (cols <= 64) return f.template run<16, 1, 4>();
   if (cols <= 128) return f.template run<32, 1, 4>();
   if (cols <= 256) return f.template run<64, 1, 4>();
@@ -363,12 +364,17 @@ bool dispatch(uint32_t cols, const F& f) {
 }
 
 struct Fwd {
-  const Norm& a;
+  Norm& a;
   bool nt;
   template <int TPR, int NV, int W>
   bool run() const {
-    constexpr int T = threads_of<TPR>;
-    hipLaunchKernelGGL((nt ? k_norm_fwd<TPR, NV, W, true> : k_norm_fwd<TPR, NV, W, false>), dim3(cdiv(a.rows, T / TPR)), dim3(T), 0, stream(), a);
+    constexpr int T = threads_of<TPR>, RPB = T / TPR;
+    constexpr uint32_t most = 1u << 21;  // workgroups: fewer than 2^32 threads in a launch
+    for (uint64_t first = 0; first < a.rows; first += uint64_t(most) * RPB) {
+      a.first = uint32_t(first);
+      hipLaunchKernelGGL((nt ? k_norm_fwd<TPR, NV, W, true> : k_norm_fwd<TPR, NV, W, false>),
+                         dim3(std::min(cdiv(a.rows - first, RPB), most)), dim3(T), 0, stream(), a);
+    }
     return check_launch("norm");
   }
 };
@@ -452,7 +458,7 @@ Norm norm_of(const NormArgs& x) {
 }  // namespace
 
 bool norm_forward(const NormArgs& x) {
-  const Norm a = norm_of(x);
+  Norm a = norm_of(x);
   const double n = double(x.rows) * x.cols, bytes = 4 * n * (x.block ? (x.n ? 4 : 3) : 2);
   ProfScope prof("norm", 10 * n, bytes);
   return dispatch(x.cols, Fwd{a, stream_nt(bytes)});

@@ -16,7 +16,9 @@
 // longer than that, workgroups go one after the other along it.  Each reads its
 // tokens once, leaves its pair in memory, waits for the pairs of those before it,
 // and then goes through its tokens again, in registers, from the state that they
-// make.  So every value moves once: 12 bytes a value forward, 24 backward.  4 x 4096
+// make.  (Every 64th leaves its last state, too, where those after it start: no more
+// than 63 pairs are read.)  So every value moves once: 12 bytes a value forward, 24
+// backward.  4 x 4096
 // tokens of 1024 channels: forward 40 us, 5.0 TB/s, backward 80 us, 5.0 TB/s, with
 // about a third of that time's vector instructions; the pass that clears the pairs 2 to
 // 4 us each.  (A thread for each channel: 6.0 ms.)
@@ -28,9 +30,10 @@
 // forward 10.5 -> 9.9, backward 13.1 -> 11.6 us).
 //
 // Waiting: a workgroup takes its place from a counter, so those before it run
-// already, and each leaves its pair before it waits for any.  A pair is one 64-bit
-// word, whose value tells whether it is there, so no other word has to be ordered
-// with it.  The states are combined in one order, whoever came first.
+// already.  Each leaves its pair before it waits for any, and a state waits for pairs
+// and an earlier state only, so the first that lacks something gets it.  A pair, or a state,
+// is one 64-bit word, whose value tells whether it is there, so no other word has to be
+// ordered with it.  They are combined in one order, whoever came first.
 #include "dce_internal.h"
 
 #include <algorithm>
@@ -45,7 +48,8 @@ struct Scan {
   ScanArgs a;
   uint32_t per, across;     // sequences of a wave; waves across a sequence's channels
   uint32_t blocks, chunks;  // workgroups of one run of tokens; of a sequence
-  unsigned long long* pairs;  // [chunks][blocks][64]
+  unsigned long long* pairs;   // [chunks][blocks][64]
+  unsigned long long* states;  // [chunks / kGroup][blocks][64]
   uint32_t* count;
 };
 
@@ -94,6 +98,8 @@ __device__ __forceinline__ void Lane::init(const Scan& s, uint32_t block) {
   n = tokens_of(a, b0 + i);
 }
 
+constexpr uint32_t kGroup = 64;  // workgroups from one state to the next
+
 // A pair that is not there yet: all bits set, as the pass before leaves them.  (A
 // product of gates has that value only as a NaN, which is then written as another.)
 constexpr unsigned long long kAbsent = ~0ull;
@@ -112,14 +118,24 @@ __device__ __forceinline__ void then(float& A, float& H, float A2, float H2) {
   A = A2 * A;
 }
 
+// What is there at p, when it is there.
+__device__ __forceinline__ unsigned long long await(const unsigned long long* p, unsigned long long v) {
+  for (uint32_t spin = 0; v == kAbsent && spin < kSpins; ++spin) {
+    __builtin_amdgcn_s_sleep(1);
+    v = look(p);
+  }
+  return v;
+}
+
 // The state that comes into this wave's run, from `first` at the sequence's
 // start; f: the run's gates, v(j): its inputs (h <- f h + v).
 template <int NW, int L, class V>
 __device__ __forceinline__ float state_in(const Scan& s, uint32_t chunk, uint32_t block, const float (&f)[L],
                                           const V& v, float first) {
   if constexpr (NW == 1) return first;
-  __shared__ float run[2][NW][64], before[2][NW][64];
+  __shared__ float run[2][NW][64], before[2][NW][64], start[64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const size_t next = size_t(s.blocks) * 64;
   unsigned long long* mine = s.pairs + block * 64 + lane;
   float A = 1.f, H = 0.f;
 #pragma unroll
@@ -131,29 +147,32 @@ __device__ __forceinline__ float state_in(const Scan& s, uint32_t chunk, uint32_
     float a = 1.f, h = 0.f;
 #pragma unroll
     for (int i = 0; i < NW; ++i) then(a, h, run[0][i][lane], run[1][i][lane]);
-    __hip_atomic_store(mine + size_t(chunk) * s.blocks * 64, pack(a, h), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(mine + chunk * next, pack(a, h), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   float h = first;
+  const uint32_t group = chunk / kGroup, from = group * kGroup, ahead = chunk - from;
   if (chunk) {
-    // each wave a share of the workgroups before, four loads in flight
-    const uint32_t lo = chunk * w / NW, hi = chunk * (w + 1) / NW;
+    // each wave a share of the group's workgroups before, four loads in flight
+    const uint32_t lo = from + ahead * w / NW, hi = from + ahead * (w + 1) / NW;
     float a = 1.f, b = 0.f;
     for (uint32_t i = lo; i < hi; i += 4) {
       unsigned long long p[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = look(mine + size_t(min(i + e, hi - 1)) * s.blocks * 64);
+      for (int e = 0; e < 4; ++e) p[e] = look(mine + min(i + e, hi - 1) * next);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        for (uint32_t spin = 0; p[e] == kAbsent && spin < kSpins; ++spin) {
-          __builtin_amdgcn_s_sleep(1);
-          p[e] = look(mine + size_t(min(i + e, hi - 1)) * s.blocks * 64);
-        }
+        p[e] = await(mine + min(i + e, hi - 1) * next, p[e]);
         if (i + e < hi) then(a, b, __uint_as_float(uint32_t(p[e] >> 32)), __uint_as_float(uint32_t(p[e])));
       }
     }
     before[0][w][lane] = a;
     before[1][w][lane] = b;
+    if (group && w == 0) {
+      const unsigned long long* p = s.states + (group - 1) * next + block * 64 + lane;
+      start[lane] = __uint_as_float(uint32_t(await(p, look(p))));
+    }
     __syncthreads();
+    if (group) h = start[lane];
 #pragma unroll
     for (int i = 0; i < NW; ++i) h = before[0][i][lane] * h + before[1][i][lane];
   }
@@ -161,6 +180,13 @@ __device__ __forceinline__ float state_in(const Scan& s, uint32_t chunk, uint32_
   for (int i = 0; i < NW; ++i)
     if (i < w) h = run[0][i][lane] * h + run[1][i][lane];
   return h;
+}
+// The state after the last wave's run, left where the next group starts.
+template <int NW>
+__device__ __forceinline__ void state_out(const Scan& s, uint32_t chunk, uint32_t block, uint32_t w, float h) {
+  if (NW > 1 && w == NW - 1 && (chunk + 1) % kGroup == 0 && chunk + 1 < s.chunks)
+    __hip_atomic_store(s.states + size_t(chunk / kGroup) * s.blocks * 64 + block * 64 + (threadIdx.x & 63), pack(1.f, h),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // The workgroup's place: block of columns, and chunk along the sequence.
@@ -211,19 +237,17 @@ __global__ void __launch_bounds__(NW * 64) k_scan_fwd(const Scan s) {
     }
   }
   float h = state_in<NW, L>(s, chunk, block, f, [&](int j) { return v[j]; }, first);
+#pragma unroll
+  for (int j = 0; j < L; ++j) v[j] = h = f[j] * h + v[j];
+  state_out<NW>(s, chunk, block, w, h);
   if (!at.live) return;
   if (whole) {
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-      h = f[j] * h + v[j];
-      at.store<NT>(a.y, size_t(t0 + j) * a.C, h);
-    }
+    for (int j = 0; j < L; ++j) at.store<NT>(a.y, size_t(t0 + j) * a.C, v[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-      h = f[j] * h + v[j];
-      if (t0 + j < a.S) at.store<NT>(a.y, size_t(t0 + j) * a.C, t0 + j < at.n ? h : 0.f);
-    }
+    for (int j = 0; j < L; ++j)
+      if (t0 + j < a.S) at.store<NT>(a.y, size_t(t0 + j) * a.C, t0 + j < at.n ? v[j] : 0.f);
   }
   if (a.last && chunk + 1 == s.chunks && w == NW - 1) a.last[at.state] = h;
 }
@@ -268,7 +292,6 @@ __global__ void __launch_bounds__(NW * 64) k_scan_bwd(const Scan s) {
     }
   }
   float h = state_in<NW, L>(s, chunk, block, f, [&](int j) { return f[j] * dy[j]; }, 0.f);
-  if (!at.live) return;
 #pragma unroll
   for (int j = 0; j < L; ++j) {
     const float d = dy[j] + h;
@@ -276,6 +299,8 @@ __global__ void __launch_bounds__(NW * 64) k_scan_bwd(const Scan s) {
     u[j] = d * u[j] * (f[j] * k[j]);
     k[j] *= d;
   }
+  state_out<NW>(s, chunk, block, w, h);
+  if (!at.live) return;
   if (!whole) {
 #pragma unroll
     for (int j = 0; j < L; ++j) {
@@ -308,10 +333,11 @@ bool run(const ScanArgs& a, const char* what) {
   s.blocks = cdiv(a.B, s.per) * s.across;
   s.chunks = cdiv(a.S, NW * L);
   if (s.chunks > 1) {
-    const size_t words = size_t(s.chunks) * s.blocks * 64 + 1;
+    const size_t pairs = size_t(s.chunks) * s.blocks * 64, words = pairs + size_t(s.chunks / kGroup) * s.blocks * 64 + 1;
     float* ws = workspace(2 * words);
     if (!ws) return false;
     s.pairs = reinterpret_cast<unsigned long long*>(ws);
+    s.states = s.pairs + pairs;
     s.count = reinterpret_cast<uint32_t*>(s.pairs + words - 1);
     hipLaunchKernelGGL(k_scan_clear, dim3(std::min(cdiv(words, 256), 1024u)), dim3(256), 0, stream(), s.pairs, words);
   }

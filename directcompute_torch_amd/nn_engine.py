@@ -977,13 +977,15 @@ class _Keeps(Function):
 
 
 def _gain_of(what, name, gain, width):
+    if width < 1:
+        raise ValueError(f"{what}: x has no last axis")
     if gain is not None and tuple(gain.shape) != (width,):
         raise ValueError(f"{what}: {name} is ({width},), not {tuple(gain.shape)}")
 
 
 class RmsNormFunc(_Keeps):
     def forward(self, x, gain, eps):
-        width = x.shape[-1]
+        width = x.shape[-1] if x.shape else 0
         _gain_of("rms_norm", "gain", gain, width)
         self.inputs = (x, gain)
         self.dims = (x.size // width, width)
@@ -1009,12 +1011,12 @@ class ResidualNormFunc(_Keeps):
 
     def forward(self, x, block, gate, post, pre, scale, eps):
         shape = tuple(x.shape)
-        width = shape[-1]
-        rows = x.size // width
+        width = shape[-1] if shape else 0
         if tuple(block.shape) != shape:
             raise ValueError(f"residual_norm: x {shape} and the block's result {tuple(block.shape)} differ")
         _gain_of("residual_norm", "post", post, width)
         _gain_of("residual_norm", "pre", pre, width)
+        rows = x.size // width
         gate_rows = 0
         if gate is not None:
             gate_rows = gate.size // width
@@ -1124,7 +1126,8 @@ class GatedScanFunc(Function):
         res = Tensor.from_gpu(h, (B, S, C), requires_grad=any(t is not None and t.requires_grad for t in self.inputs))
         self.out_handle = h    # by handle: a reference to `res` itself would be a cycle
         res._ctx = self
-        return (res, Tensor.from_gpu(last.value, (B, C))) if return_state else res
+        # the state is the program's own, past end_batch
+        return (res, Tensor.from_gpu(last.value, (B, C), track=False)) if return_state else res
 
     def _operands(self):
         return [t.gpu_buf if t is not None else None for t in (*self.inputs, self.lengths)]
@@ -1215,7 +1218,7 @@ def gated_scan(x, gate, state=None, lengths=None, return_state=False):
     what comes before the first token; None: zeros.  lengths: a tensor of batch
     values, the tokens of each sequence that count; y is zeros past them.
     return_state: also the state after the last of them, for the next call's
-    `state`; it carries no gradient."""
+    `state`; it carries no gradient, and end_batch leaves it alone."""
     return GatedScanFunc().forward(x, gate, state, lengths, return_state)
 
 

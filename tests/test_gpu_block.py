@@ -500,6 +500,13 @@ def test_gated_scan(eng, B, S, C, with_state):
     check_scan(eng, B, S, C, with_state, None, rng(B + S + C))
 
 
+@pytest.mark.parametrize("S,C,lens", [(40000, 3, None), (33000, 64, None), (20000, 7, [20000, 16385]), (50000, 2, [8192, 49999])])
+def test_gated_scan_of_long_sequences(eng, S, C, lens):
+    """Over more than the 64 workgroups from one state to the next."""
+    print("gated_scan long", S, C, lens, flush=True)
+    check_scan(eng, 2, S, C, True, lens, rng(S))
+
+
 @pytest.mark.parametrize("S,lens", [(1, [0, 1, 1]), (9, [9, 0, 4]), (40, [1, 40, 33]), (300, [300, 17, 0]), (600, [256, 257, 600]), (1500, [1, 1024, 1030]),
                                     (30, [99, -4, float("nan")]), (700, [0, 0, 0])])
 def test_gated_scan_of_lengths(eng, S, lens):
@@ -531,6 +538,8 @@ def test_gated_scan_goes_on_from_its_state(eng):
         y, state = eng.gated_scan(dev(eng, x[:, at:at + n]), dev(eng, z[:, at:at + n]), state, return_state=True)
         got.append(y.sync().copy())
         at += n
+        del y
+        eng.end_batch()  # leaves the state alone
     within("y", np.concatenate(got, 1), *ref)
     eng.end_batch()
 
@@ -712,6 +721,28 @@ def test_runs_are_alike(eng):
     first = once()
     for _ in range(2):
         assert all(np.array_equal(p, q) for p, q in zip(first, once()))
+
+
+def test_streaming_accesses_change_nothing(eng):
+    """The kernels' nontemporal forms, taken above a size, at small sizes."""
+    r = rng(71)
+    a = [r.standard_normal(s).astype(np.float32) for s in ((2, 600, 203), (203, 2000), (203, 2000), (2000, 203), (203,))]
+
+    def once():
+        T = [dev(eng, v, True) for v in a]
+        y = eng.gated_scan(T[0], T[0])
+        h, n = eng.residual_norm(y, eng.gated_mlp(y, *T[1:4]), T[4], T[4], T[4])
+        n.backward(dev(eng, a[0]))
+        got = [n.sync().copy()] + [t.grad.sync().copy() for t in T]
+        eng.end_batch()
+        return got
+    want = once()
+    eng.lib.SetStreamingThreshold(0.0)
+    try:
+        got = once()
+    finally:
+        eng.lib.SetStreamingThreshold(-1.0)
+    assert all(np.array_equal(p, q) for p, q in zip(got, want))
 
 
 def test_layers(eng):
