@@ -119,10 +119,6 @@ __device__ __forceinline__ void put_columns(float* S0, float* S1, const Side& t,
   }
 }
 
-__global__ void __launch_bounds__(kT) k_mlp_clear(uint32_t* p, uint32_t n) {
-  for (uint32_t i = blockIdx.x * kT + threadIdx.x; i < n; i += gridDim.x * kT) p[i] = 0;
-}
-
 // ---------------------------------------------------------------------------
 // Maxima and parts of up to five matrices, [rows][cols].
 // ---------------------------------------------------------------------------
@@ -132,12 +128,20 @@ struct Job {
   Side straight, across;  // of its rows, of its columns; p null: not wanted
   uint32_t c0;            // straight: the place of its columns
   int turn;               // across: 0, 1: its columns are those of Wg, Wu in turn; -1: no
+  // Bits of the largest values of the rows in each workgroup's columns, [..][rows], and of
+  // the columns in each one's rows, [..][cols]: `rowFrom` with those of the job that shares
+  // the exponents (Wg and Wu have one for each row).
+  uint32_t *rowPart, *colPart;
+  const uint32_t* rowFrom;
+  uint32_t rowCount, colCount;
 };
 constexpr int kJobs = 5;
 struct Jobs {
   Job j[kJobs];
   uint32_t start[kJobs + 1];
   uint32_t count;
+  uint32_t* clear;  // maxima that products will raise, `clears` of them
+  uint32_t clears;
 };
 __device__ __forceinline__ int find_job(const Jobs& t, uint32_t blk) {
   int i = 0;
@@ -148,39 +152,51 @@ __device__ __forceinline__ uint32_t in_turn(uint32_t c, int turn) {
   return turn < 0 ? c : (c >> 5) * 64 + uint32_t(turn) * 32 + (c & 31);
 }
 // 64 rows and 256 columns for each workgroup, 16 rows for each wave.  A width that is
-// no multiple of 4 has its last quad end with the row.
-// Several such blocks of rows for each where columns are wanted over many: an atomic on one
-// place takes some 0.4 us after the other (8192 x 128: 128 blocks 53 us).
-constexpr uint32_t kMaxRows = 64, kMaxBlocks = 64;
-__host__ __device__ inline uint32_t max_rows(const Job& j) {
-  const uint32_t blocks = j.across.p ? (j.rows + kMaxRows - 1) / kMaxRows : 1;
-  return (blocks + kMaxBlocks - 1) / kMaxBlocks * kMaxRows;
+// no multiple of 4 has its last quad end with the row.  Several such blocks for each, one
+// after the other: of columns where rows alone are wanted (a row's values are brought
+// together once), of rows where columns are and there are many.  (Atomics on one place
+// take some 0.4 us after the other: 8192 x 128, 128 blocks of rows, 53 us.)
+constexpr uint32_t kMaxRows = 64, kMaxBlocks = 32;
+struct Reach {
+  uint32_t rows, cols;  // of a workgroup
+};
+__host__ __device__ inline Reach reach(uint32_t rows, bool across) {
+  const uint32_t blocks = (rows + kMaxRows - 1) / kMaxRows;
+  return across ? Reach{(blocks + kMaxBlocks - 1) / kMaxBlocks * kMaxRows, kT} : Reach{kMaxRows, 2 * kT};
 }
 __global__ void __launch_bounds__(kT) k_mlp_max(const Jobs t) {
   __shared__ uint32_t tops[4][kT];
   const int k = find_job(t, blockIdx.x);
   const Job J = t.j[k];
-  const uint32_t id = blockIdx.x - t.start[k], wide = (J.cols + kT - 1) / kT, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const uint32_t high = max_rows(J), first = id / wide * high, c0 = id % wide * kT, c = min(c0 + lane * 4, J.cols - 4);
+  for (uint32_t i = blockIdx.x * kT + threadIdx.x; i < t.clears; i += gridDim.x * kT) t.clear[i] = 0;
+  const Reach by = reach(J.rows, J.across.p);
+  const uint32_t wide = (J.cols + by.cols - 1) / by.cols, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint32_t id = blockIdx.x - t.start[k], first = id / wide * by.rows, c0 = id % wide * by.cols;
   float top[4] = {0.f, 0.f, 0.f, 0.f};
-  for (uint32_t r0 = first + w * 16; r0 < min(first + high, J.rows); r0 += kMaxRows) {
-    f4u v[16];
+  for (uint32_t r0 = first + w * 16; r0 < min(first + by.rows, J.rows); r0 += kMaxRows) {
+    float row[16];
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) v[i] = ldus<false, f4u>(J.src + size_t(min(r0 + i, J.rows - 1)) * J.cols + c);
-    if (J.straight.p) {
+    for (uint32_t i = 0; i < 16; ++i) row[i] = 0.f;
+    for (uint32_t c1 = c0; c1 < min(c0 + by.cols, J.cols); c1 += kT) {
+      const float* p = J.src + min(c1 + lane * 4, J.cols - 4);
+      f4u v[16];
 #pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) {
-        float m = 0.f;
+      for (uint32_t i = 0; i < 16; ++i) v[i] = ldus<false, f4u>(p + size_t(min(r0 + i, J.rows - 1)) * J.cols);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m = fmaxf(m, size_of(v[i][e]));
-        m = wave_reduce(m, OpMaxR());
-        if (lane == 0 && r0 + i < J.rows && m > 0.f) atomicMax(J.straight.top + r0 + i, __float_as_uint(m));
-      }
+      for (uint32_t i = 0; i < 16; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = size_of(v[i][e]);
+          row[i] = fmaxf(row[i], x);
+          top[e] = fmaxf(top[e], x);
+        }
     }
+    if (!J.straight.p) continue;
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], size_of(v[i][e]));
+    for (uint32_t i = 0; i < 16; ++i) {
+      const float m = wave_reduce(row[i], OpMaxR());
+      if (lane == 0 && r0 + i < J.rows) J.rowPart[size_t(c0 / by.cols) * J.rows + r0 + i] = __float_as_uint(m);
+    }
   }
   if (!J.across.p) return;
 #pragma unroll
@@ -189,7 +205,7 @@ __global__ void __launch_bounds__(kT) k_mlp_max(const Jobs t) {
   // column threadIdx.x of the lanes' quads (two may be the same one)
   const uint32_t m = max(max(tops[0][threadIdx.x], tops[1][threadIdx.x]), max(tops[2][threadIdx.x], tops[3][threadIdx.x]));
   const uint32_t at = min(c0 + (threadIdx.x & ~3u), J.cols - 4) + (threadIdx.x & 3);
-  if (m) atomicMax(J.across.top + in_turn(at, J.turn), m);
+  J.colPart[size_t(first / by.rows) * J.cols + at] = m;
 }
 
 // A 128 x 128 tile through LDS.
@@ -199,6 +215,26 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
   const int k = find_job(t, blockIdx.x);
   const Job J = t.j[k];
   const uint32_t tc = (J.cols + 127) / 128, id = blockIdx.x - t.start[k], i0 = id / tc * 128, j0 = id % tc * 128;
+  // The rows' and columns' largest values; tiles at the edge leave them for the products.
+  __shared__ uint32_t tops[256];
+  {
+    const uint32_t l = threadIdx.x & 127, r = i0 + l, c = j0 + l;
+    uint32_t m = 0;
+    if (threadIdx.x < 128) {
+      if (J.straight.p && r < J.rows) {
+#pragma unroll 4
+        for (uint32_t i = 0; i < J.rowCount; ++i) m = max(m, J.rowFrom[size_t(i) * J.rows + r]);
+      }
+      if (J.straight.p && j0 == 0 && r < J.straight.rows) J.straight.top[r] = m;
+    } else {
+      if (J.across.p && c < J.cols) {
+#pragma unroll 4
+        for (uint32_t i = 0; i < J.colCount; ++i) m = max(m, J.colPart[size_t(i) * J.cols + c]);
+      }
+      if (J.across.p && i0 == 0 && in_turn(c, J.turn) < J.across.rows) J.across.top[in_turn(c, J.turn)] = m;
+    }
+    tops[threadIdx.x] = m;
+  }
   {
     // a quad of 16 rows for each thread; the last one ends with the row, as above
     const uint32_t q = threadIdx.x & 31, c = j0 + q * 4, at = min(c, J.cols - 4), off = min(c - at, 4u);
@@ -226,7 +262,7 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = tile_at<128>(S0, S1, rl, cl)[e];
       if (r < J.straight.rows && j0 + cl < J.straight.depth)
-        put8(J.straight.p + size_t(r) * J.straight.depth, J.c0 + j0 + cl, v, pow2(exp_of(field_of(J.straight.top[r]))));
+        put8(J.straight.p + size_t(r) * J.straight.depth, J.c0 + j0 + cl, v, pow2(exp_of(field_of(tops[rl]))));
     }
   }
   if (J.across.p) {
@@ -237,7 +273,7 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = tile_at<128>(S0, S1, rl, cl)[128 * e];
       if (c < J.across.rows && r < J.across.depth)
-        put8(J.across.p + size_t(c) * J.across.depth, r, v, pow2(exp_of(field_of(J.across.top[c]))));
+        put8(J.across.p + size_t(c) * J.across.depth, r, v, pow2(exp_of(field_of(tops[128 + cl]))));
     }
   }
 }
@@ -541,25 +577,44 @@ struct Places {
   }
 };
 
-// A side of whole tiles of rows, in the workspace; its maxima come after all parts.
+// The sides of a call's products, of whole tiles, and the passes that make the first ones.
 struct Plan {
   Places at;
-  size_t tops = 0;  // floats of maxima
+  size_t tops = 0, raised = 0;  // maxima, of which so many that products raise come first
   struct Made {
     Side* s;
     size_t p, top, field;
   };
   Made all[16];
   int count = 0;
+  Jobs jobs{};
+  size_t parts = 0;  // floats of the jobs' partial maxima
+  // Of a product's result (with blocks of so many values, which come first), or of a matrix.
   void side(Side& s, uint32_t rows, uint32_t depth, uint32_t block = 0) {
     s.rows = rows;
     s.depth = depth;
     all[count++] = {&s, at.take(size_t(rows) * depth), tops, block ? at.take((size_t(rows) * (depth / block) + 3) / 4) : ~size_t(0)};
     tops += rows;
+    if (block) raised = tops;
   }
-  // The workspace, with its maxima cleared; room for `more` floats at *extra.
+  // A matrix whose parts are to be made, of its rows or columns; both sides may still lack their places.
+  struct Source {
+    const float* src;
+    uint32_t rows, cols;
+    const Side *straight, *across;
+    uint32_t c0;
+    int turn;
+  };
+  Source sources[kJobs];
+  void add(const float* src, uint32_t rows, uint32_t cols, const Side* straight, const Side* across, uint32_t c0 = 0, int turn = -1) {
+    sources[jobs.count++] = {src, rows, cols, straight, across, c0, turn};
+    const Reach by = reach(rows, across);
+    if (straight) parts += size_t(cdiv(cols, by.cols)) * rows;
+    if (across) parts += size_t(cdiv(rows, by.rows)) * cols;
+  }
+  // The workspace, room for `more` floats at *extra, and the jobs.
   bool lay(size_t more, float** extra) {
-    const size_t first = at.take(tops), tail = at.take(more);
+    const size_t first = at.take(tops), tail = at.take(more), part = at.take(parts);
     float* ws = workspace(at.next);
     if (!ws) return false;
     *extra = ws + tail;
@@ -569,27 +624,49 @@ struct Plan {
       s.top = reinterpret_cast<uint32_t*>(ws + first) + all[i].top;
       s.field = all[i].field == ~size_t(0) ? nullptr : reinterpret_cast<uint8_t*>(ws + all[i].field);
     }
-    hipLaunchKernelGGL(k_mlp_clear, dim3(std::min(cdiv(tops, kT), 256u)), dim3(kT), 0, stream(),
-                       reinterpret_cast<uint32_t*>(ws + first), uint32_t(tops));
-    return check_launch("gated_mlp");
+    jobs.clear = reinterpret_cast<uint32_t*>(ws + first);
+    jobs.clears = uint32_t(raised);
+    uint32_t* next = reinterpret_cast<uint32_t*>(ws + part);
+    for (uint32_t i = 0; i < jobs.count; ++i) {
+      const Source& f = sources[i];
+      Job& j = jobs.j[i];
+      j.src = f.src;
+      j.rows = f.rows;
+      j.cols = f.cols;
+      if (f.straight) j.straight = *f.straight;
+      if (f.across) j.across = *f.across;
+      j.c0 = f.c0;
+      j.turn = f.turn;
+      const Reach by = reach(f.rows, f.across);
+      if (f.straight) {
+        const uint32_t n = cdiv(f.cols, by.cols);
+        j.rowPart = next;
+        next += size_t(n) * f.rows;
+        j.rowFrom = j.rowPart;
+        j.rowCount = n;
+        if (i && sources[i - 1].straight == f.straight) {  // behind the other's
+          Job& o = jobs.j[i - 1];
+          o.rowCount += n;
+          j.rowFrom = o.rowFrom;
+          j.rowCount = o.rowCount;
+        }
+      }
+      if (f.across) {
+        j.colPart = next;
+        j.colCount = cdiv(f.rows, by.rows);
+        next += size_t(j.colCount) * f.cols;
+      }
+    }
+    return true;
   }
 };
 
-void add(Jobs& t, const float* src, uint32_t rows, uint32_t cols, const Side& straight, const Side& across, uint32_t c0 = 0, int turn = -1) {
-  Job& j = t.j[t.count++];
-  j.src = src;
-  j.rows = rows;
-  j.cols = cols;
-  j.straight = straight;
-  j.across = across;
-  j.c0 = c0;
-  j.turn = turn;
-}
 bool run_jobs(Jobs& t) {
   uint32_t n = 0;
   for (uint32_t i = 0; i < t.count; ++i) {
     t.start[i] = n;
-    n += cdiv(t.j[i].rows, max_rows(t.j[i])) * cdiv(t.j[i].cols, kT);
+    const Reach by = reach(t.j[i].rows, t.j[i].across.p);
+    n += cdiv(t.j[i].rows, by.rows) * cdiv(t.j[i].cols, by.cols);
   }
   hipLaunchKernelGGL(k_mlp_max, dim3(n), dim3(kT), 0, stream(), t);
   if (!check_launch("gated_mlp")) return false;
@@ -667,11 +744,15 @@ void add(Prods<N>& t, const Side& p, const Side& q, bool right, uint32_t block, 
 bool mlp_forward_parts(const MlpArgs& a) {
   const uint32_t M = pad(a.rows, kTile), C = pad(a.cols, kTile), F = pad(a.hidden, kTile), O = pad(a.out, kTile);
   Plan plan;
-  Side x, w, d, m;
+  Side x{}, w{}, d{}, m{};
+  plan.side(m, M, F, 64);
   plan.side(x, M, C);
   plan.side(w, 2 * F, C);
   plan.side(d, O, F);
-  plan.side(m, M, F, 64);
+  plan.add(a.x, a.rows, a.cols, &x, nullptr);
+  plan.add(a.wg, a.cols, a.hidden, nullptr, &w, 0, 0);
+  plan.add(a.wu, a.cols, a.hidden, nullptr, &w, 0, 1);
+  plan.add(a.wd, a.hidden, a.out, nullptr, &d);
   ProfScope prof("mlp", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
   // The second product's sides get their places with the others.
   Prods<1> t1{}, t2{};
@@ -680,12 +761,7 @@ bool mlp_forward_parts(const MlpArgs& a) {
   if (!plan.lay(split(t2), &part)) return false;
   t2.a[0].p = m;
   t2.a[0].q = d;
-  Jobs t{};
-  add(t, a.x, a.rows, a.cols, x, {});
-  add(t, a.wg, a.cols, a.hidden, {}, w, 0, 0);
-  add(t, a.wu, a.cols, a.hidden, {}, w, 0, 1);
-  add(t, a.wd, a.hidden, a.out, {}, d);
-  if (!run_jobs(t)) return false;
+  if (!run_jobs(plan.jobs)) return false;
   t1.count = 1;
   Prod& g = t1.a[0];
   g.p = x;
@@ -705,18 +781,21 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
   const uint32_t M = pad(a.rows, kTile), C = pad(a.cols, kTile), F = pad(a.hidden, kTile), O = pad(a.out, kTile);
   Plan plan;
   Side yr{}, yc{}, d{}, xc{}, w{}, dr{}, dgc{}, duc{}, mc{};
-  plan.side(yr, M, O);
-  plan.side(d, F, O);
-  if (dwd) {
-    plan.side(yc, O, M);
-    plan.side(mc, F, M, 128);
-  }
-  if (dwg || dwu) plan.side(xc, C, M);
+  if (dx) plan.side(dr, M, 2 * F, 128);
+  if (dwd) plan.side(mc, F, M, 128);
   if (dwg) plan.side(dgc, F, M, 128);
   if (dwu) plan.side(duc, F, M, 128);
+  plan.side(yr, M, O);
+  plan.side(d, F, O);
+  if (dwd) plan.side(yc, O, M);
+  if (dwg || dwu) plan.side(xc, C, M);
+  if (dx) plan.side(w, C, 2 * F);
+  plan.add(dy, a.rows, a.out, &yr, dwd ? &yc : nullptr);
+  plan.add(a.wd, a.hidden, a.out, &d, nullptr);
+  if (dwg || dwu) plan.add(a.x, a.rows, a.cols, nullptr, &xc);
   if (dx) {
-    plan.side(w, C, 2 * F);
-    plan.side(dr, M, 2 * F, 128);
+    plan.add(a.wg, a.cols, a.hidden, &w, nullptr, 0);
+    plan.add(a.wu, a.cols, a.hidden, &w, nullptr, F);
   }
   ProfScope prof("mlp", 12.0 * a.rows * a.cols * a.hidden, 8.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
   // All that follow dm's in one launch, the deepest first: a last round of few workgroups
@@ -736,15 +815,7 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
   float* part;
   if (!plan.lay(split(t2), &part)) return false;
   rest();
-  Jobs t{};
-  add(t, dy, a.rows, a.out, yr, yc);
-  add(t, a.wd, a.hidden, a.out, d, {});
-  if (dwg || dwu) add(t, a.x, a.rows, a.cols, {}, xc);
-  if (dx) {
-    add(t, a.wg, a.cols, a.hidden, w, {}, 0);
-    add(t, a.wu, a.cols, a.hidden, w, {}, F);
-  }
-  if (!run_jobs(t)) return false;
+  if (!run_jobs(plan.jobs)) return false;
   Prods<1> t1{};
   t1.count = 1;
   Prod& g = t1.a[0];
