@@ -239,17 +239,17 @@ bool backward_small(const MlpArgs& a, const float* dy, float* dx, float* dwg, fl
 
 // ---------------------------------------------------------------------------
 // Up to 16 rows (new tokens): the weights are read once, on vector units.  A lane has one
-// column (of each of Wg, Wu) and sums for all rows; a workgroup has 64 columns and 128 k,
-// 16 for each of its 8 waves, all of whose loads are in flight at once.  Sums of the
-// depth's shares are left in memory and added up, in order, by what reads them: those of g
-// and u by the second product's workgroups, each for the 128 of its share, those of y by
-// a pass of its own.
+// column (of each of Wg, Wu) and sums for all rows; a workgroup has 64 columns and a share
+// of the depth, 128 k at a time, 16 for each of its 8 waves, all of whose loads are in
+// flight at once.  Sums of the shares are left in memory and added up, in order, by what
+// reads them: those of g and u by the second product's workgroups, each for its own
+// share, those of y by a pass of its own.
 // ---------------------------------------------------------------------------
 constexpr int kFew = 16, kFewWaves = 8, kFewDepth = 16 * kFewWaves;
 struct Few {
   const float *x, *w, *w2;  // w2: Wu, or null
   float* part;              // [shares][1 or 2][rows][cols]
-  uint32_t rows, depth, cols, blocks;
+  uint32_t rows, depth, cols, blocks, steps, each;  // steps of 128 k in all, and of a share
   // second product: x from g's and u's sums of `shares` shares
   const float* gu;
   uint32_t shares;
@@ -262,55 +262,91 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_mlp_few(const Few a) {
   __shared__ float S[kFewWaves][D * R * 64];
   const uint32_t share = blockIdx.x / a.blocks, block = blockIdx.x - share * a.blocks;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t k0 = share * kFewDepth, c = block * 64 + lane, col = min(c, a.cols - 1);
-  float y[D][KW];
-#pragma unroll
-  for (int i = 0; i < KW; ++i) {
-    const size_t at = size_t(min(k0 + w * KW + i, a.depth - 1)) * a.cols + col;
-    y[0][i] = a.w[at];
-    if constexpr (FIRST) y[D - 1][i] = a.w2[at];
-  }
-  // The rows' values, zeros past the depth (what the weights' clamped loads meet).
-#pragma unroll
-  for (int t = threadIdx.x; t < R * kFewDepth; t += T) {
-    const uint32_t r = t / kFewDepth, k = k0 + t % kFewDepth;
-    const bool in = r < a.rows && k < a.depth;
-    const size_t at = size_t(in ? r : 0) * a.depth + min(k, a.depth - 1);
-    float v = 0.f;
-    if constexpr (FIRST) {
-      v = a.x[at];
-    } else {
-      const size_t n = size_t(a.rows) * a.depth;
-      float g = 0.f, u = 0.f;
-#pragma unroll 8
-      for (uint32_t s = 0; s < a.shares; ++s) {
-        g += a.gu[2 * s * n + at];
-        u += a.gu[(2 * s + 1) * n + at];
-      }
-      v = act<ACT>(g) * u;
-      if (a.g && block == 0 && in) {
-        a.g[at] = g;
-        a.u[at] = u;
-      }
-    }
-    X[r][t % kFewDepth] = in ? v : 0.f;
-  }
-  __syncthreads();
+  const uint32_t c = block * 64 + lane, col = min(c, a.cols - 1);
   float acc[D][R];
 #pragma unroll
   for (int d = 0; d < D; ++d)
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[d][r] = 0.f;
+  const uint32_t end = min((share + 1) * a.each, a.steps);
+  for (uint32_t step = share * a.each; step < end; ++step) {
+    const uint32_t k0 = step * kFewDepth;
+    float y[D][KW];
 #pragma unroll
-  for (int i = 0; i < KW; i += 4)
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const f4 x = *reinterpret_cast<const f4*>(&X[r][w * KW + i]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int d = 0; d < D; ++d) acc[d][r] = fmaf(x[e], y[d][i + e], acc[d][r]);
+    for (int i = 0; i < KW; ++i) {
+      const size_t at = size_t(min(k0 + w * KW + i, a.depth - 1)) * a.cols + col;
+      y[0][i] = a.w[at];
+      if constexpr (FIRST) y[D - 1][i] = a.w2[at];
     }
+    if (step != share * a.each) __syncthreads();
+    // The rows' values, zeros past the depth, as the weights' there.
+    constexpr int EACH = (R * kFewDepth + T - 1) / T;
+    float v[EACH];
+    size_t at[EACH];
+    bool in[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const uint32_t t = threadIdx.x + j * T, r = t / kFewDepth, k = k0 + t % kFewDepth;
+      in[j] = r < a.rows && k < a.depth;
+      at[j] = size_t(in[j] ? r : 0) * a.depth + min(k, a.depth - 1);
+      if constexpr (FIRST) v[j] = a.x[at[j]];
+    }
+    if constexpr (!FIRST) {
+      const size_t n = size_t(a.rows) * a.depth;
+      float g[EACH], u[EACH];
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) g[j] = u[j] = 0.f;
+      constexpr uint32_t U = EACH > 2 ? 2 : 4;  // shares in flight
+      for (uint32_t s = 0; s < a.shares; s += U) {
+        float p[EACH][U], q[EACH][U];
+#pragma unroll
+        for (uint32_t i = 0; i < U; ++i)
+#pragma unroll
+          for (int j = 0; j < EACH; ++j) {
+            const size_t from = 2 * min(s + i, a.shares - 1) * n + at[j];
+            p[j][i] = a.gu[from];
+            q[j][i] = a.gu[from + n];
+          }
+#pragma unroll
+        for (uint32_t i = 0; i < U; ++i)
+#pragma unroll
+          for (int j = 0; j < EACH; ++j) {
+            g[j] += s + i < a.shares ? p[j][i] : 0.f;
+            u[j] += s + i < a.shares ? q[j][i] : 0.f;
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        v[j] = act<ACT>(g[j]) * u[j];
+        if (a.g && block == 0 && in[j]) {
+          a.g[at[j]] = g[j];
+          a.u[at[j]] = u[j];
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const uint32_t t = threadIdx.x + j * T;
+      if (R * kFewDepth >= T || t < R * kFewDepth) X[t / kFewDepth][t % kFewDepth] = in[j] ? v[j] : 0.f;
+    }
+    __syncthreads();
+    if (k0 + kFewDepth > a.depth) {
+#pragma unroll
+      for (int i = 0; i < KW; ++i)
+#pragma unroll
+        for (int d = 0; d < D; ++d) y[d][i] = k0 + w * KW + i < a.depth ? y[d][i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < KW; i += 4)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const f4 x = *reinterpret_cast<const f4*>(&X[r][w * KW + i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int d = 0; d < D; ++d) acc[d][r] = fmaf(x[e], y[d][i + e], acc[d][r]);
+      }
+  }
 #pragma unroll
   for (int d = 0; d < D; ++d)
 #pragma unroll
@@ -334,27 +370,34 @@ __global__ void __launch_bounds__(256) k_mlp_few_sum(const float* part, float* y
 }
 
 bool forward_few(const MlpArgs& a) {
-  const uint32_t s1 = cdiv(a.cols, kFewDepth), s2 = cdiv(a.hidden, kFewDepth);
+  Few f{}, s{};
+  auto size = [](Few& t, uint32_t depth, uint32_t cols) {
+    t.depth = depth;
+    t.cols = cols;
+    t.blocks = cdiv(cols, 64);
+    t.steps = cdiv(depth, kFewDepth);
+    // Some 512 workgroups, two a CU, and shares of 128 k only where there are fewer than one:
+    // what shares leave has to be read again (16 rows of 2048 x 8192: 76 us with shares of 128
+    // everywhere, 64 with 1024 workgroups, 53 with 512, 68 with 256; 8 of 1024 x 2816: 19.4 with
+    // shares of 128, 17.5 of 256, 19.3 of 384; of 512 x 2048: 11.2, 13.8, 18.4).
+    const uint32_t all = t.blocks * t.steps;
+    t.each = all <= 256 ? 1 : std::max(2u, cdiv(t.steps, cdiv(512, t.blocks)));
+    return cdiv(t.steps, t.each);
+  };
+  const uint32_t s1 = size(f, a.cols, a.hidden), s2 = size(s, a.hidden, a.out);
   const size_t gu = 2 * size_t(s1) * a.rows * a.hidden, ny = size_t(s2) * a.rows * a.out;
   float* ws = workspace(((gu + 63) & ~size_t(63)) + (s2 > 1 ? ny : 0));
   if (!ws) return false;
   float* part = s2 > 1 ? ws + ((gu + 63) & ~size_t(63)) : a.y;
   ProfScope prof("mlp", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
-  Few f{}, s{};
   f.x = a.x;
   f.w = a.wg;
   f.w2 = a.wu;
   f.part = ws;
   f.rows = a.rows;
-  f.depth = a.cols;
-  f.cols = a.hidden;
-  f.blocks = cdiv(a.hidden, 64);
   s.w = a.wd;
   s.part = part;
   s.rows = a.rows;
-  s.depth = a.hidden;
-  s.cols = a.out;
-  s.blocks = cdiv(a.out, 64);
   s.gu = ws;
   s.shares = s1;
   s.g = a.saved;

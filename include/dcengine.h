@@ -315,7 +315,8 @@ void GatedMlpBackward(void* gradOut, void* x, void* wGate, void* wUp, void* wDow
  * NULL: zeros).  lengths: batch floats, the tokens of each sequence that count
  * (clamped to 0 .. seq; memory past them may hold anything), or NULL: all; y is
  * zeros past them.  pLast, when not NULL, receives the state after the last token
- * that counts (batch x chans): the next call's `state`.  The backward reads the
+ * that counts (batch x chans): the next call's `state`.  Sequences of fewer than 2130706432
+ * tokens, and of 2^24 and more with fewer than four channels no more than 2^30 - 2^22 tokens in all.  The backward reads the
  * forward's result; gradients past the lengths are zeros, and none flows in
  * through *pLast. */
 void* GatedScanForward(void* x, void* gate, void* state, void* lengths, uint32_t batch,

@@ -766,3 +766,39 @@ def test_layers(eng):
     eng.Muon(params, lr=0.01).step()
     assert all(p.grad is not None and not np.array_equal(p.sync(), b) for p, b in zip(params, before))
     eng.end_batch()
+
+
+@pytest.mark.parametrize("rows", [1, 4, 7, 16])
+@pytest.mark.parametrize("size", [(2053, 5000, 131), (131, 9000, 300), (4100, 300, 2100)], ids=lambda s: "x".join(map(str, s)))
+def test_gated_mlp_of_few_tokens_and_many_weights(eng, size, rows):
+    """Shares of the depth of one and of several steps, the last one not whole."""
+    print("gated_mlp few", rows, size, flush=True)
+    check_mlp(eng, rows, *size, "gelu", rng(rows + size[0]))
+
+
+@pytest.mark.parametrize("rows", [1, 12, 40])
+def test_gated_mlp_of_a_weight_that_is_infinite(eng, rows):
+    """The last ones of their columns, where the depth ends inside a step: the
+    results that it makes infinite are that, the other outputs as before."""
+    r = rng(rows)
+    x, wg, wu, wd = (r.standard_normal(s).astype(np.float32) for s in ((rows, 300), (300, 37), (300, 37), (37, 90)))
+    t = [dev(eng, v) for v in (np.abs(x), np.abs(wg), np.abs(wu), wd)]
+    want = eng.gated_mlp(*t).sync().copy()
+    down = wd.copy()
+    down[36, 5] = np.inf
+    got = eng.gated_mlp(*t[:3], dev(eng, down)).sync()
+    assert (got[:, 5] == np.inf).all()
+    assert np.array_equal(np.delete(got, 5, 1), np.delete(want, 5, 1))
+    up = np.abs(wu)
+    up[299, 36] = np.inf
+    got = eng.gated_mlp(*t[:2], dev(eng, up), t[3]).sync()
+    assert (got == np.where(wd[36] < 0, -np.inf, np.inf)).all()
+    eng.end_batch()
+
+
+def test_gated_scan_refuses_what_no_launch_holds(eng):
+    four = dev(eng, np.zeros(4))
+    lib, b = eng.lib, four.gpu_buf
+    for sizes in ((255, 1 << 24, 1), (1, 1 << 30, 3), (2, 1 << 29, 2)):
+        assert not lib.GatedScanForward(b, b, None, None, *sizes, None) and "2^30" in eng.last_error(), sizes
+        lib.ClearLastError()
