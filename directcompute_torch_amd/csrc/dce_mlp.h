@@ -41,8 +41,24 @@ void by_act(MlpAct act, F&& f) {
   if (act == kSigmoid) f(std::integral_constant<MlpAct, kSigmoid>{});
 }
 
+// Sums of `splits` shares of n (4 or more) values, one after the other, in order.
+struct MlpSums {
+  struct One {
+    const float* part;
+    float* out;
+    uint32_t n, splits, start;
+  };
+  One s[4];
+  uint32_t count, blocks;  // of 256 threads, 4 values each
+  void add(const float* part, float* out, uint32_t n, uint32_t splits) {
+    s[count++] = {part, out, n, splits, blocks};
+    blocks += uint32_t((uint64_t(n) + 1023) / 1024);
+  }
+};
+void mlp_sum(const MlpSums& t);
+
 // On fp16 parts, for large calls.
-bool mlp_on_parts(const MlpArgs& a);
+bool mlp_on_parts(const MlpArgs& a, bool backward);
 bool mlp_forward_parts(const MlpArgs& a);
 bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd);
 

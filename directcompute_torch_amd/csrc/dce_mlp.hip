@@ -17,11 +17,18 @@ inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b);
 
 // ---------------------------------------------------------------------------
 // Products of small calls on fp32 MFMAs, C[r][c] = sum over k of A(r, k) B(c, k), in
-// tiles of 32 x 32 for each workgroup, whose waves share the depth and add up their sums
-// in LDS, in order.  No stage in between: an operand whose depth is contiguous comes by
-// 16 bytes a lane, 4 k of its row, the other one by a dword of each k, 32 neighbours
-// together.  The MFMA's two k of a step are then 4 apart, for both.  Rows and columns
-// outside are the last ones again; what comes of them is not stored.
+// tiles of 32 x 32.  1, 2, 4 or 8 of a workgroup's eight waves share a tile's depth and add
+// up their sums in LDS, in order; of a deep product with few tiles workgroups do, too, whose
+// sums a pass brings together, in order.  No stage in between: an operand whose depth is
+// contiguous comes by 16 bytes a lane, 4 k of its row, the other one by a dword of each k,
+// 32 neighbours together.  The MFMA's two k of a step are then 4 apart, for both.  Rows and
+// columns outside are the last ones again; what comes of them is not stored.
+//
+// Bound by memory latency: a wave has four octets of k in flight and then multiplies them,
+// and most calls have a wave or two of each SIMD only.  154 x 384 x 1001 (1 / 6.6 of fp32's
+// MFMA rate): the gate's product 9.6 us, y 6.2 and 3.8 for its sums, the gradient's 9.0, the
+// four others 18.4 and 4.7; 64 x 1024 x 2816, training: 82 us (with eight waves for each
+// tile and no splits 102).  Eight octets in flight, with twice the code, took 10 % more.
 // ---------------------------------------------------------------------------
 enum Op { STORE, GATE, GRAD };
 struct Side {
@@ -31,7 +38,8 @@ struct Side {
 struct Prod {
   Side a, b, b2;   // b2: GATE: Wu; STORE: of the second part
   const float* a2; // STORE: a second part of the depth, as long as the first (null: none)
-  uint32_t depth, start, across;  // first workgroup; tiles across the columns
+  uint32_t depth, start, across, tiles;  // first workgroup; tiles across the columns, in all
+  uint32_t waves, splits;  // log2 of the waves that share a tile's depth, workgroups that do
   uint32_t aDeep, bDeep;  // is the depth contiguous
   float *out, *g, *u, *du, *m;
 };
@@ -65,63 +73,92 @@ __device__ __forceinline__ void octet(const float* p, uint32_t pitch, uint32_t o
 constexpr int kWaves = 8;
 template <Op OP, MlpAct ACT>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4, 4))) k_mlp_small(const Prods all) {
-  constexpr int NW = kWaves;
-  constexpr bool DUAL = OP == GATE;
-  __shared__ float S[NW][32 * 32];
+  constexpr int NW = kWaves, D = OP == GATE ? 2 : 1;
+  __shared__ float S[D][NW][32 * 32];
   uint32_t id = blockIdx.x;
   int which = 0;
   while (which + 1 < int(all.count) && all.p[which + 1].start <= id) ++which;
   const Prod& P = all.p[which];
   id -= P.start;
-  const uint32_t r0 = id / P.across * 32, c0 = id % P.across * 32;
-  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  f16v acc[DUAL ? 2 : 1];
+  const uint32_t each = NW >> P.waves, groups = (P.tiles + each - 1) >> (3 - P.waves);  // tiles of a workgroup
+  const uint32_t sp = id / groups, first = (id - sp * groups) * each;
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t tile = min(first + (w >> P.waves), P.tiles - 1), share = (sp << P.waves) + (w & ((1u << P.waves) - 1)), shares = P.splits << P.waves;
+  f16v acc[D];
 #pragma unroll
-  for (int d = 0; d < (DUAL ? 2 : 1); ++d)
+  for (int d = 0; d < D; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
-  const uint32_t ar = min(r0 + col, P.a.n - 1), bc = min(c0 + col, P.b.n - 1);
-  const uint32_t octets = P.depth / 8, lo = octets * w / NW, hi = octets * (w + 1) / NW;
-  const bool tail = P.depth % 8 && w == NW - 1;
-  auto run = [&](auto aDeep, auto bDeep, const float* a, const float* b, const float* b2) {
+  const uint32_t ti = tile / P.across, tj = tile - ti * P.across;
+  const uint32_t ar = min(ti * 32 + col, P.a.n - 1), bc = min(tj * 32 + col, P.b.n - 1);
+  const uint32_t octets = P.depth / 8, few = octets / shares, more = octets - few * shares;
+  const uint32_t lo = share * few + min(share, more), hi = lo + few + (share < more);
+  const bool tail = P.depth % 8 && share + 1 == shares;
+  // This thread's places in the group's tile i; GRAD: g and u there, the first ones' ahead of the product.
+  size_t at[2];
+  bool in[2];
+  float g[2], u[2];
+  auto at_of = [&](uint32_t i) __attribute__((always_inline)) {
+    const uint32_t now = min(first + i, P.tiles - 1), ni = now / P.across, nj = now - ni * P.across;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t t = threadIdx.x + h * NW * 64, r = ni * 32 + t / 32, c = nj * 32 + t % 32;
+      in[h] = first + i < P.tiles && r < P.a.n && c < P.b.n;
+      at[h] = in[h] ? size_t(r) * P.b.n + c : 0;
+      if constexpr (OP == GRAD) {
+        g[h] = P.g[at[h]];
+        u[h] = P.u[at[h]];
+      }
+    }
+  };
+  at_of(0);
+  auto run = [&](auto aDeep, auto bDeep, const float* a, const float* b, const float* b2) __attribute__((always_inline)) {
     constexpr bool AD = decltype(aDeep)::value, BD = decltype(bDeep)::value;
     const uint32_t ao = (AD ? ar * P.a.pitch + 4 * half : 4 * half * P.a.pitch + ar) * 4;
     const uint32_t bo = (BD ? bc * P.b.pitch + 4 * half : 4 * half * P.b.pitch + bc) * 4;
     constexpr int U = 4;  // octets in flight
-    float x[U][4], y[U][4], z[DUAL ? U : 1][4];
-    auto mul = [&](int j) {
+    float x[U][4], y[U][4], z[D == 2 ? U : 1][4];
+    auto mul = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         acc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j][i], y[j][i], acc[0], 0, 0, 0);
-        if constexpr (DUAL) acc[DUAL ? 1 : 0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j][i], z[DUAL ? j : 0][i], acc[DUAL ? 1 : 0], 0, 0, 0);
+        if constexpr (D == 2) acc[D - 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j][i], z[D == 2 ? j : 0][i], acc[D - 1], 0, 0, 0);
       }
     };
     uint32_t o = lo;
+    auto fetch = [&](int j, uint32_t at) __attribute__((always_inline)) {
+      octet<AD, true>(a, P.a.pitch, ao, at, P.depth, half, x[j]);
+      octet<BD, true>(b, P.b.pitch, bo, at, P.depth, half, y[j]);
+      if constexpr (D == 2) octet<BD, true>(b2, P.b.pitch, bo, at, P.depth, half, z[D == 2 ? j : 0]);
+    };
     for (; o + U <= hi; o += U) {
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        octet<AD, true>(a, P.a.pitch, ao, o + j, P.depth, half, x[j]);
-        octet<BD, true>(b, P.b.pitch, bo, o + j, P.depth, half, y[j]);
-        if constexpr (DUAL) octet<BD, true>(b2, P.b.pitch, bo, o + j, P.depth, half, z[DUAL ? j : 0]);
-      }
+      for (int j = 0; j < U; ++j) fetch(j, o + j);
 #pragma unroll
       for (int j = 0; j < U; ++j) mul(j);
     }
-    for (; o < hi; ++o) {
-      octet<AD, true>(a, P.a.pitch, ao, o, P.depth, half, x[0]);
-      octet<BD, true>(b, P.b.pitch, bo, o, P.depth, half, y[0]);
-      if constexpr (DUAL) octet<BD, true>(b2, P.b.pitch, bo, o, P.depth, half, z[0]);
+    if (o < hi) {  // up to three more
+#pragma unroll
+      for (int j = 0; j < U - 1; ++j) fetch(j, min(o + j, hi - 1));
       mul(0);
+#pragma unroll
+      for (int j = 1; j < U - 1; ++j)
+        if (o + j < hi) mul(j);
     }
     if (tail) {
       octet<AD, false>(a, P.a.pitch, ao, octets, P.depth, half, x[0]);
       octet<BD, false>(b, P.b.pitch, bo, octets, P.depth, half, y[0]);
-      if constexpr (DUAL) octet<BD, false>(b2, P.b.pitch, bo, octets, P.depth, half, z[0]);
+      if constexpr (D == 2) octet<BD, false>(b2, P.b.pitch, bo, octets, P.depth, half, z[0]);
       mul(0);
     }
   };
-  auto pass = [&](const float* a, const float* b, const float* b2) {
-    if (!P.aDeep)
+  auto pass = [&](const float* a, const float* b, const float* b2) __attribute__((always_inline)) {
+    if constexpr (OP == GATE)
+      run(std::true_type{}, std::false_type{}, a, b, b2);
+    else if constexpr (OP == GRAD)
+      run(std::true_type{}, std::true_type{}, a, b, b2);
+    else if (!P.aDeep)
       run(std::false_type{}, std::false_type{}, a, b, b2);
     else if (P.bDeep)
       run(std::true_type{}, std::true_type{}, a, b, b2);
@@ -130,58 +167,104 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
   };
   pass(P.a.p, P.b.p, P.b2.p);
   if (OP == STORE && P.a2) pass(P.a2, P.b2.p, nullptr);
-  // The waves' sums: thread t takes every NW * 64-th value of the tile.
-  constexpr int EACH = 1024 / (NW * 64);
-  float v[DUAL ? 2 : 1][EACH];
 #pragma unroll
-  for (int d = 0; d < (DUAL ? 2 : 1); ++d) {
-    if (d) __syncthreads();
+  for (int d = 0; d < D; ++d)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) S[w][(8 * (e >> 2) + 4 * half + (e & 3)) * 32 + col] = acc[d][e];
-    __syncthreads();
+    for (int e = 0; e < 16; ++e) S[d][w][(8 * (e >> 2) + 4 * half + (e & 3)) * 32 + col] = acc[d][e];
+  __syncthreads();
+  // The waves' sums, a thread two values of each tile.
+  float* out = P.out + (OP == STORE ? size_t(sp) * P.a.n * P.b.n : 0);
+  for (uint32_t i = 0; i < each; ++i) {
+    if (i) at_of(i);
+    float v[2][D];
+    auto sum = [&](auto waves) __attribute__((always_inline)) {
+      constexpr int N = decltype(waves)::value;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      v[d][i] = 0.f;
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int n = 0; n < NW; ++n) v[d][i] += S[n][threadIdx.x + i * NW * 64];
-    }
-  }
+        for (int d = 0; d < D; ++d) {
+          v[h][d] = 0.f;
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const uint32_t t = threadIdx.x + i * NW * 64, r = r0 + t / 32, c = c0 + t % 32;
-    if (r >= P.a.n || c >= P.b.n) continue;
-    const size_t at = size_t(r) * P.b.n + c;
-    if constexpr (OP == STORE) P.out[at] = v[0][i];
-    if constexpr (OP == GATE) {
-      P.out[at] = act<ACT>(v[0][i]) * v[DUAL ? 1 : 0][i];
-      if (P.g) {
-        P.g[at] = v[0][i];
-        P.u[at] = v[DUAL ? 1 : 0][i];
+          for (int n = 0; n < N; ++n) v[h][d] += S[d][i * N + n][threadIdx.x + h * NW * 64];
+        }
+    };
+    if (P.waves == 3)
+      sum(std::integral_constant<int, 8>{});
+    else if (P.waves == 2)
+      sum(std::integral_constant<int, 4>{});
+    else if (P.waves == 1)
+      sum(std::integral_constant<int, 2>{});
+    else
+      sum(std::integral_constant<int, 1>{});
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (!in[h]) continue;
+      if constexpr (OP == STORE) out[at[h]] = v[h][0];
+      if constexpr (OP == GATE) {
+        out[at[h]] = act<ACT>(v[h][0]) * v[h][D - 1];
+        if (P.g) {
+          P.g[at[h]] = v[h][0];
+          P.u[at[h]] = v[h][D - 1];
+        }
       }
-    }
-    if constexpr (OP == GRAD) {
-      float d;
-      const float y = act_grad<ACT>(P.g[at], d), u = P.u[at];
-      P.out[at] = v[0][i] * u * d;
-      P.du[at] = v[0][i] * y;
-      P.m[at] = y * u;
+      if constexpr (OP == GRAD) {
+        float d;
+        const float y = act_grad<ACT>(g[h], d);
+        out[at[h]] = v[h][0] * u[h] * d;
+        P.du[at[h]] = v[h][0] * y;
+        P.m[at[h]] = y * u[h];
+      }
     }
   }
 }
 
+// How the products of a launch share their depths, such that every wave has about as many
+// octets (4096 waves are 16 for each CU, all that run at once); floats of what splits leave.
+// More than a workgroup's eight waves for a tile only where each of those would have three times
+// its share, or 12 octets: the sums are one more launch (training us without splits and with them,
+// 20 x 2048 x 8192 384 and 205, 40 x 512 x 2048 67 and 44, 154 x 384 x 1001 54 and 46; from
+// twice the share on, 300 x 256 x 512 35 for 33).
+size_t share(Prods& t, bool split) {
+  double all = 0;
+  size_t floats = 0;
+  auto octets = [](const Prod& p) { return (p.a2 ? 2.0 : 1.0) * p.depth / 8; };
+  for (uint32_t i = 0; i < t.count; ++i) {
+    Prod& p = t.p[i];
+    p.across = cdiv(p.b.n, 32);
+    p.tiles = cdiv(p.a.n, 32) * p.across;
+    all += p.tiles * octets(p);
+  }
+  const double most = std::max(1.0, all / 4096);
+  for (uint32_t i = 0; i < t.count; ++i) {
+    Prod& p = t.p[i];
+    const double depth = octets(p), want = depth / std::max(most, 4.0);
+    p.waves = 0;
+    while ((1 << p.waves) < std::min<double>(depth / most, kWaves)) ++p.waves;
+    const size_t n = size_t(p.a.n) * p.b.n;
+    p.splits = split && n >= 4 && want > 3 * kWaves ? cdiv(uint64_t(want), kWaves) : 1;
+    if (p.splits > 1) floats += (p.splits * n + 63) & ~size_t(63);
+  }
+  return floats;
+}
 template <Op OP>
-bool run_small(Prods& t, MlpAct act = kSilu) {
+bool run_small(Prods& t, MlpAct act = kSilu, float* part = nullptr) {
   uint32_t n = 0;
+  MlpSums sums{};
   for (uint32_t i = 0; i < t.count; ++i) {
     Prod& p = t.p[i];
     p.start = n;
-    p.across = cdiv(p.b.n, 32);
-    n += cdiv(p.a.n, 32) * p.across;
+    n += cdiv(p.tiles, kWaves >> p.waves) * p.splits;
+    if (p.splits == 1) continue;
+    const size_t values = size_t(p.a.n) * p.b.n;
+    sums.add(part, p.out, uint32_t(values), p.splits);
+    p.out = part;
+    part += (p.splits * values + 63) & ~size_t(63);
   }
   by_act(act, [&](auto k) {
     constexpr MlpAct A = OP == STORE ? kSilu : decltype(k)::value;
     hipLaunchKernelGGL((k_mlp_small<OP, A>), dim3(n), dim3(kWaves * 64), 0, stream(), t);
   });
+  mlp_sum(sums);
   return check_launch("gated_mlp");
 }
 Prod& add(Prods& t, const float* a, uint32_t rows, uint32_t aPitch, bool aDeep, const float* b, uint32_t cols, uint32_t bPitch, bool bDeep,
@@ -197,44 +280,50 @@ Prod& add(Prods& t, const float* a, uint32_t rows, uint32_t aPitch, bool aDeep, 
 }
 
 bool forward_small(const MlpArgs& a) {
-  const size_t n = size_t(a.rows) * a.hidden;
-  float* m = workspace(n);
+  const size_t n = size_t(a.rows) * a.hidden, at = (n + 63) & ~size_t(63);
+  Prods t{}, y{};
+  add(y, nullptr, a.rows, a.hidden, true, a.wd, a.out, a.out, false, a.hidden, a.y);
+  float* m = workspace(at + share(y, true));
   if (!m) return false;
   ProfScope prof("mlp", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
-  Prods t{};
   Prod& p = add(t, a.x, a.rows, a.cols, true, a.wg, a.hidden, a.hidden, false, a.cols, m);
   p.b2.p = a.wu;
   p.g = a.saved;
   p.u = a.saved ? a.saved + n : nullptr;
+  share(t, false);
   if (!run_small<GATE>(t, a.act)) return false;
-  Prods y{};
-  add(y, m, a.rows, a.hidden, true, a.wd, a.out, a.out, false, a.hidden, a.y);
-  return run_small<STORE>(y);
+  y.p[0].a.p = m;
+  return run_small<STORE>(y, kSilu, m + at);
 }
 
 bool backward_small(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
   const size_t n = size_t(a.rows) * a.hidden, at = (n + 63) & ~size_t(63);
-  float* dg = workspace(3 * at);
+  // Twice: how the products share first, their places once there is a workspace.
+  Prods t{}, r{};
+  auto rest = [&](float* dg) {
+    float *du = dg ? dg + at : nullptr, *m = dg ? du + at : nullptr;
+    r = {};
+    if (dx) {
+      Prod& q = add(r, dg, a.rows, a.hidden, true, a.wg, a.cols, a.hidden, true, a.hidden, dx);
+      q.a2 = dg ? du : a.x;
+      q.b2.p = a.wu;
+    }
+    if (dwd) add(r, m, a.hidden, a.hidden, false, dy, a.out, a.out, false, a.rows, dwd);
+    if (dwg) add(r, a.x, a.cols, a.cols, false, dg, a.hidden, a.hidden, false, a.rows, dwg);
+    if (dwu) add(r, a.x, a.cols, a.cols, false, du, a.hidden, a.hidden, false, a.rows, dwu);
+    return share(r, true);
+  };
+  float* dg = workspace(3 * at + rest(nullptr));
   if (!dg) return false;
-  float *du = dg + at, *m = du + at;
+  rest(dg);
   ProfScope prof("mlp", 12.0 * a.rows * a.cols * a.hidden, 8.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
-  Prods t{};
   Prod& p = add(t, dy, a.rows, a.out, true, a.wd, a.hidden, a.out, true, a.out, dg);
   p.g = a.saved;
   p.u = a.saved + n;
-  p.du = du;
-  p.m = m;
-  if (!run_small<GRAD>(t, a.act)) return false;
-  Prods r{};
-  if (dx) {
-    Prod& q = add(r, dg, a.rows, a.hidden, true, a.wg, a.cols, a.hidden, true, a.hidden, dx);
-    q.a2 = du;
-    q.b2.p = a.wu;
-  }
-  if (dwd) add(r, m, a.hidden, a.hidden, false, dy, a.out, a.out, false, a.rows, dwd);
-  if (dwg) add(r, a.x, a.cols, a.cols, false, dg, a.hidden, a.hidden, false, a.rows, dwg);
-  if (dwu) add(r, a.x, a.cols, a.cols, false, du, a.hidden, a.hidden, false, a.rows, dwu);
-  return run_small<STORE>(r);
+  p.du = dg + at;
+  p.m = p.du + at;
+  share(t, false);
+  return run_small<GRAD>(t, a.act) && run_small<STORE>(r, kSilu, dg + 3 * at);
 }
 
 // ---------------------------------------------------------------------------
@@ -244,6 +333,11 @@ bool backward_small(const MlpArgs& a, const float* dy, float* dx, float* dwg, fl
 // flight at once.  Sums of the shares are left in memory and added up, in order, by what
 // reads them: those of g and u by the second product's workgroups, each for its own
 // share, those of y by a pass of its own.
+//
+// Bound by memory.  8 rows, 1024 x 2816: 8.7, 6.8 and 3.0 us for 34.6 MB of weights, a
+// launch's own time each not far below that (on MFMAs as above 62 in all); 2048 x 8192:
+// 41 us, 4.8 TB/s; 4096 x 11008: 122 us, 4.4 TB/s.  The next step's weights loaded ahead
+// gained nothing: two workgroups a CU cover each other.
 // ---------------------------------------------------------------------------
 constexpr int kFew = 16, kFewWaves = 8, kFewDepth = 16 * kFewWaves;
 struct Few {
@@ -426,11 +520,11 @@ bool forward_few(const MlpArgs& a) {
 
 bool mlp_forward(const MlpArgs& a) {
   if (a.rows <= uint32_t(kFew)) return forward_few(a);
-  return mlp_on_parts(a) ? mlp_forward_parts(a) : forward_small(a);
+  return mlp_on_parts(a, false) ? mlp_forward_parts(a) : forward_small(a);
 }
 
 bool mlp_backward(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
-  return mlp_on_parts(a) ? mlp_backward_parts(a, dy, dx, dwg, dwu, dwd) : backward_small(a, dy, dx, dwg, dwu, dwd);
+  return mlp_on_parts(a, true) ? mlp_backward_parts(a, dy, dx, dwg, dwu, dwd) : backward_small(a, dy, dx, dwg, dwu, dwd);
 }
 
 }  // namespace dce

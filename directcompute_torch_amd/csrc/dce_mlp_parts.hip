@@ -543,20 +543,10 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
   }
 }
 
-// Sums of the splits' shares, in order.
-struct Sum {
-  const float* part;
-  float* out;
-  uint32_t n, splits, start;
-};
-struct Sums {
-  Sum s[4];
-  uint32_t count, blocks;
-};
-__global__ void __launch_bounds__(kT) k_mlp_sum(const Sums t) {
+__global__ void __launch_bounds__(kT) k_mlp_sum(const MlpSums t) {
   int k = 0;
   while (k + 1 < int(t.count) && t.s[k + 1].start <= blockIdx.x) ++k;
-  const Sum s = t.s[k];
+  const MlpSums::One s = t.s[k];
   const uint32_t i = ((blockIdx.x - s.start) * kT + threadIdx.x) * 4;
   if (i >= s.n) return;
   // the last quad ends with the matrix; fewer than 4 values there are none
@@ -701,7 +691,7 @@ size_t split(Prods<N>& t) {
 template <Op OP, int N>
 bool run_products(Prods<N>& t, MlpAct act = kSilu, float* part = nullptr, double bytes = 0) {
   uint32_t n = 0;
-  Sums sums{};
+  MlpSums sums{};
   for (uint32_t i = 0; i < t.count; ++i) {
     Prod& a = t.a[i];
     a.tm = a.p.rows / kTile;
@@ -713,8 +703,7 @@ bool run_products(Prods<N>& t, MlpAct act = kSilu, float* part = nullptr, double
     a.part = part;
     const size_t values = size_t(a.rows) * a.cols;
     part += (size_t(a.splits) * values + 63) & ~size_t(63);
-    sums.s[sums.count++] = {a.part, a.out, uint32_t(values), a.splits, sums.blocks};
-    sums.blocks += cdiv(values, 4 * kT);
+    sums.add(a.part, a.out, uint32_t(values), a.splits);
   }
   by_act(act, [&](auto k) {
     constexpr MlpAct A = OP == STORE ? kSilu : decltype(k)::value;
@@ -723,7 +712,7 @@ bool run_products(Prods<N>& t, MlpAct act = kSilu, float* part = nullptr, double
     else
       hipLaunchKernelGGL((k_mlp_product<OP, A, N, false>), dim3(n), dim3(kT), 0, stream(), t);
   });
-  if (sums.count) hipLaunchKernelGGL(k_mlp_sum, dim3(sums.blocks), dim3(kT), 0, stream(), sums);
+  mlp_sum(sums);
   return check_launch("gated_mlp");
 }
 template <int N>
@@ -740,6 +729,10 @@ void add(Prods<N>& t, const Side& p, const Side& q, bool right, uint32_t block, 
 }
 
 }  // namespace
+
+void mlp_sum(const MlpSums& t) {
+  if (t.count) hipLaunchKernelGGL(k_mlp_sum, dim3(t.blocks), dim3(kT), 0, stream(), t);
+}
 
 bool mlp_forward_parts(const MlpArgs& a) {
   const uint32_t M = pad(a.rows, kTile), C = pad(a.cols, kTile), F = pad(a.hidden, kTile), O = pad(a.out, kTile);
@@ -835,13 +828,16 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
 }
 
 // The parts of the weights are made anew at each call, which few rows do not pay for.
-// Forward and training us on fp32 / on parts: 256 x 1024 x 2816 70 and 212 / 78 and 210, 512 x
-// 512 x 2048 52 and 160 / 60 and 185, 2048 x 256 x 1024 56 and 167 / 54 and 141, 8192 x 128 x
-// 512 74 and 205 / 62 and 182, 200 x 2048 x 8192 323 and 1029 / 235 and 894.
-bool mlp_on_parts(const MlpArgs& a) {
+// Microseconds with fp32 MFMAs / on parts, forward: 256 x 1024 x 2816 63 / 73, 512 x 512 x 2048
+// 49 / 54, 256 x 1024 x 4096 84 / 82, 2048 x 256 x 1024 51 / 49, 8192 x 128 x 512 54 / 44, 200 x
+// 2048 x 8192 313 / 234.  Backward, where fp32 takes longer for its one-wave tiles: 160 x 1024 x
+// 4096 131 / 136, 1024 x 256 x 1024 62 / 70, 150 x 2048 x 8192 508 / 604, 400 x 512 x 2048 101 /
+// 84, 1024 x 384 x 1001 96 / 77, 200 x 2048 x 8192 644 / 611.
+bool mlp_on_parts(const MlpArgs& a, bool backward) {
   // a tile's rows are reached with 32-bit offsets
   if (std::max({a.rows, a.cols, a.hidden, a.out}) > (1u << 21) || std::min({a.rows, a.cols, a.hidden, a.out}) < 32) return false;
-  return (double(a.rows) - 100) * std::sqrt(double(a.cols) * a.out) * a.hidden >= 4.5e8;
+  const double weights = std::sqrt(double(a.cols) * a.out) * a.hidden;
+  return backward ? (double(a.rows) - 140) * weights >= 2.6e8 : (double(a.rows) - 100) * weights >= 4.5e8;
 }
 
 }  // namespace dce

@@ -802,3 +802,11 @@ def test_gated_scan_refuses_what_no_launch_holds(eng):
     for sizes in ((255, 1 << 24, 1), (1, 1 << 30, 3), (2, 1 << 29, 2)):
         assert not lib.GatedScanForward(b, b, None, None, *sizes, None) and "2^30" in eng.last_error(), sizes
         lib.ClearLastError()
+
+
+@pytest.mark.parametrize("size", [(400, 512, 2048, 512), (33, 300, 4100, 70), (20, 2000, 37, 2000), (3000, 1, 1, 1), (5001, 3, 2, 5), (18, 1030, 515, 33),
+                                  (70, 520, 1500, 519), (600, 40, 90, 1)], ids=lambda s: "x".join(map(str, s)))
+def test_gated_mlp_of_shared_depths(eng, size):
+    """Products whose depths waves and workgroups share in all numbers, and a call whose directions are worked out on different paths."""
+    print("gated_mlp", size, flush=True)
+    check_mlp(eng, *size, "silu", rng(sum(size)))
