@@ -442,8 +442,8 @@ __device__ __forceinline__ double block_sum256(double v, double* sh) {
 // ---------------------------------------------------------------------------
 // f = 1 / (1 + e^-z) and k = 1 - f = 1 / (1 + e^z), each within some 3 roundings of its
 // own value, from one exponential and one reciprocal (1 ulp each): e^-|z| = 2^(hi + lo),
-// hi = -|z| log2(e) rounded, lo what that leaves.  (expf and a division take 13
-// microseconds more for 16.8 million gates.)
+// hi = -|z| log2(e) rounded, lo what that leaves.  (With expf and a division the
+// recurrence over 16.8 million gates takes 3 microseconds more forward, 7 backward.)
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void sigmoid_pair(float z, float& f, float& k) {
   const float m = fabsf(z) > 128.f ? 128.f : fabsf(z);  // NaN stays

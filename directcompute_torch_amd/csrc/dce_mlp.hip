@@ -25,10 +25,11 @@ inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b);
 // columns outside are the last ones again; what comes of them is not stored.
 //
 // Bound by memory latency: a wave has four octets of k in flight and then multiplies them,
-// and most calls have a wave or two of each SIMD only.  154 x 384 x 1001 (1 / 6.6 of fp32's
-// MFMA rate): the gate's product 9.6 us, y 6.2 and 3.8 for its sums, the gradient's 9.0, the
-// four others 18.4 and 4.7; 64 x 1024 x 2816, training: 82 us (with eight waves for each
-// tile and no splits 102).  Eight octets in flight, with twice the code, took 10 % more.
+// and most calls have a wave or two of each SIMD only.  154 x 384 x 1001, training
+// (1.07 GFLOP, 7 us at the rate of a large fp32 product): the gate's product 10 us, y 6 and 3
+// for its sums, the gradient's 9, the four others 18.5 and 4; 64 x 1024 x 2816, training: 82
+// us (with eight waves for each tile and no splits 102).  Eight octets in flight, with twice
+// the code, took 10 % more.
 // ---------------------------------------------------------------------------
 enum Op { STORE, GATE, GRAD };
 struct Side {

@@ -154,8 +154,10 @@ __device__ __forceinline__ uint32_t in_turn(uint32_t c, int turn) {
 // 64 rows and 256 columns for each workgroup, 16 rows for each wave.  A width that is
 // no multiple of 4 has its last quad end with the row.  Several such blocks for each, one
 // after the other: of columns where rows alone are wanted (a row's values are brought
-// together once), of rows where columns are and there are many.  (Atomics on one place
-// take some 0.4 us after the other: 8192 x 128, 128 blocks of rows, 53 us.)
+// together once), of rows where columns are and there are many.  The workgroups' largest values go
+// side by side into memory and are brought together by k_mlp_split, for the 128 of its tile.
+// (Atomics on one place take some 0.4 us after the other: 8192 x 128, 128 blocks of rows,
+// 53 us.)  Bound by memory: 84 MB (x and three weights of 8192 x 1024 x 4096) 27 us.
 constexpr uint32_t kMaxRows = 64, kMaxBlocks = 32;
 struct Reach {
   uint32_t rows, cols;  // of a workgroup
@@ -208,7 +210,9 @@ __global__ void __launch_bounds__(kT) k_mlp_max(const Jobs t) {
   J.colPart[size_t(first / by.rows) * J.cols + at] = m;
 }
 
-// A 128 x 128 tile through LDS.
+// A 128 x 128 tile through LDS, for the matrix' rows, its columns, or both at once; a
+// value is 4 bytes as it was.  Bound by memory: of 8192 x 1024 x 4096 84 MB in and 84 out
+// forward, 3.9 TB/s in 43 us.
 __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
   __shared__ __attribute__((aligned(16))) float S0[64 * 128];
   __shared__ __attribute__((aligned(16))) float S1[64 * 128];
@@ -286,6 +290,13 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
 // so that a read of one slot of 16 rows covers the 64 banks once.  The two small
 // products have an accumulator of their own: an MFMA cuts what it adds off at the
 // scale of the largest addend, always downwards.
+//
+// Bound by the MFMAs, for which power holds the clock to 1.7 GHz.  8192 x 1024 x 4096, in us
+// and TFLOP/s of fp32 products (a large fp16 library product, divided by three: 374): g and u 437,
+// 315; y 207, 332; dx, dWd, dWg and dWu 970, 354; dm 400, 172, of which its epilogue, which reads
+// 8 bytes a hidden value and writes 20, takes more than half.  Two workgroups a CU, of 64 KB and
+// some 230 registers a lane.  With one array for both stages every read waited for the loads
+// (2.19 ms for 2.14 of a training pass).
 // ---------------------------------------------------------------------------
 enum Op { STORE, GATE, GRAD };
 struct Prod {

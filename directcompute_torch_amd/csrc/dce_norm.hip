@@ -17,9 +17,9 @@
 // its values are the quad's before it too: they are computed twice, to the same
 // bits, and left out of the sums.
 //
-// Bound by memory.  8192 x 2048, a gate for each channel: forward (16 bytes a value) 43
-// us, 6.3 TB/s; backward (24) 74 us, 5.4 TB/s, and 6 us for the sums over rows.  8191 x
-// 4096 with a gate for each value: 99 and 170 us, 6.8 and 6.3 TB/s.  Passes over more
+// Bound by memory.  8192 x 2048, a gate for each channel: forward (16 bytes a value) 44
+// to 48 us, 6.1 to 5.6 TB/s; backward (24) 74 us, 5.4 TB/s, and 6 us for the sums over rows.  8191 x
+// 4096 with a gate for each value: 97 and 170 us, 6.9 and 6.3 TB/s.  Passes over more
 // than the last cache go past it (nontemporal), which is worth 20 to 25 % there.  The
 // next row's loads ahead of time, and gains held in registers, gained nothing.
 #include "dce_internal.h"

@@ -19,7 +19,7 @@
 // make.  (Every 64th leaves its last state, too, where those after it start: no more
 // than 63 pairs are read.)  So every value moves once: 12 bytes a value forward, 24
 // backward.  4 x 4096
-// tokens of 1024 channels: forward 40 us, 5.0 TB/s, backward 80 us, 5.0 TB/s, with
+// tokens of 1024 channels: forward 42 us, 4.8 TB/s, backward 72 us, 5.6 TB/s, with
 // about a third of that time's vector instructions; the pass that clears the pairs 2 to
 // 4 us each.  (A thread for each channel: 6.0 ms.)
 //
