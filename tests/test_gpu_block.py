@@ -810,3 +810,70 @@ def test_gated_mlp_of_shared_depths(eng, size):
     """Products whose depths waves and workgroups share in all numbers, and a call whose directions are worked out on different paths."""
     print("gated_mlp", size, flush=True)
     check_mlp(eng, *size, "silu", rng(sum(size)))
+
+
+@pytest.mark.parametrize("size", [(20, 12, 16, 10), (150, 40, 70, 36), (700, 512, 1400, 512)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+def test_gated_mlp_gradients_against_differences(eng, act, size):
+    """Along a random direction of all operands, central differences in float64 of
+    the formula: off by what the gradients may be off by, and by step^2 = 1e-8
+    times third derivatives, which are sums of the slope's own terms: 1e-6 of those."""
+    M, C, F, O = size
+    r = rng(M)
+    a = {"x": r.standard_normal((M, C)), "wg": r.standard_normal((C, F)) / math.sqrt(C), "wu": r.standard_normal((C, F)) / math.sqrt(C),
+         "wd": r.standard_normal((F, O)) / math.sqrt(F)}
+    a = {k: v.astype(np.float32) for k, v in a.items()}
+    dy = r.standard_normal((M, O)).astype(np.float32)
+    T = {k: dev(eng, v, True) for k, v in a.items()}
+    eng.gated_mlp(*T.values(), act).backward(dev(eng, dy))
+    way = {k: r.standard_normal(v.shape) / math.sqrt(v.size) for k, v in a.items()}
+
+    def value(s):
+        x, wg, wu, wd = (a[k].astype(np.float64) + s * way[k] for k in a)
+        return (((act64(x @ wg, act)[0] * (x @ wu)) @ wd) * dy).sum()
+    slope = (value(1e-4) - value(-1e-4)) / 2e-4
+    ref = mlp64(*(v.astype(np.float64) for v in a.values()), act, dy.astype(np.float64))
+    terms = {k: T[k].grad.sync().astype(np.float64) * way[k] for k in a}
+    bound = sum((ref["d" + k][1] * np.abs(way[k])).sum() + 1e-6 * np.abs(terms[k]).sum() for k in a)
+    assert abs(sum(t.sum() for t in terms.values()) - slope) <= bound
+    eng.end_batch()
+
+
+def test_the_same_operand_in_two_places(eng):
+    """One matrix as gate and upward weights, one tensor as tokens and gates: the gradients of both places are added up."""
+    r = rng(8)
+    x, w, v, dy = (r.standard_normal(s).astype(np.float32) for s in ((40, 24), (24, 30), (30, 24), (40, 24)))
+    t = [dev(eng, a, True) for a in (x, w, v)]
+    eng.gated_mlp(t[0], t[1], t[1], t[2]).backward(dev(eng, dy))
+    ref = mlp64(*(a.astype(np.float64) for a in (x, w, w, v)), "silu", dy.astype(np.float64))
+    (g, eg), (u, eu) = ref["dwg"], ref["dwu"]
+    within("dw", t[1].grad.sync(), g + u, eg + eu + EPS * np.abs(g + u))
+    x, dy = r.standard_normal((2, 50, 30)).astype(np.float32), r.standard_normal((2, 50, 30)).astype(np.float32)
+    t = dev(eng, x, True)
+    eng.gated_scan(t, t).backward(dev(eng, dy))
+    ref = scan64(x.astype(np.float64), x.astype(np.float64), None, np.full(2, 50), dy.astype(np.float64))
+    (a, ea), (b, eb) = ref["dx"], ref["dz"]
+    within("dx", t.grad.sync(), a + b, ea + eb + EPS * np.abs(a + b))
+    eng.end_batch()
+
+
+@pytest.mark.parametrize("width", [3, 64, 771, 2048, 9001])
+def test_norms_keep_what_is_not_finite_in_its_row(eng, width):
+    r = rng(width)
+    x, b, dh, dn = (r.standard_normal((9, width)).astype(np.float32) for _ in range(4))
+    gate, post, pre = (r.standard_normal(width).astype(np.float32) for _ in range(3))
+
+    def run():
+        T = [dev(eng, v, True) for v in (x, b)]
+        h, n = eng.residual_norm(*T, *(dev(eng, v) for v in (gate, post, pre)))
+        h.grad = dev(eng, dh)
+        n.backward(dev(eng, dn))
+        out = [t.sync().copy() for t in (h, n, T[0].grad, T[1].grad)]
+        eng.end_batch()
+        return out
+    want = run()
+    x[1, 0], b[4, width - 1], dn[7, 1] = np.nan, np.inf, np.nan
+    got = run()
+    keep = [0, 2, 3, 5, 6, 8]
+    assert all(np.array_equal(g[keep], w[keep]) for g, w in zip(got, want))
+    assert np.isnan(got[1][1]).all() and np.isnan(got[2][7]).all()
