@@ -22,12 +22,14 @@ inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b);
 // sums a pass brings together, in order.  No stage in between: an operand whose depth is
 // contiguous comes by 16 bytes a lane, 4 k of its row, the other one by a dword of each k,
 // 32 neighbours together.  The MFMA's two k of a step are then 4 apart, for both.  Rows and
-// columns outside are the last ones again; what comes of them is not stored.
+// columns outside are the last ones again; what comes of them is not stored.  Tiles go down a
+// column first, and those next to each other run on one XCD: rows of odd length share cache
+// lines (100 x 2000 x 8001 forward 226 us without that, 179 with it).
 //
 // Bound by memory latency: a wave has four octets of k in flight and then multiplies them,
 // and most calls have a wave or two of each SIMD only.  154 x 384 x 1001, training
 // (1.07 GFLOP, 7 us at the rate of a large fp32 product): the gate's product 10 us, y 6 and 3
-// for its sums, the gradient's 9, the four others 18.5 and 4; 64 x 1024 x 2816, training: 82
+// for its sums, the gradient's 9, the four others 18.5 and 4; 64 x 1024 x 2816, training: 84
 // us (with eight waves for each tile and no splits 102).  Eight octets in flight, with twice
 // the code, took 10 % more.
 // ---------------------------------------------------------------------------
@@ -39,7 +41,7 @@ struct Side {
 struct Prod {
   Side a, b, b2;   // b2: GATE: Wu; STORE: of the second part
   const float* a2; // STORE: a second part of the depth, as long as the first (null: none)
-  uint32_t depth, start, across, tiles;  // first workgroup; tiles across the columns, in all
+  uint32_t depth, start, down, tiles;  // first workgroup; tiles of a column, in all
   uint32_t waves, splits;  // log2 of the waves that share a tile's depth, workgroups that do
   uint32_t aDeep, bDeep;  // is the depth contiguous
   float *out, *g, *u, *du, *m;
@@ -72,6 +74,11 @@ __device__ __forceinline__ void octet(const float* p, uint32_t pitch, uint32_t o
 }
 
 constexpr int kWaves = 8;
+// Workgroup L of a product's n, such that those next to each other run on one XCD.
+__device__ __forceinline__ uint32_t xcd_place(uint32_t L, uint32_t n) {
+  const uint32_t q = n >> 3, r = n & 7, x = L & 7;
+  return x * q + min(x, r) + (L >> 3);
+}
 template <Op OP, MlpAct ACT>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4, 4))) k_mlp_small(const Prods all) {
   constexpr int NW = kWaves, D = OP == GATE ? 2 : 1;
@@ -82,6 +89,7 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
   const Prod& P = all.p[which];
   id -= P.start;
   const uint32_t each = NW >> P.waves, groups = (P.tiles + each - 1) >> (3 - P.waves);  // tiles of a workgroup
+  id = xcd_place(id, groups * P.splits);
   const uint32_t sp = id / groups, first = (id - sp * groups) * each;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -91,7 +99,7 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
   for (int d = 0; d < D; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
-  const uint32_t ti = tile / P.across, tj = tile - ti * P.across;
+  const uint32_t tj = tile / P.down, ti = tile - tj * P.down;
   const uint32_t ar = min(ti * 32 + col, P.a.n - 1), bc = min(tj * 32 + col, P.b.n - 1);
   const uint32_t octets = P.depth / 8, few = octets / shares, more = octets - few * shares;
   const uint32_t lo = share * few + min(share, more), hi = lo + few + (share < more);
@@ -101,7 +109,7 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
   bool in[2];
   float g[2], u[2];
   auto at_of = [&](uint32_t i) __attribute__((always_inline)) {
-    const uint32_t now = min(first + i, P.tiles - 1), ni = now / P.across, nj = now - ni * P.across;
+    const uint32_t now = min(first + i, P.tiles - 1), nj = now / P.down, ni = now - nj * P.down;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t t = threadIdx.x + h * NW * 64, r = ni * 32 + t / 32, c = nj * 32 + t % 32;
@@ -231,8 +239,8 @@ size_t share(Prods& t, bool split) {
   auto octets = [](const Prod& p) { return (p.a2 ? 2.0 : 1.0) * p.depth / 8; };
   for (uint32_t i = 0; i < t.count; ++i) {
     Prod& p = t.p[i];
-    p.across = cdiv(p.b.n, 32);
-    p.tiles = cdiv(p.a.n, 32) * p.across;
+    p.down = cdiv(p.a.n, 32);
+    p.tiles = p.down * cdiv(p.b.n, 32);
     all += p.tiles * octets(p);
   }
   const double most = std::max(1.0, all / 4096);

@@ -9,7 +9,8 @@
 // columns the exponents cost its loop nothing.  A matrix that is summed over its rows
 // in one product and over its columns in another is split twice, with exponents each way.
 //
-// For x, dy and the weights a pass finds the maxima and another makes the parts.  What a
+// For x, dy and the weights a pass finds the maxima and another makes the parts; for Wg and Wu
+// of a forward with few rows the second does both, tile by tile.  What a
 // product leaves for the next one (m forward; dg, du, m backward) is split by its
 // epilogue, which knows the largest value of its own tile's rows and columns only: the
 // parts get that exponent, kept in a byte per row and tile, and the next product's loop
@@ -98,8 +99,12 @@ __device__ __forceinline__ void put_rows(float* S0, float* S1, const Side& t, ui
     }
   }
 }
-// Parts of a 128 x 128 tile's columns, likewise, at row c0 and value r0 of t.
-__device__ __forceinline__ void put_columns(float* S0, float* S1, const Side& t, uint32_t r0, uint32_t c0) {
+// A column's place in a side where it lies in turn with those of another matrix.
+__device__ __forceinline__ uint32_t in_turn(uint32_t c, int turn) {
+  return turn < 0 ? c : (c >> 5) * 64 + uint32_t(turn) * 32 + (c & 31);
+}
+// Parts of a 128 x 128 tile's columns, likewise, at row c0 (in turn) and value r0 of t.
+__device__ __forceinline__ void put_columns(float* S0, float* S1, const Side& t, uint32_t r0, uint32_t c0, int turn = -1) {
   for (int u = threadIdx.x; u < 128 * 16; u += kT) {
     const int c = u / 16, o = u % 16;
     const float* p = tile_at<128>(S0, S1, 8 * o, c);
@@ -110,11 +115,11 @@ __device__ __forceinline__ void put_columns(float* S0, float* S1, const Side& t,
       m = fmaxf(m, size_of(v[e]));
     }
     m = group8_reduce(m, OpMaxR());
-    const uint32_t bits = __float_as_uint(fmaxf(m, xl::dpp<xl::kRowMirror>(m)));
-    put8(t.p + size_t(c0 + c) * t.depth, r0 + 8 * o, v, pow2(exp_of(field_of(bits))));
+    const uint32_t bits = __float_as_uint(fmaxf(m, xl::dpp<xl::kRowMirror>(m))), row = in_turn(c0 + c, turn);
+    put8(t.p + size_t(row) * t.depth, r0 + 8 * o, v, pow2(exp_of(field_of(bits))));
     if (o == 0) {
-      t.field[size_t(r0 / 128) * t.rows + c0 + c] = uint8_t(field_of(bits));
-      if (bits) atomicMax(t.top + c0 + c, bits);
+      t.field[size_t(r0 / 128) * t.rows + row] = uint8_t(field_of(bits));
+      if (bits) atomicMax(t.top + row, bits);
     }
   }
 }
@@ -128,6 +133,7 @@ struct Job {
   Side straight, across;  // of its rows, of its columns; p null: not wanted
   uint32_t c0;            // straight: the place of its columns
   int turn;               // across: 0, 1: its columns are those of Wg, Wu in turn; -1: no
+  // (None where `across` has exponents of its blocks.)
   // Bits of the largest values of the rows in each workgroup's columns, [..][rows], and of
   // the columns in each one's rows, [..][cols]: `rowFrom` with those of the job that shares
   // the exponents (Wg and Wu have one for each row).
@@ -147,9 +153,6 @@ __device__ __forceinline__ int find_job(const Jobs& t, uint32_t blk) {
   int i = 0;
   while (i + 1 < int(t.count) && t.start[i + 1] <= blk) ++i;
   return i;
-}
-__device__ __forceinline__ uint32_t in_turn(uint32_t c, int turn) {
-  return turn < 0 ? c : (c >> 5) * 64 + uint32_t(turn) * 32 + (c & 31);
 }
 // 64 rows and 256 columns for each workgroup, 16 rows for each wave.  A width that is
 // no multiple of 4 has its last quad end with the row.  Several such blocks for each, one
@@ -210,8 +213,8 @@ __global__ void __launch_bounds__(kT) k_mlp_max(const Jobs t) {
   J.colPart[size_t(first / by.rows) * J.cols + at] = m;
 }
 
-// A 128 x 128 tile through LDS, for the matrix' rows, its columns, or both at once; a
-// value is 4 bytes as it was.  Bound by memory: of 8192 x 1024 x 4096 84 MB in and 84 out
+// A 128 x 128 tile through LDS, for the matrix' rows, its columns, or both at once, with
+// the exponents of the rows and columns, or for the columns with those of the tile; a value is 4 bytes as it was.  Bound by memory: of 8192 x 1024 x 4096 84 MB in and 84 out
 // forward, 3.9 TB/s in 43 us.
 __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
   __shared__ __attribute__((aligned(16))) float S0[64 * 128];
@@ -221,7 +224,8 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
   const uint32_t tc = (J.cols + 127) / 128, id = blockIdx.x - t.start[k], i0 = id / tc * 128, j0 = id % tc * 128;
   // The rows' and columns' largest values; tiles at the edge leave them for the products.
   __shared__ uint32_t tops[256];
-  {
+  const bool own = J.across.field;
+  if (!own) {
     const uint32_t l = threadIdx.x & 127, r = i0 + l, c = j0 + l;
     uint32_t m = 0;
     if (threadIdx.x < 128) {
@@ -258,6 +262,10 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
     }
   }
   __syncthreads();
+  if (own) {
+    put_columns(S0, S1, J.across, i0, j0, J.turn);
+    return;
+  }
   if (J.straight.p) {
     for (int u = threadIdx.x; u < 128 * 16; u += kT) {
       const int rl = u / 16, cl = u % 16 * 8;
@@ -298,7 +306,7 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
 // some 230 registers a lane.  With one array for both stages every read waited for the loads
 // (2.19 ms for 2.14 of a training pass).
 // ---------------------------------------------------------------------------
-enum Op { STORE, GATE, GRAD };
+enum Op { STORE, GATE, BLOCK_GATE, GRAD };  // BLOCK_GATE: the weights' parts have exponents of their blocks
 struct Prod {
   Side p, q;
   uint32_t right;          // STORE: the side whose parts have exponents of their blocks is q, not p
@@ -339,7 +347,7 @@ __device__ __forceinline__ _Float16 down(int d) { return _Float16(ldexpf(1.f, -d
 
 template <Op OP, MlpAct ACT, int N, bool NT>
 __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_mlp_product(const Prods<N> all) {
-  constexpr bool SCALED = OP == STORE;
+  constexpr bool SCALED = OP == STORE || OP == BLOCK_GATE;
   const uint32_t place = xcd_block_id();
   int which = 0;
   if constexpr (N > 1)
@@ -373,7 +381,7 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
 #pragma unroll
       for (int e = 0; e < 16; ++e) big[i][j][e] = small[i][j][e] = 0.f;
   // The scaled side's rows of this lane: their own exponent field, and the blocks'.
-  const bool right = SCALED && a.right;
+  const bool right = OP == BLOCK_GATE || (SCALED && a.right);
   const Side& sc = right ? a.q : a.p;
   const uint32_t srow = (right ? tj * kTile + wn : ti * kTile + wm) + col;
   int own[2] = {};
@@ -450,6 +458,8 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
   };
   if constexpr (!SCALED)
     loop(std::integral_constant<int, -1>{});
+  else if constexpr (OP == BLOCK_GATE)
+    loop(std::integral_constant<int, 1>{});
   else if (right)
     loop(std::integral_constant<int, 1>{});
   else
@@ -482,7 +492,7 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
         }
       }
   }
-  if constexpr (OP == GATE) {
+  if constexpr (OP == GATE || OP == BLOCK_GATE) {
     const uint32_t f = ((c0 + wn) >> 1) + col;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -607,8 +617,16 @@ struct Plan {
     int turn;
   };
   Source sources[kJobs];
+  uint32_t maxima = 0;  // the first so many have a pass over their largest values
+  bool blocks(const Side* s) const {
+    for (int i = 0; i < count; ++i)
+      if (all[i].s == s) return all[i].field != ~size_t(0);
+    return false;
+  }
   void add(const float* src, uint32_t rows, uint32_t cols, const Side* straight, const Side* across, uint32_t c0 = 0, int turn = -1) {
     sources[jobs.count++] = {src, rows, cols, straight, across, c0, turn};
+    if (across && blocks(across)) return;
+    maxima = jobs.count;
     const Reach by = reach(rows, across);
     if (straight) parts += size_t(cdiv(cols, by.cols)) * rows;
     if (across) parts += size_t(cdiv(rows, by.rows)) * cols;
@@ -638,6 +656,7 @@ struct Plan {
       if (f.across) j.across = *f.across;
       j.c0 = f.c0;
       j.turn = f.turn;
+      if (j.across.field) continue;
       const Reach by = reach(f.rows, f.across);
       if (f.straight) {
         const uint32_t n = cdiv(f.cols, by.cols);
@@ -662,14 +681,18 @@ struct Plan {
   }
 };
 
-bool run_jobs(Jobs& t) {
+// The first `maxima` of the jobs, which take their largest values beforehand, come first.
+bool run_jobs(Jobs& t, uint32_t maxima) {
   uint32_t n = 0;
-  for (uint32_t i = 0; i < t.count; ++i) {
+  for (uint32_t i = 0; i < maxima; ++i) {
     t.start[i] = n;
     const Reach by = reach(t.j[i].rows, t.j[i].across.p);
     n += cdiv(t.j[i].rows, by.rows) * cdiv(t.j[i].cols, by.cols);
   }
+  const uint32_t count = t.count;
+  t.count = maxima;
   hipLaunchKernelGGL(k_mlp_max, dim3(n), dim3(kT), 0, stream(), t);
+  t.count = count;
   if (!check_launch("gated_mlp")) return false;
   n = 0;
   for (uint32_t i = 0; i < t.count; ++i) {
@@ -749,14 +772,19 @@ bool mlp_forward_parts(const MlpArgs& a) {
   const uint32_t M = pad(a.rows, kTile), C = pad(a.cols, kTile), F = pad(a.hidden, kTile), O = pad(a.out, kTile);
   Plan plan;
   Side x{}, w{}, d{}, m{};
+  // A pass over the weights' largest values less, and exponents of their blocks in the product's
+  // loop: worth it for few rows (forward us with and without the pass, 200 x 2048 x 8192 240 and
+  // 208, 700 x 1024 x 4096 117 and 116, 4096 x 1024 x 2816 263 and 266, 8192 x 1024 x 4096 640
+  // and 650).
+  const bool blocks = a.rows <= 2048;
   plan.side(m, M, F, 64);
+  plan.side(w, 2 * F, C, blocks ? 128 : 0);
   plan.side(x, M, C);
-  plan.side(w, 2 * F, C);
   plan.side(d, O, F);
   plan.add(a.x, a.rows, a.cols, &x, nullptr);
+  plan.add(a.wd, a.hidden, a.out, nullptr, &d);
   plan.add(a.wg, a.cols, a.hidden, nullptr, &w, 0, 0);
   plan.add(a.wu, a.cols, a.hidden, nullptr, &w, 0, 1);
-  plan.add(a.wd, a.hidden, a.out, nullptr, &d);
   ProfScope prof("mlp", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
   // The second product's sides get their places with the others.
   Prods<1> t1{}, t2{};
@@ -765,11 +793,12 @@ bool mlp_forward_parts(const MlpArgs& a) {
   if (!plan.lay(split(t2), &part)) return false;
   t2.a[0].p = m;
   t2.a[0].q = d;
-  if (!run_jobs(plan.jobs)) return false;
+  if (!run_jobs(plan.jobs, plan.maxima)) return false;
   t1.count = 1;
   Prod& g = t1.a[0];
   g.p = x;
   g.q = w;
+  g.block = 128;
   g.depth = C;
   g.rows = a.rows;
   g.m = m;
@@ -778,7 +807,9 @@ bool mlp_forward_parts(const MlpArgs& a) {
     g.g = a.saved;
     g.u = a.saved + size_t(a.rows) * a.hidden;
   }
-  return run_products<GATE>(t1, a.act, nullptr, (a.saved ? 12.0 : 4.0) * M * F) && run_products<STORE>(t2, kSilu, part);
+  const double bytes = (a.saved ? 12.0 : 4.0) * M * F;
+  if (!(blocks ? run_products<BLOCK_GATE>(t1, a.act, nullptr, bytes) : run_products<GATE>(t1, a.act, nullptr, bytes))) return false;
+  return run_products<STORE>(t2, kSilu, part);
 }
 
 bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
@@ -819,7 +850,7 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
   float* part;
   if (!plan.lay(split(t2), &part)) return false;
   rest();
-  if (!run_jobs(plan.jobs)) return false;
+  if (!run_jobs(plan.jobs, plan.maxima)) return false;
   Prods<1> t1{};
   t1.count = 1;
   Prod& g = t1.a[0];
@@ -839,16 +870,16 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
 }
 
 // The parts of the weights are made anew at each call, which few rows do not pay for.
-// Microseconds with fp32 MFMAs / on parts, forward: 256 x 1024 x 2816 63 / 73, 512 x 512 x 2048
+// Microseconds with fp32 MFMAs / on parts, forward: 128 x 2048 x 8192 174 / 195, 512 x 512 x 2048
 // 49 / 54, 256 x 1024 x 4096 84 / 82, 2048 x 256 x 1024 51 / 49, 8192 x 128 x 512 54 / 44, 200 x
-// 2048 x 8192 313 / 234.  Backward, where fp32 takes longer for its one-wave tiles: 160 x 1024 x
+// 2048 x 8192 313 / 208.  Backward, where fp32 takes longer for its one-wave tiles: 160 x 1024 x
 // 4096 131 / 136, 1024 x 256 x 1024 62 / 70, 150 x 2048 x 8192 508 / 604, 400 x 512 x 2048 101 /
 // 84, 1024 x 384 x 1001 96 / 77, 200 x 2048 x 8192 644 / 611.
 bool mlp_on_parts(const MlpArgs& a, bool backward) {
   // a tile's rows are reached with 32-bit offsets
   if (std::max({a.rows, a.cols, a.hidden, a.out}) > (1u << 21) || std::min({a.rows, a.cols, a.hidden, a.out}) < 32) return false;
   const double weights = std::sqrt(double(a.cols) * a.out) * a.hidden;
-  return backward ? (double(a.rows) - 140) * weights >= 2.6e8 : (double(a.rows) - 100) * weights >= 4.5e8;
+  return backward ? (double(a.rows) - 140) * weights >= 2.6e8 : (double(a.rows) - 110) * weights >= 4.5e8;
 }
 
 }  // namespace dce
