@@ -9,6 +9,13 @@
 
 namespace dce {
 
+// Workgroup L of a product's n, such that those next to each other run on one XCD, and every XCD
+// has its part of each product of a launch (their depths differ).
+__device__ __forceinline__ uint32_t xcd_place(uint32_t L, uint32_t n) {
+  const uint32_t q = n >> 3, r = n & 7, x = L & 7;
+  return x * q + min(x, r) + (L >> 3);
+}
+
 // act(g), and its derivative d.
 template <MlpAct ACT>
 __device__ __forceinline__ float act_grad(float g, float& d) {

@@ -74,11 +74,6 @@ __device__ __forceinline__ void octet(const float* p, uint32_t pitch, uint32_t o
 }
 
 constexpr int kWaves = 8;
-// Workgroup L of a product's n, such that those next to each other run on one XCD.
-__device__ __forceinline__ uint32_t xcd_place(uint32_t L, uint32_t n) {
-  const uint32_t q = n >> 3, r = n & 7, x = L & 7;
-  return x * q + min(x, r) + (L >> 3);
-}
 template <Op OP, MlpAct ACT>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4, 4))) k_mlp_small(const Prods all) {
   constexpr int NW = kWaves, D = OP == GATE ? 2 : 1;

@@ -348,17 +348,16 @@ __device__ __forceinline__ _Float16 down(int d) { return _Float16(ldexpf(1.f, -d
 template <Op OP, MlpAct ACT, int N, bool NT>
 __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_mlp_product(const Prods<N> all) {
   constexpr bool SCALED = OP == STORE || OP == BLOCK_GATE;
-  const uint32_t place = xcd_block_id();
   int which = 0;
   if constexpr (N > 1)
-    while (which + 1 < int(all.count) && all.a[which + 1].start <= place) ++which;
+    while (which + 1 < int(all.count) && all.a[which + 1].start <= blockIdx.x) ++which;
   const Prod& a = all.a[which];
   // An array for each stage: the compiler then knows that a direct load into one is
   // nothing that a read of the other has to wait for.
   __shared__ __attribute__((aligned(16))) char S0[2 * kStageBytes];
   __shared__ __attribute__((aligned(16))) char S1[2 * kStageBytes];
   // bands of 8 rows of tiles: what an XCD runs at once reads few rows of either side
-  uint32_t id = place - a.start, sp = 0, k0 = 0, k1 = a.depth;
+  uint32_t id = xcd_place(blockIdx.x - a.start, a.tm * a.tn * a.splits), sp = 0, k0 = 0, k1 = a.depth;
   if constexpr (OP == STORE) {
     const uint32_t blocks = a.depth / kTile;
     sp = id / (a.tm * a.tn);
