@@ -702,9 +702,9 @@ bool run_jobs(Jobs& t, uint32_t maxima) {
   return check_launch("gated_mlp");
 }
 // Splits of the depths: no workgroup has more than a slot's share of the launch (two a CU),
-// or `kLeast` where that is more (1024 x 1024 x 4096, training: 631 us without splits, 426
-// with 256, 424 with 512, 446 with 2048; 1024 x 512 x 2048: 254, 183, 189, 212).  Floats of
-// their shares.
+// or `kLeast` where that is more (backward us with 256, 512, 1024 and 2048, 1024 x 1024 x 4096
+// 229, 226, 235 and 232, 400 x 512 x 2048 91, 83, 87 and 107, 256 x 1024 x 2816 113, 112, 109 and
+// 126).  Floats of their shares.
 constexpr uint32_t kLeast = 512;
 template <int N>
 size_t split(Prods<N>& t) {
@@ -871,14 +871,14 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
 // The parts of the weights are made anew at each call, which few rows do not pay for.
 // Microseconds with fp32 MFMAs / on parts, forward: 128 x 2048 x 8192 174 / 195, 512 x 512 x 2048
 // 49 / 54, 256 x 1024 x 4096 84 / 82, 2048 x 256 x 1024 51 / 49, 8192 x 128 x 512 54 / 44, 200 x
-// 2048 x 8192 313 / 208.  Backward, where fp32 takes longer for its one-wave tiles: 160 x 1024 x
-// 4096 131 / 136, 1024 x 256 x 1024 62 / 70, 150 x 2048 x 8192 508 / 604, 400 x 512 x 2048 101 /
-// 84, 1024 x 384 x 1001 96 / 77, 200 x 2048 x 8192 644 / 611.
+// 2048 x 8192 313 / 208.  Backward: 64 x 2048 x 8192 278 / 332, 96 of
+// them 345 / 335, 128 x 1024 x 4096 116 / 112, 1024 x 256 x 1024 66 / 71, 4096 x 128 x 512 73 /
+// 74, 400 x 512 x 2048 107 / 83, 1024 x 384 x 1001 100 / 76, 200 x 2048 x 8192 654 / 392.
 bool mlp_on_parts(const MlpArgs& a, bool backward) {
   // a tile's rows are reached with 32-bit offsets
   if (std::max({a.rows, a.cols, a.hidden, a.out}) > (1u << 21) || std::min({a.rows, a.cols, a.hidden, a.out}) < 32) return false;
   const double weights = std::sqrt(double(a.cols) * a.out) * a.hidden;
-  return backward ? (double(a.rows) - 140) * weights >= 2.6e8 : (double(a.rows) - 110) * weights >= 4.5e8;
+  return backward ? (double(a.rows) - 80) * weights >= 2.4e8 : (double(a.rows) - 110) * weights >= 4.5e8;
 }
 
 }  // namespace dce
