@@ -29,9 +29,10 @@ inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b);
 // Bound by memory latency: a wave has four octets of k in flight and then multiplies them,
 // and most calls have a wave or two of each SIMD only.  154 x 384 x 1001, training
 // (1.07 GFLOP, 7 us at the rate of a large fp32 product): the gate's product 10 us, y 6 and 3
-// for its sums, the gradient's 9, the four others 18.5 and 4; 64 x 1024 x 2816, training: 84
+// for its sums, the gradient's 9, the four others 18.5 and 4; 64 x 1024 x 2816, training: 81
 // us (with eight waves for each tile and no splits 102).  Eight octets in flight, with twice
-// the code, took 10 % more.
+// the code, took 10 % more.  Of many rows of large weights (64 x 2048 x 8192: each weights' gradient
+// 44 us, 49 TFLOP/s) the reads of 32 x 32 tiles from L2 bound it.
 // ---------------------------------------------------------------------------
 enum Op { STORE, GATE, GRAD };
 struct Side {
@@ -171,13 +172,23 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
   };
   pass(P.a.p, P.b.p, P.b2.p);
   if (OP == STORE && P.a2) pass(P.a2, P.b2.p, nullptr);
+  float* out = P.out + (OP == STORE ? size_t(sp) * P.a.n * P.b.n : 0);
+  if (OP == STORE && P.waves == 0) {  // nothing to add up (24 x 2048 x 8192 training 204 us through LDS, 186 without)
+    const uint32_t c = tj * 32 + col;
+    if (first + w >= P.tiles || c >= P.b.n) return;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint32_t r = ti * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+      if (r < P.a.n) out[size_t(r) * P.b.n + c] = acc[0][e];
+    }
+    return;
+  }
 #pragma unroll
   for (int d = 0; d < D; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) S[d][w][(8 * (e >> 2) + 4 * half + (e & 3)) * 32 + col] = acc[d][e];
   __syncthreads();
   // The waves' sums, a thread two values of each tile.
-  float* out = P.out + (OP == STORE ? size_t(sp) * P.a.n * P.b.n : 0);
   for (uint32_t i = 0; i < each; ++i) {
     if (i) at_of(i);
     float v[2][D];
