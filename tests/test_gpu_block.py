@@ -877,3 +877,45 @@ def test_norms_keep_what_is_not_finite_in_its_row(eng, width):
     keep = [0, 2, 3, 5, 6, 8]
     assert all(np.array_equal(g[keep], w[keep]) for g, w in zip(got, want))
     assert np.isnan(got[1][1]).all() and np.isnan(got[2][7]).all()
+
+
+@pytest.mark.parametrize("rows", [6, 40, 600, 1400, 2300])
+def test_gated_mlp_recorded(eng, rows):
+    """A recorded step through each of the block's paths, replayed with a product of
+    another size between the replays, trains as eager steps do, to the last bit."""
+    C, F, classes = 512, 1024, 7
+    r = rng(rows)
+    P0 = {n: (r.standard_normal(s) / math.sqrt(s[0])).astype(np.float32)
+          for n, s in (("wg", (C, F)), ("wu", (C, F)), ("wd", (F, C)), ("head", (C, classes)))}
+    P0["gain"] = np.ones(C, np.float32)
+    data = [(r.standard_normal((rows, C)).astype(np.float32), r.integers(0, classes, rows).astype(np.float32)) for _ in range(4)]
+
+    def model(P, x):
+        return eng.matmul(eng.residual_norm(x, eng.gated_mlp(x, P["wg"], P["wu"], P["wd"]), pre=P["gain"])[1], P["head"])
+
+    def fresh():
+        P = {n: dev(eng, a, True) for n, a in P0.items()}
+        return P, eng.AdamW(list(P.values()), lr=0.01)
+    P, opt = fresh()
+    losses = []
+    for x, y in data:
+        opt.zero_grad()
+        loss = eng.softmax_ce(model(P, dev(eng, x)), dev(eng, y))
+        loss.backward()
+        opt.step(clip=1.0)
+        losses.append(float(loss.sync()[0]))
+        eng.end_batch()
+    want = {n: t.sync().copy() for n, t in P.items()}
+    P, opt = fresh()
+    graph = eng.ComputeGraph()
+    graph.trace(lambda x: model(P, x), opt, *data[0], list(P.values()), clip=1.0)
+    for i, (x, y) in enumerate(data[1:]):
+        graph.replay(x, y)
+        a = [dev(eng, r.standard_normal(s), True) for s in ((rows + 300, 400), (400, 500), (400, 500), (500, 400))]
+        eng.gated_mlp(*a).backward(a[0])
+        assert graph.read_loss() == losses[i + 1], i
+        eng.end_batch()
+    for n, t in P.items():
+        assert np.array_equal(t.sync(), want[n]), n
+    graph.release()
+    eng.end_batch()
