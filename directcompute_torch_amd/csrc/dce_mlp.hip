@@ -17,7 +17,7 @@ inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b);
 
 // ---------------------------------------------------------------------------
 // Products of small calls on fp32 MFMAs, C[r][c] = sum over k of A(r, k) B(c, k), in
-// tiles of 32 x 32.  1, 2, 4 or 8 of a workgroup's eight waves share a tile's depth and add
+// tiles of 32 x 32 (T = 1), or 64 x 64 of large ones (T = 2).  1, 2, 4 or 8 of a workgroup's eight waves share a tile's depth and add
 // up their sums in LDS, in order; of a deep product with few tiles workgroups do, too, whose
 // sums a pass brings together, in order.  No stage in between: an operand whose depth is
 // contiguous comes by 16 bytes a lane, 4 k of its row, the other one by a dword of each k,
@@ -31,8 +31,8 @@ inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b);
 // (1.07 GFLOP, 7 us at the rate of a large fp32 product): the gate's product 10 us, y 6 and 3
 // for its sums, the gradient's 9, the four others 18.5 and 4; 64 x 1024 x 2816, training: 81
 // us (with eight waves for each tile and no splits 102).  Eight octets in flight, with twice
-// the code, took 10 % more.  Of many rows of large weights (64 x 2048 x 8192: each weights' gradient
-// 44 us, 49 TFLOP/s) the reads of 32 x 32 tiles from L2 bound it.
+// the code, took 10 % more.  Of many rows of large weights (96 x 2048 x 8192 training: 500
+// us, 58 TFLOP/s) reads from L2 bound it.
 // ---------------------------------------------------------------------------
 enum Op { STORE, GATE, GRAD };
 struct Side {
@@ -49,7 +49,7 @@ struct Prod {
 };
 struct Prods {
   Prod p[4];
-  uint32_t count;
+  uint32_t count, side;  // side of a tile, in 32
 };
 
 // Octet o of the depth, k = 8 o + 4 half + i; WHOLE: all of it is there, else zeros past the
@@ -75,8 +75,8 @@ __device__ __forceinline__ void octet(const float* p, uint32_t pitch, uint32_t o
 }
 
 constexpr int kWaves = 8;
-template <Op OP, MlpAct ACT>
-__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4, 4))) k_mlp_small(const Prods all) {
+template <Op OP, MlpAct ACT, int T>
+__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(T == 2 ? 2 : 4, T == 2 ? 2 : 4))) k_mlp_small(const Prods all) {
   constexpr int NW = kWaves, D = OP == GATE ? 2 : 1;
   __shared__ float S[D][NW][32 * 32];
   uint32_t id = blockIdx.x;
@@ -90,25 +90,34 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t tile = min(first + (w >> P.waves), P.tiles - 1), share = (sp << P.waves) + (w & ((1u << P.waves) - 1)), shares = P.splits << P.waves;
-  f16v acc[D];
+  static_assert(T == 1 || OP == STORE);
+  constexpr int N = D * T;  // blocks side by side
+  f16v acc[T][N];
 #pragma unroll
-  for (int d = 0; d < D; ++d)
+  for (int t = 0; t < T; ++t)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[t][d][e] = 0.f;
   const uint32_t tj = tile / P.down, ti = tile - tj * P.down;
-  const uint32_t ar = min(ti * 32 + col, P.a.n - 1), bc = min(tj * 32 + col, P.b.n - 1);
+  uint32_t ar[T], bc[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    ar[t] = min((ti * T + t) * 32 + col, P.a.n - 1);
+    bc[t] = min((tj * T + t) * 32 + col, P.b.n - 1);
+  }
   const uint32_t octets = P.depth / 8, few = octets / shares, more = octets - few * shares;
   const uint32_t lo = share * few + min(share, more), hi = lo + few + (share < more);
   const bool tail = P.depth % 8 && share + 1 == shares;
-  // This thread's places in the group's tile i; GRAD: g and u there, the first ones' ahead of the product.
+  // This thread's places in block (bi, bj) of the group's tile i; GRAD: g and u there, the first ones' ahead of the product.
   size_t at[2];
   bool in[2];
   float g[2], u[2];
-  auto at_of = [&](uint32_t i) __attribute__((always_inline)) {
+  auto at_of = [&](uint32_t i, int bi, int bj) __attribute__((always_inline)) {
     const uint32_t now = min(first + i, P.tiles - 1), nj = now / P.down, ni = now - nj * P.down;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t t = threadIdx.x + h * NW * 64, r = ni * 32 + t / 32, c = nj * 32 + t % 32;
+      const uint32_t t = threadIdx.x + h * NW * 64, r = (ni * T + bi) * 32 + t / 32, c = (nj * T + bj) * 32 + t % 32;
       in[h] = first + i < P.tiles && r < P.a.n && c < P.b.n;
       at[h] = in[h] ? size_t(r) * P.b.n + c : 0;
       if constexpr (OP == GRAD) {
@@ -117,25 +126,33 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
       }
     }
   };
-  at_of(0);
+  if (OP == GRAD) at_of(0, 0, 0);
   auto run = [&](auto aDeep, auto bDeep, const float* a, const float* b, const float* b2) __attribute__((always_inline)) {
     constexpr bool AD = decltype(aDeep)::value, BD = decltype(bDeep)::value;
-    const uint32_t ao = (AD ? ar * P.a.pitch + 4 * half : 4 * half * P.a.pitch + ar) * 4;
-    const uint32_t bo = (BD ? bc * P.b.pitch + 4 * half : 4 * half * P.b.pitch + bc) * 4;
-    constexpr int U = 4;  // octets in flight
-    float x[U][4], y[U][4], z[D == 2 ? U : 1][4];
+    uint32_t ao[T], bo[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      ao[t] = (AD ? ar[t] * P.a.pitch + 4 * half : 4 * half * P.a.pitch + ar[t]) * 4;
+      bo[t] = (BD ? bc[t] * P.b.pitch + 4 * half : 4 * half * P.b.pitch + bc[t]) * 4;
+    }
+    constexpr int U = 4 / T;  // octets in flight
+    float x[U][T][4], y[U][N][4];
     auto mul = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        acc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j][i], y[j][i], acc[0], 0, 0, 0);
-        if constexpr (D == 2) acc[D - 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j][i], z[D == 2 ? j : 0][i], acc[D - 1], 0, 0, 0);
-      }
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int d = 0; d < N; ++d) acc[t][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j][t][i], y[j][d][i], acc[t][d], 0, 0, 0);
     };
     uint32_t o = lo;
     auto fetch = [&](int j, uint32_t at) __attribute__((always_inline)) {
-      octet<AD, true>(a, P.a.pitch, ao, at, P.depth, half, x[j]);
-      octet<BD, true>(b, P.b.pitch, bo, at, P.depth, half, y[j]);
-      if constexpr (D == 2) octet<BD, true>(b2, P.b.pitch, bo, at, P.depth, half, z[D == 2 ? j : 0]);
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        octet<AD, true>(a, P.a.pitch, ao[t], at, P.depth, half, x[j][t]);
+        octet<BD, true>(b, P.b.pitch, bo[t], at, P.depth, half, y[j][t]);
+      }
+      if constexpr (D == 2) octet<BD, true>(b2, P.b.pitch, bo[0], at, P.depth, half, y[j][N - 1]);
     };
     for (; o + U <= hi; o += U) {
 #pragma unroll
@@ -143,7 +160,7 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
 #pragma unroll
       for (int j = 0; j < U; ++j) mul(j);
     }
-    if (o < hi) {  // up to three more
+    if (o < hi) {  // fewer
 #pragma unroll
       for (int j = 0; j < U - 1; ++j) fetch(j, min(o + j, hi - 1));
       mul(0);
@@ -152,9 +169,12 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
         if (o + j < hi) mul(j);
     }
     if (tail) {
-      octet<AD, false>(a, P.a.pitch, ao, octets, P.depth, half, x[0]);
-      octet<BD, false>(b, P.b.pitch, bo, octets, P.depth, half, y[0]);
-      if constexpr (D == 2) octet<BD, false>(b2, P.b.pitch, bo, octets, P.depth, half, z[0]);
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        octet<AD, false>(a, P.a.pitch, ao[t], octets, P.depth, half, x[0][t]);
+        octet<BD, false>(b, P.b.pitch, bo[t], octets, P.depth, half, y[0][t]);
+      }
+      if constexpr (D == 2) octet<BD, false>(b2, P.b.pitch, bo[0], octets, P.depth, half, y[0][N - 1]);
       mul(0);
     }
   };
@@ -174,60 +194,69 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
   if (OP == STORE && P.a2) pass(P.a2, P.b2.p, nullptr);
   float* out = P.out + (OP == STORE ? size_t(sp) * P.a.n * P.b.n : 0);
   if (OP == STORE && P.waves == 0) {  // nothing to add up (24 x 2048 x 8192 training 204 us through LDS, 186 without)
-    const uint32_t c = tj * 32 + col;
-    if (first + w >= P.tiles || c >= P.b.n) return;
+    if (first + w >= P.tiles) return;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const uint32_t r = ti * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
-      if (r < P.a.n) out[size_t(r) * P.b.n + c] = acc[0][e];
-    }
-    return;
-  }
+    for (int bi = 0; bi < T; ++bi)
 #pragma unroll
-  for (int d = 0; d < D; ++d)
+      for (int bj = 0; bj < T; ++bj) {
+        const uint32_t c = (tj * T + bj) * 32 + col;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) S[d][w][(8 * (e >> 2) + 4 * half + (e & 3)) * 32 + col] = acc[d][e];
-  __syncthreads();
-  // The waves' sums, a thread two values of each tile.
-  for (uint32_t i = 0; i < each; ++i) {
-    if (i) at_of(i);
-    float v[2][D];
-    auto sum = [&](auto waves) __attribute__((always_inline)) {
-      constexpr int N = decltype(waves)::value;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int d = 0; d < D; ++d) {
-          v[h][d] = 0.f;
-#pragma unroll
-          for (int n = 0; n < N; ++n) v[h][d] += S[d][i * N + n][threadIdx.x + h * NW * 64];
-        }
-    };
-    if (P.waves == 3)
-      sum(std::integral_constant<int, 8>{});
-    else if (P.waves == 2)
-      sum(std::integral_constant<int, 4>{});
-    else if (P.waves == 1)
-      sum(std::integral_constant<int, 2>{});
-    else
-      sum(std::integral_constant<int, 1>{});
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (!in[h]) continue;
-      if constexpr (OP == STORE) out[at[h]] = v[h][0];
-      if constexpr (OP == GATE) {
-        out[at[h]] = act<ACT>(v[h][0]) * v[h][D - 1];
-        if (P.g) {
-          P.g[at[h]] = v[h][0];
-          P.u[at[h]] = v[h][D - 1];
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t r = (ti * T + bi) * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+          if (r < P.a.n && c < P.b.n) out[size_t(r) * P.b.n + c] = acc[bi][bj][e];
         }
       }
-      if constexpr (OP == GRAD) {
-        float d;
-        const float y = act_grad<ACT>(g[h], d);
-        out[at[h]] = v[h][0] * u[h] * d;
-        P.du[at[h]] = v[h][0] * y;
-        P.m[at[h]] = y * u[h];
+    return;
+  }
+  // The waves' sums, block by block, a thread two values of each tile's.
+#pragma unroll
+  for (int b = 0; b < T * T; ++b) {
+    if (b) __syncthreads();
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) S[d][w][(8 * (e >> 2) + 4 * half + (e & 3)) * 32 + col] = acc[b / T][D == 2 ? d : b % T][e];
+    __syncthreads();
+    for (uint32_t i = 0; i < each; ++i) {
+      if (OP != GRAD || i || b) at_of(i, b / T, b % T);
+      float v[2][D];
+      auto sum = [&](auto waves) __attribute__((always_inline)) {
+        constexpr int W = decltype(waves)::value;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int d = 0; d < D; ++d) {
+            v[h][d] = 0.f;
+#pragma unroll
+            for (int n = 0; n < W; ++n) v[h][d] += S[d][i * W + n][threadIdx.x + h * NW * 64];
+          }
+      };
+      if (P.waves == 3)
+        sum(std::integral_constant<int, 8>{});
+      else if (P.waves == 2)
+        sum(std::integral_constant<int, 4>{});
+      else if (P.waves == 1)
+        sum(std::integral_constant<int, 2>{});
+      else
+        sum(std::integral_constant<int, 1>{});
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (!in[h]) continue;
+        if constexpr (OP == STORE) out[at[h]] = v[h][0];
+        if constexpr (OP == GATE) {
+          out[at[h]] = act<ACT>(v[h][0]) * v[h][D - 1];
+          if (P.g) {
+            P.g[at[h]] = v[h][0];
+            P.u[at[h]] = v[h][D - 1];
+          }
+        }
+        if constexpr (OP == GRAD) {
+          float d;
+          const float y = act_grad<ACT>(g[h], d);
+          out[at[h]] = v[h][0] * u[h] * d;
+          P.du[at[h]] = v[h][0] * y;
+          P.m[at[h]] = y * u[h];
+        }
       }
     }
   }
@@ -240,14 +269,22 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
 // 20 x 2048 x 8192 384 and 205, 40 x 512 x 2048 67 and 44, 154 x 384 x 1001 54 and 46; from
 // twice the share on, 300 x 256 x 512 35 for 33).
 size_t share(Prods& t, bool split) {
-  double all = 0;
   size_t floats = 0;
   auto octets = [](const Prod& p) { return (p.a2 ? 2.0 : 1.0) * p.depth / 8; };
+  auto work = [&](uint32_t side) {  // of blocks of 32 x 32
+    double all = 0;
+    for (uint32_t i = 0; i < t.count; ++i) all += double(cdiv(t.p[i].a.n, 32 * side)) * cdiv(t.p[i].b.n, 32 * side) * side * side * octets(t.p[i]);
+    return all;
+  };
+  // Tiles of 64 x 64, which halve the reads and are a quarter as many, from 64 octets of 32 x 32 for each
+  // wave on, unless their edges are much more (training us with 32 and 64, 48 x 2048 x 8192 323 and
+  // 284, 64 of them 344 and 311; from 16 octets on 64 x 1024 x 2816 89 for 81).
+  t.side = split && work(1) >= 4096 * 64 && work(2) <= 1.15 * work(1) ? 2 : 1;
+  const double all = work(t.side) / (t.side * t.side);
   for (uint32_t i = 0; i < t.count; ++i) {
     Prod& p = t.p[i];
-    p.down = cdiv(p.a.n, 32);
-    p.tiles = p.down * cdiv(p.b.n, 32);
-    all += p.tiles * octets(p);
+    p.down = cdiv(p.a.n, 32 * t.side);
+    p.tiles = p.down * cdiv(p.b.n, 32 * t.side);
   }
   const double most = std::max(1.0, all / 4096);
   for (uint32_t i = 0; i < t.count; ++i) {
@@ -277,7 +314,10 @@ bool run_small(Prods& t, MlpAct act = kSilu, float* part = nullptr) {
   }
   by_act(act, [&](auto k) {
     constexpr MlpAct A = OP == STORE ? kSilu : decltype(k)::value;
-    hipLaunchKernelGGL((k_mlp_small<OP, A>), dim3(n), dim3(kWaves * 64), 0, stream(), t);
+    if (OP == STORE && t.side == 2)
+      hipLaunchKernelGGL((k_mlp_small<OP, A, OP == STORE ? 2 : 1>), dim3(n), dim3(kWaves * 64), 0, stream(), t);
+    else
+      hipLaunchKernelGGL((k_mlp_small<OP, A, 1>), dim3(n), dim3(kWaves * 64), 0, stream(), t);
   });
   mlp_sum(sums);
   return check_launch("gated_mlp");

@@ -919,3 +919,11 @@ def test_gated_mlp_recorded(eng, rows):
         assert np.array_equal(t.sync(), want[n]), n
     graph.release()
     eng.end_batch()
+
+
+@pytest.mark.parametrize("size,need", [((60, 1501, 5003, 1499), ("x", "wg", "wu", "wd")), ((64, 300, 9000, 3800), ()), ((64, 40, 9000, 3801), ("x", "wd"))],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gated_mlp_of_some_tokens_and_many_weights(eng, size, need):
+    """Tiles of 64 x 64, of one wave and of several."""
+    print("gated_mlp some", size, flush=True)
+    check_mlp(eng, *size, "silu", rng(size[0]), need=need)
