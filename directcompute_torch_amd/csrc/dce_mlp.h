@@ -62,11 +62,36 @@ struct MlpSums {
     blocks += uint32_t((uint64_t(n) + 1023) / 1024);
   }
 };
-void mlp_sum(const MlpSums& t);
+// Four values, by thread i (of all blocks').
+__device__ __forceinline__ f4u mlp_sum_of(const MlpSums& t, uint32_t i, int* which, uint32_t* at) {
+  int k = 0;
+  while (k + 1 < int(t.count) && t.s[k + 1].start <= i / 256) ++k;
+  const MlpSums::One& s = t.s[k];
+  const uint64_t first = (uint64_t(i) - s.start * 256ull) * 4;
+  *which = first < s.n ? k : -1;
+  if (*which < 0) return f4u{0.f, 0.f, 0.f, 0.f};
+  // the last quad ends with the matrix; fewer than 4 values there are none
+  *at = min(uint32_t(first), s.n - 4);
+  f4u v = ldus<false, f4u>(s.part + *at);
+#pragma unroll 4
+  for (uint32_t j = 1; j < s.splits; ++j) v += ldus<false, f4u>(s.part + size_t(j) * s.n + *at);
+  return v;
+}
 
 // On fp16 parts, for large calls.
 bool mlp_on_parts(const MlpArgs& a, bool backward);
 bool mlp_forward_parts(const MlpArgs& a);
 bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd);
+
+// Their last launch: the splits' sums, and on fp32 what parts do not hold.
+struct MlpAgain {
+  uint32_t* any;      // of these all are zeros at first; set with any of `rows`, or for all gradients
+  uint32_t* rows;     // forward: the results' rows that are wanted
+  uint32_t* counts;   // two words: places taken, first products done
+  float* ws;          // rows x hidden floats, or mlp_again_floats
+};
+bool mlp_forward_again(const MlpArgs& a, const MlpAgain& g, const MlpSums& sums);
+size_t mlp_again_floats(const MlpArgs& a);
+bool mlp_backward_again(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd, const MlpAgain& g, const MlpSums& sums);
 
 }  // namespace dce

@@ -50,6 +50,7 @@ struct Prod {
 struct Prods {
   Prod p[4];
   uint32_t count, side;  // side of a tile, in 32
+  const uint32_t* again; // AGAIN: set for the rows that are wanted (null: all)
 };
 
 // Octet o of the depth, k = 8 o + 4 half + i; WHOLE: all of it is there, else zeros past the
@@ -75,11 +76,12 @@ __device__ __forceinline__ void octet(const float* p, uint32_t pitch, uint32_t o
 }
 
 constexpr int kWaves = 8;
-template <Op OP, MlpAct ACT, int T>
-__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(T == 2 ? 2 : 4, T == 2 ? 2 : 4))) k_mlp_small(const Prods all) {
+template <Op OP>
+using SumsOf = float[OP == GATE ? 2 : 1][kWaves][32 * 32];
+// Workgroup id of a launch's; sums start at `start`.
+template <Op OP, MlpAct ACT, int T, bool AGAIN>
+__device__ __forceinline__ void small_tiles(const Prods& all, uint32_t id, SumsOf<OP>& S, float start) {
   constexpr int NW = kWaves, D = OP == GATE ? 2 : 1;
-  __shared__ float S[D][NW][32 * 32];
-  uint32_t id = blockIdx.x;
   int which = 0;
   while (which + 1 < int(all.count) && all.p[which + 1].start <= id) ++which;
   const Prod& P = all.p[which];
@@ -88,6 +90,12 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
   id = xcd_place(id, groups * P.splits);
   const uint32_t sp = id / groups, first = (id - sp * groups) * each;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  auto wanted = [&](uint32_t r) { return r < P.a.n && (!AGAIN || !all.again || all.again[r]); };
+  if (AGAIN && all.again) {  // the same in each wave
+    bool any = false;
+    for (uint32_t t = lane; t < each * T * 32; t += 64) any |= wanted(min(first + t / (T * 32), P.tiles - 1) % P.down * (T * 32) + t % (T * 32));
+    if (!__any(any)) return;
+  }
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t tile = min(first + (w >> P.waves), P.tiles - 1), share = (sp << P.waves) + (w & ((1u << P.waves) - 1)), shares = P.splits << P.waves;
   static_assert(T == 1 || OP == STORE);
@@ -98,7 +106,7 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
 #pragma unroll
     for (int d = 0; d < N; ++d)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[t][d][e] = 0.f;
+      for (int e = 0; e < 16; ++e) acc[t][d][e] = start;
   const uint32_t tj = tile / P.down, ti = tile - tj * P.down;
   uint32_t ar[T], bc[T];
 #pragma unroll
@@ -118,7 +126,7 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t t = threadIdx.x + h * NW * 64, r = (ni * T + bi) * 32 + t / 32, c = (nj * T + bj) * 32 + t % 32;
-      in[h] = first + i < P.tiles && r < P.a.n && c < P.b.n;
+      in[h] = first + i < P.tiles && wanted(r) && c < P.b.n;
       at[h] = in[h] ? size_t(r) * P.b.n + c : 0;
       if constexpr (OP == GRAD) {
         g[h] = P.g[at[h]];
@@ -203,7 +211,7 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const uint32_t r = (ti * T + bi) * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
-          if (r < P.a.n && c < P.b.n) out[size_t(r) * P.b.n + c] = acc[bi][bj][e];
+          if (wanted(r) && c < P.b.n) out[size_t(r) * P.b.n + c] = acc[bi][bj][e];
         }
       }
     return;
@@ -262,6 +270,82 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
   }
 }
 
+template <Op OP, MlpAct ACT, int T>
+__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(T == 2 ? 2 : 4, T == 2 ? 2 : 4))) k_mlp_small(const Prods all) {
+  __shared__ SumsOf<OP> S;
+  small_tiles<OP, ACT, T, false>(all, blockIdx.x, S, 0.f);
+}
+
+__global__ void __launch_bounds__(256) k_mlp_sum(const MlpSums t) {
+  int k;
+  uint32_t at;
+  const f4u v = mlp_sum_of(t, blockIdx.x * 256 + threadIdx.x, &k, &at);
+  if (k >= 0) stus<false>(t.s[k].out + at, v);
+}
+void mlp_sum(const MlpSums& t) {
+  if (t.count) hipLaunchKernelGGL(k_mlp_sum, dim3(t.blocks), dim3(256), 0, stream(), t);
+}
+
+// The last launch of a call on parts: adds up the splits' sums, and works out again what the products
+// marked, first m (dg, du and m), then the products of them.  Most often there is nothing marked, and
+// the workgroups beyond those of the sums (all, of a call without splits: 3 us) end at once.  Else they
+// take places one by one: a second product waits for all of the first ones, which have been taken by
+// workgroups that run.
+template <bool BWD>
+struct Again {
+  Prods first, second;
+  MlpSums sums;
+  MlpAgain g;
+  uint32_t sumBlocks, n1, n2;  // workgroups for the sums; places of the first and the second products
+  uint32_t cols;               // of y
+};
+constexpr uint32_t kSpins = 1u << 22;  // a wait's end, should it come to that: the result is then NaN
+template <bool BWD, MlpAct ACT>
+__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4, 4))) k_mlp_again(const Again<BWD> t) {
+  constexpr Op FIRST = BWD ? GRAD : GATE;
+  __shared__ SumsOf<FIRST> S;
+  __shared__ uint32_t mine;
+  const uint32_t any = __hip_atomic_load(t.g.any, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (blockIdx.x < t.sumBlocks) {
+    int k;
+    uint32_t at;
+    const f4u v = mlp_sum_of(t.sums, blockIdx.x * (kWaves * 64) + threadIdx.x, &k, &at);
+    if (k < 0 || (BWD && any)) return;
+    if (!any) {
+      stus<false>(t.sums.s[k].out + at, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (!t.g.rows[(at + e) / t.cols]) t.sums.s[k].out[at + e] = v[e];
+    }
+    return;
+  }
+  if (!any) return;
+  for (;;) {
+    __syncthreads();
+    if (threadIdx.x == 0) mine = __hip_atomic_fetch_add(t.g.counts, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const uint32_t id = __builtin_amdgcn_readfirstlane(mine);
+    if (id >= t.n1 + t.n2) return;
+    if (id < t.n1) {
+      small_tiles<FIRST, ACT, 1, true>(t.first, id, S, 0.f);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+      __syncthreads();
+      if (threadIdx.x == 0) __hip_atomic_fetch_add(t.g.counts + 1, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      continue;
+    }
+    auto done = [&] { return __hip_atomic_load(t.g.counts + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == t.n1; };
+    bool there = done();
+    for (uint32_t spin = 0; !there && spin < kSpins; ++spin) {
+      __builtin_amdgcn_s_sleep(8);
+      there = done();
+    }
+    __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    small_tiles<STORE, kSilu, 1, true>(t.second, id - t.n1, reinterpret_cast<SumsOf<STORE>&>(S), there ? 0.f : NAN);
+  }
+}
+
 // How the products of a launch share their depths, such that every wave has about as many
 // octets (4096 waves are 16 for each CU, all that run at once); floats of what splits leave.
 // More than a workgroup's eight waves for a tile only where each of those would have three times
@@ -298,14 +382,21 @@ size_t share(Prods& t, bool split) {
   }
   return floats;
 }
+// The products' first workgroups, and those of all of them.
+uint32_t lay_out(Prods& t) {
+  uint32_t n = 0;
+  for (uint32_t i = 0; i < t.count; ++i) {
+    t.p[i].start = n;
+    n += cdiv(t.p[i].tiles, kWaves >> t.p[i].waves) * t.p[i].splits;
+  }
+  return n;
+}
 template <Op OP>
 bool run_small(Prods& t, MlpAct act = kSilu, float* part = nullptr) {
-  uint32_t n = 0;
+  const uint32_t n = lay_out(t);
   MlpSums sums{};
   for (uint32_t i = 0; i < t.count; ++i) {
     Prod& p = t.p[i];
-    p.start = n;
-    n += cdiv(p.tiles, kWaves >> p.waves) * p.splits;
     if (p.splits == 1) continue;
     const size_t values = size_t(p.a.n) * p.b.n;
     sums.add(part, p.out, uint32_t(values), p.splits);
@@ -334,51 +425,87 @@ Prod& add(Prods& t, const float* a, uint32_t rows, uint32_t aPitch, bool aDeep, 
   return p;
 }
 
-bool forward_small(const MlpArgs& a) {
-  const size_t n = size_t(a.rows) * a.hidden, at = (n + 63) & ~size_t(63);
-  Prods t{}, y{};
+// Floats of m, or of dg or du.
+size_t third(const MlpArgs& a) { return (size_t(a.rows) * a.hidden + 63) & ~size_t(63); }
+
+// y's product, whose m comes from the gate's.
+Prods down_product(const MlpArgs& a) {
+  Prods y{};
   add(y, nullptr, a.rows, a.hidden, true, a.wd, a.out, a.out, false, a.hidden, a.y);
-  float* m = workspace(at + share(y, true));
-  if (!m) return false;
-  ProfScope prof("mlp", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
+  return y;
+}
+// The gate's, which leaves m.
+Prods gate_product(const MlpArgs& a, float* m) {
+  Prods t{};
   Prod& p = add(t, a.x, a.rows, a.cols, true, a.wg, a.hidden, a.hidden, false, a.cols, m);
   p.b2.p = a.wu;
   p.g = a.saved;
-  p.u = a.saved ? a.saved + n : nullptr;
+  p.u = a.saved ? a.saved + size_t(a.rows) * a.hidden : nullptr;
   share(t, false);
+  return t;
+}
+
+bool forward_small(const MlpArgs& a) {
+  const size_t at = third(a);
+  Prods y = down_product(a);
+  float* m = workspace(at + share(y, true));
+  if (!m) return false;
+  ProfScope prof("mlp", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
+  Prods t = gate_product(a, m);
   if (!run_small<GATE>(t, a.act)) return false;
   y.p[0].a.p = m;
   return run_small<STORE>(y, kSilu, m + at);
 }
 
-bool backward_small(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
-  const size_t n = size_t(a.rows) * a.hidden, at = (n + 63) & ~size_t(63);
-  // Twice: how the products share first, their places once there is a workspace.
-  Prods t{}, r{};
-  auto rest = [&](float* dg) {
-    float *du = dg ? dg + at : nullptr, *m = dg ? du + at : nullptr;
-    r = {};
-    if (dx) {
-      Prod& q = add(r, dg, a.rows, a.hidden, true, a.wg, a.cols, a.hidden, true, a.hidden, dx);
-      q.a2 = dg ? du : a.x;
-      q.b2.p = a.wu;
-    }
-    if (dwd) add(r, m, a.hidden, a.hidden, false, dy, a.out, a.out, false, a.rows, dwd);
-    if (dwg) add(r, a.x, a.cols, a.cols, false, dg, a.hidden, a.hidden, false, a.rows, dwg);
-    if (dwu) add(r, a.x, a.cols, a.cols, false, du, a.hidden, a.hidden, false, a.rows, dwu);
-    return share(r, true);
-  };
-  float* dg = workspace(3 * at + rest(nullptr));
-  if (!dg) return false;
-  rest(dg);
-  ProfScope prof("mlp", 12.0 * a.rows * a.cols * a.hidden, 8.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
+// The four products that follow dm's; dg, du and m lie one after the other, `at` floats each (null: not yet).
+Prods rest_products(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd, float* dg, size_t at) {
+  float *du = dg ? dg + at : nullptr, *m = dg ? du + at : nullptr;
+  Prods r{};
+  if (dx) {
+    Prod& q = add(r, dg, a.rows, a.hidden, true, a.wg, a.cols, a.hidden, true, a.hidden, dx);
+    q.a2 = dg ? du : a.x;
+    q.b2.p = a.wu;
+  }
+  if (dwd) add(r, m, a.hidden, a.hidden, false, dy, a.out, a.out, false, a.rows, dwd);
+  if (dwg) add(r, a.x, a.cols, a.cols, false, dg, a.hidden, a.hidden, false, a.rows, dwg);
+  if (dwu) add(r, a.x, a.cols, a.cols, false, du, a.hidden, a.hidden, false, a.rows, dwu);
+  return r;
+}
+// dm's, which leaves dg, du and m.
+Prods grad_product(const MlpArgs& a, const float* dy, float* dg, size_t at) {
+  Prods t{};
   Prod& p = add(t, dy, a.rows, a.out, true, a.wd, a.hidden, a.out, true, a.out, dg);
   p.g = a.saved;
-  p.u = a.saved + n;
+  p.u = a.saved + size_t(a.rows) * a.hidden;
   p.du = dg + at;
   p.m = p.du + at;
   share(t, false);
+  return t;
+}
+
+bool backward_small(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
+  const size_t at = third(a);
+  // Twice: how the products share first, their places once there is a workspace.
+  Prods r = rest_products(a, dy, dx, dwg, dwu, dwd, nullptr, at);
+  float* dg = workspace(3 * at + share(r, true));
+  if (!dg) return false;
+  r = rest_products(a, dy, dx, dwg, dwu, dwd, dg, at);
+  share(r, true);
+  ProfScope prof("mlp", 12.0 * a.rows * a.cols * a.hidden, 8.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
+  Prods t = grad_product(a, dy, dg, at);
   return run_small<GRAD>(t, a.act) && run_small<STORE>(r, kSilu, dg + 3 * at);
+}
+
+template <bool BWD>
+bool run_again(Again<BWD>& t, MlpAct act) {
+  share(t.second, false);
+  t.first.again = t.second.again = t.g.rows;
+  t.n1 = lay_out(t.first);
+  t.n2 = lay_out(t.second);
+  t.sumBlocks = (t.sums.blocks + 1) / 2;
+  const uint32_t n = t.sumBlocks + std::min(t.n1 + t.n2, uint32_t(num_cus()));
+  by_act(act, [&](auto k) { hipLaunchKernelGGL((k_mlp_again<BWD, decltype(k)::value>), dim3(n), dim3(kWaves * 64), 0, stream(), t); });
+  return check_launch("gated_mlp");
 }
 
 // ---------------------------------------------------------------------------
@@ -572,6 +699,26 @@ bool forward_few(const MlpArgs& a) {
 }
 
 }  // namespace
+
+bool mlp_forward_again(const MlpArgs& a, const MlpAgain& g, const MlpSums& sums) {
+  Again<false> t{};
+  t.first = gate_product(a, g.ws);
+  t.second = down_product(a);
+  t.second.p[0].a.p = g.ws;
+  t.sums = sums;
+  t.g = g;
+  t.cols = a.out;
+  return run_again(t, a.act);
+}
+size_t mlp_again_floats(const MlpArgs& a) { return 3 * third(a); }
+bool mlp_backward_again(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd, const MlpAgain& g, const MlpSums& sums) {
+  Again<true> t{};
+  t.first = grad_product(a, dy, g.ws, third(a));
+  t.second = rest_products(a, dy, dx, dwg, dwu, dwd, g.ws, third(a));
+  t.sums = sums;
+  t.g = g;
+  return run_again(t, a.act);
+}
 
 bool mlp_forward(const MlpArgs& a) {
   if (a.rows <= uint32_t(kFew)) return forward_few(a);

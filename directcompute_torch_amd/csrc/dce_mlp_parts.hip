@@ -1,20 +1,27 @@
 // The gated feed-forward block on fp16 parts: the products of large calls at a
 // third of the fp16 MFMA rate, which is 16 times the fp32 one, with fp32's accuracy.
 //
-// A value x is kept as x 2^e = h + l, two fp16 values rounded to nearest, and
-// h h + (h l + l h) stands for a product.  The exponent e of a product's operand is one
-// for each row (a token's values, an output's weights), such that its largest value
-// lies in [2^14, 2^15): l's half step is then 2^-25, 2^-39 of that, and values down to
-// 2^-15 of their row's largest keep 24 bits.  As factors of the product's rows and
-// columns the exponents cost its loop nothing.  A matrix that is summed over its rows
-// in one product and over its columns in another is split twice, with exponents each way.
+// A value x is kept as x 2^e = h + l / 2^11, two fp16 values rounded to nearest, and
+// h h + (h l + l h) / 2^11 stands for a product.  The exponent e of a product's operand is one
+// for each row (a token's values, an output's weights), or for each block of a row, such that
+// the largest value lies in [2^14, 2^15): a value is then off by 2^-23 of itself, or by 2^-36,
+// 2^-50 of the largest; values down to 2^-27 of that keep 24 bits (with exponents of blocks
+// 2^-33, 2^-47 and 2^-24).  As factors of the product's rows and columns the exponents cost its
+// loop nothing.  A matrix that is summed over its rows in one product and over its columns in
+// another is split twice, with exponents each way.
+//
+// Smaller values still may be all that counts, where the other operand is zero at the large
+// ones.  So a product looks at its results (`doubt`), and rows of a forward, or gradients, that
+// parts may not hold are worked out again on fp32, by the launch that adds up the splits' sums.
 //
 // For x, dy and the weights a pass finds the maxima and another makes the parts; for Wg and Wu
 // of a forward with few rows the second does both, tile by tile.  What a
 // product leaves for the next one (m forward; dg, du, m backward) is split by its
 // epilogue, which knows the largest value of its own tile's rows and columns only: the
-// parts get that exponent, kept in a byte per row and tile, and the next product's loop
-// takes them to the row's own, that of the largest of them, by a power of two.
+// parts get that exponent, kept in a byte per row and tile, and the next product's loop takes
+// them to that of the row's largest value by a power of two.  h of such parts is a multiple of
+// 2^(kDown - 24), so that this rounds nothing; where more than 2^-kDown is asked for, the sums so
+// far go to the block's exponent instead.
 //
 // The steps, forward:  maxima -> parts of x, Wg, Wu, Wd -> g, u and m's parts (one
 // product over Wg and Wu, whose columns lie in turn, 32 by 32, so that a wave has g and
@@ -41,20 +48,25 @@ inline uint32_t pad(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
 __device__ __forceinline__ int exp_of(int field) { return min(141 - field, 127); }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ int field_of(uint32_t bits) { return int(bits >> 23); }
+// For a block: 0 is a block of zeros; values below 2^-126 have the exponent of those above.
+__device__ __forceinline__ uint8_t block_field(uint32_t bits) { return uint8_t(bits ? max(field_of(bits), 1) : 0); }
 
 // Parts in memory: 32 consecutive values of a row are 32 h, then 32 l (128 bytes).  x: 8
-// values of the row at `to`, from value c on, times `by`.
+// values of the row at `to`, from value c on, times `by`.  DOWN: h is a multiple of 2^(DOWN - 24).
+constexpr int kDown = 4;
+template <int DOWN>
 __device__ __forceinline__ void split8(const float* x, float by, h8& h, h8& l) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float v = x[i] * by;
-    h[i] = _Float16(v);
-    l[i] = _Float16(v - float(h[i]));
+    h[i] = _Float16(float(_Float16(v * (1.f / (1 << DOWN)))) * float(1 << DOWN));
+    l[i] = _Float16((v - float(h[i])) * 2048.f);
   }
 }
+template <int DOWN = 0>
 __device__ __forceinline__ void put8(float* to, uint32_t c, const float (&x)[8], float by) {
   h8 h, l;
-  split8(x, by, h, l);
+  split8<DOWN>(x, by, h, l);
   h8* p = reinterpret_cast<h8*>(to + (c & ~31u)) + (c & 31u) / 8;
   p[0] = h;
   p[4] = l;
@@ -65,7 +77,7 @@ __device__ __forceinline__ float size_of(float v) { return v == v ? fabsf(v) : I
 struct Side {
   float* p;
   uint32_t* top;   // bits of the largest value of each row
-  uint8_t* field;  // exponent field of the largest value of each row's block, [block][rows]; null: that of its row
+  uint8_t* field;  // exponent field of the largest value of each row's block (block_field), [block][rows]; null: that of its row
   uint32_t rows, depth;
 };
 
@@ -92,9 +104,9 @@ __device__ __forceinline__ void put_rows(float* S0, float* S1, const Side& t, ui
     m = group8_reduce(m, OpMaxR());
     if constexpr (OCT == 16) m = fmaxf(m, xl::dpp<xl::kRowMirror>(m));
     const uint32_t bits = __float_as_uint(m);
-    put8(t.p + size_t(r0 + r) * t.depth, c0 + 8 * o, v, pow2(exp_of(field_of(bits))));
+    put8<kDown>(t.p + size_t(r0 + r) * t.depth, c0 + 8 * o, v, pow2(exp_of(field_of(bits))));
     if (o == 0) {
-      t.field[size_t(c0 / COLS) * t.rows + r0 + r] = uint8_t(field_of(bits));
+      t.field[size_t(c0 / COLS) * t.rows + r0 + r] = block_field(bits);
       if (bits) atomicMax(t.top + r0 + r, bits);
     }
   }
@@ -116,9 +128,9 @@ __device__ __forceinline__ void put_columns(float* S0, float* S1, const Side& t,
     }
     m = group8_reduce(m, OpMaxR());
     const uint32_t bits = __float_as_uint(fmaxf(m, xl::dpp<xl::kRowMirror>(m))), row = in_turn(c0 + c, turn);
-    put8(t.p + size_t(row) * t.depth, r0 + 8 * o, v, pow2(exp_of(field_of(bits))));
+    put8<kDown>(t.p + size_t(row) * t.depth, r0 + 8 * o, v, pow2(exp_of(field_of(bits))));
     if (o == 0) {
-      t.field[size_t(r0 / 128) * t.rows + row] = uint8_t(field_of(bits));
+      t.field[size_t(r0 / 128) * t.rows + row] = block_field(bits);
       if (bits) atomicMax(t.top + row, bits);
     }
   }
@@ -299,6 +311,10 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
 // products have an accumulator of their own: an MFMA cuts what it adds off at the
 // scale of the largest addend, always downwards.
 //
+// An operand with exponents of its blocks is q, whose rows are the lanes' columns: sums that go
+// to another exponent are multiplied by one power of two for each.  (Done for every block, instead of
+// its fragments, that took the four products from 960 to 1150 us.)
+//
 // Bound by the MFMAs, for which power holds the clock to 1.7 GHz.  8192 x 1024 x 4096, in us
 // and TFLOP/s of fp32 products (a large fp16 library product, divided by three: 374): g and u 437,
 // 315; y 207, 332; dx, dWd, dWg and dWu 970, 354; dm 400, 172, of which its epilogue, which reads
@@ -306,13 +322,14 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
 // some 230 registers a lane.  With one array for both stages every read waited for the loads
 // (2.19 ms for 2.14 of a training pass).
 // ---------------------------------------------------------------------------
-enum Op { STORE, GATE, BLOCK_GATE, GRAD };  // BLOCK_GATE: the weights' parts have exponents of their blocks
+enum Op { STORE, GATE, BLOCK_GATE, GRAD };  // STORE, BLOCK_GATE: q's parts have exponents of its blocks
 struct Prod {
   Side p, q;
-  uint32_t right;          // STORE: the side whose parts have exponents of their blocks is q, not p
+  uint32_t flip;           // STORE: the result's rows are q's, else p's
   uint32_t tm, tn, depth;  // tiles; values of a row that are multiplied
-  uint32_t block;          // values of a block of the scaled side (a power of two)
+  uint32_t block;          // values of a block of q (a power of two)
   uint32_t rows, cols;     // of the result
+  uint32_t *any, *again;   // set where fp32 is to work it out: something, and the results' rows (null: all of it)
   float* out;              // STORE
   float* part;             // splits > 1: their shares of out, one after the other
   uint32_t splits;         // of the depth
@@ -342,8 +359,46 @@ __device__ __forceinline__ void load_stage(const BRes& b, uint32_t pitchBytes, u
 __device__ __forceinline__ h8 frag(const char* S, int row, int c) {
   return *reinterpret_cast<const h8*>(S + (row * 8 + (c ^ swz(row))) * 16);
 }
-// 2^-d, nothing for what is too small.
-__device__ __forceinline__ _Float16 down(int d) { return _Float16(ldexpf(1.f, -d)); }
+// Blocks that much smaller than their row are left out: 2^37 2^-60 of a block of 128 terms at most, for
+// which there is room wherever results are kept.
+constexpr int kApart = 60;
+// What a common exponent may add to the error of a product's result: max(4, sqrt(K) / 4) times 2^-24 of S, the
+// sum of its K terms' absolute values, less than fp32's own roundings make of them.  With the scaled operands
+// a, b, a value of which is off by 2^-36 (2^-33 of blocks) beside fp32's own rounding, it adds 2^-36 (sum |b| +
+// sum |a|), or 8 sum |a|.  Values are below 2^15: that is 4 times 2^-24 of S, or less, where S is K kLeast.
+template <bool SCALED>
+constexpr float kLeast = (SCALED ? 8 + 1 : 1 + 1) * 8 / 4.f;  // 2^15 2^-36 / 2^-24 = 8
+// S is at least |result|, and about a quarter of the small products' sum (|l| <= |h| but for values below
+// 2^(kDown - 14), which leave no more than 2^(kDown + 1) + 2 < 2 kLeast of a term in it): half of what `size` adds
+// up.  Each has a sign of its own, so this is enough for all but one result in 2^24 of normal operands (|result|
+// alone: the four products take 50 us more of 960).
+// For result (i, j) of the product, by one wave: is S, added up from the parts?
+template <bool SCALED>
+__device__ __forceinline__ bool held(const Prod& a, uint32_t i, uint32_t j, int top, uint32_t k0, uint32_t k1) {
+  const _Float16* p = reinterpret_cast<const _Float16*>(a.p.p + size_t(i) * a.p.depth);
+  const _Float16* q = reinterpret_cast<const _Float16*>(a.q.p + size_t(j) * a.q.depth);
+  float S = 0.f, L = 0.f;
+#pragma unroll 4
+  for (uint32_t k = k0 + (threadIdx.x & 63) * 8; k < k1; k += 512) {
+    const uint32_t at = (k & ~31u) * 2 + (k & 31);  // h, l 32 halves on
+    const h8 ph = *reinterpret_cast<const h8*>(p + at), pl = *reinterpret_cast<const h8*>(p + at + 32);
+    const h8 qh = *reinterpret_cast<const h8*>(q + at), ql = *reinterpret_cast<const h8*>(q + at + 32);
+    float f = 1.f, drop = 0.f;
+    if constexpr (SCALED) {
+      const uint8_t field = a.q.field[size_t(k / a.block) * a.q.rows + j];
+      if (!field) continue;
+      f = ldexpf(1.f, top - exp_of(field));
+      if (exp_of(field) > top + kApart) drop = 0x1p36f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = fabsf(float(ph[e]) + float(pl[e]) / 2048.f), y = fabsf(float(qh[e]) + float(ql[e]) / 2048.f) * f;
+      S += drop ? 0.f : x * y;
+      L += (SCALED ? 8.f : 1.f) * x * f + y + drop * (x * y);
+    }
+  }
+  return wave_reduce(S) * (4096.f * fmaxf(4.f, 0.25f * sqrtf(float(k1 - k0)))) >= wave_reduce(L);
+}
 
 template <Op OP, MlpAct ACT, int N, bool NT>
 __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_mlp_product(const Prods<N> all) {
@@ -379,117 +434,235 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) big[i][j][e] = small[i][j][e] = 0.f;
-  // The scaled side's rows of this lane: their own exponent field, and the blocks'.
-  const bool right = OP == BLOCK_GATE || (SCALED && a.right);
-  const Side& sc = right ? a.q : a.p;
-  const uint32_t srow = (right ? tj * kTile + wn : ti * kTile + wm) + col;
-  int own[2] = {};
+  // This lane's columns: the exponents of their largest values, those that the sums are in, and the
+  // block's factors towards them.
+  const uint32_t qrow = tj * kTile + wn + col;
+  uint32_t qtop[2];
+  int own[2], now[2];
   uint8_t next[2] = {};
   _Float16 by[2] = {};
-  if constexpr (SCALED) {
+  auto fetch_next = [&](uint32_t k) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      own[i] = exp_of(field_of(sc.top[srow + 32 * i]));
-      next[i] = sc.field[size_t(k0 / a.block) * sc.rows + srow + 32 * i];
-    }
+    for (int j = 0; j < 2; ++j) next[j] = a.q.field[size_t(min(k, k1 - 1) / a.block) * a.q.rows + qrow + 32 * j];
+  };
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    qtop[j] = a.q.top[qrow + 32 * j];
+    own[j] = now[j] = exp_of(field_of(qtop[j]));
   }
+  if constexpr (SCALED) fetch_next(k0);
   load_stage(bp, a.p.depth * 4, k0, S0);
   load_stage(bq, a.q.depth * 4, k0, S0 + kStageBytes);
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  auto loop = [&](auto side) {
-    constexpr int SIDE = decltype(side)::value;  // 0: p is scaled, 1: q, -1: neither
-    auto step = [&](uint32_t k, const char* St, char* Sn) {
-      if (k + kStep < k1) {
-        load_stage(bp, a.p.depth * 4, k + kStep, Sn);
-        load_stage(bq, a.q.depth * 4, k + kStep, Sn + kStageBytes);
+  // To the block at k.
+  auto enter = [&](uint32_t k) __attribute__((always_inline)) {
+    int d[2];
+    bool out[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int e = exp_of(next[j]);
+      out[j] = e > own[j] + kApart;
+      d[j] = next[j] && !out[j] ? e - now[j] : 0;
+    }
+    if (__any(uint32_t(d[0]) > uint32_t(kDown) || uint32_t(d[1]) > uint32_t(kDown))) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int by = uint32_t(d[j]) > uint32_t(kDown) ? d[j] : 0;
+        const float f = pow2(by);
+        now[j] += by;
+        d[j] -= by;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int t = 0; t < 16; ++t) {
+            big[i][j][t] *= f;
+            small[i][j][t] *= f;
+          }
       }
-      h8 p[2][2][2], q[2][2][2];
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) by[j] = out[j] ? _Float16(0.f) : _Float16(pow2(-d[j]));
+    fetch_next(k + a.block);
+  };
+  auto step = [&](uint32_t k, const char* St, char* Sn) {
+    if (k + kStep < k1) {
+      load_stage(bp, a.p.depth * 4, k + kStep, Sn);
+      load_stage(bq, a.q.depth * 4, k + kStep, Sn + kStageBytes);
+    }
+    h8 p[2][2][2], q[2][2][2];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          p[kk][i][e] = frag(St, wm + 32 * i + col, 4 * e + 2 * kk + half);
+          q[kk][i][e] = frag(St + kStageBytes, wn + 32 * i + col, 4 * e + 2 * kk + half);
+        }
+    if constexpr (SCALED) {
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            p[kk][i][e] = frag(St, wm + 32 * i + col, 4 * e + 2 * kk + half);
-            q[kk][i][e] = frag(St + kStageBytes, wn + 32 * i + col, 4 * e + 2 * kk + half);
-          }
-      if constexpr (SCALED) {
-        if ((k & (a.block - 1)) == 0) {
-          const uint32_t then = min(k + a.block, k1 - 1) / a.block;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            by[i] = down(exp_of(next[i]) - own[i]);
-            next[i] = sc.field[size_t(then) * sc.rows + srow + 32 * i];
-          }
-        }
-      }
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        if constexpr (SCALED) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if constexpr (SIDE == 1)
-                q[kk][i][e] *= by[i];
-              else
-                p[kk][i][e] *= by[i];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            big[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][0], big[i][j], 0, 0, 0);
-            small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][1], small[i][j], 0, 0, 0);
-            small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][1], q[kk][j][0], small[i][j], 0, 0, 0);
-          }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
-    };
-    for (uint32_t k = k0; k < k1; k += 2 * kStep) {  // the depth is a multiple of 128
-      step(k, S0, S1);
-      step(k + kStep, S1, S0);
+          for (int e = 0; e < 2; ++e) q[kk][j][e] *= by[j];
     }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          big[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][0], big[i][j], 0, 0, 0);
+          small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][0], q[kk][j][1], small[i][j], 0, 0, 0);
+          small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[kk][i][1], q[kk][j][0], small[i][j], 0, 0, 0);
+        }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
   };
-  if constexpr (!SCALED)
-    loop(std::integral_constant<int, -1>{});
-  else if constexpr (OP == BLOCK_GATE)
-    loop(std::integral_constant<int, 1>{});
-  else if (right)
-    loop(std::integral_constant<int, 1>{});
-  else
-    loop(std::integral_constant<int, 0>{});
+  for (uint32_t k = k0; k < k1; k += 2 * kStep) {  // the depth is a multiple of 128
+    if constexpr (SCALED)
+      if ((k & (a.block - 1)) == 0) enter(k);
+    step(k, S0, S1);
+    step(k + kStep, S1, S0);
+  }
   // Row 8 (e / 4) + 4 half + e % 4 of a block, column `col`.
   const uint32_t r0 = ti * kTile, c0 = tj * kTile;
   float *T0 = reinterpret_cast<float*>(S0), *T1 = reinterpret_cast<float*>(S1);
-  int eq[2];
+  auto row_of = [&](int i, int e) { return r0 + wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3); };
+  float low[2] = {INFINITY, INFINITY}, least[2];
+  uint32_t top[2][16], least_top = ~0u, none = 0;  // none: a bit for each row of p that is zeros
 #pragma unroll
-  for (int j = 0; j < 2; ++j) eq[j] = exp_of(field_of(a.q.top[c0 + wn + 32 * j + col]));
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top[i][e] = a.p.top[row_of(i, e)];
+  auto size = [&](int i, int j, int e) { return fmaf(0.25f, fabsf(small[i][j][e]), fabsf(big[i][j][e])); };
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int ep = exp_of(field_of(a.p.top[r0 + wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3)]));
+      least_top = min(least_top, top[i][e]);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) big[i][j][e] = ldexpf(big[i][j][e] + small[i][j][e], -(ep + eq[j]));
+      for (int j = 0; j < 2; ++j) {
+        big[i][j][e] += small[i][j][e] * (1.f / 2048.f);
+        low[j] = fminf(low[j], size(i, j, e));
+      }
     }
-  if constexpr (OP == STORE) {
-    float* out = a.splits > 1 ? a.part + size_t(sp) * a.rows * a.cols : a.out;
+  if (__any(least_top == 0)) {
+    low[0] = low[1] = INFINITY;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const uint32_t r = r0 + wm + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3);
+        none |= uint32_t(top[i][e] == 0) << (16 * i + e);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t n = c0 + wn + 32 * j + col;
-          if (r < a.rows && n < a.cols) out[size_t(r) * a.cols + n] = big[i][j][e];
+        for (int j = 0; j < 2; ++j) low[j] = fminf(low[j], top[i][e] ? size(i, j, e) : INFINITY);
+      }
+  }
+  bool sure = true;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    least[j] = float(k1 - k0) * (2.f * kLeast<SCALED>) * (SCALED ? pow2(now[j] - own[j]) : 1.f);
+    sure = sure && (qtop[j] == 0 || low[j] >= least[j]);
+  }
+  // Which of a wave's results parts may not hold: not those of rows of zeros, and rows that are not finite are left at that.
+  auto doubt = [&]() __attribute__((always_inline)) {
+    uint32_t pend[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (top[i][e] == 0 || top[i][e] >= 0x7f800000u) continue;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (!(size(i, j, e) >= least[j])) pend[j] |= 1u << (16 * i + e);
+      }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      bool zeros = qtop[j] == 0;
+      if constexpr (SCALED) {
+        zeros = true;  // in this split of the depth
+        for (uint32_t b = k0 / a.block; b < k1 / a.block; ++b) zeros = zeros && a.q.field[size_t(b) * a.q.rows + qrow + 32 * j] == 0;
+      }
+      if (zeros || qtop[j] >= 0x7f800000u) pend[j] = 0;
+    }
+    const bool flip = OP == STORE && a.flip;
+    uint32_t looks = 128;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      for (uint64_t m = __ballot(pend[j] != 0); m; m = __ballot(pend[j] != 0)) {
+        if (!looks--) {  // many: all of them
+          *a.any = 1;
+          if (a.again) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                  if (t >= j && (pend[t] >> (16 * i + e) & 1)) a.again[flip ? qrow + 32 * t : row_of(i, e)] = 1;
+          }
+          return;
+        }
+        const int l = __builtin_ctzll(m);
+        const uint32_t bit = __builtin_ctz(xl::rdl32(pend[j], l));
+        if (lane == l) pend[j] &= pend[j] - 1;
+        const uint32_t pr = r0 + wm + 32 * (bit >> 4) + 8 * ((bit >> 2) & 3) + 4 * (l >> 5) + (bit & 3), qr = tj * kTile + wn + 32 * j + (l & 31);
+        if (held<SCALED>(a, pr, qr, int(xl::rdl32(uint32_t(own[j]), l)), k0, k1)) continue;
+        *a.any = 1;
+        if (!a.again) return;
+        a.again[flip ? qr : pr] = 1;  // the row's others need no look
+        if (flip) {
+          if (col == (l & 31)) pend[j] = 0;
+        } else if (half == l >> 5) {
+          pend[0] &= ~(1u << bit);
+          pend[1] &= ~(1u << bit);
         }
       }
+  };
+  if (!__all(sure)) doubt();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int ep = exp_of(field_of(top[i][e]));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) big[i][j][e] = ldexpf(big[i][j][e], -(ep + now[j]));
+    }
+  if constexpr (OP == STORE) {
+    float* out = a.splits > 1 ? a.part + size_t(sp) * a.rows * a.cols : a.out;
+    if (a.flip) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const uint32_t r = qrow + 32 * j, n = row_of(i, e);
+            float* to = out + size_t(r) * a.cols + n;
+            if (r < a.rows && n + 3 < a.cols) {
+              stus<false>(to, f4u{big[i][j][e], big[i][j][e + 1], big[i][j][e + 2], big[i][j][e + 3]});
+            } else if (r < a.rows) {
+#pragma unroll
+              for (int t = 0; t < 3; ++t)
+                if (n + t < a.cols) to[t] = big[i][j][e + t];
+            }
+          }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t r = row_of(i, e);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t n = qrow + 32 * j;
+            if (r < a.rows && n < a.cols) out[size_t(r) * a.cols + n] = big[i][j][e];
+          }
+        }
+    }
   }
   if constexpr (OP == GATE || OP == BLOCK_GATE) {
     const uint32_t f = ((c0 + wn) >> 1) + col;
@@ -541,6 +714,15 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
           small[i][j][e] = du;
           u[i][j][e] = m;
         }
+    if (__any(none != 0)) {  // a token without a gradient has no part in dWd: its m, however large, is none (not finite: NaN)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (none >> (16 * i + e) & 1) u[i][j][e] *= 0.f;
+    }
     auto tile = [&](const f16v (&v)[2][2]) {
       __syncthreads();
 #pragma unroll
@@ -561,20 +743,6 @@ __global__ void __launch_bounds__(kT) __attribute__((amdgpu_waves_per_eu(2))) k_
     tile(u);
     put_columns(T0, T1, a.mc, r0, c0);
   }
-}
-
-__global__ void __launch_bounds__(kT) k_mlp_sum(const MlpSums t) {
-  int k = 0;
-  while (k + 1 < int(t.count) && t.s[k + 1].start <= blockIdx.x) ++k;
-  const MlpSums::One s = t.s[k];
-  const uint32_t i = ((blockIdx.x - s.start) * kT + threadIdx.x) * 4;
-  if (i >= s.n) return;
-  // the last quad ends with the matrix; fewer than 4 values there are none
-  const uint32_t at = min(i, s.n - 4);
-  f4u v = ldus<false, f4u>(s.part + at);
-#pragma unroll 4
-  for (uint32_t k = 1; k < s.splits; ++k) v += ldus<false, f4u>(s.part + size_t(k) * s.n + at);
-  stus<false>(s.out + at, v);
 }
 
 // Places in the workspace.
@@ -607,6 +775,13 @@ struct Plan {
     tops += rows;
     if (block) raised = tops;
   }
+  // Words that products set (after the sides of blocks, which come first).
+  size_t words = 0;
+  void flags(uint32_t n) {
+    words = tops;
+    tops += n;
+    raised = tops;
+  }
   // A matrix whose parts are to be made, of its rows or columns; both sides may still lack their places.
   struct Source {
     const float* src;
@@ -630,12 +805,18 @@ struct Plan {
     if (straight) parts += size_t(cdiv(cols, by.cols)) * rows;
     if (across) parts += size_t(cdiv(rows, by.rows)) * cols;
   }
-  // The workspace, room for `more` floats at *extra, and the jobs.
-  bool lay(size_t more, float** extra) {
+  // The workspace, room for `more` floats at *extra, and the jobs.  `free`: what is there for fp32 when
+  // the products are done, up to the sides' end, `least` floats.
+  float* free;
+  uint32_t* flag;
+  bool lay(size_t more, float** extra, size_t least) {
+    at.next = std::max(at.next, (least + 63) & ~size_t(63));
     const size_t first = at.take(tops), tail = at.take(more), part = at.take(parts);
     float* ws = workspace(at.next);
     if (!ws) return false;
     *extra = ws + tail;
+    free = ws;
+    flag = reinterpret_cast<uint32_t*>(ws + first) + words;
     for (int i = 0; i < count; ++i) {
       Side& s = *all[i].s;
       s.p = ws + all[i].p;
@@ -702,15 +883,15 @@ bool run_jobs(Jobs& t, uint32_t maxima) {
   return check_launch("gated_mlp");
 }
 // Splits of the depths: no workgroup has more than a slot's share of the launch (two a CU),
-// or `kLeast` where that is more (backward us with 256, 512, 1024 and 2048, 1024 x 1024 x 4096
+// or `kSplitLeast` where that is more (backward us with 256, 512, 1024 and 2048, 1024 x 1024 x 4096
 // 229, 226, 235 and 232, 400 x 512 x 2048 91, 83, 87 and 107, 256 x 1024 x 2816 113, 112, 109 and
 // 126).  Floats of their shares.
-constexpr uint32_t kLeast = 512;
+constexpr uint32_t kSplitLeast = 512;
 template <int N>
 size_t split(Prods<N>& t) {
   double all = 0;
   for (uint32_t i = 0; i < t.count; ++i) all += double(t.a[i].p.rows / kTile) * (t.a[i].q.rows / kTile) * t.a[i].depth;
-  const double most = std::max<double>(kLeast, all / (2 * num_cus()));
+  const double most = std::max<double>(kSplitLeast, all / (2 * num_cus()));
   size_t floats = 0;
   for (uint32_t i = 0; i < t.count; ++i) {
     Prod& a = t.a[i];
@@ -721,10 +902,10 @@ size_t split(Prods<N>& t) {
 }
 // `bytes`: what the launch reads and writes but once (of 4.0e8, g and u: nontemporal accesses
 // to them take the gate's product from 454 to 438 us, of 9.4e8 the gradient's from 407 to 377).
+// `sums`: what the splits leave to be added up.
 template <Op OP, int N>
-bool run_products(Prods<N>& t, MlpAct act = kSilu, float* part = nullptr, double bytes = 0) {
+bool run_products(Prods<N>& t, MlpAct act = kSilu, float* part = nullptr, double bytes = 0, MlpSums* sums = nullptr) {
   uint32_t n = 0;
-  MlpSums sums{};
   for (uint32_t i = 0; i < t.count; ++i) {
     Prod& a = t.a[i];
     a.tm = a.p.rows / kTile;
@@ -736,7 +917,7 @@ bool run_products(Prods<N>& t, MlpAct act = kSilu, float* part = nullptr, double
     a.part = part;
     const size_t values = size_t(a.rows) * a.cols;
     part += (size_t(a.splits) * values + 63) & ~size_t(63);
-    sums.add(a.part, a.out, uint32_t(values), a.splits);
+    sums->add(a.part, a.out, uint32_t(values), a.splits);
   }
   by_act(act, [&](auto k) {
     constexpr MlpAct A = OP == STORE ? kSilu : decltype(k)::value;
@@ -745,15 +926,14 @@ bool run_products(Prods<N>& t, MlpAct act = kSilu, float* part = nullptr, double
     else
       hipLaunchKernelGGL((k_mlp_product<OP, A, N, false>), dim3(n), dim3(kT), 0, stream(), t);
   });
-  mlp_sum(sums);
   return check_launch("gated_mlp");
 }
 template <int N>
-void add(Prods<N>& t, const Side& p, const Side& q, bool right, uint32_t block, uint32_t rows, uint32_t cols, float* out) {
+void add(Prods<N>& t, const Side& p, const Side& q, bool flip, uint32_t block, uint32_t rows, uint32_t cols, float* out) {
   Prod& a = t.a[t.count++];
   a.p = p;
   a.q = q;
-  a.right = right;
+  a.flip = flip;
   a.depth = p.depth;
   a.block = block;
   a.rows = rows;
@@ -762,10 +942,6 @@ void add(Prods<N>& t, const Side& p, const Side& q, bool right, uint32_t block, 
 }
 
 }  // namespace
-
-void mlp_sum(const MlpSums& t) {
-  if (t.count) hipLaunchKernelGGL(k_mlp_sum, dim3(t.blocks), dim3(kT), 0, stream(), t);
-}
 
 bool mlp_forward_parts(const MlpArgs& a) {
   const uint32_t M = pad(a.rows, kTile), C = pad(a.cols, kTile), F = pad(a.hidden, kTile), O = pad(a.out, kTile);
@@ -777,6 +953,7 @@ bool mlp_forward_parts(const MlpArgs& a) {
   // and 650).
   const bool blocks = a.rows <= 2048;
   plan.side(m, M, F, 64);
+  plan.flags(3 + M);
   plan.side(w, 2 * F, C, blocks ? 128 : 0);
   plan.side(x, M, C);
   plan.side(d, O, F);
@@ -784,14 +961,16 @@ bool mlp_forward_parts(const MlpArgs& a) {
   plan.add(a.wd, a.hidden, a.out, nullptr, &d);
   plan.add(a.wg, a.cols, a.hidden, nullptr, &w, 0, 0);
   plan.add(a.wu, a.cols, a.hidden, nullptr, &w, 0, 1);
-  ProfScope prof("mlp", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
+  ProfScope prof("mlp_parts", 6.0 * a.rows * a.cols * a.hidden, 4.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
   // The second product's sides get their places with the others.
   Prods<1> t1{}, t2{};
-  add(t2, m, d, false, 64, a.rows, a.out, a.y);
+  add(t2, d, m, true, 64, a.rows, a.out, a.y);
   float* part;
-  if (!plan.lay(split(t2), &part)) return false;
-  t2.a[0].p = m;
-  t2.a[0].q = d;
+  if (!plan.lay(split(t2), &part, size_t(a.rows) * a.hidden)) return false;
+  t2.a[0].p = d;
+  t2.a[0].q = m;
+  t2.a[0].any = plan.flag;
+  t2.a[0].again = plan.flag + 3;
   if (!run_jobs(plan.jobs, plan.maxima)) return false;
   t1.count = 1;
   Prod& g = t1.a[0];
@@ -801,6 +980,8 @@ bool mlp_forward_parts(const MlpArgs& a) {
   g.depth = C;
   g.rows = a.rows;
   g.m = m;
+  g.any = plan.flag;
+  g.again = plan.flag + 3;
   g.hidden = a.hidden;
   if (a.saved) {
     g.g = a.saved;
@@ -808,7 +989,8 @@ bool mlp_forward_parts(const MlpArgs& a) {
   }
   const double bytes = (a.saved ? 12.0 : 4.0) * M * F;
   if (!(blocks ? run_products<BLOCK_GATE>(t1, a.act, nullptr, bytes) : run_products<GATE>(t1, a.act, nullptr, bytes))) return false;
-  return run_products<STORE>(t2, kSilu, part);
+  MlpSums sums{};
+  return run_products<STORE>(t2, kSilu, part, 0, &sums) && mlp_forward_again(a, {plan.flag, plan.flag + 3, plan.flag + 1, plan.free}, sums);
 }
 
 bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg, float* dwu, float* dwd) {
@@ -819,6 +1001,7 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
   if (dwd) plan.side(mc, F, M, 128);
   if (dwg) plan.side(dgc, F, M, 128);
   if (dwu) plan.side(duc, F, M, 128);
+  plan.flags(3);
   plan.side(yr, M, O);
   plan.side(d, F, O);
   if (dwd) plan.side(yc, O, M);
@@ -831,23 +1014,26 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
     plan.add(a.wg, a.cols, a.hidden, &w, nullptr, 0);
     plan.add(a.wu, a.cols, a.hidden, &w, nullptr, F);
   }
-  ProfScope prof("mlp", 12.0 * a.rows * a.cols * a.hidden, 8.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
+  ProfScope prof("mlp_parts", 12.0 * a.rows * a.cols * a.hidden, 8.0 * (2.0 * a.rows * a.cols + 3.0 * a.cols * a.hidden));
   // All that follow dm's in one launch, the deepest first: a last round of few workgroups
   // instead of four.  Twice: their sizes first, their places once they have them.
   Prods<4> t2{};
   auto rest = [&] {
     const Prods<4> had = t2;
     t2 = {};
-    if (dx && 2 * F >= M) add(t2, dr, w, false, 128, a.rows, a.cols, dx);
-    if (dwd) add(t2, mc, yc, false, 128, a.hidden, a.out, dwd);
-    if (dwg) add(t2, xc, dgc, true, 128, a.cols, a.hidden, dwg);
-    if (dwu) add(t2, xc, duc, true, 128, a.cols, a.hidden, dwu);
-    if (dx && 2 * F < M) add(t2, dr, w, false, 128, a.rows, a.cols, dx);
-    for (uint32_t i = 0; i < had.count; ++i) t2.a[i].splits = had.a[i].splits;
+    if (dx && 2 * F >= M) add(t2, w, dr, true, 128, a.rows, a.cols, dx);
+    if (dwd) add(t2, yc, mc, true, 128, a.hidden, a.out, dwd);
+    if (dwg) add(t2, xc, dgc, false, 128, a.cols, a.hidden, dwg);
+    if (dwu) add(t2, xc, duc, false, 128, a.cols, a.hidden, dwu);
+    if (dx && 2 * F < M) add(t2, w, dr, true, 128, a.rows, a.cols, dx);
+    for (uint32_t i = 0; i < t2.count; ++i) {
+      t2.a[i].splits = had.a[i].splits;
+      t2.a[i].any = plan.flag;
+    }
   };
   rest();
   float* part;
-  if (!plan.lay(split(t2), &part)) return false;
+  if (!plan.lay(split(t2), &part, mlp_again_floats(a))) return false;
   rest();
   if (!run_jobs(plan.jobs, plan.maxima)) return false;
   Prods<1> t1{};
@@ -860,12 +1046,15 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
   g.hidden = a.hidden;
   g.g = a.saved;
   g.u = a.saved + size_t(a.rows) * a.hidden;
+  g.any = plan.flag;
   g.dr = dr;
   g.dgc = dgc;
   g.duc = duc;
   g.mc = mc;
   if (!run_products<GRAD>(t1, a.act, nullptr, 28.0 * M * F)) return false;
-  return run_products<STORE>(t2, kSilu, part);
+  MlpSums sums{};
+  return run_products<STORE>(t2, kSilu, part, 0, &sums) &&
+         mlp_backward_again(a, dy, dx, dwg, dwu, dwd, {plan.flag, nullptr, plan.flag + 1, plan.free}, sums);
 }
 
 // The parts of the weights are made anew at each call, which few rows do not pay for.

@@ -303,7 +303,10 @@ void ResidualNormBackward(void* gradH, void* gradNormed, void* h, void* block, v
  * fewer than 2^29 values in each matrix and in rows x hidden.  act: 0 silu, 1 gelu (by erf), 2 relu, 3
  * sigmoid.  pSaved, when not NULL, receives x Wg and x Wu (2 * rows * hidden
  * floats) for the backward, which gives each gradient only when its pointer is
- * not NULL. */
+ * not NULL.  A result of K terms is off by sqrt(K) + 8 roundings (2^-24) of the sum
+ * of its terms' absolute values at most, as a chain of fp32 operations is, whatever
+ * the operands' sizes.  Large calls make a row of y, or a gradient that sums over
+ * rows, NaN as a whole where an operand of it is not finite. */
 void* GatedMlpForward(void* x, void* wGate, void* wUp, void* wDown, uint32_t rows, uint32_t cols,
                       uint32_t hidden, uint32_t outCols, uint32_t act, void** pSaved);
 void GatedMlpBackward(void* gradOut, void* x, void* wGate, void* wUp, void* wDown, void* saved,
