@@ -983,6 +983,23 @@ def _gain_of(what, name, gain, width):
         raise ValueError(f"{what}: {name} is ({width},), not {tuple(gain.shape)}")
 
 
+def _gate_rows(gate, shape):
+    """Rows of a residual gate for x of `shape`, each for an equal share of x's rows in turn; None
+    where the gate's shape does not say that.  Leading axes as x's, the rest ones or left out."""
+    if not gate.shape or gate.shape[-1] != shape[-1]:
+        return None
+    lead, axes = tuple(gate.shape[:-1]), tuple(shape[:-1])
+    rows, of = int(np.prod(lead, dtype=np.int64)), int(np.prod(axes, dtype=np.int64))
+    if rows in (1, of) and (rows == 1 or lead in ((of,), axes)):
+        return rows
+    if len(axes) == 1:   # tokens side by side: a gate's row for as many of them each
+        return rows if len(lead) == 1 and rows and of % rows == 0 else None
+    own = lead
+    while own and own[-1] == 1:
+        own = own[:-1]
+    return rows if len(lead) <= len(axes) and own == axes[:len(own)] else None
+
+
 class RmsNormFunc(_Keeps):
     def forward(self, x, gain, eps):
         width = x.shape[-1] if x.shape else 0
@@ -1019,10 +1036,10 @@ class ResidualNormFunc(_Keeps):
         rows = x.size // width
         gate_rows = 0
         if gate is not None:
-            gate_rows = gate.size // width
-            if not gate.shape or gate.shape[-1] != width or rows % gate_rows:
-                raise ValueError(f"residual_norm: a gate of {tuple(gate.shape)} for {shape}: rows of {width} values, "
-                                 f"a number of them that divides {rows}")
+            gate_rows = _gate_rows(gate, shape)
+            if gate_rows is None:
+                raise ValueError(f"residual_norm: a gate of {tuple(gate.shape)} for {shape}: ({width},), or x's leading axes and "
+                                 f"{width}" + (f", or a number of rows that divides {rows}" if len(shape) == 2 else ""))
         # pre is here for its place in the traversal: its gradient may come from this node
         self.inputs = (x, block, gate, post, pre)
         self.dims = (rows, width, gate_rows, float(scale))
@@ -1199,9 +1216,10 @@ def residual_norm(x, block, gate=None, post=None, pre=None, scale=1.0, eps=1e-6)
     """The step from one block of a residual stream to the next, in one pass:
     h = scale * x + gate * u, where u is `block` (a block's result, of x's shape)
     or, with a gain `post`, its rms_norm.  With a gain `pre` returns (h, rms_norm(h,
-    pre)), the second the next block's input; else h.  gate: rows of x's last
-    axis, each for an equal share of x's rows in turn: (width,) for all of them,
-    (batch, width) for x of (batch, seq, width), or x's shape."""
+    pre)), the second the next block's input; else h.  gate: (width,) for all of
+    x's rows, (batch, width) or (batch, 1, width) for x of (batch, seq, width), or
+    x's shape, also as (batch * seq, width); for x of (rows, width) any number of
+    rows that divides x's, each for as many of them in turn."""
     return ResidualNormFunc().forward(x, block, gate, post, pre, scale, eps)
 
 

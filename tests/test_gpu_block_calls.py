@@ -1,0 +1,46 @@
+"""Calls of the block's operators that their documentation allows or refuses."""
+import numpy as np
+import pytest
+
+from tests.helpers import rng
+from tests.test_gpu_block import dev
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("shape,gate,spread", [
+    ((3, 5, 8), (8,), (1, 1, 8)), ((3, 5, 8), (1, 8), (1, 1, 8)), ((3, 5, 8), (1, 1, 8), (1, 1, 8)), ((3, 5, 8), (3, 8), (3, 1, 8)),
+    ((3, 5, 8), (3, 1, 8), (3, 1, 8)), ((3, 5, 8), (3, 5, 8), (3, 5, 8)), ((3, 5, 8), (15, 8), (3, 5, 8)), ((1, 5, 8), (5, 8), (1, 5, 8)),
+    ((2, 3, 4, 8), (2, 8), (2, 1, 1, 8)), ((2, 3, 4, 8), (2, 3, 8), (2, 3, 1, 8)), ((2, 3, 4, 8), (2, 3, 1, 8), (2, 3, 1, 8)),
+    ((4, 8), (4, 8), (4, 8)), ((3, 1, 8), (3, 8), (3, 1, 8)), ((8,), (8,), (8,))], ids=str)
+def test_residual_gates(eng, shape, gate, spread):
+    r = rng(len(shape))
+    x, b, g = (r.standard_normal(s).astype(np.float32) for s in (shape, shape, gate))
+    T = [dev(eng, v, True) for v in (x, b, g)]
+    h = eng.residual_norm(*T)
+    h.backward(dev(eng, np.ones(shape)))
+    assert np.allclose(h.sync(), x + g.reshape(spread) * b, rtol=0, atol=2 ** -20)
+    axes = tuple(i for i, n in enumerate(spread) if n == 1)
+    assert np.allclose(T[2].grad.sync().reshape(spread), b.sum(axes, keepdims=True), rtol=0, atol=b.size * 2 ** -22)
+    eng.end_batch()
+
+
+def test_residual_gate_of_tokens_side_by_side(eng):
+    r = rng(4)
+    x, b, g = (r.standard_normal(s).astype(np.float32) for s in ((12, 8), (12, 8), (3, 8)))
+    h = eng.residual_norm(*(dev(eng, v) for v in (x, b, g)))
+    assert np.allclose(h.sync(), x + np.repeat(g, 4, 0) * b, rtol=0, atol=2 ** -20)
+    eng.end_batch()
+
+
+@pytest.mark.parametrize("shape,gate", [((3, 5, 8), (5, 8)), ((3, 5, 8), (1, 5, 8)), ((4, 2, 8), (2, 8)), ((2, 4, 8), (4, 8)), ((3, 5, 8), (3, 5)),
+                                        ((3, 5, 8), (5, 3, 8)), ((3, 5, 8), (3, 5, 1, 8)), ((2, 3, 4, 8), (6, 8)), ((12, 8), (5, 8)),
+                                        ((3, 5, 8), (0, 8)), ((12, 8), (0, 8)), ((12, 8), (2, 2, 8))], ids=str)
+def test_residual_gates_refused(eng, shape, gate):
+    """A gate for each position, among others, does not say which rows are its."""
+    class Shaped:   # no buffer of no values can be made
+        gpu_buf, size, requires_grad = None, int(np.prod(gate)), False
+    Shaped.shape = gate
+    x = dev(eng, np.zeros(shape))
+    with pytest.raises(ValueError, match="gate"):
+        eng.residual_norm(x, x, gate=Shaped())
