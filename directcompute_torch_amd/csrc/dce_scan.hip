@@ -76,7 +76,7 @@ struct Lane {
 __device__ __forceinline__ uint32_t tokens_of(const ScanArgs& a, uint32_t b) {
   if (!a.len) return a.S;
   const float n = a.len[b];
-  return n >= 1.f ? (n < float(a.S) ? uint32_t(n) : a.S) : 0u;  // NaN: none
+  return n >= 1.f ? min(uint32_t(fminf(n, 0x1p31f)), a.S) : 0u;  // NaN: none; S may be no float
 }
 
 __device__ __forceinline__ void Lane::init(const Scan& s, uint32_t block) {

@@ -316,7 +316,8 @@ void GatedMlpBackward(void* gradOut, void* x, void* wGate, void* wUp, void* wDow
 /* Gated linear recurrence over [batch][seq][chans]: f = sigmoid(gate), y_t = f_t
  * y_(t-1) + (1 - f_t) x_t for every channel, from `state` (batch x chans values, or
  * NULL: zeros).  lengths: batch floats, the tokens of each sequence that count
- * (clamped to 0 .. seq; memory past them may hold anything), or NULL: all; y is
+ * (clamped to 0 .. seq, beyond 2^24 those that a float can be; memory past them may
+ * hold anything), or NULL: all; y is
  * zeros past them.  pLast, when not NULL, receives the state after the last token
  * that counts (batch x chans): the next call's `state`.  Sequences of fewer than 2130706432
  * tokens, and of 2^24 and more with fewer than four channels no more than 2^30 - 2^22 tokens in all.  The backward reads the

@@ -44,3 +44,20 @@ def test_residual_gates_refused(eng, shape, gate):
     x = dev(eng, np.zeros(shape))
     with pytest.raises(ValueError, match="gate"):
         eng.residual_norm(x, x, gate=Shaped())
+
+
+def test_scan_lengths_beyond_2_24(eng):
+    """A length that is a float of its own, next to a sequence's length that is none."""
+    S = 2 ** 24 + 1
+    print("gated_scan of", S, "tokens", flush=True)
+    x = np.zeros((1, S, 1), np.float32)
+    x[0, -3:, 0] = 1, 2, 4
+    z = dev(eng, np.zeros((1, S, 1)))
+    for n, want in ((2 ** 24 - 1, [0.5, 0, 0]), (2 ** 24, [0.5, 1.25, 0]), (2 ** 24 + 2, [0.5, 1.25, 2.625]), (2.0 ** 40, [0.5, 1.25, 2.625])):
+        T = dev(eng, x, True)
+        y, last = eng.gated_scan(T, z, lengths=dev(eng, [n]), return_state=True)
+        y.backward(dev(eng, np.ones((1, S, 1))))
+        live = np.count_nonzero(want)
+        assert y.sync()[0, -3:, 0].tolist() == want and last.sync()[0, 0] == want[live - 1], n
+        assert (T.grad.sync()[0, -3:, 0] > 0).tolist() == [i < live for i in range(3)], n
+        eng.end_batch()
