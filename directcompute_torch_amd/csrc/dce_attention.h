@@ -36,7 +36,7 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 __device__ __forceinline__ uint32_t keys_of(const Attn& a, uint32_t b) {
   if (!a.len) return a.T;
   const float n = a.len[b];
-  return n >= 1.f ? (n < float(a.T) ? uint32_t(n) : a.T) : 0u;  // NaN: none
+  return n >= 1.f ? min(uint32_t(fminf(n, 0x1p31f)), a.T) : 0u;  // NaN: none; T may be no float
 }
 // Keys that row n sees (row n of the problem, `len` keys in the sequence).
 __device__ __forceinline__ uint32_t limit_of(const Attn& a, uint32_t n, uint32_t len) {

@@ -61,3 +61,20 @@ def test_scan_lengths_beyond_2_24(eng):
         assert y.sync()[0, -3:, 0].tolist() == want and last.sync()[0, 0] == want[live - 1], n
         assert (T.grad.sync()[0, -3:, 0] > 0).tolist() == [i < live for i in range(3)], n
         eng.end_batch()
+
+
+@pytest.mark.parametrize("queries", [1, 40])
+def test_attention_lengths_beyond_2_24(eng, queries):
+    """The last key would take all weight, if it counted."""
+    T, D = 2 ** 24 + 1, 4
+    print("attention to", T, "keys", flush=True)
+    k, v = np.zeros((1, T, 1, D), np.float32), np.zeros((1, T, 1, D), np.float32)
+    k[0, -1], v[0, -1] = 100, 1
+    q, k, v = dev(eng, np.ones((1, queries, 1, D))), dev(eng, k), dev(eng, v, True)
+    for n, want in ((2 ** 24 - 1, 0), (2 ** 24, 0), (2 ** 24 + 2, 1)):
+        v.grad = None
+        o = eng.attention(q, k, v, lengths=dev(eng, [n]))
+        o.backward(dev(eng, np.ones((1, queries, 1, D))))
+        assert np.allclose(o.sync(), want, atol=1e-6), n
+        assert np.allclose(v.grad.sync()[0, -1], queries * want, atol=1e-3), n
+        eng.end_batch()
