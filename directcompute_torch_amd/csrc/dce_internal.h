@@ -441,14 +441,17 @@ __device__ __forceinline__ double block_sum256(double v, double* sh) {
 
 // ---------------------------------------------------------------------------
 // f = 1 / (1 + e^-z) and k = 1 - f = 1 / (1 + e^z), each within some 3 roundings of its
-// own value, from one exponential and one reciprocal (1 ulp each): e^-|z| = 2^(hi + lo),
-// hi = -|z| log2(e) rounded, lo what that leaves.  (With expf and a division the
+// own value (below 2^-126: and half of 2^-149), from one exponential and one reciprocal (1 ulp each):
+// e^-|z| = 2^(hi + lo), hi = -|z| log2(e) rounded, lo what that leaves.  The exponential
+// alone gives zero below 2^-126, for |z| above 87.3.  (With expf and a division the
 // recurrence over 16.8 million gates takes 3 microseconds more forward, 7 backward.)
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void sigmoid_pair(float z, float& f, float& k) {
+#pragma clang fp contract(off)  // hi + up is of the rounded hi
   const float m = fabsf(z) > 128.f ? 128.f : fabsf(z);  // NaN stays
   const float hi = m * -1.44269502f, lo = fmaf(m, -1.92596303e-8f, fmaf(m, -1.44269502f, -hi));
-  const float p = __builtin_amdgcn_exp2f(hi), e = fmaf(p, lo * 0.693147181f, p);
+  const int up = hi < -120.f ? 64 : 0;
+  const float p = __builtin_amdgcn_exp2f(hi + float(up)), e = ldexpf(fmaf(p, lo * 0.693147181f, p), -up);
   const float big = __builtin_amdgcn_rcpf(1.f + e), small = e * big;
   f = z >= 0.f ? big : small;
   k = z >= 0.f ? small : big;

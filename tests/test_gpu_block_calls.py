@@ -78,3 +78,30 @@ def test_attention_lengths_beyond_2_24(eng, queries):
         assert np.allclose(o.sync(), want, atol=1e-6), n
         assert np.allclose(v.grad.sync()[0, -1], queries * want, atol=1e-3), n
         eng.end_batch()
+
+
+def test_gates_below_the_normal_numbers(eng):
+    """Gates of e^-87 to e^-104 times values of 2^126: off by 8 roundings of the result and by what the
+    gate's own rounding, half of 2^-149, makes of it."""
+    z = np.linspace(-104, -86, 400).astype(np.float32)
+    big = np.float32(2.0 ** 126)
+    want = np.exp(z.astype(np.float64)) * float(big)
+    tol = 8 * 2.0 ** -24 * want + 2.0 ** -150 * float(big)
+
+    def vec(v):
+        return dev(eng, np.broadcast_to(np.float32(v), (1, 1, 400)), True)
+    none, state = vec(0), dev(eng, np.full((1, 400), big), True)
+    gate = dev(eng, z.reshape(1, 1, 400), True)
+    y = eng.gated_scan(none, gate, state)
+    assert (np.abs(y.sync()[0, 0] - want) <= tol).all()
+    y.backward(vec(big))
+    assert (np.abs(state.grad.sync()[0] - want) <= tol).all()
+    x = vec(big)
+    y = eng.gated_scan(x, dev(eng, -z.reshape(1, 1, 400)))
+    assert (np.abs(y.sync()[0, 0] - want) <= tol).all()
+    y.backward(vec(big))
+    assert (np.abs(x.grad.sync()[0, 0] - want) <= tol).all()
+    for rows in (1, 40):   # each hidden unit its own output
+        y = eng.gated_mlp(dev(eng, np.ones((rows, 1))), dev(eng, z[None]), dev(eng, np.full((1, 400), big)), dev(eng, np.eye(400)), "sigmoid")
+        assert (np.abs(y.sync() - want) <= tol).all()
+    eng.end_batch()
