@@ -175,6 +175,8 @@ def bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.BeginProfileRegion.restype = ctypes.c_bool
     lib.EndProfileRegion.argtypes = []
     lib.EndProfileRegion.restype = ctypes.c_bool
+    lib.SetWaitLimit.argtypes = [c_uint]
+    lib.SetWaitLimit.restype = c_uint
     lib.SetStreamingThreshold.argtypes = [ctypes.c_double]
     lib.SetStreamingThreshold.restype = ctypes.c_double
     lib.ResetProfile.argtypes = []

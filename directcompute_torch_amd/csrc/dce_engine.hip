@@ -42,6 +42,7 @@ static uint64_t g_poolHits = 0, g_poolMisses = 0, g_poolBytes = 0;
 static uint64_t g_poolCapBytes = 0;
 
 double g_streamBytes = kStreamBytes;
+Waits g_waits = {kSpins, nullptr};
 
 static float* g_ws = nullptr;
 static size_t g_wsFloats = 0;
@@ -701,6 +702,12 @@ bool InitEngine(void) {
     set_error("InitEngine: scratch allocation failed");
     return false;
   }
+  if (hipHostMalloc((void**)&g_waits.ended, sizeof(uint32_t), hipHostMallocDefault) != hipSuccess) {
+    hipGetLastError();
+    set_error("InitEngine: pinned allocation failed");
+    return false;
+  }
+  *g_waits.ended = 0;
   if (!noalloc_setup(g_device)) return false;
   g_init = true;
   g_err[0] = 0;
@@ -742,6 +749,12 @@ void UpdateBuffer(void* handle, float* data) {
   upload(b->ptr, data, b->count);
 }
 
+// After the stream has been waited for.
+static void report_waits() {
+  if (!__atomic_exchange_n(g_waits.ended, 0u, __ATOMIC_RELAXED)) return;
+  set_error("a workgroup's wait for another one ended: results of an earlier call are NaN");
+}
+
 void ReadBuffer(void* handle, float* dst) {
   if (!handle || !dst || !g_init) return;
   if (refuse_in_capture("ReadBuffer")) return;
@@ -752,6 +765,7 @@ void ReadBuffer(void* handle, float* dst) {
     set_error("ReadBuffer: copy failed");
   }
   if (hipStreamSynchronize(g_stream) != hipSuccess) set_error("ReadBuffer: stream error");
+  report_waits();
 }
 
 void ClearBuffer(void* handle) {
@@ -765,7 +779,9 @@ void ClearBuffer(void* handle) {
 void FlushGPU(void) {}
 
 void SyncGPU(void) {
-  if (g_init && !refuse_in_capture("SyncGPU")) hipStreamSynchronize(g_stream);
+  if (!g_init || refuse_in_capture("SyncGPU")) return;
+  hipStreamSynchronize(g_stream);
+  report_waits();
 }
 
 void WarmPool(uint32_t* sizes, uint32_t numSizes, uint32_t copies) {
@@ -1882,6 +1898,12 @@ bool EndProfileRegion(void) {
 double SetStreamingThreshold(double bytes) {
   const double prev = g_streamBytes;
   g_streamBytes = bytes < 0 ? kStreamBytes : bytes;
+  return prev;
+}
+
+uint32_t SetWaitLimit(uint32_t spins) {
+  const uint32_t prev = g_waits.spins;
+  g_waits.spins = std::min(spins, kSpins);
   return prev;
 }
 

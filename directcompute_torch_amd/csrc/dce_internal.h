@@ -278,6 +278,19 @@ __device__ __forceinline__ void stu(void* p, const V& v) {
 constexpr double kStreamBytes = 256.0 * 1024 * 1024;
 extern double g_streamBytes;
 inline bool stream_nt(double bytes) { return bytes > g_streamBytes; }
+
+// Waits of one workgroup for others that run already.  They end after so many looks, should what
+// is waited for never come; the results are then NaN, and `ended`, in host memory, is set, which the next
+// blocking call reports.
+struct Waits {
+  uint32_t spins;
+  uint32_t* ended;
+  __device__ __forceinline__ void report() const {
+    __hip_atomic_store(ended, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  }
+};
+constexpr uint32_t kSpins = 1u << 22;
+extern Waits g_waits;
 __device__ __forceinline__ f4 ldnt4(const float* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const f4*>(p));
 }

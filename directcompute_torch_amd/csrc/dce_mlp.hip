@@ -298,8 +298,8 @@ struct Again {
   MlpAgain g;
   uint32_t sumBlocks, n1, n2;  // workgroups for the sums; places of the first and the second products
   uint32_t cols;               // of y
+  Waits waits;
 };
-constexpr uint32_t kSpins = 1u << 22;  // a wait's end, should it come to that: the result is then NaN
 template <bool BWD, MlpAct ACT>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4, 4))) k_mlp_again(const Again<BWD> t) {
   constexpr Op FIRST = BWD ? GRAD : GATE;
@@ -336,10 +336,11 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
     }
     auto done = [&] { return __hip_atomic_load(t.g.counts + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == t.n1; };
     bool there = done();
-    for (uint32_t spin = 0; !there && spin < kSpins; ++spin) {
+    for (uint32_t spin = 0; !there && spin < t.waits.spins; ++spin) {
       __builtin_amdgcn_s_sleep(8);
       there = done();
     }
+    if (!there) t.waits.report();
     __syncthreads();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     small_tiles<STORE, kSilu, 1, true>(t.second, id - t.n1, reinterpret_cast<SumsOf<STORE>&>(S), there ? 0.f : NAN);
@@ -500,6 +501,7 @@ template <bool BWD>
 bool run_again(Again<BWD>& t, MlpAct act) {
   share(t.second, false);
   t.first.again = t.second.again = t.g.rows;
+  t.waits = g_waits;
   t.n1 = lay_out(t.first);
   t.n2 = lay_out(t.second);
   t.sumBlocks = (t.sums.blocks + 1) / 2;

@@ -30,7 +30,7 @@
 // forward 10.5 -> 9.9, backward 13.1 -> 11.6 us).
 //
 // Waiting: a workgroup takes its place from a counter, so those before it run
-// already.  Each leaves its pair before it waits for any, and a state waits for pairs
+// already (a wait that ends all the same is reported).  Each leaves its pair before it waits for any, and a state waits for pairs
 // and an earlier state only, so the first that lacks something gets it.  A pair, or a state,
 // is one 64-bit word, whose value tells whether it is there, so no other word has to be
 // ordered with it.  They are combined in one order, whoever came first.
@@ -51,6 +51,7 @@ struct Scan {
   unsigned long long* pairs;   // [chunks][blocks][64]
   unsigned long long* states;  // [chunks / kGroup][blocks][64]
   uint32_t* count;
+  Waits waits;
 };
 
 // A lane's channel.  Tokens are reached from a place that a wave's lanes share, with
@@ -103,7 +104,6 @@ constexpr uint32_t kGroup = 64;  // workgroups from one state to the next
 // A pair that is not there yet: all bits set, as the pass before leaves them.  (A
 // product of gates has that value only as a NaN, which is then written as another.)
 constexpr unsigned long long kAbsent = ~0ull;
-constexpr uint32_t kSpins = 1u << 22;  // a wait's end, should a pair never come: the result is then NaN
 __device__ __forceinline__ unsigned long long pack(float A, float H) {
   const unsigned long long v = (static_cast<unsigned long long>(__float_as_uint(A)) << 32) | __float_as_uint(H);
   return v == kAbsent ? 0x7fc000007fc00000ull : v;
@@ -118,12 +118,13 @@ __device__ __forceinline__ void then(float& A, float& H, float A2, float H2) {
   A = A2 * A;
 }
 
-// What is there at p, when it is there.
-__device__ __forceinline__ unsigned long long await(const unsigned long long* p, unsigned long long v) {
-  for (uint32_t spin = 0; v == kAbsent && spin < kSpins; ++spin) {
+// What is there at p, when it is there (where a wait ends before, NaN).
+__device__ __forceinline__ unsigned long long await(const Waits& waits, const unsigned long long* p, unsigned long long v) {
+  for (uint32_t spin = 0; v == kAbsent && spin < waits.spins; ++spin) {
     __builtin_amdgcn_s_sleep(1);
     v = look(p);
   }
+  if (v == kAbsent) waits.report();
   return v;
 }
 
@@ -161,7 +162,7 @@ __device__ __forceinline__ float state_in(const Scan& s, uint32_t chunk, uint32_
       for (int e = 0; e < 4; ++e) p[e] = look(mine + min(i + e, hi - 1) * next);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        p[e] = await(mine + min(i + e, hi - 1) * next, p[e]);
+        p[e] = await(s.waits, mine + min(i + e, hi - 1) * next, p[e]);
         if (i + e < hi) then(a, b, __uint_as_float(uint32_t(p[e] >> 32)), __uint_as_float(uint32_t(p[e])));
       }
     }
@@ -169,7 +170,7 @@ __device__ __forceinline__ float state_in(const Scan& s, uint32_t chunk, uint32_
     before[1][w][lane] = b;
     if (group && w == 0) {
       const unsigned long long* p = s.states + (group - 1) * next + block * 64 + lane;
-      start[lane] = __uint_as_float(uint32_t(await(p, look(p))));
+      start[lane] = __uint_as_float(uint32_t(await(s.waits, p, look(p))));
     }
     __syncthreads();
     if (group) h = start[lane];
@@ -332,6 +333,7 @@ bool run(const ScanArgs& a, const char* what) {
   s.across = cdiv(a.C, 64);
   s.blocks = cdiv(a.B, s.per) * s.across;
   s.chunks = cdiv(a.S, NW * L);
+  s.waits = g_waits;
   if (s.chunks > 1) {
     const size_t pairs = size_t(s.chunks) * s.blocks * 64, words = pairs + size_t(s.chunks / kGroup) * s.blocks * 64 + 1;
     float* ws = workspace(2 * words);

@@ -358,6 +358,13 @@ bool EndProfileRegion(void);
  * at small sizes. */
 double SetStreamingThreshold(double bytes);
 
+/* Looks after which a workgroup stops waiting for another one's result (the gated
+ * recurrence, and large gated feed-forward calls that fall back on fp32): at most the
+ * default, some seconds, which no call comes near.  A wait that ends leaves NaN, and
+ * the next ReadBuffer or SyncGPU leaves an error for GetLastErrorString.  Returns the
+ * previous limit.  It exists so that tests can see that. */
+uint32_t SetWaitLimit(uint32_t spins);
+
 /* Record / replay of queued work as a HIP graph: the MI355X form of the
  * reference's ComputeGraph (nn_engine.py:2505-2771), which records RunShader
  * dispatches and replays them through RunSequence (engine.cpp:952).  Between

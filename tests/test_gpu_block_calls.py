@@ -105,3 +105,24 @@ def test_gates_below_the_normal_numbers(eng):
         y = eng.gated_mlp(dev(eng, np.ones((rows, 1))), dev(eng, z[None]), dev(eng, np.full((1, 400), big)), dev(eng, np.eye(400)), "sigmoid")
         assert (np.abs(y.sync() - want) <= tol).all()
     eng.end_batch()
+
+
+def test_waits_that_end_are_reported(eng):
+    """With no looks beyond the first: a run of tokens that does not find the ones before it leaves NaN,
+    and the next blocking call an error; runs that do find them are right.  With the usual limit all are."""
+    r = rng(9)
+    x, z = (dev(eng, r.standard_normal((1, 200_000, 64))) for _ in range(2))
+    want = eng.gated_scan(x, z).sync().copy()
+    eng.lib.ClearLastError()
+    before = eng.lib.SetWaitLimit(0)
+    try:
+        for _ in range(3):
+            got = eng.gated_scan(x, z).sync()
+            bad = np.isnan(got)
+            assert bad.any() == ("wait" in eng.last_error())
+            assert np.array_equal(got[~bad], want[~bad])
+            eng.lib.ClearLastError()
+    finally:
+        assert eng.lib.SetWaitLimit(before) == 0
+    assert np.array_equal(eng.gated_scan(x, z).sync(), want) and not eng.last_error()
+    eng.end_batch()
