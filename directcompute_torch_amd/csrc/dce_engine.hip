@@ -1696,8 +1696,8 @@ static bool scan_args(const char* what, void* x, void* gate, void* state, void* 
     set_error("%s: %u x %u tokens of %u channels (no zeros, some 2^31 tokens or states and 2^32 values at most)", what, batch, seq, chans);
     return false;
   }
-  // A wave has 64 channels, fewer only of so long a sequence: a launch has 2^32 threads at most.
-  if (chans < 4 && seq >= (1u << 24) && n / chans > (1u << 30) - (1u << 22)) {
+  // A wave has 64 channels, fewer only of so long a sequence: a launch has fewer than 2^32 threads.
+  if (chans <= 4 && seq >= (1u << 24) && n / chans > (1u << 30) - (1u << 22)) {
     set_error("%s: %u x %u tokens (of a few channels, fewer than 2^30)", what, batch, seq);
     return false;
   }

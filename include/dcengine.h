@@ -320,7 +320,7 @@ void GatedMlpBackward(void* gradOut, void* x, void* wGate, void* wUp, void* wDow
  * hold anything), or NULL: all; y is
  * zeros past them.  pLast, when not NULL, receives the state after the last token
  * that counts (batch x chans): the next call's `state`.  Sequences of fewer than 2130706432
- * tokens, and of 2^24 and more with fewer than four channels no more than 2^30 - 2^22 tokens in all.  The backward reads the
+ * tokens, and of 2^24 and more with up to four channels no more than 2^30 - 2^22 tokens in all.  The backward reads the
  * forward's result; gradients past the lengths are zeros, and none flows in
  * through *pLast. */
 void* GatedScanForward(void* x, void* gate, void* state, void* lengths, uint32_t batch,
