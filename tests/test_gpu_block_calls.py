@@ -130,7 +130,8 @@ def test_waits_that_end_are_reported(eng):
 
 def test_scan_of_four_channels_that_no_launch_holds(eng):
     """2^32 threads, where one channel less was refused already."""
-    b = dev(eng, np.zeros(4)).gpu_buf
+    four = dev(eng, np.zeros(4))
+    b = four.gpu_buf
     for sizes in ((1, (1 << 30) - 1, 4), (1, (1 << 30) - (1 << 22) + 1, 4), (63, 17_043_520, 4)):
         assert not eng.lib.GatedScanForward(b, b, None, None, *sizes, None) and "2^30" in eng.last_error(), sizes
         eng.lib.ClearLastError()
