@@ -98,6 +98,28 @@ __device__ __forceinline__ float row_sum(float v, float* sh) {
   return v;
 }
 
+// 1 / sqrt(mean of a row's squares + eps).  Rows whose squares would leave fp32's range (and, where eps
+// does not hide it, fall below it) are added up scaled.
+template <int TPR, int NV, int W>
+__device__ __forceinline__ float inv_rms(const Span<W> (&s)[NV], const float (&v)[NV][W], uint32_t cols, float eps, float* sh) {
+  auto squares = [&](float by) {
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float x = v[j][e] * by;
+        sum += e >= s[j].dup ? x * x : 0.f;
+      }
+    return row_sum<TPR>(sum, sh);
+  };
+  float sum = squares(1.f), by = 1.f;
+  if (!(sum < 0x1p120f)) by = 0x1p-64f;
+  if (sum < 0x1p-70f && eps < 0x1p-70f) by = 0x1p64f;
+  if (by != 1.f) sum = squares(by);
+  return by / sqrtf(sum / float(cols) + eps * by * by);
+}
+
 template <int TPR>
 constexpr int threads_of = TPR < 256 ? 256 : TPR;
 
@@ -118,12 +140,7 @@ __global__ void __launch_bounds__(threads_of<TPR>) k_norm_fwd(const Norm a) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) s[j].template load<NT>(a.block + base, b[j]);
     if (a.post) {
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int e = 0; e < W; ++e) sum += e >= s[j].dup ? b[j][e] * b[j][e] : 0.f;
-      const float r = 1.f / sqrtf(row_sum<TPR>(sum, sh) / float(a.cols) + a.eps);
+      const float r = inv_rms<TPR>(s, b, a.cols, a.eps, sh);
       if (a.r1 && lane == 0) a.r1[row] = r;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -147,12 +164,7 @@ __global__ void __launch_bounds__(threads_of<TPR>) k_norm_fwd(const Norm a) {
     }
   }
   if (!a.n) return;
-  float sum = 0.f;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int e = 0; e < W; ++e) sum += e >= s[j].dup ? x[j][e] * x[j][e] : 0.f;
-  const float r = 1.f / sqrtf(row_sum<TPR>(sum, sh) / float(a.cols) + a.eps);
+  const float r = inv_rms<TPR>(s, x, a.cols, a.eps, sh);
   if (a.r2 && lane == 0) a.r2[row] = r;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {

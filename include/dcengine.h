@@ -281,6 +281,7 @@ bool MuonBatch(void** params, void** grads, void** momenta, uint32_t* rows, uint
  *   with gain `pre` (both NULL: none).  gate: gateRows x cols values, each of
  *   its rows for rows / gateRows rows in turn (1: all of them; rows: a value
  *   each), or NULL: 1.
+ * Rows of any size; gradients through rows of up to 2^110.
  * pStats, when not NULL, receives the rows' factors for the backward (RmsNorm:
  * rows floats; ResidualNorm: 2 * rows, NULL when it has neither norm). */
 void* RmsNorm(void* x, void* gain, uint32_t rows, uint32_t cols, float eps, void** pStats);

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from tests.helpers import rng
-from tests.test_gpu_block import dev
+from tests.test_gpu_block import EPS, dev, norm64, within
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +137,32 @@ def test_scan_of_four_channels_that_no_launch_holds(eng):
         eng.lib.ClearLastError()
     assert not eng.lib.GatedScanForward(b, b, None, None, 1, (1 << 30) - (1 << 22), 4, None) and "holds" in eng.last_error()
     eng.lib.ClearLastError()
+
+
+@pytest.mark.parametrize("width", [3, 30, 100, 300, 771, 1500, 3000, 9001])
+def test_norms_of_rows_of_all_sizes(eng, width):
+    """Rows of 2^-100 to 2^110 whose squares fp32 does not hold, each beside ordinary ones."""
+    r = rng(width)
+    sizes = np.exp2(np.array([0, 70, 110, 0, -100, -70, 60, -60, 0, 30, -30, 100]))[:, None]
+    M = len(sizes)
+    a = {"x": r.standard_normal((M, width)) * sizes, "block": r.standard_normal((M, width)) * sizes[::-1], "post": r.standard_normal(width),
+         "pre": r.standard_normal(width), "dh": np.zeros((M, width)), "dn": r.standard_normal((M, width))}
+    a = {k: v.astype(np.float32) for k, v in a.items()}
+    ref = {k: v.astype(np.float64) for k, v in a.items()}
+    T = {k: dev(eng, v, k not in ("dh", "dn")) for k, v in a.items()}
+    y = eng.rms_norm(T["block"], T["post"], 0.0)
+    want = norm64(ref["block"], np.zeros((M, width)), None, None, ref["post"], 1.0, 0.0, ref["dh"], ref["dn"])
+    within("rms_norm", y.sync(), want["n"][0], 24 * EPS * want["n"][1])
+    y.backward(T["dn"])
+    within("dx", T["block"].grad.sync(), want["dx"][0], 64 * EPS * want["dx"][1])
+    eng.end_batch()
+    for eps in (0.0, 1e-6):
+        T = {k: dev(eng, v, k not in ("dh", "dn")) for k, v in a.items()}
+        h, n = eng.residual_norm(T["x"], T["block"], post=T["post"], pre=T["pre"], eps=eps)
+        want = norm64(ref["x"], ref["block"], None, ref["post"], ref["pre"], 1.0, eps, ref["dh"], ref["dn"])
+        within("h", h.sync(), want["h"][0], 24 * EPS * want["h"][1])
+        within("n", n.sync(), want["n"][0], 24 * EPS * want["n"][1])
+        n.backward(T["dn"])
+        for k in ("x", "block", "post", "pre"):
+            within("d" + k, T[k].grad.sync(), want["d" + k][0], 64 * EPS * want["d" + k][1])
+        eng.end_batch()
