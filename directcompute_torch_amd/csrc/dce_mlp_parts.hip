@@ -1057,17 +1057,22 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
          mlp_backward_again(a, dy, dx, dwg, dwu, dwd, {plan.flag, nullptr, plan.flag + 1, plan.free}, sums);
 }
 
-// The parts of the weights are made anew at each call, which few rows do not pay for.
-// Microseconds with fp32 MFMAs / on parts, forward: 128 x 2048 x 8192 174 / 195, 512 x 512 x 2048
-// 49 / 54, 256 x 1024 x 4096 84 / 82, 2048 x 256 x 1024 51 / 49, 8192 x 128 x 512 54 / 44, 200 x
-// 2048 x 8192 313 / 208.  Backward: 64 x 2048 x 8192 278 / 332, 96 of
-// them 345 / 335, 128 x 1024 x 4096 116 / 112, 1024 x 256 x 1024 66 / 71, 4096 x 128 x 512 73 /
-// 74, 400 x 512 x 2048 107 / 83, 1024 x 384 x 1001 100 / 76, 200 x 2048 x 8192 654 / 392.
+// The parts of the weights are made anew at each call, which few rows do not pay for; and the narrower
+// the products, the more of their time goes into their epilogues.
+// Microseconds on fp32 MFMAs / on parts, forward: 128 x 4096 x 8192 332 / 363, 160 x 2048 x 8192 262 / 207,
+// 192 x 1024 x 4096 72 / 83, 256 of them 84 / 84, 512 x 512 x 2048 48 / 59, 700 of them 71 / 59, 2048 x 256 x
+// 1024 49 / 53, 3000 of them 69 / 54, 4096 x 128 x 512 33 / 44, 8192 of them 53 / 47, 16384 x 64 x 256 35 / 42,
+// 32768 of them 60 / 54.  Backward: 96 x 4096 x 8192 582 / 608, 96 x 2048 x 8192 331 / 352, 128 of them 363 / 356,
+// 128 x 1024 x 4096 116 / 115, 192 of them 165 / 127, 150 x 512 x 8192 147 / 123, 500 x 600 x 1000 68 / 81, 256 x 512 x
+// 2048 61 / 78, 400 of them 101 / 88, 700 x 384 x 1001 73 / 78, 1024 of them 96 / 82, 1024 x 256 x 1024 63 / 76, 2048 of
+// them 130 / 86, 4096 x 128 x 512 67 / 78, 8192 of them 130 / 100, 6000 x 100 x 700 146 / 98, 20000 x 90 x 300 184 / 164,
+// 32768 x 64 x 256 150 / 218.
 bool mlp_on_parts(const MlpArgs& a, bool backward) {
   // a tile's rows are reached with 32-bit offsets
   if (std::max({a.rows, a.cols, a.hidden, a.out}) > (1u << 21) || std::min({a.rows, a.cols, a.hidden, a.out}) < 32) return false;
-  const double weights = std::sqrt(double(a.cols) * a.out) * a.hidden;
-  return backward ? (double(a.rows) - 80) * weights >= 2.4e8 : (double(a.rows) - 110) * weights >= 4.5e8;
+  const double width = std::sqrt(double(a.cols) * a.out);
+  return backward ? a.rows > 90 && width >= 80 && (a.rows - 90.0) * (width - 40) * a.hidden >= 2.3e8
+                  : (a.rows - 115.0) * width * a.hidden >= 5.2e8;
 }
 
 }  // namespace dce
