@@ -19,6 +19,7 @@ export/import, and the Python-side profilers.
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 
 import numpy as np
@@ -986,18 +987,21 @@ def _gain_of(what, name, gain, width):
 def _gate_rows(gate, shape):
     """Rows of a residual gate for x of `shape`, each for an equal share of x's rows in turn; None
     where the gate's shape does not say that.  Leading axes as x's, the rest ones or left out."""
-    if not gate.shape or gate.shape[-1] != shape[-1]:
+    own, width = tuple(gate.shape), shape[-1]
+    if not own or own[-1] != width or not gate.size:
         return None
-    lead, axes = tuple(gate.shape[:-1]), tuple(shape[:-1])
-    rows, of = int(np.prod(lead, dtype=np.int64)), int(np.prod(axes, dtype=np.int64))
-    if rows in (1, of) and (rows == 1 or lead in ((of,), axes)):
+    lead, rows = own[:-1], gate.size // width
+    if rows == 1 or (len(own) <= len(shape) and lead == shape[:len(lead)]):
+        return rows
+    axes = shape[:-1]
+    of = math.prod(axes)
+    if lead == (of,):
         return rows
     if len(axes) == 1:   # tokens side by side: a gate's row for as many of them each
-        return rows if len(lead) == 1 and rows and of % rows == 0 else None
-    own = lead
-    while own and own[-1] == 1:
-        own = own[:-1]
-    return rows if len(lead) <= len(axes) and own == axes[:len(own)] else None
+        return rows if len(lead) == 1 and of % rows == 0 else None
+    while lead[-1] == 1:
+        lead = lead[:-1]
+    return rows if len(own) <= len(shape) and lead == axes[:len(lead)] else None
 
 
 class RmsNormFunc(_Keeps):
