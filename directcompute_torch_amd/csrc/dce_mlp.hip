@@ -31,8 +31,9 @@ inline uint32_t cdiv(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b);
 // (1.07 GFLOP, 7 us at the rate of a large fp32 product): the gate's product 10 us, y 6 and 3
 // for its sums, the gradient's 9, the four others 18.5 and 4; 64 x 1024 x 2816, training: 81
 // us (with eight waves for each tile and no splits 102).  Eight octets in flight, with twice
-// the code, took 10 % more.  Of many rows of large weights (96 x 2048 x 8192 training: 500
-// us, 58 TFLOP/s) reads from L2 bound it.
+// the code, took 10 % more.  Many rows of large weights (96 x 2048 x 8192 training: 465 us, 62
+// TFLOP/s, more than the plain form's 391) wait for L2 as much as they multiply: MFMAs busy 22 to 48 %, 7 to 12
+// TB/s from L2, dm's product 22; each weight is read once for 32 rows.
 // ---------------------------------------------------------------------------
 enum Op { STORE, GATE, GRAD };
 struct Side {

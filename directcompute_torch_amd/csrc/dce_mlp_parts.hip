@@ -172,7 +172,7 @@ __device__ __forceinline__ int find_job(const Jobs& t, uint32_t blk) {
 // together once), of rows where columns are and there are many.  The workgroups' largest values go
 // side by side into memory and are brought together by k_mlp_split, for the 128 of its tile.
 // (Atomics on one place take some 0.4 us after the other: 8192 x 128, 128 blocks of rows,
-// 53 us.)  Bound by memory: 84 MB (x and three weights of 8192 x 1024 x 4096) 27 us.
+// 53 us.)  Bound by memory: of 8192 x 1024 x 4096 84 MB (x and three weights) 19 us, 117 MB backward 30.
 constexpr uint32_t kMaxRows = 64, kMaxBlocks = 32;
 struct Reach {
   uint32_t rows, cols;  // of a workgroup
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kT) k_mlp_max(const Jobs t) {
 
 // A 128 x 128 tile through LDS, for the matrix' rows, its columns, or both at once, with
 // the exponents of the rows and columns, or for the columns with those of the tile; a value is 4 bytes as it was.  Bound by memory: of 8192 x 1024 x 4096 84 MB in and 84 out
-// forward, 3.9 TB/s in 43 us.
+// forward, 34 us, 117 and 151 backward, 51 us, 5 TB/s.
 __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
   __shared__ __attribute__((aligned(16))) float S0[64 * 128];
   __shared__ __attribute__((aligned(16))) float S1[64 * 128];
@@ -316,10 +316,10 @@ __global__ void __launch_bounds__(kT) k_mlp_split(const Jobs t) {
 // its fragments, that took the four products from 960 to 1150 us.)
 //
 // Bound by the MFMAs, for which power holds the clock to 1.7 GHz.  8192 x 1024 x 4096, in us
-// and TFLOP/s of fp32 products (a large fp16 library product, divided by three: 374): g and u 437,
-// 315; y 207, 332; dx, dWd, dWg and dWu 970, 354; dm 400, 172, of which its epilogue, which reads
-// 8 bytes a hidden value and writes 20, takes more than half.  Two workgroups a CU, of 64 KB and
-// some 230 registers a lane.  With one array for both stages every read waited for the loads
+// and TFLOP/s of fp32 products (a large fp16 library product, divided by three: 374): g and u 421,
+// 326; y 216, 318; dx, dWd, dWg and dWu 1000, 344; dm 390, 176, of which its epilogue, which reads
+// 8 bytes a hidden value and writes 20, takes more than half.  The look at the results is 1 to 2 us of
+// a tile's.  Two workgroups a CU, of 64 KB and some 200 to 220 registers a lane.  With one array for both stages every read waited for the loads
 // (2.19 ms for 2.14 of a training pass).
 // ---------------------------------------------------------------------------
 enum Op { STORE, GATE, BLOCK_GATE, GRAD };  // STORE, BLOCK_GATE: q's parts have exponents of its blocks
@@ -1057,22 +1057,28 @@ bool mlp_backward_parts(const MlpArgs& a, const float* dy, float* dx, float* dwg
          mlp_backward_again(a, dy, dx, dwg, dwu, dwd, {plan.flag, nullptr, plan.flag + 1, plan.free}, sums);
 }
 
-// The parts of the weights are made anew at each call, which few rows do not pay for; and the narrower
-// the products, the more of their time goes into their epilogues.
+// The parts of the weights are made anew at each call, which few rows do not pay for.
 // Microseconds on fp32 MFMAs / on parts, forward: 128 x 4096 x 8192 332 / 363, 160 x 2048 x 8192 262 / 207,
 // 192 x 1024 x 4096 72 / 83, 256 of them 84 / 84, 512 x 512 x 2048 48 / 59, 700 of them 71 / 59, 2048 x 256 x
 // 1024 49 / 53, 3000 of them 69 / 54, 4096 x 128 x 512 33 / 44, 8192 of them 53 / 47, 16384 x 64 x 256 35 / 42,
-// 32768 of them 60 / 54.  Backward: 96 x 4096 x 8192 582 / 608, 96 x 2048 x 8192 331 / 352, 128 of them 363 / 356,
-// 128 x 1024 x 4096 116 / 115, 192 of them 165 / 127, 150 x 512 x 8192 147 / 123, 500 x 600 x 1000 68 / 81, 256 x 512 x
-// 2048 61 / 78, 400 of them 101 / 88, 700 x 384 x 1001 73 / 78, 1024 of them 96 / 82, 1024 x 256 x 1024 63 / 76, 2048 of
-// them 130 / 86, 4096 x 128 x 512 67 / 78, 8192 of them 130 / 100, 6000 x 100 x 700 146 / 98, 20000 x 90 x 300 184 / 164,
-// 32768 x 64 x 256 150 / 218.
+// 32768 of them 60 / 54.
+// Backward, a fit to such times of 58 sizes (rows of 48 to 65536, widths of 33 to 4096), within 30 % of each; the side it
+// takes is the faster one, or within 3 %: on fp32 by the tiles' values, on parts by what dm's epilogue moves, the
+// products, the weights' parts and the tokens'.  96 x 2048 x 8192 331 / 352, 128 of them 363 / 356, 128 x 1024 x 4096
+// 116 / 115, 192 of them 165 / 127, 150 x 512 x 8192 147 / 123, 500 x 600 x 1000 68 / 81, 256 x 512 x 2048 61 / 78, 400 of
+// them 101 / 88, 1024 x 256 x 1024 63 / 76, 2048 of them 130 / 86, 4096 x 128 x 512 67 / 78, 8192 of them 130 / 100, 6112 x 71
+// x 5862 1163 / 634, 32768 x 64 x 256 150 / 218, 30000 x 96 x 200 173 / 200.
 bool mlp_on_parts(const MlpArgs& a, bool backward) {
   // a tile's rows are reached with 32-bit offsets
   if (std::max({a.rows, a.cols, a.hidden, a.out}) > (1u << 21) || std::min({a.rows, a.cols, a.hidden, a.out}) < 32) return false;
   const double width = std::sqrt(double(a.cols) * a.out);
-  return backward ? a.rows > 90 && width >= 80 && (a.rows - 90.0) * (width - 40) * a.hidden >= 2.3e8
-                  : (a.rows - 115.0) * width * a.hidden >= 5.2e8;
+  if (!backward) return (a.rows - 115.0) * width * a.hidden >= 5.2e8;
+  const uint32_t w = uint32_t(width);
+  auto values = [&](uint32_t tile) { return 1e-6 * pad(a.rows, tile) * pad(a.hidden, tile); };  // in whole tiles, millions
+  const double fp32 = (12 + values(32) * (5.3 + 0.18 * pad(w, 32))) * (w % 8 ? 1 + 14 / width : 1);  // a depth's last octet value by value
+  const double parts = 54 + values(kTile) * (7.7 + 0.0256 * pad(w, kTile)) +
+                       13e-6 * width * a.hidden * std::min(1.0, 0.3 + width / 2000) + 1.9e-3 * a.rows;
+  return parts < fp32;
 }
 
 }  // namespace dce
